@@ -306,6 +306,88 @@ int nf_ce_fwd_bwd(const void *hidden, const void *weight,
                   int32_t *bad_targets, void *workspace,
                   size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Log probabilities of given tokens: for each row m of hidden [M, D] with a
+ * target in [0, V) other than ignore_index, with z = hidden[m] . weight^T
+ * (weight [V, D]) and p = softmax(z),
+ *   logprobs[m] = z[target] - lse,   entropy[m] = -sum p log p,
+ *   top_logprobs / top_ids [m, 0 .. top_k - 1]: the largest z - lse in falling
+ *   order and their columns (equal ones: the lower column first);
+ * the other rows give 0 (column -1).  top_k at most 32 and V; 0: neither
+ * pointer is used.  dtype (hidden, weight): bf16 or f32; values fp32.  No
+ * kernel of the reference computes these; sizes, chunk_rows and the target
+ * rules are those of nf_ce_fwd.  `state`
+ * (nf_token_logprobs_state_bytes) holds the compacted rows, their log-sum-exp
+ * and entropy for the backward; `workspace` nothing between calls.  A size
+ * call returns 0 for arguments beyond the kernels.
+ * ---------------------------------------------------------------------- */
+size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V,
+                                     int dtype);
+size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t V,
+                                       int64_t chunk_rows, int top_k,
+                                       int dtype);
+int nf_token_logprobs_fwd(const void *hidden, const void *weight,
+                          const int64_t *targets, int64_t M, int64_t D,
+                          int64_t V, int64_t ignore_index, int64_t chunk_rows,
+                          int top_k, int dtype, float *logprobs,
+                          float *entropy, float *top_logprobs,
+                          int64_t *top_ids, void *state, size_t state_bytes,
+                          void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* The gradient for upstream g_logprobs, g_entropy (fp32 [M]; either may be
+ * NULL: zero): with g, h a row's two and H its entropy,
+ *   dz = g (onehot(target) - p) - h p (z - lse + H),
+ *   dhidden = dz weight,  dweight = dz^T hidden
+ * (either may be NULL: not formed).  `weight` and `state` are the forward's;
+ * the logits are formed again.  The same bits every run. */
+size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,
+                                       int64_t chunk_rows, int dtype);
+int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, int64_t V,
+                          int64_t chunk_rows, int dtype, void *state,
+                          size_t state_bytes, const float *g_logprobs,
+                          const float *g_entropy, void *dhidden, int dt_hidden,
+                          void *dweight, int dt_weight, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Embedding lookup: out[m, :] = scale * table[ids[m], :]  (no counterpart in
+ * the reference's kernels, whose models use nn.Embedding).  ids int64 [M]; table [V, D] with row stride
+ * ld_table; out [M, D] dense.  fp32 arithmetic, one rounding.  An id outside
+ * [0, V) gives a row of zeros.  out has the table's element type, or bf16 /
+ * fp16 with an fp32 table.
+ * ---------------------------------------------------------------------- */
+int nf_embedding_fwd(const int64_t *ids, const void *table, int64_t ld_table,
+                     float scale, int64_t M, int64_t D, int64_t V, void *out,
+                     int dt_table, int dt_out, void *stream);
+
+/* Its gradient: dtable[v, :] = scale * sum of dout[m, :] over the m with
+ * ids[m] == v, in order of m within fixed groups (the same bits every run);
+ * rows no token holds, and the row padding_id (-1: none), are zero.  ids
+ * outside [0, V) count nowhere.  Every row of dtable [V, D] (dense) is
+ * written.  workspace: nf_embedding_bwd_workspace bytes (0: sizes beyond the
+ * kernels), 16-byte aligned; it holds nothing between calls. */
+size_t nf_embedding_bwd_workspace(int64_t M, int64_t D, int64_t V);
+int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t padding_id,
+                     float scale, int64_t M, int64_t D, int64_t V,
+                     void *dtable, int dt_out, int dt_table, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Dropout from a counter-based generator, over n contiguous elements:
+ *   out[i] = residual[i] + (kept(i) ? x[i] * 65536 / (65536 - threshold) : 0)
+ * (residual may be NULL).  Element i takes bits 16 (i % 8) .. + 15 of the
+ * Philox4x32-10 block with counter (i / 8, offset) and key seed, and is kept
+ * where they are >= threshold (0: all kept; 65536: none).  The seed is
+ * *seed_ptr, read on the device (a replayed graph takes its value then), or
+ * `seed` where seed_ptr is NULL.  The backward is the same call on the
+ * upstream gradient without a residual.  Types: dt_x == dt_out, or either
+ * fp32 and the other 16 bits; residual has dt_out.
+ * ---------------------------------------------------------------------- */
+int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
+               int32_t threshold, const int64_t *seed_ptr, int64_t seed,
+               int64_t offset, int dt_x, int dt_out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,484 @@
+// Embedding lookup, out[m] = scale * table[ids[m]], and its gradient,
+// dtable[v] = scale * sum over the m with ids[m] = v of dout[m], by sorted tokens: no
+// atomics on values, every sum in a fixed order, every row of dtable written once.
+//
+// An id outside [0, V) gives a row of zeros and no gradient; the padding id is looked
+// up like any other and gives no gradient.
+//
+// The gradient takes three launches:
+//   emb_sort:   block b owns the ids [b R, (b + 1) R).  It reads all M ids twice: first
+//               counting its own (per wavefront and id, in LDS) and the ids below its
+//               range, which gives every id's first position in the sorted order without
+//               a word from another block; then placing its tokens, in order.  It writes
+//               zeros to the rows of its ids that no token holds.
+//   emb_reduce: the sorted positions in spans of kSpan, one wavefront a span (and 64
+//               vectors of columns): a run of one id that lies inside the span is summed
+//               and written; a piece of a run that crosses a span's border goes to the
+//               workspace as an fp32 partial row.
+//   emb_join:   the partial rows of each run that crosses borders, added in order.
+// So the work of a token that holds half the batch is spread like any other.
+#include <initializer_list>
+
+#include "nf_device.h"
+
+namespace nf {
+namespace {
+
+// VE consecutive elements, aligned to their size (up to 16 bytes).
+template <typename T, int VE>
+__device__ __forceinline__ void load_n(const T *p, float (&v)[VE]) {
+  if constexpr (VE == 8) {
+    Chunk8<T>::load(p, v);
+  } else if constexpr (VE == 2) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 a = *reinterpret_cast<const t2 *>(p);
+    v[0] = to_f32(a[0]);
+    v[1] = to_f32(a[1]);
+  } else {
+    v[0] = to_f32(p[0]);
+  }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void store_n(T *p, const float (&v)[VE]) {
+  if constexpr (VE == 8) {
+    Chunk8<T>::store(p, v);
+  } else if constexpr (VE == 2) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    t2 a;
+    a[0] = from_f32<T>(v[0]);
+    a[1] = from_f32<T>(v[1]);
+    *reinterpret_cast<t2 *>(p) = a;
+  } else {
+    p[0] = from_f32<T>(v[0]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// forward: a group of 2^glog lanes takes a row, VE columns a lane and step
+// ---------------------------------------------------------------------------
+constexpr int kFwdThreads = 256;
+
+template <typename W, typename O, int VE>
+__global__ __launch_bounds__(kFwdThreads) void emb_fwd_kernel(
+    const int64_t *__restrict__ ids, const W *__restrict__ table, int64_t ldt, float scale,
+    int64_t M, int64_t D, int64_t V, O *__restrict__ out, int glog) {
+  const int g = threadIdx.x & ((1 << glog) - 1);
+  const int64_t m = (int64_t)blockIdx.x * (kFwdThreads >> glog) + (threadIdx.x >> glog);
+  if (m >= M) return;
+  const int64_t id = ids[m];
+  const bool live = id >= 0 && id < V;
+  const W *src = table + (live ? id : 0) * ldt;
+  O *dst = out + m * D;
+  const int64_t step = (int64_t)VE << glog;
+  constexpr int kUnroll = 4;
+  for (int64_t c0 = (int64_t)g * VE; c0 < D; c0 += kUnroll * step) {
+    float v[kUnroll][VE];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (c0 + u * step < D) load_n<W, VE>(src + c0 + u * step, v[u]);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (c0 + u * step < D) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[u][i] = live ? v[u][i] * scale : 0.f;
+        store_n<O, VE>(dst + c0 + u * step, v[u]);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// gradient
+// ---------------------------------------------------------------------------
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kMaxRange = 512;  // ids per block
+constexpr int kSpan = 32;       // sorted positions per wavefront of emb_reduce
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
+
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d);
+    if (l >= d) v += o;
+  }
+  return v;
+}
+
+// first[v]: the sorted position of id v's first token (first[V]: the number of tokens
+// that count); perm, sid: the token and the id at each position.
+template <typename W, int VE>
+__global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
+    const int64_t *__restrict__ ids, int64_t M, int64_t V, int64_t pad, int R,
+    int *__restrict__ first, int *__restrict__ perm, int *__restrict__ sid,
+    W *__restrict__ dtable, int64_t D) {
+  __shared__ int hist[kSortWaves][kMaxRange];
+  __shared__ int total[kMaxRange];
+  __shared__ int below_w[kSortWaves];
+  __shared__ int scan_w[kSortWaves];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t lo = (int64_t)blockIdx.x * R;
+  const int64_t hi = lo + R < V ? lo + R : V;
+  for (int k = l; k < R; k += 64) hist[w][k] = 0;  // the wavefront's own row
+  const int64_t seg = ((M + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
+  const int64_t m0 = (int64_t)w * seg, m1 = m0 + seg < M ? m0 + seg : M;
+  __syncthreads();
+  int below = 0;
+  constexpr int kBatch = 4;
+  for (int64_t b = m0; b < m1; b += 64 * kBatch) {
+    int64_t id[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t m = b + u * 64 + l;
+      id[u] = m < m1 ? ids[m] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const bool counts = id[u] >= 0 && id[u] < V && id[u] != pad;
+      below += counts && id[u] < lo ? 1 : 0;
+      if (counts && id[u] >= lo && id[u] < hi) atomicAdd(&hist[w][id[u] - lo], 1);
+    }
+  }
+  below = wave_inclusive_sum(below);
+  if (l == 63) below_w[w] = below;
+  __syncthreads();
+  // per id: the counts of the wavefronts before, and the total
+  int mine = 0;
+  if ((int)threadIdx.x < R) {
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) {
+      const int h = hist[k][threadIdx.x];
+      hist[k][threadIdx.x] = mine;
+      mine += h;
+    }
+    total[threadIdx.x] = mine;
+  }
+  const int incl = wave_inclusive_sum(mine);
+  if (l == 63) scan_w[w] = incl;
+  __syncthreads();
+  int start = incl - mine;
+  for (int k = 0; k < kSortWaves; ++k) {
+    start += below_w[k];
+    start += k < w ? scan_w[k] : 0;
+  }
+  if ((int)threadIdx.x < R) {
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) hist[k][threadIdx.x] += start;
+    if (lo + threadIdx.x < V) {
+      first[lo + threadIdx.x] = start;
+      if (lo + threadIdx.x == V - 1) first[V] = start + mine;
+    }
+  }
+  __syncthreads();
+  // rows without a token
+  const float zero[VE] = {};
+  for (int64_t v = lo + w; v < hi; v += kSortWaves)
+    if (total[v - lo] == 0)
+      for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) store_n<W, VE>(dtable + v * D + c, zero);
+  // the tokens of the range in order: a wavefront ranks 64 at a time, id by id
+  const uint64_t lower = (1ull << l) - 1ull;
+  volatile int *next = hist[w];
+  for (int64_t b = m0; b < m1; b += 64 * kBatch) {
+    int64_t ib[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t m = b + u * 64 + l;
+      ib[u] = m < m1 ? ids[m] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int64_t id = ib[u];
+      const bool in = id >= lo && id < hi && id != pad;
+      const int key = in ? (int)(id - lo) : -1;
+      uint64_t todo = __ballot(in);
+      while (todo) {
+        const int lead = __ffsll((unsigned long long)todo) - 1;
+        const int k = __builtin_amdgcn_readlane(key, lead);
+        const uint64_t same = __ballot(key == k);
+        const int at = next[k];
+        if (key == k) {
+          const int pos = at + __popcll(same & lower);
+          perm[pos] = (int)(b + u * 64 + l);
+          sid[pos] = (int)id;
+          if (l == lead) next[k] = at + __popcll(same);
+        }
+        todo &= ~same;
+      }
+    }
+  }
+}
+
+// O: dout's type, W: dtable's.  part[2 s] is the head of span s (the end, or all, of a
+// run begun before it), part[2 s + 1] its tail (the begin of a run that goes on).
+template <typename O, typename W, int VE>
+__global__ __launch_bounds__(256) void emb_reduce_kernel(
+    const O *__restrict__ dout, int64_t ldo, const int *__restrict__ first,
+    const int *__restrict__ perm, const int *__restrict__ sid, int64_t V, int64_t D, float scale,
+    W *__restrict__ dtable, float *__restrict__ part) {
+  const int n = first[V];
+  const int l = threadIdx.x & 63;
+  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t t0 = s * kSpan;
+  if (t0 >= n) return;
+  const int cnt = n - t0 < kSpan ? (int)(n - t0) : kSpan;
+  const int64_t c = ((int64_t)blockIdx.y * 64 + l) * VE;
+  const bool cin = c < D;
+  const int tok = l < cnt ? perm[t0 + l] : 0;
+  const int id = l < cnt ? sid[t0 + l] : -1;
+  const int before = t0 > 0 ? sid[t0 - 1] : -1;
+  const int after = t0 + cnt < n ? sid[t0 + cnt] : -1;
+  float acc[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  bool begun_before = before == __builtin_amdgcn_readlane(id, 0);
+  constexpr int kBatch = 8;
+  for (int j0 = 0; j0 < cnt; j0 += kBatch) {
+    float v[kBatch][VE];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (j0 + u < cnt && cin)
+        load_n<O, VE>(dout + (int64_t)__builtin_amdgcn_readlane(tok, j0 + u) * ldo + c, v[u]);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int j = j0 + u;
+      if (j >= cnt) break;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] += v[u][i];
+      const int here = __builtin_amdgcn_readlane(id, j);
+      const bool last = j + 1 == cnt;
+      const int then = last ? after : __builtin_amdgcn_readlane(id, j + 1 < 64 ? j + 1 : 63);
+      if (last || then != here) {
+        const bool goes_on = then == here;
+        if (cin) {
+          if (begun_before || goes_on) {
+            store_n<float, VE>(part + (2 * s + (begun_before ? 0 : 1)) * D + c, acc);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) acc[i] *= scale;
+            store_n<W, VE>(dtable + (int64_t)here * D + c, acc);
+          }
+        }
+        begun_before = false;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+      }
+    }
+  }
+}
+
+// Block (s, y): the run that begins in span s and goes on past it, if there is one: its
+// tail there and the heads of the spans after it.  Wavefront k adds the pieces k, k + 16,
+// k + 32, ... in that order, the first wavefront the 16 sums.
+template <typename W, int VE>
+__global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
+    const int *__restrict__ first, const int *__restrict__ sid, int64_t V, int64_t D, float scale,
+    const float *__restrict__ part, W *__restrict__ dtable) {
+  __shared__ float sums[kJoinWaves][64 * VE];
+  const int n = first[V];
+  const int64_t s = blockIdx.x, end = (s + 1) * kSpan;  // a border between two spans
+  if (end >= n) return;
+  const int id = sid[end - 1];
+  if (sid[end] != id || first[id] < s * kSpan) return;  // no run crosses, or it began before
+  const int64_t pieces = (first[id + 1] - 1) / kSpan - s + 1;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = ((int64_t)blockIdx.y * 64 + l) * VE;
+  const bool cin = c < D;
+  float acc[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  if (cin) {
+    constexpr int kBatch = 4;
+    for (int64_t p0 = w; p0 < pieces; p0 += kJoinWaves * kBatch) {
+      float v[kBatch][VE];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int64_t p = p0 + u * kJoinWaves;
+        if (p < pieces) load_n<float, VE>(part + (2 * (s + p) + (p == 0 ? 1 : 0)) * D + c, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (p0 + u * kJoinWaves < pieces)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[i] += v[u][i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sums[w][l * VE + i] = acc[i];
+  __syncthreads();
+  if (w == 0 && cin) {
+    const int waves = pieces < kJoinWaves ? (int)pieces : kJoinWaves;
+    for (int k = 1; k < waves; ++k)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] += sums[k][l * VE + i];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] *= scale;
+    store_n<W, VE>(dtable + (int64_t)id * D + c, acc);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// Columns a lane takes at once: 8 where every row starts on 16 bytes, 2 where every row
+// starts on a pair, else 1.
+int vector_width(std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> lds,
+                 int64_t D) {
+  auto fits = [&](int ve, uintptr_t bytes) {
+    for (const void *p : ptrs)
+      if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+    for (int64_t ld : lds)
+      if (ld % ve) return false;
+    return D % ve == 0;
+  };
+  return fits(8, 16) ? 8 : fits(2, 8) ? 2 : 1;
+}
+
+template <typename W, typename O>
+int run_fwd(const int64_t *ids, const W *table, int64_t ldt, float scale, int64_t M, int64_t D,
+            int64_t V, O *out, hipStream_t s) {
+  const int ve = vector_width({table, out}, {ldt}, D);
+  const int64_t vecs = (D + ve - 1) / ve;
+  int glog = 3;
+  while (glog < 6 && ((int64_t)1 << glog) < vecs) ++glog;
+  const int64_t rows = kFwdThreads >> glog;
+  const unsigned grid = (unsigned)((M + rows - 1) / rows);
+  if (ve == 8)
+    emb_fwd_kernel<W, O, 8><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
+  else if (ve == 2)
+    emb_fwd_kernel<W, O, 2><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
+  else
+    emb_fwd_kernel<W, O, 1><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
+  return check_launch("nf_embedding_fwd");
+}
+
+struct BwdPlan {
+  int R;               // ids per block of emb_sort
+  int64_t blocks;      // of emb_sort
+  int64_t spans;
+  size_t first, perm, sid, part, total;
+};
+BwdPlan bwd_plan(int64_t M, int64_t D, int64_t V) {
+  auto align = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  BwdPlan p;
+  const int64_t r = (V + 255) / 256;
+  p.R = (int)(r < 1 ? 1 : (r > kMaxRange ? kMaxRange : r));
+  p.blocks = (V + p.R - 1) / p.R;
+  p.spans = (M + kSpan - 1) / kSpan;
+  size_t o = 0;
+  p.first = o;
+  o = align(o + (size_t)(V + 1) * sizeof(int));
+  p.perm = o;
+  o = align(o + (size_t)M * sizeof(int));
+  p.sid = o;
+  o = align(o + (size_t)M * sizeof(int));
+  p.part = o;
+  o = align(o + (size_t)p.spans * 2 * (size_t)D * sizeof(float));
+  p.total = o;
+  return p;
+}
+
+template <typename O, typename W, int VE>
+int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int64_t M, int64_t D,
+               int64_t V, W *dtable, char *ws, hipStream_t s) {
+  const BwdPlan p = bwd_plan(M, D, V);
+  int *first = reinterpret_cast<int *>(ws + p.first);
+  int *perm = reinterpret_cast<int *>(ws + p.perm);
+  int *sid = reinterpret_cast<int *>(ws + p.sid);
+  float *part = reinterpret_cast<float *>(ws + p.part);
+  const unsigned cols = (unsigned)((D + 64 * VE - 1) / (64 * VE));
+  emb_sort_kernel<W, VE><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(ids, M, V, pad, p.R, first,
+                                                                     perm, sid, dtable, D);
+  if (int e = check_launch("emb_sort")) return e;
+  if (M == 0) return NF_OK;
+  emb_reduce_kernel<O, W, VE><<<dim3((unsigned)((p.spans + 3) / 4), cols), 256, 0, s>>>(
+      dout, D, first, perm, sid, V, D, scale, dtable, part);
+  if (int e = check_launch("emb_reduce")) return e;
+  if (p.spans < 2) return NF_OK;  // no border to cross
+  emb_join_kernel<W, VE><<<dim3((unsigned)(p.spans - 1), cols), kJoinThreads, 0, s>>>(
+      first, sid, V, D, scale, part, dtable);
+  return check_launch("emb_join");
+}
+
+template <typename O, typename W>
+int run_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int64_t M, int64_t D,
+            int64_t V, W *dtable, char *ws, hipStream_t s) {
+  const int ve = vector_width({dout, dtable}, {}, D);
+  if (ve == 8) return launch_bwd<O, W, 8>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
+  if (ve == 2) return launch_bwd<O, W, 2>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
+  return launch_bwd<O, W, 1>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
+}
+
+// The table's type and out's: equal, or an fp32 table with rows in 16 bits.
+bool types_ok(int dt_table, int dt_out) {
+  return is_dtype(dt_table) && is_dtype(dt_out) &&
+         (dt_table == dt_out || dt_table == NF_DTYPE_F32);
+}
+bool sizes_ok(int64_t M, int64_t D, int64_t V) {
+  // D: at most 65535 column blocks of 64 elements in a grid
+  const int64_t i32 = 0x7fffffffLL, cap = (int64_t)1 << 40;
+  return M >= 0 && D > 0 && V > 0 && M < i32 && D <= 65535 * 64 && V < i32 && V * D <= cap &&
+         M * D <= cap;
+}
+
+}  // namespace
+}  // namespace nf
+
+using namespace nf;
+
+extern "C" int nf_embedding_fwd(const int64_t *ids, const void *table, int64_t ld_table,
+                                float scale, int64_t M, int64_t D, int64_t V, void *out,
+                                int dt_table, int dt_out, void *stream) {
+  if (!sizes_ok(M, D, V) || ld_table < D)
+    return set_error(NF_ERR_ARG, "nf_embedding_fwd: bad shape M=%lld D=%lld V=%lld ld=%lld",
+                     (long long)M, (long long)D, (long long)V, (long long)ld_table);
+  if (!types_ok(dt_table, dt_out))
+    return set_error(NF_ERR_DTYPE, "nf_embedding_fwd: dtypes %d -> %d", dt_table, dt_out);
+  if (M == 0) return NF_OK;
+  if (!ids || !table || !out) return set_error(NF_ERR_ARG, "nf_embedding_fwd: null pointer");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define NF_EMB(CW, CO, W, O)                                                                   \
+  if (dt_table == CW && dt_out == CO)                                                          \
+    return run_fwd<W, O>(ids, static_cast<const W *>(table), ld_table, scale, M, D, V,         \
+                         static_cast<O *>(out), s);
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_F32, float, float)
+  NF_EMB(NF_DTYPE_BF16, NF_DTYPE_BF16, bf16, bf16)
+  NF_EMB(NF_DTYPE_F16, NF_DTYPE_F16, f16, f16)
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_BF16, float, bf16)
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_F16, float, f16)
+#undef NF_EMB
+  return set_error(NF_ERR_DTYPE, "nf_embedding_fwd: dtypes %d -> %d", dt_table, dt_out);
+}
+
+extern "C" size_t nf_embedding_bwd_workspace(int64_t M, int64_t D, int64_t V) {
+  if (!sizes_ok(M, D, V)) return 0;
+  return bwd_plan(M, D, V).total;
+}
+
+extern "C" int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t padding_id,
+                                float scale, int64_t M, int64_t D, int64_t V, void *dtable,
+                                int dt_out, int dt_table, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+  if (!sizes_ok(M, D, V))
+    return set_error(NF_ERR_ARG, "nf_embedding_bwd: bad shape M=%lld D=%lld V=%lld",
+                     (long long)M, (long long)D, (long long)V);
+  if (!types_ok(dt_table, dt_out))
+    return set_error(NF_ERR_DTYPE, "nf_embedding_bwd: dtypes %d -> %d", dt_out, dt_table);
+  if (!dtable || (M > 0 && (!dout || !ids)))
+    return set_error(NF_ERR_ARG, "nf_embedding_bwd: null pointer");
+  const size_t need = nf_embedding_bwd_workspace(M, D, V);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return set_error(NF_ERR_WORKSPACE, "nf_embedding_bwd: workspace %zu bytes < required %zu",
+                     workspace_bytes, need);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+#define NF_EMB(CW, CO, W, O)                                                                 \
+  if (dt_table == CW && dt_out == CO)                                                        \
+    return run_bwd<O, W>(static_cast<const O *>(dout), ids, padding_id, scale, M, D, V,      \
+                         static_cast<W *>(dtable), ws, s);
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_F32, float, float)
+  NF_EMB(NF_DTYPE_BF16, NF_DTYPE_BF16, bf16, bf16)
+  NF_EMB(NF_DTYPE_F16, NF_DTYPE_F16, f16, f16)
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_BF16, float, bf16)
+  NF_EMB(NF_DTYPE_F32, NF_DTYPE_F16, float, f16)
+#undef NF_EMB
+  return set_error(NF_ERR_DTYPE, "nf_embedding_bwd: dtypes %d -> %d", dt_out, dt_table);
+}

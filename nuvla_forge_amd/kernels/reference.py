@@ -1,13 +1,18 @@
-"""Eager PyTorch formulations of the three fused ops (``force_reference=True``).
+"""Eager PyTorch formulations of the fused ops (``force_reference=True``).
 
 Same names and semantics as ``nuvla_forge/kernels/reference.py``: the
 reference's own non-fused path, which its ``force_reference`` switch selects
 and its DiT/nuVLA models run with ``fused=False``.  These run on whatever
 device the inputs live on, through ATen; they are never chosen implicitly.
 The parity oracle the tests use is a separate NumPy restatement (``oracle/``).
+
+The last three (token log probabilities, embedding lookup, dropout) have no
+counterpart there.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn.functional as F
@@ -44,3 +49,67 @@ def chunked_cross_entropy_ref(hidden, lm_weight, targets, ignore_index=-100):
     """Unchunked mean cross entropy over hidden @ lm_weight.T (reference.py:77-96)."""
     logits = F.linear(hidden.float(), lm_weight.float())
     return F.cross_entropy(logits, targets, ignore_index=ignore_index, reduction="mean")
+
+
+def token_logprobs_ref(hidden, lm_weight, targets, top_k=0, chunk_size=1024, ignore_index=-100):
+    """(logprobs, entropy, top_logprobs, top_ids) over hidden @ lm_weight.T in fp32, rows taken
+    ``chunk_size`` at a time; the last two are None for ``top_k`` 0.  Rows whose target is
+    ``ignore_index`` or outside [0, V) give 0 (and id -1) and no gradient."""
+    v, w, parts = lm_weight.shape[0], lm_weight.float(), []
+    for at in range(0, max(hidden.shape[0], 1), chunk_size):
+        tg = targets[at:at + chunk_size]
+        live = (tg != ignore_index) & (tg >= 0) & (tg < v)
+        logp = F.linear(hidden[at:at + chunk_size].float(), w).log_softmax(-1)
+        own = logp.gather(1, torch.where(live, tg, 0)[:, None])[:, 0]
+        ent = -(logp.exp() * logp).sum(-1)
+        got = [torch.where(live, own, 0.0), torch.where(live, ent, 0.0)]
+        if top_k:
+            val, idx = torch.sort(logp.detach(), dim=-1, descending=True, stable=True)
+            got += [torch.where(live[:, None], val[:, :top_k], 0.0),
+                    torch.where(live[:, None], idx[:, :top_k], -1)]
+        parts.append(got)
+    out = [torch.cat([got[i] for got in parts]) for i in range(len(parts[0]))]
+    return tuple(out) if top_k else (*out, None, None)
+
+
+def embedding_ref(ids, table, scale, padding_idx, out_dtype):
+    """scale * table[ids] in fp32, cast to ``out_dtype``; 0 for ids outside [0, V), no gradient
+    from positions that hold ``padding_idx``."""
+    live = ((ids >= 0) & (ids < table.shape[0]))[..., None]
+    rows = table[torch.where(live[..., 0], ids, 0).long()].float()
+    if padding_idx is not None:
+        rows = torch.where((ids == padding_idx)[..., None], rows.detach(), rows)
+    return torch.where(live, rows * scale, 0.0).to(out_dtype)
+
+
+def _philox_words(seed, block, offset):
+    """The four 32-bit words of Philox4x32-10 under key ``seed`` (an int or int64 tensor) for the
+    counters (block, offset), as int64."""
+    low = 0xFFFFFFFF
+    k0, k1 = seed & low, (seed >> 32) & low
+    c0, c1 = block & low, (block >> 32) & low
+    c2, c3 = (torch.full_like(block, x & low) for x in (offset, offset >> 32))
+    for r in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # wraps; the low 64 bits are the product's
+        c0, c1, c2, c3 = (((b >> 32) & low) ^ c1 ^ ((k0 + r * 0x9E3779B9) & low), b & low,
+                          ((a >> 32) & low) ^ c3 ^ ((k1 + r * 0xBB67AE85) & low), a & low)
+    return c0, c1, c2, c3
+
+
+def dropout_keep(shape, threshold, seed, offset, device):
+    """The mask of ``fused_dropout``: True where an element is kept."""
+    n = math.prod(shape)
+    if isinstance(seed, torch.Tensor):
+        seed = seed.reshape(())
+    words = torch.stack(_philox_words(seed, torch.arange((n + 7) // 8, device=device), offset), 1)
+    parts = torch.stack((words & 0xFFFF, words >> 16), 2).reshape(-1)
+    return (parts[:n] >= threshold).view(shape)
+
+
+def dropout_ref(x, threshold, seed, offset, residual):
+    """residual + (kept ? x * 65536 / (65536 - threshold) : 0) in fp32, cast to the residual's
+    type (x's without one)."""
+    keep = dropout_keep(x.shape, threshold, seed, offset, x.device)
+    f = 65536.0 / (65536 - threshold) if threshold < 65536 else 0.0
+    y = torch.where(keep, x.float() * f, 0.0)
+    return y.to(x.dtype) if residual is None else (y + residual.float()).to(residual.dtype)

@@ -1,0 +1,263 @@
+"""Token log probabilities, embedding lookup and dropout without a GPU: the eager
+formulations that host tensors take, the generator against its published values, the
+gradient formulas against differences, the refusals of the Python entries and of the
+C ABI.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from nuvla_forge_amd import _lib
+from nuvla_forge_amd.kernels import (
+    chunked_token_logprobs,
+    embedding_lookup,
+    fused_dropout,
+)
+from nuvla_forge_amd.kernels.reference import _philox_words, dropout_keep
+from nuvla_forge_amd.kernels.utils import DeviceMismatchError
+
+from .token_ops_ref import logprobs64
+
+NF_OK, NF_ERR_ARG, NF_ERR_DTYPE, NF_ERR_WORKSPACE = 0, -1, -2, -3
+FAKE = 4096  # a non-null pointer value; every call below returns before using it
+
+
+def _err() -> str:
+    return _lib.lib().nf_last_error().decode()
+
+
+# ---------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("counter, key, want", [
+    # the known answers that the generator's authors publish (Random123, kat_vectors)
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_philox_known_answers(counter, key, want):
+    def signed(lo, hi):  # 64 bits as int64 holds them
+        x = lo | hi << 32
+        return x - (1 << 64) if x >> 63 else x
+
+    got = _philox_words(signed(*key), torch.tensor([signed(*counter[:2])]), signed(*counter[2:]))
+    assert tuple(int(w) for w in got) == want
+
+
+def test_dropout_eager_values_and_gradient():
+    x = torch.arange(1.0, 41.0).view(5, 8).requires_grad_(True)
+    r = torch.full((5, 8), 100.0)
+    keep = dropout_keep((5, 8), 16384, 7, 3, "cpu")
+    out = fused_dropout(x, 0.25, 7, offset=3, residual=r)
+    assert torch.equal(out, torch.where(keep, x.detach() * (4 / 3), 0.0) + r)
+    out.sum().backward()
+    assert torch.equal(x.grad, keep.float() * (65536 / 49152))
+    # the mask goes by the element's place, not by strides or by how the seed is given
+    y = fused_dropout(x.detach().t().contiguous().t(), 0.25, torch.tensor([7]), offset=3)
+    assert torch.equal(y, torch.where(keep, x.detach() * (4 / 3), 0.0))
+    assert not torch.equal(keep, dropout_keep((5, 8), 16384, 7, 4, "cpu"))
+    assert not torch.equal(keep, dropout_keep((5, 8), 16384, 8, 3, "cpu"))
+
+
+def test_dropout_rate():
+    """n Bernoulli draws: the kept share is within 6 standard deviations of 1 - p."""
+    n = 1 << 20
+    for p in (0.02, 0.5, 0.9):
+        t = math.floor(p * 65536 + 0.5)
+        kept = dropout_keep((n,), t, 12345, 0, "cpu").double().mean().item()
+        q = 1 - t / 65536
+        assert abs(kept - q) < 6 * math.sqrt(q * (1 - q) / n), (p, kept)
+
+
+def test_dropout_refusals():
+    x = torch.zeros(4, 4)
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="p must be"):
+            fused_dropout(x, p, 0)
+    with pytest.raises(ValueError, match="offset"):
+        fused_dropout(x, 0.1, 0, offset=-1)
+    with pytest.raises(ValueError, match="seed"):
+        fused_dropout(x, 0.1, 1 << 63)
+    with pytest.raises(ValueError, match="seed"):
+        fused_dropout(x, 0.1, torch.tensor([1, 2]))
+    with pytest.raises(ValueError, match="seed"):
+        fused_dropout(x, 0.1, torch.tensor([1.0]))
+    with pytest.raises(ValueError, match="shape mismatch"):
+        fused_dropout(x, 0.1, 0, residual=torch.zeros(4))
+    with pytest.raises(TypeError, match="residual"):
+        fused_dropout(x, 0.1, 0, residual=torch.zeros(4, 4, dtype=torch.bfloat16))
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        fused_dropout(x.double(), 0.1, 0)
+    with pytest.raises(DeviceMismatchError):
+        fused_dropout(x, 0.1, 0, residual=torch.zeros(4, 4, device="meta"))
+
+
+def test_dropout_c_abi_refusals():
+    f = _lib.lib().nf_dropout
+    ok = [FAKE, None, FAKE, 64, 100, None, 1, 0, 1, 1, None]
+    for i, bad, rc in ((3, -1, NF_ERR_ARG), (4, -1, NF_ERR_ARG), (4, 65537, NF_ERR_ARG),
+                       (7, -1, NF_ERR_ARG), (0, None, NF_ERR_ARG), (2, None, NF_ERR_ARG),
+                       (8, 3, NF_ERR_DTYPE), (9, 2, NF_ERR_DTYPE), (9, -1, NF_ERR_DTYPE),
+                       (3, 1 << 50, NF_ERR_ARG)):
+        assert f(*(ok[:i] + [bad] + ok[i + 1:])) == rc, (i, bad, _err())
+    assert f(None, None, None, 0, 100, None, 1, 0, 1, 1, None) == NF_OK  # empty: no launch
+
+
+# ---------------------------------------------------------------------------
+# embedding lookup
+# ---------------------------------------------------------------------------
+def test_embedding_eager_values_and_gradient():
+    table = torch.randn(6, 3, generator=torch.Generator().manual_seed(0)).requires_grad_(True)
+    ids = torch.tensor([[1, 5, 1], [0, -2, 6]], dtype=torch.int32)
+    out = embedding_lookup(ids, table, scale=2.0, padding_idx=0)
+    want = torch.stack([table[i] * 2 if 0 <= i < 6 else torch.zeros(3)
+                        for i in ids.flatten().tolist()]).view(2, 3, 3)
+    assert torch.equal(out, want.detach())
+    dout = torch.arange(1.0, 19.0).view(2, 3, 3)
+    out.backward(dout)
+    grad = torch.zeros(6, 3)
+    grad[1] = 2 * (dout[0, 0] + dout[0, 2])
+    grad[5] = 2 * dout[0, 1]
+    assert torch.equal(table.grad, grad)  # none from the padding id or outside the table
+    assert embedding_lookup(ids, table, out_dtype=torch.bfloat16).dtype == torch.bfloat16
+    assert embedding_lookup(ids[:0], table).shape == (0, 3, 3)
+
+
+def test_embedding_refusals():
+    table, ids = torch.zeros(6, 3), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="table"):
+        embedding_lookup(ids, torch.zeros(6))
+    with pytest.raises(ValueError, match="table"):
+        embedding_lookup(ids, torch.zeros(0, 3))
+    with pytest.raises(TypeError, match="ids"):
+        embedding_lookup(ids.float(), table)
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding_lookup(ids, table, padding_idx=6)
+    with pytest.raises(TypeError, match="table in"):
+        embedding_lookup(ids, table.bfloat16(), out_dtype=torch.float32)
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        embedding_lookup(ids, table.double())
+    with pytest.raises(DeviceMismatchError):
+        embedding_lookup(ids.to("meta"), table)
+
+
+def test_embedding_c_abi_refusals():
+    L = _lib.lib()
+    ok = [FAKE, FAKE, 64, 1.0, 16, 64, 100, FAKE, 1, 1, None]
+    for i, bad, rc in ((2, 63, NF_ERR_ARG), (4, -1, NF_ERR_ARG), (5, 0, NF_ERR_ARG),
+                       (6, 0, NF_ERR_ARG), (0, None, NF_ERR_ARG), (1, None, NF_ERR_ARG),
+                       (7, None, NF_ERR_ARG), (8, 2, NF_ERR_DTYPE), (9, 0, NF_ERR_DTYPE),
+                       (4, 1 << 31, NF_ERR_ARG)):
+        assert L.nf_embedding_fwd(*(ok[:i] + [bad] + ok[i + 1:])) == rc, (i, bad, _err())
+    need = L.nf_embedding_bwd_workspace(16, 64, 100)
+    assert need > 0 and L.nf_embedding_bwd_workspace(-1, 64, 100) == 0
+    assert L.nf_embedding_bwd_workspace(16, 1 << 23, 100) == 0
+    ok = [FAKE, FAKE, -1, 1.0, 16, 64, 100, FAKE, 1, 1, FAKE, need, None]
+    for i, bad, rc in ((4, -1, NF_ERR_ARG), (5, 0, NF_ERR_ARG), (0, None, NF_ERR_ARG),
+                       (1, None, NF_ERR_ARG), (7, None, NF_ERR_ARG), (9, 2, NF_ERR_DTYPE),
+                       (8, 0, NF_ERR_DTYPE), (10, None, NF_ERR_WORKSPACE),
+                       (10, FAKE + 8, NF_ERR_WORKSPACE), (11, need - 1, NF_ERR_WORKSPACE)):
+        assert L.nf_embedding_bwd(*(ok[:i] + [bad] + ok[i + 1:])) == rc, (i, bad, _err())
+
+
+# ---------------------------------------------------------------------------
+# token log probabilities
+# ---------------------------------------------------------------------------
+def _case(m=7, d=5, v=11, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    h, w = torch.randn(m, d, generator=g), torch.randn(v, d, generator=g)
+    t = torch.randint(0, v, (m,), generator=g)
+    t[2], t[4], t[5] = -100, v, -1
+    return h, w, t, torch.randn(m, generator=g), torch.randn(m, generator=g)
+
+
+def test_logprobs_formula_against_differences():
+    """The 64-bit gradient that the GPU tests hold the kernels to, against central
+    differences of its own values: truncation ~ eps^2, rounding ~ 2^-53 / eps."""
+    h, w, t, g, gh = (x.double() if x.is_floating_point() else x for x in _case())
+    want = logprobs64(h, w, t, g, gh)
+    eps = 1e-5
+    for name, x in (("dh", h), ("dw", w)):
+        num = torch.zeros_like(x)
+        for i in range(x.numel()):
+            val = []
+            for step in (eps, -eps):
+                y = x.clone()
+                y.view(-1)[i] += step
+                r = logprobs64(*((y, w) if name == "dh" else (h, y)), t, g, gh)
+                val.append((r["logprobs"] * g + r["entropy"] * gh).sum())
+            num.view(-1)[i] = (val[0] - val[1]) / (2 * eps)
+        assert (num - want[name]).abs().max() < 1e-8, name
+
+
+@pytest.mark.parametrize("chunk_size", [3, 1024])
+def test_logprobs_eager(chunk_size):
+    h, w, t, g, gh = _case()
+    h.requires_grad_(True), w.requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, top_k=4, chunk_size=chunk_size)
+    want = logprobs64(h, w, t, g, gh, 4)
+    dh, dw = torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh])
+    for name, x in dict(logprobs=out.logprobs, entropy=out.entropy, dh=dh, dw=dw,
+                        top_logprobs=out.top_logprobs).items():
+        assert (x.double() - want[name]).abs().max() < 5e-6, name
+    assert torch.equal(out.top_ids, want["top_ids"])
+    assert not out.top_logprobs.requires_grad
+    for row in (2, 4, 5):  # left out
+        assert out.logprobs[row] == 0 and out.entropy[row] == 0
+        assert (out.top_ids[row] == -1).all() and (dh[row] == 0).all()
+    none = chunked_token_logprobs(h, w, t)
+    assert none.top_logprobs is None and none.top_ids is None
+    assert chunked_token_logprobs(h[:0], w, t[:0], top_k=2).top_ids.shape == (0, 2)
+
+
+def test_logprobs_refusals():
+    h, w, t, *_ = _case()
+    with pytest.raises(ValueError, match="expected"):
+        chunked_token_logprobs(h[0], w, t)
+    with pytest.raises(ValueError, match="expected"):
+        chunked_token_logprobs(h, w[:, :4], t)
+    with pytest.raises(ValueError, match="targets"):
+        chunked_token_logprobs(h, w, t[:3])
+    for k in (-1, 12, 33):
+        with pytest.raises(ValueError, match="top_k"):
+            chunked_token_logprobs(h, w, t, top_k=k)
+    with pytest.raises(ValueError, match="chunk_size"):
+        chunked_token_logprobs(h, w, t, chunk_size=0)
+    with pytest.raises(ValueError, match="empty"):
+        chunked_token_logprobs(h, w[:0], t)
+    with pytest.raises(DeviceMismatchError):
+        chunked_token_logprobs(h, w.to("meta"), t)
+
+
+def test_logprobs_c_abi_refusals():
+    L = _lib.lib()
+    st, fw = (L.nf_token_logprobs_state_bytes(16, 64, 100, 1),
+              L.nf_token_logprobs_fwd_workspace(16, 64, 100, 1024, 5, 1))
+    bw = L.nf_token_logprobs_bwd_workspace(16, 64, 100, 1024, 1)
+    assert st > 0 and fw > 0 and bw > 0
+    assert L.nf_token_logprobs_state_bytes(16, 64, 100, 2) == 0
+    assert L.nf_token_logprobs_fwd_workspace(16, 64, 100, 1024, 33, 1) == 0
+    assert L.nf_token_logprobs_fwd_workspace(16, 64, 4, 1024, 5, 1) == 0
+    assert L.nf_token_logprobs_bwd_workspace(16, 64, 100, 0, 1) == 0
+    ok = [FAKE, FAKE, FAKE, 16, 64, 100, -100, 1024, 5, 1, FAKE, FAKE, FAKE, FAKE, FAKE, st, FAKE,
+          fw, None]
+    bad = [(3, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (5, 1 << 32, NF_ERR_ARG), (7, 0, NF_ERR_ARG),
+           (8, -1, NF_ERR_ARG), (8, 33, NF_ERR_ARG), (9, 2, NF_ERR_DTYPE),
+           (14, FAKE + 8, NF_ERR_WORKSPACE), (15, st - 1, NF_ERR_WORKSPACE),
+           (16, None, NF_ERR_WORKSPACE), (17, fw - 1, NF_ERR_WORKSPACE)]
+    bad += [(i, None, NF_ERR_ARG) for i in (0, 1, 2, 10, 11, 12, 13, 14)]
+    for i, x, rc in bad:
+        assert L.nf_token_logprobs_fwd(*(ok[:i] + [x] + ok[i + 1:])) == rc, (i, x, _err())
+    ok = [FAKE, 16, 64, 100, 1024, 1, FAKE, st, FAKE, None, FAKE, 1, FAKE, 1, FAKE, bw, None]
+    bad = [(1, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (5, 2, NF_ERR_DTYPE), (0, None, NF_ERR_ARG),
+           (6, None, NF_ERR_ARG), (7, st - 1, NF_ERR_WORKSPACE), (11, 3, NF_ERR_DTYPE),
+           (13, -1, NF_ERR_DTYPE), (14, None, NF_ERR_WORKSPACE), (15, bw - 1, NF_ERR_WORKSPACE)]
+    for i, x, rc in bad:
+        assert L.nf_token_logprobs_bwd(*(ok[:i] + [x] + ok[i + 1:])) == rc, (i, x, _err())
+    nothing = ok[:10] + [None, 1, None, 1] + ok[14:]
+    assert L.nf_token_logprobs_bwd(*nothing) == NF_OK  # no gradient wanted: no launch

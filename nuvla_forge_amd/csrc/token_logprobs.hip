@@ -12,7 +12,8 @@
 // Forward (nf_token_logprobs_fwd):
 //   1. ce_compact: the valid rows in order.  lp_gather: Hc = hidden[rows], and zeros (id
 //      -1) into the outputs of the other rows.
-//   2. per chunk of rows: the logits, then lp_rows: a block per row.
+//   2. per chunk of rows: lp_logits, the logits tile by tile, of which statistics and
+//      records of strips are left; lp_finish: the row's values from those.
 // Backward (nf_token_logprobs_bwd), with g and h the upstream gradients of a row's logprob
 // and entropy H:
 //   dz = g (onehot - p) - h p (z - lse + H)
@@ -81,93 +82,377 @@ __global__ __launch_bounds__(kGatherThreads) void lp_gather_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// 2. a row's outputs from its logits: the maximum, then S = sum exp(z - max) and
-// T = sum (z - max) exp(z - max) (log p and the entropy follow: lse = max + log S,
-// H = log S - T / S), then the top_k largest, each the largest entry after the one
-// before it in the order (value down, column up).
+// 2. The logits, never stored.  What a pass leaves of a token's logits, strip by strip of
+// the vocabulary:
+//   Stat, per statistics strip: the maximum mx, S = sum exp(z - mx) and
+//     T = sum (z - mx) exp(z - mx);
+//   Rec (with top_k), per strip of 32 logits: the largest (the first of equals), its place
+//     in the strip, and the second largest, rounded up to 16 bits.
+// A strip's 32 columns are column(strip, c), c = 0 .. 31, rising in c.  The top_k largest
+// logits of a row lie in the top_k strips whose largest come first; a second largest that
+// could be among them makes lp_finish form that strip's logits again, in the same order of
+// sums and so to the same bits.
 // ---------------------------------------------------------------------------
-constexpr int kRowThreads = 256;
+struct __attribute__((aligned(16))) Stat {
+  float mx, s, t, pad;
+};
+struct __attribute__((aligned(8))) Rec {
+  float first;
+  uint32_t rest;  // bits 31..16: the second largest as the top half of an fp32; 5..0: place
+};
+constexpr uint32_t kNoPlace = 63;  // no logit of the strip compares (all NaN)
 
+// The least bf16 value >= x, as bits 31..16 (what is left of a NaN does not matter).
+__device__ __forceinline__ uint32_t bf16_up(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u >> 31 ? u : u + 0xffffu) & 0xffff0000u;
+}
+
+// The columns of a strip.  Pass over block tiles (wtm: rows of a wavefront's tile): a strip
+// is 32 of the logits that one lane holds for a token, two 32-row MFMA tiles of its half of
+// the lanes; skinny pass (wtm 0): 32 columns in a row.
+struct Strips {
+  int wtm;
+  __host__ __device__ int per_stat() const { return wtm ? wtm / 32 : 1; }
+  __device__ __forceinline__ int column(int strip, int c) const {
+    if (!wtm) return strip * 32 + c;
+    const int per = wtm / 32, stat = strip / per, k = strip % per;  // k = half * (per / 2) + q
+    const int half = k / (per / 2), q = k % (per / 2);
+    return stat * wtm + (2 * q + (c >> 4)) * 32 + 8 * ((c & 15) >> 2) + 4 * half + (c & 3);
+  }
+};
+
+// One block tile: acc = W_tile Hc_tile^T (rows: vocabulary, columns: tokens), so a lane
+// holds 16 TM logits of each of its TN tokens and the strip's values are reductions in
+// registers.  stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
+template <class C, bool BUF, bool TOP>
+__global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
+    const typename C::TI *W, const typename C::TI *Hc, int64_t V, int64_t D, int64_t j0,
+    int64_t crows, const int *n_ptr, const int *tcol, Stat *stats, int nstat, Rec *recs,
+    float *tgt, int vtiles, int ttiles) {
+  __shared__ __attribute__((aligned(16))) char smem[C::LDS_BYTES];
+  int vt, tt;
+  gemm::group_tile(gemm::xcd_order(blockIdx.x, vtiles * ttiles), vtiles, ttiles,
+                   gemm::kTileGroup, vt, tt);
+  const int64_t cnt = chunk_count(n_ptr, j0, crows);
+  const int64_t v0 = (int64_t)vt * C::BM;
+  const int64_t t0 = (int64_t)tt * C::BN;
+  if (t0 >= cnt) return;
+  floatx16 acc[C::TM][C::TN];
+  gemm::mainloop<C, BUF>(W, D, Hc + j0 * D, D, V, cnt, D, v0, t0, smem, acc);
+
+  const int l = threadIdx.x & 63, half = l >> 5;
+  const int w = threadIdx.x >> 6, wm = w / C::WN, wn = w % C::WN;
+  const int64_t vtile0 = v0 + wm * C::WTM;
+  const int64_t crow0 = vtile0 + 4 * half;
+  const int stat = vt * C::WM + wm;
+  // rows past the vocabulary: -inf, which adds nothing and comes after any logit
+  if (vtile0 + C::WTM > V) {
+    const int vlim = (int)(V - crow0 < C::WTM ? V - crow0 : C::WTM);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (i * 32 + 8 * (r >> 2) + (r & 3) >= vlim) acc[i][j][r] = -INFINITY;
+  }
+  constexpr int NS = C::TM / 2;  // strips of a lane and token
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) {
+    const int64_t tok = t0 + wn * C::WTN + j * 32 + (l & 31);
+    float mx = -INFINITY;
+    if constexpr (TOP) {
+      float first[NS], second[NS];
+      uint32_t place[NS];
+#pragma unroll
+      for (int q = 0; q < NS; ++q) {
+        first[q] = second[q] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float x = acc[2 * q + (c >> 4)][j][c & 15];
+          second[q] = __builtin_amdgcn_fmed3f(first[q], second[q], x);
+          first[q] = fmaxf(first[q], x);
+        }
+        place[q] = kNoPlace;
+#pragma unroll
+        for (int c = 31; c >= 0; --c)
+          place[q] = acc[2 * q + (c >> 4)][j][c & 15] == first[q] ? (uint32_t)c : place[q];
+        mx = fmaxf(mx, first[q]);
+      }
+      if (tok < cnt) {
+        Rec *dst = recs + (tok * nstat + stat) * (2 * NS) + half * NS;
+#pragma unroll
+        for (int q = 0; q < NS; ++q) dst[q] = Rec{first[q], bf16_up(second[q]) | place[q]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[i][j][r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (tok < cnt) {  // the target logit, from the one lane that holds it
+      const int64_t loc64 = (int64_t)tcol[j0 + tok] - vtile0;
+      const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
+      if (loc >= 0 && ((loc >> 2) & 1) == half) {
+        const int want = ((loc >> 5) << 4) | (((loc & 31) >> 3) << 2) | (loc & 3);
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z = (i * 16 + r == want) ? acc[i][j][r] : z;
+        tgt[tok] = z;
+      }
+    }
+    float s = 0.f, t = 0.f;
+    const float base = mx == -INFINITY ? 0.f : mx;  // a strip of -inf (and NaN) alone
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = acc[i][j][r] - base;
+        const float e = exp_f32(x);
+        s += e;
+        t += fmaxf(x, kFar) * e;  // e is 0 where x is -inf, and a NaN where it is one
+      }
+    s += __shfl_xor(s, 32);
+    t += __shfl_xor(t, 32);
+    if (half == 0 && tok < cnt) stats[tok * nstat + stat] = Stat{mx, s, t, 0.f};
+  }
+}
+
+// A row of at most 16 tokens against 16 vocabulary rows, k in order in steps of 32, as the
+// block tiles' K loop takes them: a: rows of W, b: rows of H.  The lane supplies and k-vectors
+// are those of v_mfma_f32_16x16x32_bf16: row lane % 16, k 8 (lane / 16) .. + 7.
+template <typename TI>
+struct Dot16;
+template <>
+struct Dot16<bf16> {
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  struct Frag {
+    u32x4 v;
+  };
+  // `p`: the lane's row; rows that do not exist are null (zeros)
+  template <bool VK>
+  __device__ __forceinline__ static Frag load(const bf16 *p, int64_t k, int64_t D) {
+    return Frag{load_vec<bf16, VK>(p, 0, p ? 0 : 1, 1, k + 8 * ((threadIdx.x & 63) >> 4), D)};
+  }
+  __device__ __forceinline__ void add(const Frag &a, const Frag &b) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v),
+                                                  __builtin_bit_cast(bf16x8, b.v), acc, 0, 0, 0);
+  }
+  __device__ __forceinline__ floatx4 done() const { return acc; }
+};
+template <>
+struct Dot16<float> {  // the products of mainloop_split, in its order
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f}, low = {0.f, 0.f, 0.f, 0.f};
+  struct Frag {
+    u32x4 part[3];
+  };
+  template <bool VK>
+  __device__ __forceinline__ static Frag load(const float *p, int64_t k, int64_t D) {
+    u32x4 x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      x[h] = load_vec<float, VK>(p, 0, p ? 0 : 1, 1, k + 8 * ((threadIdx.x & 63) >> 4) + 4 * h, D);
+    Frag f;
+    split8(x, f.part);
+    return f;
+  }
+  __device__ __forceinline__ static floatx4 mul(const u32x4 &a, const u32x4 &b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ void add(const Frag &a, const Frag &b) {
+    acc = mul(a.part[0], b.part[0], acc);
+    low = mul(a.part[1], b.part[0], low);
+    low = mul(a.part[2], b.part[0], low);
+    low = mul(a.part[0], b.part[1], low);
+    low = mul(a.part[1], b.part[1], low);
+    low = mul(a.part[0], b.part[2], low);
+  }
+  __device__ __forceinline__ floatx4 done() const {
+    floatx4 r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r[q] = __builtin_isfinite(acc[q]) ? acc[q] + low[q] : acc[q];
+    return r;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// 3. a row's outputs, one wavefront a row: the statistics joined in a fixed order
+// (log p and the entropy follow: lse = mx + log S, H = log S - T / S), then the
+// alternatives from the strips' records.
+// ---------------------------------------------------------------------------
+constexpr int kFinishThreads = 256;
+
+__device__ __forceinline__ Stat join(const Stat &a, const Stat &b) {
+  const float m = fmaxf(a.mx, b.mx), base = m == -INFINITY ? 0.f : m;
+  const float xa = fmaxf(a.mx - base, kFar), xb = fmaxf(b.mx - base, kFar);
+  const float ea = exp_f32(a.mx - base), eb = exp_f32(b.mx - base);
+  return Stat{m, a.s * ea + b.s * eb, (a.t + a.s * xa) * ea + (b.t + b.s * xb) * eb, 0.f};
+}
+
+// (va, column ia) comes before (vb, ib): the larger value, of equals the lower column
 __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) {
   return va > vb || (va == vb && ia < ib);
 }
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float *sh, F op) {
-  for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d));
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh[0];
-  for (int k = 1; k < kRowThreads / 64; ++k) v = op(v, sh[k]);
-  __syncthreads();
-  return v;
+// the wavefront's first (v, i) in that order, in every lane; `tag` goes with it
+__device__ __forceinline__ void wave_first(float &v, int &i, int &tag) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float ov = __shfl_xor(v, d);
+    const int oi = __shfl_xor(i, d), ot = __shfl_xor(tag, d);
+    if (before(ov, oi, v, i)) {
+      v = ov;
+      i = oi;
+      tag = ot;
+    }
+  }
 }
 
-__global__ __launch_bounds__(kRowThreads) void lp_rows_kernel(
-    const float *__restrict__ Z, int64_t ldz, int64_t V, const int *n_ptr, int64_t j0,
-    int64_t crows, const int *__restrict__ rows, const int *__restrict__ tcol,
-    float *__restrict__ lse_out, float *__restrict__ ent_out, RowOut out) {
-  __shared__ float sh[kRowThreads / 64];
-  __shared__ float sv[kRowThreads / 64];
-  __shared__ int si[kRowThreads / 64];
-  const int64_t row = blockIdx.x;
+template <typename TI, bool VK>
+__global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
+    const TI *W, const TI *Hc, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
+    const Rec *__restrict__ recs, Strips strips, const float *__restrict__ tgt, const int *n_ptr,
+    int64_t j0, int64_t crows, const int *__restrict__ rows, float *__restrict__ lse_out,
+    float *__restrict__ ent_out, RowOut out) {
+  constexpr int kWaves = kFinishThreads / 64;
+  // the logits of strips formed again, 32 a strip; what is left of a row's own strips
+  __shared__ float again[kWaves][kMaxTop * 32];
+  __shared__ float first_v[kWaves][kMaxTop];
+  __shared__ int first_i[kWaves][kMaxTop], first_s[kWaves][kMaxTop], slot[kWaves][kMaxTop];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * kWaves + w;
   if (row >= chunk_count(n_ptr, j0, crows)) return;
-  const float *z = Z + row * ldz;
-  float mx = -INFINITY;
-  for (int64_t c = threadIdx.x; c < V; c += kRowThreads) mx = fmaxf(mx, z[c]);
-  mx = block_reduce(mx, sh, [](float a, float b) { return fmaxf(a, b); });
-  float s = 0.f, t = 0.f;
-  for (int64_t c = threadIdx.x; c < V; c += kRowThreads) {
-    const float x = z[c] - mx;
-    const float e = exp_f32(x);
-    s += e;
-    t += x < kFar ? 0.f : x * e;
-  }
-  auto add = [](float a, float b) { return a + b; };
-  s = block_reduce(s, sh, add);
-  t = block_reduce(t, sh, add);
-  const float ls = log_f32(s), lse = mx + ls, ent = ls - t / s;
+  const Stat *st = stats + row * nstat;
+  Stat a{-INFINITY, 0.f, 0.f, 0.f};
+  for (int k = l; k < nstat; k += 64) a = join(a, st[k]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+    a = join(a, Stat{__shfl_xor(a.mx, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f});
+  const float ls = log_f32(a.s), lse = a.mx + ls, ent = ls - a.t / a.s;
   const int64_t m = rows[j0 + row];
-  if (threadIdx.x == 0) {
+  if (l == 0) {
     lse_out[j0 + row] = lse;
     ent_out[j0 + row] = ent;
-    out.logprob[m] = z[tcol[j0 + row]] - lse;
+    out.logprob[m] = tgt[row] - lse;
     out.entropy[m] = ent;
   }
+  const int K = out.top_k;
+  if (K == 0) return;
+  // the K strips whose first logits come first, in order
+  const int nrec = nstat * strips.per_stat();
+  const Rec *rc = recs + row * nrec;
   float pv = INFINITY;
-  int pi = -1;
-  for (int k = 0; k < out.top_k; ++k) {
+  int pi = -1, found = 0;
+  for (int k = 0; k < K; ++k) {
     float bv = -INFINITY;
-    int bi = 0x7fffffff;
-    for (int64_t c = threadIdx.x; c < V; c += kRowThreads) {
-      const float v = z[c];
-      if (before(pv, pi, v, (int)c) && before(v, (int)c, bv, bi)) {
-        bv = v;
-        bi = (int)c;
+    int bi = 0x7fffffff, bs = -1;
+    for (int q = l; q < nrec; q += 64) {
+      const Rec r = rc[q];
+      const uint32_t place = r.rest & 63u;
+      if (place == kNoPlace) continue;
+      const int col = strips.column(q, (int)place);
+      if (col < V && before(pv, pi, r.first, col) && before(r.first, col, bv, bi)) {
+        bv = r.first;
+        bi = col;
+        bs = q;
       }
     }
-    for (int d = 32; d; d >>= 1) {
-      const float ov = __shfl_xor(bv, d);
-      const int oi = __shfl_xor(bi, d);
-      if (before(ov, oi, bv, bi)) {
-        bv = ov;
-        bi = oi;
-      }
+    wave_first(bv, bi, bs);
+    if (bs < 0) break;  // the same in every lane
+    if (l == 0) {
+      first_v[w][k] = bv;
+      first_i[w][k] = bi;
+      first_s[w][k] = bs;
     }
-    if ((threadIdx.x & 63) == 0) {
-      sv[threadIdx.x >> 6] = bv;
-      si[threadIdx.x >> 6] = bi;
+    pv = bv;
+    pi = bi;
+    ++found;
+  }
+  // a strip whose second logit may come before the last of them is formed again.  With
+  // fewer than K strips every strip is among them, and each is formed again.
+  const float last = found < K ? -INFINITY : pv;
+  int nagain = 0;
+  for (int k = 0; k < found; ++k) {
+    const int strip = first_s[w][k];
+    const float second = __uint_as_float(rc[strip].rest & 0xffff0000u);
+    if (!(second >= last)) {
+      if (l == 0) slot[w][k] = -1;
+      continue;
     }
-    __syncthreads();
-    for (int q = 0; q < kRowThreads / 64; ++q)
-      if (before(sv[q], si[q], bv, bi)) {
-        bv = sv[q];
-        bi = si[q];
+    const TI *hrow = Hc + (j0 + row) * D;
+    Dot16<TI> acc[2];
+    const TI *wrow[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int col = strips.column(strip, 16 * h + (l & 15));
+      wrow[h] = col < V ? W + (int64_t)col * D : nullptr;
+    }
+    for (int64_t kk = 0; kk < D; kk += 32) {
+      const auto b = Dot16<TI>::template load<VK>(hrow, kk, D);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc[h].add(Dot16<TI>::template load<VK>(wrow[h], kk, D), b);
+    }
+    // every column of the product is this token: lane l has places 4 (l / 16) .. + 3
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floatx4 z = acc[h].done();
+      if ((l & 15) == 0)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) again[w][nagain * 32 + 16 * h + 4 * (l >> 4) + q] = z[q];
+    }
+    if (l == 0) slot[w][k] = nagain;
+    ++nagain;
+  }
+  // one wavefront's own LDS: its writes are done before its reads below
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  // the K first of those strips' logits, in order
+  pv = INFINITY;
+  pi = -1;
+  for (int k = 0; k < K; ++k) {
+    float bv = -INFINITY;
+    int bi = 0x7fffffff, tag = -1;
+    if (nagain == 0) {
+      if (k < found) {
+        bv = first_v[w][k];
+        bi = first_i[w][k];
+        tag = 0;
       }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      out.top_lp[m * out.top_k + k] = bi < V ? bv - lse : __builtin_nanf("");
-      out.top_id[m * out.top_k + k] = bi < V ? bi : -1;
+    } else {
+      for (int q = l; q < found * 32; q += 64) {
+        const int f = q >> 5, c = q & 31, sl = slot[w][f];
+        float v;
+        int col;
+        if (sl >= 0) {
+          v = again[w][sl * 32 + c];
+          col = strips.column(first_s[w][f], c);
+        } else {
+          if (c) continue;
+          v = first_v[w][f];
+          col = first_i[w][f];
+        }
+        if (col < V && before(pv, pi, v, col) && before(v, col, bv, bi)) {
+          bv = v;
+          bi = col;
+          tag = 0;
+        }
+      }
+      wave_first(bv, bi, tag);
+    }
+    if (l == 0) {
+      out.top_lp[m * K + k] = tag < 0 ? __builtin_nanf("") : bv - lse;
+      out.top_id[m * K + k] = tag < 0 ? -1 : bi;
+    }
+    if (tag < 0) {  // none left: they compare with nothing
+      pv = -INFINITY;
+      pi = 0x7fffffff;
+      continue;
     }
     pv = bv;
     pi = bi;
@@ -250,9 +535,9 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float x = acc[i][j][r] - lse;
-        x = x < kFar ? kFar : x;  // a NaN stays one
-        const float dz = exp_f32(x) * (a - h * x);
+        const float x = acc[i][j][r] - lse;
+        // exp is 0 where x is -inf, and a NaN where it is one
+        const float dz = exp_f32(x) * (a - h * fmaxf(x, kFar));
         acc[i][j][r] = i * 16 + r == want ? dz + g : dz;
       }
     store.column(j, acc);
@@ -300,18 +585,27 @@ struct View {
         Hc(reinterpret_cast<TI *>(s + L.hc)) {}
 };
 
+// A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
+// the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
 struct FwdPlan {
-  int64_t crows, ldz;
-  size_t z, total;
+  int64_t crows;
+  int nstat, vtiles;
+  size_t stats, recs, tgt, total;
 };
 template <typename TI>
-FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows) {
+FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k) {
+  using C = MainCfg<TI>;
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
-  p.crows = chunk_rows < mcap ? round_up(chunk_rows, 256) : mcap;
-  p.ldz = round_up(V, 8);
-  p.z = 0;
-  p.total = align256((size_t)p.crows * p.ldz * sizeof(float));
+  p.crows = chunk_rows < mcap / 8 ? round_up(8 * chunk_rows, 256) : mcap;
+  p.vtiles = (int)((V + C::BM - 1) / C::BM);
+  p.nstat = p.vtiles * C::WM;
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
+  p.stats = take((size_t)p.crows * p.nstat * sizeof(Stat));
+  p.recs = take(top_k ? (size_t)p.crows * p.nstat * (C::WTM / 32) * sizeof(Rec) : 0);
+  p.tgt = take((size_t)p.crows * sizeof(float));
+  p.total = o;
   return p;
 }
 
@@ -321,8 +615,10 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
             hipStream_t s) {
   using C = MainCfg<TI>;
   const View<TI> S(state_layout<TI>(M, D), state);
-  const FwdPlan P = fwd_plan<TI>(M, V, chunk_rows);
-  float *Z = reinterpret_cast<float *>(ws + P.z);
+  const FwdPlan P = fwd_plan<TI>(M, V, chunk_rows, out.top_k);
+  Stat *stats = reinterpret_cast<Stat *>(ws + P.stats);
+  Rec *recs = reinterpret_cast<Rec *>(ws + P.recs);
+  float *tgt = reinterpret_cast<float *>(ws + P.tgt);
   int e;
   ce::ce_compact_kernel<<<1, ce::kCompactThreads, 0, s>>>(targets, M, V, ignore_index, S.rows,
                                                           S.tcol, S.pos, S.n, S.inv, nullptr);
@@ -337,19 +633,38 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
     lp_gather_kernel<TI, false><<<(unsigned)blocks, kGatherThreads, 0, s>>>(H, D, S.rows, S.pos,
                                                                             S.n, M, S.Hc, out);
   if ((e = check_launch("lp_gather"))) return e;
+  const bool vk = buf_ok<TI>(S.Hc, D, M, D) && buf_ok<TI>(W, D, V, D);
+  const bool vw = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(W);
+  const Strips strips{C::WTM};
   for (int64_t j0 = 0; j0 < M; j0 += P.crows) {
     const int64_t rows = M - j0 < P.crows ? M - j0 : P.crows;
-    auto jz = make_job<C>(S.Hc + j0 * D, D, W, D, nullptr, Z, NF_DTYPE_F32, nullptr, P.ldz, rows,
-                          V, D);
-    jz.dyn = S.n;
-    jz.dyn_base = j0;
-    jz.dyn_rows = 1;
-    auto none = jz;
-    none.tiles = 0;
-    if ((e = launch_gemm_store<C>(jz, none, s))) return e;
-    lp_rows_kernel<<<(unsigned)rows, kRowThreads, 0, s>>>(Z, P.ldz, V, S.n, j0, rows, S.rows,
-                                                          S.tcol, S.lse, S.ent, out);
-    if ((e = check_launch("lp_rows"))) return e;
+    const int ttiles = (int)((rows + C::BN - 1) / C::BN);
+    const unsigned grid = (unsigned)(P.vtiles * ttiles);
+#define NF_LP_LOGITS(BUF, TOP)                                                                \
+  lp_logits_kernel<C, BUF, TOP><<<grid, C::NT, 0, s>>>(W, S.Hc, V, D, j0, rows, S.n, S.tcol,  \
+                                                       stats, P.nstat, recs, tgt, P.vtiles,   \
+                                                       ttiles)
+    if (vk && out.top_k)
+      NF_LP_LOGITS(true, true);
+    else if (vk)
+      NF_LP_LOGITS(true, false);
+    else if (out.top_k)
+      NF_LP_LOGITS(false, true);
+    else
+      NF_LP_LOGITS(false, false);
+#undef NF_LP_LOGITS
+    if ((e = check_launch("lp_logits"))) return e;
+    const unsigned fin = (unsigned)((rows + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
+#define NF_LP_FINISH(VK)                                                                      \
+  lp_finish_kernel<TI, VK><<<fin, kFinishThreads, 0, s>>>(W, S.Hc, V, D, stats, P.nstat, recs, \
+                                                          strips, tgt, S.n, j0, rows, S.rows, \
+                                                          S.lse, S.ent, out)
+    if (vw)
+      NF_LP_FINISH(true);
+    else
+      NF_LP_FINISH(false);
+#undef NF_LP_FINISH
+    if ((e = check_launch("lp_finish"))) return e;
   }
   return NF_OK;
 }
@@ -460,8 +775,8 @@ extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t 
   if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype) || top_k < 0 ||
       top_k > kMaxTop || top_k > V)
     return 0;
-  return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows).total
-                                : fwd_plan<float>(M, V, chunk_rows).total;
+  return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows, top_k).total
+                                : fwd_plan<float>(M, V, chunk_rows, top_k).total;
 }
 
 extern "C" size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,

@@ -108,17 +108,17 @@ __device__ __forceinline__ uint32_t bf16_up(float x) {
   return (u >> 31 ? u : u + 0xffffu) & 0xffff0000u;
 }
 
-// The columns of a strip.  Pass over block tiles (wtm: rows of a wavefront's tile): a strip
-// is 32 of the logits that one lane holds for a token, two 32-row MFMA tiles of its half of
-// the lanes; skinny pass (wtm 0): 32 columns in a row.
+// The columns of a strip.  Pass over block tiles (2^lw strips to a statistics strip, which is
+// a wavefront's 32 << lw rows): a strip is 32 of the logits that one lane holds for a token, two
+// 32-row MFMA tiles of its half of the lanes; skinny pass (lw 0): 32 columns in a row.
 struct Strips {
-  int wtm;
-  __host__ __device__ int per_stat() const { return wtm ? wtm / 32 : 1; }
+  int lw;
+  __host__ __device__ int per_stat() const { return 1 << lw; }
   __device__ __forceinline__ int column(int strip, int c) const {
-    if (!wtm) return strip * 32 + c;
-    const int per = wtm / 32, stat = strip / per, k = strip % per;  // k = half * (per / 2) + q
-    const int half = k / (per / 2), q = k % (per / 2);
-    return stat * wtm + (2 * q + (c >> 4)) * 32 + 8 * ((c & 15) >> 2) + 4 * half + (c & 3);
+    if (!lw) return strip * 32 + c;
+    const int stat = strip >> lw, k = strip & ((1 << lw) - 1);  // k = half << (lw - 1) | q
+    const int half = k >> (lw - 1), q = k & ((1 << (lw - 1)) - 1);
+    return (stat << (lw + 5)) + (2 * q + (c >> 4)) * 32 + 8 * ((c & 15) >> 2) + 4 * half + (c & 3);
   }
 };
 
@@ -280,6 +280,121 @@ struct Dot16<float> {  // the products of mainloop_split, in its order
   }
 };
 
+// A row's target as the call gives it: its column, or -1 where the row does not count.
+__device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, int64_t V,
+                                             int64_t ignore_index) {
+  const int64_t t = targets[m];
+  return t != ignore_index && t >= 0 && t < V ? (int)t : -1;
+}
+
+// The logits of at most 16 NT rows, hidden used as it lies (no compaction).  What bounds it is
+// reading W once, so a wavefront streams 32 rows of W past the matrix pipe straight from
+// memory, kDepth steps of 32 k loaded ahead, and the hidden rows come from the caches.  A
+// wavefront's 32 columns are one strip: for token lane % 16 (+ 16 nt) a lane has columns
+// 16 h + 4 (lane / 16) + q, joined over the four lane groups.  V 32000, D 2048, 8 rows: see
+// nf_token_logprobs_fwd's dispatch.
+constexpr int kSkinnyThreads = 256, kSkinnyRows = 64;
+
+template <typename TI, int NT, bool VK>
+__global__ __launch_bounds__(kSkinnyThreads) void lp_skinny_kernel(
+    const TI *__restrict__ W, const TI *__restrict__ H, const int64_t *__restrict__ targets,
+    int64_t M, int64_t V, int64_t D, int64_t ignore_index, Stat *__restrict__ stats, int nstat,
+    Rec *__restrict__ recs, float *__restrict__ tgt) {
+  using Frag = typename Dot16<TI>::Frag;
+  const int l = threadIdx.x & 63;
+  const int64_t strip = (int64_t)blockIdx.x * (kSkinnyThreads / 64) + (threadIdx.x >> 6);
+  const int64_t v0 = strip * 32;
+  if (v0 >= V) return;
+  const TI *wrow[2], *hrow[NT];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t v = v0 + 16 * h + (l & 15);
+    wrow[h] = v < V ? W + v * D : nullptr;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t m = 16 * n + (l & 15);
+    hrow[n] = m < M ? H + m * D : nullptr;
+  }
+  Dot16<TI> acc[2][NT];
+  constexpr int kDepth = sizeof(TI) == 2 ? (NT == 1 ? 8 : NT == 2 ? 4 : 2) : 2;
+  for (int64_t k0 = 0; k0 < D; k0 += 32 * kDepth) {
+    Frag a[kDepth][2], b[kDepth][NT];
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        a[u][h] = Dot16<TI>::template load<VK>(wrow[h], k0 + 32 * u, D);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        b[u][n] = Dot16<TI>::template load<VK>(hrow[n], k0 + 32 * u, D);
+    }
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[h][n].add(a[u][h], b[u][n]);
+  }
+  const int grp = l >> 4;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t tok = 16 * n + (l & 15);
+    float z[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floatx4 d = acc[h][n].done();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        z[4 * h + q] = v0 + 16 * h + 4 * grp + q < V ? d[q] : -INFINITY;
+    }
+    float first = -INFINITY, second = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      second = __builtin_amdgcn_fmed3f(first, second, z[e]);
+      first = fmaxf(first, z[e]);
+    }
+    int place = (int)kNoPlace;
+#pragma unroll
+    for (int e = 7; e >= 0; --e)
+      place = z[e] == first ? 16 * (e >> 2) + 4 * grp + (e & 3) : place;
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+      const float of = __shfl_xor(first, d), os = __shfl_xor(second, d);
+      const int op = __shfl_xor(place, d);
+      second = fmaxf(fminf(first, of), fmaxf(second, os));
+      place = of > first || (of == first && op < place) ? op : place;
+      first = fmaxf(first, of);
+    }
+    const float base = first == -INFINITY ? 0.f : first;
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = z[e] - base;
+      const float ex = exp_f32(x);
+      s += ex;
+      t += fmaxf(x, kFar) * ex;
+    }
+    s += __shfl_xor(s, 16);
+    t += __shfl_xor(t, 16);
+    s += __shfl_xor(s, 32);
+    t += __shfl_xor(t, 32);
+    if (tok >= M) continue;
+    if (grp == 0) {
+      stats[tok * nstat + strip] = Stat{first, s, t, 0.f};
+      if (recs) recs[tok * nstat + strip] = Rec{first, bf16_up(second) | (uint32_t)place};
+    }
+    const int64_t loc = (int64_t)target_column(targets, tok, V, ignore_index) - v0;
+    if (loc >= 0 && loc < 32 && ((loc & 15) >> 2) == grp) {
+      const int want = 4 * (int)(loc >> 4) + (int)(loc & 3);
+      float x = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x = e == want ? z[e] : x;
+      tgt[tok] = x;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // 3. a row's outputs, one wavefront a row: the statistics joined in a fixed order
 // (log p and the entropy follow: lse = mx + log S, H = log S - T / S), then the
@@ -313,42 +428,22 @@ __device__ __forceinline__ void wave_first(float &v, int &i, int &tag) {
   }
 }
 
-template <typename TI, bool VK>
-__global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
-    const TI *W, const TI *Hc, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
-    const Rec *__restrict__ recs, Strips strips, const float *__restrict__ tgt, const int *n_ptr,
-    int64_t j0, int64_t crows, const int *__restrict__ rows, float *__restrict__ lse_out,
-    float *__restrict__ ent_out, RowOut out) {
-  constexpr int kWaves = kFinishThreads / 64;
-  // the logits of strips formed again, 32 a strip; what is left of a row's own strips
-  __shared__ float again[kWaves][kMaxTop * 32];
-  __shared__ float first_v[kWaves][kMaxTop];
-  __shared__ int first_i[kWaves][kMaxTop], first_s[kWaves][kMaxTop], slot[kWaves][kMaxTop];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + w;
-  if (row >= chunk_count(n_ptr, j0, crows)) return;
-  const Stat *st = stats + row * nstat;
-  Stat a{-INFINITY, 0.f, 0.f, 0.f};
-  for (int k = l; k < nstat; k += 64) a = join(a, st[k]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1)
-    a = join(a, Stat{__shfl_xor(a.mx, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f});
-  const float ls = log_f32(a.s), lse = a.mx + ls, ent = ls - a.t / a.s;
-  const int64_t m = rows[j0 + row];
-  if (l == 0) {
-    lse_out[j0 + row] = lse;
-    ent_out[j0 + row] = ent;
-    out.logprob[m] = tgt[row] - lse;
-    out.entropy[m] = ent;
-  }
-  const int K = out.top_k;
-  if (K == 0) return;
-  // the K strips whose first logits come first, in order
-  const int nrec = nstat * strips.per_stat();
-  const Rec *rc = recs + row * nrec;
-  float pv = INFINITY;
-  int pi = -1, found = 0;
-  for (int k = 0; k < K; ++k) {
+// A row's chosen strips, in the order of their first logits, and the logits that can be among
+// its top_k: the firsts of strips that have no other, all of those that were formed again.
+struct Chosen {
+  float v[kMaxTop];
+  int strip[kMaxTop];
+  float cand_v[kMaxTop * 32];
+  int cand_col[kMaxTop * 32];
+};
+
+// The strips whose first logits come first among those after (pv, pi), from entry `found` on;
+// how many there are then.  Every round reads the records again.
+__device__ __forceinline__ int choose_slow(const Rec *rc, int nrec, const Strips &strips,
+                                           int64_t V, int K, Chosen &ch, int found, float pv,
+                                           int pi) {
+  const int l = threadIdx.x & 63;
+  for (; found < K; ++found) {
     float bv = -INFINITY;
     int bi = 0x7fffffff, bs = -1;
     for (int q = l; q < nrec; q += 64) {
@@ -365,37 +460,204 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     wave_first(bv, bi, bs);
     if (bs < 0) break;  // the same in every lane
     if (l == 0) {
-      first_v[w][k] = bv;
-      first_i[w][k] = bi;
-      first_s[w][k] = bs;
+      ch.v[found] = bv;
+      ch.strip[found] = bs;
     }
     pv = bv;
     pi = bi;
-    ++found;
   }
-  // a strip whose second logit may come before the last of them is formed again.  With
-  // fewer than K strips every strip is among them, and each is formed again.
-  const float last = found < K ? -INFINITY : pv;
-  int nagain = 0;
-  for (int k = 0; k < found; ++k) {
-    const int strip = first_s[w][k];
-    const float second = __uint_as_float(rc[strip].rest & 0xffff0000u);
-    if (!(second >= last)) {
-      if (l == 0) slot[w][k] = -1;
-      continue;
+  return found;
+}
+
+// The same with the first logits in registers, NR a lane (lane l: strips l, l + 64, ...): each
+// lane keeps its maximum; a round takes the wavefront's and clears the register that held it.
+// Of equal values the lower column: within a lane the earlier register (64 strips are whole
+// statistics strips), between lanes by the records.  Ends at logits of -inf, which choose_slow
+// orders.
+template <int NR>
+__device__ __forceinline__ int choose(const Rec *rc, int nrec, const Strips &strips, int64_t V,
+                                      int K, Chosen &ch) {
+  const int l = threadIdx.x & 63;
+  float v[NR], best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int q = l + 64 * i;
+    v[i] = q < nrec ? rc[q].first : -INFINITY;
+    best = fmaxf(best, v[i]);
+  }
+  auto column_of = [&](int strip) { return strips.column(strip, (int)(rc[strip].rest & 63u)); };
+  int found = 0, pi = -1;
+  float pv = INFINITY;
+  while (found < K) {
+    const float mx = wave_max(best);
+    if (mx == -INFINITY) break;
+    const uint64_t held = __ballot(best == mx);
+    // the register that holds it, in every lane that has it
+    int at = 0;
+#pragma unroll
+    for (int i = NR - 1; i >= 0; --i) at = v[i] == mx ? i : at;
+    int win = __ffsll((unsigned long long)held) - 1;
+    if (held & (held - 1)) {  // more than one lane: seldom
+      int col = (held >> l) & 1 ? column_of(l + 64 * at) : 0x7fffffff, tag = l;
+      float same = 0.f;
+      wave_first(same, col, tag);
+      win = __builtin_amdgcn_readfirstlane(tag);
     }
-    const TI *hrow = Hc + (j0 + row) * D;
+    const int slot = __builtin_amdgcn_readlane(at, win), strip = win + 64 * slot;
+    if (l == 0) {
+      ch.v[found] = mx;
+      ch.strip[found] = strip;
+    }
+    ++found;
+    pv = mx;
+    pi = strip;  // its column is looked up below, if need be
+    best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      v[i] = l == win && i == slot ? -INFINITY : v[i];
+      best = fmaxf(best, v[i]);
+    }
+  }
+  if (found == K) return K;
+  return choose_slow(rc, nrec, strips, V, K, ch, found, pv, found ? column_of(pi) : -1);
+}
+
+// A wavefront's own LDS writes are done before its later reads.
+__device__ __forceinline__ void wave_lds_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// NR: records in a lane's registers (0: more than fit, read in every round).  `targets`: the
+// skinny pass, whose rows are not compacted: rows that do not count get their zeros here, and
+// the state is written for the backward.
+template <typename TI, bool VK, int NR>
+__global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
+    const TI *W, const TI *H, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
+    const Rec *__restrict__ recs, Strips strips, const float *__restrict__ tgt, int64_t j0,
+    int64_t crows, int *n_ptr, int *rows, int *tcol, int *pos, TI *Hc,
+    const int64_t *__restrict__ targets, int64_t ignore_index, float *__restrict__ lse_out,
+    float *__restrict__ ent_out, RowOut out) {
+  constexpr int kWaves = kFinishThreads / 64;
+  __shared__ Chosen chosen_w[kWaves];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * kWaves + w;
+  const int K = out.top_k;
+  int64_t m;
+  const TI *hrow;
+  if (targets) {
+    if (row >= crows) return;
+    m = row;
+    hrow = H + row * D;
+    const int tc = target_column(targets, row, V, ignore_index);
+    constexpr int VE = VK ? 16 / (int)sizeof(TI) : 1;
+    for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
+      if constexpr (VK) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (tc >= 0) x = *reinterpret_cast<const u32x4 *>(hrow + c);
+        *reinterpret_cast<u32x4 *>(Hc + row * D + c) = x;
+      } else {
+        Hc[row * D + c] = tc >= 0 ? hrow[c] : static_cast<TI>(0.f);
+      }
+    }
+    if (l == 0) {
+      rows[row] = (int)row;
+      pos[row] = (int)row;
+      tcol[row] = tc;
+      if (row == 0) *n_ptr = (int)crows;
+    }
+    if (tc < 0) {
+      if (l == 0) {
+        lse_out[row] = 0.f;
+        ent_out[row] = 0.f;
+        out.logprob[row] = 0.f;
+        out.entropy[row] = 0.f;
+      }
+      if (l < K) {
+        out.top_lp[row * K + l] = 0.f;
+        out.top_id[row * K + l] = -1;
+      }
+      return;
+    }
+  } else {
+    if (row >= chunk_count(n_ptr, j0, crows)) return;
+    m = rows[j0 + row];
+    hrow = H + (j0 + row) * D;
+  }
+  const Stat *st = stats + row * nstat;
+  Stat a{-INFINITY, 0.f, 0.f, 0.f};
+  for (int k = l; k < nstat; k += 64) a = join(a, st[k]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+    a = join(a, Stat{__shfl_xor(a.mx, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f});
+  const float ls = log_f32(a.s), lse = a.mx + ls, ent = ls - a.t / a.s;
+  if (l == 0) {
+    lse_out[j0 + row] = lse;
+    ent_out[j0 + row] = ent;
+    out.logprob[m] = tgt[row] - lse;
+    out.entropy[m] = ent;
+  }
+  if (K == 0) return;
+  Chosen &ch = chosen_w[w];
+  const int nrec = nstat * strips.per_stat();
+  const Rec *rc = recs + row * nrec;
+  int found;
+  if constexpr (NR > 0)
+    found = choose<NR>(rc, nrec, strips, V, K, ch);
+  else
+    found = choose_slow(rc, nrec, strips, V, K, ch, 0, INFINITY, -1);
+  wave_lds_fence();  // lane 0 wrote `ch` for all
+  // a strip whose second logit may come before the last of them is formed again; with fewer
+  // than K strips every strip is among them, and each is formed again
+  const float last = found < K ? -INFINITY : ch.v[K - 1];
+  bool need = false;
+  int col = -1;
+  float val = 0.f;
+  if (l < found) {
+    const uint32_t rest = rc[ch.strip[l]].rest;
+    need = __uint_as_float(rest & 0xffff0000u) >= last;
+    col = strips.column(ch.strip[l], (int)(rest & 63u));
+    val = ch.v[l];
+  }
+  const uint64_t redo = __ballot(need);
+  if (redo == 0) {  // the first logits of the chosen strips are the row's K first
+    if (l < K) {
+      out.top_lp[m * K + l] = l < found ? val - lse : __builtin_nanf("");
+      out.top_id[m * K + l] = l < found ? col : -1;
+    }
+    return;
+  }
+  const uint64_t alone = __ballot(l < found && !need);
+  int n = __popcll(alone);  // candidates
+  if ((alone >> l) & 1) {
+    const int q = __popcll(alone & ((1ull << l) - 1ull));
+    ch.cand_v[q] = val;
+    ch.cand_col[q] = col;
+  }
+  for (uint64_t todo = redo; todo; todo &= todo - 1, n += 32) {
+    const int strip = ch.strip[__ffsll((unsigned long long)todo) - 1];
     Dot16<TI> acc[2];
     const TI *wrow[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int col = strips.column(strip, 16 * h + (l & 15));
-      wrow[h] = col < V ? W + (int64_t)col * D : nullptr;
+      const int c = strips.column(strip, 16 * h + (l & 15));
+      wrow[h] = c < V ? W + (int64_t)c * D : nullptr;
     }
-    for (int64_t kk = 0; kk < D; kk += 32) {
-      const auto b = Dot16<TI>::template load<VK>(hrow, kk, D);
+    constexpr int kDepth = sizeof(TI) == 2 ? 8 : 2;
+    for (int64_t k0 = 0; k0 < D; k0 += 32 * kDepth) {
+      typename Dot16<TI>::Frag fa[kDepth][2], fb[kDepth];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc[h].add(Dot16<TI>::template load<VK>(wrow[h], kk, D), b);
+      for (int u = 0; u < kDepth; ++u) {
+        fb[u] = Dot16<TI>::template load<VK>(hrow, k0 + 32 * u, D);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          fa[u][h] = Dot16<TI>::template load<VK>(wrow[h], k0 + 32 * u, D);
+      }
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[h].add(fa[u][h], fb[u]);
     }
     // every column of the product is this token: lane l has places 4 (l / 16) .. + 3
 #pragma unroll
@@ -403,59 +665,36 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
       const floatx4 z = acc[h].done();
       if ((l & 15) == 0)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) again[w][nagain * 32 + 16 * h + 4 * (l >> 4) + q] = z[q];
+        for (int q = 0; q < 4; ++q) {
+          const int c = 16 * h + 4 * (l >> 4) + q;
+          ch.cand_v[n + c] = z[q];
+          ch.cand_col[n + c] = strips.column(strip, c);
+        }
     }
-    if (l == 0) slot[w][k] = nagain;
-    ++nagain;
   }
-  // one wavefront's own LDS: its writes are done before its reads below
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  // the K first of those strips' logits, in order
-  pv = INFINITY;
-  pi = -1;
+  wave_lds_fence();
+  // the K first of the candidates, in order
+  float pv = INFINITY;
+  int pi = -1;
   for (int k = 0; k < K; ++k) {
     float bv = -INFINITY;
     int bi = 0x7fffffff, tag = -1;
-    if (nagain == 0) {
-      if (k < found) {
-        bv = first_v[w][k];
-        bi = first_i[w][k];
+    for (int q = l; q < n; q += 64) {
+      const float x = ch.cand_v[q];
+      const int c = ch.cand_col[q];
+      if (c < V && before(pv, pi, x, c) && before(x, c, bv, bi)) {
+        bv = x;
+        bi = c;
         tag = 0;
       }
-    } else {
-      for (int q = l; q < found * 32; q += 64) {
-        const int f = q >> 5, c = q & 31, sl = slot[w][f];
-        float v;
-        int col;
-        if (sl >= 0) {
-          v = again[w][sl * 32 + c];
-          col = strips.column(first_s[w][f], c);
-        } else {
-          if (c) continue;
-          v = first_v[w][f];
-          col = first_i[w][f];
-        }
-        if (col < V && before(pv, pi, v, col) && before(v, col, bv, bi)) {
-          bv = v;
-          bi = col;
-          tag = 0;
-        }
-      }
-      wave_first(bv, bi, tag);
     }
+    wave_first(bv, bi, tag);
     if (l == 0) {
       out.top_lp[m * K + k] = tag < 0 ? __builtin_nanf("") : bv - lse;
       out.top_id[m * K + k] = tag < 0 ? -1 : bi;
     }
-    if (tag < 0) {  // none left: they compare with nothing
-      pv = -INFINITY;
-      pi = 0x7fffffff;
-      continue;
-    }
-    pv = bv;
-    pi = bi;
+    pv = tag < 0 ? -INFINITY : bv;  // none left: nothing comes after the last place
+    pi = tag < 0 ? 0x7fffffff : bi;
   }
 }
 
@@ -521,11 +760,14 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     int want = -1;  // the register that holds the target, if this lane does
     if (tok < cnt) {
       const int64_t m = in.rows[j0 + tok];
-      g = in.g ? in.g[m] : 0.f;
-      h = in.h ? in.h[m] : 0.f;
+      const int tc = in.tcol[j0 + tok];
+      if (tc >= 0) {  // else a row that does not count: its hidden row is zero here
+        g = in.g ? in.g[m] : 0.f;
+        h = in.h ? in.h[m] : 0.f;
+      }
       lse = in.lse[j0 + tok];
       ent = in.ent[j0 + tok];
-      const int64_t loc64 = (int64_t)in.tcol[j0 + tok] - vtile0;
+      const int64_t loc64 = (int64_t)tc - vtile0;
       const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
       if (loc >= 0 && ((loc >> 2) & 1) == half)
         want = ((loc >> 5) << 4) | (((loc & 31) >> 3) << 2) | (loc & 3);
@@ -588,8 +830,10 @@ struct View {
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
 struct FwdPlan {
+  bool skinny;  // at most kSkinnyRows rows: the skinny pass
   int64_t crows;
   int nstat, vtiles;
+  Strips strips;
   size_t stats, recs, tgt, total;
 };
 template <typename TI>
@@ -597,16 +841,43 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k) {
   using C = MainCfg<TI>;
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
-  p.crows = chunk_rows < mcap / 8 ? round_up(8 * chunk_rows, 256) : mcap;
+  p.skinny = M <= kSkinnyRows;
+  p.crows = p.skinny ? M : chunk_rows < mcap / 8 ? round_up(8 * chunk_rows, 256) : mcap;
   p.vtiles = (int)((V + C::BM - 1) / C::BM);
-  p.nstat = p.vtiles * C::WM;
+  p.nstat = p.skinny ? (int)((V + 31) / 32) : p.vtiles * C::WM;
+  p.strips = Strips{p.skinny ? 0 : C::WTM == 128 ? 2 : 1};
+  static_assert(C::WTM == 128 || C::WTM == 64, "strips of a wavefront's tile");
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
   p.stats = take((size_t)p.crows * p.nstat * sizeof(Stat));
-  p.recs = take(top_k ? (size_t)p.crows * p.nstat * (C::WTM / 32) * sizeof(Rec) : 0);
+  p.recs = take(top_k ? (size_t)p.crows * p.nstat * p.strips.per_stat() * sizeof(Rec) : 0);
   p.tgt = take((size_t)p.crows * sizeof(float));
   p.total = o;
   return p;
+}
+
+template <typename TI>
+int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan &P,
+                  const Stat *stats, const Rec *recs, const float *tgt, int64_t j0, int64_t rows,
+                  const View<TI> &S, const int64_t *targets, int64_t ignore_index,
+                  const RowOut &out, hipStream_t s) {
+  const bool vk = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(W) && aligned16(H);
+  const unsigned grid = (unsigned)((rows + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
+  const int nrec = P.nstat * P.strips.per_stat();
+#define NF_LP_FINISH(VK, NR)                                                                   \
+  lp_finish_kernel<TI, VK, NR><<<grid, kFinishThreads, 0, s>>>(                                \
+      W, H, V, D, stats, P.nstat, recs, P.strips, tgt, j0, rows, S.n, S.rows, S.tcol, S.pos,   \
+      S.Hc, targets, ignore_index, S.lse, S.ent, out)
+  if (vk && nrec <= 64 * 16)
+    NF_LP_FINISH(true, 16);
+  else if (vk && nrec <= 64 * 32)
+    NF_LP_FINISH(true, 32);
+  else if (vk)
+    NF_LP_FINISH(true, 0);
+  else
+    NF_LP_FINISH(false, 0);
+#undef NF_LP_FINISH
+  return check_launch("lp_finish");
 }
 
 template <typename TI>
@@ -617,13 +888,34 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
   const View<TI> S(state_layout<TI>(M, D), state);
   const FwdPlan P = fwd_plan<TI>(M, V, chunk_rows, out.top_k);
   Stat *stats = reinterpret_cast<Stat *>(ws + P.stats);
-  Rec *recs = reinterpret_cast<Rec *>(ws + P.recs);
+  Rec *recs = out.top_k ? reinterpret_cast<Rec *>(ws + P.recs) : nullptr;
   float *tgt = reinterpret_cast<float *>(ws + P.tgt);
+  const int64_t VE = 16 / (int64_t)sizeof(TI);
   int e;
+  if (P.skinny) {
+    const bool vk = D % VE == 0 && aligned16(H) && aligned16(W);
+    const unsigned grid = (unsigned)((V + 127) / 128);
+#define NF_LP_SKINNY(NT, VK)                                                                   \
+  lp_skinny_kernel<TI, NT, VK><<<grid, kSkinnyThreads, 0, s>>>(W, H, targets, M, V, D,         \
+                                                               ignore_index, stats, P.nstat,   \
+                                                               recs, tgt)
+    if (vk && M <= 16)
+      NF_LP_SKINNY(1, true);
+    else if (vk && M <= 32)
+      NF_LP_SKINNY(2, true);
+    else if (vk)
+      NF_LP_SKINNY(4, true);
+    else
+      NF_LP_SKINNY(4, false);
+#undef NF_LP_SKINNY
+    if ((e = check_launch("lp_skinny"))) return e;
+    return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, targets, ignore_index,
+                             out, s);
+  }
   ce::ce_compact_kernel<<<1, ce::kCompactThreads, 0, s>>>(targets, M, V, ignore_index, S.rows,
                                                           S.tcol, S.pos, S.n, S.inv, nullptr);
   if ((e = check_launch("ce_compact"))) return e;
-  const bool vec = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(H) && aligned16(S.Hc);
+  const bool vec = D % VE == 0 && aligned16(H) && aligned16(S.Hc);
   int64_t blocks = (M + 3) / 4;
   if (blocks > 4096) blocks = 4096;
   if (vec)
@@ -634,8 +926,6 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
                                                                             S.n, M, S.Hc, out);
   if ((e = check_launch("lp_gather"))) return e;
   const bool vk = buf_ok<TI>(S.Hc, D, M, D) && buf_ok<TI>(W, D, V, D);
-  const bool vw = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(W);
-  const Strips strips{C::WTM};
   for (int64_t j0 = 0; j0 < M; j0 += P.crows) {
     const int64_t rows = M - j0 < P.crows ? M - j0 : P.crows;
     const int ttiles = (int)((rows + C::BN - 1) / C::BN);
@@ -654,17 +944,9 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
       NF_LP_LOGITS(false, false);
 #undef NF_LP_LOGITS
     if ((e = check_launch("lp_logits"))) return e;
-    const unsigned fin = (unsigned)((rows + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
-#define NF_LP_FINISH(VK)                                                                      \
-  lp_finish_kernel<TI, VK><<<fin, kFinishThreads, 0, s>>>(W, S.Hc, V, D, stats, P.nstat, recs, \
-                                                          strips, tgt, S.n, j0, rows, S.rows, \
-                                                          S.lse, S.ent, out)
-    if (vw)
-      NF_LP_FINISH(true);
-    else
-      NF_LP_FINISH(false);
-#undef NF_LP_FINISH
-    if ((e = check_launch("lp_finish"))) return e;
+    if ((e = launch_finish<TI>(W, S.Hc, V, D, P, stats, recs, tgt, j0, rows, S, nullptr,
+                               ignore_index, out, s)))
+      return e;
   }
   return NF_OK;
 }

@@ -357,6 +357,174 @@ struct ChunkedCE : torch::autograd::Function<ChunkedCE> {
 };
 
 // ---------------------------------------------------------------------------
+// token log probabilities
+// ---------------------------------------------------------------------------
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  // {logprobs, entropy, top_logprobs, top_ids}; `keep` what the backward reads
+  static variable_list run(const Tensor &hidden, const Tensor &weight, const Tensor &targets,
+                           int64_t top_k, int64_t chunk_rows, int64_t ignore_index,
+                           at::ScalarType cdt, Tensor &w, Tensor &state) {
+    const int64_t m = hidden.size(0), d = hidden.size(1), v = weight.size(0);
+    const int code = code_of(cdt);
+    const Tensor h = hidden.to(cdt).contiguous(), tg = targets.contiguous();
+    w = weight.to(cdt).contiguous();
+    const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
+    Tensor lp = at::empty({m}, f32), ent = at::empty({m}, f32), top = at::empty({m, top_k}, f32);
+    Tensor ids = at::empty({m, top_k}, f32.dtype(at::kLong));
+    const size_t ns = nf_token_logprobs_state_bytes(m, d, v, code);
+    const size_t nw = nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, (int)top_k, code);
+    TORCH_CHECK_VALUE(ns && nw, "chunked_token_logprobs: shape M=", m, " D=", d, " V=", v,
+                      " is beyond the kernels");
+    state = bytes(ns, hidden);
+    Tensor ws = bytes(nw, hidden);
+    check(nf_token_logprobs_fwd(h.data_ptr(), w.data_ptr(), tg.data_ptr<int64_t>(), m, d, v,
+                                ignore_index, chunk_rows, (int)top_k, code, lp.data_ptr<float>(),
+                                ent.data_ptr<float>(), top.data_ptr<float>(),
+                                ids.data_ptr<int64_t>(), state.data_ptr(), ns, ws.data_ptr(), nw,
+                                stream_of(hidden)),
+          "nf_token_logprobs_fwd");
+    return {lp, ent, top, ids};
+  }
+  static variable_list forward(AutogradContext *ctx, const Tensor &hidden, const Tensor &weight,
+                               const Tensor &targets, int64_t top_k, int64_t chunk_rows,
+                               int64_t ignore_index, int64_t compute) {
+    const c10::DeviceGuard guard(hidden.device());
+    const auto cdt = (at::ScalarType)compute;
+    Tensor w, state;
+    const variable_list out =
+        run(hidden, weight, targets, top_k, chunk_rows, ignore_index, cdt, w, state);
+    ctx->save_for_backward({w, state});
+    ctx->saved_data["s"] = std::vector<int64_t>{hidden.size(0), hidden.size(1), weight.size(0),
+                                                chunk_rows, code_of(cdt),
+                                                (int64_t)hidden.scalar_type(),
+                                                (int64_t)weight.scalar_type()};
+    ctx->mark_non_differentiable({out[2], out[3]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list res(7);
+    if (!grads[0].defined() && !grads[1].defined()) return res;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &w = saved[0], &state = saved[1];
+    const c10::DeviceGuard guard(w.device());
+    const auto s = ctx->saved_data["s"].toIntVector();
+    const int64_t m = s[0], d = s[1], v = s[2], chunk_rows = s[3];
+    const int code = (int)s[4];
+    const auto th = (at::ScalarType)s[5], tw = (at::ScalarType)s[6];
+    Tensor g[2];
+    for (int i = 0; i < 2; ++i) {
+      if (!grads[i].defined()) continue;
+      TORCH_CHECK_VALUE(grads[i].device() == w.device(), "chunked_token_logprobs backward: an "
+                        "upstream gradient is not on the forward's device");
+      g[i] = grads[i].to(at::kFloat).contiguous();
+    }
+    if (ctx->needs_input_grad(0)) res[0] = at::empty({m, d}, w.options().dtype(th));
+    if (ctx->needs_input_grad(1)) res[1] = at::empty({v, d}, w.options().dtype(tw));
+    const size_t nw = nf_token_logprobs_bwd_workspace(m, d, v, chunk_rows, code);
+    Tensor ws = bytes(nw, state);
+    check(nf_token_logprobs_bwd(w.data_ptr(), m, d, v, chunk_rows, code, state.data_ptr(),
+                                (size_t)state.numel(), (const float *)ptr(g[0]),
+                                (const float *)ptr(g[1]), ptr(res[0]), code_of(th), ptr(res[1]),
+                                code_of(tw), ws.data_ptr(), nw, stream_of(w)),
+          "nf_token_logprobs_bwd");
+    return res;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// embedding lookup
+// ---------------------------------------------------------------------------
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor run(const Tensor &ids, const Tensor &table, double scale, at::ScalarType out_t) {
+    const int64_t m = ids.numel(), v = table.size(0), d = table.size(1);
+    std::vector<int64_t> sizes = ids.sizes().vec();
+    sizes.push_back(d);
+    Tensor out = at::empty(sizes, table.options().dtype(out_t).requires_grad(false));
+    check(nf_embedding_fwd(ids.data_ptr<int64_t>(), table.data_ptr(), table.stride(0),
+                           (float)scale, m, d, v, out.data_ptr(), code_of(table), code_of(out_t),
+                           stream_of(table)),
+          "nf_embedding_fwd");
+    return out;
+  }
+  static Tensor forward(AutogradContext *ctx, const Tensor &ids, const Tensor &table,
+                        double scale, int64_t pad, int64_t out_t) {
+    const c10::DeviceGuard guard(table.device());
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["s"] = std::vector<int64_t>{table.size(0), table.size(1), pad,
+                                                (int64_t)table.scalar_type()};
+    return run(ids, table, scale, (at::ScalarType)out_t);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &ids = saved[0];
+    const c10::DeviceGuard guard(ids.device());
+    const auto s = ctx->saved_data["s"].toIntVector();
+    const int64_t m = ids.numel(), v = s[0], d = s[1];
+    const auto tt = (at::ScalarType)s[3];
+    TORCH_CHECK_VALUE(grads[0].device() == ids.device(),
+                      "embedding_lookup backward: dout is not on the forward's device");
+    const Tensor g = grads[0].contiguous();
+    Tensor dtable = at::empty({v, d}, g.options().dtype(tt));
+    const size_t nw = nf_embedding_bwd_workspace(m, d, v);
+    Tensor ws = bytes(nw, ids);
+    check(nf_embedding_bwd(g.data_ptr(), ids.data_ptr<int64_t>(), s[2],
+                           (float)ctx->saved_data["scale"].toDouble(), m, d, v,
+                           dtable.data_ptr(), code_of(g), code_of(tt), ws.data_ptr(), nw,
+                           stream_of(g)),
+          "nf_embedding_bwd");
+    return {Tensor(), dtable, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------
+// dropout
+// ---------------------------------------------------------------------------
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor run(const Tensor &x, const Tensor &res, at::ScalarType out_t, int64_t threshold,
+                    const Tensor &seed_t, int64_t seed, int64_t offset) {
+    Tensor out = at::empty(x.sizes(), x.options().dtype(out_t).requires_grad(false));
+    check(nf_dropout(x.data_ptr(), ptr(res), out.data_ptr(), x.numel(), (int32_t)threshold,
+                     (const int64_t *)ptr(seed_t), seed, offset, code_of(x), code_of(out_t),
+                     stream_of(x)),
+          "nf_dropout");
+    return out;
+  }
+  static Tensor forward(AutogradContext *ctx, const Tensor &x,
+                        const std::optional<Tensor> &residual,
+                        const std::optional<Tensor> &seed_in, int64_t threshold, int64_t seed,
+                        int64_t offset) {
+    const c10::DeviceGuard guard(x.device());
+    Tensor r, seed_t;
+    if (residual) r = residual->contiguous();
+    if (seed_in) seed_t = *seed_in;
+    if (seed_in) ctx->save_for_backward({seed_t});
+    ctx->saved_data["s"] =
+        std::vector<int64_t>{threshold, seed, offset, (int64_t)x.scalar_type(), seed_t.defined(),
+                             r.defined()};
+    return run(x.contiguous(), r, r.defined() ? r.scalar_type() : x.scalar_type(), threshold,
+               seed_t, seed, offset);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto s = ctx->saved_data["s"].toIntVector();
+    variable_list res(6);
+    // an argument that was left out has no edge: the residual's is the second, if there is one
+    if (s[5] && ctx->needs_input_grad(1)) res[1] = grads[0];
+    if (!ctx->needs_input_grad(0)) return res;
+    Tensor seed_t;
+    if (s[4]) {
+      seed_t = ctx->get_saved_variables()[0];
+      TORCH_CHECK_VALUE(grads[0].device() == seed_t.device(),
+                        "fused_dropout backward: dout is not on the forward's device");
+    }
+    const c10::DeviceGuard guard(grads[0].device());
+    res[0] = run(grads[0].contiguous(), Tensor(), (at::ScalarType)s[3], s[0], seed_t, s[1], s[2]);
+    return res;
+  }
+};
+
+// ---------------------------------------------------------------------------
 // entries
 // ---------------------------------------------------------------------------
 // The call's leading `n` arguments as tensors; false when one is not.
@@ -463,11 +631,128 @@ PyObject *py_ce(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+bool wants_grad(std::initializer_list<const Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor *t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Python ints from args[at ..]; false when one is not, or does not fit.
+template <int N>
+bool ints(PyObject *const *args, int at, int64_t (&v)[N]) {
+  for (int i = 0; i < N; ++i) {
+    if (!PyLong_CheckExact(args[at + i])) return false;
+    v[i] = PyLong_AsLongLong(args[at + i]);
+    if (v[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  return true;
+}
+
+// hidden [M, D], lm_weight [V, D], targets [M], top_k, chunk rows, ignore index, compute type
+// (0 fp32, 1 bf16) -> (logprobs, entropy, top_logprobs, top_ids)
+PyObject *py_token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[3];
+  int64_t v[4];
+  if (!tensors(args, nargs, 7, t) || !quiet() || !ints(args, 3, v)) Py_RETURN_NONE;
+  const c10::Device dev = t[0].device();
+  for (const Tensor &x : t)
+    if (!plain(x, dev)) Py_RETURN_NONE;
+  if (t[0].dim() != 2 || t[1].dim() != 2 || t[0].size(1) != t[1].size(1) || t[0].numel() == 0 ||
+      t[1].numel() == 0 || t[2].dim() != 1 || t[2].size(0) != t[0].size(0) ||
+      code_of(t[0]) < 0 || code_of(t[1]) < 0 || t[2].scalar_type() != at::kLong || v[0] < 0 ||
+      v[0] > 32 || v[0] > t[1].size(0) || v[1] <= 0)
+    Py_RETURN_NONE;
+  const at::ScalarType cdt = v[3] == NF_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
+  const variable_list r = unlocked([&]() -> variable_list {
+    if (wants_grad({&t[0], &t[1]}))
+      return TokenLogprobs::apply(t[0], t[1], t[2], v[0], v[1], v[2], (int64_t)cdt);
+    const c10::DeviceGuard guard(dev);
+    const at::NoGradGuard no_grad;
+    Tensor w, state;
+    return TokenLogprobs::run(t[0], t[1], t[2], v[0], v[1], v[2], cdt, w, state);
+  });
+  PyObject *tuple = PyTuple_New(4);
+  if (!tuple) return nullptr;
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(r[i]));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
+// ids, table [V, D], scale, padding id (-1: none), out's type (NF_DTYPE_*)
+PyObject *py_embedding(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[2];
+  if (!tensors(args, nargs, 5, t) || !quiet()) Py_RETURN_NONE;
+  int64_t v[2];
+  if (!PyFloat_CheckExact(args[2]) || !ints(args, 3, v)) Py_RETURN_NONE;
+  const double scale = PyFloat_AS_DOUBLE(args[2]);
+  const c10::Device dev = t[1].device();
+  if (!plain(t[0], dev) || !plain(t[1], dev) || t[0].scalar_type() != at::kLong ||
+      !t[0].is_contiguous() || t[0].numel() == 0 || t[1].dim() != 2 || t[1].numel() == 0 ||
+      code_of(t[1]) < 0 || t[1].stride(1) != 1 || t[1].stride(0) < t[1].size(1))
+    Py_RETURN_NONE;
+  const at::ScalarType out_t = v[1] == NF_DTYPE_F32    ? at::kFloat
+                               : v[1] == NF_DTYPE_BF16 ? at::kBFloat16
+                                                       : at::kHalf;
+  if (out_t != t[1].scalar_type() && t[1].scalar_type() != at::kFloat) Py_RETURN_NONE;
+  return THPVariable_Wrap(unlocked([&]() -> Tensor {
+    if (wants_grad({&t[1]})) return Embedding::apply(t[0], t[1], scale, v[0], (int64_t)out_t);
+    const c10::DeviceGuard guard(dev);
+    return Embedding::run(t[0], t[1], scale, out_t);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+// x, residual or None, threshold, seed (int, or an int64 tensor of one element), offset
+PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !quiet() || !THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  const Tensor x = THPVariable_Unpack(args[0]);
+  const c10::Device dev = x.device();
+  Tensor r, seed_t;
+  int64_t threshold[1], seed[1] = {0}, offset[1];
+  if (args[1] != Py_None) {
+    if (!THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    r = THPVariable_Unpack(args[1]);
+    if (!plain(r, dev) || r.sizes() != x.sizes() ||
+        (r.scalar_type() != x.scalar_type() && r.scalar_type() != at::kFloat))
+      Py_RETURN_NONE;
+  }
+  if (THPVariable_CheckExact(args[3])) {
+    seed_t = THPVariable_Unpack(args[3]);
+    if (!plain(seed_t, dev) || seed_t.scalar_type() != at::kLong || seed_t.numel() != 1)
+      Py_RETURN_NONE;
+  } else if (!ints(args, 3, seed)) {
+    Py_RETURN_NONE;
+  }
+  if (!plain(x, dev) || code_of(x) < 0 || x.numel() == 0 || !ints(args, 2, threshold) ||
+      !ints(args, 4, offset) || threshold[0] < 0 || threshold[0] > 65536 || offset[0] < 0)
+    Py_RETURN_NONE;
+  auto given = [](const Tensor &v) { return v.defined() ? std::optional<Tensor>(v) : std::nullopt; };
+  return THPVariable_Wrap(unlocked([&]() -> Tensor {
+    if (wants_grad({&x, &r}))
+      return Dropout::apply(x, given(r), given(seed_t), threshold[0], seed[0], offset[0]);
+    const c10::DeviceGuard guard(dev);
+    const Tensor rc = r.defined() ? r.contiguous() : r;
+    return Dropout::run(x.contiguous(), rc, rc.defined() ? rc.scalar_type() : x.scalar_type(),
+                        threshold[0], seed_t, seed[0], offset[0]);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"seam", (PyCFunction)(void (*)(void))py_seam, METH_FASTCALL, nullptr},
     {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL, nullptr},
     {"gate_up", (PyCFunction)(void (*)(void))py_gate_up, METH_FASTCALL, nullptr},
     {"ce", (PyCFunction)(void (*)(void))py_ce, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void (*)(void))py_token_logprobs, METH_FASTCALL, nullptr},
+    {"embedding", (PyCFunction)(void (*)(void))py_embedding, METH_FASTCALL, nullptr},
+    {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

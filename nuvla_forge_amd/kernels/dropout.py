@@ -111,7 +111,12 @@ def fused_dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: i
     formulation, with the same mask.
     """
     threshold = dropout_threshold(p)
+    fused = use_fused(x, "fused_dropout", force_reference)
+    if fused:  # the plain call runs in C++; any other (None) takes the Function below
+        out = _lib.native().dropout(x, residual, threshold, seed, offset)
+        if out is not None:
+            return out
     _check(x, seed, offset, residual)
-    if not use_fused(x, "fused_dropout", force_reference):
+    if not fused:
         return dropout_ref(x, threshold, seed, offset, residual)
     return _FusedDropout.apply(x, residual, threshold, seed, offset)

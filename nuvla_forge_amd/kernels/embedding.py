@@ -81,6 +81,14 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     The gradient has the table's type and is the same bits every run.  Host tensors take
     the eager formulation.
     """
+    fused = use_fused(table, "embedding_lookup", force_reference)
+    if fused and table.dim() == 2 and (padding_idx is None or 0 <= padding_idx < table.shape[0]):
+        # the plain call runs in C++; any other (None) takes the Function below
+        out = _lib.native().embedding(ids, table, float(scale),
+                                      -1 if padding_idx is None else padding_idx,
+                                      _lib.DTYPE_CODE.get(out_dtype or table.dtype))
+        if out is not None:
+            return out
     if table.dim() != 2 or 0 in table.shape:
         raise ValueError(f"embedding_lookup: table [V, D] expected, got {tuple(table.shape)}")
     if ids.dtype not in (torch.int64, torch.int32):
@@ -94,6 +102,6 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         raise TypeError(f"embedding_lookup: rows of a {table.dtype} table in {out_dtype}; expected "
                         f"{table.dtype}")
     check_devices("embedding_lookup", "table", dict(table=table, ids=ids))
-    if not use_fused(table, "embedding_lookup", force_reference):
+    if not fused:
         return embedding_ref(ids, table, scale, padding_idx, out_dtype)
     return _EmbeddingLookup.apply(ids, table, float(scale), padding_idx, out_dtype)

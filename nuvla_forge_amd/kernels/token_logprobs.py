@@ -161,9 +161,16 @@ def chunked_token_logprobs(
 
     Host tensors run the eager row-chunk loop.
     """
+    fused = use_fused(hidden, "chunked_token_logprobs", force_reference)
+    if fused:  # the plain call runs in C++; any other (None) takes the Function below
+        out = _lib.native().token_logprobs(
+            hidden, lm_weight, targets, top_k, chunk_size, ignore_index,
+            _lib.dtype_code(_compute_dtype(hidden, lm_weight)))
+        if out is not None:
+            return TokenLogprobs(*out) if top_k else TokenLogprobs(out[0], out[1], None, None)
     _check(hidden, lm_weight, targets, top_k)
     chunk_rows = chunk_rows_for(chunk_size)
-    if not use_fused(hidden, "chunked_token_logprobs", force_reference):
+    if not fused:
         return TokenLogprobs(*token_logprobs_ref(hidden, lm_weight, targets, top_k, chunk_rows,
                                                  ignore_index))
     lp, ent, top_lp, top_ids = _TokenLogprobs.apply(hidden, lm_weight, targets, int(top_k),

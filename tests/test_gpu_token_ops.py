@@ -481,6 +481,67 @@ def test_logprobs_make_no_host_sync(cuda):
 
 
 # ---------------------------------------------------------------------------
+# the C++ host side against the Functions in Python
+# ---------------------------------------------------------------------------
+class _NoNative:
+    """Every entry answers None: the call takes its Function in Python."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_plain_calls_match_the_functions(cuda, monkeypatch, grad):
+    note(f"native token ops grad={grad}")
+    h, w, t, g, gh = _head(70, 64, 900, BF16, cuda)
+    ids = torch.randint(0, 900, (5, 14), generator=gen(1)).to(cuda)
+    table, x = randn((900, 64), gen(2), F32, cuda), randn((70, 64), gen(3), BF16, cuda)
+    r, seed = randn((70, 64), gen(4), F32, cuda), torch.tensor([5], device=cuda)
+
+    def calls():
+        a, b, c, y, z = (v.detach().clone().requires_grad_(grad) for v in (h, w, table, x, r))
+        lp = chunked_token_logprobs(a, b, t, top_k=4)
+        emb = embedding_lookup(ids, c, scale=3.0, padding_idx=2, out_dtype=BF16)
+        out = fused_dropout(y, 0.3, seed, offset=2, residual=z)
+        one = fused_dropout(y, 0.3, 5, offset=2)
+        res = [*lp, emb, out, one]
+        assert [v.requires_grad for v in res] == [grad, grad, False, False, grad, grad, grad]
+        if grad:
+            res += torch.autograd.grad([lp.logprobs, lp.entropy, emb, out], [a, b, c, y, z],
+                                       [g, gh, torch.ones_like(emb), torch.ones_like(out)])
+            res += torch.autograd.grad(one, y, torch.ones_like(one))
+        return res
+
+    native = calls()
+    from nuvla_forge_amd import _lib
+
+    with monkeypatch.context() as mp:
+        mp.setattr(_lib, "native", _NoNative)
+        general = calls()
+    for p, q in zip(native, general, strict=True):
+        assert p.dtype == q.dtype and torch.equal(p, q)
+
+
+def test_calls_that_are_not_plain_raise_as_documented(cuda):
+    note("token ops refusals on the device")
+    h, w, t, *_ = _head(10, 64, 900, BF16, cuda)
+    with pytest.raises(ValueError, match="top_k"):
+        chunked_token_logprobs(h, w, t, top_k=33)
+    with pytest.raises(ValueError, match="on cpu"):
+        chunked_token_logprobs(h, w, t.cpu())
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding_lookup(t, w, padding_idx=900)
+    with pytest.raises(TypeError, match="table in"):
+        embedding_lookup(t, w, out_dtype=F32)
+    with pytest.raises(ValueError, match="shape mismatch"):
+        fused_dropout(h, 0.1, 0, residual=h[:5])
+    with pytest.raises(TypeError, match="residual"):
+        fused_dropout(h.float(), 0.1, 0, residual=h)
+    with pytest.raises(ValueError, match="on cpu"):
+        fused_dropout(h, 0.1, torch.tensor([1]))
+
+
+# ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("b, t, d, v", [(2, 16, 64, 500), (4, 33, 96, 3001)])

@@ -318,18 +318,21 @@ int nf_ce_fwd_bwd(const void *hidden, const void *weight,
  * kernel of the reference computes these; sizes, chunk_rows and the target
  * rules are those of nf_ce_fwd.  `state`
  * (nf_token_logprobs_state_bytes) holds the compacted rows, their log-sum-exp
- * and entropy for the backward; `workspace` nothing between calls.  A size
- * call returns 0 for arguments beyond the kernels.
+ * and entropy for the backward; `workspace` nothing between calls.  With
+ * `keep` (a backward will come; bf16, more than 128 rows) the state also holds
+ * exp(z - strip maximum) in 16 bits where one chunk takes every row, so the
+ * backward need not form the logits again.  The three take the same `keep`.
+ * A size call returns 0 for arguments beyond the kernels.
  * ---------------------------------------------------------------------- */
 size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V,
-                                     int dtype);
+                                     int64_t chunk_rows, int keep, int dtype);
 size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t V,
                                        int64_t chunk_rows, int top_k,
                                        int dtype);
 int nf_token_logprobs_fwd(const void *hidden, const void *weight,
                           const int64_t *targets, int64_t M, int64_t D,
                           int64_t V, int64_t ignore_index, int64_t chunk_rows,
-                          int top_k, int dtype, float *logprobs,
+                          int top_k, int keep, int dtype, float *logprobs,
                           float *entropy, float *top_logprobs,
                           int64_t *top_ids, void *state, size_t state_bytes,
                           void *workspace, size_t workspace_bytes,
@@ -339,12 +342,12 @@ int nf_token_logprobs_fwd(const void *hidden, const void *weight,
  * NULL: zero): with g, h a row's two and H its entropy,
  *   dz = g (onehot(target) - p) - h p (z - lse + H),
  *   dhidden = dz weight,  dweight = dz^T hidden
- * (either may be NULL: not formed).  `weight` and `state` are the forward's;
- * the logits are formed again.  The same bits every run. */
+ * (either may be NULL: not formed).  `weight` and `state` are the forward's,
+ * and may serve again.  The same bits every run. */
 size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,
                                        int64_t chunk_rows, int dtype);
 int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, int64_t V,
-                          int64_t chunk_rows, int dtype, void *state,
+                          int64_t chunk_rows, int keep, int dtype, void *state,
                           size_t state_bytes, const float *g_logprobs,
                           const float *g_entropy, void *dhidden, int dt_hidden,
                           void *dweight, int dt_weight, void *workspace,

@@ -88,17 +88,18 @@ SIGNATURES = {
         _I32,
         [_P, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _SZ, _P],
     ),
-    "nf_token_logprobs_state_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "nf_token_logprobs_state_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I32, _I32]),
     "nf_token_logprobs_fwd_workspace": (_SZ, [_I64, _I64, _I64, _I64, _I32, _I32]),
     "nf_token_logprobs_fwd": (
         _I32,
-        [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P, _SZ,
-         _P],
+        [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P, _SZ, _P,
+         _SZ, _P],
     ),
     "nf_token_logprobs_bwd_workspace": (_SZ, [_I64, _I64, _I64, _I64, _I32]),
     "nf_token_logprobs_bwd": (
         _I32,
-        [_P, _I64, _I64, _I64, _I64, _I32, _P, _SZ, _P, _P, _P, _I32, _P, _I32, _P, _SZ, _P],
+        [_P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _SZ, _P, _P, _P, _I32, _P, _I32, _P, _SZ,
+         _P],
     ),
     "nf_embedding_fwd": (
         _I32, [_P, _P, _I64, _F32, _I64, _I64, _I64, _P, _I32, _I32, _P],

@@ -363,7 +363,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   // {logprobs, entropy, top_logprobs, top_ids}; `keep` what the backward reads
   static variable_list run(const Tensor &hidden, const Tensor &weight, const Tensor &targets,
                            int64_t top_k, int64_t chunk_rows, int64_t ignore_index,
-                           at::ScalarType cdt, Tensor &w, Tensor &state) {
+                           at::ScalarType cdt, bool keep, Tensor &w, Tensor &state) {
     const int64_t m = hidden.size(0), d = hidden.size(1), v = weight.size(0);
     const int code = code_of(cdt);
     const Tensor h = hidden.to(cdt).contiguous(), tg = targets.contiguous();
@@ -371,14 +371,14 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
     Tensor lp = at::empty({m}, f32), ent = at::empty({m}, f32), top = at::empty({m, top_k}, f32);
     Tensor ids = at::empty({m, top_k}, f32.dtype(at::kLong));
-    const size_t ns = nf_token_logprobs_state_bytes(m, d, v, code);
+    const size_t ns = nf_token_logprobs_state_bytes(m, d, v, chunk_rows, keep, code);
     const size_t nw = nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, (int)top_k, code);
     TORCH_CHECK_VALUE(ns && nw, "chunked_token_logprobs: shape M=", m, " D=", d, " V=", v,
                       " is beyond the kernels");
     state = bytes(ns, hidden);
     Tensor ws = bytes(nw, hidden);
     check(nf_token_logprobs_fwd(h.data_ptr(), w.data_ptr(), tg.data_ptr<int64_t>(), m, d, v,
-                                ignore_index, chunk_rows, (int)top_k, code, lp.data_ptr<float>(),
+                                ignore_index, chunk_rows, (int)top_k, keep, code, lp.data_ptr<float>(),
                                 ent.data_ptr<float>(), top.data_ptr<float>(),
                                 ids.data_ptr<int64_t>(), state.data_ptr(), ns, ws.data_ptr(), nw,
                                 stream_of(hidden)),
@@ -392,7 +392,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     const auto cdt = (at::ScalarType)compute;
     Tensor w, state;
     const variable_list out =
-        run(hidden, weight, targets, top_k, chunk_rows, ignore_index, cdt, w, state);
+        run(hidden, weight, targets, top_k, chunk_rows, ignore_index, cdt, true, w, state);
     ctx->save_for_backward({w, state});
     ctx->saved_data["s"] = std::vector<int64_t>{hidden.size(0), hidden.size(1), weight.size(0),
                                                 chunk_rows, code_of(cdt),
@@ -423,7 +423,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     if (ctx->needs_input_grad(1)) res[1] = at::empty({v, d}, w.options().dtype(tw));
     const size_t nw = nf_token_logprobs_bwd_workspace(m, d, v, chunk_rows, code);
     Tensor ws = bytes(nw, state);
-    check(nf_token_logprobs_bwd(w.data_ptr(), m, d, v, chunk_rows, code, state.data_ptr(),
+    check(nf_token_logprobs_bwd(w.data_ptr(), m, d, v, chunk_rows, 1, code, state.data_ptr(),
                                 (size_t)state.numel(), (const float *)ptr(g[0]),
                                 (const float *)ptr(g[1]), ptr(res[0]), code_of(th), ptr(res[1]),
                                 code_of(tw), ws.data_ptr(), nw, stream_of(w)),
@@ -674,7 +674,7 @@ PyObject *py_token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     const c10::DeviceGuard guard(dev);
     const at::NoGradGuard no_grad;
     Tensor w, state;
-    return TokenLogprobs::run(t[0], t[1], t[2], v[0], v[1], v[2], cdt, w, state);
+    return TokenLogprobs::run(t[0], t[1], t[2], v[0], v[1], v[2], cdt, false, w, state);
   });
   PyObject *tuple = PyTuple_New(4);
   if (!tuple) return nullptr;

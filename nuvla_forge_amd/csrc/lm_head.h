@@ -107,9 +107,11 @@ static __global__ __launch_bounds__(kCompactThreads) void ce_compact_kernel(
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int e_swz(int t) { return 8 * (((t >> 3) ^ (t & 7)) & 31); }
 
-template <class C, bool SB>
+// TS: the stored type (16 bits with a 16-bit C).
+template <class C, bool SB, typename TS = typename C::TI>
 struct EStore {
-  using TI = typename C::TI;
+  using TI = TS;
+  static_assert(sizeof(TS) == sizeof(typename C::TI), "as wide as the product's inputs");
   static constexpr int ES = (int)sizeof(TI);
   static constexpr bool kStaged = ES == 2 && C::BM == 256 && C::BN == 256 && C::NT == 512 &&
                                   C::LDS_BYTES >= 256 * 512;
@@ -239,11 +241,14 @@ struct EStore {
 // splitk_reduce_kernel would have written to dHc, then scales by g: the same
 // operations in the same order, so the same bits, with one launch and one
 // fp32 pass over the rows fewer.
+// second > 0: row p's gradient is the sum of compacted rows p and second + p (a dz held as two
+// terms: see token_logprobs.hip).
 struct SplitRows {
   const float *part;
   int S;
   int64_t j0, crows;
   const float *cfac;
+  int64_t second = 0;
 };
 template <int VE>
 __global__ __launch_bounds__(256) void ce_scatter_dh_kernel(const float *__restrict__ dHc,
@@ -258,43 +263,52 @@ __global__ __launch_bounds__(256) void ce_scatter_dh_kernel(const float *__restr
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / dv, c = (i - m * dv) * VE;
-    const int p = pos[m];
+    const int first = pos[m];
     float v[VE];
-    if (sp.S > 1 && p >= sp.j0) {
-      const float *src = sp.part + (p - sp.j0) * D + c;
-      float a[VE];
+    auto take = [&](int64_t p, float (&v)[VE]) {
+      if (sp.S > 1 && p >= sp.j0) {
+        const float *src = sp.part + (p - sp.j0) * D + c;
+        float a[VE];
 #pragma unroll
-      for (int k = 0; k < VE; ++k) a[k] = 0.f;
-      // slices added in order, 8 loads in flight per batch
-      constexpr int kBatch = 8;
-      for (int q0 = 0; q0 < sp.S; q0 += kBatch) {
-        float t[kBatch][VE];
+        for (int k = 0; k < VE; ++k) a[k] = 0.f;
+        // slices added in order, 8 loads in flight per batch
+        constexpr int kBatch = 8;
+        for (int q0 = 0; q0 < sp.S; q0 += kBatch) {
+          float t[kBatch][VE];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          if (q0 + u < sp.S) {
-            if constexpr (VE == 4) {
-              const float4 w = *reinterpret_cast<const float4 *>(src + (q0 + u) * slice);
-              t[u][0] = w.x; t[u][1] = w.y; t[u][2] = w.z; t[u][3] = w.w;
-            } else {
-              t[u][0] = src[(q0 + u) * slice];
+          for (int u = 0; u < kBatch; ++u) {
+            if (q0 + u < sp.S) {
+              if constexpr (VE == 4) {
+                const float4 w = *reinterpret_cast<const float4 *>(src + (q0 + u) * slice);
+                t[u][0] = w.x; t[u][1] = w.y; t[u][2] = w.z; t[u][3] = w.w;
+              } else {
+                t[u][0] = src[(q0 + u) * slice];
+              }
             }
           }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+            if (q0 + u < sp.S)
+#pragma unroll
+              for (int k = 0; k < VE; ++k) a[k] += t[u][k];
         }
+        const float f = sp.cfac[p] * 1.f;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-          if (q0 + u < sp.S)
-#pragma unroll
-            for (int k = 0; k < VE; ++k) a[k] += t[u][k];
+        for (int k = 0; k < VE; ++k) v[k] = a[k] * f;
+      } else if constexpr (VE == 4) {
+        const float4 q = p >= 0 ? *reinterpret_cast<const float4 *>(dHc + p * D + c)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+      } else {
+        v[0] = p >= 0 ? dHc[p * D + c] : 0.f;
       }
-      const float f = sp.cfac[p] * 1.f;
+    };
+    take(first, v);
+    if (sp.second > 0 && first >= 0) {
+      float t[VE];
+      take(sp.second + first, t);
 #pragma unroll
-      for (int k = 0; k < VE; ++k) v[k] = a[k] * f;
-    } else if constexpr (VE == 4) {
-      const float4 q = p >= 0 ? *reinterpret_cast<const float4 *>(dHc + (int64_t)p * D + c)
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-      v[0] = p >= 0 ? dHc[(int64_t)p * D + c] : 0.f;
+      for (int k = 0; k < VE; ++k) v[k] += t[k];
     }
 #pragma unroll
     for (int k = 0; k < VE; ++k) store_dyn(dH, dt, m * D + c + k, v[k] * g);
@@ -392,7 +406,8 @@ inline int64_t line_stride(int64_t n, size_t es, std::initializer_list<int64_t> 
   return lines;
 }
 
-template <typename TI>
+// BOTH: 16-bit E may be held in both layouts where they fit (see below); else always once.
+template <typename TI, bool BOTH>
 inline Plan plan_shape(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
   using C = MainCfg<TI>;
   const size_t es = sizeof(TI);
@@ -416,7 +431,7 @@ inline Plan plan_shape(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
     //    1.41-1.46 ms against 1.64 in two chunks);
     //  * chunks of 2 chunk_rows rows held once, beside the fp32 accumulator.
     const int64_t budget = 2 * ((chunk_rows < M ? chunk_rows : M) + D);
-    P.single = D < 2048 || 2 * mcap > budget;
+    P.single = !BOTH || D < 2048 || 2 * mcap > budget;
     const int64_t cr = P.single && mcap > budget ? round_up(2 * want, 256) : mcap;
     P.crows = cr > mcap ? mcap : cr;
   } else {
@@ -470,7 +485,7 @@ inline Plan plan_shape(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
 
 // A thread keeps its last shape's plan: the size calls and the launches of
 // every step ask for the same one.
-template <typename TI>
+template <typename TI, bool BOTH = true>
 inline Plan make_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
   struct Kept {
     int64_t M, D, V, chunk_rows;
@@ -478,7 +493,7 @@ inline Plan make_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
   };
   static thread_local Kept kept{0, 0, 0, 0, {}};
   if (kept.M != M || kept.D != D || kept.V != V || kept.chunk_rows != chunk_rows)
-    kept = {M, D, V, chunk_rows, plan_shape<TI>(M, D, V, chunk_rows)};
+    kept = {M, D, V, chunk_rows, plan_shape<TI, BOTH>(M, D, V, chunk_rows)};
   return kept.P;
 }
 

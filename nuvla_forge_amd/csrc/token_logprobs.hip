@@ -9,16 +9,18 @@
 // Only valid rows (target != ignore_index, inside [0, V)) do any work: they are compacted
 // on the device and every later kernel sizes itself by the device count.
 //
-// Forward (nf_token_logprobs_fwd):
+// Forward (nf_token_logprobs_fwd), more than 64 rows:
 //   1. ce_compact: the valid rows in order.  lp_gather: Hc = hidden[rows], and zeros (id
 //      -1) into the outputs of the other rows.
 //   2. per chunk of rows: lp_logits, the logits tile by tile, of which statistics and
 //      records of strips are left; lp_finish: the row's values from those.
+// Up to 64 rows: lp_skinny, one pass over weight, and lp_finish.
 // Backward (nf_token_logprobs_bwd), with g and h the upstream gradients of a row's logprob
 // and entropy H:
 //   dz = g (onehot - p) - h p (z - lse + H)
-//   lp_dz:  z formed again tile by tile (W Hc^T, as in the cross entropy's logits) and
-//           turned into dz in the accumulators; one rounding to the input type;
+//   dz is formed from what the forward kept of every logit (lp_from_kept), or from the
+//   logits formed again tile by tile (lp_dz: W Hc^T, as in the cross entropy's logits), and
+//   rounded once to the input type;
 //   then the cross entropy's gradient products, dW (+)= dz^T Hc and dHc = dz W, and the
 //   scatter of dHc to the hidden rows.
 #include "lm_head.h"
@@ -37,7 +39,8 @@ constexpr float kFar = -200.f;
 
 // ---------------------------------------------------------------------------
 // 1. Hc[r, :] = hidden[rows[r], :] for r < n, 0 for n <= r < M; rows m that are not
-// valid get 0 in every output (id -1).  One wavefront per row.
+// valid get 0 in every output (id -1).  One wavefront per row.  lo0 > 0: Hc has 2 lo0 >= 2 M
+// rows, the second lo0 as the first (see few_rows).
 // ---------------------------------------------------------------------------
 constexpr int kGatherThreads = 256;
 
@@ -51,12 +54,13 @@ struct RowOut {
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kGatherThreads) void lp_gather_kernel(
     const T *__restrict__ H, int64_t D, const int *__restrict__ rows, const int *__restrict__ pos,
-    const int *n_ptr, int64_t M, T *__restrict__ Hc, RowOut out) {
+    const int *n_ptr, int64_t M, int64_t lo0, T *__restrict__ Hc, RowOut out) {
   constexpr int kWaves = kGatherThreads / 64;
   constexpr int VE = VEC ? 16 / (int)sizeof(T) : 1;
   const int64_t n = *n_ptr;
   const int l = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); r < M;
+  const int64_t R = lo0 > 0 ? lo0 : M;
+  for (int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); r < R;
        r += (int64_t)gridDim.x * kWaves) {
     const T *h = r < n ? H + (int64_t)rows[r] * D : nullptr;
     for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
@@ -64,11 +68,14 @@ __global__ __launch_bounds__(kGatherThreads) void lp_gather_kernel(
         u32x4 v = {0u, 0u, 0u, 0u};
         if (h) v = *reinterpret_cast<const u32x4 *>(h + c);
         *reinterpret_cast<u32x4 *>(Hc + r * D + c) = v;
+        if (lo0 > 0) *reinterpret_cast<u32x4 *>(Hc + (lo0 + r) * D + c) = v;
       } else {
-        Hc[r * D + c] = h ? h[c] : static_cast<T>(0.f);
+        const T v = h ? h[c] : static_cast<T>(0.f);
+        Hc[r * D + c] = v;
+        if (lo0 > 0) Hc[(lo0 + r) * D + c] = v;
       }
     }
-    if (pos[r] < 0) {
+    if (r < M && pos[r] < 0) {
       if (l == 0) {
         out.logprob[r] = 0.f;
         out.entropy[r] = 0.f;
@@ -125,12 +132,25 @@ struct Strips {
 // One block tile: acc = W_tile Hc_tile^T (rows: vocabulary, columns: tokens), so a lane
 // holds 16 TM logits of each of its TN tokens and the strip's values are reductions in
 // registers.  stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
-template <class C, bool BUF, bool TOP>
+// KEEP (16-bit inputs): exp(z - mx), mx the strip's maximum, is kept for the backward in
+// fp16, E [crows, ldp]: half a step of 2^-11 of each, and what is below 2^-24 of the strip's
+// largest is lost.  With bf16, 2^-8, its rounding would add to dz's own.  Blocks past the
+// tiles run the transposes of `tp`.
+template <class C, bool BUF, bool SB, bool TOP, bool KEEP>
 __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
     const typename C::TI *W, const typename C::TI *Hc, int64_t V, int64_t D, int64_t j0,
     int64_t crows, const int *n_ptr, const int *tcol, Stat *stats, int nstat, Rec *recs,
-    float *tgt, int vtiles, int ttiles) {
+    float *tgt, f16 *E, int64_t ldp, int vtiles, int ttiles, gemm::TpJobs tp) {
   __shared__ __attribute__((aligned(16))) char smem[C::LDS_BYTES];
+  if constexpr (KEEP) {
+    static_assert(C::LDS_BYTES >= gemm::kTpRegionRows * gemm::kTpRegionPitch * 2,
+                  "transpose region does not fit the LDS");
+    const int q = (int)blockIdx.x - vtiles * ttiles;
+    if (q >= 0) {
+      if (q < tp.n) gemm::tp_jobs_run<C::NT>(tp, q, reinterpret_cast<uint16_t *>(smem));
+      return;
+    }
+  }
   int vt, tt;
   gemm::group_tile(gemm::xcd_order(blockIdx.x, vtiles * ttiles), vtiles, ttiles,
                    gemm::kTileGroup, vt, tt);
@@ -158,6 +178,9 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
           if (i * 32 + 8 * (r >> 2) + (r & 3) >= vlim) acc[i][j][r] = -INFINITY;
   }
   constexpr int NS = C::TM / 2;  // strips of a lane and token
+  using TS = typename std::conditional<KEEP, f16, typename C::TI>::type;
+  ce::EStore<C, SB, TS> store;
+  if constexpr (KEEP) store.init(E, ldp, nullptr, 0, V, crows, v0, t0, cnt, smem);
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + wn * C::WTN + j * 32 + (l & 31);
@@ -215,11 +238,14 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
         const float e = exp_f32(x);
         s += e;
         t += fmaxf(x, kFar) * e;  // e is 0 where x is -inf, and a NaN where it is one
+        if constexpr (KEEP) acc[i][j][r] = e;
       }
     s += __shfl_xor(s, 32);
     t += __shfl_xor(t, 32);
     if (half == 0 && tok < cnt) stats[tok * nstat + stat] = Stat{mx, s, t, 0.f};
+    if constexpr (KEEP) store.column(j, acc);
   }
+  if constexpr (KEEP) store.finish();
 }
 
 // A row of at most 16 tokens against 16 vocabulary rows, k in order in steps of 32, as the
@@ -536,9 +562,9 @@ template <typename TI, bool VK, int NR>
 __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     const TI *W, const TI *H, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
     const Rec *__restrict__ recs, Strips strips, const float *__restrict__ tgt, int64_t j0,
-    int64_t crows, int *n_ptr, int *rows, int *tcol, int *pos, TI *Hc,
+    int64_t crows, int *n_ptr, int *rows, int *tcol, int *pos, TI *Hc, int64_t lo0,
     const int64_t *__restrict__ targets, int64_t ignore_index, float *__restrict__ lse_out,
-    float *__restrict__ ent_out, RowOut out) {
+    float *__restrict__ ent_out, float *__restrict__ lp_out, RowOut out) {
   constexpr int kWaves = kFinishThreads / 64;
   __shared__ Chosen chosen_w[kWaves];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -547,20 +573,24 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
   int64_t m;
   const TI *hrow;
   if (targets) {
-    if (row >= crows) return;
+    if (row >= (lo0 > 0 ? lo0 : crows)) return;
     m = row;
     hrow = H + row * D;
-    const int tc = target_column(targets, row, V, ignore_index);
+    const int tc = row < crows ? target_column(targets, row, V, ignore_index) : -1;
     constexpr int VE = VK ? 16 / (int)sizeof(TI) : 1;
     for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
       if constexpr (VK) {
         u32x4 x = {0u, 0u, 0u, 0u};
         if (tc >= 0) x = *reinterpret_cast<const u32x4 *>(hrow + c);
         *reinterpret_cast<u32x4 *>(Hc + row * D + c) = x;
+        if (lo0 > 0) *reinterpret_cast<u32x4 *>(Hc + (lo0 + row) * D + c) = x;
       } else {
-        Hc[row * D + c] = tc >= 0 ? hrow[c] : static_cast<TI>(0.f);
+        const TI x = tc >= 0 ? hrow[c] : static_cast<TI>(0.f);
+        Hc[row * D + c] = x;
+        if (lo0 > 0) Hc[(lo0 + row) * D + c] = x;
       }
     }
+    if (row >= crows) return;  // padding of the two copies
     if (l == 0) {
       rows[row] = (int)row;
       pos[row] = (int)row;
@@ -595,6 +625,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
   if (l == 0) {
     lse_out[j0 + row] = lse;
     ent_out[j0 + row] = ent;
+    lp_out[j0 + row] = tgt[row] - lse;
     out.logprob[m] = tgt[row] - lse;
     out.entropy[m] = ent;
   }
@@ -702,16 +733,28 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
 // backward: dz of one chunk, in the layouts of ce::EStore
 // ---------------------------------------------------------------------------
 struct RowIn {
-  const int *n, *rows, *tcol;       // compacted rows
-  const float *lse, *ent;           // per compacted row
-  const float *g, *h;               // upstream, per row of hidden; either may be null
+  const int *n, *rows, *tcol;        // compacted rows
+  const float *lse, *ent, *lp;       // per compacted row
+  const float *g, *h;                // upstream, per row of hidden; either may be null
 };
+
+// With few rows one entry of dz can make up most of a gradient, and its one rounding to 16
+// bits all of the gradient's error (up to 2^-8, measured 3.8e-3 where 1.7e-3 is what the
+// output's own rounding leaves; over many rows the roundings average out).  Up to kFewRows
+// rows dz is therefore held as two 16-bit terms, dz = hi + lo: row r of the products is hi,
+// row lo0 + r is lo, on a second copy of the hidden row.  The rows come free: the tiles have
+// 256 of them.
+constexpr int64_t kFewRows = 128;
+template <typename TI>
+int64_t few_rows(int64_t M) {  // lo0; 0: dz is one term
+  return sizeof(TI) == 2 && M <= kFewRows ? round_up(M, 8) : 0;
+}
 
 template <class C, bool BUF, bool SB>
 __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     const typename C::TI *W, const typename C::TI *Hc, int64_t V, int64_t D, int64_t j0,
-    int64_t crows, RowIn in, float *ones, typename C::TI *E, int64_t ldp, typename C::TI *ET,
-    int64_t ldet, int vtiles, int ttiles, gemm::TpJobs tp) {
+    int64_t crows, RowIn in, int64_t lo0, int *two, float *ones, typename C::TI *E, int64_t ldp,
+    typename C::TI *ET, int64_t ldet, int vtiles, int ttiles, gemm::TpJobs tp) {
   using TI = typename C::TI;
   constexpr int ES = (int)sizeof(TI);
   __shared__ __attribute__((aligned(16))) char smem[C::LDS_BYTES];
@@ -727,10 +770,12 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
   int vt, tt;
   gemm::group_tile(gemm::xcd_order(blockIdx.x, vtiles * ttiles), vtiles, ttiles,
                    gemm::kTileGroup, vt, tt);
-  const int64_t cnt = chunk_count(in.n, j0, crows);
+  const int64_t live = chunk_count(in.n, j0, crows);
+  const int64_t cnt = lo0 > 0 ? 2 * lo0 : live;
   const int64_t v0 = (int64_t)vt * C::BM;
   const int64_t t0 = (int64_t)tt * C::BN;
   if (t0 >= cnt) return;
+  if (lo0 > 0 && blockIdx.x == 0 && threadIdx.x == 0) *two = (int)cnt;
   // the gradient products' row factor is one: dz carries every factor
   if (vt == 0 && threadIdx.x < C::BN && t0 + threadIdx.x < cnt) ones[j0 + t0 + threadIdx.x] = 1.f;
   floatx16 acc[C::TM][C::TN];
@@ -758,15 +803,17 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     const int64_t tok = t0 + wn * C::WTN + j * 32 + (l & 31);
     float g = 0.f, h = 0.f, lse = 0.f, ent = 0.f;
     int want = -1;  // the register that holds the target, if this lane does
-    if (tok < cnt) {
-      const int64_t m = in.rows[j0 + tok];
-      const int tc = in.tcol[j0 + tok];
+    const bool low = lo0 > 0 && tok >= lo0;
+    const int64_t row = j0 + (low ? tok - lo0 : tok);
+    if (row - j0 < live) {
+      const int64_t m = in.rows[row];
+      const int tc = in.tcol[row];
       if (tc >= 0) {  // else a row that does not count: its hidden row is zero here
         g = in.g ? in.g[m] : 0.f;
         h = in.h ? in.h[m] : 0.f;
       }
-      lse = in.lse[j0 + tok];
-      ent = in.ent[j0 + tok];
+      lse = in.lse[row];
+      ent = in.ent[row];
       const int64_t loc64 = (int64_t)tc - vtile0;
       const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
       if (loc >= 0 && ((loc >> 2) & 1) == half)
@@ -781,22 +828,89 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
         // exp is 0 where x is -inf, and a NaN where it is one
         const float dz = exp_f32(x) * (a - h * fmaxf(x, kFar));
         acc[i][j][r] = i * 16 + r == want ? dz + g : dz;
+        if constexpr (ES == 2)
+          if (low) acc[i][j][r] -= static_cast<float>(static_cast<TI>(acc[i][j][r]));
       }
     store.column(j, acc);
   }
   store.finish();
 }
 
+// dz of one chunk from what the forward kept, E [crows, ldp] in fp16: with mx the strip's
+// maximum, p = E exp(mx - lse) and z - lse = log E + mx - lse.  The target's own entry is
+// formed from the row's logprob, which is exact in fp32: 1 - p of a sure token would be lost
+// in E's rounding.  A thread takes 8 columns of a row (they lie in one strip).
+constexpr int kKeptThreads = 256;
+constexpr int64_t kKeptCols = (int64_t)1 << 26;  // the grid's second extent ends at 65535 blocks
+
+template <int WTM>
+__global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
+    const f16 *__restrict__ E, bf16 *__restrict__ dz, int64_t ldp, int64_t V,
+    const Stat *__restrict__ stats, int nstat, RowIn in, float *__restrict__ ones) {
+  const int64_t row = blockIdx.x, live = *in.n;
+  if (row >= (live + 7) / 8 * 8) return;
+  const int64_t c = ((int64_t)blockIdx.y * kKeptThreads + threadIdx.x) * 8;
+  if (c >= ldp) return;
+  float v[8];
+  if (row >= live) {  // the products' K padding
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    Chunk8<bf16>::store(dz + row * ldp + c, v);
+    return;
+  }
+  const int64_t m = in.rows[row];
+  const float g = in.g ? in.g[m] : 0.f, h = in.h ? in.h[m] : 0.f;
+  const float lse = in.lse[row], ent = in.ent[row], a = -(g + h * ent);
+  if (c == 0) ones[row] = 1.f;
+  Chunk8<f16>::load(E + row * ldp + c, v);
+  if (c < V) {
+    const float o = stats[row * nstat + c / WTM].mx - lse;
+    const float f = exp_f32(o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // log 0 = -inf goes with p = 0; a NaN stays one through p
+      const float x = h != 0.f ? fmaxf(log_f32(v[i]) + o, kFar) : 0.f;
+      v[i] = v[i] * f * (a - h * x);
+    }
+    const int64_t t = in.tcol[row] - c;
+    if (t >= 0 && t < 8) {
+      const float lp = in.lp[row];
+      const float own = exp_f32(lp) * (a - h * fmaxf(lp, kFar)) + g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i == t ? own : v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  }
+  Chunk8<bf16>::store(dz + row * ldp + c, v);
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// What the forward keeps for the backward.
+template <typename TI>
+ce::Plan grad_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
+  const int64_t lo0 = few_rows<TI>(M);
+  return ce::make_plan<TI, false>(lo0 > 0 ? 2 * lo0 : M, D, V, chunk_rows);
+}
+
+// What the forward keeps for the backward: the rows, and, with `keep`, where one chunk takes
+// every row (by chunk_rows' bound on memory), exp(z - mx) of every logit with the strips'
+// statistics and the transposes of weight and of the rows that the products read: the
+// backward then forms dz in one pass over it instead of forming the logits again (M 4096,
+// D 2048, V 32000: see nf_token_logprobs_bwd).
 struct State {
-  size_t scal, rows, tcol, pos, lse, ent, hc, total;
+  bool kept;
+  int nstat;
+  int64_t lo0;
+  size_t scal, rows, tcol, pos, lse, ent, lp, hc, e, stats, wt, hct, total;
 };
 template <typename TI>
-State state_layout(int64_t M, int64_t D) {
+State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool keep) {
+  using C = MainCfg<TI>;
   State s{};
+  s.lo0 = few_rows<TI>(M);
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
   s.scal = take(64);
@@ -805,7 +919,19 @@ State state_layout(int64_t M, int64_t D) {
   s.pos = take((size_t)M * sizeof(int));
   s.lse = take((size_t)M * sizeof(float));
   s.ent = take((size_t)M * sizeof(float));
-  s.hc = take((size_t)M * D * sizeof(TI));
+  s.lp = take((size_t)M * sizeof(float));
+  s.hc = take((size_t)(s.lo0 > 0 ? 2 * s.lo0 : M) * D * sizeof(TI));
+  if (sizeof(TI) == 2 && keep && M > kFewRows && V <= kKeptCols) {
+    const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
+    if (L.nch == 1) {
+      s.kept = true;
+      s.nstat = (int)((V + C::BM - 1) / C::BM) * C::WM;
+      s.e = take((size_t)L.crows * L.ldp * sizeof(f16));
+      s.stats = take((size_t)L.crows * s.nstat * sizeof(Stat));
+      s.wt = take((size_t)D * L.ldwt * sizeof(TI));
+      s.hct = take((size_t)D * L.ldht * sizeof(TI));
+    }
+  }
   s.total = o;
   return s;
 }
@@ -814,8 +940,10 @@ struct View {
   int *n;
   float *inv;
   int *rows, *tcol, *pos;
-  float *lse, *ent;
-  TI *Hc;
+  float *lse, *ent, *lp;
+  TI *Hc, *Wt, *Hct;
+  f16 *E;
+  Stat *stats;
   View(const State &L, char *s)
       : n(reinterpret_cast<int *>(s + L.scal)),
         inv(reinterpret_cast<float *>(s + L.scal + 16)),
@@ -824,8 +952,41 @@ struct View {
         pos(reinterpret_cast<int *>(s + L.pos)),
         lse(reinterpret_cast<float *>(s + L.lse)),
         ent(reinterpret_cast<float *>(s + L.ent)),
-        Hc(reinterpret_cast<TI *>(s + L.hc)) {}
+        lp(reinterpret_cast<float *>(s + L.lp)),
+        Hc(reinterpret_cast<TI *>(s + L.hc)),
+        Wt(reinterpret_cast<TI *>(s + L.wt)),
+        Hct(reinterpret_cast<TI *>(s + L.hct)),
+        E(reinterpret_cast<f16 *>(s + L.e)),
+        stats(reinterpret_cast<Stat *>(s + L.stats)) {}
 };
+
+// W^T (the dH product's B operand) and Hc^T (the dW product's), both zero-padded: as extra
+// blocks (`tp`) of a launch of tiles where their rows are whole 16-byte vectors of 16-bit
+// elements, else by launches of their own.
+template <typename TI>
+int transposes(const TI *W, const TI *Hc, int64_t Mb, int64_t D, int64_t V, const ce::Plan &L,
+               TI *Wt, TI *Hct, gemm::TpJobs &tp, hipStream_t s) {
+  using U = typename std::conditional<sizeof(TI) == 2, uint16_t, uint32_t>::type;
+  tp = gemm::TpJobs{};
+  if (sizeof(TI) == 2 && D % 8 == 0 && aligned16(W)) {
+    auto add = [&](int j, const TI *in, int64_t R, TI *out, int64_t ldo) {
+      tp.in[j] = reinterpret_cast<const uint16_t *>(in);
+      tp.out[j] = reinterpret_cast<uint16_t *>(out);
+      tp.R[j] = R;
+      tp.Cn[j] = D;
+      tp.ldi[j] = D;
+      tp.ldo[j] = ldo;
+      tp.rb[j] = (int)((ldo + gemm::kTpRegionRows - 1) / gemm::kTpRegionRows);
+      tp.cb[j] = (int)((D + gemm::kTpRegionCols - 1) / gemm::kTpRegionCols);
+      tp.n += tp.rb[j] * tp.cb[j];
+    };
+    add(0, W, V, Wt, L.ldwt);
+    add(1, Hc, Mb, Hct, L.ldht);
+    return NF_OK;
+  }
+  if (int e = launch_transpose<U>(W, V, D, D, Wt, L.ldwt, s)) return e;
+  return launch_transpose<U>(Hc, Mb, D, D, Hct, L.ldht, s);
+}
 
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
@@ -837,19 +998,21 @@ struct FwdPlan {
   size_t stats, recs, tgt, total;
 };
 template <typename TI>
-FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k) {
+FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept) {
   using C = MainCfg<TI>;
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
   p.skinny = M <= kSkinnyRows;
-  p.crows = p.skinny ? M : chunk_rows < mcap / 8 ? round_up(8 * chunk_rows, 256) : mcap;
+  p.crows = p.skinny ? M
+            : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
+                                             : mcap;
   p.vtiles = (int)((V + C::BM - 1) / C::BM);
   p.nstat = p.skinny ? (int)((V + 31) / 32) : p.vtiles * C::WM;
   p.strips = Strips{p.skinny ? 0 : C::WTM == 128 ? 2 : 1};
   static_assert(C::WTM == 128 || C::WTM == 64, "strips of a wavefront's tile");
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
-  p.stats = take((size_t)p.crows * p.nstat * sizeof(Stat));
+  p.stats = take(kept ? 0 : (size_t)p.crows * p.nstat * sizeof(Stat));
   p.recs = take(top_k ? (size_t)p.crows * p.nstat * p.strips.per_stat() * sizeof(Rec) : 0);
   p.tgt = take((size_t)p.crows * sizeof(float));
   p.total = o;
@@ -859,15 +1022,16 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k) {
 template <typename TI>
 int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan &P,
                   const Stat *stats, const Rec *recs, const float *tgt, int64_t j0, int64_t rows,
-                  const View<TI> &S, const int64_t *targets, int64_t ignore_index,
+                  const View<TI> &S, int64_t lo0, const int64_t *targets, int64_t ignore_index,
                   const RowOut &out, hipStream_t s) {
   const bool vk = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(W) && aligned16(H);
-  const unsigned grid = (unsigned)((rows + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
+  const int64_t waves = targets && lo0 > 0 ? lo0 : rows;
+  const unsigned grid = (unsigned)((waves + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
   const int nrec = P.nstat * P.strips.per_stat();
 #define NF_LP_FINISH(VK, NR)                                                                   \
   lp_finish_kernel<TI, VK, NR><<<grid, kFinishThreads, 0, s>>>(                                \
       W, H, V, D, stats, P.nstat, recs, P.strips, tgt, j0, rows, S.n, S.rows, S.tcol, S.pos,   \
-      S.Hc, targets, ignore_index, S.lse, S.ent, out)
+      S.Hc, lo0, targets, ignore_index, S.lse, S.ent, S.lp, out)
   if (vk && nrec <= 64 * 16)
     NF_LP_FINISH(true, 16);
   else if (vk && nrec <= 64 * 32)
@@ -882,12 +1046,13 @@ int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan 
 
 template <typename TI>
 int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t D, int64_t V,
-            int64_t ignore_index, int64_t chunk_rows, const RowOut &out, char *state, char *ws,
-            hipStream_t s) {
+            int64_t ignore_index, int64_t chunk_rows, bool keep, const RowOut &out, char *state,
+            char *ws, hipStream_t s) {
   using C = MainCfg<TI>;
-  const View<TI> S(state_layout<TI>(M, D), state);
-  const FwdPlan P = fwd_plan<TI>(M, V, chunk_rows, out.top_k);
-  Stat *stats = reinterpret_cast<Stat *>(ws + P.stats);
+  const State L = state_layout<TI>(M, D, V, chunk_rows, keep);
+  const View<TI> S(L, state);
+  const FwdPlan P = fwd_plan<TI>(M, V, chunk_rows, out.top_k, L.kept);
+  Stat *stats = L.kept ? S.stats : reinterpret_cast<Stat *>(ws + P.stats);
   Rec *recs = out.top_k ? reinterpret_cast<Rec *>(ws + P.recs) : nullptr;
   float *tgt = reinterpret_cast<float *>(ws + P.tgt);
   const int64_t VE = 16 / (int64_t)sizeof(TI);
@@ -909,8 +1074,8 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
       NF_LP_SKINNY(4, false);
 #undef NF_LP_SKINNY
     if ((e = check_launch("lp_skinny"))) return e;
-    return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, targets, ignore_index,
-                             out, s);
+    return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, L.lo0, targets,
+                             ignore_index, out, s);
   }
   ce::ce_compact_kernel<<<1, ce::kCompactThreads, 0, s>>>(targets, M, V, ignore_index, S.rows,
                                                           S.tcol, S.pos, S.n, S.inv, nullptr);
@@ -919,32 +1084,60 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
   int64_t blocks = (M + 3) / 4;
   if (blocks > 4096) blocks = 4096;
   if (vec)
-    lp_gather_kernel<TI, true><<<(unsigned)blocks, kGatherThreads, 0, s>>>(H, D, S.rows, S.pos,
-                                                                           S.n, M, S.Hc, out);
+    lp_gather_kernel<TI, true><<<(unsigned)blocks, kGatherThreads, 0, s>>>(
+        H, D, S.rows, S.pos, S.n, M, L.lo0, S.Hc, out);
   else
-    lp_gather_kernel<TI, false><<<(unsigned)blocks, kGatherThreads, 0, s>>>(H, D, S.rows, S.pos,
-                                                                            S.n, M, S.Hc, out);
+    lp_gather_kernel<TI, false><<<(unsigned)blocks, kGatherThreads, 0, s>>>(
+        H, D, S.rows, S.pos, S.n, M, L.lo0, S.Hc, out);
   if ((e = check_launch("lp_gather"))) return e;
   const bool vk = buf_ok<TI>(S.Hc, D, M, D) && buf_ok<TI>(W, D, V, D);
+  gemm::TpJobs tp{};
+  int64_t ldp = 0;
+  bool sb = false;
+  if (L.kept) {
+    const ce::Plan G = grad_plan<TI>(M, D, V, chunk_rows);
+    ldp = G.ldp;
+    sb = sb_ok(G.crows * ldp * (int64_t)sizeof(f16));
+    if ((e = transposes<TI>(W, S.Hc, M, D, V, G, S.Wt, S.Hct, tp, s))) return e;
+  }
   for (int64_t j0 = 0; j0 < M; j0 += P.crows) {
     const int64_t rows = M - j0 < P.crows ? M - j0 : P.crows;
     const int ttiles = (int)((rows + C::BN - 1) / C::BN);
-    const unsigned grid = (unsigned)(P.vtiles * ttiles);
-#define NF_LP_LOGITS(BUF, TOP)                                                                \
-  lp_logits_kernel<C, BUF, TOP><<<grid, C::NT, 0, s>>>(W, S.Hc, V, D, j0, rows, S.n, S.tcol,  \
-                                                       stats, P.nstat, recs, tgt, P.vtiles,   \
-                                                       ttiles)
-    if (vk && out.top_k)
-      NF_LP_LOGITS(true, true);
+    const unsigned grid = (unsigned)(P.vtiles * ttiles + tp.n);
+    // kept: the chunk is every row, and E's extent that of its buffer
+#define NF_LP_LOGITS(BUF, SB, TOP, KEEP)                                                      \
+  lp_logits_kernel<C, BUF, SB, TOP, KEEP><<<grid, C::NT, 0, s>>>(                             \
+      W, S.Hc, V, D, j0, P.crows, S.n, S.tcol, stats, P.nstat, recs, tgt, S.E, ldp, P.vtiles, \
+      ttiles, tp)
+    bool launched = false;
+    if constexpr (sizeof(TI) == 2) {
+      launched = L.kept;
+      if (L.kept && vk && sb && out.top_k)
+        NF_LP_LOGITS(true, true, true, true);
+      else if (L.kept && vk && sb)
+        NF_LP_LOGITS(true, true, false, true);
+      else if (L.kept && vk && out.top_k)
+        NF_LP_LOGITS(true, false, true, true);
+      else if (L.kept && vk)
+        NF_LP_LOGITS(true, false, false, true);
+      else if (L.kept && out.top_k)
+        NF_LP_LOGITS(false, false, true, true);
+      else if (L.kept)
+        NF_LP_LOGITS(false, false, false, true);
+    }
+    if (launched)
+      ;
+    else if (vk && out.top_k)
+      NF_LP_LOGITS(true, false, true, false);
     else if (vk)
-      NF_LP_LOGITS(true, false);
+      NF_LP_LOGITS(true, false, false, false);
     else if (out.top_k)
-      NF_LP_LOGITS(false, true);
+      NF_LP_LOGITS(false, false, true, false);
     else
-      NF_LP_LOGITS(false, false);
+      NF_LP_LOGITS(false, false, false, false);
 #undef NF_LP_LOGITS
     if ((e = check_launch("lp_logits"))) return e;
-    if ((e = launch_finish<TI>(W, S.Hc, V, D, P, stats, recs, tgt, j0, rows, S, nullptr,
+    if ((e = launch_finish<TI>(W, S.Hc, V, D, P, stats, recs, tgt, j0, rows, S, L.lo0, nullptr,
                                ignore_index, out, s)))
       return e;
   }
@@ -952,64 +1145,60 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
 }
 
 template <typename TI>
-int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, char *state,
-            const float *g, const float *h, void *dH, int dt_h, void *dW, int dt_w, char *ws,
-            hipStream_t s) {
+int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool keep,
+            char *state, const float *g, const float *h, void *dH, int dt_h, void *dW, int dt_w,
+            char *ws, hipStream_t s) {
   using C = MainCfg<TI>;
-  using U = typename std::conditional<sizeof(TI) == 2, uint16_t, uint32_t>::type;
-  const View<TI> K(state_layout<TI>(M, D), state);
-  const ce::Plan L = ce::make_plan<TI>(M, D, V, chunk_rows);
+  const State KL = state_layout<TI>(M, D, V, chunk_rows, keep);
+  const View<TI> K(KL, state);
+  const int64_t lo0 = KL.lo0, Mb = lo0 > 0 ? 2 * lo0 : M;  // rows of the products
+  const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
   ce::StateView<TI> S(L, ws);
-  S.n = K.n;
-  S.pos = K.pos;
+  int *const two = S.n;
+  if (lo0 == 0) S.n = K.n;  // else *two, by lp_dz
   float *part = reinterpret_cast<float *>(ws + L.s_total);
-  int e;
-  // W^T (the dH product's B operand) and Hc^T (the dW product's), both zero-padded: by
-  // extra blocks of the first dz launch where their rows are whole 16-byte vectors of
-  // 16-bit elements, else by launches of their own
+  const RowIn in{K.n, K.rows, K.tcol, K.lse, K.ent, K.lp, g, h};
+  TI *const PT = L.single ? nullptr : S.PT;
   gemm::TpJobs tp{};
   const gemm::TpJobs none{};
-  const bool fold = sizeof(TI) == 2 && D % 8 == 0 && aligned16(W);
-  if (fold) {
-    auto add = [&](int j, const TI *in, int64_t R, TI *out, int64_t ldo) {
-      tp.in[j] = reinterpret_cast<const uint16_t *>(in);
-      tp.out[j] = reinterpret_cast<uint16_t *>(out);
-      tp.R[j] = R;
-      tp.Cn[j] = D;
-      tp.ldi[j] = D;
-      tp.ldo[j] = ldo;
-      tp.rb[j] = (int)((ldo + gemm::kTpRegionRows - 1) / gemm::kTpRegionRows);
-      tp.cb[j] = (int)((D + gemm::kTpRegionCols - 1) / gemm::kTpRegionCols);
-      tp.n += tp.rb[j] * tp.cb[j];
-    };
-    add(0, W, V, S.Wt, L.ldwt);
-    add(1, K.Hc, M, S.Hct, L.ldht);
-  } else {
-    if ((e = launch_transpose<U>(W, V, D, D, S.Wt, L.ldwt, s))) return e;
-    if ((e = launch_transpose<U>(K.Hc, M, D, D, S.Hct, L.ldht, s))) return e;
+  int e;
+  if (KL.kept) {
+    S.Wt = K.Wt;
+    S.Hct = K.Hct;
+  } else if ((e = transposes<TI>(W, K.Hc, Mb, D, V, L, S.Wt, S.Hct, tp, s))) {
+    return e;
   }
-  const bool vk = buf_ok<TI>(K.Hc, D, M, D) && buf_ok<TI>(W, D, V, D);
+  const bool vk = buf_ok<TI>(K.Hc, D, Mb, D) && buf_ok<TI>(W, D, V, D);
   const bool sb = sb_ok(L.crows * L.ldp * (int64_t)sizeof(TI)) &&
                   (L.single || sb_ok(V * L.crows * (int64_t)sizeof(TI)));
-  const RowIn in{K.n, K.rows, K.tcol, K.lse, K.ent, g, h};
-  TI *const PT = L.single ? nullptr : S.PT;
   for (int64_t c = 0; c < L.nch; ++c) {
     const int64_t j0 = c * L.crows;
     const gemm::TpJobs &tj = c == 0 ? tp : none;
     const unsigned grid = (unsigned)(L.vtiles * L.ttiles) + (unsigned)tj.n;
-    if (vk && sb)
-      lp_dz_kernel<C, true, true><<<grid, C::NT, 0, s>>>(W, K.Hc, V, D, j0, L.crows, in, S.cfac,
-                                                         S.P, L.ldp, PT, L.crows, L.vtiles,
-                                                         L.ttiles, tj);
+#define NF_LP_DZ(BUF, SB)                                                                      \
+  lp_dz_kernel<C, BUF, SB><<<grid, C::NT, 0, s>>>(W, K.Hc, V, D, j0, L.crows, in, lo0, two,    \
+                                                  S.cfac, S.P, L.ldp, PT, L.crows, L.vtiles,   \
+                                                  L.ttiles, tj)
+    bool formed = false;
+    if constexpr (sizeof(TI) == 2) {
+      formed = KL.kept;
+      if (KL.kept) {
+        const dim3 kg((unsigned)round_up(M, 8),
+                      (unsigned)((L.ldp / 8 + kKeptThreads - 1) / kKeptThreads));
+        lp_from_kept_kernel<C::WTM><<<kg, kKeptThreads, 0, s>>>(K.E, S.P, L.ldp, V, K.stats,
+                                                                KL.nstat, in, S.cfac);
+      }
+    }
+    if (formed)
+      ;
+    else if (vk && sb)
+      NF_LP_DZ(true, true);
     else if (vk)
-      lp_dz_kernel<C, true, false><<<grid, C::NT, 0, s>>>(W, K.Hc, V, D, j0, L.crows, in, S.cfac,
-                                                          S.P, L.ldp, PT, L.crows, L.vtiles,
-                                                          L.ttiles, tj);
+      NF_LP_DZ(true, false);
     else
-      lp_dz_kernel<C, false, false><<<grid, C::NT, 0, s>>>(W, K.Hc, V, D, j0, L.crows, in,
-                                                           S.cfac, S.P, L.ldp, PT, L.crows,
-                                                           L.vtiles, L.ttiles, tj);
-    if ((e = check_launch("lp_dz"))) return e;
+      NF_LP_DZ(false, false);
+#undef NF_LP_DZ
+    if ((e = check_launch(formed ? "lp_from_kept" : "lp_dz"))) return e;
     const bool last = c + 1 == L.nch;
     if ((e = ce::launch_grads<TI>(L, S, c, D, V, c > 0 ? S.dWacc : nullptr,
                                   last ? dW : S.dWacc, last ? dt_w : NF_DTYPE_F32, nullptr, part,
@@ -1018,7 +1207,7 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, ch
       return e;
   }
   if (!dH) return NF_OK;
-  const ce::SplitRows sp{part, L.split.S, (L.nch - 1) * L.crows, L.crows, S.cfac};
+  const ce::SplitRows sp{part, L.split.S, (L.nch - 1) * L.crows, L.crows, S.cfac, lo0};
   const bool vec = D % 4 == 0;
   int64_t blocks = (M * (vec ? D / 4 : D) + 255) / 256;
   if (blocks > 4096) blocks = 4096;
@@ -1031,9 +1220,10 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, ch
   return check_launch("ce_scatter_dh");
 }
 
+// fp32 plans hold E in both layouts; what kept states hold themselves is still in the count.
 template <typename TI>
 size_t bwd_bytes(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
-  const ce::Plan L = ce::make_plan<TI>(M, D, V, chunk_rows);
+  const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
   return L.s_total + L.b_total + 256;
 }
 
@@ -1047,9 +1237,11 @@ using ce::ce_check_shape;
 using ce::ce_sizes_ok;
 using ce::dtype_ok;
 
-extern "C" size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V, int dtype) {
-  if (!ce_sizes_ok(M, D, V) || !dtype_ok(dtype)) return 0;
-  return dtype == NF_DTYPE_BF16 ? state_layout<bf16>(M, D).total : state_layout<float>(M, D).total;
+extern "C" size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V,
+                                                int64_t chunk_rows, int keep, int dtype) {
+  if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype)) return 0;
+  return dtype == NF_DTYPE_BF16 ? state_layout<bf16>(M, D, V, chunk_rows, keep != 0).total
+                                : state_layout<float>(M, D, V, chunk_rows, keep != 0).total;
 }
 
 extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t V,
@@ -1057,8 +1249,8 @@ extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t 
   if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype) || top_k < 0 ||
       top_k > kMaxTop || top_k > V)
     return 0;
-  return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows, top_k).total
-                                : fwd_plan<float>(M, V, chunk_rows, top_k).total;
+  return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows, top_k, false).total
+                                : fwd_plan<float>(M, V, chunk_rows, top_k, false).total;
 }
 
 extern "C" size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,
@@ -1071,7 +1263,7 @@ extern "C" size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t 
 extern "C" int nf_token_logprobs_fwd(const void *hidden, const void *weight,
                                      const int64_t *targets, int64_t M, int64_t D, int64_t V,
                                      int64_t ignore_index, int64_t chunk_rows, int top_k,
-                                     int dtype, float *logprobs, float *entropy,
+                                     int keep, int dtype, float *logprobs, float *entropy,
                                      float *top_logprobs, int64_t *top_ids, void *state,
                                      size_t state_bytes, void *workspace,
                                      size_t workspace_bytes, void *stream) {
@@ -1084,7 +1276,7 @@ extern "C" int nf_token_logprobs_fwd(const void *hidden, const void *weight,
       (top_k > 0 && (!top_logprobs || !top_ids)))
     return set_error(NF_ERR_ARG, "%s: null pointer", fn);
   if (int e = ce_check_dtype(fn, dtype)) return e;
-  const size_t sb = nf_token_logprobs_state_bytes(M, D, V, dtype);
+  const size_t sb = nf_token_logprobs_state_bytes(M, D, V, chunk_rows, keep, dtype);
   if (state_bytes < sb || !aligned16(state))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu bytes < required %zu", fn, state_bytes, sb);
   const size_t wb = nf_token_logprobs_fwd_workspace(M, D, V, chunk_rows, top_k, dtype);
@@ -1096,13 +1288,13 @@ extern "C" int nf_token_logprobs_fwd(const void *hidden, const void *weight,
   const RowOut out{logprobs, entropy, top_logprobs, top_ids, top_k};
   if (dtype == NF_DTYPE_BF16)
     return fwd_run<bf16>((const bf16 *)hidden, (const bf16 *)weight, targets, M, D, V,
-                         ignore_index, chunk_rows, out, st, ws, s);
+                         ignore_index, chunk_rows, keep != 0, out, st, ws, s);
   return fwd_run<float>((const float *)hidden, (const float *)weight, targets, M, D, V,
-                        ignore_index, chunk_rows, out, st, ws, s);
+                        ignore_index, chunk_rows, keep != 0, out, st, ws, s);
 }
 
 extern "C" int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, int64_t V,
-                                     int64_t chunk_rows, int dtype, void *state,
+                                     int64_t chunk_rows, int keep, int dtype, void *state,
                                      size_t state_bytes, const float *g_logprobs,
                                      const float *g_entropy, void *dhidden, int dt_hidden,
                                      void *dweight, int dt_weight, void *workspace,
@@ -1114,7 +1306,7 @@ extern "C" int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, i
   if (int e = ce_check_dtype(fn, dtype)) return e;
   if ((dhidden && !is_dtype(dt_hidden)) || (dweight && !is_dtype(dt_weight)))
     return set_error(NF_ERR_DTYPE, "%s: gradient dtypes %d, %d", fn, dt_hidden, dt_weight);
-  const size_t sb = nf_token_logprobs_state_bytes(M, D, V, dtype);
+  const size_t sb = nf_token_logprobs_state_bytes(M, D, V, chunk_rows, keep, dtype);
   if (state_bytes < sb || !aligned16(state))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu bytes < required %zu", fn, state_bytes, sb);
   const size_t wb = nf_token_logprobs_bwd_workspace(M, D, V, chunk_rows, dtype);
@@ -1125,8 +1317,8 @@ extern "C" int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, i
   hipStream_t s = static_cast<hipStream_t>(stream);
   char *st = static_cast<char *>(state), *ws = static_cast<char *>(workspace);
   if (dtype == NF_DTYPE_BF16)
-    return bwd_run<bf16>((const bf16 *)weight, M, D, V, chunk_rows, st, g_logprobs, g_entropy,
+    return bwd_run<bf16>((const bf16 *)weight, M, D, V, chunk_rows, keep != 0, st, g_logprobs, g_entropy,
                          dhidden, dt_hidden, dweight, dt_weight, ws, s);
-  return bwd_run<float>((const float *)weight, M, D, V, chunk_rows, st, g_logprobs, g_entropy,
+  return bwd_run<float>((const float *)weight, M, D, V, chunk_rows, keep != 0, st, g_logprobs, g_entropy,
                         dhidden, dt_hidden, dweight, dt_weight, ws, s);
 }

@@ -74,7 +74,11 @@ class _TokenLogprobs(torch.autograd.Function):
             ctx.save_for_backward(w)
             return logprobs, entropy, top_lp, top_ids
         L, code = _lib.lib(), _lib.dtype_code(cdt)
-        st_bytes = L.nf_token_logprobs_state_bytes(m, d, v, code)
+        # what a backward reads instead of forming the logits again (asked of the inputs: inside
+        # a Function no gradient is being recorded)
+        keep = any(ctx.needs_input_grad[:2])
+        ctx.keep = keep
+        st_bytes = L.nf_token_logprobs_state_bytes(m, d, v, chunk_rows, keep, code)
         ws_bytes = L.nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, top_k, code)
         if not st_bytes or not ws_bytes:
             raise ValueError(f"chunked_token_logprobs: shape M={m} D={d} V={v} is beyond the "
@@ -84,7 +88,7 @@ class _TokenLogprobs(torch.autograd.Function):
         with device_of(hidden):
             _lib.check(
                 L.nf_token_logprobs_fwd(h.data_ptr(), w.data_ptr(), tg.data_ptr(), m, d, v,
-                                        ignore_index, chunk_rows, top_k, code,
+                                        ignore_index, chunk_rows, top_k, keep, code,
                                         logprobs.data_ptr(), entropy.data_ptr(),
                                         top_lp.data_ptr(), top_ids.data_ptr(), state.data_ptr(),
                                         st_bytes, ws.data_ptr(), ws_bytes,
@@ -119,7 +123,7 @@ class _TokenLogprobs(torch.autograd.Function):
         ow = dw if dw is None or dw.dtype == wide[1] else torch.empty_like(dw, dtype=wide[1])
         with device_of(w):
             _lib.check(
-                L.nf_token_logprobs_bwd(w.data_ptr(), m, d, v, chunk_rows, code,
+                L.nf_token_logprobs_bwd(w.data_ptr(), m, d, v, chunk_rows, ctx.keep, code,
                                         state.data_ptr(), state.numel(), _lib.ptr(g),
                                         _lib.ptr(h), _lib.ptr(oh), _lib.dtype_code(wide[0]),
                                         _lib.ptr(ow), _lib.dtype_code(wide[1]), ws.data_ptr(),

@@ -421,6 +421,37 @@ def test_logprobs_one_gradient_at_a_time(cuda):
                 assert ((x.double() - ref[name]).abs() <= ref["tol_" + name]).all()
 
 
+@pytest.mark.parametrize("m, chunk_size", [(3, 1024), (100, 1024), (300, 1024), (300, 1)])
+def test_logprobs_backward_twice(cuda, m, chunk_size):
+    """What the forward kept serves again: two backward passes of one graph give the same bits."""
+    note(f"logprobs twice {m} {chunk_size}")
+    h, w, t, g, gh = _head(m, 64, 1500, BF16, cuda)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, chunk_size=chunk_size)
+    first = torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh], retain_graph=True)
+    again = torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_logprobs_gradient_of_few_rows_is_rounded_once(cuda):
+    """With few rows dz is held as two bf16 terms (2^-16 of it left), so the gradients are off by
+    little more than their own rounding."""
+    note("logprobs few rows")
+    for m in (1, 2, 9, 65, 128):
+        h, w, t, g, gh = _head(m, 128, 2003, BF16, cuda, seed=m, std=0.5)
+        h, w = h.requires_grad_(True), w.requires_grad_(True)
+        out = chunked_token_logprobs(h, w, t)
+        ref = logprobs64(h.float(), w.float(), t, g, gh)  # fp32's bounds, without bf16's
+        for x, name in zip(torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh]),
+                           ("dh", "dw")):
+            off = (x.double() - ref[name]).abs()
+            size = torch.zeros_like(off)
+            tol = ref["tol_" + name] * 2 + half_step(BF16) * ref[name].abs()
+            # 2^-16 of dz, against the sum of |dz||w| or |dz||h|: from the bound of one bf16 term
+            one = logprobs64(h, w, t, g, gh)["tol_" + name]
+            assert (off <= tol + 2.0 ** -7 * one + size).all(), (m, name, (off / tol).max())
+
+
 def test_logprobs_types_and_views(cuda):
     note("logprobs types")
     h, w, t, g, gh = _head(50, 64, 700, F32, cuda)

@@ -236,28 +236,28 @@ def test_logprobs_refusals():
 
 def test_logprobs_c_abi_refusals():
     L = _lib.lib()
-    st, fw = (L.nf_token_logprobs_state_bytes(16, 64, 100, 1),
+    st, fw = (L.nf_token_logprobs_state_bytes(16, 64, 100, 1024, 1, 1),
               L.nf_token_logprobs_fwd_workspace(16, 64, 100, 1024, 5, 1))
     bw = L.nf_token_logprobs_bwd_workspace(16, 64, 100, 1024, 1)
     assert st > 0 and fw > 0 and bw > 0
-    assert L.nf_token_logprobs_state_bytes(16, 64, 100, 2) == 0
+    assert L.nf_token_logprobs_state_bytes(16, 64, 100, 1024, 1, 2) == 0
     assert L.nf_token_logprobs_fwd_workspace(16, 64, 100, 1024, 33, 1) == 0
     assert L.nf_token_logprobs_fwd_workspace(16, 64, 4, 1024, 5, 1) == 0
     assert L.nf_token_logprobs_bwd_workspace(16, 64, 100, 0, 1) == 0
-    ok = [FAKE, FAKE, FAKE, 16, 64, 100, -100, 1024, 5, 1, FAKE, FAKE, FAKE, FAKE, FAKE, st, FAKE,
-          fw, None]
+    ok = [FAKE, FAKE, FAKE, 16, 64, 100, -100, 1024, 5, 1, 1, FAKE, FAKE, FAKE, FAKE, FAKE, st,
+          FAKE, fw, None]
     bad = [(3, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (5, 1 << 32, NF_ERR_ARG), (7, 0, NF_ERR_ARG),
-           (8, -1, NF_ERR_ARG), (8, 33, NF_ERR_ARG), (9, 2, NF_ERR_DTYPE),
-           (14, FAKE + 8, NF_ERR_WORKSPACE), (15, st - 1, NF_ERR_WORKSPACE),
-           (16, None, NF_ERR_WORKSPACE), (17, fw - 1, NF_ERR_WORKSPACE)]
-    bad += [(i, None, NF_ERR_ARG) for i in (0, 1, 2, 10, 11, 12, 13, 14)]
+           (8, -1, NF_ERR_ARG), (8, 33, NF_ERR_ARG), (10, 2, NF_ERR_DTYPE),
+           (15, FAKE + 8, NF_ERR_WORKSPACE), (16, st - 1, NF_ERR_WORKSPACE),
+           (17, None, NF_ERR_WORKSPACE), (18, fw - 1, NF_ERR_WORKSPACE)]
+    bad += [(i, None, NF_ERR_ARG) for i in (0, 1, 2, 11, 12, 13, 14, 15)]
     for i, x, rc in bad:
         assert L.nf_token_logprobs_fwd(*(ok[:i] + [x] + ok[i + 1:])) == rc, (i, x, _err())
-    ok = [FAKE, 16, 64, 100, 1024, 1, FAKE, st, FAKE, None, FAKE, 1, FAKE, 1, FAKE, bw, None]
-    bad = [(1, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (5, 2, NF_ERR_DTYPE), (0, None, NF_ERR_ARG),
-           (6, None, NF_ERR_ARG), (7, st - 1, NF_ERR_WORKSPACE), (11, 3, NF_ERR_DTYPE),
-           (13, -1, NF_ERR_DTYPE), (14, None, NF_ERR_WORKSPACE), (15, bw - 1, NF_ERR_WORKSPACE)]
+    ok = [FAKE, 16, 64, 100, 1024, 1, 1, FAKE, st, FAKE, None, FAKE, 1, FAKE, 1, FAKE, bw, None]
+    bad = [(1, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (6, 2, NF_ERR_DTYPE), (0, None, NF_ERR_ARG),
+           (7, None, NF_ERR_ARG), (8, st - 1, NF_ERR_WORKSPACE), (12, 3, NF_ERR_DTYPE),
+           (14, -1, NF_ERR_DTYPE), (15, None, NF_ERR_WORKSPACE), (16, bw - 1, NF_ERR_WORKSPACE)]
     for i, x, rc in bad:
         assert L.nf_token_logprobs_bwd(*(ok[:i] + [x] + ok[i + 1:])) == rc, (i, x, _err())
-    nothing = ok[:10] + [None, 1, None, 1] + ok[14:]
+    nothing = ok[:11] + [None, 1, None, 1] + ok[15:]
     assert L.nf_token_logprobs_bwd(*nothing) == NF_OK  # no gradient wanted: no launch

@@ -68,6 +68,12 @@ def logprobs64(h, w, t, g, gh, k=0, ignore=-100, chunk=2048):
         # and what is below 2^-126, fp32's and bf16's normal range, may become zero
         bracket = gs.abs() + ghs.abs() * (xs.abs() + ent.abs() + 1)
         edz = (p * ep * 2 + 2.0 ** -126) * bracket + r * dz.abs() + 2.0 ** -126
+        if w.dtype == torch.bfloat16 and m > 128:
+            # exp(z - strip maximum) may be kept in fp16: off by half a step, 2^-11 of itself,
+            # or 2^-25 among its subnormals, of at most the row's largest p; p (z - lse) by that
+            # times |z - lse| + 2
+            edz += 2 * (2.0 ** -11 * p + 2.0 ** -25 * p.amax(1, keepdim=True)) * (
+                bracket + ghs.abs())
         acc = (v + 2) * 2.0 ** -24 if f32 else (v / 16 + 16) * 2.0 ** -24
         out["tol_dh"].append(edz @ wd.abs() + acc * (dz.abs() @ wd.abs()))
         tol_dw += edz.T @ hs.abs() + (m + 2) * 2.0 ** -24 * (dz.abs().T @ hs.abs())

@@ -557,7 +557,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 // NR: records in a lane's registers (0: more than fit, read in every round).  `targets`: the
 // skinny pass, whose rows are not compacted: rows that do not count get their zeros here, and
-// the state is written for the backward.
+// the state is written for the backward (Hc null: none will come).
 template <typename TI, bool VK, int NR>
 __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     const TI *W, const TI *H, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     hrow = H + row * D;
     const int tc = row < crows ? target_column(targets, row, V, ignore_index) : -1;
     constexpr int VE = VK ? 16 / (int)sizeof(TI) : 1;
-    for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
+    for (int64_t c = (int64_t)l * VE; Hc && c < D; c += 64 * VE) {
       if constexpr (VK) {
         u32x4 x = {0u, 0u, 0u, 0u};
         if (tc >= 0) x = *reinterpret_cast<const u32x4 *>(hrow + c);
@@ -1022,8 +1022,8 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept)
 template <typename TI>
 int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan &P,
                   const Stat *stats, const Rec *recs, const float *tgt, int64_t j0, int64_t rows,
-                  const View<TI> &S, int64_t lo0, const int64_t *targets, int64_t ignore_index,
-                  const RowOut &out, hipStream_t s) {
+                  const View<TI> &S, TI *hc, int64_t lo0, const int64_t *targets,
+                  int64_t ignore_index, const RowOut &out, hipStream_t s) {
   const bool vk = D % (16 / (int64_t)sizeof(TI)) == 0 && aligned16(W) && aligned16(H);
   const int64_t waves = targets && lo0 > 0 ? lo0 : rows;
   const unsigned grid = (unsigned)((waves + kFinishThreads / 64 - 1) / (kFinishThreads / 64));
@@ -1031,7 +1031,7 @@ int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan 
 #define NF_LP_FINISH(VK, NR)                                                                   \
   lp_finish_kernel<TI, VK, NR><<<grid, kFinishThreads, 0, s>>>(                                \
       W, H, V, D, stats, P.nstat, recs, P.strips, tgt, j0, rows, S.n, S.rows, S.tcol, S.pos,   \
-      S.Hc, lo0, targets, ignore_index, S.lse, S.ent, S.lp, out)
+      hc, lo0, targets, ignore_index, S.lse, S.ent, S.lp, out)
   if (vk && nrec <= 64 * 16)
     NF_LP_FINISH(true, 16);
   else if (vk && nrec <= 64 * 32)
@@ -1074,8 +1074,8 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
       NF_LP_SKINNY(4, false);
 #undef NF_LP_SKINNY
     if ((e = check_launch("lp_skinny"))) return e;
-    return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, L.lo0, targets,
-                             ignore_index, out, s);
+    return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, keep ? S.Hc : nullptr,
+                             keep ? L.lo0 : 0, targets, ignore_index, out, s);
   }
   ce::ce_compact_kernel<<<1, ce::kCompactThreads, 0, s>>>(targets, M, V, ignore_index, S.rows,
                                                           S.tcol, S.pos, S.n, S.inv, nullptr);
@@ -1137,7 +1137,7 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
       NF_LP_LOGITS(false, false, false, false);
 #undef NF_LP_LOGITS
     if ((e = check_launch("lp_logits"))) return e;
-    if ((e = launch_finish<TI>(W, S.Hc, V, D, P, stats, recs, tgt, j0, rows, S, L.lo0, nullptr,
+    if ((e = launch_finish<TI>(W, S.Hc, V, D, P, stats, recs, tgt, j0, rows, S, S.Hc, L.lo0, nullptr,
                                ignore_index, out, s)))
       return e;
   }

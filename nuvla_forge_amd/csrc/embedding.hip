@@ -6,15 +6,17 @@
 // up like any other and gives no gradient.
 //
 // The gradient takes three launches:
-//   emb_sort:   block b owns the ids [b R, (b + 1) R).  It reads all M ids twice: first
-//               counting its own (per wavefront and id, in LDS) and the ids below its
-//               range, which gives every id's first position in the sorted order without
-//               a word from another block; then placing its tokens, in order.  It writes
-//               zeros to the rows of its ids that no token holds.
-//   emb_reduce: the sorted positions in spans of kSpan, one wavefront a span (and 64
-//               vectors of columns): a run of one id that lies inside the span is summed
-//               and written; a piece of a run that crosses a span's border goes to the
-//               workspace as an fp32 partial row.
+//   emb_sort:   block b of nb (a power of two) owns the ids that are b modulo nb, so that
+//               frequent ids next to each other fall to different blocks; the order of
+//               the sort is by block, then by id.  It reads all M ids, counting its own
+//               (per wavefront and id, in LDS) and those of the blocks before it, which
+//               gives every id's first position without a word from another block; then
+//               it places its tokens, in order.
+//   emb_reduce: the sorted positions in spans, one wavefront a span (and 64 vectors of
+//               columns): a run of one id that lies inside the span is summed and written;
+//               a piece of a run that crosses a span's border goes to the workspace as an
+//               fp32 partial row.  Among these blocks, others write zeros to the rows of
+//               ids that no token holds: the sums wait for memory, the zeros only write.
 //   emb_join:   the partial rows of each run that crosses borders, added in order.
 // So the work of a token that holds half the batch is spread like any other.
 #include <initializer_list>
@@ -90,9 +92,22 @@ __global__ __launch_bounds__(kFwdThreads) void emb_fwd_kernel(
 // gradient
 // ---------------------------------------------------------------------------
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kMaxRange = 512;  // ids per block
-constexpr int kSpan = 32;       // sorted positions per wavefront of emb_reduce
-constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
+constexpr int kMaxIds = 512;    // ids per block
+constexpr int kListed = 512;    // tokens a wavefront notes in LDS
+constexpr int kZeroIds = 64;    // ids a wavefront looks at for rows to clear
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+
+// The ids' places: block id % nb, and in it id / nb; R ids a block.
+struct Order {
+  int log_nb, R;
+  __device__ __forceinline__ int64_t place(int64_t id) const {
+    return (id & (((int64_t)1 << log_nb) - 1)) * R + (id >> log_nb);
+  }
+  __host__ __device__ int64_t places() const { return (int64_t)R << log_nb; }
+};
+struct Token {
+  int m, id;
+};
 
 __device__ __forceinline__ int wave_inclusive_sum(int v) {
   const int l = threadIdx.x & 63;
@@ -104,26 +119,30 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
   return v;
 }
 
-// first[v]: the sorted position of id v's first token (first[V]: the number of tokens
-// that count); perm, sid: the token and the id at each position.
-template <typename W, int VE>
+// first[place]: the sorted position of that id's first token (first[places]: the number of
+// tokens that count); sorted: the token and its id at each position.
+//
+// A block's time goes into reading the ids (M 65536: 0.5 MB a block from the L2s) and
+// into placing its tokens, where most of them belong to a few blocks.
 __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
-    const int64_t *__restrict__ ids, int64_t M, int64_t V, int64_t pad, int R,
-    int *__restrict__ first, int *__restrict__ perm, int *__restrict__ sid,
-    W *__restrict__ dtable, int64_t D) {
-  __shared__ int hist[kSortWaves][kMaxRange];
-  __shared__ int total[kMaxRange];
+    const int64_t *__restrict__ ids, int64_t M, int64_t V, int64_t pad, Order ord,
+    int *__restrict__ first, Token *__restrict__ sorted) {
+  __shared__ int hist[kSortWaves][kMaxIds];
+  __shared__ int list_m[kSortWaves][kListed];
+  __shared__ int list_key[kSortWaves][kListed];
   __shared__ int below_w[kSortWaves];
   __shared__ int scan_w[kSortWaves];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t lo = (int64_t)blockIdx.x * R;
-  const int64_t hi = lo + R < V ? lo + R : V;
+  const int blk = blockIdx.x, mask = (1 << ord.log_nb) - 1, R = ord.R;
+  const uint64_t lower = (1ull << l) - 1ull;
   for (int k = l; k < R; k += 64) hist[w][k] = 0;  // the wavefront's own row
   const int64_t seg = ((M + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int64_t m0 = (int64_t)w * seg, m1 = m0 + seg < M ? m0 + seg : M;
   __syncthreads();
-  int below = 0;
-  constexpr int kBatch = 4;
+  // 64 tokens from m on: the key of those that are the block's, else -1; and how many
+  // belong to blocks before it
+  int below = 0, noted = 0;
+  constexpr int kBatch = 8;
   for (int64_t b = m0; b < m1; b += 64 * kBatch) {
     int64_t id[kBatch];
 #pragma unroll
@@ -134,8 +153,20 @@ __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const bool counts = id[u] >= 0 && id[u] < V && id[u] != pad;
-      below += counts && id[u] < lo ? 1 : 0;
-      if (counts && id[u] >= lo && id[u] < hi) atomicAdd(&hist[w][id[u] - lo], 1);
+      const int owner = (int)id[u] & mask;
+      below += counts && owner < blk ? 1 : 0;
+      const bool in = counts && owner == blk;
+      const uint64_t ins = __ballot(in);
+      if (!ins) continue;
+      if (in) {
+        const int key = (int)(id[u] >> ord.log_nb), at = noted + __popcll(ins & lower);
+        atomicAdd(&hist[w][key], 1);
+        if (at < kListed) {
+          list_m[w][at] = (int)(b + u * 64 + l);
+          list_key[w][at] = key;
+        }
+      }
+      noted += __popcll(ins);
     }
   }
   below = wave_inclusive_sum(below);
@@ -150,7 +181,6 @@ __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
       hist[k][threadIdx.x] = mine;
       mine += h;
     }
-    total[threadIdx.x] = mine;
   }
   const int incl = wave_inclusive_sum(mine);
   if (l == 63) scan_w[w] = incl;
@@ -163,88 +193,129 @@ __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
   if ((int)threadIdx.x < R) {
 #pragma unroll
     for (int k = 0; k < kSortWaves; ++k) hist[k][threadIdx.x] += start;
-    if (lo + threadIdx.x < V) {
-      first[lo + threadIdx.x] = start;
-      if (lo + threadIdx.x == V - 1) first[V] = start + mine;
-    }
+    first[(int64_t)blk * R + threadIdx.x] = start;
+    if (blk == mask && (int)threadIdx.x == R - 1) first[ord.places()] = start + mine;
   }
   __syncthreads();
-  // rows without a token
-  const float zero[VE] = {};
-  for (int64_t v = lo + w; v < hi; v += kSortWaves)
-    if (total[v - lo] == 0)
-      for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) store_n<W, VE>(dtable + v * D + c, zero);
-  // the tokens of the range in order: a wavefront ranks 64 at a time (a loop over their
-  // different ids took 430 of the 448 us that 65536 tokens by Zipf's law cost here, V 128256)
+  // the block's tokens in order: a wavefront ranks 64 at a time, the lanes that share an id
+  // found by one ballot a bit (a loop over the different ids took 430 of the 448 us that
+  // 65536 tokens by Zipf's law cost here, V 128256)
   int bits = 0;
   while ((1 << bits) < R) ++bits;
-  const uint64_t lower = (1ull << l) - 1ull;
   volatile int *next = hist[w];
-  for (int64_t b = m0; b < m1; b += 64 * kBatch) {
-    int64_t ib[kBatch];
+  auto place = [&](bool in, int m, int key) {
+    uint64_t same = __ballot(in);
+    for (int k = 0; k < bits; ++k) {
+      const uint64_t set = __ballot((key >> k) & 1);
+      same &= (key >> k) & 1 ? set : ~set;
+    }
+    if (in) {
+      const int at = next[key];
+      sorted[at + __popcll(same & lower)] = Token{m, (key << ord.log_nb) | blk};
+      if ((same & lower) == 0) next[key] = at + __popcll(same);
+    }
+  };
+  if (noted <= kListed) {
+    for (int q = 0; q < noted; q += 64) {
+      const bool in = q + l < noted;
+      place(in, in ? list_m[w][q + l] : 0, in ? list_key[w][q + l] : 0);
+    }
+    return;
+  }
+  for (int64_t b = m0; b < m1; b += 64 * kBatch) {  // more than were noted: once more over the ids
+    int64_t id[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int64_t m = b + u * 64 + l;
-      ib[u] = m < m1 ? ids[m] : -1;
+      id[u] = m < m1 ? ids[m] : -1;
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-        const int64_t id = ib[u];
-      const bool in = id >= lo && id < hi && id != pad;
-      uint64_t same = __ballot(in);
-      if (!same) continue;
-      // the lanes with this lane's id, by one ballot a bit
-      const int key = in ? (int)(id - lo) : 0;
-      for (int k = 0; k < bits; ++k) {
-        const uint64_t set = __ballot((key >> k) & 1);
-        same &= (key >> k) & 1 ? set : ~set;
-      }
-      if (in) {
-        const int at = next[key], pos = at + __popcll(same & lower);
-        perm[pos] = (int)(b + u * 64 + l);
-        sid[pos] = (int)id;
-        if ((same & lower) == 0) next[key] = at + __popcll(same);
-      }
+      const bool in =
+          id[u] >= 0 && id[u] < V && id[u] != pad && ((int)id[u] & mask) == blk;
+      if (__ballot(in)) place(in, (int)(b + u * 64 + l), in ? (int)(id[u] >> ord.log_nb) : 0);
     }
   }
 }
 
-// O: dout's type, W: dtable's.  part[2 s] is the head of span s (the end, or all, of a
-// run begun before it), part[2 s + 1] its tail (the begin of a run that goes on).
+// VE elements as they lie in memory.
+template <typename T, int VE>
+struct Raw {
+  T v[VE];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (VE == 8) {
+      u32x4 a[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) a[i] = reinterpret_cast<const u32x4 *>(p)[i];
+      __builtin_memcpy(v, a, sizeof(v));
+    } else if constexpr (VE == 2) {
+      typedef T t2 __attribute__((ext_vector_type(2)));
+      const t2 a = *reinterpret_cast<const t2 *>(p);
+      v[0] = a[0];
+      v[1] = a[1];
+    } else {
+      v[0] = *p;
+    }
+  }
+};
+
+// O: dout's type, W: dtable's.  Blocks [0, nsum) of the interleaved order sum, a wavefront a
+// (span, column part), parts of a span next to each other so that a row of dout is read
+// whole at one time; the other blocks clear.  part[2 s] is the head of span s (the end, or
+// all, of a run begun before it), part[2 s + 1] its tail (the begin of a run that goes on).
 template <typename O, typename W, int VE>
 __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const O *__restrict__ dout, int64_t ldo, const int *__restrict__ first,
-    const int *__restrict__ perm, const int *__restrict__ sid, int64_t V, int64_t D, float scale,
-    W *__restrict__ dtable, float *__restrict__ part) {
-  const int n = first[V];
-  const int l = threadIdx.x & 63;
-  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t t0 = s * kSpan;
+    const Token *__restrict__ sorted, Order ord, int64_t V, int64_t D, float scale, int span,
+    int cols, int64_t nclear, W *__restrict__ dtable, float *__restrict__ part) {
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  // clearing blocks spread evenly among the others
+  const int64_t b = blockIdx.x, blocks = gridDim.x;
+  const int64_t before_b = b * nclear / blocks;
+  if ((b + 1) * nclear / blocks != before_b) {
+    const int64_t v0 = (before_b * 4 + w) * kZeroIds;
+    const int64_t v = v0 + l;
+    const int64_t at = ord.place(v < V ? v : 0);
+    uint64_t empty = __ballot(v < V && first[at + 1] == first[at]);
+    const float zero[VE] = {};
+    for (; empty; empty &= empty - 1) {
+      W *row = dtable + (v0 + __ffsll((unsigned long long)empty) - 1) * D;
+      for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) store_n<W, VE>(row + c, zero);
+    }
+    return;
+  }
+  const int n = first[ord.places()];
+  const int64_t u = (b - before_b) * 4 + w, s = u / cols;
+  const int64_t t0 = s * span;
   if (t0 >= n) return;
-  const int cnt = n - t0 < kSpan ? (int)(n - t0) : kSpan;
-  const int64_t c = ((int64_t)blockIdx.y * 64 + l) * VE;
+  const int cnt = n - t0 < span ? (int)(n - t0) : span;
+  const int64_t c = ((u - s * cols) * 64 + l) * VE;
   const bool cin = c < D;
-  const int tok = l < cnt ? perm[t0 + l] : 0;
-  const int id = l < cnt ? sid[t0 + l] : -1;
-  const int before = t0 > 0 ? sid[t0 - 1] : -1;
-  const int after = t0 + cnt < n ? sid[t0 + cnt] : -1;
+  const Token own = l < cnt ? sorted[t0 + l] : Token{0, -1};
+  const int tok = own.m, id = own.id;
+  const int before = t0 > 0 ? sorted[t0 - 1].id : -1;
+  const int after = t0 + cnt < n ? sorted[t0 + cnt].id : -1;
   float acc[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.f;
   bool begun_before = before == __builtin_amdgcn_readlane(id, 0);
   constexpr int kBatch = 8;
+  Raw<O, VE> cur[kBatch], nxt[kBatch];
+  auto fetch = [&](int j0, Raw<O, VE> (&r)[kBatch]) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (j0 + q < cnt && cin)
+        r[q].load(dout + (int64_t)__builtin_amdgcn_readlane(tok, j0 + q) * ldo + c);
+  };
+  fetch(0, cur);
   for (int j0 = 0; j0 < cnt; j0 += kBatch) {
-    float v[kBatch][VE];
+    fetch(j0 + kBatch, nxt);  // under way while this batch is added
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (j0 + u < cnt && cin)
-        load_n<O, VE>(dout + (int64_t)__builtin_amdgcn_readlane(tok, j0 + u) * ldo + c, v[u]);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int j = j0 + u;
+    for (int q = 0; q < kBatch; ++q) {
+      const int j = j0 + q;
       if (j >= cnt) break;
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += v[u][i];
+      for (int i = 0; i < VE; ++i) acc[i] += to_f32(cur[q].v[i]);
       const int here = __builtin_amdgcn_readlane(id, j);
       const bool last = j + 1 == cnt;
       const int then = last ? after : __builtin_amdgcn_readlane(id, j + 1 < 64 ? j + 1 : 63);
@@ -264,23 +335,27 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
         for (int i = 0; i < VE; ++i) acc[i] = 0.f;
       }
     }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) cur[q] = nxt[q];
   }
 }
 
 // Block (s, y): the run that begins in span s and goes on past it, if there is one: its
-// tail there and the heads of the spans after it.  Wavefront k adds the pieces k, k + 16,
-// k + 32, ... in that order, the first wavefront the 16 sums.
+// tail there and the heads of the spans after it.  Wavefront k adds the pieces k, k + 8,
+// k + 16, ... in that order, the first wavefront the 8 sums.
 template <typename W, int VE>
 __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
-    const int *__restrict__ first, const int *__restrict__ sid, int64_t V, int64_t D, float scale,
-    const float *__restrict__ part, W *__restrict__ dtable) {
+    const int *__restrict__ first, const Token *__restrict__ sorted, Order ord, int64_t D,
+    float scale, int span, const float *__restrict__ part, W *__restrict__ dtable) {
   __shared__ float sums[kJoinWaves][64 * VE];
-  const int n = first[V];
-  const int64_t s = blockIdx.x, end = (s + 1) * kSpan;  // a border between two spans
+  const int n = first[ord.places()];
+  const int64_t s = blockIdx.x, end = (s + 1) * span;  // a border between two spans
   if (end >= n) return;
-  const int id = sid[end - 1];
-  if (sid[end] != id || first[id] < s * kSpan) return;  // no run crosses, or it began before
-  const int64_t pieces = (first[id + 1] - 1) / kSpan - s + 1;
+  const int id = sorted[end - 1].id;
+  if (sorted[end].id != id) return;  // no run crosses
+  const int64_t at = ord.place(id);
+  if (first[at] < s * span) return;  // it began before
+  const int64_t pieces = (first[at + 1] - 1) / span - s + 1;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t c = ((int64_t)blockIdx.y * 64 + l) * VE;
   const bool cin = c < D;
@@ -288,7 +363,7 @@ __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.f;
   if (cin) {
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     for (int64_t p0 = w; p0 < pieces; p0 += kJoinWaves * kBatch) {
       float v[kBatch][VE];
 #pragma unroll
@@ -353,25 +428,27 @@ int run_fwd(const int64_t *ids, const W *table, int64_t ldt, float scale, int64_
 }
 
 struct BwdPlan {
-  int R;               // ids per block of emb_sort
-  int64_t blocks;      // of emb_sort
+  Order ord;  // 2^log_nb blocks of emb_sort
+  int span;   // sorted positions per wavefront of emb_reduce
   int64_t spans;
-  size_t first, perm, sid, part, total;
+  size_t first, sorted, part, total;
 };
 BwdPlan bwd_plan(int64_t M, int64_t D, int64_t V) {
   auto align = [](size_t x) { return (x + 255) & ~(size_t)255; };
   BwdPlan p;
-  const int64_t r = (V + 255) / 256;
-  p.R = (int)(r < 1 ? 1 : (r > kMaxRange ? kMaxRange : r));
-  p.blocks = (V + p.R - 1) / p.R;
-  p.spans = (M + kSpan - 1) / kSpan;
+  int log_nb = 8;  // a block a CU, more where an id's counter would not fit the LDS
+  while (((V - 1) >> log_nb) + 1 > kMaxIds) ++log_nb;
+  p.ord = Order{log_nb, (int)(((V - 1) >> log_nb) + 1)};
+  // spans of 32 positions where that leaves 8192 wavefronts (32 a CU) and more, else of 16
+  // or 8: fewer positions end sooner, but leave more partial rows
+  const int64_t cols = (D + 511) / 512;
+  p.span = M * cols >= 32 * 8192 ? 32 : M * cols >= 16 * 8192 ? 16 : 8;
+  p.spans = (M + p.span - 1) / p.span;
   size_t o = 0;
   p.first = o;
-  o = align(o + (size_t)(V + 1) * sizeof(int));
-  p.perm = o;
-  o = align(o + (size_t)M * sizeof(int));
-  p.sid = o;
-  o = align(o + (size_t)M * sizeof(int));
+  o = align(o + (size_t)(p.ord.places() + 1) * sizeof(int));
+  p.sorted = o;
+  o = align(o + (size_t)M * sizeof(Token));
   p.part = o;
   o = align(o + (size_t)p.spans * 2 * (size_t)D * sizeof(float));
   p.total = o;
@@ -383,20 +460,20 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
                int64_t V, W *dtable, char *ws, hipStream_t s) {
   const BwdPlan p = bwd_plan(M, D, V);
   int *first = reinterpret_cast<int *>(ws + p.first);
-  int *perm = reinterpret_cast<int *>(ws + p.perm);
-  int *sid = reinterpret_cast<int *>(ws + p.sid);
+  Token *sorted = reinterpret_cast<Token *>(ws + p.sorted);
   float *part = reinterpret_cast<float *>(ws + p.part);
   const unsigned cols = (unsigned)((D + 64 * VE - 1) / (64 * VE));
-  emb_sort_kernel<W, VE><<<(unsigned)p.blocks, kSortThreads, 0, s>>>(ids, M, V, pad, p.R, first,
-                                                                     perm, sid, dtable, D);
+  emb_sort_kernel<<<1u << p.ord.log_nb, kSortThreads, 0, s>>>(ids, M, V, pad, p.ord, first,
+                                                              sorted);
   if (int e = check_launch("emb_sort")) return e;
-  if (M == 0) return NF_OK;
-  emb_reduce_kernel<O, W, VE><<<dim3((unsigned)((p.spans + 3) / 4), cols), 256, 0, s>>>(
-      dout, D, first, perm, sid, V, D, scale, dtable, part);
+  const int64_t nsum = (p.spans * cols + 3) / 4, nclear = (V + 4 * kZeroIds - 1) / (4 * kZeroIds);
+  if (nsum + nclear > 0x7fffffffLL) return set_error(NF_ERR_ARG, "nf_embedding_bwd: too large");
+  emb_reduce_kernel<O, W, VE><<<(unsigned)(nsum + nclear), 256, 0, s>>>(
+      dout, D, first, sorted, p.ord, V, D, scale, p.span, (int)cols, nclear, dtable, part);
   if (int e = check_launch("emb_reduce")) return e;
   if (p.spans < 2) return NF_OK;  // no border to cross
   emb_join_kernel<W, VE><<<dim3((unsigned)(p.spans - 1), cols), kJoinThreads, 0, s>>>(
-      first, sid, V, D, scale, part, dtable);
+      first, sorted, p.ord, D, scale, p.span, part, dtable);
   return check_launch("emb_join");
 }
 

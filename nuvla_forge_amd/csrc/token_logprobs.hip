@@ -1233,20 +1233,29 @@ size_t bwd_bytes(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
 using namespace nf;
 using namespace nf::lp;
 using ce::ce_check_dtype;
-using ce::ce_check_shape;
-using ce::ce_sizes_ok;
 using ce::dtype_ok;
+
+namespace {
+// Columns are ints, padded to whole block tiles: V at most 2^30.
+constexpr int64_t kMaxCols = (int64_t)1 << 30;
+bool sizes_ok(int64_t M, int64_t D, int64_t V) { return ce::ce_sizes_ok(M, D, V) && V <= kMaxCols; }
+int check_shape(const char *fn, int64_t M, int64_t D, int64_t V) {
+  if (int e = ce::ce_check_shape(fn, M, D, V)) return e;
+  if (V > kMaxCols) return set_error(NF_ERR_ARG, "%s: V exceeds 2^30", fn);
+  return NF_OK;
+}
+}  // namespace
 
 extern "C" size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V,
                                                 int64_t chunk_rows, int keep, int dtype) {
-  if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype)) return 0;
+  if (!sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype)) return 0;
   return dtype == NF_DTYPE_BF16 ? state_layout<bf16>(M, D, V, chunk_rows, keep != 0).total
                                 : state_layout<float>(M, D, V, chunk_rows, keep != 0).total;
 }
 
 extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t V,
                                                   int64_t chunk_rows, int top_k, int dtype) {
-  if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype) || top_k < 0 ||
+  if (!sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype) || top_k < 0 ||
       top_k > kMaxTop || top_k > V)
     return 0;
   return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows, top_k, false).total
@@ -1255,7 +1264,7 @@ extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t 
 
 extern "C" size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,
                                                   int64_t chunk_rows, int dtype) {
-  if (!ce_sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype)) return 0;
+  if (!sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype)) return 0;
   return dtype == NF_DTYPE_BF16 ? bwd_bytes<bf16>(M, D, V, chunk_rows)
                                 : bwd_bytes<float>(M, D, V, chunk_rows);
 }
@@ -1268,7 +1277,7 @@ extern "C" int nf_token_logprobs_fwd(const void *hidden, const void *weight,
                                      size_t state_bytes, void *workspace,
                                      size_t workspace_bytes, void *stream) {
   const char *fn = "nf_token_logprobs_fwd";
-  if (int e = ce_check_shape(fn, M, D, V)) return e;
+  if (int e = check_shape(fn, M, D, V)) return e;
   if (chunk_rows <= 0) return set_error(NF_ERR_ARG, "%s: chunk_rows must be > 0", fn);
   if (top_k < 0 || top_k > kMaxTop || top_k > V)
     return set_error(NF_ERR_ARG, "%s: top_k=%d outside [0, min(%d, V)]", fn, top_k, kMaxTop);
@@ -1300,7 +1309,7 @@ extern "C" int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, i
                                      void *dweight, int dt_weight, void *workspace,
                                      size_t workspace_bytes, void *stream) {
   const char *fn = "nf_token_logprobs_bwd";
-  if (int e = ce_check_shape(fn, M, D, V)) return e;
+  if (int e = check_shape(fn, M, D, V)) return e;
   if (chunk_rows <= 0) return set_error(NF_ERR_ARG, "%s: chunk_rows must be > 0", fn);
   if (!weight || !state) return set_error(NF_ERR_ARG, "%s: null pointer", fn);
   if (int e = ce_check_dtype(fn, dtype)) return e;

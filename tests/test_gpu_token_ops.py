@@ -386,6 +386,65 @@ def test_logprobs_nan_stays_in_its_row(cuda):
             assert dh[2].isnan().all() and torch.isfinite(dh[rest]).all()
 
 
+@pytest.mark.parametrize("m", [6, 100, 290])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logprobs_rows_left_out_may_hold_anything(cuda, m, dtype):
+    """NaN and infinities in a row that is left out, and in its upstream gradients, reach nothing."""
+    note(f"logprobs ignored nan {m} {dtype}")
+    h, w, t, g, gh = _head(m, 64, 900, dtype, cuda, ignored=0.0)
+    t[2] = -100
+    h[2, ::3], h[2, 1] = float("nan"), float("inf")
+    g[2], gh[2] = float("nan"), float("inf")
+    ref = logprobs64(torch.where(torch.isfinite(h), h, 0.0), w, t, torch.where(t >= 0, g, 0.0),
+                     torch.where(t >= 0, gh, 0.0))
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, top_k=2)
+    assert out.logprobs[2] == 0 and out.entropy[2] == 0 and (out.top_ids[2] == -1).all()
+    for x, name in zip(torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh]),
+                       ("dh", "dw")):
+        assert ((x.double() - ref[name]).abs() <= ref["tol_" + name]).all(), name
+
+
+def test_logprobs_past_two_gib(cuda):
+    """What is kept for the backward takes more than 2 GiB: 32-bit offsets do not reach it."""
+    note("logprobs past 2 GiB")
+    m, d, v = 16700, 32, 65601
+    h, w, t, g, gh = _head(m, d, v, BF16, cuda, grid=True)
+    assert 2 * 16896 * 65664 > 1 << 31
+    for chunk_size in (m, 1024):
+        _logprobs_check(h, w, t, g, gh, 3, chunk_size=chunk_size)
+
+
+def test_token_ops_from_two_threads_on_two_streams(cuda):
+    note("token ops threads")
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(seed):
+        h, w, t, g, gh = _head(200, 64, 1500, BF16, cuda, seed=seed)
+        table = randn((1500, 64), gen(seed), F32, cuda)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        res = []
+        with torch.cuda.stream(stream):
+            for _ in range(6):
+                a, b, c = (x.detach().requires_grad_(True) for x in (h, w, table))
+                lp = chunked_token_logprobs(a, b, t, top_k=3)
+                emb = embedding_lookup(t.clamp(min=0), c, out_dtype=BF16)
+                out = fused_dropout(emb, 0.2, seed, residual=a)
+                res.append([*lp, out, *torch.autograd.grad(
+                    [lp.logprobs, lp.entropy, out], [a, b, c], [g, gh, torch.ones_like(out)])])
+            stream.synchronize()
+        return res
+
+    torch.cuda.synchronize()
+    alone = [work(s)[0] for s in (1, 2)]
+    with ThreadPoolExecutor(2) as ex:
+        both = list(ex.map(work, (1, 2)))
+    for want, got in zip(alone, both):
+        for one in got:
+            assert all(torch.equal(p, q) for p, q in zip(want, one, strict=True))
+
+
 @pytest.mark.parametrize("m", [5, 290])
 def test_logprobs_rows_left_out(cuda, m):
     note(f"logprobs ignored {m}")

@@ -244,6 +244,7 @@ def test_logprobs_c_abi_refusals():
     assert L.nf_token_logprobs_fwd_workspace(16, 64, 100, 1024, 33, 1) == 0
     assert L.nf_token_logprobs_fwd_workspace(16, 64, 4, 1024, 5, 1) == 0
     assert L.nf_token_logprobs_bwd_workspace(16, 64, 100, 0, 1) == 0
+    assert L.nf_token_logprobs_fwd_workspace(16, 1, (1 << 30) + 1, 1024, 0, 1) == 0
     ok = [FAKE, FAKE, FAKE, 16, 64, 100, -100, 1024, 5, 1, 1, FAKE, FAKE, FAKE, FAKE, FAKE, st,
           FAKE, fw, None]
     bad = [(3, 0, NF_ERR_ARG), (4, 0, NF_ERR_ARG), (5, 1 << 32, NF_ERR_ARG), (7, 0, NF_ERR_ARG),

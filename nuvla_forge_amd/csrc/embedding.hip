@@ -5,7 +5,7 @@
 // An id outside [0, V) gives a row of zeros and no gradient; the padding id is looked
 // up like any other and gives no gradient.
 //
-// The gradient takes three launches:
+// The gradient of up to 1024 tokens is one launch (emb_few); of more, three:
 //   emb_sort:   block b of nb (a power of two) owns the ids that are b modulo nb, so that
 //               frequent ids next to each other fall to different blocks; the order of
 //               the sort is by block, then by id.  It reads all M ids, counting its own
@@ -392,6 +392,118 @@ __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
   }
 }
 
+// Few tokens (at most kFewTokens): the whole gradient in one launch, without a workspace.
+// Block b owns the ids that are b modulo the grid, as in emb_sort, a thread looks at one
+// token, and the block sorts its own in LDS.  A wavefront takes an id: zeros to its row where
+// it has no token, else the sum; on an id of more than kLongRun tokens all wavefronts sum a
+// part each, and the parts are added in order.  V 32000, bf16, 1024 tokens, in a graph,
+// against the three launches: D 384 8.8 us against 16.3 (tokens by Zipf's law 10.3 against
+// 16.7, all the same 19.3 against 19.4), D 2048 23.8 against 27.7 (27.5 against 27.9; all the
+// same, where one block reads every row, 67 against 33).
+constexpr int kFewTokens = 1024, kLongRun = 32;
+constexpr int kFewThreads = 1024, kFewWaves = kFewThreads / 64;
+
+template <typename O, typename W, int VE>
+__global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
+    const O *__restrict__ dout, const int64_t *__restrict__ ids, int M, int64_t V, int64_t D,
+    int64_t pad, float scale, Order ord, W *__restrict__ dtable) {
+  static_assert(kFewTokens == kFewThreads && kMaxIds <= kFewThreads, "a token, an id a thread");
+  __shared__ int hist[kFewWaves][kMaxIds];
+  __shared__ int start[kMaxIds + 1], tok[kFewTokens];  // an id's first place; the tokens by id
+  __shared__ int scan_w[kFewWaves];
+  __shared__ int long_n, long_id[kFewTokens / kLongRun];
+  __shared__ float sums[kFewWaves][64 * VE];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, R = ord.R;
+  const int blk = blockIdx.x, mask = (1 << ord.log_nb) - 1;
+  const uint64_t lower = (1ull << l) - 1ull;
+  for (int k = l; k < R; k += 64) hist[w][k] = 0;  // the wavefront's own row
+  if (threadIdx.x == 0) long_n = 0;
+  const int64_t id = (int)threadIdx.x < M ? ids[threadIdx.x] : -1;
+  const bool in = id >= 0 && id < V && id != pad && ((int)id & mask) == blk;
+  const int key = in ? (int)(id >> ord.log_nb) : 0;
+  uint64_t same = __ballot(in);  // the lanes with this lane's id
+  if (same)
+    for (int k = 0; (1 << k) < R; ++k) {
+      const uint64_t set = __ballot((key >> k) & 1);
+      same &= (key >> k) & 1 ? set : ~set;
+    }
+  if (in && (same & lower) == 0) hist[w][key] = __popcll(same);
+  __syncthreads();
+  int mine = 0;
+  if ((int)threadIdx.x < R) {
+#pragma unroll
+    for (int k = 0; k < kFewWaves; ++k) {
+      const int h = hist[k][threadIdx.x];
+      hist[k][threadIdx.x] = mine;
+      mine += h;
+    }
+    if (mine > kLongRun) long_id[atomicAdd(&long_n, 1)] = threadIdx.x;  // in any order
+  }
+  const int incl = wave_inclusive_sum(mine);
+  if (l == 63) scan_w[w] = incl;
+  __syncthreads();
+  int at = incl - mine;
+  for (int k = 0; k < w; ++k) at += scan_w[k];
+  if ((int)threadIdx.x < R) start[threadIdx.x] = at;
+  if ((int)threadIdx.x == R - 1) start[R] = at + mine;
+  __syncthreads();
+  if (in) tok[start[key] + hist[w][key] + __popcll(same & lower)] = threadIdx.x;
+  __syncthreads();
+  // tokens [a, b) of the sorted order at the lane's columns from c on
+  auto sum = [&](int a, int b, int64_t c, float (&acc)[VE]) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+    constexpr int kBatch = 8;
+    for (int j0 = a; j0 < b; j0 += kBatch) {
+      Raw<O, VE> r[kBatch];
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q)
+        if (j0 + q < b) r[q].load(dout + (int64_t)tok[j0 + q] * D + c);
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q)
+        if (j0 + q < b)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[i] += to_f32(r[q].v[i]);
+    }
+  };
+  auto put = [&](int k, int64_t c, float (&acc)[VE]) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] *= scale;
+    store_n<W, VE>(dtable + (((int64_t)k << ord.log_nb) | blk) * D + c, acc);
+  };
+  for (int k = w; k < R; k += kFewWaves) {
+    const int a = start[k], b = start[k + 1];
+    if ((((int64_t)k << ord.log_nb) | blk) >= V || b - a > kLongRun) continue;
+    for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
+      float acc[VE];
+      sum(a, b, c, acc);  // zeros where a == b
+      put(k, c, acc);
+    }
+  }
+  for (int q = 0; q < long_n; ++q) {
+    const int k = long_id[q], a = start[k], b = start[k + 1];
+    const int per = (b - a + kFewWaves - 1) / kFewWaves;
+    const int pa = a + w * per < b ? a + w * per : b, pb = pa + per < b ? pa + per : b;
+    for (int64_t c0 = 0; c0 < D; c0 += 64 * VE) {
+      const int64_t c = c0 + (int64_t)l * VE;
+      float acc[VE];
+      if (c < D) {
+        sum(pa, pb, c, acc);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) sums[w][l * VE + i] = acc[i];
+      }
+      __syncthreads();
+      if (w == 0 && c < D) {
+        for (int p = 1; p < kFewWaves; ++p)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[i] += sums[p][l * VE + i];
+        put(k, c, acc);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -462,6 +574,11 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
   int *first = reinterpret_cast<int *>(ws + p.first);
   Token *sorted = reinterpret_cast<Token *>(ws + p.sorted);
   float *part = reinterpret_cast<float *>(ws + p.part);
+  if (M <= kFewTokens) {
+    emb_few_kernel<O, W, VE><<<1u << p.ord.log_nb, kFewThreads, 0, s>>>(
+        dout, ids, (int)M, V, D, pad, scale, p.ord, dtable);
+    return check_launch("emb_few");
+  }
   const unsigned cols = (unsigned)((D + 64 * VE - 1) / (64 * VE));
   emb_sort_kernel<<<1u << p.ord.log_nb, kSortThreads, 0, s>>>(ids, M, V, pad, p.ord, first,
                                                               sorted);
@@ -471,7 +588,6 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
   emb_reduce_kernel<O, W, VE><<<(unsigned)(nsum + nclear), 256, 0, s>>>(
       dout, D, first, sorted, p.ord, V, D, scale, p.span, (int)cols, nclear, dtable, part);
   if (int e = check_launch("emb_reduce")) return e;
-  if (p.spans < 2) return NF_OK;  // no border to cross
   emb_join_kernel<W, VE><<<dim3((unsigned)(p.spans - 1), cols), kJoinThreads, 0, s>>>(
       first, sorted, p.ord, D, scale, p.span, part, dtable);
   return check_launch("emb_join");

@@ -461,6 +461,7 @@ struct Chosen {
   int strip[kMaxTop];
   float cand_v[kMaxTop * 32];
   int cand_col[kMaxTop * 32];
+  float again[32];  // a strip's logits
 };
 
 // The strips whose first logits come first among those after (pv, pi), from entry `found` on;
@@ -666,7 +667,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     ch.cand_v[q] = val;
     ch.cand_col[q] = col;
   }
-  for (uint64_t todo = redo; todo; todo &= todo - 1, n += 32) {
+  for (uint64_t todo = redo; todo; todo &= todo - 1) {
     const int strip = ch.strip[__ffsll((unsigned long long)todo) - 1];
     Dot16<TI> acc[2];
     const TI *wrow[2];
@@ -696,36 +697,46 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
       const floatx4 z = acc[h].done();
       if ((l & 15) == 0)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = 16 * h + 4 * (l >> 4) + q;
-          ch.cand_v[n + c] = z[q];
-          ch.cand_col[n + c] = strips.column(strip, c);
-        }
+        for (int q = 0; q < 4; ++q) ch.again[16 * h + 4 * (l >> 4) + q] = z[q];
     }
+    wave_lds_fence();
+    // those that do not come after the last of the chosen strips' firsts (NaN: none)
+    const float x = ch.again[l & 31];
+    const int c = strips.column(strip, l & 31);
+    const uint64_t may = __ballot(l < 32 && c < V && x >= last);
+    if ((may >> l) & 1) {
+      const int q = n + __popcll(may & ((1ull << l) - 1ull));
+      ch.cand_v[q] = x;
+      ch.cand_col[q] = c;
+    }
+    n += __popcll(may);
+    wave_lds_fence();
   }
   wave_lds_fence();
-  // the K first of the candidates, in order
-  float pv = INFINITY;
-  int pi = -1;
-  for (int k = 0; k < K; ++k) {
-    float bv = -INFINITY;
-    int bi = 0x7fffffff, tag = -1;
-    for (int q = l; q < n; q += 64) {
-      const float x = ch.cand_v[q];
-      const int c = ch.cand_col[q];
-      if (c < V && before(pv, pi, x, c) && before(x, c, bv, bi)) {
-        bv = x;
-        bi = c;
-        tag = 0;
-      }
+  // a candidate's place is the number of those before it
+  for (int q0 = 0; q0 < n; q0 += 64) {
+    const int q = q0 + l;
+    const float x = q < n ? ch.cand_v[q] : 0.f;
+    const int c = q < n ? ch.cand_col[q] : 0;
+    int place = 0;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+      const float y = j0 + l < n ? ch.cand_v[j0 + l] : 0.f;
+      const int d = j0 + l < n ? ch.cand_col[j0 + l] : 0;
+      const int m0 = n - j0 < 64 ? n - j0 : 64;
+      for (int j = 0; j < m0; ++j)
+        place += before(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(y), j)),
+                        __builtin_amdgcn_readlane(d, j), x, c)
+                     ? 1
+                     : 0;
     }
-    wave_first(bv, bi, tag);
-    if (l == 0) {
-      out.top_lp[m * K + k] = tag < 0 ? __builtin_nanf("") : bv - lse;
-      out.top_id[m * K + k] = tag < 0 ? -1 : bi;
+    if (q < n && place < K) {
+      out.top_lp[m * K + place] = x - lse;
+      out.top_id[m * K + place] = c;
     }
-    pv = tag < 0 ? -INFINITY : bv;  // none left: nothing comes after the last place
-    pi = tag < 0 ? 0x7fffffff : bi;
+  }
+  if (l >= n && l < K) {  // none left that compares
+    out.top_lp[m * K + l] = __builtin_nanf("");
+    out.top_id[m * K + l] = -1;
   }
 }
 

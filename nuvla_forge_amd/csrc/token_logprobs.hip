@@ -9,12 +9,13 @@
 // Only valid rows (target != ignore_index, inside [0, V)) do any work: they are compacted
 // on the device and every later kernel sizes itself by the device count.
 //
-// Forward (nf_token_logprobs_fwd), more than 64 rows:
+// Forward (nf_token_logprobs_fwd), more than 256 rows:
 //   1. ce_compact: the valid rows in order.  lp_gather: Hc = hidden[rows], and zeros (id
 //      -1) into the outputs of the other rows.
 //   2. per chunk of rows: lp_logits, the logits tile by tile, of which statistics and
 //      records of strips are left; lp_finish: the row's values from those.
-// Up to 64 rows: lp_skinny, one pass over weight, and lp_finish.
+// Up to 256 rows: the same without the compaction, on smaller tiles (MidCfg); fp32 up to 32
+// rows: lp_skinny, one pass over weight, and lp_finish.
 // Backward (nf_token_logprobs_bwd), with g and h the upstream gradients of a row's logprob
 // and entropy H:
 //   dz = g (onehot - p) - h p (z - lse + H)
@@ -129,18 +130,27 @@ struct Strips {
   }
 };
 
+// A row's target as the call gives it: its column, or -1 where the row does not count.
+__device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, int64_t V,
+                                             int64_t ignore_index) {
+  const int64_t t = targets[m];
+  return t != ignore_index && t >= 0 && t < V ? (int)t : -1;
+}
+
 // One block tile: acc = W_tile Hc_tile^T (rows: vocabulary, columns: tokens), so a lane
 // holds 16 TM logits of each of its TN tokens and the strip's values are reductions in
 // registers.  stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
 // KEEP (16-bit inputs): exp(z - mx), mx the strip's maximum, is kept for the backward in
 // fp16, E [crows, ldp]: half a step of 2^-11 of each, and what is below 2^-24 of the strip's
 // largest is lost.  With bf16, 2^-8, its rounding would add to dz's own.  Blocks past the
-// tiles run the transposes of `tp`.
+// tiles run the transposes of `tp`.  `targets`: Hc is hidden as it lies, all crows rows of it
+// (a middling number of rows, which are not compacted).
 template <class C, bool BUF, bool SB, bool TOP, bool KEEP>
 __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
     const typename C::TI *W, const typename C::TI *Hc, int64_t V, int64_t D, int64_t j0,
-    int64_t crows, const int *n_ptr, const int *tcol, Stat *stats, int nstat, Rec *recs,
-    float *tgt, f16 *E, int64_t ldp, int vtiles, int ttiles, gemm::TpJobs tp) {
+    int64_t crows, const int *n_ptr, const int *tcol, const int64_t *targets,
+    int64_t ignore_index, Stat *stats, int nstat, Rec *recs, float *tgt, f16 *E, int64_t ldp,
+    int vtiles, int ttiles, gemm::TpJobs tp) {
   __shared__ __attribute__((aligned(16))) char smem[C::LDS_BYTES];
   if constexpr (KEEP) {
     static_assert(C::LDS_BYTES >= gemm::kTpRegionRows * gemm::kTpRegionPitch * 2,
@@ -154,7 +164,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
   int vt, tt;
   gemm::group_tile(gemm::xcd_order(blockIdx.x, vtiles * ttiles), vtiles, ttiles,
                    gemm::kTileGroup, vt, tt);
-  const int64_t cnt = chunk_count(n_ptr, j0, crows);
+  const int64_t cnt = targets ? crows : chunk_count(n_ptr, j0, crows);
   const int64_t v0 = (int64_t)vt * C::BM;
   const int64_t t0 = (int64_t)tt * C::BN;
   if (t0 >= cnt) return;
@@ -216,7 +226,8 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
     }
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (tok < cnt) {  // the target logit, from the one lane that holds it
-      const int64_t loc64 = (int64_t)tcol[j0 + tok] - vtile0;
+      const int col = targets ? target_column(targets, tok, V, ignore_index) : tcol[j0 + tok];
+      const int64_t loc64 = (int64_t)col - vtile0;
       const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
       if (loc >= 0 && ((loc >> 2) & 1) == half) {
         const int want = ((loc >> 5) << 4) | (((loc & 31) >> 3) << 2) | (loc & 3);
@@ -306,20 +317,18 @@ struct Dot16<float> {  // the products of mainloop_split, in its order
   }
 };
 
-// A row's target as the call gives it: its column, or -1 where the row does not count.
-__device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, int64_t V,
-                                             int64_t ignore_index) {
-  const int64_t t = targets[m];
-  return t != ignore_index && t >= 0 && t < V ? (int)t : -1;
-}
-
-// The logits of at most 16 NT rows, hidden used as it lies (no compaction).  What bounds it is
-// reading W once, so a wavefront streams 32 rows of W past the matrix pipe straight from
-// memory, kDepth steps of 32 k loaded ahead, and the hidden rows come from the caches.  A
-// wavefront's 32 columns are one strip: for token lane % 16 (+ 16 nt) a lane has columns
-// 16 h + 4 (lane / 16) + q, joined over the four lane groups.  V 32000, D 2048, 8 rows: see
-// nf_token_logprobs_fwd's dispatch.
-constexpr int kSkinnyThreads = 256, kSkinnyRows = 64;
+// The logits of at most 16 NT rows of fp32, hidden used as it lies (no compaction).  What bounds
+// it is reading W once: a wavefront streams 32 rows of W past the matrix pipe straight from
+// memory, two steps of 32 k at a time, and the hidden rows come from the caches.  A wavefront's
+// 32 columns are one strip: for token lane % 16 (+ 16 nt) a lane has columns 16 h +
+// 4 (lane / 16) + q, joined over the four lane groups.  V 32000, with lp_finish, in a graph,
+// against the tiles of MidCfg (which split 128 rows for every block): D 2048, 16 rows 66 us
+// against 116, 32 rows 80 against 116, 64 rows 117 against 116; D 384 24, 28 and 39 against
+// 31, 32 and 32.  In bf16 the tiles are the faster from 8 rows on (D 2048 26.6 us against 31.2, 64
+// rows 27.9 against 55).
+constexpr int kSkinnyThreads = 256;
+template <typename TI>
+constexpr int64_t kSkinnyRows = sizeof(TI) == 4 ? 32 : 0;
 
 template <typename TI, int NT, bool VK>
 __global__ __launch_bounds__(kSkinnyThreads) void lp_skinny_kernel(
@@ -343,7 +352,7 @@ __global__ __launch_bounds__(kSkinnyThreads) void lp_skinny_kernel(
     hrow[n] = m < M ? H + m * D : nullptr;
   }
   Dot16<TI> acc[2][NT];
-  constexpr int kDepth = sizeof(TI) == 2 ? (NT == 1 ? 8 : NT == 2 ? 4 : 2) : 2;
+  constexpr int kDepth = 2;
   for (int64_t k0 = 0; k0 < D; k0 += 32 * kDepth) {
     Frag a[kDepth][2], b[kDepth][NT];
 #pragma unroll
@@ -557,8 +566,8 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // NR: records in a lane's registers (0: more than fit, read in every round).  `targets`: the
-// skinny pass, whose rows are not compacted: rows that do not count get their zeros here, and
-// the state is written for the backward (Hc null: none will come).
+// pass whose rows are not compacted: rows that do not count get their zeros here, and the state
+// is written for the backward (Hc null: none will come).
 template <typename TI, bool VK, int NR>
 __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     const TI *W, const TI *H, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
@@ -999,28 +1008,66 @@ int transposes(const TI *W, const TI *Hc, int64_t Mb, int64_t D, int64_t V, cons
   return launch_transpose<U>(Hc, Mb, D, D, Hct, L.ldht, s);
 }
 
+// Tilings for up to 64, 128 and 256 rows, where the cross entropy's tile of 256 x 256 leaves
+// half of the CUs without a block and most of its token columns empty: 128 rows of W a block
+// (V 32000 is a block a CU) and more stages.  What bounds them is reading W once.  bf16, V
+// 32000, forward in a graph, against the main tiles after a compaction: D 2048, 8 rows 26.6 us
+// (the 131 MB of W partly in the Infinity Cache) against 59, 128 rows 36.9 against 60, 256 rows
+// 43 against 61; D 384 12.1 against 25, 15.3 against 25, 17.8 against 26.  fp32, 128 rows: D
+// 2048 130 us against 161, D 384 33 against 45.
+template <typename TI>
+struct MidCfg;
+template <>
+struct MidCfg<bf16> {
+  using T64 = DCfg<128, 64, 2, 2, 4, 64>;
+  using T128 = DCfg<128, 128, 2, 2, 4, 64>;
+  using T256 = DCfg<128, 256, 2, 4, 3, 64>;
+};
+template <>
+struct MidCfg<float> {
+  using T64 = SplitCfg<128, 128, 2, 2>;
+  using T128 = T64;
+  using T256 = SplitCfg<256, 128, 4, 2>;
+};
+
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
 struct FwdPlan {
-  bool skinny;  // at most kSkinnyRows rows: the skinny pass
+  int form;  // 0: the skinny pass; 64, 128, 256: MidCfg's tiles; -1: the main tiles, compacted
   int64_t crows;
-  int nstat, vtiles;
+  int nstat, vtiles, ttiles;
   Strips strips;
   size_t stats, recs, tgt, total;
 };
+template <class C>
+void tile_plan(FwdPlan &p, int64_t V) {
+  static_assert(C::WTM == 128 || C::WTM == 64, "strips of a wavefront's tile");
+  p.vtiles = (int)((V + C::BM - 1) / C::BM);
+  p.ttiles = (int)((p.crows + C::BN - 1) / C::BN);
+  p.nstat = p.vtiles * C::WM;
+  p.strips = Strips{C::WTM == 128 ? 2 : 1};
+}
 template <typename TI>
 FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept) {
-  using C = MainCfg<TI>;
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
-  p.skinny = M <= kSkinnyRows;
-  p.crows = p.skinny ? M
+  p.form = M <= kSkinnyRows<TI> ? 0 : kept || M > 256 ? -1 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  p.crows = p.form >= 0 ? M
             : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
                                              : mcap;
-  p.vtiles = (int)((V + C::BM - 1) / C::BM);
-  p.nstat = p.skinny ? (int)((V + 31) / 32) : p.vtiles * C::WM;
-  p.strips = Strips{p.skinny ? 0 : C::WTM == 128 ? 2 : 1};
-  static_assert(C::WTM == 128 || C::WTM == 64, "strips of a wavefront's tile");
+  using F = MidCfg<TI>;
+  if (p.form == 64)
+    tile_plan<typename F::T64>(p, V);
+  else if (p.form == 128)
+    tile_plan<typename F::T128>(p, V);
+  else if (p.form == 256)
+    tile_plan<typename F::T256>(p, V);
+  else
+    tile_plan<MainCfg<TI>>(p, V);
+  if (p.form == 0) {
+    p.nstat = (int)((V + 31) / 32);
+    p.strips = Strips{0};
+  }
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
   p.stats = take(kept ? 0 : (size_t)p.crows * p.nstat * sizeof(Stat));
@@ -1068,23 +1115,55 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
   float *tgt = reinterpret_cast<float *>(ws + P.tgt);
   const int64_t VE = 16 / (int64_t)sizeof(TI);
   int e;
-  if (P.skinny) {
-    const bool vk = D % VE == 0 && aligned16(H) && aligned16(W);
-    const unsigned grid = (unsigned)((V + 127) / 128);
+  if constexpr (kSkinnyRows<TI> > 0) {
+    if (P.form == 0) {
+      const bool vk = D % VE == 0 && aligned16(H) && aligned16(W);
+      const unsigned grid = (unsigned)((V + 127) / 128);
 #define NF_LP_SKINNY(NT, VK)                                                                   \
   lp_skinny_kernel<TI, NT, VK><<<grid, kSkinnyThreads, 0, s>>>(W, H, targets, M, V, D,         \
                                                                ignore_index, stats, P.nstat,   \
                                                                recs, tgt)
-    if (vk && M <= 16)
-      NF_LP_SKINNY(1, true);
-    else if (vk && M <= 32)
-      NF_LP_SKINNY(2, true);
-    else if (vk)
-      NF_LP_SKINNY(4, true);
-    else
-      NF_LP_SKINNY(4, false);
+      if (vk && M <= 16)
+        NF_LP_SKINNY(1, true);
+      else if (vk)
+        NF_LP_SKINNY(2, true);
+      else
+        NF_LP_SKINNY(2, false);
 #undef NF_LP_SKINNY
-    if ((e = check_launch("lp_skinny"))) return e;
+      if ((e = check_launch("lp_skinny"))) return e;
+      return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, keep ? S.Hc : nullptr,
+                               keep ? L.lo0 : 0, targets, ignore_index, out, s);
+    }
+  }
+  if (P.form > 0) {
+    const bool vk = buf_ok<TI>(H, D, M, D) && buf_ok<TI>(W, D, V, D);
+    const unsigned grid = (unsigned)(P.vtiles * P.ttiles);
+    const gemm::TpJobs none{};
+#define NF_LP_MID(T, BUF, TOP)                                                                 \
+  lp_logits_kernel<typename MidCfg<TI>::T, BUF, false, TOP, false>                             \
+      <<<grid, MidCfg<TI>::T::NT, 0, s>>>(W, H, V, D, 0, M, nullptr, nullptr, targets,         \
+                                          ignore_index, stats, P.nstat, recs, tgt, nullptr, 0, \
+                                          P.vtiles, P.ttiles, none)
+#define NF_LP_MID_T(T)                 \
+  do {                                 \
+    if (vk && recs)                    \
+      NF_LP_MID(T, true, true);        \
+    else if (vk)                       \
+      NF_LP_MID(T, true, false);       \
+    else if (recs)                     \
+      NF_LP_MID(T, false, true);       \
+    else                               \
+      NF_LP_MID(T, false, false);      \
+  } while (0)
+    if (P.form == 64)
+      NF_LP_MID_T(T64);
+    else if (P.form == 128)
+      NF_LP_MID_T(T128);
+    else
+      NF_LP_MID_T(T256);
+#undef NF_LP_MID_T
+#undef NF_LP_MID
+    if ((e = check_launch("lp_logits"))) return e;
     return launch_finish<TI>(W, H, V, D, P, stats, recs, tgt, 0, M, S, keep ? S.Hc : nullptr,
                              keep ? L.lo0 : 0, targets, ignore_index, out, s);
   }
@@ -1118,8 +1197,8 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
     // kept: the chunk is every row, and E's extent that of its buffer
 #define NF_LP_LOGITS(BUF, SB, TOP, KEEP)                                                      \
   lp_logits_kernel<C, BUF, SB, TOP, KEEP><<<grid, C::NT, 0, s>>>(                             \
-      W, S.Hc, V, D, j0, P.crows, S.n, S.tcol, stats, P.nstat, recs, tgt, S.E, ldp, P.vtiles, \
-      ttiles, tp)
+      W, S.Hc, V, D, j0, P.crows, S.n, S.tcol, nullptr, 0, stats, P.nstat, recs, tgt, S.E,    \
+      ldp, P.vtiles, ttiles, tp)
     bool launched = false;
     if constexpr (sizeof(TI) == 2) {
       launched = L.kept;

@@ -113,7 +113,8 @@ struct GemmJob {
   int64_t dyn_base;  // the extent is *dyn - dyn_base, clamped to [0, M or K]
   int dyn_rows;      // 1: the dynamic extent is M; 0: it is K
   // bt: B is given N-major, B[k, n] at B[k * ldb + n] (columns up to ldb may
-  // be read; 16-bit inputs, DCfg only).  ct: C is stored
+  // be read; 16-bit inputs, DCfg only; with a K that is no multiple of 8, A's rows hold zeros up
+  // to one).  ct: C is stored
   // transposed, element (m, n) at C[n * ldc + m] (no K split); Cin keeps
   // [M, ldcin].
   int bt, ct;
@@ -623,8 +624,12 @@ GemmJob<typename C::TI> make_job(const typename C::TI *A, int64_t lda, const typ
 template <typename TI>
 bool job_buf_ok(const GemmJob<TI> &j) {
   if (j.tiles == 0) return true;
-  if (j.bt)  // B's K rows of ldb elements, read as whole 16-byte vectors
-    return buf_ok<TI>(j.A, j.lda, j.M, j.K) && buf_ok<TI>(j.B, j.ldb, j.K, j.ldb);
+  if (j.bt) {  // B's K rows of ldb elements, read as whole 16-byte vectors
+    // A's too: its rows hold zeros from K up to a whole vector
+    const int64_t ka = (j.K + 7) / 8 * 8;
+    return (ka == j.K || ka <= j.lda) && buf_ok<TI>(j.A, j.lda, j.M, ka) &&
+           buf_ok<TI>(j.B, j.ldb, j.K, j.ldb);
+  }
   return buf_ok<TI>(j.A, j.lda, j.M, j.K) && buf_ok<TI>(j.B, j.ldb, j.N, j.K);
 }
 // every buffer the epilogue addresses through a 32-bit offset is under 2 GiB

@@ -155,14 +155,16 @@ struct EStore {
           // the chunk's rows, up to the K padding of the dW product)
           const int64_t c = crow0 + o;
           if constexpr (ES == 2) {
+            // c and ldp are multiples of 4: the four entries are one 8-byte vector
+            u32x2 pk = {0u, 0u};
+            if (tok < cnt) __builtin_memcpy(&pk, ev, 8);
+            eout.st64((tok * ldp + c) * ES, tok < cnt8 && c < ldp, pk);
+            if (both)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const TI e = tok < cnt ? ev[q] : static_cast<TI>(0.f);
-              uint16_t bits;
-              __builtin_memcpy(&bits, &e, 2);
-              eout.st16((tok * ldp + c + q) * ES, tok < cnt && c + q < ldp, bits);
-              etout.st16(((c + q) * ldet + tok) * ES, c + q < V && tok < cnt8, bits);
-            }
+              for (int q = 0; q < 4; ++q) {
+                const uint16_t bits = (uint16_t)(pk[q >> 1] >> (16 * (q & 1)));
+                etout.st16(((c + q) * ldet + tok) * ES, c + q < V && tok < cnt8, bits);
+              }
           } else {
             // c and ldp are multiples of 4: the four entries are one vector
             u32x4 pk;
@@ -529,10 +531,12 @@ struct StateView {
 // caller (the backward's scatter adds them).  want_w, want_h: the products that
 // are formed (a gradient that nobody asked for costs nothing).
 // C, CT: the tilings of the products with a K-contiguous and an N-major B.
+// Wn: weight as it lies, [V, D], for the dH product in the place of its transpose (single).
 template <typename TI, class C, class CT>
 int launch_grads_tiled(const Plan &L, const StateView<TI> &S, int64_t c, int64_t D, int64_t V,
                  const float *dw_in, void *dw_out, int dt_w, const float *g, float *part,
-                 hipStream_t s, bool final_dw, bool reduce_dh, bool want_w, bool want_h) {
+                 hipStream_t s, bool final_dw, bool reduce_dh, bool want_w, bool want_h,
+                 const TI *Wn) {
   const int64_t j0 = c * L.crows;
   // single: dW^T (+)= Hct_c P_c, [D, V], with P read N-major; the fp32
   // accumulator holds dW^T [D, ldp] and the final product stores dW [V, D]
@@ -549,8 +553,11 @@ int launch_grads_tiled(const Plan &L, const StateView<TI> &S, int64_t c, int64_t
   jw.dyn = S.n;
   jw.dyn_base = j0;
   jw.dyn_rows = 0;  // K: the chunk's rows
-  auto jh = make_job<C>(S.P, L.ldp, S.Wt, L.ldwt, nullptr, S.dHc + j0 * D, NF_DTYPE_F32,
-                        nullptr, D, L.crows, D, L.ldp);
+  auto jh = Wn ? make_job<CT>(S.P, L.ldp, Wn, D, nullptr, S.dHc + j0 * D, NF_DTYPE_F32, nullptr,
+                              D, L.crows, D, V)
+               : make_job<C>(S.P, L.ldp, S.Wt, L.ldwt, nullptr, S.dHc + j0 * D, NF_DTYPE_F32,
+                             nullptr, D, L.crows, D, L.ldp);
+  if (Wn) jh.bt = 1;
   jh.dyn = S.n;
   jh.dyn_base = j0;
   jh.dyn_rows = 1;  // M: the chunk's rows
@@ -572,15 +579,16 @@ template <typename TI>
 int launch_grads(const Plan &L, const StateView<TI> &S, int64_t c, int64_t D, int64_t V,
                  const float *dw_in, void *dw_out, int dt_w, const float *g, float *part,
                  hipStream_t s, bool final_dw, bool reduce_dh = true, bool want_w = true,
-                 bool want_h = true) {
+                 bool want_h = true, const TI *Wn = nullptr) {
   using C = MainCfg<TI>;
   if constexpr (sizeof(TI) == 2) {
     if (L.d192)
       return launch_grads_tiled<TI, Cols192Cfg, Rows192Cfg>(L, S, c, D, V, dw_in, dw_out, dt_w, g,
-                                                            part, s, final_dw, reduce_dh, want_w, want_h);
+                                                            part, s, final_dw, reduce_dh, want_w,
+                                                            want_h, Wn);
   }
   return launch_grads_tiled<TI, C, C>(L, S, c, D, V, dw_in, dw_out, dt_w, g, part, s, final_dw,
-                                      reduce_dh, want_w, want_h);
+                                      reduce_dh, want_w, want_h, Wn);
 }
 
 // Sizes whose buffers could exist: M, V, D within int32 and each operand

@@ -909,6 +909,15 @@ __global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+// Whether the dH product of M rows reads weight as it lies (its K loop over an N-major operand
+// is the slower one, 1.9 against 1.65 us a stage, and there are M / 256 rows of tiles) and not
+// a transpose made for it (which moves V D twice).  bf16, V 32000, forward and backward: D 2048,
+// 5 rows 157 us against 220, 300 rows 232 against 282, 512 rows 276 against 328, 768 rows 413
+// against 414; D 384 62 against 73, 88 against 94, 112 against 107, 131 against 136.
+inline bool weight_as_is(int64_t M, int64_t D, int64_t V) {
+  return M <= 256 + D / 4 && D % 8 == 0 && sb_ok(V * D * (int64_t)sizeof(bf16));
+}
+
 template <typename TI>
 ce::Plan grad_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
   const int64_t lo0 = few_rows<TI>(M);
@@ -918,10 +927,13 @@ ce::Plan grad_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
 // What the forward keeps for the backward: the rows, and, with `keep`, where one chunk takes
 // every row (by chunk_rows' bound on memory), exp(z - mx) of every logit with the strips'
 // statistics and the transposes of weight and of the rows that the products read: the
-// backward then forms dz in one pass over it instead of forming the logits again (M 4096,
-// D 2048, V 32000: see nf_token_logprobs_bwd).
+// backward then forms dz in one pass over it instead of forming the logits again.  M 4096,
+// D 2048, V 32000, 10% left out: forward and backward 1513 us, against 1828 with the logits
+// formed twice (the kernel lp_from_kept takes 96 us, 5.5 TB/s, in the place of 528 of lp_dz;
+// keeping costs lp_logits 60).  Up to 256 rows forming them again on MidCfg's tiles is the
+// faster: D 2048, 200 rows 207 us against 229.
 struct State {
-  bool kept;
+  bool kept, as_is;  // as_is: no transpose of weight among it
   int nstat;
   int64_t lo0;
   size_t scal, rows, tcol, pos, lse, ent, lp, hc, e, stats, wt, hct, total;
@@ -941,14 +953,15 @@ State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool kee
   s.ent = take((size_t)M * sizeof(float));
   s.lp = take((size_t)M * sizeof(float));
   s.hc = take((size_t)(s.lo0 > 0 ? 2 * s.lo0 : M) * D * sizeof(TI));
-  if (sizeof(TI) == 2 && keep && M > kFewRows && V <= kKeptCols) {
+  if (sizeof(TI) == 2 && keep && M > 256 && V <= kKeptCols) {
     const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
     if (L.nch == 1) {
       s.kept = true;
       s.nstat = (int)((V + C::BM - 1) / C::BM) * C::WM;
       s.e = take((size_t)L.crows * L.ldp * sizeof(f16));
       s.stats = take((size_t)L.crows * s.nstat * sizeof(Stat));
-      s.wt = take((size_t)D * L.ldwt * sizeof(TI));
+      s.as_is = weight_as_is(M, D, V);
+      s.wt = take(s.as_is ? 0 : (size_t)D * L.ldwt * sizeof(TI));
       s.hct = take((size_t)D * L.ldht * sizeof(TI));
     }
   }
@@ -985,7 +998,7 @@ struct View {
 // elements, else by launches of their own.
 template <typename TI>
 int transposes(const TI *W, const TI *Hc, int64_t Mb, int64_t D, int64_t V, const ce::Plan &L,
-               TI *Wt, TI *Hct, gemm::TpJobs &tp, hipStream_t s) {
+               TI *Wt, TI *Hct, gemm::TpJobs &tp, hipStream_t s) {  // Wt null: Hc^T alone
   using U = typename std::conditional<sizeof(TI) == 2, uint16_t, uint32_t>::type;
   tp = gemm::TpJobs{};
   if (sizeof(TI) == 2 && D % 8 == 0 && aligned16(W)) {
@@ -1000,11 +1013,12 @@ int transposes(const TI *W, const TI *Hc, int64_t Mb, int64_t D, int64_t V, cons
       tp.cb[j] = (int)((D + gemm::kTpRegionCols - 1) / gemm::kTpRegionCols);
       tp.n += tp.rb[j] * tp.cb[j];
     };
-    add(0, W, V, Wt, L.ldwt);
-    add(1, Hc, Mb, Hct, L.ldht);
+    add(0, Hc, Mb, Hct, L.ldht);
+    if (Wt) add(1, W, V, Wt, L.ldwt);
     return NF_OK;
   }
-  if (int e = launch_transpose<U>(W, V, D, D, Wt, L.ldwt, s)) return e;
+  if (Wt)
+    if (int e = launch_transpose<U>(W, V, D, D, Wt, L.ldwt, s)) return e;
   return launch_transpose<U>(Hc, Mb, D, D, Hct, L.ldht, s);
 }
 
@@ -1030,10 +1044,21 @@ struct MidCfg<float> {
   using T256 = SplitCfg<256, 128, 4, 2>;
 };
 
+// The tiling for `rows` rows: 64, 128, 256, or -1: the main tiles, which are also the better
+// ones where V alone makes 256 of them (V 128256, D 1024, 128 rows: 180 us against 188; fp32
+// lp_dz of 47 rows, V 85667, D 1432: 50 us more on the smaller tiles).  bf16 of up to 64 rows
+// gains from its 64 columns at every V.
+template <typename TI>
+int mid_form(int64_t rows, int64_t V) {
+  if (rows <= 64 && (sizeof(TI) == 2 || V <= 65536)) return 64;
+  if (rows > 256 || V > 65536) return -1;
+  return rows <= 128 ? 128 : 256;
+}
+
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
 struct FwdPlan {
-  int form;  // 0: the skinny pass; 64, 128, 256: MidCfg's tiles; -1: the main tiles, compacted
+  int form;  // 0: the skinny pass; 64, 128, 256: MidCfg's tiles; -1: the main ones, compacted
   int64_t crows;
   int nstat, vtiles, ttiles;
   Strips strips;
@@ -1051,7 +1076,7 @@ template <typename TI>
 FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept) {
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
-  p.form = M <= kSkinnyRows<TI> ? 0 : kept || M > 256 ? -1 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  p.form = M <= kSkinnyRows<TI> ? 0 : mid_form<TI>(M, V);
   p.crows = p.form >= 0 ? M
             : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
                                              : mcap;
@@ -1188,7 +1213,8 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
     const ce::Plan G = grad_plan<TI>(M, D, V, chunk_rows);
     ldp = G.ldp;
     sb = sb_ok(G.crows * ldp * (int64_t)sizeof(f16));
-    if ((e = transposes<TI>(W, S.Hc, M, D, V, G, S.Wt, S.Hct, tp, s))) return e;
+    if ((e = transposes<TI>(W, S.Hc, M, D, V, G, L.as_is ? nullptr : S.Wt, S.Hct, tp, s)))
+      return e;
   }
   for (int64_t j0 = 0; j0 < M; j0 += P.crows) {
     const int64_t rows = M - j0 < P.crows ? M - j0 : P.crows;
@@ -1252,11 +1278,15 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
   gemm::TpJobs tp{};
   const gemm::TpJobs none{};
   int e;
+  const TI *Wn = nullptr;
   if (KL.kept) {
     S.Wt = K.Wt;
     S.Hct = K.Hct;
-  } else if ((e = transposes<TI>(W, K.Hc, Mb, D, V, L, S.Wt, S.Hct, tp, s))) {
-    return e;
+    Wn = KL.as_is ? W : nullptr;
+  } else {
+    Wn = sizeof(TI) == 2 && weight_as_is(Mb, D, V) ? W : nullptr;
+    if ((e = transposes<TI>(W, K.Hc, Mb, D, V, L, Wn || !dH ? nullptr : S.Wt, S.Hct, tp, s)))
+      return e;
   }
   const bool vk = buf_ok<TI>(K.Hc, D, Mb, D) && buf_ok<TI>(W, D, V, D);
   const bool sb = sb_ok(L.crows * L.ldp * (int64_t)sizeof(TI)) &&
@@ -1264,11 +1294,19 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
   for (int64_t c = 0; c < L.nch; ++c) {
     const int64_t j0 = c * L.crows;
     const gemm::TpJobs &tj = c == 0 ? tp : none;
-    const unsigned grid = (unsigned)(L.vtiles * L.ttiles) + (unsigned)tj.n;
-#define NF_LP_DZ(BUF, SB)                                                                      \
-  lp_dz_kernel<C, BUF, SB><<<grid, C::NT, 0, s>>>(W, K.Hc, V, D, j0, L.crows, in, lo0, two,    \
-                                                  S.cfac, S.P, L.ldp, PT, L.crows, L.vtiles,   \
-                                                  L.ttiles, tj)
+#define NF_LP_DZ(CFG, BUF, SB)                                                                 \
+  do {                                                                                         \
+    const int vt = (int)((V + CFG::BM - 1) / CFG::BM), tt = (int)((cap + CFG::BN - 1) / CFG::BN); \
+    lp_dz_kernel<CFG, BUF, SB><<<(unsigned)(vt * tt + tj.n), CFG::NT, 0, s>>>(                 \
+        W, K.Hc, V, D, j0, L.crows, in, lo0, two, S.cfac, S.P, L.ldp, PT, L.crows, vt, tt, tj); \
+  } while (0)
+    // rows of the chunk, padding included (the products read up to 7 rows past them)
+    const int64_t cap = Mb - j0 < L.crows ? round_up(Mb - j0, 8) : L.crows;
+    const int form = mid_form<TI>(Mb, V);
+    using F = MidCfg<TI>;
+    using T64 = typename F::T64;
+    using T128 = typename F::T128;
+    using T256 = typename F::T256;
     bool formed = false;
     if constexpr (sizeof(TI) == 2) {
       formed = KL.kept;
@@ -1281,19 +1319,25 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
     }
     if (formed)
       ;
+    else if (vk && sb && form == 64)
+      NF_LP_DZ(T64, true, true);
+    else if (vk && sb && form == 128)
+      NF_LP_DZ(T128, true, true);
+    else if (vk && sb && form == 256)
+      NF_LP_DZ(T256, true, true);
     else if (vk && sb)
-      NF_LP_DZ(true, true);
+      NF_LP_DZ(C, true, true);
     else if (vk)
-      NF_LP_DZ(true, false);
+      NF_LP_DZ(C, true, false);
     else
-      NF_LP_DZ(false, false);
+      NF_LP_DZ(C, false, false);
 #undef NF_LP_DZ
     if ((e = check_launch(formed ? "lp_from_kept" : "lp_dz"))) return e;
     const bool last = c + 1 == L.nch;
     if ((e = ce::launch_grads<TI>(L, S, c, D, V, c > 0 ? S.dWacc : nullptr,
                                   last ? dW : S.dWacc, last ? dt_w : NF_DTYPE_F32, nullptr, part,
                                   s, /*final_dw=*/last, /*reduce_dh=*/!last, dW != nullptr,
-                                  dH != nullptr)))
+                                  dH != nullptr, Wn)))
       return e;
   }
   if (!dH) return NF_OK;

@@ -8,8 +8,8 @@
 // steps of 2^-16 and a kept element is scaled by 65536 / (65536 - threshold), which
 // keeps the mean exact.  32 bits an element would cost twice the generator.
 //
-// A chunk of 8 elements is a thread's 16-byte vector (bf16, fp16) or two (fp32), fp32
-// arithmetic, one rounding at the store.  A dropped element gives the residual exactly,
+// A chunk of 8 elements is a thread's 16-byte vector (bf16, fp16) or two (fp32), at any
+// alignment, fp32 arithmetic, one rounding at the store.  A dropped element gives the residual exactly,
 // whatever x holds there (infinities and NaN too).
 #include "nf_device.h"
 
@@ -41,7 +41,7 @@ __device__ __forceinline__ void philox8(uint64_t seed, uint64_t b, uint64_t offs
 }
 
 // I: x's type; O: the residual's and out's.
-template <typename I, typename O, bool RES, bool VEC>
+template <typename I, typename O, bool RES>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(
     const I *__restrict__ x, const O *__restrict__ res, O *__restrict__ out, int64_t n,
     uint32_t threshold, float scale, const int64_t *__restrict__ seed_ptr, int64_t seed,
@@ -50,44 +50,37 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(
   if (c * 8 >= n) return;
   const int64_t rem = n - c * 8;
   const int valid = rem >= 8 ? 8 : (int)rem;
-  float xv[8], rv[8];
-  load8<I, VEC>(x + c * 8, valid, xv);
-  if constexpr (RES) load8<O, VEC>(res + c * 8, valid, rv);
+  Any8<I> xv;
+  Any8<O> rv;
+  xv.load(x + c * 8, valid);
+  if constexpr (RES) rv.load(res + c * 8, valid);
   uint32_t word[4];
   philox8((uint64_t)(seed_ptr ? *seed_ptr : seed), (uint64_t)c, (uint64_t)offset, word);
+  float out8[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint32_t part = (word[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-    const float y = part >= threshold ? xv[j] * scale : 0.f;
-    xv[j] = RES ? y + rv[j] : y;
+    const float y = part >= threshold ? to_f32(xv.v[j]) * scale : 0.f;
+    out8[j] = RES ? y + to_f32(rv.v[j]) : y;
   }
-  store8<O, VEC>(out + c * 8, valid, xv);
+  rv.set(out8);
+  rv.store(out + c * 8, valid);
 }
 
 template <typename I, typename O>
 int launch(const void *x, const void *res, void *out, int64_t n, uint32_t threshold,
            const int64_t *seed_ptr, int64_t seed, int64_t offset, hipStream_t s) {
   const float scale = threshold < 65536u ? 65536.f / (float)(65536u - threshold) : 0.f;
-  const bool vec = aligned16(x) && aligned16(out) && (!res || aligned16(res));
   const unsigned grid = (unsigned)(((n + 7) / 8 + kBlock - 1) / kBlock);
   const I *xp = static_cast<const I *>(x);
   const O *rp = static_cast<const O *>(res);
   O *op = static_cast<O *>(out);
-  if (res) {
-    if (vec)
-      dropout_kernel<I, O, true, true><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold, scale,
-                                                               seed_ptr, seed, offset);
-    else
-      dropout_kernel<I, O, true, false><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold, scale,
-                                                                seed_ptr, seed, offset);
-  } else {
-    if (vec)
-      dropout_kernel<I, O, false, true><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold, scale,
-                                                                seed_ptr, seed, offset);
-    else
-      dropout_kernel<I, O, false, false><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold,
-                                                                 scale, seed_ptr, seed, offset);
-  }
+  if (res)
+    dropout_kernel<I, O, true><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold, scale, seed_ptr,
+                                                       seed, offset);
+  else
+    dropout_kernel<I, O, false><<<grid, kBlock, 0, s>>>(xp, rp, op, n, threshold, scale, seed_ptr,
+                                                        seed, offset);
   return check_launch("nf_dropout");
 }
 

@@ -19,48 +19,47 @@
 //               ids that no token holds: the sums wait for memory, the zeros only write.
 //   emb_join:   the partial rows of each run that crosses borders, added in order.
 // So the work of a token that holds half the batch is spread like any other.
-#include <initializer_list>
-
 #include "nf_device.h"
 
 namespace nf {
 namespace {
 
-// VE consecutive elements, aligned to their size (up to 16 bytes).
-template <typename T, int VE>
-__device__ __forceinline__ void load_n(const T *p, float (&v)[VE]) {
-  if constexpr (VE == 8) {
-    Chunk8<T>::load(p, v);
-  } else if constexpr (VE == 2) {
-    typedef T t2 __attribute__((ext_vector_type(2)));
-    const t2 a = *reinterpret_cast<const t2 *>(p);
-    v[0] = to_f32(a[0]);
-    v[1] = to_f32(a[1]);
-  } else {
-    v[0] = to_f32(p[0]);
-  }
+// Rows are taken in pieces of 8 columns, with 16-byte accesses whatever their alignment (an
+// odd D starts rows on any element, and the device takes global accesses on any byte: D 1645,
+// bf16, element by element took 104 us where this takes 38).  A last piece that would
+// pass the row's end starts at D - 8 and repeats columns of the one before: the same values
+// to the same places.  VEC: D >= 8; else a row is one piece of D elements.
+template <bool VEC>
+__device__ __forceinline__ int64_t piece(int64_t c, int64_t D) {
+  return VEC && c > D - 8 ? D - 8 : c;
 }
-template <typename T, int VE>
-__device__ __forceinline__ void store_n(T *p, const float (&v)[VE]) {
-  if constexpr (VE == 8) {
-    Chunk8<T>::store(p, v);
-  } else if constexpr (VE == 2) {
-    typedef T t2 __attribute__((ext_vector_type(2)));
-    t2 a;
-    a[0] = from_f32<T>(v[0]);
-    a[1] = from_f32<T>(v[1]);
-    *reinterpret_cast<t2 *>(p) = a;
-  } else {
-    p[0] = from_f32<T>(v[0]);
+
+template <typename T>
+struct Raw : Any8<T> {
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T *p, int64_t D) {
+    if constexpr (VEC)
+      Any8<T>::load(p);
+    else
+      Any8<T>::load(p, (int)D);
   }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8u(T *p, int64_t D, const float (&f)[8]) {
+  Any8<T> r;
+  r.set(f);
+  if constexpr (VEC)
+    r.store(p);
+  else
+    r.store(p, (int)D);
 }
 
 // ---------------------------------------------------------------------------
-// forward: a group of 2^glog lanes takes a row, VE columns a lane and step
+// forward: a group of 2^glog lanes takes a row, 8 columns a lane and step
 // ---------------------------------------------------------------------------
 constexpr int kFwdThreads = 256;
 
-template <typename W, typename O, int VE>
+template <typename W, typename O, bool VEC>
 __global__ __launch_bounds__(kFwdThreads) void emb_fwd_kernel(
     const int64_t *__restrict__ ids, const W *__restrict__ table, int64_t ldt, float scale,
     int64_t M, int64_t D, int64_t V, O *__restrict__ out, int glog) {
@@ -71,19 +70,20 @@ __global__ __launch_bounds__(kFwdThreads) void emb_fwd_kernel(
   const bool live = id >= 0 && id < V;
   const W *src = table + (live ? id : 0) * ldt;
   O *dst = out + m * D;
-  const int64_t step = (int64_t)VE << glog;
+  const int64_t step = (int64_t)8 << glog;
   constexpr int kUnroll = 4;
-  for (int64_t c0 = (int64_t)g * VE; c0 < D; c0 += kUnroll * step) {
-    float v[kUnroll][VE];
+  for (int64_t c0 = (int64_t)g * 8; c0 < D; c0 += kUnroll * step) {
+    Raw<W> r[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (c0 + u * step < D) load_n<W, VE>(src + c0 + u * step, v[u]);
+      if (c0 + u * step < D) r[u].template load<VEC>(src + piece<VEC>(c0 + u * step, D), D);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (c0 + u * step < D) {
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[u][i] = live ? v[u][i] * scale : 0.f;
-        store_n<O, VE>(dst + c0 + u * step, v[u]);
+        for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(r[u].v[i]) * scale : 0.f;
+        store8u<O, VEC>(dst + piece<VEC>(c0 + u * step, D), D, v);
       }
   }
 }
@@ -238,32 +238,11 @@ __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
   }
 }
 
-// VE elements as they lie in memory.
-template <typename T, int VE>
-struct Raw {
-  T v[VE];
-  __device__ __forceinline__ void load(const T *p) {
-    if constexpr (VE == 8) {
-      u32x4 a[sizeof(T) / 2];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) a[i] = reinterpret_cast<const u32x4 *>(p)[i];
-      __builtin_memcpy(v, a, sizeof(v));
-    } else if constexpr (VE == 2) {
-      typedef T t2 __attribute__((ext_vector_type(2)));
-      const t2 a = *reinterpret_cast<const t2 *>(p);
-      v[0] = a[0];
-      v[1] = a[1];
-    } else {
-      v[0] = *p;
-    }
-  }
-};
-
 // O: dout's type, W: dtable's.  Blocks [0, nsum) of the interleaved order sum, a wavefront a
 // (span, column part), parts of a span next to each other so that a row of dout is read
 // whole at one time; the other blocks clear.  part[2 s] is the head of span s (the end, or
 // all, of a run begun before it), part[2 s + 1] its tail (the begin of a run that goes on).
-template <typename O, typename W, int VE>
+template <typename O, typename W, bool VEC>
 __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const O *__restrict__ dout, int64_t ldo, const int *__restrict__ first,
     const Token *__restrict__ sorted, Order ord, int64_t V, int64_t D, float scale, int span,
@@ -277,10 +256,11 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const int64_t v = v0 + l;
     const int64_t at = ord.place(v < V ? v : 0);
     uint64_t empty = __ballot(v < V && first[at + 1] == first[at]);
-    const float zero[VE] = {};
+    const float zero[8] = {};
     for (; empty; empty &= empty - 1) {
       W *row = dtable + (v0 + __ffsll((unsigned long long)empty) - 1) * D;
-      for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) store_n<W, VE>(row + c, zero);
+      for (int64_t c = (int64_t)l * 8; c < D; c += 512)
+        store8u<W, VEC>(row + piece<VEC>(c, D), D, zero);
     }
     return;
   }
@@ -289,23 +269,24 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
   const int64_t t0 = s * span;
   if (t0 >= n) return;
   const int cnt = n - t0 < span ? (int)(n - t0) : span;
-  const int64_t c = ((u - s * cols) * 64 + l) * VE;
-  const bool cin = c < D;
+  const int64_t c8 = ((u - s * cols) * 64 + l) * 8, c = piece<VEC>(c8, D);
+  const bool cin = c8 < D;
   const Token own = l < cnt ? sorted[t0 + l] : Token{0, -1};
   const int tok = own.m, id = own.id;
   const int before = t0 > 0 ? sorted[t0 - 1].id : -1;
   const int after = t0 + cnt < n ? sorted[t0 + cnt].id : -1;
-  float acc[VE];
+  float acc[8];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   bool begun_before = before == __builtin_amdgcn_readlane(id, 0);
   constexpr int kBatch = 8;
-  Raw<O, VE> cur[kBatch], nxt[kBatch];
-  auto fetch = [&](int j0, Raw<O, VE> (&r)[kBatch]) {
+  Raw<O> cur[kBatch], nxt[kBatch];
+  auto fetch = [&](int j0, Raw<O> (&r)[kBatch]) {
 #pragma unroll
     for (int q = 0; q < kBatch; ++q)
       if (j0 + q < cnt && cin)
-        r[q].load(dout + (int64_t)__builtin_amdgcn_readlane(tok, j0 + q) * ldo + c);
+        r[q].template load<VEC>(dout + (int64_t)__builtin_amdgcn_readlane(tok, j0 + q) * ldo + c,
+                                D);
   };
   fetch(0, cur);
   for (int j0 = 0; j0 < cnt; j0 += kBatch) {
@@ -315,7 +296,7 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
       const int j = j0 + q;
       if (j >= cnt) break;
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += to_f32(cur[q].v[i]);
+      for (int i = 0; i < 8; ++i) acc[i] += to_f32(cur[q].v[i]);
       const int here = __builtin_amdgcn_readlane(id, j);
       const bool last = j + 1 == cnt;
       const int then = last ? after : __builtin_amdgcn_readlane(id, j + 1 < 64 ? j + 1 : 63);
@@ -323,16 +304,16 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
         const bool goes_on = then == here;
         if (cin) {
           if (begun_before || goes_on) {
-            store_n<float, VE>(part + (2 * s + (begun_before ? 0 : 1)) * D + c, acc);
+            store8u<float, VEC>(part + (2 * s + (begun_before ? 0 : 1)) * D + c, D, acc);
           } else {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) acc[i] *= scale;
-            store_n<W, VE>(dtable + (int64_t)here * D + c, acc);
+            for (int i = 0; i < 8; ++i) acc[i] *= scale;
+            store8u<W, VEC>(dtable + (int64_t)here * D + c, D, acc);
           }
         }
         begun_before = false;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
       }
     }
 #pragma unroll
@@ -343,11 +324,11 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
 // Block (s, y): the run that begins in span s and goes on past it, if there is one: its
 // tail there and the heads of the spans after it.  Wavefront k adds the pieces k, k + 8,
 // k + 16, ... in that order, the first wavefront the 8 sums.
-template <typename W, int VE>
+template <typename W, bool VEC>
 __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
     const int *__restrict__ first, const Token *__restrict__ sorted, Order ord, int64_t D,
     float scale, int span, const float *__restrict__ part, W *__restrict__ dtable) {
-  __shared__ float sums[kJoinWaves][64 * VE];
+  __shared__ float sums[kJoinWaves][512];
   const int n = first[ord.places()];
   const int64_t s = blockIdx.x, end = (s + 1) * span;  // a border between two spans
   if (end >= n) return;
@@ -357,38 +338,39 @@ __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
   if (first[at] < s * span) return;  // it began before
   const int64_t pieces = (first[at + 1] - 1) / span - s + 1;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = ((int64_t)blockIdx.y * 64 + l) * VE;
-  const bool cin = c < D;
-  float acc[VE];
+  const int64_t c8 = ((int64_t)blockIdx.y * 64 + l) * 8, c = piece<VEC>(c8, D);
+  const bool cin = c8 < D;
+  float acc[8];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
   if (cin) {
     constexpr int kBatch = 8;
     for (int64_t p0 = w; p0 < pieces; p0 += kJoinWaves * kBatch) {
-      float v[kBatch][VE];
+      Raw<float> v[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int64_t p = p0 + u * kJoinWaves;
-        if (p < pieces) load_n<float, VE>(part + (2 * (s + p) + (p == 0 ? 1 : 0)) * D + c, v[u]);
+        if (p < pieces)
+          v[u].template load<VEC>(part + (2 * (s + p) + (p == 0 ? 1 : 0)) * D + c, D);
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
         if (p0 + u * kJoinWaves < pieces)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) acc[i] += v[u][i];
+          for (int i = 0; i < 8; ++i) acc[i] += v[u].v[i];
     }
   }
 #pragma unroll
-  for (int i = 0; i < VE; ++i) sums[w][l * VE + i] = acc[i];
+  for (int i = 0; i < 8; ++i) sums[w][l * 8 + i] = acc[i];
   __syncthreads();
   if (w == 0 && cin) {
     const int waves = pieces < kJoinWaves ? (int)pieces : kJoinWaves;
     for (int k = 1; k < waves; ++k)
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += sums[k][l * VE + i];
+      for (int i = 0; i < 8; ++i) acc[i] += sums[k][l * 8 + i];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] *= scale;
-    store_n<W, VE>(dtable + (int64_t)id * D + c, acc);
+    for (int i = 0; i < 8; ++i) acc[i] *= scale;
+    store8u<W, VEC>(dtable + (int64_t)id * D + c, D, acc);
   }
 }
 
@@ -403,7 +385,7 @@ __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
 constexpr int kFewTokens = 1024, kLongRun = 32;
 constexpr int kFewThreads = 1024, kFewWaves = kFewThreads / 64;
 
-template <typename O, typename W, int VE>
+template <typename O, typename W, bool VEC>
 __global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
     const O *__restrict__ dout, const int64_t *__restrict__ ids, int M, int64_t V, int64_t D,
     int64_t pad, float scale, Order ord, W *__restrict__ dtable) {
@@ -412,7 +394,7 @@ __global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
   __shared__ int start[kMaxIds + 1], tok[kFewTokens];  // an id's first place; the tokens by id
   __shared__ int scan_w[kFewWaves];
   __shared__ int long_n, long_id[kFewTokens / kLongRun];
-  __shared__ float sums[kFewWaves][64 * VE];
+  __shared__ float sums[kFewWaves][512];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, R = ord.R;
   const int blk = blockIdx.x, mask = (1 << ord.log_nb) - 1;
   const uint64_t lower = (1ull << l) - 1ull;
@@ -450,32 +432,33 @@ __global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
   if (in) tok[start[key] + hist[w][key] + __popcll(same & lower)] = threadIdx.x;
   __syncthreads();
   // tokens [a, b) of the sorted order at the lane's columns from c on
-  auto sum = [&](int a, int b, int64_t c, float (&acc)[VE]) {
+  auto sum = [&](int a, int b, int64_t c, float (&acc)[8]) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     constexpr int kBatch = 8;
     for (int j0 = a; j0 < b; j0 += kBatch) {
-      Raw<O, VE> r[kBatch];
+      Raw<O> r[kBatch];
 #pragma unroll
       for (int q = 0; q < kBatch; ++q)
-        if (j0 + q < b) r[q].load(dout + (int64_t)tok[j0 + q] * D + c);
+        if (j0 + q < b) r[q].template load<VEC>(dout + (int64_t)tok[j0 + q] * D + c, D);
 #pragma unroll
       for (int q = 0; q < kBatch; ++q)
         if (j0 + q < b)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) acc[i] += to_f32(r[q].v[i]);
+          for (int i = 0; i < 8; ++i) acc[i] += to_f32(r[q].v[i]);
     }
   };
-  auto put = [&](int k, int64_t c, float (&acc)[VE]) {
+  auto put = [&](int k, int64_t c, float (&acc)[8]) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] *= scale;
-    store_n<W, VE>(dtable + (((int64_t)k << ord.log_nb) | blk) * D + c, acc);
+    for (int i = 0; i < 8; ++i) acc[i] *= scale;
+    store8u<W, VEC>(dtable + (((int64_t)k << ord.log_nb) | blk) * D + c, D, acc);
   };
   for (int k = w; k < R; k += kFewWaves) {
     const int a = start[k], b = start[k + 1];
     if ((((int64_t)k << ord.log_nb) | blk) >= V || b - a > kLongRun) continue;
-    for (int64_t c = (int64_t)l * VE; c < D; c += 64 * VE) {
-      float acc[VE];
+    for (int64_t c8 = (int64_t)l * 8; c8 < D; c8 += 512) {
+      const int64_t c = piece<VEC>(c8, D);
+      float acc[8];
       sum(a, b, c, acc);  // zeros where a == b
       put(k, c, acc);
     }
@@ -484,19 +467,19 @@ __global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
     const int k = long_id[q], a = start[k], b = start[k + 1];
     const int per = (b - a + kFewWaves - 1) / kFewWaves;
     const int pa = a + w * per < b ? a + w * per : b, pb = pa + per < b ? pa + per : b;
-    for (int64_t c0 = 0; c0 < D; c0 += 64 * VE) {
-      const int64_t c = c0 + (int64_t)l * VE;
-      float acc[VE];
-      if (c < D) {
+    for (int64_t c0 = 0; c0 < D; c0 += 512) {
+      const int64_t c8 = c0 + (int64_t)l * 8, c = piece<VEC>(c8, D);
+      float acc[8];
+      if (c8 < D) {
         sum(pa, pb, c, acc);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) sums[w][l * VE + i] = acc[i];
+        for (int i = 0; i < 8; ++i) sums[w][l * 8 + i] = acc[i];
       }
       __syncthreads();
-      if (w == 0 && c < D) {
+      if (w == 0 && c8 < D) {
         for (int p = 1; p < kFewWaves; ++p)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) acc[i] += sums[p][l * VE + i];
+          for (int i = 0; i < 8; ++i) acc[i] += sums[p][l * 8 + i];
         put(k, c, acc);
       }
       __syncthreads();
@@ -507,35 +490,20 @@ __global__ __launch_bounds__(kFewThreads) void emb_few_kernel(
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Columns a lane takes at once: 8 where every row starts on 16 bytes, 2 where every row
-// starts on a pair, else 1.
-int vector_width(std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> lds,
-                 int64_t D) {
-  auto fits = [&](int ve, uintptr_t bytes) {
-    for (const void *p : ptrs)
-      if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
-    for (int64_t ld : lds)
-      if (ld % ve) return false;
-    return D % ve == 0;
-  };
-  return fits(8, 16) ? 8 : fits(2, 8) ? 2 : 1;
-}
-
 template <typename W, typename O>
 int run_fwd(const int64_t *ids, const W *table, int64_t ldt, float scale, int64_t M, int64_t D,
             int64_t V, O *out, hipStream_t s) {
-  const int ve = vector_width({table, out}, {ldt}, D);
-  const int64_t vecs = (D + ve - 1) / ve;
+  const int64_t pieces = (D + 7) / 8;
   int glog = 3;
-  while (glog < 6 && ((int64_t)1 << glog) < vecs) ++glog;
+  while (glog < 6 && ((int64_t)1 << glog) < pieces) ++glog;
   const int64_t rows = kFwdThreads >> glog;
   const unsigned grid = (unsigned)((M + rows - 1) / rows);
-  if (ve == 8)
-    emb_fwd_kernel<W, O, 8><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
-  else if (ve == 2)
-    emb_fwd_kernel<W, O, 2><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
+  if (D >= 8)
+    emb_fwd_kernel<W, O, true><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out,
+                                                            glog);
   else
-    emb_fwd_kernel<W, O, 1><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out, glog);
+    emb_fwd_kernel<W, O, false><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out,
+                                                             glog);
   return check_launch("nf_embedding_fwd");
 }
 
@@ -567,7 +535,7 @@ BwdPlan bwd_plan(int64_t M, int64_t D, int64_t V) {
   return p;
 }
 
-template <typename O, typename W, int VE>
+template <typename O, typename W, bool VEC>
 int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int64_t M, int64_t D,
                int64_t V, W *dtable, char *ws, hipStream_t s) {
   const BwdPlan p = bwd_plan(M, D, V);
@@ -575,20 +543,20 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
   Token *sorted = reinterpret_cast<Token *>(ws + p.sorted);
   float *part = reinterpret_cast<float *>(ws + p.part);
   if (M <= kFewTokens) {
-    emb_few_kernel<O, W, VE><<<1u << p.ord.log_nb, kFewThreads, 0, s>>>(
+    emb_few_kernel<O, W, VEC><<<1u << p.ord.log_nb, kFewThreads, 0, s>>>(
         dout, ids, (int)M, V, D, pad, scale, p.ord, dtable);
     return check_launch("emb_few");
   }
-  const unsigned cols = (unsigned)((D + 64 * VE - 1) / (64 * VE));
+  const unsigned cols = (unsigned)((D + 511) / 512);
   emb_sort_kernel<<<1u << p.ord.log_nb, kSortThreads, 0, s>>>(ids, M, V, pad, p.ord, first,
                                                               sorted);
   if (int e = check_launch("emb_sort")) return e;
   const int64_t nsum = (p.spans * cols + 3) / 4, nclear = (V + 4 * kZeroIds - 1) / (4 * kZeroIds);
   if (nsum + nclear > 0x7fffffffLL) return set_error(NF_ERR_ARG, "nf_embedding_bwd: too large");
-  emb_reduce_kernel<O, W, VE><<<(unsigned)(nsum + nclear), 256, 0, s>>>(
+  emb_reduce_kernel<O, W, VEC><<<(unsigned)(nsum + nclear), 256, 0, s>>>(
       dout, D, first, sorted, p.ord, V, D, scale, p.span, (int)cols, nclear, dtable, part);
   if (int e = check_launch("emb_reduce")) return e;
-  emb_join_kernel<W, VE><<<dim3((unsigned)(p.spans - 1), cols), kJoinThreads, 0, s>>>(
+  emb_join_kernel<W, VEC><<<dim3((unsigned)(p.spans - 1), cols), kJoinThreads, 0, s>>>(
       first, sorted, p.ord, D, scale, p.span, part, dtable);
   return check_launch("emb_join");
 }
@@ -596,10 +564,8 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
 template <typename O, typename W>
 int run_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int64_t M, int64_t D,
             int64_t V, W *dtable, char *ws, hipStream_t s) {
-  const int ve = vector_width({dout, dtable}, {}, D);
-  if (ve == 8) return launch_bwd<O, W, 8>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
-  if (ve == 2) return launch_bwd<O, W, 2>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
-  return launch_bwd<O, W, 1>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
+  return D >= 8 ? launch_bwd<O, W, true>(dout, ids, pad, scale, M, D, V, dtable, ws, s)
+                : launch_bwd<O, W, false>(dout, ids, pad, scale, M, D, V, dtable, ws, s);
 }
 
 // The table's type and out's: equal, or an fp32 table with rows in 16 bits.
@@ -608,9 +574,9 @@ bool types_ok(int dt_table, int dt_out) {
          (dt_table == dt_out || dt_table == NF_DTYPE_F32);
 }
 bool sizes_ok(int64_t M, int64_t D, int64_t V) {
-  // D: at most 65535 column blocks of 64 elements in a grid
+  // D: at most 65535 column blocks of 512 elements in a grid
   const int64_t i32 = 0x7fffffffLL, cap = (int64_t)1 << 40;
-  return M >= 0 && D > 0 && V > 0 && M < i32 && D <= 65535 * 64 && V < i32 && V * D <= cap &&
+  return M >= 0 && D > 0 && V > 0 && M < i32 && D <= 65535 * 512 && V < i32 && V * D <= cap &&
          M * D <= cap;
 }
 

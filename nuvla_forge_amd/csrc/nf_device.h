@@ -257,6 +257,52 @@ __device__ __forceinline__ void store8_dyn(void *p, int dt, int64_t off, const f
 }
 
 // ---------------------------------------------------------------------------
+// 8 elements as they lie in memory, at any alignment of their type: 16-byte accesses all the
+// same (the device takes global accesses on any byte), for rows of a width that is no
+// multiple of 8 and for views.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Any8 {
+  T v[8];
+  static constexpr int kWords = (int)sizeof(T) / 2;
+  __device__ __forceinline__ void load(const T *p) {
+    u32x4 a[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      __builtin_memcpy(&a[i], reinterpret_cast<const char *>(p) + 16 * i, 16);
+    __builtin_memcpy(v, a, sizeof(v));
+  }
+  __device__ __forceinline__ void load(const T *p, int valid) {
+    if (valid >= 8) {
+      load(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < valid ? p[i] : static_cast<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(f[i]);
+  }
+  __device__ __forceinline__ void store(T *p) const {
+    u32x4 a[kWords];
+    __builtin_memcpy(a, v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      __builtin_memcpy(reinterpret_cast<char *>(p) + 16 * i, &a[i], 16);
+  }
+  __device__ __forceinline__ void store(T *p, int valid) const {
+    if (valid >= 8) {
+      store(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < valid) p[i] = v[i];
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
 // Wavefront reductions.  Steps inside a 16-lane DPP row use quad_perm and the
 // row mirrors (each pairs every lane with a partner in the other half of its
 // group, so after four steps all 16 lanes hold the row total); the two

@@ -918,6 +918,18 @@ inline bool weight_as_is(int64_t M, int64_t D, int64_t V) {
   return M <= 256 + D / 4 && D % 8 == 0 && sb_ok(V * D * (int64_t)sizeof(bf16));
 }
 
+// The tiling for `rows` rows, as MidCfg names them, or -1: the main tiles, which are also the
+// better ones where the smaller ones' 128 rows make more than a block a CU (V 43813, D 304, 178
+// rows, forward and backward: 91 us against 109; V 128256, D 1024, 128 rows, forward 180
+// against 188; fp32, V 85667, D 1432, 47 rows 1168 against 1287).  bf16 of up to 64 rows gains
+// from its 64 columns at every V.
+template <typename TI>
+int mid_form(int64_t rows, int64_t V) {
+  if (rows <= 64 && (sizeof(TI) == 2 || V <= 32768)) return 64;
+  if (rows > 256 || V > 32768) return -1;
+  return rows <= 128 ? 128 : 256;
+}
+
 template <typename TI>
 ce::Plan grad_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
   const int64_t lo0 = few_rows<TI>(M);
@@ -930,8 +942,8 @@ ce::Plan grad_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
 // backward then forms dz in one pass over it instead of forming the logits again.  M 4096,
 // D 2048, V 32000, 10% left out: forward and backward 1513 us, against 1828 with the logits
 // formed twice (the kernel lp_from_kept takes 96 us, 5.5 TB/s, in the place of 528 of lp_dz;
-// keeping costs lp_logits 60).  Up to 256 rows forming them again on MidCfg's tiles is the
-// faster: D 2048, 200 rows 207 us against 229.
+// keeping costs lp_logits 60).  178 rows, D 1024: 123 us against 129; with a narrower D forming
+// them again on MidCfg's tiles is the faster (D 384: 73 against 75).
 struct State {
   bool kept, as_is;  // as_is: no transpose of weight among it
   int nstat;
@@ -953,7 +965,8 @@ State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool kee
   s.ent = take((size_t)M * sizeof(float));
   s.lp = take((size_t)M * sizeof(float));
   s.hc = take((size_t)(s.lo0 > 0 ? 2 * s.lo0 : M) * D * sizeof(TI));
-  if (sizeof(TI) == 2 && keep && M > 256 && V <= kKeptCols) {
+  if (sizeof(TI) == 2 && keep && M > kFewRows && V <= kKeptCols &&
+      (D >= 1024 || mid_form<TI>(M, V) < 0)) {
     const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
     if (L.nch == 1) {
       s.kept = true;
@@ -1044,16 +1057,6 @@ struct MidCfg<float> {
   using T256 = SplitCfg<256, 128, 4, 2>;
 };
 
-// The tiling for `rows` rows: 64, 128, 256, or -1: the main tiles, which are also the better
-// ones where V alone makes 256 of them (V 128256, D 1024, 128 rows: 180 us against 188; fp32
-// lp_dz of 47 rows, V 85667, D 1432: 50 us more on the smaller tiles).  bf16 of up to 64 rows
-// gains from its 64 columns at every V.
-template <typename TI>
-int mid_form(int64_t rows, int64_t V) {
-  if (rows <= 64 && (sizeof(TI) == 2 || V <= 65536)) return 64;
-  if (rows > 256 || V > 65536) return -1;
-  return rows <= 128 ? 128 : 256;
-}
 
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
@@ -1076,7 +1079,7 @@ template <typename TI>
 FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept) {
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
-  p.form = M <= kSkinnyRows<TI> ? 0 : mid_form<TI>(M, V);
+  p.form = M <= kSkinnyRows<TI> ? 0 : kept ? -1 : mid_form<TI>(M, V);
   p.crows = p.form >= 0 ? M
             : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
                                              : mcap;
@@ -1119,6 +1122,8 @@ int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan 
     NF_LP_FINISH(true, 16);
   else if (vk && nrec <= 64 * 32)
     NF_LP_FINISH(true, 32);
+  else if (vk && nrec <= 64 * 64)
+    NF_LP_FINISH(true, 64);
   else if (vk)
     NF_LP_FINISH(true, 0);
   else

@@ -156,7 +156,7 @@ def test_embedding_c_abi_refusals():
         assert L.nf_embedding_fwd(*(ok[:i] + [bad] + ok[i + 1:])) == rc, (i, bad, _err())
     need = L.nf_embedding_bwd_workspace(16, 64, 100)
     assert need > 0 and L.nf_embedding_bwd_workspace(-1, 64, 100) == 0
-    assert L.nf_embedding_bwd_workspace(16, 1 << 23, 100) == 0
+    assert L.nf_embedding_bwd_workspace(16, 1 << 26, 100) == 0
     ok = [FAKE, FAKE, -1, 1.0, 16, 64, 100, FAKE, 1, 1, FAKE, need, None]
     for i, bad, rc in ((4, -1, NF_ERR_ARG), (5, 0, NF_ERR_ARG), (0, None, NF_ERR_ARG),
                        (1, None, NF_ERR_ARG), (7, None, NF_ERR_ARG), (9, 2, NF_ERR_DTYPE),

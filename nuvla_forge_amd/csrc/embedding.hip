@@ -44,18 +44,21 @@ struct Raw : Any8<T> {
       Any8<T>::load(p, (int)D);
   }
 };
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool NT = false>
 __device__ __forceinline__ void store8u(T *p, int64_t D, const float (&f)[8]) {
   Any8<T> r;
   r.set(f);
   if constexpr (VEC)
-    r.store(p);
+    r.template store<NT>(p);
   else
     r.store(p, (int)D);
 }
 
 // ---------------------------------------------------------------------------
-// forward: a group of 2^glog lanes takes a row, 8 columns a lane and step
+// forward: a group of 2^glog lanes takes a row, 8 columns a lane and step.  What bounds it is
+// memory: bf16, 65536 tokens by Zipf's law, V 128256, D 2048, 64 us for the 268 MB written and
+// as much read (a third of it from HBM), 78 without the non-temporal hint on the stores; 8192
+// tokens, D 1024 6.0 us, 7.0 without.
 // ---------------------------------------------------------------------------
 constexpr int kFwdThreads = 256;
 
@@ -83,7 +86,7 @@ __global__ __launch_bounds__(kFwdThreads) void emb_fwd_kernel(
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = live ? to_f32(r[u].v[i]) * scale : 0.f;
-        store8u<O, VEC>(dst + piece<VEC>(c0 + u * step, D), D, v);
+        store8u<O, VEC, true>(dst + piece<VEC>(c0 + u * step, D), D, v);
       }
   }
 }

@@ -261,6 +261,7 @@ __device__ __forceinline__ void store8_dyn(void *p, int dt, int64_t off, const f
 // same (the device takes global accesses on any byte), for rows of a width that is no
 // multiple of 8 and for views.
 // ---------------------------------------------------------------------------
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 template <typename T>
 struct Any8 {
   T v[8];
@@ -284,16 +285,24 @@ struct Any8 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(f[i]);
   }
+  // NT: with the non-temporal hint (outputs that the kernel does not read again)
+  template <bool NT = false>
   __device__ __forceinline__ void store(T *p) const {
     u32x4 a[kWords];
     __builtin_memcpy(a, v, sizeof(v));
 #pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      __builtin_memcpy(reinterpret_cast<char *>(p) + 16 * i, &a[i], 16);
+    for (int i = 0; i < kWords; ++i) {
+      u32x4_any *q = reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(p) + 16 * i);
+      if constexpr (NT)
+        __builtin_nontemporal_store(a[i], q);
+      else
+        *q = a[i];
+    }
   }
+  template <bool NT = false>
   __device__ __forceinline__ void store(T *p, int valid) const {
     if (valid >= 8) {
-      store(p);
+      store<NT>(p);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)

@@ -1105,6 +1105,15 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept)
   return p;
 }
 
+// Enough for either form: a state that is kept takes every row in one chunk, on the main tiles.
+template <typename TI>
+size_t fwd_bytes(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, int top_k) {
+  const size_t plain = fwd_plan<TI>(M, V, chunk_rows, top_k, false).total;
+  if (!state_layout<TI>(M, D, V, chunk_rows, true).kept) return plain;
+  const size_t kept = fwd_plan<TI>(M, V, chunk_rows, top_k, true).total;
+  return kept > plain ? kept : plain;
+}
+
 template <typename TI>
 int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan &P,
                   const Stat *stats, const Rec *recs, const float *tgt, int64_t j0, int64_t rows,
@@ -1397,8 +1406,8 @@ extern "C" size_t nf_token_logprobs_fwd_workspace(int64_t M, int64_t D, int64_t 
   if (!sizes_ok(M, D, V) || chunk_rows <= 0 || !dtype_ok(dtype) || top_k < 0 ||
       top_k > kMaxTop || top_k > V)
     return 0;
-  return dtype == NF_DTYPE_BF16 ? fwd_plan<bf16>(M, V, chunk_rows, top_k, false).total
-                                : fwd_plan<float>(M, V, chunk_rows, top_k, false).total;
+  return dtype == NF_DTYPE_BF16 ? fwd_bytes<bf16>(M, D, V, chunk_rows, top_k)
+                                : fwd_bytes<float>(M, D, V, chunk_rows, top_k);
 }
 
 extern "C" size_t nf_token_logprobs_bwd_workspace(int64_t M, int64_t D, int64_t V,

@@ -305,6 +305,18 @@ def test_logprobs_in_chunks(cuda, dtype):
     assert torch.equal(whole.top_ids, part.top_ids)
 
 
+@pytest.mark.parametrize("m, d, v, chunk_size", [(1100, 1024, 1001, 8), (129, 1024, 100, 1024),
+                                                 (700, 384, 3001, 1)])
+def test_logprobs_kept_in_one_small_chunk(cuda, m, d, v, chunk_size):
+    """The accumulator's share of the memory bound keeps every row's logits at once."""
+    note(f"logprobs kept {m} {d} {v} {chunk_size}")
+    args = _head(m, d, v, BF16, cuda, grid=True)
+    few, _ = _logprobs_check(*args, 20, chunk_size=chunk_size)
+    many, _ = _logprobs_check(*args, 20, chunk_size=4096)
+    for a, b in zip(few, many):
+        assert torch.equal(a, b)
+
+
 def test_logprobs_ties_go_to_the_lower_token(cuda):
     """Equal rows of the head far apart, and a hidden row of zeros: every logit equal."""
     note("logprobs ties")

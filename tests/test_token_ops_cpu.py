@@ -262,3 +262,15 @@ def test_logprobs_c_abi_refusals():
         assert L.nf_token_logprobs_bwd(*(ok[:i] + [x] + ok[i + 1:])) == rc, (i, x, _err())
     nothing = ok[:11] + [None, 1, None, 1] + ok[15:]
     assert L.nf_token_logprobs_bwd(*nothing) == NF_OK  # no gradient wanted: no launch
+
+
+@pytest.mark.parametrize("m, d, v, chunk_rows", [(1024, 1024, 520, 8), (4096, 2048, 32000, 64),
+                                                 (129, 1024, 100, 1024), (256, 1024, 300, 1)])
+def test_logprobs_workspace_holds_what_a_kept_forward_writes(m, d, v, chunk_rows):
+    """Where the state holds 16 bits of every logit, the forward takes every row at once: whole
+    blocks of 256 rows by 256 columns with an 8-byte record per 32 columns, and 4 bytes a row."""
+    L = _lib.lib()
+    mcap, tiles = -(-m // 256) * 256, -(-v // 256)
+    assert L.nf_token_logprobs_state_bytes(m, d, v, chunk_rows, 1, 1) >= 2 * mcap * v
+    assert (L.nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, 5, 1)
+            >= mcap * tiles * 8 * 8 + mcap * 4)

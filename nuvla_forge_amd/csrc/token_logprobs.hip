@@ -825,10 +825,12 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     int want = -1;  // the register that holds the target, if this lane does
     const bool low = lo0 > 0 && tok >= lo0;
     const int64_t row = j0 + (low ? tok - lo0 : tok);
+    bool counts = false;
     if (row - j0 < live) {
       const int64_t m = in.rows[row];
       const int tc = in.tcol[row];
-      if (tc >= 0) {  // else a row that does not count: its hidden row is zero here
+      counts = tc >= 0;
+      if (counts) {
         g = in.g ? in.g[m] : 0.f;
         h = in.h ? in.h[m] : 0.f;
       }
@@ -838,6 +840,14 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
       const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
       if (loc >= 0 && ((loc >> 2) & 1) == half)
         want = ((loc >> 5) << 4) | (((loc & 31) >> 3) << 2) | (loc & 3);
+    }
+    // a row that does not count, or of the padding: its hidden row is zero here, but an
+    // infinity in weight makes a NaN of its logits
+    if (!counts) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     }
     const float a = -(g + h * ent);
 #pragma unroll

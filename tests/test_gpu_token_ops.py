@@ -417,6 +417,28 @@ def test_logprobs_rows_left_out_may_hold_anything(cuda, m, dtype):
         assert ((x.double() - ref[name]).abs() <= ref["tol_" + name]).all(), name
 
 
+@pytest.mark.parametrize("m", [6, 100, 290])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logprobs_infinite_weight_and_rows_left_out(cuda, m, dtype):
+    """A token that a weight of -inf rules out has probability 0 in every row; the rows left out,
+    which the products see as zeros, add no 0 * inf to weight's gradient."""
+    note(f"logprobs inf weight {m} {dtype}")
+    h, w, t, g, gh = _head(m, 64, 900, dtype, cuda, ignored=0.3)
+    h[:, 0] = h[:, 0].abs() + 0.125
+    t = torch.where(t == 7, 8, t)
+    t[0], t[1] = -100, 8  # both kinds at every size
+    w[7, 0] = float("-inf")
+    h[0, 0] = 0.0  # 0 * inf where it does not count
+    out = chunked_token_logprobs(h, w.requires_grad_(True), t)
+    (dw,) = torch.autograd.grad([out.logprobs, out.entropy], [w], [g, gh])
+    rest = torch.arange(900, device=cuda) != 7
+    ref = logprobs64(h, w.detach()[rest], torch.where(t > 7, t - 1, t), g, gh)
+    assert ((out.logprobs.double() - ref["logprobs"]).abs() <= ref["tol_lp"]).all()
+    assert ((out.entropy.double() - ref["entropy"]).abs() <= ref["tol_ent"]).all()
+    assert (dw[7] == 0).all()
+    assert ((dw[rest].double() - ref["dw"]).abs() <= ref["tol_dw"]).all()
+
+
 def test_logprobs_past_two_gib(cuda):
     """What is kept for the backward takes more than 2 GiB: 32-bit offsets do not reach it."""
     note("logprobs past 2 GiB")

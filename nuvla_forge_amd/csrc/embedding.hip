@@ -26,7 +26,7 @@ namespace {
 
 // Rows are taken in pieces of 8 columns, with 16-byte accesses whatever their alignment (an
 // odd D starts rows on any element, and the device takes global accesses on any byte: D 1645,
-// bf16, element by element took 104 us where this takes 38).  A last piece that would
+// bf16, forward and backward, element by element took 104 us where this takes 54).  A last piece that would
 // pass the row's end starts at D - 8 and repeats columns of the one before: the same values
 // to the same places.  VEC: D >= 8; else a row is one piece of D elements.
 template <bool VEC>
@@ -126,7 +126,8 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
 // tokens that count); sorted: the token and its id at each position.
 //
 // A block's time goes into reading the ids (M 65536: 0.5 MB a block from the L2s) and
-// into placing its tokens, where most of them belong to a few blocks.
+// into placing its tokens, where most of them belong to a few blocks: 24 us for 65536 tokens
+// by Zipf's law, V 128256.
 __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
     const int64_t *__restrict__ ids, int64_t M, int64_t V, int64_t pad, Order ord,
     int *__restrict__ first, Token *__restrict__ sorted) {
@@ -245,6 +246,8 @@ __global__ __launch_bounds__(kSortThreads) void emb_sort_kernel(
 // (span, column part), parts of a span next to each other so that a row of dout is read
 // whole at one time; the other blocks clear.  part[2 s] is the head of span s (the end, or
 // all, of a run begun before it), part[2 s + 1] its tail (the begin of a run that goes on).
+// What bounds it is memory: bf16, 65536 tokens by Zipf's law, V 128256, D 2048 164 us for the
+// 268 MB read and 525 MB written, 4.8 TB/s.
 template <typename O, typename W, bool VEC>
 __global__ __launch_bounds__(256) void emb_reduce_kernel(
     const O *__restrict__ dout, int64_t ldo, const int *__restrict__ first,
@@ -326,7 +329,8 @@ __global__ __launch_bounds__(256) void emb_reduce_kernel(
 
 // Block (s, y): the run that begins in span s and goes on past it, if there is one: its
 // tail there and the heads of the spans after it.  Wavefront k adds the pieces k, k + 8,
-// k + 16, ... in that order, the first wavefront the 8 sums.
+// k + 16, ... in that order, the first wavefront the 8 sums.  Its time is the latency of the
+// longest run (24 us where one token holds a twelfth of 65536), which the 8 wavefronts share.
 template <typename W, bool VEC>
 __global__ __launch_bounds__(kJoinThreads) void emb_join_kernel(
     const int *__restrict__ first, const Token *__restrict__ sorted, Order ord, int64_t D,

@@ -142,6 +142,8 @@ __device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, 
 // registers.  What bounds it: the products at D 2048 (bf16, 3686 rows, V 32000: 455 us, 1.06
 // PFLOP/s); at D 384 the epilogue, which nothing overlaps (11920 rows, V 50001: 590 us for 458
 // GFLOP, 690 with the records: their stores ~50, the places ~30, the second largest ~20).
+// Two blocks of half the token columns a CU, 32 k a stage, to overlap it: level without records
+// (613 us against 608), 766 against 788 with them, and 20% slower at D 2048.
 // stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
 // KEEP (16-bit inputs): exp(z - mx), mx the strip's maximum, is kept for the backward in
 // fp16, E [crows, ldp]: half a step of 2^-11 of each, and what is below 2^-24 of the strip's
@@ -251,9 +253,24 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
         const float x = acc[i][j][r] - base;
         const float e = exp_f32(x);
         s += e;
-        t += fmaxf(x, kFar) * e;  // e is 0 where x is -inf, and a NaN where it is one
-        if constexpr (KEEP) acc[i][j][r] = e;
+        t += (KEEP ? fmaxf(x, kFar) : x) * e;
+        acc[i][j][r] = KEEP ? e : x;
       }
+    // -inf * 0 is a NaN: without KEEP, where x is still there, a strip with a logit of -inf (or
+    // past the vocabulary) and no NaN is summed again with x bounded.  Bounding every x costs 3%
+    // of the tall head (12289 rows, D 384, V 50001, 20 alternatives 772 us against 747).
+    if constexpr (!KEEP) {
+      if (t != t && s == s) {
+        t = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float x = acc[i][j][r];
+            t += fmaxf(x, kFar) * exp_f32(x);
+          }
+      }
+    }
     s += __shfl_xor(s, 32);
     t += __shfl_xor(t, 32);
     if (half == 0 && tok < cnt) stats[tok * nstat + stat] = Stat{mx, s, t, 0.f};

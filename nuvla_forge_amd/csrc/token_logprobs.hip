@@ -494,6 +494,13 @@ struct Chosen {
   float again[32];  // a strip's logits
 };
 
+// A wavefront's own LDS writes are done before its later reads.
+__device__ __forceinline__ void wave_lds_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
 // The strips whose first logits come first among those after (pv, pi), from entry `found` on;
 // how many there are then.  Every round reads the records again.
 __device__ __forceinline__ int choose_slow(const Rec *rc, int nrec, const Strips &strips,
@@ -526,11 +533,20 @@ __device__ __forceinline__ int choose_slow(const Rec *rc, int nrec, const Strips
   return found;
 }
 
-// The same with the first logits in registers, NR a lane (lane l: strips l, l + 64, ...): each
-// lane keeps its maximum; a round takes the wavefront's and clears the register that held it.
-// Of equal values the lower column: within a lane the earlier register (64 strips are whole
-// statistics strips), between lanes by the records.  Ends at logits of -inf, which choose_slow
-// orders.
+// The same with the first logits in registers, NR a lane (lane l: strips l, l + 64, ...).
+//
+// From kRankedTop alternatives on: the K-th largest of the 64 lanes' maxima bounds what can be
+// among them from below, and what is left by it, about 64 log(64 / (64 - K)) strips, is ranked.
+// Forward in a graph against the rounds below, bf16: D 384, 12289 rows, V 50001, 20 alternatives
+// 714 us against 767, 8 699 against 716, 4 level, 2 690 against 688; 4096 rows, V 5000, 8 61
+// against 66; 8 rows, D 2048, V 32000, 32 49 against 62, 8 29.8 against 31.7, 1 29.5 against 28.6.
+//
+// Fewer, or more than 64 left (equal logits), or less than K lanes with a logit above -inf: in
+// rounds.  Each lane keeps its maximum; a round takes the wavefront's and clears the register
+// that held it.  Of equal values the lower column: within a lane the earlier register (64 strips
+// are whole statistics strips), between lanes by the records.  Ends at logits of -inf, which
+// choose_slow orders.
+constexpr int kRankedTop = 4;
 template <int NR>
 __device__ __forceinline__ int choose(const Rec *rc, int nrec, const Strips &strips, int64_t V,
                                       int K, Chosen &ch) {
@@ -543,6 +559,45 @@ __device__ __forceinline__ int choose(const Rec *rc, int nrec, const Strips &str
     best = fmaxf(best, v[i]);
   }
   auto column_of = [&](int strip) { return strips.column(strip, (int)(rc[strip].rest & 63u)); };
+  if (K >= kRankedTop) {
+    // `last`: the K-th largest of the lanes' maxima, equal ones counted; K firsts are no less
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j)
+      above += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(best), j)) > best ? 1 : 0;
+    const float last = -wave_max(above < K ? -best : -INFINITY);
+    int n = 0;
+    if (last > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const uint64_t may = __ballot(v[i] >= last);
+        if (!may) continue;
+        const int q = n + __popcll(may & ((1ull << l) - 1ull));
+        if (((may >> l) & 1) && q < 64) {
+          ch.cand_v[q] = v[i];
+          ch.cand_col[q] = l + 64 * i;
+        }
+        n += __popcll(may);
+      }
+    }
+    if (n > 0 && n <= 64) {
+      wave_lds_fence();
+      const float x = l < n ? ch.cand_v[l] : -INFINITY;
+      const int strip = l < n ? ch.cand_col[l] : 0;
+      const int col = column_of(strip);
+      int place = 0;
+      for (int j = 0; j < n; ++j)
+        place += before(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), j)),
+                        __builtin_amdgcn_readlane(col, j), x, col)
+                     ? 1
+                     : 0;
+      if (l < n && place < K) {
+        ch.v[place] = x;
+        ch.strip[place] = strip;
+      }
+      return K;
+    }
+  }
   int found = 0, pi = -1;
   float pv = INFINITY;
   while (found < K) {
@@ -577,13 +632,6 @@ __device__ __forceinline__ int choose(const Rec *rc, int nrec, const Strips &str
   }
   if (found == K) return K;
   return choose_slow(rc, nrec, strips, V, K, ch, found, pv, found ? column_of(pi) : -1);
-}
-
-// A wavefront's own LDS writes are done before its later reads.
-__device__ __forceinline__ void wave_lds_fence() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
 }
 
 // NR: records in a lane's registers (0: more than fit, read in every round).  `targets`: the

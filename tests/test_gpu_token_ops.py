@@ -333,6 +333,33 @@ def test_logprobs_ties_go_to_the_lower_token(cuda):
         assert abs(out.entropy[1].item() - math.log(v)) < 1e-5
 
 
+@pytest.mark.parametrize("k", [1, 4, 8, 32])
+@pytest.mark.parametrize("m, v", [(3, 70), (3, 32000), (300, 5000), (300, 130000)])
+def test_logprobs_many_equal_logits(cuda, m, v, k):
+    """Rows of equal logits, and rows whose best k - 1, k, 65 and 66 logits alone are equal."""
+    note(f"logprobs equal {m} {v} {k}")
+    h, w = torch.zeros(m, 64, device=cuda), torch.zeros(v, 64, device=cuda)
+    places = torch.randperm(v, generator=gen(v + k))
+    for c, n in enumerate((k - 1, k, 65, 66)):
+        w[places[:min(n, v)], c] = 1.0
+        h[c % m, :4] = 0.0
+        h[c % m, c] = 2.0
+    if m > 4:
+        h[4, 0], h[5, 2] = -2.0, -2.0  # the equal ones last
+    w[:, 8] = -torch.arange(v, device=cuda) / 2.0 ** 20  # falling: exact in fp32 and its parts
+    if m > 6:
+        h[6, 8] = 1.0
+    t = torch.zeros(m, dtype=torch.int64, device=cuda)
+    out = chunked_token_logprobs(h, w, t, top_k=k)
+    val, idx = torch.sort(h @ w.T, dim=1, descending=True, stable=True)
+    assert torch.equal(out.top_ids, idx[:, :k])
+    want = torch.log_softmax((h @ w.T).double(), 1).gather(1, idx[:, :k])
+    # logits are exact; log S and the difference: 2^-22 of them, log 130000 < 12, and V / 64 + 64
+    # roundings of S
+    tol = 2.0 ** -22 * 16 + (v / 64 + 64) * 2.0 ** -24
+    assert ((out.top_logprobs.double() - want).abs() <= tol).all()
+
+
 def test_logprobs_alternatives_crowded_in_one_place(cuda):
     """The most probable tokens next to each other, at every place of the vocabulary's tiles."""
     note("logprobs crowded")

@@ -140,8 +140,8 @@ __device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, 
 // One block tile: acc = W_tile Hc_tile^T (rows: vocabulary, columns: tokens), so a lane
 // holds 16 TM logits of each of its TN tokens and the strip's values are reductions in
 // registers.  What bounds it: the products at D 2048 (bf16, 3686 rows, V 32000: 455 us, 1.06
-// PFLOP/s); at D 384 the epilogue, which nothing overlaps (11920 rows, V 50001: 590 us for 458
-// GFLOP, 690 with the records: their stores ~50, the places ~30, the second largest ~20).
+// PFLOP/s); at D 384 the epilogue, which nothing overlaps (11920 rows, V 50001: 570 us for 458
+// GFLOP, 665 with the records: their stores ~50, the places ~30, the second largest ~20).
 // Two blocks of half the token columns a CU, 32 k a stage, to overlap it: level without records
 // (613 us against 608), 766 against 788 with them, and 20% slower at D 2048.
 // stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(kSkinnyThreads) void lp_skinny_kernel(
 // 3. a row's outputs, one wavefront a row: the statistics joined in a fixed order
 // (log p and the entropy follow: lse = mx + log S, H = log S - T / S), then the
 // alternatives from the strips' records.  Its time is latency: 8 rows, V 32000, 8 alternatives
-// 9 us, 3686 rows 32 us, of which the strips formed again (D 2048, at most a few a row) are most.
+// 8 us, 3686 rows 28 us, of which the strips formed again (D 2048, at most a few a row) are most.
 // ---------------------------------------------------------------------------
 constexpr int kFinishThreads = 256;
 
@@ -1122,6 +1122,9 @@ int transposes(const TI *W, const TI *Hc, int64_t Mb, int64_t D, int64_t V, cons
 // (the 131 MB of W partly in the Infinity Cache) against 59, 128 rows 36.9 against 60, 256 rows
 // 43 against 61; D 384 12.1 against 25, 15.3 against 25, 17.8 against 26.  fp32, 128 rows: D
 // 2048 130 us against 161, D 384 33 against 45.
+// Tall64: fp32 of 33 to 64 rows where the 128 rows of W would make more than a block a CU, with no
+// empty token columns: 64 rows, V 85667, D 1024 158 us against 178 on the main tiles, V 33000 70
+// against 89, V 128256, D 2048 320 against 356, D 256 57 against 69.
 template <typename TI>
 struct MidCfg;
 template <>
@@ -1135,17 +1138,20 @@ struct MidCfg<float> {
   using T64 = SplitCfg<128, 128, 2, 2>;
   using T128 = T64;
   using T256 = SplitCfg<256, 128, 4, 2>;
+  using Tall64 = SplitCfg<256, 64, 4, 1>;
 };
 
 // A chunk's statistics and records take 3/8 V bytes a row (fp32: 1/2 V) against the 4 V of
 // the logits that chunk_rows bounds, so a chunk has up to 8 chunk_rows rows.
 struct FwdPlan {
-  int form;  // 0: the skinny pass; 64, 128, 256: MidCfg's tiles; -1: the main ones, compacted
+  // 0: the skinny pass; 64, 128, 256: MidCfg's tiles; kTall64: Tall64; -1: the main ones, compacted
+  int form;
   int64_t crows;
   int nstat, vtiles, ttiles;
   Strips strips;
   size_t stats, recs, tgt, total;
 };
+constexpr int kTall64 = 63;
 template <class C>
 void tile_plan(FwdPlan &p, int64_t V) {
   static_assert(C::WTM == 128 || C::WTM == 64, "strips of a wavefront's tile");
@@ -1159,6 +1165,7 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept)
   FwdPlan p{};
   const int64_t mcap = round_up(M, 256);
   p.form = M <= kSkinnyRows<TI> ? 0 : kept ? -1 : mid_form<TI>(M, V);
+  if (sizeof(TI) == 4 && p.form < 0 && M <= 64) p.form = kTall64;
   p.crows = p.form >= 0 ? M
             : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
                                              : mcap;
@@ -1169,8 +1176,11 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept)
     tile_plan<typename F::T128>(p, V);
   else if (p.form == 256)
     tile_plan<typename F::T256>(p, V);
-  else
+  else if (p.form < 0)
     tile_plan<MainCfg<TI>>(p, V);
+  if constexpr (sizeof(TI) == 4) {
+    if (p.form == kTall64) tile_plan<typename F::Tall64>(p, V);
+  }
   if (p.form == 0) {
     p.nstat = (int)((V + 31) / 32);
     p.strips = Strips{0};
@@ -1277,8 +1287,11 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
       NF_LP_MID_T(T64);
     else if (P.form == 128)
       NF_LP_MID_T(T128);
-    else
+    else if (P.form == 256)
       NF_LP_MID_T(T256);
+    if constexpr (sizeof(TI) == 4) {
+      if (P.form == kTall64) NF_LP_MID_T(Tall64);
+    }
 #undef NF_LP_MID_T
 #undef NF_LP_MID
     if ((e = check_launch("lp_logits"))) return e;

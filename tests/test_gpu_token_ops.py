@@ -296,6 +296,14 @@ def test_logprobs_match_definition(cuda, m, d, v, k, dtype):
     _logprobs_check(*_head(m, d, v, dtype, cuda, seed=m), k, ids=False)
 
 
+@pytest.mark.parametrize("m", [33, 64])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logprobs_few_rows_of_a_large_vocabulary(cuda, m, dtype):
+    note(f"logprobs few rows {m} {dtype}")
+    for d, v, k in ((72, 33001, 8), (37, 40000, 20)):
+        _logprobs_check(*_head(m, d, v, dtype, cuda, seed=m + d, grid=True), k)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_logprobs_in_chunks(cuda, dtype):
     note(f"logprobs chunks {dtype}")

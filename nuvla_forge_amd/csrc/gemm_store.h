@@ -113,11 +113,13 @@ struct GemmJob {
   int64_t dyn_base;  // the extent is *dyn - dyn_base, clamped to [0, M or K]
   int dyn_rows;      // 1: the dynamic extent is M; 0: it is K
   // bt: B is given N-major, B[k, n] at B[k * ldb + n] (columns up to ldb may
-  // be read; 16-bit inputs, DCfg only; with a K that is no multiple of 8, A's rows hold zeros up
-  // to one).  ct: C is stored
+  // be read; 16-bit inputs, DCfg only).  ct: C is stored
   // transposed, element (m, n) at C[n * ldc + m] (no K split); Cin keeps
   // [M, ldcin].
   int bt, ct;
+  // a_zeros: A's rows hold zeros from K up to a multiple of 8 (inside lda), so an N-major B
+  // with a K that is none can take A in whole vectors too; else what lies there is not read
+  int a_zeros;
   int ct_vec;     // ct with M and ldc multiples of 8: the LDS-transposed store
   int64_t ldcin;  // row stride of Cin (make_job: ldc)
 };
@@ -615,6 +617,7 @@ GemmJob<typename C::TI> make_job(const typename C::TI *A, int64_t lda, const typ
   j.dyn_base = 0;
   j.dyn_rows = 0;
   j.bt = 0;
+  j.a_zeros = 0;
   j.ct = 0;
   j.ct_vec = 0;
   j.ldcin = ldc;
@@ -625,9 +628,8 @@ template <typename TI>
 bool job_buf_ok(const GemmJob<TI> &j) {
   if (j.tiles == 0) return true;
   if (j.bt) {  // B's K rows of ldb elements, read as whole 16-byte vectors
-    // A's too: its rows hold zeros from K up to a whole vector
-    const int64_t ka = (j.K + 7) / 8 * 8;
-    return (ka == j.K || ka <= j.lda) && buf_ok<TI>(j.A, j.lda, j.M, ka) &&
+    const int64_t ka = j.a_zeros ? (j.K + 7) / 8 * 8 : j.K;
+    return ka <= j.lda && buf_ok<TI>(j.A, j.lda, j.M, ka) &&
            buf_ok<TI>(j.B, j.ldb, j.K, j.ldb);
   }
   return buf_ok<TI>(j.A, j.lda, j.M, j.K) && buf_ok<TI>(j.B, j.ldb, j.N, j.K);

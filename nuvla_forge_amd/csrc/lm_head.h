@@ -557,7 +557,10 @@ int launch_grads_tiled(const Plan &L, const StateView<TI> &S, int64_t c, int64_t
                               D, L.crows, D, V)
                : make_job<C>(S.P, L.ldp, S.Wt, L.ldwt, nullptr, S.dHc + j0 * D, NF_DTYPE_F32,
                              nullptr, D, L.crows, D, L.ldp);
-  if (Wn) jh.bt = 1;
+  if (Wn) {
+    jh.bt = 1;
+    jh.a_zeros = 1;  // E's columns V .. ldp
+  }
   jh.dyn = S.n;
   jh.dyn_base = j0;
   jh.dyn_rows = 1;  // M: the chunk's rows

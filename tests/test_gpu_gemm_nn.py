@@ -40,3 +40,22 @@ def test_gemm_nn_matches_numpy(cuda, m, n, k, ldb, ct):
     got = np64(c).T if ct else np64(c)
     assert on.rel_err(got, want) < 1e-5
 
+
+
+@pytest.mark.parametrize("m,n,k,lda", [(100, 200, 37, 40), (300, 256, 300, 320), (8, 8, 1, 8)])
+@pytest.mark.parametrize("ct", [0, 1])
+def test_gemm_nn_reads_no_column_past_k(cuda, m, n, k, lda, ct):
+    """A is a view of wider rows, K no multiple of 8: what lies beside it stays out of the
+    product, NaN as well."""
+    note(f"gemm_nn beside a view m={m} n={n} k={k} lda={lda} ct={ct}")
+    g = gen(m + n + k)
+    wide = torch.full((m, lda), float("nan"), dtype=torch.bfloat16, device=cuda)
+    wide[:, :k] = randn((m, k), g, torch.bfloat16, cuda)
+    b = randn((k, n), g, torch.bfloat16, cuda)
+    c = torch.full((n, m) if ct else (m, n), float("nan"), device=cuda)
+    L = _measure.lib()
+    _lib.check(L.nf_gemm_nn(wide.data_ptr(), lda, b.data_ptr(), n, c.data_ptr(), c.stride(0), m, n,
+                            k, ct, _lib.stream_of(b)), "nf_gemm_nn")
+    torch.cuda.synchronize()
+    got = np64(c).T if ct else np64(c)
+    assert on.rel_err(got, np64(wide)[:, :k] @ np64(b)) < 1e-5

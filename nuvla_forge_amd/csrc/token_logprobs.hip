@@ -3,8 +3,11 @@
 //   lse = log sum exp z,   logprob = z[target] - lse,
 //   entropy = -sum p (z - lse),  p = exp(z - lse),
 //   and the top_k largest z with their columns (ties: the lower column first),
-// and the gradient of logprob and entropy by hidden and weight.  The [M, V] logits are
-// never held at once; all on the caller's stream, sums in fixed orders, no atomics.
+// and the gradient of logprob and entropy by hidden and weight.  lse is held as mx + ls, mx the
+// row's largest logit and ls = log sum exp(z - mx), and z - lse formed as (z - mx) - ls: their sum
+// rounded to fp32 would lose what of ls lies below half a step of mx (3e-5 at logits of 1000).
+// The [M, V] logits are never held at once; all on the caller's stream, sums in fixed orders,
+// no atomics.
 //
 // Only valid rows (target != ignore_index, inside [0, V)) do any work: they are compacted
 // on the device and every later kernel sizes itself by the device count.
@@ -642,8 +645,9 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     const TI *W, const TI *H, int64_t V, int64_t D, const Stat *__restrict__ stats, int nstat,
     const Rec *__restrict__ recs, Strips strips, const float *__restrict__ tgt, int64_t j0,
     int64_t crows, int *n_ptr, int *rows, int *tcol, int *pos, TI *Hc, int64_t lo0,
-    const int64_t *__restrict__ targets, int64_t ignore_index, float *__restrict__ lse_out,
-    float *__restrict__ ent_out, float *__restrict__ lp_out, RowOut out) {
+    const int64_t *__restrict__ targets, int64_t ignore_index, float *__restrict__ mx_out,
+    float *__restrict__ ls_out, float *__restrict__ ent_out, float *__restrict__ lp_out,
+    RowOut out) {
   constexpr int kWaves = kFinishThreads / 64;
   __shared__ Chosen chosen_w[kWaves];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -678,7 +682,8 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
     }
     if (tc < 0) {
       if (l == 0) {
-        lse_out[row] = 0.f;
+        mx_out[row] = 0.f;
+        ls_out[row] = 0.f;
         ent_out[row] = 0.f;
         out.logprob[row] = 0.f;
         out.entropy[row] = 0.f;
@@ -700,12 +705,14 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1)
     a = join(a, Stat{__shfl_xor(a.mx, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d), 0.f});
-  const float ls = log_f32(a.s), lse = a.mx + ls, ent = ls - a.t / a.s;
+  const float ls = log_f32(a.s), ent = ls - a.t / a.s;
+  auto logprob = [&](float z) { return (z - a.mx) - ls; };
   if (l == 0) {
-    lse_out[j0 + row] = lse;
+    mx_out[j0 + row] = a.mx;
+    ls_out[j0 + row] = ls;
     ent_out[j0 + row] = ent;
-    lp_out[j0 + row] = tgt[row] - lse;
-    out.logprob[m] = tgt[row] - lse;
+    lp_out[j0 + row] = logprob(tgt[row]);
+    out.logprob[m] = logprob(tgt[row]);
     out.entropy[m] = ent;
   }
   if (K == 0) return;
@@ -733,7 +740,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
   const uint64_t redo = __ballot(need);
   if (redo == 0) {  // the first logits of the chosen strips are the row's K first
     if (l < K) {
-      out.top_lp[m * K + l] = l < found ? val - lse : __builtin_nanf("");
+      out.top_lp[m * K + l] = l < found ? logprob(val) : __builtin_nanf("");
       out.top_id[m * K + l] = l < found ? col : -1;
     }
     return;
@@ -808,7 +815,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
                      : 0;
     }
     if (q < n && place < K) {
-      out.top_lp[m * K + place] = x - lse;
+      out.top_lp[m * K + place] = logprob(x);
       out.top_id[m * K + place] = c;
     }
   }
@@ -824,7 +831,7 @@ __global__ __launch_bounds__(kFinishThreads) void lp_finish_kernel(
 // ---------------------------------------------------------------------------
 struct RowIn {
   const int *n, *rows, *tcol;        // compacted rows
-  const float *lse, *ent, *lp;       // per compacted row
+  const float *mx, *ls, *ent, *lp;   // per compacted row: lse = mx + ls
   const float *g, *h;                // upstream, per row of hidden; either may be null
 };
 
@@ -891,7 +898,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + wn * C::WTN + j * 32 + (l & 31);
-    float g = 0.f, h = 0.f, lse = 0.f, ent = 0.f;
+    float g = 0.f, h = 0.f, mx = 0.f, ls = 0.f, ent = 0.f;
     int want = -1;  // the register that holds the target, if this lane does
     const bool low = lo0 > 0 && tok >= lo0;
     const int64_t row = j0 + (low ? tok - lo0 : tok);
@@ -904,7 +911,8 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
         g = in.g ? in.g[m] : 0.f;
         h = in.h ? in.h[m] : 0.f;
       }
-      lse = in.lse[row];
+      mx = in.mx[row];
+      ls = in.ls[row];
       ent = in.ent[row];
       const int64_t loc64 = (int64_t)tc - vtile0;
       const int loc = (int)(loc64 >= 0 && loc64 < C::WTM ? loc64 : -1);
@@ -924,7 +932,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float x = acc[i][j][r] - lse;
+        const float x = (acc[i][j][r] - mx) - ls;
         // exp is 0 where x is -inf, and a NaN where it is one
         const float dz = exp_f32(x) * (a - h * fmaxf(x, kFar));
         acc[i][j][r] = i * 16 + r == want ? dz + g : dz;
@@ -938,8 +946,8 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
 
 // dz of one chunk from what the forward kept, E [crows, ldp] in fp16: with mx the strip's
 // maximum, p = E exp(mx - lse) and z - lse = log E + mx - lse.  The target's own entry is
-// formed from the row's logprob, which is exact in fp32: 1 - p of a sure token would be lost
-// in E's rounding.  A thread takes 8 columns of a row (they lie in one strip).
+// formed from the row's logprob, an fp32 value: 1 - p of a sure token would be lost in E's
+// rounding.  A thread takes 8 columns of a row (they lie in one strip).
 constexpr int kKeptThreads = 256;
 constexpr int64_t kKeptCols = (int64_t)1 << 26;  // the grid's second extent ends at 65535 blocks
 
@@ -960,11 +968,11 @@ __global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
   }
   const int64_t m = in.rows[row];
   const float g = in.g ? in.g[m] : 0.f, h = in.h ? in.h[m] : 0.f;
-  const float lse = in.lse[row], ent = in.ent[row], a = -(g + h * ent);
+  const float mx = in.mx[row], ls = in.ls[row], ent = in.ent[row], a = -(g + h * ent);
   if (c == 0) ones[row] = 1.f;
   Chunk8<f16>::load(E + row * ldp + c, v);
   if (c < V) {
-    const float o = stats[row * nstat + c / WTM].mx - lse;
+    const float o = (stats[row * nstat + c / WTM].mx - mx) - ls;
     const float f = exp_f32(o);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -1028,7 +1036,7 @@ struct State {
   bool kept, as_is;  // as_is: no transpose of weight among it
   int nstat;
   int64_t lo0;
-  size_t scal, rows, tcol, pos, lse, ent, lp, hc, e, stats, wt, hct, total;
+  size_t scal, rows, tcol, pos, mx, ls, ent, lp, hc, e, stats, wt, hct, total;
 };
 template <typename TI>
 State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool keep) {
@@ -1041,7 +1049,8 @@ State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool kee
   s.rows = take((size_t)M * sizeof(int));
   s.tcol = take((size_t)M * sizeof(int));
   s.pos = take((size_t)M * sizeof(int));
-  s.lse = take((size_t)M * sizeof(float));
+  s.mx = take((size_t)M * sizeof(float));
+  s.ls = take((size_t)M * sizeof(float));
   s.ent = take((size_t)M * sizeof(float));
   s.lp = take((size_t)M * sizeof(float));
   s.hc = take((size_t)(s.lo0 > 0 ? 2 * s.lo0 : M) * D * sizeof(TI));
@@ -1066,7 +1075,7 @@ struct View {
   int *n;
   float *inv;
   int *rows, *tcol, *pos;
-  float *lse, *ent, *lp;
+  float *mx, *ls, *ent, *lp;
   TI *Hc, *Wt, *Hct;
   f16 *E;
   Stat *stats;
@@ -1076,7 +1085,8 @@ struct View {
         rows(reinterpret_cast<int *>(s + L.rows)),
         tcol(reinterpret_cast<int *>(s + L.tcol)),
         pos(reinterpret_cast<int *>(s + L.pos)),
-        lse(reinterpret_cast<float *>(s + L.lse)),
+        mx(reinterpret_cast<float *>(s + L.mx)),
+        ls(reinterpret_cast<float *>(s + L.ls)),
         ent(reinterpret_cast<float *>(s + L.ent)),
         lp(reinterpret_cast<float *>(s + L.lp)),
         Hc(reinterpret_cast<TI *>(s + L.hc)),
@@ -1215,7 +1225,7 @@ int launch_finish(const TI *W, const TI *H, int64_t V, int64_t D, const FwdPlan 
 #define NF_LP_FINISH(VK, NR)                                                                   \
   lp_finish_kernel<TI, VK, NR><<<grid, kFinishThreads, 0, s>>>(                                \
       W, H, V, D, stats, P.nstat, recs, P.strips, tgt, j0, rows, S.n, S.rows, S.tcol, S.pos,   \
-      hc, lo0, targets, ignore_index, S.lse, S.ent, S.lp, out)
+      hc, lo0, targets, ignore_index, S.mx, S.ls, S.ent, S.lp, out)
   if (vk && nrec <= 64 * 16)
     NF_LP_FINISH(true, 16);
   else if (vk && nrec <= 64 * 32)
@@ -1379,7 +1389,7 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
   int *const two = S.n;
   if (lo0 == 0) S.n = K.n;  // else *two, by lp_dz
   float *part = reinterpret_cast<float *>(ws + L.s_total);
-  const RowIn in{K.n, K.rows, K.tcol, K.lse, K.ent, K.lp, g, h};
+  const RowIn in{K.n, K.rows, K.tcol, K.mx, K.ls, K.ent, K.lp, g, h};
   TI *const PT = L.single ? nullptr : S.PT;
   gemm::TpJobs tp{};
   const gemm::TpJobs none{};

@@ -1,0 +1,59 @@
+"""Token log probabilities, embedding lookup and dropout on the GPU where few calls go: large
+logits, very peaked rows, second derivatives, operands that are not aligned, sizes at the borders
+between kernels.  Against 64 bits, within bounds derived beside each.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from nuvla_forge_amd.kernels import chunked_token_logprobs
+
+from .helpers import gen, note
+from .token_ops_ref import logprobs64
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F16 = torch.bfloat16, torch.float32, torch.float16
+
+
+# ---------------------------------------------------------------------------
+# token log probabilities
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m", [3, 20, 100, 300])
+def test_logprobs_do_not_depend_on_a_shift_of_the_logits(cuda, m, dtype):
+    """960 added to every logit changes nothing: the values of sure tokens too, whose log
+    probability is far below a step of the logits.
+
+    h in 1/16 and w in 1/1024: every logit is exact (below 2^10 in steps of 2^-14), and so is its
+    difference from the largest.  What is left is exp's, log's and their arguments' roundings,
+    2^-21 of 1 + |x|, and those of a sum of V terms in 64 or more pieces, (V / 64 + 64) 2^-24."""
+    note(f"logprobs shift {m} {dtype}")
+    g, d, v, k = gen(m), 16, 3001, 8
+    h, w = torch.randn(m, d, generator=g), torch.randn(v, d, generator=g) * 0.25
+    t = torch.randint(0, v, (m,), generator=g)
+    h[:, 0] = 0.0
+    h[:, 1] = torch.where(torch.arange(m) % 3 == 0, 4.0, 0.0)  # a third of the rows: sure of one
+    w[:, 1] = 0.0
+    sure = torch.arange(v) % 997 == 5
+    w[sure, 1] = 3.0 + 2.5 * torch.arange(int(sure.sum()))
+    t[::3] = int(sure.nonzero()[-1])
+    h, w = ((x * s).round().div(s).to(dtype).to(cuda) for x, s in ((h, 16), (w, 1024)))
+    t, up = t.to(cuda), torch.randn(2, m, generator=g).to(cuda)
+    ref = logprobs64(h, w, t, *up, k)  # without the shift
+    h[:, 0], w[:, 0] = 32.0, 30.0
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, top_k=k)
+    tol = (v / 64 + 64) * 2.0 ** -24
+    for x, y in ((out.logprobs, ref["logprobs"]), (out.top_logprobs, ref["top_logprobs"])):
+        assert ((x.double() - y).abs() <= tol + 2.0 ** -21 * (1 + y.abs())).all()
+    assert torch.equal(out.top_ids, ref["top_ids"])
+    assert ((out.entropy.double() - ref["entropy"]).abs() <= ref["tol_ent"]).all()
+    # the gradients but for the shift's own column are those without it
+    for x, name in zip(torch.autograd.grad([out.logprobs, out.entropy], [h, w], list(up)),
+                       ("dh", "dw")):
+        off = (x.double() - ref[name]).abs()[:, 1:]
+        assert (off <= ref["tol_" + name][:, 1:]).all(), (name, off.max())

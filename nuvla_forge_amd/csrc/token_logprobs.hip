@@ -140,6 +140,8 @@ __device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, 
   return t != ignore_index && t >= 0 && t < V ? (int)t : -1;
 }
 
+constexpr float kKeptScale = 32768.f;
+
 // One block tile: acc = W_tile Hc_tile^T (rows: vocabulary, columns: tokens), so a lane
 // holds 16 TM logits of each of its TN tokens and the strip's values are reductions in
 // registers.  What bounds it: the products at D 2048 (bf16, 3686 rows, V 32000: 455 us, 1.06
@@ -148,9 +150,11 @@ __device__ __forceinline__ int target_column(const int64_t *targets, int64_t m, 
 // Two blocks of half the token columns a CU, 32 k a stage, to overlap it: level without records
 // (613 us against 608), 766 against 788 with them, and 20% slower at D 2048.
 // stats [crows, nstat], recs [crows, nstat * WTM / 32], tgt [crows].
-// KEEP (16-bit inputs): exp(z - mx), mx the strip's maximum, is kept for the backward in
-// fp16, E [crows, ldp]: half a step of 2^-11 of each, and what is below 2^-24 of the strip's
-// largest is lost.  With bf16, 2^-8, its rounding would add to dz's own.  Blocks past the
+// KEEP (16-bit inputs): kKeptScale exp(z - mx), mx the strip's maximum, is kept for the backward
+// in fp16, E [crows, ldp]: half a step of 2^-11 of each down to 2^-29 of the strip's largest (20
+// nats below it), half of 2^-39 of the largest of what is below that.  With bf16, 2^-8, its
+// rounding would add to dz's own; the scale, a power of two, puts the largest at the upper end of
+// fp16's range.  Blocks past the
 // tiles run the transposes of `tp`.  `targets`: Hc is hidden as it lies, all crows rows of it
 // (a middling number of rows, which are not compacted).
 template <class C, bool BUF, bool SB, bool TOP, bool KEEP>
@@ -257,7 +261,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
         const float e = exp_f32(x);
         s += e;
         t += (KEEP ? fmaxf(x, kFar) : x) * e;
-        acc[i][j][r] = KEEP ? e : x;
+        acc[i][j][r] = KEEP ? e * kKeptScale : x;
       }
     // -inf * 0 is a NaN: without KEEP, where x is still there, a strip with a logit of -inf (or
     // past the vocabulary) and no NaN is summed again with x bounded.  Bounding every x costs 3%
@@ -945,7 +949,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
 }
 
 // dz of one chunk from what the forward kept, E [crows, ldp] in fp16: with mx the strip's
-// maximum, p = E exp(mx - lse) and z - lse = log E + mx - lse.  The target's own entry is
+// maximum and e = E / kKeptScale, p = e exp(mx - lse) and z - lse = log e + mx - lse.  The target's own entry is
 // formed from the row's logprob, an fp32 value: 1 - p of a sure token would be lost in E's
 // rounding.  A thread takes 8 columns of a row (they lie in one strip).
 constexpr int kKeptThreads = 256;
@@ -976,6 +980,7 @@ __global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
     const float f = exp_f32(o);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      v[i] *= 1.f / kKeptScale;
       // log 0 = -inf goes with p = 0; a NaN stays one through p
       const float x = h != 0.f ? fmaxf(log_f32(v[i]) + o, kFar) : 0.f;
       v[i] = v[i] * f * (a - h * x);

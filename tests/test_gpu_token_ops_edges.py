@@ -57,3 +57,40 @@ def test_logprobs_do_not_depend_on_a_shift_of_the_logits(cuda, m, dtype):
                        ("dh", "dw")):
         off = (x.double() - ref[name]).abs()[:, 1:]
         assert (off <= ref["tol_" + name][:, 1:]).all(), (name, off.max())
+
+
+@pytest.mark.parametrize("chunk_size", [1024, 1])
+@pytest.mark.parametrize("far", [9.0, 13.0, 18.0, 24.0])
+def test_logprobs_gradient_of_tokens_far_below_a_sure_one(cuda, far, chunk_size):
+    """Every row is sure of one token, and the others are ``far`` nats below: those next to it
+    (of its strip) have their gradient in weight like those far away, whether or not what the
+    forward kept of the logits (exp(z - strip maximum) in 16 bits) is what the backward reads.
+
+    Every row is alike (h, z), so dw[v] = h sum_m dz[m, v] with no cancellation between the p of
+    different rows.  dz of a token is off by p's error, r = 2^-8 for its rounding to bf16, and
+    for what was kept 2^-11 of itself or, more than 20 nats below the strip's largest, 2^-40 of that;
+    p's by exp's argument, 2^-21 (1 + far), and by the sum's roundings, (V / 64 + 64) 2^-24."""
+    note(f"logprobs far below {far} {chunk_size}")
+    m, d, v, at = 300, 8, 4099, 1000
+    h, w = torch.zeros(m, d), torch.zeros(v, d)
+    h[:, 0] = 1.0
+    w[at, 0] = far  # exact in bf16
+    w[:, 1] = torch.arange(v) % 7 / 8.0  # h[:, 1] is 0: seen by dh alone
+    h, w = (x.to(BF16).to(cuda).requires_grad_(True) for x in (h, w))
+    t = torch.full((m,), at, device=cuda)
+    g = torch.linspace(0.5, 1.5, m, device=cuda)
+    out = chunked_token_logprobs(h, w, t, chunk_size=chunk_size)
+    (dw,) = torch.autograd.grad(out.logprobs, w, g)
+    z = w.detach().double()[:, 0]
+    p = (z - torch.logsumexp(z, 0)).exp()
+    want = -p * g.double().sum()
+    want[at] += g.double().sum()
+    size = p * g.double().sum()
+    rel = 2.0 ** -8 + 2.0 ** -11 + 2 * ((v / 64 + 64) * 2.0 ** -24 + 2.0 ** -21 * (1 + far))
+    tol = rel * size + 2.0 ** -40 * g.double().sum() + (m + 2) * 2.0 ** -24 * size
+    tol += 2.0 ** -8 * (want.abs() + tol)  # dw's own rounding
+    # the sure token's 1 - p, from its fp32 log probability: 2^-23 and the sum's roundings of 1
+    tol[at] += 2 * (v / 64 + 66) * 2.0 ** -24 * g.double().sum()
+    off = (dw.double()[:, 0] - want).abs()
+    assert (off <= tol).all(), (off / tol).max()
+    assert (dw[:, 1:] == 0).all()

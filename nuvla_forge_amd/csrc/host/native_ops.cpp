@@ -15,6 +15,8 @@
 // autograd frees them after the backward.  Nothing is kept between calls.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -57,6 +59,30 @@ void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Tensor bytes(size_t n, const Tensor &like) {
   return at::empty({(int64_t)(n > 0 ? n : 1)}, like.options().dtype(at::kByte));
+}
+
+// What a backward returns, `recording`: under create_graph.  The kernels record nothing, so a
+// derivative taken through their results would leave terms out without a word; the results get a
+// node that raises when one reaches it.  Its edges are the backward's own and those of the
+// upstream gradients, so that it is reached by whichever of them the derivative is taken.
+variable_list first_order_only(const char *op, bool recording, const variable_list &grads,
+                               variable_list out) {
+  if (!recording) return out;
+  torch::autograd::edge_list edges;
+  if (const auto here = torch::autograd::get_current_node()) edges = here->next_edges();
+  for (const Tensor &g : grads)
+    if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+  const std::shared_ptr<torch::autograd::Node> node(
+      new torch::autograd::Error(std::string(op) + ": second derivatives are not supported on the "
+                                 "device; force_reference=True runs a formulation that has them",
+                                 std::move(edges)),
+      torch::autograd::deleteNode);
+  for (Tensor &t : out)
+    if (t.defined()) {
+      t = t.detach();
+      torch::autograd::set_history(t, node);
+    }
+  return out;
 }
 
 // Nothing that could see or replace the ops of the general path is active.
@@ -428,7 +454,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
                                 (const float *)ptr(g[1]), ptr(res[0]), code_of(th), ptr(res[1]),
                                 code_of(tw), ws.data_ptr(), nw, stream_of(w)),
           "nf_token_logprobs_bwd");
-    return res;
+    return first_order_only("chunked_token_logprobs", at::GradMode::is_enabled(), grads,
+                            std::move(res));
   }
 };
 
@@ -745,7 +772,29 @@ PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// op's name, the upstream gradients and the results of a backward in Python (tuples of tensors and
+// Nones) -> the results under create_graph (see first_order_only above)
+PyObject *py_first_order_only(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 3 && PyUnicode_Check(args[0]) && PyTuple_Check(args[1]) &&
+                       PyTuple_Check(args[2]),
+                   "first_order_only: (name, gradients, results) expected");
+  variable_list v[2];
+  for (int k = 0; k < 2; ++k)
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[1 + k]); ++i) {
+      PyObject *const o = PyTuple_GET_ITEM(args[1 + k], i);
+      v[k].push_back(THPVariable_Check(o) ? THPVariable_Unpack(o) : Tensor());
+    }
+  const variable_list r = first_order_only(PyUnicode_AsUTF8(args[0]), true, v[0], v[1]);
+  PyObject *tuple = PyTuple_New((Py_ssize_t)r.size());
+  if (!tuple) return nullptr;
+  for (size_t i = 0; i < r.size(); ++i) PyTuple_SET_ITEM(tuple, (Py_ssize_t)i, THPVariable_Wrap(r[i]));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
+    {"first_order_only", (PyCFunction)(void (*)(void))py_first_order_only, METH_FASTCALL, nullptr},
     {"seam", (PyCFunction)(void (*)(void))py_seam, METH_FASTCALL, nullptr},
     {"swiglu", (PyCFunction)(void (*)(void))py_swiglu, METH_FASTCALL, nullptr},
     {"gate_up", (PyCFunction)(void (*)(void))py_gate_up, METH_FASTCALL, nullptr},

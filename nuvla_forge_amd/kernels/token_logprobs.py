@@ -29,7 +29,7 @@ import torch
 from .. import _lib
 from .chunked_ce import _compute_dtype, chunk_rows_for
 from .reference import token_logprobs_ref
-from .utils import check_devices, device_of, use_fused
+from .utils import check_devices, device_of, first_order_only, use_fused
 
 MAX_TOP_K = 32
 
@@ -132,8 +132,9 @@ class _TokenLogprobs(torch.autograd.Function):
                                         ws_bytes, _lib.stream_of(w)),
                 "nf_token_logprobs_bwd",
             )
-        return (None if oh is None else oh.to(ctx.types[0]),
-                None if ow is None else ow.to(ctx.types[1]), *none[2:])
+        return first_order_only("chunked_token_logprobs", (g_lp, g_ent),
+                                (None if oh is None else oh.to(ctx.types[0]),
+                                 None if ow is None else ow.to(ctx.types[1]), *none[2:]))
 
 
 def chunked_token_logprobs(
@@ -164,6 +165,8 @@ def chunked_token_logprobs(
         first).  Rows left out give 0, their alternatives token -1, and no gradient.
         ``logprobs`` and ``entropy`` carry gradients, the alternatives none.  A row with a
         NaN among its logits has NaN values, and -1 for alternatives it cannot order.
+
+    Second derivatives are not supported on the device: taking one raises.
 
     Host tensors run the eager row-chunk loop.
     """

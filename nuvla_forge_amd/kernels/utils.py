@@ -94,6 +94,14 @@ def use_fused(t: torch.Tensor, op: str, force_reference: bool = False) -> bool:
     return True
 
 
+def first_order_only(op: str, grads: tuple, results: tuple) -> tuple:
+    """``results`` of ``op``'s backward, for its upstream ``grads`` (either may hold None).
+
+    Under ``create_graph=True`` they raise when a second derivative is taken through them: the
+    kernels record nothing, and the terms would otherwise be left out without a word."""
+    return _lib.native().first_order_only(op, grads, results) if torch.is_grad_enabled() else results
+
+
 class device_of:
     """Make t's device current for the launch (no-op when it already is).
 

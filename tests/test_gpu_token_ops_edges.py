@@ -10,9 +10,10 @@ import math
 import pytest
 import torch
 
+from nuvla_forge_amd import _lib
 from nuvla_forge_amd.kernels import chunked_token_logprobs
 
-from .helpers import gen, note
+from .helpers import gen, note, randn
 from .token_ops_ref import logprobs64
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,44 @@ def test_logprobs_gradient_of_tokens_far_below_a_sure_one(cuda, far, chunk_size)
     off = (dw.double()[:, 0] - want).abs()
     assert (off <= tol).all(), (off / tol).max()
     assert (dw[:, 1:] == 0).all()
+
+
+class _NoNative:
+    """No plain call is taken by the C++ host side: each runs its Function in Python."""
+
+    def __init__(self, module):
+        self.first_order_only = module.first_order_only
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.fixture(params=["native", "python"])
+def route(request, monkeypatch):
+    """Both host sides of a call."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "native", lambda m=_lib.native(): _NoNative(m))
+    return request.param
+
+
+@pytest.mark.parametrize("m, dtype", [(5, BF16), (300, BF16), (40, F32)])
+def test_logprobs_second_derivatives_raise(cuda, route, m, dtype):
+    """Under create_graph the gradients are those without it; a derivative through them raises
+    beside terms that have one, and by the upstream gradient."""
+    note(f"logprobs second derivative {m} {dtype} {route}")
+    g = gen(m)
+    h, w = (randn(s, g, dtype, cuda).requires_grad_(True) for s in ((m, 16), (50, 16)))
+    t = torch.randint(0, 50, (m,), generator=g).to(cuda)
+    up = randn((m,), g, F32, cuda).requires_grad_(True)
+    want = torch.autograd.grad(chunked_token_logprobs(h, w, t).logprobs, [h, w], up)
+    got = torch.autograd.grad(chunked_token_logprobs(h, w, t).logprobs, [h, w], up,
+                              create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for leaf in (h, w, up):
+        with pytest.raises(RuntimeError, match="chunked_token_logprobs: second derivatives"):
+            torch.autograd.grad((got[0].float() ** 2).sum() + (h * h).sum(), leaf,
+                                retain_graph=True, allow_unused=True)
+    loss = chunked_token_logprobs(h, w, t).entropy.sum()
+    (dw,) = torch.autograd.grad(loss, w, create_graph=True)
+    with pytest.raises(RuntimeError, match="chunked_token_logprobs: second derivatives"):
+        (dw.float().sum() + (w * w).sum()).backward()

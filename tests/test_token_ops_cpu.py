@@ -18,7 +18,7 @@ from nuvla_forge_amd.kernels import (
     fused_dropout,
 )
 from nuvla_forge_amd.kernels.reference import _philox_words, dropout_keep
-from nuvla_forge_amd.kernels.utils import DeviceMismatchError
+from nuvla_forge_amd.kernels.utils import DeviceMismatchError, first_order_only
 
 from .token_ops_ref import logprobs64
 
@@ -274,3 +274,46 @@ def test_logprobs_workspace_holds_what_a_kept_forward_writes(m, d, v, chunk_rows
     assert L.nf_token_logprobs_state_bytes(m, d, v, chunk_rows, 1, 1) >= 2 * mcap * v
     assert (L.nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, 5, 1)
             >= mcap * tiles * 8 * 8 + mcap * 4)
+
+
+# ---------------------------------------------------------------------------
+# second derivatives
+# ---------------------------------------------------------------------------
+class _Cube(torch.autograd.Function):
+    """x^3 by code that autograd does not see, as the kernels' gradients are."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return x ** 3
+
+    @staticmethod
+    def backward(ctx, g):
+        (x,) = ctx.saved_tensors
+        dx = torch.from_numpy(3 * x.detach().numpy() ** 2 * g.detach().numpy())
+        return first_order_only("cube", (g,), (dx,))[0]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_first_order_only(graph):
+    """The gradient under create_graph has its value and may be used; a derivative through it
+    raises, by the input and by the upstream gradient, beside other terms too."""
+    x = torch.tensor([1.0, -2.0], requires_grad=True)
+    g = torch.tensor([0.5, 4.0], requires_grad=True)
+    y = x + 0  # not a leaf
+    out = _Cube.apply(y) + x
+    (dx,) = torch.autograd.grad(out, x, g, create_graph=graph)
+    assert torch.equal(dx.detach(), g.detach() * (3 * x.detach() ** 2 + 1))
+    assert dx.requires_grad == graph
+    if graph:
+        for leaf in (x, g, y):
+            with pytest.raises(RuntimeError, match="cube: second derivatives"):
+                torch.autograd.grad((dx + x * y).sum(), leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="cube: second derivatives"):
+            (dx ** 2).sum().backward()
+        (dx2,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="cube: second derivatives"):
+            (dx2 * x).sum().backward()
+        other = torch.ones(2, requires_grad=True)  # what does not go through it is free
+        (d,) = torch.autograd.grad((dx.detach() * other).sum(), other)
+        assert torch.equal(d, dx.detach())

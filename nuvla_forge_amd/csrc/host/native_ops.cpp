@@ -521,7 +521,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x,
                         const std::optional<Tensor> &residual,
                         const std::optional<Tensor> &seed_in, int64_t threshold, int64_t seed,
-                        int64_t offset) {
+                        int64_t offset, int64_t out_t) {
     const c10::DeviceGuard guard(x.device());
     Tensor r, seed_t;
     if (residual) r = residual->contiguous();
@@ -530,12 +530,11 @@ struct Dropout : torch::autograd::Function<Dropout> {
     ctx->saved_data["s"] =
         std::vector<int64_t>{threshold, seed, offset, (int64_t)x.scalar_type(), seed_t.defined(),
                              r.defined()};
-    return run(x.contiguous(), r, r.defined() ? r.scalar_type() : x.scalar_type(), threshold,
-               seed_t, seed, offset);
+    return run(x.contiguous(), r, (at::ScalarType)out_t, threshold, seed_t, seed, offset);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto s = ctx->saved_data["s"].toIntVector();
-    variable_list res(6);
+    variable_list res(7);
     // an argument that was left out has no edge: the residual's is the second, if there is one
     if (s[5] && ctx->needs_input_grad(1)) res[1] = grads[0];
     if (!ctx->needs_input_grad(0)) return res;
@@ -546,7 +545,12 @@ struct Dropout : torch::autograd::Function<Dropout> {
                         "fused_dropout backward: dout is not on the forward's device");
     }
     const c10::DeviceGuard guard(grads[0].device());
-    res[0] = run(grads[0].contiguous(), Tensor(), (at::ScalarType)s[3], s[0], seed_t, s[1], s[2]);
+    if (at::GradMode::is_enabled() && grads[0].requires_grad())  // dx is linear in dout
+      res[0] = Dropout::apply(grads[0], std::optional<Tensor>(),
+                              s[4] ? std::optional<Tensor>(seed_t) : std::nullopt, s[0], s[1],
+                              s[2], s[3]);
+    else
+      res[0] = run(grads[0].contiguous(), Tensor(), (at::ScalarType)s[3], s[0], seed_t, s[1], s[2]);
     return res;
   }
 };
@@ -760,14 +764,15 @@ PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (!plain(x, dev) || code_of(x) < 0 || x.numel() == 0 || !ints(args, 2, threshold) ||
       !ints(args, 4, offset) || threshold[0] < 0 || threshold[0] > 65536 || offset[0] < 0)
     Py_RETURN_NONE;
+  const at::ScalarType out_t = r.defined() ? r.scalar_type() : x.scalar_type();
   auto given = [](const Tensor &v) { return v.defined() ? std::optional<Tensor>(v) : std::nullopt; };
   return THPVariable_Wrap(unlocked([&]() -> Tensor {
     if (wants_grad({&x, &r}))
-      return Dropout::apply(x, given(r), given(seed_t), threshold[0], seed[0], offset[0]);
+      return Dropout::apply(x, given(r), given(seed_t), threshold[0], seed[0], offset[0],
+                            (int64_t)out_t);
     const c10::DeviceGuard guard(dev);
     const Tensor rc = r.defined() ? r.contiguous() : r;
-    return Dropout::run(x.contiguous(), rc, rc.defined() ? rc.scalar_type() : x.scalar_type(),
-                        threshold[0], seed_t, seed[0], offset[0]);
+    return Dropout::run(x.contiguous(), rc, out_t, threshold[0], seed_t, seed[0], offset[0]);
   }));
   END_HANDLE_TH_ERRORS
 }

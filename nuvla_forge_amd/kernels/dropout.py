@@ -66,10 +66,10 @@ def _launch(x, residual, out, threshold, seed, offset):
 
 class _FusedDropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, threshold, seed, offset):
+    def forward(ctx, x, residual, threshold, seed, offset, out_dtype):
         x = x.contiguous()
         r = None if residual is None else residual.contiguous()
-        out = torch.empty(x.shape, dtype=x.dtype if r is None else r.dtype, device=x.device)
+        out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
         _launch(x, r, out, threshold, seed, offset)
         ctx.call = (threshold, seed if not isinstance(seed, torch.Tensor) else None, offset)
         ctx.x_dtype = x.dtype
@@ -83,11 +83,9 @@ class _FusedDropout(torch.autograd.Function):
         if seed is None:
             (seed,) = ctx.saved_tensors
         dx = None
-        if ctx.needs_input_grad[0]:
-            g = dout.contiguous()
-            dx = torch.empty(g.shape, dtype=ctx.x_dtype, device=g.device)
-            _launch(g, None, dx, threshold, seed, offset)
-        return dx, dout if ctx.needs_input_grad[1] else None, None, None, None
+        if ctx.needs_input_grad[0]:  # linear in dout, and so the operator once more
+            dx = _FusedDropout.apply(dout, None, threshold, seed, offset, ctx.x_dtype)
+        return dx, dout if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
 def fused_dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: int = 0,
@@ -108,7 +106,7 @@ def fused_dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: i
     A dropped element gives 0 (or the residual) whatever x holds there.  The mask is
     computed again in the backward, from the seed as it was in the forward: a seed
     tensor that was changed in place in between raises.  Host tensors take the eager
-    formulation, with the same mask.
+    formulation, with the same mask.  Derivatives of any order.
     """
     threshold = dropout_threshold(p)
     fused = use_fused(x, "fused_dropout", force_reference)
@@ -119,4 +117,5 @@ def fused_dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, offset: i
     _check(x, seed, offset, residual)
     if not fused:
         return dropout_ref(x, threshold, seed, offset, residual)
-    return _FusedDropout.apply(x, residual, threshold, seed, offset)
+    return _FusedDropout.apply(x, residual, threshold, seed, offset,
+                               x.dtype if residual is None else residual.dtype)

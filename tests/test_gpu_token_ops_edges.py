@@ -11,7 +11,9 @@ import pytest
 import torch
 
 from nuvla_forge_amd import _lib
-from nuvla_forge_amd.kernels import chunked_token_logprobs
+from nuvla_forge_amd.kernels import chunked_token_logprobs, fused_dropout
+from nuvla_forge_amd.kernels.dropout import dropout_threshold
+from nuvla_forge_amd.kernels.reference import dropout_keep
 
 from .helpers import gen, note, randn
 from .token_ops_ref import logprobs64
@@ -136,3 +138,41 @@ def test_logprobs_second_derivatives_raise(cuda, route, m, dtype):
     (dw,) = torch.autograd.grad(loss, w, create_graph=True)
     with pytest.raises(RuntimeError, match="chunked_token_logprobs: second derivatives"):
         (dw.float().sum() + (w * w).sum()).backward()
+
+
+# ---------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("xt, rt", [(F32, None), (F32, F32), (BF16, F32)])
+@pytest.mark.parametrize("by_tensor", [False, True])
+def test_dropout_second_derivatives(cuda, route, xt, rt, by_tensor):
+    """sum((r + drop(x))^3) with r = x (or without a residual): first, second and third
+    derivatives by x.  With f the factor of an element (0 where dropped) and s = f + 1 (f without
+    a residual), y = s x and the k-th derivative is s^k times that of y^3.
+
+    A gradient passes through a handful of fp32 products and sums, each 2^-24 of the terms'
+    absolute sum, and (bf16) roundings of the branch's value and of its gradient, 2^-8 each of its
+    share."""
+    note(f"dropout second derivative {xt} {rt} {by_tensor} {route}")
+    g = gen(3)
+    x = randn((33, 40), g, xt, cuda).float().requires_grad_(True)
+    v = randn((33, 40), g, F32, cuda)
+    seed = torch.tensor([21], device=cuda) if by_tensor else 21
+    y = fused_dropout(x.to(xt), 0.25, seed, offset=4, residual=None if rt is None else x)
+    t = dropout_threshold(0.25)
+    f = dropout_keep(x.shape, t, 21, 4, "cpu").to(cuda).double() * (65536 / (65536 - t))
+    s = f if rt is None else f + 1
+    xd, vd, step = x.detach().double(), v.double(), 2.0 ** -7 if xt == BF16 else 2.0 ** -20
+    (d1,) = torch.autograd.grad((y.float() ** 3).sum(), x, create_graph=True)
+    (d2,) = torch.autograd.grad((d1 * v).sum(), x, create_graph=True)
+    (d3,) = torch.autograd.grad((d2 * v).sum(), x)
+    for got, want in ((d1, 3 * s ** 3 * xd ** 2), (d2, 6 * s ** 3 * xd * vd),
+                      (d3, 6 * s ** 3 * vd ** 2)):
+        assert ((got.double() - want).abs() <= 4 * step * want.abs() + 1e-30).all()
+    # the gradient of what was a gradient: dout's own
+    up = randn((33, 40), g, y.dtype, cuda).requires_grad_(True)
+    y = fused_dropout(x.to(xt), 0.25, seed, offset=4, residual=None if rt is None else x)
+    (dx,) = torch.autograd.grad(y, x, up, create_graph=True)
+    (du,) = torch.autograd.grad(dx, up, v)
+    assert du.dtype == up.dtype
+    assert ((du.double() - s * vd).abs() <= 4 * step * (s * vd).abs()).all()

@@ -462,6 +462,26 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 // ---------------------------------------------------------------------------
 // embedding lookup
 // ---------------------------------------------------------------------------
+// The lookup's gradient as an operator of its own: linear in dout, its gradient the lookup again.
+struct EmbeddingGrad : torch::autograd::Function<EmbeddingGrad> {
+  static Tensor run(const Tensor &dout, const Tensor &ids, int64_t v, double scale, int64_t pad,
+                    at::ScalarType table_t) {
+    const int64_t m = ids.numel(), d = dout.size(-1);
+    const Tensor g = dout.contiguous();
+    Tensor dtable = at::empty({v, d}, g.options().dtype(table_t).requires_grad(false));
+    const size_t nw = nf_embedding_bwd_workspace(m, d, v);
+    Tensor ws = bytes(nw, ids);
+    check(nf_embedding_bwd(g.data_ptr(), ids.data_ptr<int64_t>(), pad, (float)scale, m, d, v,
+                           dtable.data_ptr(), code_of(g), code_of(table_t), ws.data_ptr(), nw,
+                           stream_of(g)),
+          "nf_embedding_bwd");
+    return dtable;
+  }
+  static Tensor forward(AutogradContext *ctx, const Tensor &dout, const Tensor &ids, int64_t v,
+                        double scale, int64_t pad, int64_t table_t);
+  static variable_list backward(AutogradContext *ctx, variable_list grads);
+};
+
 struct Embedding : torch::autograd::Function<Embedding> {
   static Tensor run(const Tensor &ids, const Tensor &table, double scale, at::ScalarType out_t) {
     const int64_t m = ids.numel(), v = table.size(0), d = table.size(1);
@@ -479,8 +499,8 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const c10::DeviceGuard guard(table.device());
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["s"] = std::vector<int64_t>{table.size(0), table.size(1), pad,
-                                                (int64_t)table.scalar_type()};
+    ctx->saved_data["s"] =
+        std::vector<int64_t>{table.size(0), pad, (int64_t)table.scalar_type()};
     return run(ids, table, scale, (at::ScalarType)out_t);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -488,22 +508,40 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const Tensor &ids = saved[0];
     const c10::DeviceGuard guard(ids.device());
     const auto s = ctx->saved_data["s"].toIntVector();
-    const int64_t m = ids.numel(), v = s[0], d = s[1];
-    const auto tt = (at::ScalarType)s[3];
+    const double scale = ctx->saved_data["scale"].toDouble();
     TORCH_CHECK_VALUE(grads[0].device() == ids.device(),
                       "embedding_lookup backward: dout is not on the forward's device");
-    const Tensor g = grads[0].contiguous();
-    Tensor dtable = at::empty({v, d}, g.options().dtype(tt));
-    const size_t nw = nf_embedding_bwd_workspace(m, d, v);
-    Tensor ws = bytes(nw, ids);
-    check(nf_embedding_bwd(g.data_ptr(), ids.data_ptr<int64_t>(), s[2],
-                           (float)ctx->saved_data["scale"].toDouble(), m, d, v,
-                           dtable.data_ptr(), code_of(g), code_of(tt), ws.data_ptr(), nw,
-                           stream_of(g)),
-          "nf_embedding_bwd");
+    const bool recording = at::GradMode::is_enabled() && grads[0].requires_grad();
+    const Tensor dtable =
+        recording ? EmbeddingGrad::apply(grads[0], ids, s[0], scale, s[1], s[2])
+                  : EmbeddingGrad::run(grads[0], ids, s[0], scale, s[1], (at::ScalarType)s[2]);
     return {Tensor(), dtable, Tensor(), Tensor(), Tensor()};
   }
 };
+
+Tensor EmbeddingGrad::forward(AutogradContext *ctx, const Tensor &dout, const Tensor &ids,
+                              int64_t v, double scale, int64_t pad, int64_t table_t) {
+  const c10::DeviceGuard guard(ids.device());
+  ctx->save_for_backward({ids});
+  ctx->saved_data["scale"] = scale;
+  ctx->saved_data["s"] = std::vector<int64_t>{pad, (int64_t)dout.scalar_type()};
+  return run(dout, ids, v, scale, pad, (at::ScalarType)table_t);
+}
+variable_list EmbeddingGrad::backward(AutogradContext *ctx, variable_list grads) {
+  const variable_list saved = ctx->get_saved_variables();
+  const c10::DeviceGuard guard(saved[0].device());
+  const auto s = ctx->saved_data["s"].toIntVector();
+  // the padding id's rows, which gave nothing, get nothing: as those outside the table
+  const Tensor ids = s[0] < 0 ? saved[0] : saved[0].masked_fill(saved[0].eq(s[0]), -1);
+  TORCH_CHECK_VALUE(grads[0].device() == ids.device(),
+                    "embedding_lookup backward: a gradient is not on the forward's device");
+  const Tensor g = grads[0].contiguous();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const bool recording = at::GradMode::is_enabled() && g.requires_grad();
+  const Tensor ddout = recording ? Embedding::apply(ids, g, scale, -1, s[1])
+                                 : Embedding::run(ids, g, scale, (at::ScalarType)s[1]);
+  return {ddout, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+}
 
 // ---------------------------------------------------------------------------
 // dropout

@@ -40,8 +40,16 @@ class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
-        v, d, scale, pad, dtype = ctx.call
-        g = dout.reshape(-1, d).contiguous()
+        g = dout.reshape(-1, ctx.call[1])
+        return None, _EmbeddingGrad.apply(g, flat, *ctx.call), None, None, None
+
+
+class _EmbeddingGrad(torch.autograd.Function):
+    """The lookup's gradient, [V, D]: linear in dout, its own gradient the lookup again."""
+
+    @staticmethod
+    def forward(ctx, dout, flat, v, d, scale, pad, dtype):
+        g = dout.contiguous()
         check_devices("embedding_lookup backward", "the forward's ids", dict(dout=g),
                       device=flat.device)
         m = flat.numel()
@@ -57,7 +65,17 @@ class _EmbeddingLookup(torch.autograd.Function):
                                    _lib.stream_of(g)),
                 "nf_embedding_bwd",
             )
-        return None, dtable, None, None, None
+        ctx.save_for_backward(flat)
+        ctx.call = (scale, pad, g.dtype)
+        return dtable
+
+    @staticmethod
+    def backward(ctx, gg):
+        (flat,) = ctx.saved_tensors
+        scale, pad, dtype = ctx.call
+        # the padding id's rows, which gave nothing, get nothing: as those outside the table
+        ids = flat if pad < 0 else flat.masked_fill(flat == pad, -1)
+        return _EmbeddingLookup.apply(ids, gg, scale, None, dtype), *(None,) * 6
 
 
 def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
@@ -78,8 +96,8 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         [*ids.shape, D].  An id outside [0, V) gives a row of zeros and no gradient: the
         call reads nothing back to the host, so it cannot raise for one.
 
-    The gradient has the table's type and is the same bits every run.  Host tensors take
-    the eager formulation.
+    The gradient has the table's type and is the same bits every run; derivatives of any
+    order.  Host tensors take the eager formulation.
     """
     fused = use_fused(table, "embedding_lookup", force_reference)
     if fused and table.dim() == 2 and (padding_idx is None or 0 <= padding_idx < table.shape[0]):

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from nuvla_forge_amd import _lib
-from nuvla_forge_amd.kernels import chunked_token_logprobs, fused_dropout
+from nuvla_forge_amd.kernels import chunked_token_logprobs, embedding_lookup, fused_dropout
 from nuvla_forge_amd.kernels.dropout import dropout_threshold
 from nuvla_forge_amd.kernels.reference import dropout_keep
 
@@ -176,3 +176,38 @@ def test_dropout_second_derivatives(cuda, route, xt, rt, by_tensor):
     (du,) = torch.autograd.grad(dx, up, v)
     assert du.dtype == up.dtype
     assert ((du.double() - s * vd).abs() <= 4 * step * (s * vd).abs()).all()
+
+
+# ---------------------------------------------------------------------------
+# embedding lookup
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("m, pad", [(60, None), (60, 3), (1500, 3)])
+@pytest.mark.parametrize("dtype, od", [(F32, None), (F32, BF16), (BF16, None)])
+def test_embedding_second_derivatives(cuda, route, m, pad, dtype, od):
+    """sum(c out^3) of the lookup, and an upstream gradient's own gradient, against the dense
+    formulas in 64 bits.  The derivatives by table row v hold sums of n terms each:
+    (n + 8) 2^-24 of their absolute sum, and where rows or gradients are bf16 four roundings of
+    2^-8 of it."""
+    note(f"embedding second derivative {m} {pad} {dtype} {od} {route}")
+    g, v, d, scale = gen(m), 40, 24, 2.0
+    table = randn((v, d), g, dtype, cuda).requires_grad_(True)
+    ids = torch.randint(-2, v + 2, (m,), generator=g).to(cuda)
+    c, vt = randn((m, d), g, F32, cuda), randn((v, d), g, dtype, cuda)
+    live = (ids >= 0) & (ids < v)
+    hot = torch.nn.functional.one_hot(torch.where(live, ids, 0), v).double() * live[:, None]
+    back = hot if pad is None else hot * (ids != pad)[:, None]  # what carries a gradient
+    out = embedding_lookup(ids, table, scale=scale, padding_idx=pad, out_dtype=od)
+    (d1,) = torch.autograd.grad((c * out.float() ** 3).sum(), table, create_graph=True)
+    (d2,) = torch.autograd.grad((d1.float() * vt).sum(), table, create_graph=True)
+    (d3,) = torch.autograd.grad((d2.float() * vt).sum(), table)
+    e, cd, u = hot @ table.detach().double() * scale, c.double(), back @ vt.double() * scale
+    step = (m + 8) * 2.0 ** -24 + (2.0 ** -6 if BF16 in (dtype, od) else 0)
+    for got, term in ((d1, 3 * cd * e ** 2), (d2, 6 * cd * e * u), (d3, 6 * cd * u * u)):
+        want, size = back.T @ term * scale, back.T @ term.abs() * scale
+        assert got.dtype == dtype
+        assert ((got.double() - want).abs() <= step * size).all()
+    up = randn((m, d), g, out.dtype, cuda).requires_grad_(True)
+    out = embedding_lookup(ids, table, scale=scale, padding_idx=pad, out_dtype=od)
+    (dt,) = torch.autograd.grad(out, table, up, create_graph=True)
+    (du,) = torch.autograd.grad(dt, up, vt)
+    assert du.dtype == up.dtype and torch.equal(du.double(), u.to(du.dtype).double())

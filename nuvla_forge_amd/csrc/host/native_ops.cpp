@@ -73,9 +73,9 @@ variable_list first_order_only(const char *op, bool recording, const variable_li
   for (const Tensor &g : grads)
     if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
   const std::shared_ptr<torch::autograd::Node> node(
-      new torch::autograd::Error(std::string(op) + ": second derivatives are not supported on the "
-                                 "device; force_reference=True runs a formulation that has them",
-                                 std::move(edges)),
+      new torch::autograd::Error(
+          std::string(op) + ": second derivatives are not supported on the device",
+          std::move(edges)),
       torch::autograd::deleteNode);
   for (Tensor &t : out)
     if (t.defined()) {
@@ -167,7 +167,8 @@ struct Seam : torch::autograd::Function<Seam> {
     res[3] = dweight;
     res[4] = dscale;
     res[5] = dshift;
-    return res;
+    return first_order_only("fused_adaln_residual_rmsnorm", at::GradMode::is_enabled(), grads,
+                            std::move(res));
   }
 };
 
@@ -218,7 +219,7 @@ struct SwiGLU : torch::autograd::Function<SwiGLU> {
     check(nf_swiglu_bwd(g.data_ptr(), a.data_ptr(), b.data_ptr(), da.data_ptr(), db.data_ptr(),
                         a.numel(), code_of(a), stream_of(a)),
           "nf_swiglu_bwd");
-    return {da, db};
+    return first_order_only("fused_swiglu", at::GradMode::is_enabled(), grads, {da, db});
   }
 };
 
@@ -273,6 +274,7 @@ struct GateUp : torch::autograd::Function<GateUp> {
     Tensor x = s[0], wg = s[1], wu = s[2];
     const Tensor &a = s[3], &b = s[4];
     const c10::DeviceGuard guard(x.device());
+    const bool recording = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     const auto dt = ctx->saved_data["dt"].toIntVector();
     const Tensor dact = grads[0].to(at::kBFloat16).contiguous();
@@ -326,7 +328,8 @@ struct GateUp : torch::autograd::Function<GateUp> {
                                m, d, h, NF_DTYPE_BF16, ws.data_ptr(), nb, st),
             "nf_gemm_swiglu_bwd");
     }
-    return {dx, need_g ? dg.to(tg) : dg, need_u ? du.to(tu) : du};
+    return first_order_only("fused_gate_up_swiglu", recording, grads,
+                            {dx, need_g ? dg.to(tg) : dg, need_u ? du.to(tu) : du});
   }
 };
 
@@ -378,7 +381,8 @@ struct ChunkedCE : torch::autograd::Function<ChunkedCE> {
                     g.data_ptr<float>(), dh.data_ptr(), code_of(th), dw.data_ptr(), code_of(tw),
                     ws.data_ptr(), nw, stream_of(state)),
           "nf_ce_bwd");
-    return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor()};
+    return first_order_only("chunked_cross_entropy", at::GradMode::is_enabled(), grads,
+                            {dh, dw, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 

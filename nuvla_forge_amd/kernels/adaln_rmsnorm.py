@@ -31,7 +31,7 @@ import torch
 
 from .. import _lib
 from .reference import adaln_residual_rmsnorm_ref
-from .utils import check_devices, device_of, use_fused
+from .utils import check_devices, device_of, first_order_only, use_fused
 
 MAX_N = 16384  # widest row the kernels take (the reference's own limit, :262)
 
@@ -133,8 +133,9 @@ class _FusedAdaLNResidualRMSNorm(torch.autograd.Function):
                 ),
                 "nf_adaln_bwd_full",
             )
-        return (dx if need[0] else None, dy if need[1] else None,
-                dgate, dweight, dscale, dshift, None, None)
+        return first_order_only("fused_adaln_residual_rmsnorm", (dh_up, dout),
+                                (dx if need[0] else None, dy if need[1] else None,
+                                 dgate, dweight, dscale, dshift, None, None))
 
 
 def fused_adaln_residual_rmsnorm(
@@ -152,6 +153,8 @@ def fused_adaln_residual_rmsnorm(
 
     Falls back to the eager PyTorch formulation for host tensors, for rows
     wider than 16384 and under ``force_reference=True``, as the reference does.
+
+    Second derivatives are not supported on the device: taking one raises.
 
     Returns:
         (h, out) — the updated residual stream and the modulated branch input,

@@ -53,7 +53,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .utils import check_devices, device_of, use_fused
+from .utils import check_devices, device_of, first_order_only, use_fused
 
 # Opt-in: raise ValueError for targets outside [0, V) that are not
 # ignore_index.  The check reads one device int back to the host (a
@@ -233,7 +233,8 @@ class _ChunkedCrossEntropy(torch.autograd.Function):
         (state,) = ctx.saved_tensors
         dh, dw = _backward_hip(ctx.call, state, grad_output, ctx.hidden_dtype,
                                ctx.weight_dtype, ctx.device)
-        return dh, dw, None, None, None, None
+        return first_order_only("chunked_cross_entropy", (grad_output,),
+                                (dh, dw, None, None, None, None))
 
 
 def chunked_cross_entropy(
@@ -259,6 +260,8 @@ def chunked_cross_entropy(
         Scalar fp32 loss, mean-reduced over non-ignored tokens (0 if none).
 
     Host tensors run the reference's eager row-chunk loop, as in the reference.
+    Second derivatives are not supported: on the device taking one raises, the eager loop
+    computes its gradients in the forward and, as the reference's, leaves them out.
     """
     if not VALIDATE_TARGETS and use_fused(hidden, "chunked_cross_entropy", force_reference):
         # the plain call runs in C++; any other (None) takes the Function above

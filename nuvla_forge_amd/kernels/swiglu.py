@@ -19,7 +19,7 @@ import torch.nn.functional as F
 
 from .. import _lib
 from .reference import swiglu_ref
-from .utils import check_devices, device_of, use_fused
+from .utils import check_devices, device_of, first_order_only, use_fused
 
 
 def _check(a: torch.Tensor, b: torch.Tensor) -> None:
@@ -64,7 +64,7 @@ class _FusedSwiGLU(torch.autograd.Function):
                                 db.data_ptr(), a.numel(), _lib.dtype_code(a), _lib.stream_of(a)),
                 "nf_swiglu_bwd",
             )
-        return da, db
+        return first_order_only("fused_swiglu", (dout,), (da, db))
 
 
 class _FusedGateUpSwiGLU(torch.autograd.Function):
@@ -167,8 +167,9 @@ class _FusedGateUpSwiGLU(torch.autograd.Function):
                                          ws.data_ptr(), nbytes, st),
                     "nf_gemm_swiglu_bwd",
                 )
-        return (dx.to(tx) if need_x else None, dwg.to(tg) if need_g else None,
-                dwu.to(tu) if need_u else None)
+        return first_order_only("fused_gate_up_swiglu", (dact,),
+                                (dx.to(tx) if need_x else None, dwg.to(tg) if need_g else None,
+                                 dwu.to(tu) if need_u else None))
 
 
 def _gate_up_eager(x, w_gate, w_up):
@@ -191,6 +192,7 @@ def fused_gate_up_swiglu(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
     the inputs are bf16, or under bf16 autocast (as the Linears would); other
     dtypes take the two Linears and the fused SwiGLU kernel.  Host tensors
     take the eager formulation.  Gradients come back in each input's dtype.
+    Second derivatives are not supported on the device: taking one raises.
     """
     if not use_fused(x, "fused_gate_up_swiglu", force_reference):
         return _gate_up_eager(x, w_gate, w_up)
@@ -235,6 +237,7 @@ def fused_swiglu(a: torch.Tensor, b: torch.Tensor, force_reference: bool = False
         force_reference: run the eager PyTorch formulation instead.
 
     Host tensors take the eager formulation, as in the reference (swiglu.py:104).
+    Second derivatives are not supported on the device: taking one raises.
     """
     if not use_fused(a, "fused_swiglu", force_reference):
         return swiglu_ref(a, b)

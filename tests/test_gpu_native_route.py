@@ -333,3 +333,39 @@ def test_native_route_from_several_threads(cuda):
         for outs in ex.map(work, range(4)):
             for got in outs:
                 _same(got, want)
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_second_derivatives_raise(cuda, monkeypatch, python):
+    """Under create_graph the gradients are those without it; a derivative through them raises
+    beside terms that have one."""
+    note(f"second derivatives python={python}")
+
+    class NoNative:
+        first_order_only = _lib.native().first_order_only
+
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    if python:
+        monkeypatch.setattr(_lib, "native", NoNative)
+    inputs, up, t = _seam_inputs(cuda, F32, BF16)
+    g = gen(13)
+    x, wg, wu = (randn(s, g, BF16, cuda, std=0.3) for s in ((40, 64), (48, 64), (48, 64)))
+    targets = torch.randint(0, 48, (40,), generator=g).to(cuda)
+    calls = {
+        "fused_adaln_residual_rmsnorm":
+            (lambda *v: fused_adaln_residual_rmsnorm(*v, tokens_per_sample=t)[1], inputs),
+        "fused_swiglu": (fused_swiglu, [x, x.flip(0)]),
+        "fused_gate_up_swiglu": (fused_gate_up_swiglu, [x, wg, wu]),
+        "chunked_cross_entropy": (lambda h, w: chunked_cross_entropy(h, w, targets), [x, wg]),
+    }
+    for name, (op, args) in calls.items():
+        leaves = [v.detach().clone().requires_grad_(True) for v in args]
+        want = torch.autograd.grad(op(*leaves).float().sum(), leaves)
+        got = torch.autograd.grad(op(*leaves).float().sum(), leaves, create_graph=True)
+        _same(got, want)
+        for leaf in leaves:
+            with pytest.raises(RuntimeError, match=name + ": second derivatives"):
+                torch.autograd.grad(got[0].float().sum() + (leaf * leaf).float().sum(), leaf,
+                                    retain_graph=True)

@@ -54,19 +54,26 @@ def chunked_cross_entropy_ref(hidden, lm_weight, targets, ignore_index=-100):
 def token_logprobs_ref(hidden, lm_weight, targets, top_k=0, chunk_size=1024, ignore_index=-100):
     """(logprobs, entropy, top_logprobs, top_ids) over hidden @ lm_weight.T in fp32, rows taken
     ``chunk_size`` at a time; the last two are None for ``top_k`` 0.  Rows whose target is
-    ``ignore_index`` or outside [0, V) give 0 (and id -1) and no gradient."""
+    ``ignore_index`` or outside [0, V) give 0 (and id -1) and no gradient, whatever they hold; a
+    logit of -inf has no part in the entropy; alternatives go by their logits, NaN by none."""
     v, w, parts = lm_weight.shape[0], lm_weight.float(), []
     for at in range(0, max(hidden.shape[0], 1), chunk_size):
         tg = targets[at:at + chunk_size]
         live = (tg != ignore_index) & (tg >= 0) & (tg < v)
-        logp = F.linear(hidden[at:at + chunk_size].float(), w).log_softmax(-1)
+        # rows left out: zeros before the product (their gradient stops there) and after it (an
+        # infinity in w makes a NaN of 0)
+        h = torch.where(live[:, None], hidden[at:at + chunk_size], 0.0).float()
+        z = torch.where(live[:, None], F.linear(h, w), 0.0)
+        logp = z.log_softmax(-1)
         own = logp.gather(1, torch.where(live, tg, 0)[:, None])[:, 0]
-        ent = -(logp.exp() * logp).sum(-1)
+        ent = -(logp.exp() * logp.clamp(min=-200.0)).sum(-1)  # exp(-200) is 0: 0 * -inf is not
         got = [torch.where(live, own, 0.0), torch.where(live, ent, 0.0)]
         if top_k:
-            val, idx = torch.sort(logp.detach(), dim=-1, descending=True, stable=True)
-            got += [torch.where(live[:, None], val[:, :top_k], 0.0),
-                    torch.where(live[:, None], idx[:, :top_k], -1)]
+            idx = torch.sort(z.detach(), dim=-1, descending=True, stable=True)[1]  # NaN first
+            place = torch.arange(top_k, device=z.device) + z.isnan().sum(-1, keepdim=True)
+            idx = idx.gather(1, place.clamp(max=v - 1))
+            got += [torch.where(live[:, None], logp.detach().gather(1, idx), 0.0),
+                    torch.where(live[:, None] & (place < v), idx, -1)]
         parts.append(got)
     out = [torch.cat([got[i] for got in parts]) for i in range(len(parts[0]))]
     return tuple(out) if top_k else (*out, None, None)

@@ -215,6 +215,51 @@ def test_logprobs_eager(chunk_size):
     assert chunked_token_logprobs(h[:0], w, t[:0], top_k=2).top_ids.shape == (0, 2)
 
 
+def test_logprobs_eager_rows_left_out_may_hold_anything():
+    """NaN and infinities in rows that are left out, and an infinite weight beside them, reach no
+    gradient."""
+    h, w, t, g, gh = _case()
+    clean = logprobs64(h, w, t, g, gh)
+    h[2], h[4, 0], h[5, 1] = float("nan"), float("inf"), float("-inf")
+    h.requires_grad_(True), w.requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, top_k=2)
+    dh, dw = torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh])
+    assert (dh[[2, 4, 5]] == 0).all() and (out.entropy[[2, 4, 5]] == 0).all()
+    assert (dh.double() - clean["dh"]).abs().max() < 5e-6
+    assert (dw.double() - clean["dw"]).abs().max() < 5e-6
+    w = w.detach().clone()
+    w[3, 0] = float("-inf")
+    h = h.detach().abs().nan_to_num(1.0, posinf=1.0)
+    h[2, 0] = 0.0  # 0 * inf where it does not count
+    (dw,) = torch.autograd.grad(
+        sum(x.sum() for x in chunked_token_logprobs(h, w.requires_grad_(True), t)[:2]), w)
+    # p of token 3 is 0: dz there is 1 where it is the row's own token, else 0
+    assert torch.isfinite(dw).all() and torch.allclose(dw[3], h[t == 3].sum(0), rtol=1e-6)
+
+
+def test_logprobs_eager_logits_of_minus_infinity_and_nan():
+    """A token that an infinite weight rules out has no part in the entropy; alternatives go by
+    the logits, which may differ where the log probabilities' fp32 values no longer do; a NaN is
+    no alternative."""
+    h, w, t, *_ = _case()
+    h = h.abs() + 0.125
+    t = torch.where(t == 3, 4, t)
+    rest = torch.arange(11) != 3
+    want = chunked_token_logprobs(h, w[rest], torch.where(t > 3, t - 1, t), top_k=3)
+    w[3, 0] = float("-inf")
+    out = chunked_token_logprobs(h, w, t, top_k=11)
+    live = (t >= 0) & (t < 11)
+    assert (out.logprobs[live] - want.logprobs[live]).abs().max() < 1e-5
+    assert (out.entropy[live] - want.entropy[live]).abs().max() < 1e-5
+    assert (out.top_ids[live, -1] == 3).all() and (out.top_logprobs[live, -1] < -1e30).all()
+    tiny = torch.tensor([[1e-9], [3e-9], [2e-9], [3e-9]])
+    out = chunked_token_logprobs(torch.ones(1, 1), tiny, torch.tensor([0]), top_k=4)
+    assert out.top_ids.tolist() == [[1, 3, 2, 0]] and out.top_logprobs.unique().numel() == 1
+    tiny[1] = float("nan")
+    out = chunked_token_logprobs(torch.ones(1, 1), tiny, torch.tensor([0]), top_k=4)
+    assert out.top_ids.tolist() == [[3, 2, 0, -1]] and out.top_logprobs.isnan().all()
+
+
 def test_logprobs_refusals():
     h, w, t, *_ = _case()
     with pytest.raises(ValueError, match="expected"):

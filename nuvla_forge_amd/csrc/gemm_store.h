@@ -628,8 +628,9 @@ template <typename TI>
 bool job_buf_ok(const GemmJob<TI> &j) {
   if (j.tiles == 0) return true;
   if (j.bt) {  // B's K rows of ldb elements, read as whole 16-byte vectors
+    // (a dynamic K's static bound may pass lda: the rows end at the count, padded to 8)
     const int64_t ka = j.a_zeros ? (j.K + 7) / 8 * 8 : j.K;
-    return ka <= j.lda && buf_ok<TI>(j.A, j.lda, j.M, ka) &&
+    return (ka == j.K || ka <= j.lda) && buf_ok<TI>(j.A, j.lda, j.M, ka) &&
            buf_ok<TI>(j.B, j.ldb, j.K, j.ldb);
   }
   return buf_ok<TI>(j.A, j.lda, j.M, j.K) && buf_ok<TI>(j.B, j.ldb, j.N, j.K);

@@ -99,6 +99,50 @@ def test_logprobs_gradient_of_tokens_far_below_a_sure_one(cuda, far, chunk_size)
     assert (dw[:, 1:] == 0).all()
 
 
+def _head(m, d, v, dtype, dev, seed, ignored=0.2):
+    """Inputs on which every logit is exact in fp32: h in 1/16, w in 1/1024."""
+    g = gen(seed)
+    h, w = torch.randn(m, d, generator=g), torch.randn(v, d, generator=g) * 2 / math.sqrt(d)
+    h, w = (h * 16).round() / 16, (w * 1024).round() / 1024
+    t = torch.randint(0, v, (m,), generator=g)
+    t[torch.rand(m, generator=g) < ignored] = -100
+    up = torch.randn(2, m, generator=g)
+    return h.to(dtype).to(dev), w.to(dtype).to(dev), t.to(dev), up[0].to(dev), up[1].to(dev)
+
+
+def _holds(h, w, t, g, gh, k, **kw):
+    """Values, alternatives and gradients within the bounds of logprobs64."""
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    out = chunked_token_logprobs(h, w, t, top_k=k, **kw)
+    ref = logprobs64(h, w, t, g, gh, k)
+    got = dict(logprobs=out.logprobs, entropy=out.entropy)
+    got["dh"], got["dw"] = torch.autograd.grad([out.logprobs, out.entropy], [h, w], [g, gh])
+    for name, tol in (("logprobs", "lp"), ("entropy", "ent"), ("dh", "dh"), ("dw", "dw")):
+        off = (got[name].double() - ref[name]).abs()
+        assert (off <= ref["tol_" + tol]).all(), (name, (off / ref["tol_" + tol]).max())
+    if k:
+        assert torch.equal(out.top_ids, ref["top_ids"])
+        off = (out.top_logprobs.double() - ref["top_logprobs"]).abs()
+        assert (off <= ref["tol_lp"][:, None] + 2.0 ** -22 * ref["top_logprobs"].abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m, d, v", [(5, 64, 1000), (70, 64, 33001), (100, 1024, 2003),
+                                     (200, 1024, 2003), (300, 64, 2003), (1100, 1024, 1001)])
+@pytest.mark.parametrize("off", [(1, 0), (0, 1), (3, 5)])
+def test_logprobs_operands_that_begin_between_vectors(cuda, m, d, v, dtype, off):
+    """Contiguous hidden and weight that do not begin on 16 bytes, as views into larger buffers:
+    with the state kept and not, weight read as it lies or transposed for aligned ones."""
+    note(f"logprobs misaligned {m} {d} {v} {dtype} {off}")
+    h, w, t, g, gh = _head(m, d, v, dtype, cuda, m + d)
+
+    def moved(x, by):
+        flat = torch.empty(x.numel() + by, dtype=x.dtype, device=cuda)
+        return flat[by:].view(x.shape).copy_(x)
+
+    _holds(moved(h, off[0]), moved(w, off[1]), t, g, gh, 5)
+
+
 class _NoNative:
     """No plain call is taken by the C++ host side: each runs its Function in Python."""
 

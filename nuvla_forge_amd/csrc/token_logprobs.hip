@@ -12,13 +12,13 @@
 // Only valid rows (target != ignore_index, inside [0, V)) do any work: they are compacted
 // on the device and every later kernel sizes itself by the device count.
 //
-// Forward (nf_token_logprobs_fwd), more than 256 rows:
+// Forward (nf_token_logprobs_fwd), more than 256 rows, or more than 64 over V > 32768:
 //   1. ce_compact: the valid rows in order.  lp_gather: Hc = hidden[rows], and zeros (id
 //      -1) into the outputs of the other rows.
 //   2. per chunk of rows: lp_logits, the logits tile by tile, of which statistics and
 //      records of strips are left; lp_finish: the row's values from those.
-// Up to 256 rows: the same without the compaction, on smaller tiles (MidCfg); fp32 up to 32
-// rows: lp_skinny, one pass over weight, and lp_finish.
+// Fewer: the same without the compaction, on smaller tiles (MidCfg); fp32 up to 32 rows:
+// lp_skinny, one pass over weight, and lp_finish.
 // Backward (nf_token_logprobs_bwd), with g and h the upstream gradients of a row's logprob
 // and entropy H:
 //   dz = g (onehot - p) - h p (z - lse + H)

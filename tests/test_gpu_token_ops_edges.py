@@ -143,6 +143,17 @@ def test_logprobs_operands_that_begin_between_vectors(cuda, m, d, v, dtype, off)
     _holds(moved(h, off[0]), moved(w, off[1]), t, g, gh, 5)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m", [65, 100, 128, 129, 256, 257])
+def test_logprobs_of_middling_rows_over_a_large_vocabulary(cuda, m, dtype):
+    """More than 32768 tokens and 65 rows: compacted, also where dz is held in two terms."""
+    note(f"logprobs middling {m} {dtype}")
+    for d, v, k in ((64, 33001, 8), (37, 40000, 20), (72, 32769, 0)):
+        _holds(*_head(m, d, v, dtype, cuda, m + d, ignored=0.3), k)
+    h, w, t, g, gh = _head(m, 64, 33001, dtype, cuda, m)
+    _holds(h, w, torch.full_like(t, -100), g, gh, 3)  # none left
+
+
 class _NoNative:
     """No plain call is taken by the C++ host side: each runs its Function in Python."""
 

@@ -15,7 +15,8 @@ from nuvla_forge_amd.kernels import chunked_token_logprobs, embedding_lookup, fu
 from nuvla_forge_amd.kernels.dropout import dropout_threshold
 from nuvla_forge_amd.kernels.reference import dropout_keep
 
-from .helpers import gen, note, randn
+from .helpers import assert_graph_replays_match, gen, note, randn
+from .test_gpu_token_ops import _embedding_check
 from .token_ops_ref import logprobs64
 
 pytestmark = pytest.mark.gpu
@@ -266,3 +267,91 @@ def test_embedding_second_derivatives(cuda, route, m, pad, dtype, od):
     (dt,) = torch.autograd.grad(out, table, up, create_graph=True)
     (du,) = torch.autograd.grad(dt, up, vt)
     assert du.dtype == up.dtype and torch.equal(du.double(), u.to(du.dtype).double())
+
+
+# The gradient of more than 1024 tokens: the sort, the spans' sums and the join of runs that cross
+# spans, of 8 sorted positions, or of 16 and 32 from 131072 and 262144 (token, 512 columns) pairs on.
+@pytest.mark.parametrize("span, m, d", [(8, 1300, 8), (8, 1300, 7), (8, 1300, 1), (8, 1300, 1032),
+                                        (16, 135001, 8), (16, 66001, 520), (32, 270001, 8),
+                                        (32, 270003, 5)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_gradient_runs_at_span_borders(cuda, span, m, d, dtype):
+    """Runs that end one before, at and one past a border between spans, that take a span exactly,
+    and that cross one and several; the tokens of ids below 256 are sorted by id, so the counts
+    say where each run lies.  Many tokens of one id on top: more than a wavefront notes."""
+    note(f"embedding spans {span} {m} {d} {dtype}")
+    counts = [span - 1, 1, span, span + 1, span - 1, 2 * span, 1, 3 * span - 2, 1, span, 9 * span + 1,
+              span - 1, 12 * span, 1, 1, span - 2, 70 * span + 3]
+    counts = [c for i, c in enumerate(counts) if sum(counts[:i + 1]) < m]
+    counts += [m - sum(counts)]
+    ids = torch.repeat_interleave(torch.arange(len(counts)) * 3, torch.tensor(counts))
+    ids = ids[torch.randperm(m, generator=gen(m))].to(cuda)
+    _embedding_check(ids, randn((60, d), gen(d), dtype, cuda), scale=0.5)
+
+
+@pytest.mark.parametrize("m", [1025, 3000, 20000])
+@pytest.mark.parametrize("d", [5, 40, 520])
+def test_embedding_gradient_of_many_tokens_that_do_not_count(cuda, m, d):
+    note(f"embedding many ids {m} {d}")
+    g = gen(m + d)
+    table = randn((50, d), g, F32, cuda)
+    ids = torch.randint(-20, 70, (m,), generator=g)
+    ids[:4] = torch.tensor([1 << 40, -(1 << 40), (1 << 63) - 1, -(1 << 63)])
+    _embedding_check(ids.to(cuda), table, pad=7)
+    _embedding_check(torch.full((m,), 7, device=cuda), table, pad=7)  # nothing but padding
+    _embedding_check(torch.full((m,), -1, device=cuda), table)
+    _embedding_check(torch.full((m,), 49, device=cuda), table, pad=0)  # one id, the last
+    ids = torch.full((m,), 7)
+    ids[m // 2] = 8  # one token that counts
+    _embedding_check(ids.to(cuda), table, pad=7)
+    _embedding_check(ids.view(-1, 1).to(cuda).expand(m, 2)[:, 1], table.t().contiguous().t())
+
+
+@pytest.mark.parametrize("v", [131072, 131073, 140001, 300000])
+def test_embedding_gradient_over_a_large_vocabulary(cuda, v):
+    """More ids than 256 blocks of 512 hold: several share the bits that name a block, the first
+    and the last of the table among them."""
+    note(f"embedding large vocabulary {v}")
+    g = gen(v)
+    for m in (3000, 700):
+        ids = torch.randint(0, v, (m,), generator=g)
+        ids[::3] = torch.randint(0, 40, (len(ids[::3]),), generator=g) * 512 + 3
+        ids[:6] = torch.tensor([0, v - 1, v - 1, v, -1, 0])
+        _embedding_check(ids.to(cuda), randn((v, 16), g, F32, cuda), pad=3)
+
+
+def test_embedding_gradient_of_many_tokens_in_a_graph_and_in_threads(cuda):
+    note("embedding many tokens: graph, streams, threads")
+    from concurrent.futures import ThreadPoolExecutor
+
+    def inputs(seed):
+        g = gen(seed)
+        ids = (torch.rand(5000, generator=g) ** 3 * 1000).long().to(cuda)
+        return ids, randn((1000, 96), g, BF16, cuda), randn((5000, 96), g, BF16, cuda)
+
+    def make(seed=1):
+        ids, table, dout = inputs(seed)
+        leaf = table.requires_grad_(True)
+
+        def step():
+            out = embedding_lookup(ids, leaf, scale=2.0, padding_idx=0)
+            return [out.detach(), *torch.autograd.grad(out, leaf, dout)]
+
+        return step
+
+    assert_graph_replays_match(make)
+    alone = [make(s)() for s in (1, 2)]
+    steps = [make(s) for s in (1, 2)]
+    torch.cuda.synchronize()
+
+    def work(step):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            res = [step() for _ in range(8)]
+        stream.synchronize()
+        return res
+
+    with ThreadPoolExecutor(2) as ex:
+        for want, got in zip(alone, ex.map(work, steps)):
+            for one in got:
+                assert all(torch.equal(a, b) for a, b in zip(want, one, strict=True))

@@ -118,8 +118,8 @@ extern "C" int nf_dropout(const void *x, const void *residual, void *out, int64_
     return set_error(NF_ERR_DTYPE, "nf_dropout: dtypes %d -> %d", dt_x, dt_out);
   if (n == 0) return NF_OK;
   if (!x || !out) return set_error(NF_ERR_ARG, "nf_dropout: null pointer");
-  if ((n + 7) / 8 > (int64_t)0x7fffffff * kBlock)
-    return set_error(NF_ERR_ARG, "nf_dropout: n too large");
+  if ((n + 7) / 8 > kMaxLaunchThreads - kBlock)
+    return set_error(NF_ERR_ARG, "nf_dropout: n=%lld too large (at most about 2^35)", (long long)n);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t t = (uint32_t)threshold;
 #define NF_DROPOUT(CX, CO, I, O) \

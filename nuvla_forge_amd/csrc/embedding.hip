@@ -504,7 +504,11 @@ int run_fwd(const int64_t *ids, const W *table, int64_t ldt, float scale, int64_
   int glog = 3;
   while (glog < 6 && ((int64_t)1 << glog) < pieces) ++glog;
   const int64_t rows = kFwdThreads >> glog;
-  const unsigned grid = (unsigned)((M + rows - 1) / rows);
+  const int64_t blocks = (M + rows - 1) / rows;
+  if (blocks * kFwdThreads > kMaxLaunchThreads)
+    return set_error(NF_ERR_ARG, "nf_embedding_fwd: M=%lld too large (2^26 at D > 256, to 2^29 at "
+                     "D <= 64)", (long long)M);
+  const unsigned grid = (unsigned)blocks;
   if (D >= 8)
     emb_fwd_kernel<W, O, true><<<grid, kFwdThreads, 0, s>>>(ids, table, ldt, scale, M, D, V, out,
                                                             glog);
@@ -555,11 +559,10 @@ int launch_bwd(const O *dout, const int64_t *ids, int64_t pad, float scale, int6
     return check_launch("emb_few");
   }
   const unsigned cols = (unsigned)((D + 511) / 512);
+  const int64_t nsum = (p.spans * cols + 3) / 4, nclear = (V + 4 * kZeroIds - 1) / (4 * kZeroIds);
   emb_sort_kernel<<<1u << p.ord.log_nb, kSortThreads, 0, s>>>(ids, M, V, pad, p.ord, first,
                                                               sorted);
   if (int e = check_launch("emb_sort")) return e;
-  const int64_t nsum = (p.spans * cols + 3) / 4, nclear = (V + 4 * kZeroIds - 1) / (4 * kZeroIds);
-  if (nsum + nclear > 0x7fffffffLL) return set_error(NF_ERR_ARG, "nf_embedding_bwd: too large");
   emb_reduce_kernel<O, W, VEC><<<(unsigned)(nsum + nclear), 256, 0, s>>>(
       dout, D, first, sorted, p.ord, V, D, scale, p.span, (int)cols, nclear, dtable, part);
   if (int e = check_launch("emb_reduce")) return e;
@@ -585,6 +588,16 @@ bool sizes_ok(int64_t M, int64_t D, int64_t V) {
   const int64_t i32 = 0x7fffffffLL, cap = (int64_t)1 << 40;
   return M >= 0 && D > 0 && V > 0 && M < i32 && D <= 65535 * 512 && V < i32 && V * D <= cap &&
          M * D <= cap;
+}
+// The gradient's: what its launches take, V blocks of the sort, the spans and cleared rows of the
+// sums, the spans of the join.
+bool bwd_sizes_ok(int64_t M, int64_t D, int64_t V) {
+  if (!sizes_ok(M, D, V)) return false;
+  const BwdPlan p = bwd_plan(M, D, V);
+  const int64_t cols = (D + 511) / 512;
+  const int64_t sums = (p.spans * cols + 3) / 4 + (V + 4 * kZeroIds - 1) / (4 * kZeroIds);
+  return ((int64_t)kSortThreads << p.ord.log_nb) <= kMaxLaunchThreads &&
+         sums * 256 <= kMaxLaunchThreads && p.spans * kJoinThreads <= kMaxLaunchThreads;
 }
 
 }  // namespace
@@ -617,7 +630,7 @@ extern "C" int nf_embedding_fwd(const int64_t *ids, const void *table, int64_t l
 }
 
 extern "C" size_t nf_embedding_bwd_workspace(int64_t M, int64_t D, int64_t V) {
-  if (!sizes_ok(M, D, V)) return 0;
+  if (!bwd_sizes_ok(M, D, V)) return 0;
   return bwd_plan(M, D, V).total;
 }
 
@@ -625,7 +638,7 @@ extern "C" int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t pa
                                 float scale, int64_t M, int64_t D, int64_t V, void *dtable,
                                 int dt_out, int dt_table, void *workspace,
                                 size_t workspace_bytes, void *stream) {
-  if (!sizes_ok(M, D, V))
+  if (!bwd_sizes_ok(M, D, V))
     return set_error(NF_ERR_ARG, "nf_embedding_bwd: bad shape M=%lld D=%lld V=%lld",
                      (long long)M, (long long)D, (long long)V);
   if (!types_ok(dt_table, dt_out))

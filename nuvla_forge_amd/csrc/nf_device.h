@@ -386,6 +386,9 @@ __device__ __forceinline__ float exp_f32(float x) {
 // ---------------------------------------------------------------------------
 namespace nf {
 int set_error(int code, const char *fmt, ...);
+
+// Threads of a launch along one extent: the runtime refuses more than 32 bits of them.
+constexpr int64_t kMaxLaunchThreads = 0xffffffffLL;
 int check_launch(const char *what);
 inline bool is_dtype(int dt) {
   return dt == NF_DTYPE_F32 || dt == NF_DTYPE_BF16 || dt == NF_DTYPE_F16;

@@ -954,6 +954,7 @@ __global__ NF_GEMM_BOUNDS(C) void lp_dz_kernel(
 // rounding.  A thread takes 8 columns of a row (they lie in one strip).
 constexpr int kKeptThreads = 256;
 constexpr int64_t kKeptCols = (int64_t)1 << 26;  // the grid's second extent ends at 65535 blocks
+constexpr int64_t kKeptRows = kMaxLaunchThreads / kKeptThreads - 8;  // and its first
 
 template <int WTM>
 __global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
@@ -1061,7 +1062,7 @@ State state_layout(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool kee
   s.ent = take((size_t)M * sizeof(float));
   s.lp = take((size_t)M * sizeof(float));
   s.hc = take((size_t)(s.lo0 > 0 ? 2 * s.lo0 : M) * D * sizeof(TI));
-  if (sizeof(TI) == 2 && keep && M > kFewRows && V <= kKeptCols &&
+  if (sizeof(TI) == 2 && keep && M > kFewRows && M <= kKeptRows && V <= kKeptCols &&
       (D >= 1024 || mid_form<TI>(M, V) < 0)) {
     const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
     if (L.nch == 1) {
@@ -1186,6 +1187,13 @@ FwdPlan fwd_plan(int64_t M, int64_t V, int64_t chunk_rows, int top_k, bool kept)
   p.crows = p.form >= 0 ? M
             : chunk_rows < mcap / 8 && !kept ? round_up(8 * chunk_rows, 256)
                                              : mcap;
+  if (p.form < 0 && !kept) {
+    // what one launch takes: 64 logits a thread or more, and in lp_finish 64 threads a row
+    int64_t most = kMaxLaunchThreads / round_up(V, 256) * 64;
+    if (most > kMaxLaunchThreads / 64) most = kMaxLaunchThreads / 64;
+    most = most < 256 ? 256 : most / 256 * 256;
+    if (p.crows > most) p.crows = most;
+  }
   using F = MidCfg<TI>;
   if (p.form == 64)
     tile_plan<typename F::T64>(p, V);

@@ -362,3 +362,25 @@ def test_first_order_only(graph):
         other = torch.ones(2, requires_grad=True)  # what does not go through it is free
         (d,) = torch.autograd.grad((dx.detach() * other).sum(), other)
         assert torch.equal(d, dx.detach())
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """A launch has at most 2^32 - 1 threads along an extent: calls that would need more are
+    refused before any of their kernels, or take more launches."""
+    L = _lib.lib()
+    for n in ((1 << 35) + 1, 1 << 36):
+        assert L.nf_dropout(FAKE, None, FAKE, n, 100, None, 1, 0, 1, 1, None) == NF_ERR_ARG
+    for m, d in ((1 << 26, 512), (1 << 27, 200), (1 << 28, 128), (1 << 29, 64)):
+        assert L.nf_embedding_fwd(FAKE, FAKE, d, 1.0, m, d, 9, FAKE, 1, 1, None) == NF_ERR_ARG
+    for m, d, v in ((1 << 29, 8, 100), (100, 1, (1 << 30) + 1), ((1 << 31) - 1, 512, 1 << 30)):
+        assert L.nf_embedding_bwd_workspace(m, d, v) == 0
+        args = [FAKE, FAKE, -1, 1.0, m, d, v, FAKE, 1, 1, FAKE, 1 << 50, None]
+        assert L.nf_embedding_bwd(*args) == NF_ERR_ARG
+    assert L.nf_embedding_bwd_workspace(1 << 27, 64, 1 << 29) > 0
+    # 16 bytes a row and 128 logits; a launch of 2^20 tokens by 2^18 rows, not 2^20
+    assert 0 < L.nf_token_logprobs_fwd_workspace(1 << 20, 16, 1 << 20, 1 << 20, 0, 1) < 1 << 36
+    assert L.nf_token_logprobs_fwd_workspace(1 << 10, 16, 1 << 30, 1 << 20, 0, 0) > 0
+    # exponentials are kept for fewer than 2^24 rows
+    few, many = ((1 << 24) - 256, 1 << 24)
+    st = [L.nf_token_logprobs_state_bytes(m, 8, 64, 1 << 25, 1, 1) / m for m in (few, many)]
+    assert st[0] >= 2 * 64 and st[1] < 64

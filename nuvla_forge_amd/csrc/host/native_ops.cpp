@@ -389,6 +389,16 @@ struct ChunkedCE : torch::autograd::Function<ChunkedCE> {
 // ---------------------------------------------------------------------------
 // token log probabilities
 // ---------------------------------------------------------------------------
+// `t` ([R, D], contiguous) from a whole 16-byte vector on: a copy of a view that begins between
+// two, which every kernel of the call would read element by element.  Forward and backward, bf16,
+// V 32000, weight off by one element: 100 rows, D 2048 926 us, 296 with the copy (215 aligned), 5
+// rows 555, 241 and 163, 200 rows, D 1024 414, 148 and 125.
+Tensor from_vector(const Tensor &t) {
+  const bool whole = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ||
+                     t.size(1) * t.element_size() % 16 != 0;
+  return whole ? t : t.clone();
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   // {logprobs, entropy, top_logprobs, top_ids}; `keep` what the backward reads
   static variable_list run(const Tensor &hidden, const Tensor &weight, const Tensor &targets,
@@ -396,8 +406,8 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
                            at::ScalarType cdt, bool keep, Tensor &w, Tensor &state) {
     const int64_t m = hidden.size(0), d = hidden.size(1), v = weight.size(0);
     const int code = code_of(cdt);
-    const Tensor h = hidden.to(cdt).contiguous(), tg = targets.contiguous();
-    w = weight.to(cdt).contiguous();
+    const Tensor h = from_vector(hidden.to(cdt).contiguous()), tg = targets.contiguous();
+    w = from_vector(weight.to(cdt).contiguous());
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
     Tensor lp = at::empty({m}, f32), ent = at::empty({m}, f32), top = at::empty({m, top_k}, f32);
     Tensor ids = at::empty({m, top_k}, f32.dtype(at::kLong));

@@ -1007,9 +1007,7 @@ __global__ __launch_bounds__(kKeptThreads) void lp_from_kept_kernel(
 // is the slower one, 1.9 against 1.65 us a stage, and there are M / 256 rows of tiles) and not
 // a transpose made for it (which moves V D twice).  bf16, V 32000, forward and backward: D 2048,
 // 5 rows 157 us against 220, 300 rows 232 against 282, 512 rows 276 against 328, 768 rows 413
-// against 414; D 384 62 against 73, 88 against 94, 112 against 107, 131 against 136.  A weight
-// that does not begin on 16 bytes (a view into a larger buffer) is always transposed: the products
-// would read it element by element.
+// against 414; D 384 62 against 73, 88 against 94, 112 against 107, 131 against 136.
 inline bool weight_as_is(int64_t M, int64_t D, int64_t V) {
   return M <= 256 + D / 4 && D % 8 == 0 && sb_ok(V * D * (int64_t)sizeof(bf16));
 }
@@ -1413,14 +1411,9 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
   if (KL.kept) {
     S.Wt = K.Wt;
     S.Hct = K.Hct;
-    Wn = KL.as_is && aligned16(W) ? W : nullptr;
-    if (KL.as_is && !Wn && dH) {  // the state has no transpose, but W cannot be read as it lies
-      using U = typename std::conditional<sizeof(TI) == 2, uint16_t, uint32_t>::type;
-      S.Wt = reinterpret_cast<TI *>(ws + L.s_wt);
-      if ((e = launch_transpose<U>(W, V, D, D, S.Wt, L.ldwt, s))) return e;
-    }
+    Wn = KL.as_is ? W : nullptr;
   } else {
-    Wn = sizeof(TI) == 2 && weight_as_is(Mb, D, V) && aligned16(W) ? W : nullptr;
+    Wn = sizeof(TI) == 2 && weight_as_is(Mb, D, V) ? W : nullptr;
     if ((e = transposes<TI>(W, K.Hc, Mb, D, V, L, Wn || !dH ? nullptr : S.Wt, S.Hct, tp, s)))
       return e;
   }

@@ -57,12 +57,19 @@ def _check(hidden, lm_weight, targets, top_k):
                   dict(hidden=hidden, lm_weight=lm_weight, targets=targets))
 
 
+def _from_vector(x):
+    """``x`` (contiguous) from a whole 16-byte vector on: a copy of a view that begins between
+    two, which every kernel of the call would read element by element."""
+    whole = x.data_ptr() % 16 == 0 or x.shape[1] * x.element_size() % 16 != 0
+    return x if whole else x.clone()
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, lm_weight, targets, top_k, chunk_rows, ignore_index):
         (m, d), v, dev = hidden.shape, lm_weight.shape[0], hidden.device
         cdt = _compute_dtype(hidden, lm_weight)
-        h, w = hidden.to(cdt).contiguous(), lm_weight.to(cdt).contiguous()
+        h, w = (_from_vector(x.to(cdt).contiguous()) for x in (hidden, lm_weight))
         tg = targets.to(torch.int64).contiguous()
         logprobs = torch.empty(m, dtype=torch.float32, device=dev)
         entropy = torch.empty_like(logprobs)

@@ -319,9 +319,10 @@ int nf_ce_fwd_bwd(const void *hidden, const void *weight,
  * rules are those of nf_ce_fwd.  `state`
  * (nf_token_logprobs_state_bytes) holds the compacted rows, their log-sum-exp
  * and entropy for the backward; `workspace` nothing between calls.  With
- * `keep` (a backward will come) the state may also hold exp(z - strip maximum)
- * in 16 bits (bf16, more than 128 rows, one chunk for every row), so the
- * backward need not form the logits again.  The three take the same `keep`.
+ * `keep` (a backward will come; without it nf_token_logprobs_bwd refuses the
+ * state) the state may also hold exp(z - strip maximum) in 16 bits (bf16, more
+ * than 128 rows, one chunk for every row), so the backward need not form the
+ * logits again.  The three take the same `keep`.
  * A size call returns 0 for arguments beyond the kernels.
  * ---------------------------------------------------------------------- */
 size_t nf_token_logprobs_state_bytes(int64_t M, int64_t D, int64_t V,

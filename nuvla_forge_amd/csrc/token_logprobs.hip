@@ -1575,6 +1575,8 @@ extern "C" int nf_token_logprobs_bwd(const void *weight, int64_t M, int64_t D, i
   if (int e = check_shape(fn, M, D, V)) return e;
   if (chunk_rows <= 0) return set_error(NF_ERR_ARG, "%s: chunk_rows must be > 0", fn);
   if (!weight || !state) return set_error(NF_ERR_ARG, "%s: null pointer", fn);
+  if (!keep)  // few rows are then left where they lie, and the state has none of them
+    return set_error(NF_ERR_ARG, "%s: a state made without keep serves no backward", fn);
   if (int e = ce_check_dtype(fn, dtype)) return e;
   if ((dhidden && !is_dtype(dt_hidden)) || (dweight && !is_dtype(dt_weight)))
     return set_error(NF_ERR_DTYPE, "%s: gradient dtypes %d, %d", fn, dt_hidden, dt_weight);

@@ -384,3 +384,14 @@ def test_sizes_beyond_a_launch_are_refused():
     few, many = ((1 << 24) - 256, 1 << 24)
     st = [L.nf_token_logprobs_state_bytes(m, 8, 64, 1 << 25, 1, 1) / m for m in (few, many)]
     assert st[0] >= 2 * 64 and st[1] < 64
+
+
+def test_logprobs_backward_refuses_a_state_without_keep():
+    """Without ``keep`` the forward of few rows copies none of them for a backward."""
+    L = _lib.lib()
+    for m in (16, 4096):
+        st = L.nf_token_logprobs_state_bytes(m, 64, 100, 1024, 0, 1)
+        bw = L.nf_token_logprobs_bwd_workspace(m, 64, 100, 1024, 1)
+        assert L.nf_token_logprobs_bwd(FAKE, m, 64, 100, 1024, 0, 1, FAKE, st, FAKE, None, FAKE, 1,
+                                       FAKE, 1, FAKE, bw, None) == NF_ERR_ARG
+        assert "keep" in _err()

@@ -385,7 +385,7 @@ int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t padding_id,
  * where they are >= threshold (0: all kept; 65536: none).  The seed is
  * *seed_ptr, read on the device (a replayed graph takes its value then), or
  * `seed` where seed_ptr is NULL.  The backward is the same call on the
- * upstream gradient without a residual.  n at most 2^35 - 512.  Types: dt_x == dt_out, or either
+ * upstream gradient without a residual.  n at most 2^35 - 520.  Types: dt_x == dt_out, or either
  * fp32 and the other 16 bits; residual has dt_out.
  * ---------------------------------------------------------------------- */
 int nf_dropout(const void *x, const void *residual, void *out, int64_t n,

@@ -1389,6 +1389,26 @@ int fwd_run(const TI *H, const TI *W, const int64_t *targets, int64_t M, int64_t
   return NF_OK;
 }
 
+// The backward's plan and workspace: the cross entropy's, without the room for transposes that the
+// call does not make (weight's where it is read as it lies; both where the state was kept).
+template <typename TI>
+ce::Plan bwd_plan(int64_t M, int64_t D, int64_t V, int64_t chunk_rows, const State &s) {
+  ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
+  const size_t wt = L.s_hct - L.s_wt, hct = L.s_p - L.s_hct;
+  const int64_t Mb = s.lo0 > 0 ? 2 * s.lo0 : M;
+  const bool no_wt = s.kept || (sizeof(TI) == 2 && weight_as_is(Mb, D, V));
+  const size_t less = (no_wt ? wt : 0) + (s.kept ? hct : 0);
+  if (no_wt) L.s_hct -= wt;
+  for (size_t *at : {&L.s_p, &L.s_pt, &L.s_dhc, &L.s_dwacc, &L.s_total}) *at -= less;
+  return L;
+}
+template <typename TI>
+size_t bwd_bytes(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
+  const ce::Plan L =
+      bwd_plan<TI>(M, D, V, chunk_rows, state_layout<TI>(M, D, V, chunk_rows, true));
+  return L.s_total + L.b_total + 256;
+}
+
 template <typename TI>
 int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bool keep,
             char *state, const float *g, const float *h, void *dH, int dt_h, void *dW, int dt_w,
@@ -1397,7 +1417,7 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
   const State KL = state_layout<TI>(M, D, V, chunk_rows, keep);
   const View<TI> K(KL, state);
   const int64_t lo0 = KL.lo0, Mb = lo0 > 0 ? 2 * lo0 : M;  // rows of the products
-  const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
+  const ce::Plan L = bwd_plan<TI>(M, D, V, chunk_rows, KL);
   ce::StateView<TI> S(L, ws);
   int *const two = S.n;
   if (lo0 == 0) S.n = K.n;  // else *two, by lp_dz
@@ -1481,13 +1501,6 @@ int bwd_run(const TI *W, int64_t M, int64_t D, int64_t V, int64_t chunk_rows, bo
     ce::ce_scatter_dh_kernel<1><<<(unsigned)blocks, 256, 0, s>>>(S.dHc, D, K.pos, M, nullptr, dH,
                                                                  dt_h, sp);
   return check_launch("ce_scatter_dh");
-}
-
-// fp32 plans hold E in both layouts; what kept states hold themselves is still in the count.
-template <typename TI>
-size_t bwd_bytes(int64_t M, int64_t D, int64_t V, int64_t chunk_rows) {
-  const ce::Plan L = grad_plan<TI>(M, D, V, chunk_rows);
-  return L.s_total + L.b_total + 256;
 }
 
 }  // namespace lp

@@ -155,6 +155,46 @@ def test_logprobs_of_middling_rows_over_a_large_vocabulary(cuda, m, dtype):
     _holds(h, w, torch.full_like(t, -100), g, gh, 3)  # none left
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m, d, v, chunk_rows", [(5, 72, 1003, 1024), (100, 64, 33001, 1024),
+                                                 (200, 1024, 2003, 1024), (300, 64, 2003, 1),
+                                                 (1000, 136, 5001, 1024), (700, 37, 999, 300)])
+def test_logprobs_buffers_of_exactly_the_size_asked_for(cuda, m, d, v, chunk_rows, dtype):
+    """The C entries with a state and workspaces of the bytes that the size calls name: what lies
+    behind them stays as it was, and the results are those of the public call."""
+    note(f"logprobs exact buffers {m} {d} {v} {chunk_rows} {dtype}")
+    L, k = _lib.lib(), 4
+    h, w, t, g, gh = _head(m, d, v, dtype, cuda, m)
+    a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    out = chunked_token_logprobs(a, b, t, top_k=k, chunk_size=chunk_rows)
+    want = [*out, *torch.autograd.grad([out.logprobs, out.entropy], [a, b], [g, gh])]
+    code, st = _lib.dtype_code(h), _lib.stream_of(h)
+
+    def room(n):
+        assert n > 0
+        x = torch.full((n + 4096,), 171, dtype=torch.uint8, device=cuda)
+        return x, n
+
+    state, fw, bw = (room(n) for n in (
+        L.nf_token_logprobs_state_bytes(m, d, v, chunk_rows, 1, code),
+        L.nf_token_logprobs_fwd_workspace(m, d, v, chunk_rows, k, code),
+        L.nf_token_logprobs_bwd_workspace(m, d, v, chunk_rows, code)))
+    lp, ent = torch.empty(m, device=cuda), torch.empty(m, device=cuda)
+    top, ids = torch.empty(m, k, device=cuda), torch.empty(m, k, dtype=torch.int64, device=cuda)
+    dh, dw = torch.empty_like(h), torch.empty_like(w)
+    _lib.check(L.nf_token_logprobs_fwd(
+        h.data_ptr(), w.data_ptr(), t.data_ptr(), m, d, v, -100, chunk_rows, k, 1, code,
+        lp.data_ptr(), ent.data_ptr(), top.data_ptr(), ids.data_ptr(), state[0].data_ptr(),
+        state[1], fw[0].data_ptr(), fw[1], st), "fwd")
+    _lib.check(L.nf_token_logprobs_bwd(
+        w.data_ptr(), m, d, v, chunk_rows, 1, code, state[0].data_ptr(), state[1],
+        g.data_ptr(), gh.data_ptr(), dh.data_ptr(), code, dw.data_ptr(), code, bw[0].data_ptr(),
+        bw[1], st), "bwd")
+    for x, n in (state, fw, bw):
+        assert (x[n:] == 171).all()
+    assert all(torch.equal(x, y) for x, y in zip((lp, ent, top, ids, dh, dw), want))
+
+
 class _NoNative:
     """No plain call is taken by the C++ host side: each runs its Function in Python."""
 

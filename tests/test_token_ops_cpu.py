@@ -395,3 +395,15 @@ def test_logprobs_backward_refuses_a_state_without_keep():
         assert L.nf_token_logprobs_bwd(FAKE, m, 64, 100, 1024, 0, 1, FAKE, st, FAKE, None, FAKE, 1,
                                        FAKE, 1, FAKE, bw, None) == NF_ERR_ARG
         assert "keep" in _err()
+
+
+@pytest.mark.parametrize("m, d, v, kept", [(4096, 2048, 32000, True), (8, 2048, 128256, False),
+                                           (200, 1024, 32000, True), (4096, 2048, 128256, True)])
+def test_logprobs_backward_asks_for_no_transpose_that_it_does_not_make(m, d, v, kept):
+    """Weight's transpose is in the state, or weight is read as it lies: the backward's workspace
+    has no room for one, beside dz in bf16 (rows of whole lines of 64) and dh in fp32 where the
+    rows are many."""
+    L = _lib.lib()
+    need = L.nf_token_logprobs_bwd_workspace(m, d, v, 1024, 1)
+    many = 2 * (-(-m // 256) * 256) * (v + 64) + 4 * m * d if kept and m > 256 else 0
+    assert need < many + 2 * d * v

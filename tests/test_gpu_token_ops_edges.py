@@ -395,3 +395,81 @@ def test_embedding_gradient_of_many_tokens_in_a_graph_and_in_threads(cuda):
         for want, got in zip(alone, ex.map(work, steps)):
             for one in got:
                 assert all(torch.equal(a, b) for a, b in zip(want, one, strict=True))
+
+
+# ---------------------------------------------------------------------------
+# what sees or replaces a call
+# ---------------------------------------------------------------------------
+def _calls(dev):
+    """Each operator as a function of its differentiable inputs, and those."""
+    g = gen(17)
+    h, w, t, *_ = _head(140, 1024, 900, BF16, dev, 17)
+    ids = torch.randint(0, 40, (50,), generator=g).to(dev)
+    seed = torch.tensor([3], device=dev)
+    x, r = randn((20, 24), g, BF16, dev), randn((20, 24), g, F32, dev)
+    return {
+        "logprobs": (lambda a, b: chunked_token_logprobs(a, b, t, top_k=3)[:2], [h, w]),
+        "few": (lambda a, b: chunked_token_logprobs(a, b, t[:6], top_k=3)[:2], [h[:6], w]),
+        "embedding": (lambda a: (embedding_lookup(ids, a, padding_idx=1, out_dtype=BF16),),
+                      [randn((40, 24), g, F32, dev)]),
+        "dropout": (lambda a, b: (fused_dropout(a, 0.3, seed, offset=1, residual=b),), [x, r]),
+    }
+
+
+def _run(op, args):
+    leaves = [v.detach().clone().requires_grad_(True) for v in args]
+    outs = op(*leaves)
+    ups = [torch.linspace(-1, 1, o.numel(), device=o.device).view(o.shape).to(o.dtype) for o in outs]
+    return [*(o.detach() for o in outs), *torch.autograd.grad(outs, leaves, ups)]
+
+
+@pytest.mark.parametrize("name", ["logprobs", "few", "embedding", "dropout"])
+def test_token_ops_saved_tensors_go_through_the_hooks(cuda, route, name):
+    note(f"token ops saved-tensor hooks {name} {route}")
+    op, args = _calls(cuda)[name]
+    plain, packed = _run(op, args), []
+
+    def pack(v):
+        packed.append(v.shape)
+        return v.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v.to(cuda)):
+        hooked = _run(op, args)
+    assert len(packed) == (2 if name in ("logprobs", "few") else 1)
+    assert all(torch.equal(a, b) for a, b in zip(plain, hooked, strict=True))
+
+
+@pytest.mark.parametrize("name", ["logprobs", "few", "embedding", "dropout"])
+def test_token_ops_under_modes_tracing_and_transforms(cuda, name):
+    """Dispatch and function modes see the general path, which gives the same; a trace runs it;
+    transforms that the Functions have no rule for are refused."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    note(f"token ops modes {name}")
+    op, args = _calls(cuda)[name]
+    plain, seen = _run(op, args), []
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, a=(), kw=None):
+            seen.append(str(func))
+            return func(*a, **(kw or {}))
+
+    class Functions(TorchFunctionMode):
+        def __torch_function__(self, func, types, a=(), kw=None):
+            return func(*a, **(kw or {}))
+
+    for mode in (Dispatch, Functions):
+        with mode():
+            got = _run(op, args)
+        assert all(torch.equal(a, b) for a, b in zip(plain, got, strict=True))
+    assert any("empty" in f for f in seen)
+    traced = torch.jit.trace(op, tuple(args), check_trace=False)
+    # (what a call without a backward gives: it sums on other tiles)
+    assert all(torch.equal(a, b) for a, b in zip(op(*args), traced(*args), strict=True))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda *v: op(*v)[0])(*(v[None] for v in args))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(args[0], torch.ones_like(args[0]))
+        with pytest.raises(RuntimeError):
+            op(dual, *args[1:])

@@ -56,8 +56,9 @@ __device__ __forceinline__ void store8u(T *p, int64_t D, const float (&f)[8]) {
 
 // ---------------------------------------------------------------------------
 // forward: a group of 2^glog lanes takes a row, 8 columns a lane and step.  What bounds it is
-// memory: bf16, 65536 tokens by Zipf's law, V 128256, D 2048, 64 us for the 268 MB written and
-// as much read (a third of it from HBM), 78 without the non-temporal hint on the stores; 8192
+// memory: bf16, 65536 tokens by Zipf's law, V 128256, D 2048, back to back 61 us for the 268 MB
+// written and as much read (a third of it from HBM), 78 without the non-temporal hint on the
+// stores; 76-83 between training steps, which leave nothing of the table in the caches; 8192
 // tokens, D 1024 6.0 us, 7.0 without.
 // ---------------------------------------------------------------------------
 constexpr int kFwdThreads = 256;

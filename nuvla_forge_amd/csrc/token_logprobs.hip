@@ -264,8 +264,8 @@ __global__ NF_GEMM_BOUNDS(C) void lp_logits_kernel(
         acc[i][j][r] = KEEP ? e * kKeptScale : x;
       }
     // -inf * 0 is a NaN: without KEEP, where x is still there, a strip with a logit of -inf (or
-    // past the vocabulary) and no NaN is summed again with x bounded.  Bounding every x costs 3%
-    // of the tall head (12289 rows, D 384, V 50001, 20 alternatives 772 us against 747).
+    // past the vocabulary) and no NaN is summed again with x bounded.  Bounding every x costs 4%
+    // of the tall head (12289 rows, D 384, V 50001, 20 alternatives 756 us against 728).
     if constexpr (!KEEP) {
       if (t != t && s == s) {
         t = 0.f;
@@ -1013,10 +1013,11 @@ inline bool weight_as_is(int64_t M, int64_t D, int64_t V) {
 }
 
 // The tiling for `rows` rows, as MidCfg names them, or -1: the main tiles, which are also the
-// better ones where the smaller ones' 128 rows make more than a block a CU (V 43813, D 304, 178
-// rows, forward and backward: 91 us against 109; V 128256, D 1024, 128 rows, forward 180
-// against 188; fp32, V 85667, D 1432, 47 rows 1168 against 1287).  bf16 of up to 64 rows gains
-// from its 64 columns at every V.
+// better ones where the smaller ones' 128 rows make more than a block a CU, from 256 * 128 =
+// 32768 tokens on (V 43813, D 304, 178 rows, forward and backward: 91 us against 109; V 128256,
+// D 1024, 128 rows, forward 180 against 188; the fp32 backward, V 85667, D 1432, 47 rows, with
+// the forward 1176 against 1233, V 50001, D 384, 33 rows 200 against 217; that forward takes
+// Tall64).  bf16 of up to 64 rows gains from its 64 columns at every V.
 template <typename TI>
 int mid_form(int64_t rows, int64_t V) {
   if (rows <= 64 && (sizeof(TI) == 2 || V <= 32768)) return 64;

@@ -7,11 +7,11 @@ policy-gradient training, scoring and reporting alternatives need of a head whos
 loss ``chunked_cross_entropy`` computes.  Both per-token values have gradients.
 
 The device path is two calls, as the cross entropy's.  ``nf_token_logprobs_fwd`` compacts
-the rows that count on the device and keeps them with each row's log-sum-exp and entropy and, where a backward
-will follow and one chunk takes every row (bf16, more than 128 rows), the exponential of
-every logit in 16 bits; ``nf_token_logprobs_bwd`` forms the logits' gradient from those, or
-from the logits formed again, and runs the cross entropy's gradient products.  No call
-synchronises with the host.
+the rows that count on the device and keeps them with each row's largest logit, the logarithm
+of its sum and its entropy and, where a backward will follow and one chunk takes every row
+(bf16, more than 128 rows), the exponential of every logit in 16 bits;
+``nf_token_logprobs_bwd`` forms the logits' gradient from those, or from the logits formed
+again, and runs the cross entropy's gradient products.  No call synchronises with the host.
 
 Element types and ``chunk_size`` are the cross entropy's: bf16 inputs, or any under bf16
 autocast, run bf16 MFMA with fp32 accumulation; fp32 inputs bf16 products over three-part

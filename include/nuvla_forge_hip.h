@@ -370,7 +370,8 @@ int nf_embedding_fwd(const int64_t *ids, const void *table, int64_t ld_table,
  * rows no token holds, and the row padding_id (-1: none), are zero.  ids
  * outside [0, V) count nowhere.  Every row of dtable [V, D] (dense) is
  * written.  workspace: nf_embedding_bwd_workspace bytes (0: sizes beyond the
- * kernels: M over 2^28, V over 2^30), 16-byte aligned; it holds nothing between calls. */
+ * kernels, M over 2^28 or V over 2^30 among them), 16-byte aligned; it holds
+ * nothing between calls. */
 size_t nf_embedding_bwd_workspace(int64_t M, int64_t D, int64_t V);
 int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t padding_id,
                      float scale, int64_t M, int64_t D, int64_t V,
@@ -385,8 +386,8 @@ int nf_embedding_bwd(const void *dout, const int64_t *ids, int64_t padding_id,
  * where they are >= threshold (0: all kept; 65536: none).  The seed is
  * *seed_ptr, read on the device (a replayed graph takes its value then), or
  * `seed` where seed_ptr is NULL.  The backward is the same call on the
- * upstream gradient without a residual.  n at most 2^35 - 520.  Types: dt_x == dt_out, or either
- * fp32 and the other 16 bits; residual has dt_out.
+ * upstream gradient without a residual.  n at most 2^35 - 520.  Types:
+ * dt_x == dt_out, or either fp32 and the other 16 bits; residual has dt_out.
  * ---------------------------------------------------------------------- */
 int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
                int32_t threshold, const int64_t *seed_ptr, int64_t seed,

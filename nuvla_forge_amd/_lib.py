@@ -22,6 +22,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); the order follows the C declarations
@@ -108,6 +109,24 @@ SIGNATURES = {
     "nf_embedding_bwd": (
         _I32,
         [_P, _P, _I64, _F32, _I64, _I64, _I64, _P, _I32, _I32, _P, _SZ, _P],
+    ),
+    "nf_attention_state_bytes": (_SZ, [*[_I64] * 6, _I32, _I32, _I32]),
+    "nf_attention_fwd_workspace": (_SZ, [*[_I64] * 6, _I32]),
+    "nf_attention_fwd": (
+        _I32,
+        [*[_P, _I64, _I64, _I64] * 3, _P, _I64, _I64, *[_I64] * 6, _I32, _F32, _I32, _I32, _P,
+         _P, _SZ, _P, _SZ, _P],
+    ),
+    "nf_attention_bwd_workspace": (_SZ, [*[_I64] * 6, _I32]),
+    "nf_attention_bwd": (
+        _I32,
+        [*[_P, _I64, _I64, _I64] * 3, _P, _P, _I64, _I64, _I64, *[_I64] * 6, _I32, _F32, _I32,
+         _I32, _P, _SZ, _P, _P, _P, _P, _SZ, _P],
+    ),
+    "nf_rotary": (
+        _I32,
+        [*[_P, _I64, _I64, _I64, _P, _I64] * 2, _P, _I64, _I32, _I64, _I64, _I64, _P, _I32, _F64,
+         _I32, _I32, _I32, _I32, _P],
     ),
     "nf_dropout": (
         _I32, [_P, _P, _P, _I64, ctypes.c_int32, _P, _I64, _I64, _I32, _I32, _P],

@@ -1,0 +1,352 @@
+// What the attention kernels share: the rows of a key head, tiles in LDS, the matrix products'
+// operands and the masks.
+//
+// Rows.  The G = H / Hk query heads of a key head are one problem of R = Tq G rows, row r being
+// query t = r / G of head hk G + r % G: a few tokens still fill a tile, and dK and dV sum over a
+// group's heads in the order of the rows.
+//
+// Products.  All are formed as 32 x 32 tiles with the softmax's axis down the accumulator and the
+// kernel's own row (forward, dQ) or key (dK, dV) across it, in v_mfma_f32_32x32x16_{bf16,f16} or
+// v_mfma_f32_32x32x2_f32:
+//
+//   forward, dQ   S^T = K Q^T      O^T  += V^T P^T     dP^T = V dO^T    dQ^T += K^T dS^T
+//   dK, dV        S   = Q K^T      dV^T += dO^T P      dP   = dO V^T    dK^T += Q^T dS
+//
+// so that lane l holds, for its own column l % 32, the 16 entries 8 (i / 4) + 4 (l / 32) + i % 4
+// of the other axis: a row's statistics are a lane's scalars (joined once between lanes l and
+// l + 32), and the exponentials are the next product's right operand where they lie.  That
+// product sums over the axis in the order in which the lanes hold it: its left operand, read
+// transposed from LDS, takes the same order.
+//
+// Tiles.  Rows of DP elements, copied from memory to LDS by the buffer unit; 16-byte vectors
+// XOR-swizzled by row.  Rows past the end, columns past D and keys that the mask drops come from
+// beyond the buffer's bound, as zeros: what memory holds there is never read.
+#pragma once
+
+#include "gemm_core.h"
+
+namespace nf {
+namespace attn {
+
+using gemm::bf16x8;
+using gemm::floatx16;
+using gemm::lds_ptr_t;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s *lds_v4s;
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr uint32_t kOob = 0x80000000u;
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A tensor [B, T, heads, D] of unit last stride; strides in bytes.
+struct View {
+  const char *p;
+  int64_t b, t, h;
+};
+
+struct Shape {
+  int B, Tq, Tk, H, Hk, G, D;
+  int R;          // rows of a key head: Tq G
+  int nvec;       // 16-byte vectors of a row that hold columns
+  int off;        // causal: row t sees keys up to t + off = t + Tk - Tq
+  int causal;
+  int words;      // mask words (64 keys each) of a sample
+  uint32_t ginv;  // ceil(2^32 / G), 0 for G = 1
+  float c;        // |scale| log2(e)
+  float scale;
+  uint32_t flip;  // scale < 0: the sign bits of one operand of S are flipped
+  const uint64_t *bits;  // [B, words]: the keys that may be attended; null: all
+};
+
+// x / G for the small x of a tile
+__device__ __forceinline__ int div_g(const Shape &s, int x) {
+  return s.ginv ? (int)__umulhi((uint32_t)x, s.ginv) : x;
+}
+
+// Block -> (key head of a sample, tile).  Blocks go to the 8 XCDs in turn; the tiles of a head stay
+// on 8 / gcd(heads, 8) of them, so that its keys and values are in few L2s, dealt in turn, so that
+// the long and the short tiles of a causal call are spread evenly.  False: no tile for the block.
+__device__ __forceinline__ bool place(int heads, int tiles, int *head, int *tile) {
+  const int i = blockIdx.x, xcd = i & 7;
+  const int low = heads & -heads, g = low < 8 ? low : 8;  // gcd(heads, 8)
+  const int64_t s = (int64_t)(i >> 3) * (8 / g) + xcd / g;
+  if (s >= (int64_t)(heads / g) * tiles) return false;
+  *head = xcd % g + g * (int)(s / tiles);
+  *tile = (int)(s % tiles);
+  return true;
+}
+inline int64_t place_grid(int64_t heads, int64_t tiles) {
+  const int64_t low = heads & -heads, g = low < 8 ? low : 8;
+  return (heads / g * tiles + 8 / g - 1) / (8 / g) * 8;
+}
+
+// ---------------------------------------------------------------------------
+// tiles
+// ---------------------------------------------------------------------------
+template <typename T, int DP>
+struct Tile {
+  static constexpr int ROW = DP * (int)sizeof(T);  // bytes
+  static constexpr int NV = ROW / 16;              // vectors of a row: 8, 16 or 32
+  static constexpr int KS = ROW / 32;              // steps of a product over a row
+  static constexpr int NB = DP / 32;               // 32-wide column blocks
+  static constexpr int VE = 16 / (int)sizeof(T);
+  // The 16 rows that 16 lanes read at one vector, and the 4 rows that a transposing read of 16
+  // lanes covers 32 bytes of, lie in different banks (64 of 4 bytes).
+  __device__ __forceinline__ static int swz(int row) {
+    if constexpr (NV == 8)  // two rows to a bank cycle
+      return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    else
+      return (row & 3) << 2 | ((row >> 2) & 3);
+  }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char *p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), (short)0, 0x7fffffff, 0x00020000);
+}
+
+// ROWS rows to LDS: `at(row, &in)` gives a row's byte offset from p and whether it exists.
+template <typename T, int DP, int ROWS, class F>
+__device__ __forceinline__ void copy_tile(const char *p, int nvec, char *lds, int wave, F &&at) {
+  using C = Tile<T, DP>;
+  constexpr int CW = ROWS * C::NV / kThreads;
+  static_assert(CW >= 1 && ROWS * C::NV % kThreads == 0, "a tile is whole 1 KB copies a wavefront");
+  const int l = threadIdx.x & 63;
+  const auto rsrc = buffer(p);
+#pragma unroll
+  for (int c = 0; c < CW; ++c) {
+    const int chunk = wave * CW + c;
+    const int row = chunk * (64 / C::NV) + l / C::NV;
+    const int vec = (l % C::NV) ^ C::swz(row);
+    bool in;
+    const uint32_t o = at(row, &in) + (uint32_t)vec * 16u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(lds + chunk * 1024), 16,
+                                             in && vec < nvec ? o : kOob, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ floatx16 mma(const u32x4 &a, const u32x4 &b, floatx16 acc) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), acc,
+                                                 0, 0, 0);
+    return acc;
+  } else if constexpr (__is_same(T, bf16)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  }
+}
+
+// acc[n] += rows 32 kb .. + 31 of the tile times the columns held in b[n] (one row of DP elements
+// a lane: vector 2 k + lane / 32 of it at step k).
+template <typename T, int DP, int N>
+__device__ __forceinline__ void mma_rows(const char *tile, int kb,
+                                         const u32x4 (&b)[N][Tile<T, DP>::KS], floatx16 (&acc)[N]) {
+  using C = Tile<T, DP>;
+  const int l = threadIdx.x & 63, h = l >> 5, row = l & 31;
+  const char *p = tile + (kb * 32 + row) * C::ROW;
+  const int sw = C::swz(row);
+#pragma unroll
+  for (int k = 0; k < C::KS; ++k) {
+    const u32x4 a = *reinterpret_cast<const u32x4 *>(p + ((2 * k + h) ^ sw) * 16);
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] = mma<T>(a, b[n][k], acc[n]);
+  }
+}
+
+// The 16 values of a lane as the right operand over their axis: two vectors of 8 in 16 bits.
+template <typename T>
+struct Packed {
+  u32x4 v[2];
+  __device__ __forceinline__ void set(const floatx16 &x) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      t8 y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = static_cast<T>(x[8 * s + i]);
+      v[s] = __builtin_bit_cast(u32x4, y);
+    }
+  }
+};
+template <>
+struct Packed<float> {
+  floatx16 v;
+  __device__ __forceinline__ void set(const floatx16 &x) { v = x; }
+};
+
+// acc[n][nb] += (columns 32 nb .. + 31 of rows 32 kb .. + 31 of the tile)^T x[n], over those rows
+// in the order in which the lanes hold x.
+template <typename T, int DP, int N>
+__device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<T> (&x)[N],
+                                         floatx16 (&acc)[N][Tile<T, DP>::NB]) {
+  using C = Tile<T, DP>;
+  const int l = threadIdx.x & 63, h = l >> 5;
+  const char *p = tile + kb * 32 * C::ROW;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = 8 * (i / 4) + 4 * h + i % 4;
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb) {
+        const int vec = (8 * nb + (l & 31) / 4) ^ C::swz(row);
+        const float a = *reinterpret_cast<const float *>(p + row * C::ROW + vec * 16 + (l & 3) * 4);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[n].v[i], acc[n][nb], 0, 0, 0);
+      }
+    }
+  } else {
+    // A transposing read: of each 16 lanes, lane a + 4 q addresses row q at columns 4 a .. 4 a + 3
+    // and lane i receives column i of the four rows.
+    const int j = l & 15, r0 = 4 * h + (j >> 2);
+    const int vec = 2 * ((l >> 4) & 1) + ((j & 3) >> 1), in = (j & 1) * 8;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int nb = 0; nb < C::NB; ++nb) {
+        const int ra = 16 * s + r0, rb = ra + 8;
+        const char *pa = p + ra * C::ROW + (((4 * nb + vec) ^ C::swz(ra)) << 4) + in;
+        const char *pb = p + rb * C::ROW + (((4 * nb + vec) ^ C::swz(rb)) << 4) + in;
+        const v4s u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)pa);
+        const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)pb);
+        const u32x4 a =
+            __builtin_bit_cast(u32x4, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n][nb] = mma<T>(a, x[n].v[s], acc[n][nb]);
+      }
+  }
+}
+
+// A row of a tensor as mma_rows' right operand: zeros past the row's vectors, or for no row.
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(const char *p, bool in, int nvec, uint32_t flip,
+                                         u32x4 (&v)[Tile<T, DP>::KS]) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int k = 0; k < Tile<T, DP>::KS; ++k) {
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (in && 2 * k + h < nvec) x = *reinterpret_cast<const u32x4 *>(p + (2 * k + h) * 16);
+    v[k] = x ^ flip;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// lanes l and l + 32
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ floatx16 splat(float x) {
+  floatx16 v;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = x;
+  return v;
+}
+
+// The other axis's index of entry i of a lane, within 32.
+__device__ __forceinline__ int entry(int i) {
+  return 8 * (i / 4) + 4 * ((threadIdx.x & 63) >> 5) + i % 4;
+}
+
+// ---------------------------------------------------------------------------
+// tiles of keys
+// ---------------------------------------------------------------------------
+// The keys of a tile that the mask leaves, 64 to a word; TK = 32: the tile's half of a word.
+template <int TK>
+struct KeyBits {
+  static constexpr int N = TK > 64 ? TK / 64 : 1;
+  uint64_t w[N];
+  __device__ __forceinline__ void load(const uint64_t *bits, int words, int tile) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!bits) {
+        w[i] = ~0ull;
+      } else if constexpr (TK == 32) {
+        w[i] = (bits[tile >> 1] >> (32 * (tile & 1))) & 0xffffffffull;
+      } else {
+        w[i] = tile * N + i < words ? bits[tile * N + i] : 0ull;
+      }
+    }
+  }
+  __device__ __forceinline__ bool any() const {
+    uint64_t x = w[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) x |= w[i];
+    return x != 0;
+  }
+  __device__ __forceinline__ bool all() const {
+    uint64_t x = w[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) x &= w[i];
+    return (TK == 32 ? (x | ~0xffffffffull) : x) == ~0ull;
+  }
+  __device__ __forceinline__ bool has(int row) const {
+    uint64_t x = w[0];
+    if constexpr (N == 2) x = row >= 64 ? w[1] : w[0];
+    if constexpr (N == 4) x = row >= 128 ? (row >= 192 ? w[3] : w[2]) : (row >= 64 ? w[1] : w[0]);
+    return (x >> (row & 63)) & 1;
+  }
+};
+
+// 16 accumulated columns of 4 consecutive rows: a lane's entries 4 quad .. + 3 of column block nb,
+// written to row p of D elements.
+template <typename T>
+__device__ __forceinline__ void store_quad(T *p, int d, int D, const float (&v)[4]) {
+  if (d + 4 <= D) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = from_f32<T>(v[i]);
+    __builtin_memcpy(p + d, &x, sizeof(x));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < D) p[d + i] = from_f32<T>(v[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+struct Sizes {  // what a call is about, as its entry points take it
+  int64_t B, Tq, Tk, H, Hk, D;
+  int dtype;
+  int es() const { return dtype == NF_DTYPE_F32 ? 4 : 2; }
+  int64_t rows() const { return Tq * (H / Hk); }
+  int64_t words() const { return (Tk + 63) / 64; }
+  int dp() const { return D <= 64 ? 64 : 128; }
+};
+// NF_OK, or the error that is set
+int check_sizes(const char *op, const Sizes &z);
+int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
+              const Sizes &z, int64_t group, View *v);
+Shape make_shape(const Sizes &z, int causal, float scale, const uint64_t *bits);
+
+// The state's parts, in bytes from its start: log-sum-exps, mask words, what out's rounding left.
+struct State {
+  size_t lse, bits, low, total;
+};
+State state_of(const Sizes &z, bool mask, bool keep);
+
+}  // namespace attn
+}  // namespace nf

@@ -1,0 +1,438 @@
+// Attention, backward: the probabilities are formed again from the row's log-sum-exp L,
+//
+//   P = 2^(c S - L),  delta = rowsum(dO O),  dS = P (dP - delta)  with  dP = dO V^T
+//   dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q,
+//
+// in two launches: one over tiles of rows for delta and dQ, one over tiles of keys for dK and dV.
+// Each sums in an order of its own that no other block takes part in (no atomics: the same bits
+// every run), at the price of S and dP formed twice (seven products of a tile where five would do).
+// delta is formed from O's two parts, rounded and left over: out of the rounded part alone it would
+// be the largest error of dS where a row attends few keys.
+#include <math.h>
+
+#include "attention.h"
+
+namespace nf {
+namespace attn {
+namespace {
+
+struct BwdArgs {
+  Shape s;
+  View q, k, v, dout;
+  const char *out, *low;
+  const float *lse;
+  float *ndelta;  // [B Hk, R]: -delta
+  char *dq, *dk, *dv;
+  int tiles;
+};
+
+// fp16 holds 2^-24 to 65504, and gradients may lie anywhere: dS is scaled by a power of two of its
+// column's own (a row's in dQ, a key's in dK), chosen so that its largest entry so far is about
+// 2^kTop; a larger one scales what is accumulated.  Other types take dS as it is.
+constexpr int kTop = 12;
+template <typename T, int NB>
+struct Ranged {
+  __device__ __forceinline__ void fit(floatx16 &, floatx16 (&)[NB]) {}
+  __device__ __forceinline__ float undo() const { return 1.f; }
+};
+template <int NB>
+struct Ranged<f16, NB> {
+  int e = -1000;  // entries are below 2^e; none so far
+  __device__ __forceinline__ void fit(floatx16 &x, floatx16 (&acc)[NB]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = pair_max(top);
+    const bool real = top > 0.f && top < kInf;
+    const int now = real ? __builtin_amdgcn_frexp_expf(top) : -1000;
+    if (__any(now > e + 2)) {
+      const int up = now > e ? now : e;
+      const float f = e == -1000 ? 0.f : ldexpf(1.f, e - up);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        if (e != up) acc[n] *= f;
+      e = up;
+    }
+    const int by = e == -1000 ? 0 : kTop - e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = ldexpf(x[i], by);
+  }
+  // what the accumulated sum is to be multiplied by
+  __device__ __forceinline__ float undo() const { return e == -1000 ? 1.f : ldexpf(1.f, e - kTop); }
+};
+// fp16: P carries a factor 2^kPExp into dV's product
+template <typename T>
+constexpr float kPExp = __is_same(T, f16) ? 15.f : 0.f;
+
+// KW as in the forward: 1, a wavefront has 32 rows of its own; 4, the wavefronts share a block's 32
+// rows and take a quarter of each tile's keys.
+template <typename T, int DP, int KW>
+struct Dq {
+  using C = Tile<T, DP>;
+  static constexpr int BR = KW == 1 ? 32 * kWaves : 32;
+  static constexpr int TK = KW == 4 ? 128 : (C::ROW > 256 ? 32 : 64);
+  static constexpr int NK = KW == 4 ? 1 : TK / 32;
+  static constexpr int TILE = TK * C::ROW;
+  static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int LDS = STAGES * 2 * TILE;
+};
+
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(
+    BwdArgs a) {
+  using F = Dq<T, DP, KW>;
+  using C = Tile<T, DP>;
+  __shared__ __attribute__((aligned(16))) char smem[F::LDS];
+  const Shape &s = a.s;
+  int bh, job;
+  if (!place(s.B * s.Hk, a.tiles, &bh, &job)) return;
+  const int tile = a.tiles - 1 - job;
+  const int b = bh / s.Hk, hk = bh % s.Hk;
+  const int l = threadIdx.x & 63, h = l >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = tile * F::BR + (KW == 1 ? 32 * wave : 0);
+  const int rows_end = min(tile * F::BR + F::BR, s.R);
+
+  const int r = r0 + (l & 31);
+  const int rc = min(r, s.R - 1), t = rc / s.G, g = rc - t * s.G;
+  const int64_t row = (int64_t)bh * s.R + rc;
+  const int64_t at_out = (((int64_t)b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
+  u32x4 q[1][C::KS], dout[1][C::KS];
+  load_row<T, DP>(a.dout.p + b * a.dout.b + t * a.dout.t + (int64_t)(hk * s.G + g) * a.dout.h,
+                  r < s.R, s.nvec, 0u, dout[0]);
+  float nd = 0.f;  // -delta: the lane's half of the columns, then both
+  {
+    const T *out = reinterpret_cast<const T *>(a.out) + at_out;
+    const T *low = a.low ? reinterpret_cast<const T *>(a.low) + at_out : nullptr;
+#pragma unroll
+    for (int k = 0; k < C::KS; ++k) {
+      T d[C::VE];
+      __builtin_memcpy(d, &dout[0][k], 16);
+#pragma unroll
+      for (int i = 0; i < C::VE; ++i) {
+        const int col = (2 * k + h) * C::VE + i;
+        if (col < s.D) {
+          float o = to_f32(out[col]);
+          if (low) o += to_f32(low[col]);
+          nd = fmaf(-to_f32(d[i]), o, nd);
+        }
+      }
+    }
+    nd = pair_sum(nd);
+    if (r < s.R && h == 0 && (KW == 1 || wave == 0)) a.ndelta[row] = nd;
+  }
+  if (!a.dq) return;  // the call is for delta alone
+  load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
+                  s.flip, q[0]);
+  const float lse = a.lse[row];
+  const int last = s.causal ? t + s.off : s.Tk - 1;
+  const int wave_least = s.causal ? min(r0, s.R - 1) / s.G + s.off : s.Tk - 1;
+  const int wave_last = s.causal ? min(r0 + 31, s.R - 1) / s.G + s.off : s.Tk - 1;
+  const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
+  const int end = block_last < 0 ? 0 : block_last / F::TK + 1;
+
+  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
+  const char *kp = a.k.p + b * a.k.b + hk * a.k.h, *vp = a.v.p + b * a.v.b + hk * a.v.h;
+  KeyBits<F::TK> cur, nxt;
+  auto seek = [&](int i, KeyBits<F::TK> &w) {
+    for (; i < end; ++i) {
+      w.load(bits, s.words, i);
+      if (w.any()) break;
+    }
+    return i;
+  };
+  auto copy = [&](int i, const KeyBits<F::TK> &w, char *buf) {
+    const int left = s.Tk - i * F::TK;
+    const bool whole = w.all();
+    const uint32_t kt = (uint32_t)a.k.t, vt = (uint32_t)a.v.t;
+    copy_tile<T, DP, F::TK>(kp + (int64_t)i * F::TK * a.k.t, s.nvec, buf, wave,
+                            [&](int rw, bool *in) {
+                              *in = rw < left && (whole || w.has(rw));
+                              return (uint32_t)rw * kt;
+                            });
+    copy_tile<T, DP, F::TK>(vp + (int64_t)i * F::TK * a.v.t, s.nvec, buf + F::TILE, wave,
+                            [&](int rw, bool *in) {
+                              *in = rw < left && (whole || w.has(rw));
+                              return (uint32_t)rw * vt;
+                            });
+  };
+
+  floatx16 dq[1][C::NB];
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n) dq[0][n] = splat(0.f);
+  Ranged<T, C::NB> range;
+
+  int at = seek(0, cur), buf = 0;
+  if (at < end) copy(at, cur, smem);
+  while (at < end) {
+    const int next = seek(at + 1, nxt);
+    gemm::wait_vm_barrier<0>();
+    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
+    const int key0 = at * F::TK + (KW == 4 ? 32 * wave : 0);
+    if (key0 <= wave_last && key0 < s.Tk) {
+      const int kb0 = KW == 4 ? wave : 0;
+      const bool edge = key0 + 32 * F::NK - 1 > min(wave_least, s.Tk - 1) || !cur.all();
+#pragma unroll
+      for (int i = 0; i < F::NK; ++i) {
+        floatx16 p[1] = {splat(0.f)}, dp[1] = {splat(nd)};
+        mma_rows<T, DP, 1>(kt, kb0 + i, q, p);
+        mma_rows<T, DP, 1>(vt, kb0 + i, dout, dp);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[0][e] *= exp2_(fmaf(p[0][e], s.c, -lse));
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int in = 32 * i + entry(e);
+            const bool live = key0 + in <= last && cur.has(32 * kb0 + in);
+            dp[0][e] = live ? dp[0][e] : 0.f;
+          }
+        }
+        range.fit(dp[0], dq[0]);
+        Packed<T> x[1];
+        x[0].set(dp[0]);
+        mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
+      }
+    }
+    if (F::STAGES == 1) {
+      __syncthreads();
+      if (next < end) copy(next, nxt, smem);
+    } else {
+      buf ^= 1;
+    }
+    at = next;
+    cur = nxt;
+  }
+  const float f = s.scale * range.undo();
+  if constexpr (KW == 4) {
+    __syncthreads();
+    float *os = reinterpret_cast<float *>(smem);  // [4][DP][32]
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        os[(wave * DP + 32 * n + entry(e)) * 32 + (l & 31)] = dq[0][n][e] * f;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (((32 * n + 8 * (e / 4)) * 4) / DP != wave) continue;
+        const int i = (32 * n + entry(e)) * 32 + (l & 31);
+        dq[0][n][e] = ((os[i] + os[DP * 32 + i]) + os[2 * DP * 32 + i]) + os[3 * DP * 32 + i];
+      }
+  }
+  if (r >= s.R) return;
+  T *to = reinterpret_cast<T *>(a.dq) + at_out;
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = dq[0][n][4 * e4 + i] * (KW == 4 ? 1.f : f);
+      store_quad<T>(to, 32 * n + entry(4 * e4), s.D, x);
+    }
+}
+
+// A block has 128 keys, a wavefront 32, and goes over the rows.
+template <typename T, int DP>
+struct Dkv {
+  using C = Tile<T, DP>;
+  static constexpr int BK = 32 * kWaves;
+  static constexpr int TR = C::ROW > 256 ? 32 : 64;  // rows of a tile
+  static constexpr int TILE = TR * C::ROW;
+  static constexpr int STAGE = 2 * TILE + 2 * 256;  // q, dout, log-sum-exps, -deltas
+  static constexpr int LDS = 2 * STAGE;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
+  using F = Dkv<T, DP>;
+  using C = Tile<T, DP>;
+  __shared__ __attribute__((aligned(16))) char smem[F::LDS];
+  const Shape &s = a.s;
+  int bh, tile;
+  if (!place(s.B * s.Hk, a.tiles, &bh, &tile)) return;  // causal: the first keys have most rows
+  const int b = bh / s.Hk, hk = bh % s.Hk;
+  const int l = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  const int key0 = tile * F::BK + 32 * wave;
+  const int key = key0 + (l & 31);
+  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
+  const bool live = key < s.Tk && (!bits || (bits[key >> 6] >> (key & 63) & 1));
+  const bool work = __any(live);
+  u32x4 k[1][C::KS], v[1][C::KS];
+  load_row<T, DP>(a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t, live, s.nvec, s.flip, k[0]);
+  load_row<T, DP>(a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t, live, s.nvec, 0u, v[0]);
+  // causal: row r sees the key from r = (key - off) G on
+  const int from = s.causal ? max(key - s.off, 0) : 0;
+  const int64_t rmin64 = (int64_t)from * s.G;
+  const int rmin = (int)(rmin64 < s.R ? rmin64 : s.R);
+  const int wave_full = s.causal ? max(key0 + 31 - s.off, 0) : 0;  // from this t on, every key
+  const int block_from = s.causal ? max(tile * F::BK - s.off, 0) : 0;
+  const int end = (s.R + F::TR - 1) / F::TR;
+  int at = (int)min((int64_t)block_from * s.G / F::TR, (int64_t)end);
+  const int wave_at = s.causal ? (int)min((int64_t)max(key0 - s.off, 0) * s.G / F::TR, (int64_t)end)
+                               : 0;
+
+  const char *qp = a.q.p + b * a.q.b + (int64_t)hk * s.G * a.q.h;
+  const char *dp = a.dout.p + b * a.dout.b + (int64_t)hk * s.G * a.dout.h;
+  const char *lp = reinterpret_cast<const char *>(a.lse + (int64_t)bh * s.R);
+  const char *np = reinterpret_cast<const char *>(a.ndelta + (int64_t)bh * s.R);
+  auto copy = [&](int i, char *buf) {
+    const int row0 = i * F::TR, t0 = row0 / s.G, g0 = row0 - t0 * s.G, left = s.R - row0;
+    auto rows = [&](const View &w) {
+      return [&, wt = (uint32_t)w.t, wh = (uint32_t)w.h](int row, bool *in) {
+        *in = row < left;
+        const int x = g0 + row, dt = div_g(s, x), g = x - dt * s.G;
+        return (uint32_t)dt * wt + (uint32_t)g * wh;
+      };
+    };
+    copy_tile<T, DP, F::TR>(qp + (int64_t)t0 * a.q.t, s.nvec, buf, wave, rows(a.q));
+    copy_tile<T, DP, F::TR>(dp + (int64_t)t0 * a.dout.t, s.nvec, buf + F::TILE, wave, rows(a.dout));
+    if (wave < 2) {
+      const auto rsrc = buffer((wave == 0 ? lp : np) + (int64_t)row0 * 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (lds_ptr_t)(buf + 2 * F::TILE + 256 * wave), 4, l < left ? l * 4u : kOob, 0, 0, 0);
+    }
+  };
+
+  floatx16 dk[1][C::NB], dv[1][C::NB];
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n) dk[0][n] = dv[0][n] = splat(0.f);
+  Ranged<T, C::NB> range;
+
+  int buf = 0;
+  if (at < end) copy(at, smem);
+  for (; at < end; ++at) {
+    gemm::wait_vm_barrier<0>();
+    if (at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
+    const char *qt = smem + buf * F::STAGE, *dt = qt + F::TILE;
+    const float *lse = reinterpret_cast<const float *>(qt + 2 * F::TILE), *nd = lse + 64;
+    if (work && at >= wave_at) {
+      const bool edge = s.causal && (int64_t)at * F::TR < (int64_t)wave_full * s.G;
+#pragma unroll
+      for (int i = 0; i < F::TR / 32; ++i) {
+        floatx16 p[1] = {splat(0.f)}, ds[1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
+        mma_rows<T, DP, 1>(qt, i, k, p);
+        mma_rows<T, DP, 1>(dt, i, v, ds);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
+        Packed<T> x[1];
+        x[0].set(p[0]);
+        mma_cols<T, DP, 1>(dt, i, x, dv);
+        range.fit(ds[0], dk[0]);
+        x[0].set(ds[0]);
+        mma_cols<T, DP, 1>(qt, i, x, dk);
+      }
+    }
+    buf ^= 1;
+  }
+  if (key >= s.Tk) return;
+  const int64_t to = (((int64_t)b * s.Tk + key) * s.Hk + hk) * s.D;
+  const float fv = live ? exp2_(-kPExp<T>) : 0.f;
+  const float fk = live ? s.scale * exp2_(-kPExp<T>) * range.undo() : 0.f;
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      float x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a key that is left out: zeros, whatever was formed
+        x[i] = live ? dk[0][n][4 * e4 + i] * fk : 0.f;
+        y[i] = live ? dv[0][n][4 * e4 + i] * fv : 0.f;
+      }
+      if (a.dk) store_quad<T>(reinterpret_cast<T *>(a.dk) + to, 32 * n + entry(4 * e4), s.D, x);
+      if (a.dv) store_quad<T>(reinterpret_cast<T *>(a.dv) + to, 32 * n + entry(4 * e4), s.D, y);
+    }
+}
+
+template <typename T, int DP>
+int launch(BwdArgs a, hipStream_t st) {
+  const int64_t heads = (int64_t)a.s.B * a.s.Hk;
+  if (a.s.R <= 32) {
+    a.tiles = 1;
+    attn_dq_kernel<T, DP, 4><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+  } else {
+    a.tiles = (a.s.R + Dq<T, DP, 1>::BR - 1) / Dq<T, DP, 1>::BR;
+    attn_dq_kernel<T, DP, 1><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+  }
+  if (a.dk || a.dv) {
+    a.tiles = (a.s.Tk + Dkv<T, DP>::BK - 1) / Dkv<T, DP>::BK;
+    attn_dkv_kernel<T, DP><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+  }
+  return check_launch("nf_attention_bwd");
+}
+
+size_t delta_bytes(const Sizes &z) { return (size_t)(z.B * z.Hk * z.rows()) * 4; }
+
+}  // namespace
+}  // namespace attn
+}  // namespace nf
+
+using namespace nf;
+using namespace nf::attn;
+
+extern "C" size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                                             int64_t Hk, int64_t D, int dtype) {
+  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
+  return check_sizes("nf_attention_bwd_workspace", z) ? 0 : delta_bytes(z);
+}
+
+extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
+                                int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
+                                int64_t v_t, int64_t v_h, const void *out, const void *dout,
+                                int64_t g_b, int64_t g_t, int64_t g_h, int64_t B, int64_t Tq,
+                                int64_t Tk, int64_t H, int64_t Hk, int64_t D, int causal,
+                                float scale, int has_mask, int dtype, const void *state,
+                                size_t state_bytes, void *dq, void *dk, void *dv, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+  const char *op = "nf_attention_bwd";
+  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
+  if (const int rc = check_sizes(op, z)) return rc;
+  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
+  if (B == 0 || Tq == 0 || (!dq && !dk && !dv)) return NF_OK;
+  if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
+  const State parts = state_of(z, has_mask, true);
+  if (state_bytes < parts.total || workspace_bytes < delta_bytes(z))
+    return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
+                     state_bytes, parts.total, workspace_bytes, delta_bytes(z));
+  if (!out || !state || !aligned16(state) || !workspace || !aligned16(workspace))
+    return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
+  BwdArgs a = {};
+  if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
+  if (const int rc = make_view(op, "k", k, k_b, k_t, k_h, z, 0, &a.k)) return rc;
+  if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
+  if (const int rc = make_view(op, "dout", dout, g_b, g_t, g_h, z, H / Hk, &a.dout)) return rc;
+  const char *st = static_cast<const char *>(state);
+  a.s = make_shape(z, causal, scale,
+                   has_mask ? reinterpret_cast<const uint64_t *>(st + parts.bits) : nullptr);
+  a.out = static_cast<const char *>(out);
+  a.low = z.es() == 2 ? st + parts.low : nullptr;
+  a.lse = reinterpret_cast<const float *>(st + parts.lse);
+  a.ndelta = static_cast<float *>(workspace);
+  a.dq = static_cast<char *>(dq);
+  a.dk = static_cast<char *>(dk);
+  a.dv = static_cast<char *>(dv);
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+#define NF_ATTN(DT, T) \
+  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, hs) : launch<T, 128>(a, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16)
+  NF_ATTN(NF_DTYPE_F16, f16)
+  NF_ATTN(NF_DTYPE_F32, float)
+#undef NF_ATTN
+  return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
+}

@@ -1,0 +1,483 @@
+// Attention, forward: out = softmax(scale q k^T over the keys that may be attended) v.
+//
+// One pass over the keys with a running maximum m and sum l: with c = |scale| log2(e) and S the
+// bare products, p = 2^(c S - m), l += sum p, O += p v; where m grows, O and l are scaled by
+// 2^(m_old - m_new); out = O / l, and the row's log-sum-exp is m + log2(l).
+#include <math.h>
+
+#include "attention.h"
+
+namespace nf {
+namespace attn {
+namespace {
+
+// m is raised only when a logit passes it by kSlack (in powers of two): p is then at most 2^kSlack,
+// which every type holds, and most tiles leave O as it is.
+constexpr float kSlack = 8.f;
+// fp16 ends at 2^-24: p carries a factor 2^7, so that it is normal down to 2^-21 of the largest.
+template <typename T>
+constexpr float kBias = __is_same(T, f16) ? 7.f : 0.f;
+
+struct FwdArgs {
+  Shape s;
+  View q, k, v;
+  char *out;     // [B, Tq, H, D]
+  char *low;     // what out's rounding left, the same layout; null: not kept
+  float *lse;    // [B Hk, R] in powers of two; null: not kept
+  float *part;   // splits > 1: O [splits][B Hk R][DP], then (m, l) pairs
+  int splits, tiles;
+};
+
+// KW = 1: a wavefront has 32 rows of its own, a block 128.  KW = 4: a block has 32 rows, and a
+// wavefront a quarter of each tile's keys.
+template <typename T, int DP, int KW>
+struct Fwd {
+  using C = Tile<T, DP>;
+  static constexpr int BR = KW == 1 ? 32 * kWaves : 32;           // rows of a block
+  static constexpr int TK = KW == 4 ? 128 : (C::ROW > 256 ? 32 : 64);  // keys of a tile
+  static constexpr int NK = KW == 4 ? 1 : TK / 32;                // of those, 32s of a wavefront
+  static constexpr int TILE = TK * C::ROW;
+  static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int LDS = STAGES * 2 * TILE;
+};
+
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
+    FwdArgs a) {
+  using F = Fwd<T, DP, KW>;
+  using C = Tile<T, DP>;
+  __shared__ __attribute__((aligned(16))) char smem[F::LDS];
+  const Shape &s = a.s;
+  int bh, job;
+  if (!place(s.B * s.Hk, a.tiles * a.splits, &bh, &job)) return;
+  const int split = job % a.splits;
+  const int tile = a.tiles - 1 - job / a.splits;  // causal: the longest first
+  const int b = bh / s.Hk, hk = bh % s.Hk;
+  const int l = threadIdx.x & 63, h = l >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = tile * F::BR + (KW == 1 ? 32 * wave : 0);  // the wavefront's first row
+  const int rows_end = min(tile * F::BR + F::BR, s.R);
+
+  // the lane's row
+  const int r = r0 + (l & 31);
+  const int rc = min(r, s.R - 1), t = rc / s.G, g = rc - t * s.G;
+  u32x4 q[1][C::KS];
+  load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
+                  s.flip, q[0]);
+  const int last = s.causal ? t + s.off : s.Tk - 1;  // the lane's last key
+  // the wavefront's and the block's
+  const int first_t = min(r0, s.R - 1) / s.G;
+  const int wave_least = s.causal ? first_t + s.off : s.Tk - 1;
+  const int wave_last = s.causal ? min(r0 + 31, s.R - 1) / s.G + s.off : s.Tk - 1;
+  const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
+  int end = block_last < 0 ? 0 : block_last / F::TK + 1, at = 0;
+  if (a.splits > 1) {
+    const int all = (s.Tk + F::TK - 1) / F::TK;
+    at = (int)((int64_t)all * split / a.splits);
+    end = min(end, (int)((int64_t)all * (split + 1) / a.splits));
+  }
+
+  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
+  const char *kp = a.k.p + b * a.k.b + hk * a.k.h, *vp = a.v.p + b * a.v.b + hk * a.v.h;
+  KeyBits<F::TK> cur, nxt;
+  auto seek = [&](int i, KeyBits<F::TK> &w) {  // the next tile that has keys
+    for (; i < end; ++i) {
+      w.load(bits, s.words, i);
+      if (w.any()) break;
+    }
+    return i;
+  };
+  auto copy = [&](int i, const KeyBits<F::TK> &w, char *buf) {
+    const int left = s.Tk - i * F::TK;
+    const bool whole = w.all();
+    const uint32_t kt = (uint32_t)a.k.t, vt = (uint32_t)a.v.t;
+    copy_tile<T, DP, F::TK>(kp + (int64_t)i * F::TK * a.k.t, s.nvec, buf, wave,
+                            [&](int row, bool *in) {
+                              *in = row < left && (whole || w.has(row));
+                              return (uint32_t)row * kt;
+                            });
+    copy_tile<T, DP, F::TK>(vp + (int64_t)i * F::TK * a.v.t, s.nvec, buf + F::TILE, wave,
+                            [&](int row, bool *in) {
+                              *in = row < left && (whole || w.has(row));
+                              return (uint32_t)row * vt;
+                            });
+  };
+
+  floatx16 o[1][C::NB];
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n) o[0][n] = splat(0.f);
+  float m = -kInf, sum = 0.f;  // sum: of the lane's own entries
+
+  at = seek(at, cur);
+  int buf = 0;
+  if (at < end) copy(at, cur, smem);
+  while (at < end) {
+    const int next = seek(at + 1, nxt);
+    gemm::wait_vm_barrier<0>();
+    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
+    const int key0 = at * F::TK + (KW == 4 ? 32 * wave : 0);
+    if (key0 <= wave_last && key0 < s.Tk) {
+      const int kb0 = KW == 4 ? wave : 0;
+      floatx16 p[F::NK];
+#pragma unroll
+      for (int i = 0; i < F::NK; ++i) {
+        floatx16 acc[1] = {splat(0.f)};
+        mma_rows<T, DP, 1>(kt, kb0 + i, q, acc);
+        p[i] = acc[0];
+      }
+      if (key0 + 32 * F::NK - 1 > min(wave_least, s.Tk - 1) || !cur.all()) {
+#pragma unroll
+        for (int i = 0; i < F::NK; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int in = 32 * i + entry(e);
+            const bool live = key0 + in <= last && cur.has(32 * kb0 + in);
+            p[i][e] = live ? p[i][e] : -kInf;
+          }
+      }
+      float top = p[0][0];
+#pragma unroll
+      for (int i = 0; i < F::NK; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, p[i][e]);
+      top = pair_max(top) * s.c - kBias<T>;
+      if (__any(top > m + kSlack)) {
+        const float up = fmaxf(m, top);
+        const float f = exp2_(m - (up == -kInf ? 0.f : up));
+        m = up;
+        sum *= f;
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) o[0][n] *= f;
+      }
+      const float base = m == -kInf ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < F::NK; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p[i][e] = exp2_(fmaf(p[i][e], s.c, -base));
+          sum += p[i][e];
+        }
+        Packed<T> x[1];
+        x[0].set(p[i]);
+        mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
+      }
+    }
+    if (F::STAGES == 1) {
+      __syncthreads();
+      if (next < end) copy(next, nxt, smem);
+    } else {
+      buf ^= 1;
+    }
+    at = next;
+    cur = nxt;
+  }
+  sum = pair_sum(sum);
+
+  if constexpr (KW == 4) {  // the four wavefronts' parts of the same rows
+    __syncthreads();
+    float *stat = reinterpret_cast<float *>(smem);  // [4][2][32], then O [4][DP][32]
+    float *os = stat + 4 * 64;
+    if (h == 0) {
+      stat[wave * 64 + l] = m;
+      stat[wave * 64 + 32 + l] = sum;
+    }
+    __syncthreads();
+    float top = -kInf, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w * 64 + (l & 31)]);
+    const float base = top == -kInf ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      total += stat[w * 64 + 32 + (l & 31)] * exp2_(stat[w * 64 + (l & 31)] - base);
+    const float f = exp2_(m - base);
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        os[(wave * DP + 32 * n + entry(e)) * 32 + (l & 31)] = o[0][n][e] * f;
+    __syncthreads();
+    // wavefront w takes columns w DP / 4 .. of every row
+    m = top;
+    sum = total;
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (((32 * n + 8 * (e / 4)) * 4) / DP != wave) continue;
+        const int at_ = (32 * n + entry(e)) * 32 + (l & 31);
+        o[0][n][e] = ((os[at_] + os[DP * 32 + at_]) + os[2 * DP * 32 + at_]) + os[3 * DP * 32 + at_];
+      }
+  }
+  if (r >= s.R) return;
+  const bool lead = KW == 1 || wave == 0;
+  const int64_t row = (int64_t)bh * s.R + r;
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)s.B * s.Hk * s.R;
+    float *op = a.part + ((int64_t)split * rows + row) * DP;
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
+        const float x[4] = {o[0][n][4 * e4], o[0][n][4 * e4 + 1], o[0][n][4 * e4 + 2],
+                            o[0][n][4 * e4 + 3]};
+        store_quad<float>(op, 32 * n + entry(4 * e4), DP, x);
+      }
+    if (lead && h == 0) {
+      float *ml = a.part + (int64_t)a.splits * rows * DP + ((int64_t)split * rows + row) * 2;
+      ml[0] = m;
+      ml[1] = sum;
+    }
+    return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: 0; a NaN stays one
+  const int64_t to = (((int64_t)b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
+  T *out = reinterpret_cast<T *>(a.out) + to;
+  T *low = a.low ? reinterpret_cast<T *>(a.low) + to : nullptr;
+#pragma unroll
+  for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
+      float x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = o[0][n][4 * e4 + i] * inv;
+        y[i] = x[i] - to_f32(from_f32<T>(x[i]));
+      }
+      store_quad<T>(out, 32 * n + entry(4 * e4), s.D, x);
+      if (low) store_quad<T>(low, 32 * n + entry(4 * e4), s.D, y);
+    }
+  if (a.lse && lead && h == 0) a.lse[row] = sum == 0.f ? kInf : m + __log2f(sum);
+}
+
+// Joins the splits of a row, in their order: one wavefront a row, a lane DP / 64 columns.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
+  const Shape &s = a.s;
+  const int64_t rows = (int64_t)s.B * s.Hk * s.R;
+  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int l = threadIdx.x & 63;
+  const float *ml = a.part + (int64_t)a.splits * rows * DP;
+  float top = -kInf;
+  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, ml[(i * rows + row) * 2]);
+  const float base = top == -kInf ? 0.f : top;
+  float sum = 0.f, o[DP / 64];
+#pragma unroll
+  for (int j = 0; j < DP / 64; ++j) o[j] = 0.f;
+  for (int i = 0; i < a.splits; ++i) {
+    const float f = exp2_(ml[(i * rows + row) * 2] - base);
+    sum += ml[(i * rows + row) * 2 + 1] * f;
+    const float *p = a.part + (i * rows + row) * DP;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) o[j] += p[l + 64 * j] * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t bh = row / s.R, r = row % s.R;
+  const int64_t b = bh / s.Hk, hk = bh % s.Hk, t = r / s.G, g = r % s.G;
+  const int64_t to = ((b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
+#pragma unroll
+  for (int j = 0; j < DP / 64; ++j) {
+    const int d = l + 64 * j;
+    if (d >= s.D) continue;
+    const float x = o[j] * inv;
+    reinterpret_cast<T *>(a.out)[to + d] = from_f32<T>(x);
+    if (a.low) reinterpret_cast<T *>(a.low)[to + d] = from_f32<T>(x - to_f32(from_f32<T>(x)));
+  }
+  if (a.lse && l == 0) a.lse[row] = sum == 0.f ? kInf : top + __log2f(sum);
+}
+
+// The mask's bytes [B, Tk] as words of 64 keys: a wavefront a word.
+__global__ __launch_bounds__(kThreads) void attn_bits_kernel(const uint8_t *mask, int64_t mb,
+                                                             int64_t mt, int B, int Tk, int words,
+                                                             uint64_t *bits) {
+  const int64_t i = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (i >= (int64_t)B * words) return;
+  const int64_t b = i / words, key = (i % words) * 64 + (threadIdx.x & 63);
+  const uint64_t w = __ballot(key < Tk && mask[b * mb + key * mt] != 0);
+  if ((threadIdx.x & 63) == 0) bits[i] = w;
+}
+
+struct Plan {
+  int kw, tiles, splits;
+};
+
+// Up to 32 rows a key head: the wavefronts of a block share them.  The keys are split over blocks
+// where the blocks are fewer than kFill, into parts of at least 4 tiles.
+Plan plan_of(const Sizes &z) {
+  constexpr int64_t kFill = 512;
+  Plan p;
+  const int64_t R = z.rows(), heads = z.B * z.Hk;
+  p.kw = R <= 32 ? 4 : 1;
+  p.tiles = (int)((R + (p.kw == 4 ? 31 : 127)) / (p.kw == 4 ? 32 : 128));
+  const int tk = p.kw == 4 ? 128 : (z.dp() * z.es() > 256 ? 32 : 64);
+  const int64_t steps = (z.Tk + tk - 1) / tk, blocks = heads * p.tiles;
+  int64_t n = blocks >= kFill / 2 ? 1 : kFill / blocks;
+  if (n > steps / 4) n = steps / 4;
+  p.splits = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+  return p;
+}
+
+size_t part_bytes(const Sizes &z) {
+  const Plan p = plan_of(z);
+  if (p.splits <= 1) return 0;
+  return (size_t)p.splits * (size_t)(z.B * z.Hk * z.rows()) * (size_t)(z.dp() + 2) * 4;
+}
+
+template <typename T, int DP>
+int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
+  const unsigned grid =
+      (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.splits);
+  if (p.kw == 4)
+    attn_fwd_kernel<T, DP, 4><<<grid, kThreads, 0, st>>>(a);
+  else
+    attn_fwd_kernel<T, DP, 1><<<grid, kThreads, 0, st>>>(a);
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
+    attn_join_kernel<T, DP><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+  }
+  return check_launch("nf_attention_fwd");
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// host, shared with the backward
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxBlocks = (int64_t)1 << 23;
+
+int check_sizes(const char *op, const Sizes &z) {
+  if (!is_dtype(z.dtype)) return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, z.dtype);
+  if (z.B < 0 || z.Tq < 0 || z.Tk < 0 || z.H <= 0 || z.Hk <= 0 || z.H % z.Hk)
+    return set_error(NF_ERR_ARG, "%s: B=%lld Tq=%lld Tk=%lld H=%lld Hk=%lld", op, (long long)z.B,
+                     (long long)z.Tq, (long long)z.Tk, (long long)z.H, (long long)z.Hk);
+  if (z.D <= 0 || z.D > 128)
+    return set_error(NF_ERR_ARG, "%s: D=%lld outside [1, 128]", op, (long long)z.D);
+  const int64_t most = (int64_t)1 << 30;
+  if (z.B > most || z.H > most / 1024 || z.Tq > most || z.Tk > most || z.rows() > most ||
+      z.B * z.Hk > most || z.B * z.Hk * ((z.rows() + 31) / 32 + 1) > kMaxBlocks ||
+      z.B * z.Hk * ((z.Tk + 31) / 32 + 1) > kMaxBlocks)
+    return set_error(NF_ERR_ARG, "%s: B=%lld Tq=%lld Tk=%lld H=%lld Hk=%lld too large", op,
+                     (long long)z.B, (long long)z.Tq, (long long)z.Tk, (long long)z.H,
+                     (long long)z.Hk);
+  return NF_OK;
+}
+
+// `group`: heads between the first and the last element that a tile of one key head reads.
+int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
+              const Sizes &z, int64_t group, View *v) {
+  const int es = z.es();
+  if (!p) return set_error(NF_ERR_ARG, "%s: %s is null", op, name);
+  if (!aligned16(p) || sb * es % 16 || st * es % 16 || sh * es % 16 || sb < 0 || st < 0 || sh < 0)
+    return set_error(NF_ERR_ARG, "%s: %s: rows of 16-byte vectors expected", op, name);
+  // a tile's offsets, 128 rows and a group of heads, fit the buffer unit's 31 bits
+  const int64_t most = (int64_t)1 << 30;
+  if (st > most / 512 || sh > most || 130 * st * es + group * sh * es >= most)
+    return set_error(NF_ERR_ARG, "%s: %s: strides too large", op, name);
+  *v = View{static_cast<const char *>(p), sb * es, st * es, sh * es};
+  return NF_OK;
+}
+
+Shape make_shape(const Sizes &z, int causal, float scale, const uint64_t *bits) {
+  Shape s;
+  s.B = (int)z.B;
+  s.Tq = (int)z.Tq;
+  s.Tk = (int)z.Tk;
+  s.H = (int)z.H;
+  s.Hk = (int)z.Hk;
+  s.G = (int)(z.H / z.Hk);
+  s.D = (int)z.D;
+  s.R = (int)z.rows();
+  const int ve = 16 / z.es();
+  s.nvec = (int)((z.D + ve - 1) / ve);
+  s.off = (int)(z.Tk - z.Tq);
+  s.causal = causal;
+  s.words = (int)z.words();
+  s.ginv = s.G == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + s.G - 1) / s.G);
+  // 0 times a barred key's -infinity would be no number: a scale that rounds every logit to 0
+  s.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+  s.scale = scale;
+  s.flip = scale < 0.f ? (z.es() == 2 ? 0x80008000u : 0x80000000u) : 0u;
+  s.bits = bits;
+  return s;
+}
+
+State state_of(const Sizes &z, bool mask, bool keep) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  State t;
+  t.lse = 0;
+  t.bits = keep ? up((size_t)(z.B * z.Hk * z.rows()) * 4) : 0;
+  t.low = t.bits + (mask ? up((size_t)(z.B * z.words()) * 8) : 0);
+  t.total = t.low + (keep && z.es() == 2 ? up((size_t)(z.B * z.Tq * z.H * z.D) * 2) : 0);
+  return t;
+}
+
+}  // namespace attn
+}  // namespace nf
+
+using namespace nf;
+using namespace nf::attn;
+
+extern "C" size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk,
+                                           int64_t D, int has_mask, int keep, int dtype) {
+  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
+  return check_sizes("nf_attention_state_bytes", z) ? 0 : state_of(z, has_mask, keep).total;
+}
+
+extern "C" size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                                             int64_t Hk, int64_t D, int dtype) {
+  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
+  if (check_sizes("nf_attention_fwd_workspace", z) || B * Tq * Tk == 0) return 0;
+  return part_bytes(z);
+}
+
+extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
+                                int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
+                                int64_t v_t, int64_t v_h, const uint8_t *key_mask, int64_t mask_b,
+                                int64_t mask_t, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                                int64_t Hk, int64_t D, int causal, float scale, int keep, int dtype,
+                                void *out, void *state, size_t state_bytes, void *workspace,
+                                size_t workspace_bytes, void *stream) {
+  const char *op = "nf_attention_fwd";
+  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
+  if (const int rc = check_sizes(op, z)) return rc;
+  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
+  if (B == 0 || Tq == 0) return NF_OK;
+  if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
+  const State parts = state_of(z, key_mask != nullptr, keep);
+  if (state_bytes < parts.total || workspace_bytes < part_bytes(z))
+    return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
+                     state_bytes, parts.total, workspace_bytes, part_bytes(z));
+  if (!out || (parts.total && (!state || !aligned16(state))) ||
+      (part_bytes(z) && (!workspace || !aligned16(workspace))))
+    return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
+  FwdArgs a = {};
+  if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
+  if (const int rc = make_view(op, "k", k, k_b, k_t, k_h, z, 0, &a.k)) return rc;
+  if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
+  char *st = static_cast<char *>(state);
+  uint64_t *bits = key_mask ? reinterpret_cast<uint64_t *>(st + parts.bits) : nullptr;
+  a.s = make_shape(z, causal, scale, bits);
+  a.out = static_cast<char *>(out);
+  a.low = keep && z.es() == 2 ? st + parts.low : nullptr;
+  a.lse = keep ? reinterpret_cast<float *>(st + parts.lse) : nullptr;
+  a.part = static_cast<float *>(workspace);
+  const Plan p = plan_of(z);
+  a.splits = p.splits;
+  a.tiles = p.tiles;
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  if (key_mask) {
+    const int64_t n = B * z.words();
+    attn_bits_kernel<<<(unsigned)((n + kWaves - 1) / kWaves), kThreads, 0, hs>>>(
+        key_mask, mask_b, mask_t, a.s.B, a.s.Tk, a.s.words, bits);
+  }
+#define NF_ATTN(DT, T)                                                   \
+  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, p, hs) : launch<T, 128>(a, p, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16)
+  NF_ATTN(NF_DTYPE_F16, f16)
+  NF_ATTN(NF_DTYPE_F32, float)
+#undef NF_ATTN
+  return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
+}

@@ -36,6 +36,8 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 constexpr int64_t kMaxRow = 16384;  // widest adaLN row the kernels take
+constexpr int64_t kMaxHead = 128;   // widest attention head
+constexpr int64_t kMaxPairs = 256, kMaxTurned = 1024;  // most rotary pairs, widest rotary head
 
 int code_of(at::ScalarType t) {
   switch (t) {
@@ -608,6 +610,189 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 // ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+// [B, T, heads, D] with the strides as nf_attention_* take them
+struct Heads {
+  Tensor t;
+  int64_t b, s, h;
+  explicit Heads(const Tensor &x) : t(x) {
+    b = x.size(0) == 1 ? 0 : x.stride(0);
+    s = x.size(1) == 1 ? 0 : x.stride(1);
+    h = x.size(2) == 1 ? 0 : x.stride(2);
+  }
+};
+
+// `t` where its rows are whole 16-byte vectors within the kernels' reach, else a copy (zeros past
+// D up to the next vector).
+Heads head_rows(const Tensor &t) {
+  const int64_t e = 16 / t.element_size(), d = t.size(3);
+  const int64_t far = ((int64_t)1 << 30) / t.element_size();
+  const Heads v(t);
+  const bool whole = d % e == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                     (t.stride(3) == 1 || d == 1) && v.b % e == 0 && v.s % e == 0 &&
+                     v.h % e == 0 && v.s <= far / 512 && 130 * v.s + t.size(2) * v.h < far;
+  if (whole) return v;
+  if (d % e) return Heads(at::constant_pad_nd(t, {0, e - d % e}, 0));
+  return Heads(t.clone(at::MemoryFormat::Contiguous));
+}
+
+struct Attention : torch::autograd::Function<Attention> {
+  struct Sizes {
+    int64_t B, Tq, Tk, H, Hk, D;
+  };
+  static Sizes sizes(const Tensor &q, const Tensor &k) {
+    return {q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), q.size(3)};
+  }
+  static Tensor run(const Sizes &z, const Heads &q, const Heads &k, const Heads &v,
+                    const Tensor &mask, bool causal, double scale, bool keep, Tensor &state) {
+    const int dt = code_of(q.t);
+    Tensor out = at::empty({z.B, z.Tq, z.H, z.D}, q.t.options().requires_grad(false));
+    const size_t n_state = nf_attention_state_bytes(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, mask.defined(),
+                                                    keep, dt);
+    const size_t n_ws = nf_attention_fwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, dt);
+    Tensor ws;
+    if (n_state) state = bytes(n_state, out);
+    if (n_ws) ws = bytes(n_ws, out);
+    const int64_t mb = mask.defined() && z.B > 1 ? mask.stride(0) : 0;
+    const int64_t mt = mask.defined() && z.Tk > 1 ? mask.stride(1) : 0;
+    check(nf_attention_fwd(q.t.data_ptr(), q.b, q.s, q.h, k.t.data_ptr(), k.b, k.s, k.h,
+                           v.t.data_ptr(), v.b, v.s, v.h, (const uint8_t *)ptr(mask), mb, mt, z.B,
+                           z.Tq, z.Tk, z.H, z.Hk, z.D, causal, (float)scale, keep, dt,
+                           out.data_ptr(), ptr(state), n_state, ptr(ws), n_ws, stream_of(out)),
+          "nf_attention_fwd");
+    return out;
+  }
+  static Tensor forward(AutogradContext *ctx, const Tensor &q_in, const Tensor &k_in,
+                        const Tensor &v_in, const std::optional<Tensor> &mask, bool causal,
+                        double scale) {
+    const c10::DeviceGuard guard(q_in.device());
+    const Heads q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in);
+    Tensor state;
+    const Tensor out = run(sizes(q_in, k_in), q, k, v, mask ? *mask : Tensor(), causal, scale,
+                           true, state);
+    ctx->save_for_backward({q.t, k.t, v.t, out, state});
+    ctx->saved_data["s"] = std::vector<int64_t>{causal, mask.has_value(), q_in.size(3)};
+    ctx->saved_data["f"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list res(6);
+    const variable_list t = ctx->get_saved_variables();
+    const auto s = ctx->saved_data["s"].toIntVector();
+    const Tensor &out = t[3], &state = t[4];
+    const c10::DeviceGuard guard(out.device());
+    TORCH_CHECK_VALUE(grads[0].device() == out.device(),
+                      "fused_attention backward: dout is not on the forward's device");
+    const Heads q(t[0]), k(t[1]), v(t[2]), g = head_rows(grads[0].to(out.scalar_type()));
+    Sizes z = sizes(q.t, k.t);
+    z.D = s[2];
+    const auto opts = out.options().requires_grad(false);
+    if (ctx->needs_input_grad(0)) res[0] = at::empty({z.B, z.Tq, z.H, z.D}, opts);
+    for (int i : {1, 2})
+      if (ctx->needs_input_grad(i)) res[i] = at::empty({z.B, z.Tk, z.Hk, z.D}, opts);
+    const int dt = code_of(out);
+    const size_t n_ws = nf_attention_bwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, dt);
+    Tensor ws = bytes(n_ws, out);
+    check(nf_attention_bwd(q.t.data_ptr(), q.b, q.s, q.h, k.t.data_ptr(), k.b, k.s, k.h,
+                           v.t.data_ptr(), v.b, v.s, v.h, out.data_ptr(), g.t.data_ptr(), g.b, g.s,
+                           g.h, z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, (int)s[0],
+                           (float)ctx->saved_data["f"].toDouble(), (int)s[1], dt, state.data_ptr(),
+                           (size_t)state.numel(), ptr(res[0]), ptr(res[1]), ptr(res[2]),
+                           ws.data_ptr(), n_ws, stream_of(out)),
+          "nf_attention_bwd");
+    return first_order_only("fused_attention", at::GradMode::is_enabled(), grads, std::move(res));
+  }
+};
+
+// ---------------------------------------------------------------------------
+// rotary positions
+// ---------------------------------------------------------------------------
+struct Rotary : torch::autograd::Function<Rotary> {
+  // q and k turned; either may be undefined.  call: joint, interleaved, then the sections
+  static variable_list run(const Tensor &q_in, const Tensor &k_in, const Tensor &pos,
+                           const std::vector<int64_t> &call, double base, bool inverse) {
+    const Tensor &like = q_in.defined() ? q_in : k_in;
+    Tensor x[2] = {q_in, k_in}, y[2];
+    int64_t st[2][3] = {}, heads[2] = {0, 0};
+    for (int i = 0; i < 2; ++i) {
+      if (!x[i].defined()) continue;
+      if (x[i].stride(3) != 1 && x[i].size(3) != 1) x[i] = x[i].contiguous();
+      y[i] = at::empty(x[i].sizes(), x[i].options().requires_grad(false));
+      for (int j = 0; j < 3; ++j) st[i][j] = x[i].stride(j);
+      heads[i] = x[i].size(2);
+    }
+    const int axes = (int)call.size() - 2;
+    int32_t sections[4];
+    for (int i = 0; i < axes; ++i) sections[i] = (int32_t)call[2 + i];
+    const int64_t B = like.size(0), T = like.size(1);
+    const bool shared = pos.dim() == 2 || pos.size(0) == 1;
+    const int kind = pos.scalar_type() == at::kLong ? 0 : pos.scalar_type() == at::kInt ? 1 : 2;
+    check(nf_rotary(ptr(x[0]), st[0][0], st[0][1], st[0][2], ptr(y[0]), heads[0], ptr(x[1]),
+                    st[1][0], st[1][1], st[1][2], ptr(y[1]), heads[1], pos.data_ptr(),
+                    shared ? 0 : T * axes, kind, B, T, like.size(3), sections, axes, base,
+                    (int)call[0], (int)call[1], inverse, code_of(like), stream_of(like)),
+          "nf_rotary");
+    return {y[0], y[1]};
+  }
+  // the tensors that are there, turned; what_of: 1 q, 2 k, 3 both
+  static variable_list forward(AutogradContext *ctx, const std::optional<Tensor> &q,
+                               const std::optional<Tensor> &k, const Tensor &pos,
+                               const std::vector<int64_t> &call, double base, bool inverse) {
+    const c10::DeviceGuard guard(pos.device());
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({pos});
+    ctx->saved_data["c"] = call;
+    ctx->saved_data["b"] = base;
+    ctx->saved_data["i"] = inverse;
+    ctx->saved_data["q"] = q.has_value();
+    ctx->saved_data["k"] = k.has_value();
+    variable_list y = run(q ? *q : Tensor(), k ? *k : Tensor(), pos, call, base, inverse);
+    variable_list there;
+    for (Tensor &t : y)
+      if (t.defined()) there.push_back(t);
+    return there;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    // an argument that was left out has neither an output nor an edge
+    const bool has[2] = {ctx->saved_data["q"].toBool(), ctx->saved_data["k"].toBool()};
+    Tensor g[2];
+    for (int i = 0, at = 0; i < 2; ++i) {
+      if (!has[i]) continue;
+      if (ctx->needs_input_grad(at)) g[i] = grads[at];
+      ++at;
+    }
+    variable_list res(6);
+    if (!g[0].defined() && !g[1].defined()) return res;
+    const Tensor pos = ctx->get_saved_variables()[0];
+    const auto call = ctx->saved_data["c"].toIntVector();
+    const double base = ctx->saved_data["b"].toDouble();
+    const bool inverse = ctx->saved_data["i"].toBool();
+    bool recording = false;
+    for (const Tensor &t : g) {
+      TORCH_CHECK_VALUE(!t.defined() || t.device() == pos.device(),
+                        "fused_rotary backward: a gradient is not on the forward's device");
+      recording |= at::GradMode::is_enabled() && t.defined() && t.requires_grad();
+    }
+    const c10::DeviceGuard guard(pos.device());
+    if (!recording) {
+      const variable_list y = run(g[0], g[1], pos, call, base, !inverse);
+      res[0] = y[0];
+      res[1] = y[1];
+    } else {  // linear in the gradients
+      auto given = [](const Tensor &v) {
+        return v.defined() ? std::optional<Tensor>(v) : std::nullopt;
+      };
+      const variable_list y = Rotary::apply(given(g[0]), given(g[1]), pos, call, base, !inverse);
+      size_t at = 0;
+      for (int i = 0; i < 2; ++i)
+        if (g[i].defined()) res[i] = y[at++];
+    }
+    return res;
+  }
+};
+
+// ---------------------------------------------------------------------------
 // entries
 // ---------------------------------------------------------------------------
 // The call's leading `n` arguments as tensors; false when one is not.
@@ -829,6 +1014,106 @@ PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// q [B, Tq, H, D], k, v [B, Tk, Hk, D], key_mask [B, Tk] or None, causal, scale
+PyObject *py_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[3], mask;
+  if (!tensors(args, nargs, 6, t) || !quiet() || !PyFloat_CheckExact(args[5])) Py_RETURN_NONE;
+  const c10::Device dev = t[0].device();
+  for (const Tensor &x : t)
+    if (!plain(x, dev) || x.dim() != 4 || x.numel() == 0 || code_of(x) < 0 ||
+        x.scalar_type() != t[0].scalar_type())
+      Py_RETURN_NONE;
+  if (t[1].sizes() != t[2].sizes() || t[1].size(0) != t[0].size(0) ||
+      t[1].size(3) != t[0].size(3) || t[0].size(2) % t[1].size(2) || t[0].size(3) > kMaxHead)
+    Py_RETURN_NONE;
+  if (args[3] != Py_None) {
+    if (!THPVariable_CheckExact(args[3])) Py_RETURN_NONE;
+    mask = THPVariable_Unpack(args[3]);
+    if (!plain(mask, dev) || mask.scalar_type() != at::kBool || mask.dim() != 2 ||
+        mask.size(0) != t[1].size(0) || mask.size(1) != t[1].size(1))
+      Py_RETURN_NONE;
+  }
+  const bool causal = args[4] == Py_True;
+  const double scale = PyFloat_AS_DOUBLE(args[5]);
+  if (!std::isfinite((float)scale)) Py_RETURN_NONE;
+  return THPVariable_Wrap(unlocked([&]() -> Tensor {
+    if (wants_grad({&t[0], &t[1], &t[2]}))
+      return Attention::apply(t[0], t[1], t[2],
+                              mask.defined() ? std::optional<Tensor>(mask) : std::nullopt, causal,
+                              scale);
+    const c10::DeviceGuard guard(dev);
+    const at::NoGradGuard no_grad;
+    Tensor state;
+    return Attention::run(Attention::sizes(t[0], t[1]), head_rows(t[0]), head_rows(t[1]),
+                          head_rows(t[2]), mask, causal, scale, false, state);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+// q [B, T, H, D], k [B, T, Hk, D] or None, positions [B, T, axes] or [T, axes], sections (a tuple
+// of ints), base, ladder, interleaved -> (q, k)
+PyObject *py_rotary(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7 || !quiet() || !THPVariable_CheckExact(args[0]) ||
+      !THPVariable_CheckExact(args[2]) || !PyTuple_CheckExact(args[3]) ||
+      !PyFloat_CheckExact(args[4]) || !PyUnicode_CheckExact(args[5]))
+    Py_RETURN_NONE;
+  const Tensor q = THPVariable_Unpack(args[0]), pos = THPVariable_Unpack(args[2]);
+  Tensor k;
+  const c10::Device dev = q.device();
+  if (!plain(q, dev) || q.dim() != 4 || q.numel() == 0 || code_of(q) < 0 || !plain(pos, dev) ||
+      !pos.is_contiguous() || pos.requires_grad())
+    Py_RETURN_NONE;
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+  if (args[1] != Py_None) {
+    if (!THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    k = THPVariable_Unpack(args[1]);
+    if (!plain(k, dev) || k.dim() != 4 || k.numel() == 0 || k.scalar_type() != q.scalar_type() ||
+        k.size(0) != B || k.size(1) != T || k.size(3) != D)
+      Py_RETURN_NONE;
+  }
+  const Py_ssize_t axes = PyTuple_GET_SIZE(args[3]);
+  if (axes < 1 || axes > 4) Py_RETURN_NONE;
+  std::vector<int64_t> call(2 + axes);
+  const bool joint = PyUnicode_CompareWithASCIIString(args[5], "joint") == 0;
+  if (!joint && PyUnicode_CompareWithASCIIString(args[5], "axis") != 0) Py_RETURN_NONE;
+  call[0] = joint;
+  call[1] = args[6] == Py_True;
+  int64_t pairs = 0;
+  for (Py_ssize_t i = 0; i < axes; ++i) {
+    PyObject *const o = PyTuple_GET_ITEM(args[3], i);
+    if (!PyLong_CheckExact(o)) Py_RETURN_NONE;
+    const int64_t n = PyLong_AsLongLong(o);
+    if (n == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (n < 0 || n > kMaxPairs) Py_RETURN_NONE;
+    call[2 + i] = n;
+    pairs += n;
+  }
+  const double base = PyFloat_AS_DOUBLE(args[4]);
+  const at::ScalarType pt = pos.scalar_type();
+  if (pairs < 1 || pairs > kMaxPairs || 2 * pairs > D || D > kMaxTurned || !(base > 0.0) ||
+      !std::isfinite(base) || (pt != at::kLong && pt != at::kInt && pt != at::kFloat) ||
+      pos.size(-1) != axes || pos.dim() < 2 || pos.dim() > 3 || pos.size(-2) != T ||
+      (pos.dim() == 3 && pos.size(0) != B && pos.size(0) != 1))
+    Py_RETURN_NONE;
+  const variable_list r = unlocked([&]() -> variable_list {
+    if (wants_grad({&q, &k}))
+      return Rotary::apply(std::optional<Tensor>(q),
+                           k.defined() ? std::optional<Tensor>(k) : std::nullopt, pos, call, base,
+                           false);
+    const c10::DeviceGuard guard(dev);
+    const at::NoGradGuard no_grad;
+    return Rotary::run(q, k, pos, call, base, false);
+  });
+  PyObject *tuple = PyTuple_New(2);
+  if (!tuple) return nullptr;
+  for (int i = 0; i < 2; ++i)
+    PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap((size_t)i < r.size() ? r[i] : Tensor()));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
 // op's name, the upstream gradients and the results of a backward in Python (tuples of tensors and
 // Nones) -> the results under create_graph (see first_order_only above)
 PyObject *py_first_order_only(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -858,6 +1143,8 @@ PyMethodDef kMethods[] = {
     {"ce", (PyCFunction)(void (*)(void))py_ce, METH_FASTCALL, nullptr},
     {"token_logprobs", (PyCFunction)(void (*)(void))py_token_logprobs, METH_FASTCALL, nullptr},
     {"embedding", (PyCFunction)(void (*)(void))py_embedding, METH_FASTCALL, nullptr},
+    {"attention", (PyCFunction)(void (*)(void))py_attention, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
     {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods,

@@ -120,3 +120,48 @@ def dropout_ref(x, threshold, seed, offset, residual):
     f = 65536.0 / (65536 - threshold) if threshold < 65536 else 0.0
     y = torch.where(keep, x.float() * f, 0.0)
     return y.to(x.dtype) if residual is None else (y + residual.float()).to(residual.dtype)
+
+
+def attention_ref(q, k, v, causal, key_mask, scale):
+    """softmax(scale q k^T) v in fp32 over the keys that a row may attend, cast to q's type; a
+    row without one gives 0.  Keys that ``key_mask`` drops are replaced, not multiplied away."""
+    b, tq, h, d = q.shape
+    tk, hk = k.shape[1:3]
+    if key_mask is not None:
+        k, v = (torch.where(key_mask[..., None, None], t, 0.0) for t in (k, v))
+    qf = q.float().reshape(b, tq, hk, h // hk, d).permute(0, 2, 3, 1, 4)  # [B, Hk, G, Tq, D]
+    kf = k.float().permute(0, 2, 3, 1).contiguous()[:, :, None]
+    vf = v.float().permute(0, 2, 1, 3).contiguous()[:, :, None]
+    z = torch.matmul(qf, kf) * scale
+    barred = torch.zeros(b, 1, 1, tq, tk, dtype=torch.bool, device=q.device)
+    if causal:
+        barred = barred | torch.ones(tq, tk, dtype=torch.bool, device=q.device).triu(tk - tq + 1)
+    if key_mask is not None:
+        barred = barred | ~key_mask[:, None, None, None]
+    z = z.masked_fill(barred, -math.inf)
+    top = z.detach().amax(-1, keepdim=True) if tk else z.new_zeros(*z.shape[:-1], 1)
+    e = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
+    total = e.sum(-1, keepdim=True)
+    out = torch.matmul(e / torch.where(total == 0.0, 1.0, total), vf)
+    return out.permute(0, 3, 1, 2, 4).reshape(b, tq, h, d).to(q.dtype)
+
+
+def rotary_ref(x, positions, sections, base, joint, interleaved):
+    """x [B, T, heads, D] with pair j turned by its axis's coordinate times its frequency: angles
+    in fp64, the turn in fp32, cast to x's type."""
+    pairs, turns, axis = sum(sections), [], []
+    for a, n in enumerate(sections):
+        for i in range(n):
+            turns.append(base ** -(len(turns) / pairs if joint else i / n))
+            axis.append(a)
+    freq = torch.tensor(turns, dtype=torch.float64, device=x.device)
+    angle = (positions.detach()[..., axis].double() * freq)[..., None, :]
+    cos, sin = angle.cos().float(), angle.sin().float()
+    y = x.float()
+    if interleaved:
+        u, v = y[..., 0:2 * pairs:2], y[..., 1:2 * pairs:2]
+    else:
+        u, v = y[..., :pairs], y[..., pairs:2 * pairs]
+    u, v = u * cos - v * sin, u * sin + v * cos
+    turned = torch.stack((u, v), -1).flatten(-2) if interleaved else torch.cat((u, v), -1)
+    return torch.cat((turned, y[..., 2 * pairs:]), -1).to(x.dtype)

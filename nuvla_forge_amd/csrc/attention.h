@@ -271,40 +271,86 @@ __device__ __forceinline__ int entry(int i) {
 // ---------------------------------------------------------------------------
 // tiles of keys
 // ---------------------------------------------------------------------------
-// The keys of a tile that the mask leaves, 64 to a word; TK = 32: the tile's half of a word.
-template <int TK>
-struct KeyBits {
-  static constexpr int N = TK > 64 ? TK / 64 : 1;
-  uint64_t w[N];
-  __device__ __forceinline__ void load(const uint64_t *bits, int words, int tile) {
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {  // in scalar registers
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// The keys of 32 that a lane's row may attend: those up to `last` (of the 32; negative: none) whose
+// bit is in `word`, shifted so that entry i is bit 8 (i / 4) + i % 4 for every lane.
+__device__ __forceinline__ uint32_t live32(int last, uint32_t word) {
+  const uint32_t upto = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
+  return (upto & word) >> (4 * ((threadIdx.x & 63) >> 5));
+}
+// x where entry i is live, else `other`.
+__device__ __forceinline__ float keep(float x, uint32_t live, int i, uint32_t other) {
+  const uint32_t m = (uint32_t)((int32_t)(live << (31 - (8 * (i / 4) + i % 4))) >> 31);
+  return __uint_as_float((__float_as_uint(x) & m) | (other & ~m));
+}
+constexpr uint32_t kMinusInf = 0xff800000u;
+
+// A key head's keys and values, tile by tile of TK, into LDS: K, then V.  MASKED: with the sample's
+// mask words; tiles without a key are passed over.
+template <typename T, int DP, int TK, bool MASKED>
+struct KeyTiles {
+  static constexpr int TILE = TK * Tile<T, DP>::ROW;
+  static constexpr int N = MASKED ? (TK + 63) / 64 : 0;
+  struct Bits {
+    uint64_t w[N ? N : 1];
+    // the 32 of them from key 32 i of the tile
+    __device__ __forceinline__ uint32_t half(int i) const {
+      if constexpr (!MASKED) return ~0u;
+      uint64_t x = w[0];
+      if constexpr (N == 2) x = i >= 2 ? w[1] : w[0];
+      return (uint32_t)(x >> (32 * (i & 1)));
+    }
+  };
+  const Shape &s;
+  const char *k, *v;
+  int64_t kt, vt;  // bytes from key to key
+  const uint64_t *bits;
+  int end;  // the first tile that is not wanted
+
+  __device__ __forceinline__ KeyTiles(const Shape &s_, const View &kv, const View &vv, int b,
+                                      int hk, int end_)
+      : s(s_), k(kv.p + b * kv.b + hk * kv.h), v(vv.p + b * vv.b + hk * vv.h), kt(kv.t), vt(vv.t),
+        bits(MASKED ? s_.bits + (int64_t)b * s_.words : nullptr), end(end_) {}
+
+  // the first tile from i on that has keys, and its bits
+  __device__ __forceinline__ int seek(int i, Bits &x) const {
+    if constexpr (MASKED) {
+      for (; i < end; ++i) {
+        uint64_t any = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (!bits) {
-        w[i] = ~0ull;
-      } else if constexpr (TK == 32) {
-        w[i] = (bits[tile >> 1] >> (32 * (tile & 1))) & 0xffffffffull;
-      } else {
-        w[i] = tile * N + i < words ? bits[tile * N + i] : 0ull;
+        for (int j = 0; j < N; ++j) {
+          if constexpr (TK == 32)
+            x.w[j] = uniform(bits[i >> 1] >> (32 * (i & 1))) & 0xffffffffull;
+          else
+            x.w[j] = i * N + j < s.words ? uniform(bits[i * N + j]) : 0ull;
+          any |= x.w[j];
+        }
+        if (any) break;
       }
     }
+    return i;
   }
-  __device__ __forceinline__ bool any() const {
-    uint64_t x = w[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) x |= w[i];
-    return x != 0;
+  __device__ __forceinline__ void copy_one(const char *p, int64_t step, int i, const Bits &x,
+                                           char *lds, int wave) const {
+    const int left = s.Tk - i * TK;
+    const uint32_t st = (uint32_t)step;
+    copy_tile<T, DP, TK>(p + (int64_t)i * TK * step, s.nvec, lds, wave, [&](int row, bool *in) {
+      *in = row < left;
+      if constexpr (MASKED) {
+        uint64_t w = x.w[0];
+        if constexpr (N == 2) w = row >= 64 ? x.w[1] : x.w[0];
+        *in = *in && (w >> (row & 63) & 1);
+      }
+      return (uint32_t)row * st;
+    });
   }
-  __device__ __forceinline__ bool all() const {
-    uint64_t x = w[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) x &= w[i];
-    return (TK == 32 ? (x | ~0xffffffffull) : x) == ~0ull;
-  }
-  __device__ __forceinline__ bool has(int row) const {
-    uint64_t x = w[0];
-    if constexpr (N == 2) x = row >= 64 ? w[1] : w[0];
-    if constexpr (N == 4) x = row >= 128 ? (row >= 192 ? w[3] : w[2]) : (row >= 64 ? w[1] : w[0]);
-    return (x >> (row & 63)) & 1;
+  __device__ __forceinline__ void copy(int i, const Bits &x, char *lds, int wave) const {
+    copy_one(k, kt, i, x, lds, wave);
+    copy_one(v, vt, i, x, lds + TILE, wave);
   }
 };
 

@@ -10,6 +10,8 @@
 // be the largest error of dS where a row attends few keys.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention.h"
 
 namespace nf {
@@ -66,21 +68,22 @@ constexpr float kPExp = __is_same(T, f16) ? 15.f : 0.f;
 
 // KW as in the forward: 1, a wavefront has 32 rows of its own; 4, the wavefronts share a block's 32
 // rows and take a quarter of each tile's keys.
-template <typename T, int DP, int KW>
+template <typename T, int DP, int KW, bool MASKED>
 struct Dq {
   using C = Tile<T, DP>;
   static constexpr int BR = KW == 1 ? 32 * kWaves : 32;
   static constexpr int TK = KW == 4 ? 128 : (C::ROW > 256 ? 32 : 64);
   static constexpr int NK = KW == 4 ? 1 : TK / 32;
-  static constexpr int TILE = TK * C::ROW;
+  using Keys = KeyTiles<T, DP, TK, MASKED>;
+  static constexpr int TILE = Keys::TILE;
   static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
   static constexpr int LDS = STAGES * 2 * TILE;
 };
 
-template <typename T, int DP, int KW>
+template <typename T, int DP, int KW, bool MASKED>
 __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(
     BwdArgs a) {
-  using F = Dq<T, DP, KW>;
+  using F = Dq<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
@@ -106,17 +109,23 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
     const T *low = a.low ? reinterpret_cast<const T *>(a.low) + at_out : nullptr;
 #pragma unroll
     for (int k = 0; k < C::KS; ++k) {
-      T d[C::VE];
+      const int col = (2 * k + h) * C::VE;
+      const int valid = min(max(s.D - col, 0), C::VE);
+      T d[C::VE], o[C::VE] = {}, w[C::VE] = {};
       __builtin_memcpy(d, &dout[0][k], 16);
+      if (valid == C::VE) {
+        __builtin_memcpy(o, out + col, 16);
+        if (low) __builtin_memcpy(w, low + col, 16);
+      } else {
 #pragma unroll
-      for (int i = 0; i < C::VE; ++i) {
-        const int col = (2 * k + h) * C::VE + i;
-        if (col < s.D) {
-          float o = to_f32(out[col]);
-          if (low) o += to_f32(low[col]);
-          nd = fmaf(-to_f32(d[i]), o, nd);
+        for (int i = 0; i < C::VE; ++i) {
+          if (i < valid) o[i] = out[col + i];
+          if (i < valid && low) w[i] = low[col + i];
         }
       }
+#pragma unroll
+      for (int i = 0; i < C::VE; ++i)
+        nd = fmaf(-to_f32(d[i]), to_f32(o[i]) + to_f32(w[i]), nd);
     }
     nd = pair_sum(nd);
     if (r < s.R && h == 0 && (KW == 1 || wave == 0)) a.ndelta[row] = nd;
@@ -126,83 +135,55 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
                   s.flip, q[0]);
   const float lse = a.lse[row];
   const int last = s.causal ? t + s.off : s.Tk - 1;
-  const int wave_least = s.causal ? min(r0, s.R - 1) / s.G + s.off : s.Tk - 1;
-  const int wave_last = s.causal ? min(r0 + 31, s.R - 1) / s.G + s.off : s.Tk - 1;
+  const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
   const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
   const int end = block_last < 0 ? 0 : block_last / F::TK + 1;
-
-  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
-  const char *kp = a.k.p + b * a.k.b + hk * a.k.h, *vp = a.v.p + b * a.v.b + hk * a.v.h;
-  KeyBits<F::TK> cur, nxt;
-  auto seek = [&](int i, KeyBits<F::TK> &w) {
-    for (; i < end; ++i) {
-      w.load(bits, s.words, i);
-      if (w.any()) break;
-    }
-    return i;
-  };
-  auto copy = [&](int i, const KeyBits<F::TK> &w, char *buf) {
-    const int left = s.Tk - i * F::TK;
-    const bool whole = w.all();
-    const uint32_t kt = (uint32_t)a.k.t, vt = (uint32_t)a.v.t;
-    copy_tile<T, DP, F::TK>(kp + (int64_t)i * F::TK * a.k.t, s.nvec, buf, wave,
-                            [&](int rw, bool *in) {
-                              *in = rw < left && (whole || w.has(rw));
-                              return (uint32_t)rw * kt;
-                            });
-    copy_tile<T, DP, F::TK>(vp + (int64_t)i * F::TK * a.v.t, s.nvec, buf + F::TILE, wave,
-                            [&](int rw, bool *in) {
-                              *in = rw < left && (whole || w.has(rw));
-                              return (uint32_t)rw * vt;
-                            });
-  };
+  const int full = MASKED ? 0 : min(end, (block_least + 1) / F::TK);
 
   floatx16 dq[1][C::NB];
 #pragma unroll
   for (int n = 0; n < C::NB; ++n) dq[0][n] = splat(0.f);
   Ranged<T, C::NB> range;
 
-  int at = seek(0, cur), buf = 0;
-  if (at < end) copy(at, cur, smem);
-  while (at < end) {
-    const int next = seek(at + 1, nxt);
+  const typename F::Keys keys(s, a.k, a.v, b, hk, end);
+  typename F::Keys::Bits cur, nxt;
+  int at = keys.seek(0, cur), buf = 0;
+  if (at < end) keys.copy(at, cur, smem, wave);
+  auto step = [&](auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE, wave);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
-    const int key0 = at * F::TK + (KW == 4 ? 32 * wave : 0);
-    if (key0 <= wave_last && key0 < s.Tk) {
-      const int kb0 = KW == 4 ? wave : 0;
-      const bool edge = key0 + 32 * F::NK - 1 > min(wave_least, s.Tk - 1) || !cur.all();
+    const int kb0 = KW == 4 ? wave : 0;
 #pragma unroll
-      for (int i = 0; i < F::NK; ++i) {
-        floatx16 p[1] = {splat(0.f)}, dp[1] = {splat(nd)};
-        mma_rows<T, DP, 1>(kt, kb0 + i, q, p);
-        mma_rows<T, DP, 1>(vt, kb0 + i, dout, dp);
+    for (int i = 0; i < F::NK; ++i) {
+      floatx16 p[1] = {splat(0.f)}, dp[1] = {splat(nd)};
+      mma_rows<T, DP, 1>(kt, kb0 + i, q, p);
+      mma_rows<T, DP, 1>(vt, kb0 + i, dout, dp);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dp[0][e] *= exp2_(fmaf(p[0][e], s.c, -lse));
-        if (edge) {
+      for (int e = 0; e < 16; ++e) dp[0][e] *= exp2_(fmaf(p[0][e], s.c, -lse));
+      if constexpr (EDGE) {
+        const uint32_t live = live32(last - (at * F::TK + 32 * (kb0 + i)), cur.half(kb0 + i));
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int in = 32 * i + entry(e);
-            const bool live = key0 + in <= last && cur.has(32 * kb0 + in);
-            dp[0][e] = live ? dp[0][e] : 0.f;
-          }
-        }
-        range.fit(dp[0], dq[0]);
-        Packed<T> x[1];
-        x[0].set(dp[0]);
-        mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
+        for (int e = 0; e < 16; ++e) dp[0][e] = keep(dp[0][e], live, e, 0u);
       }
+      range.fit(dp[0], dq[0]);
+      Packed<T> x[1];
+      x[0].set(dp[0]);
+      mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) copy(next, nxt, smem);
+      if (next < end) keys.copy(next, nxt, smem, wave);
     } else {
       buf ^= 1;
     }
     at = next;
     cur = nxt;
-  }
+  };
+  while (at < full) step(std::false_type{});
+  while (at < end) step(std::true_type{});
   const float f = s.scale * range.undo();
   if constexpr (KW == 4) {
     __syncthreads();
@@ -263,7 +244,6 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int key = key0 + (l & 31);
   const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
   const bool live = key < s.Tk && (!bits || (bits[key >> 6] >> (key & 63) & 1));
-  const bool work = __any(live);
   u32x4 k[1][C::KS], v[1][C::KS];
   load_row<T, DP>(a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t, live, s.nvec, s.flip, k[0]);
   load_row<T, DP>(a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t, live, s.nvec, 0u, v[0]);
@@ -271,12 +251,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int from = s.causal ? max(key - s.off, 0) : 0;
   const int64_t rmin64 = (int64_t)from * s.G;
   const int rmin = (int)(rmin64 < s.R ? rmin64 : s.R);
-  const int wave_full = s.causal ? max(key0 + 31 - s.off, 0) : 0;  // from this t on, every key
-  const int block_from = s.causal ? max(tile * F::BK - s.off, 0) : 0;
   const int end = (s.R + F::TR - 1) / F::TR;
+  const int block_from = s.causal ? max(tile * F::BK - s.off, 0) : 0;
   int at = (int)min((int64_t)block_from * s.G / F::TR, (int64_t)end);
-  const int wave_at = s.causal ? (int)min((int64_t)max(key0 - s.off, 0) * s.G / F::TR, (int64_t)end)
-                               : 0;
+  // from this tile on, every row sees every key of the block
+  const int64_t every = s.causal ? (int64_t)max(tile * F::BK + F::BK - 1 - s.off, 0) * s.G : 0;
+  const int full = (int)min((every + F::TR - 1) / F::TR, (int64_t)end);
 
   const char *qp = a.q.p + b * a.q.b + (int64_t)hk * s.G * a.q.h;
   const char *dp = a.dout.p + b * a.dout.b + (int64_t)hk * s.G * a.dout.h;
@@ -307,40 +287,41 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
 
   int buf = 0;
   if (at < end) copy(at, smem);
-  for (; at < end; ++at) {
+  auto step = [&](auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
     gemm::wait_vm_barrier<0>();
     if (at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
     const char *qt = smem + buf * F::STAGE, *dt = qt + F::TILE;
     const float *lse = reinterpret_cast<const float *>(qt + 2 * F::TILE), *nd = lse + 64;
-    if (work && at >= wave_at) {
-      const bool edge = s.causal && (int64_t)at * F::TR < (int64_t)wave_full * s.G;
 #pragma unroll
-      for (int i = 0; i < F::TR / 32; ++i) {
-        floatx16 p[1] = {splat(0.f)}, ds[1];
+    for (int i = 0; i < F::TR / 32; ++i) {
+      floatx16 p[1] = {splat(0.f)}, ds[1];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
-        mma_rows<T, DP, 1>(qt, i, k, p);
-        mma_rows<T, DP, 1>(dt, i, v, ds);
+      for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
+      mma_rows<T, DP, 1>(qt, i, k, p);
+      mma_rows<T, DP, 1>(dt, i, v, ds);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
+      if constexpr (EDGE) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
-        Packed<T> x[1];
-        x[0].set(p[0]);
-        mma_cols<T, DP, 1>(dt, i, x, dv);
-        range.fit(ds[0], dk[0]);
-        x[0].set(ds[0]);
-        mma_cols<T, DP, 1>(qt, i, x, dk);
+          p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
+      Packed<T> x[1];
+      x[0].set(p[0]);
+      mma_cols<T, DP, 1>(dt, i, x, dv);
+      range.fit(ds[0], dk[0]);
+      x[0].set(ds[0]);
+      mma_cols<T, DP, 1>(qt, i, x, dk);
     }
     buf ^= 1;
-  }
+    ++at;
+  };
+  while (at < full) step(std::true_type{});
+  while (at < end) step(std::false_type{});
   if (key >= s.Tk) return;
   const int64_t to = (((int64_t)b * s.Tk + key) * s.Hk + hk) * s.D;
   const float fv = live ? exp2_(-kPExp<T>) : 0.f;
@@ -365,10 +346,18 @@ int launch(BwdArgs a, hipStream_t st) {
   const int64_t heads = (int64_t)a.s.B * a.s.Hk;
   if (a.s.R <= 32) {
     a.tiles = 1;
-    attn_dq_kernel<T, DP, 4><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+    const unsigned grid = (unsigned)place_grid(heads, a.tiles);
+    if (a.s.bits)
+      attn_dq_kernel<T, DP, 4, true><<<grid, kThreads, 0, st>>>(a);
+    else
+      attn_dq_kernel<T, DP, 4, false><<<grid, kThreads, 0, st>>>(a);
   } else {
-    a.tiles = (a.s.R + Dq<T, DP, 1>::BR - 1) / Dq<T, DP, 1>::BR;
-    attn_dq_kernel<T, DP, 1><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+    a.tiles = (a.s.R + 32 * kWaves - 1) / (32 * kWaves);
+    const unsigned grid = (unsigned)place_grid(heads, a.tiles);
+    if (a.s.bits)
+      attn_dq_kernel<T, DP, 1, true><<<grid, kThreads, 0, st>>>(a);
+    else
+      attn_dq_kernel<T, DP, 1, false><<<grid, kThreads, 0, st>>>(a);
   }
   if (a.dk || a.dv) {
     a.tiles = (a.s.Tk + Dkv<T, DP>::BK - 1) / Dkv<T, DP>::BK;

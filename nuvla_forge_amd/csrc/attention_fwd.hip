@@ -5,6 +5,8 @@
 // 2^(m_old - m_new); out = O / l, and the row's log-sum-exp is m + log2(l).
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention.h"
 
 namespace nf {
@@ -30,21 +32,22 @@ struct FwdArgs {
 
 // KW = 1: a wavefront has 32 rows of its own, a block 128.  KW = 4: a block has 32 rows, and a
 // wavefront a quarter of each tile's keys.
-template <typename T, int DP, int KW>
+template <typename T, int DP, int KW, bool MASKED>
 struct Fwd {
   using C = Tile<T, DP>;
-  static constexpr int BR = KW == 1 ? 32 * kWaves : 32;           // rows of a block
+  static constexpr int BR = KW == 1 ? 32 * kWaves : 32;                // rows of a block
   static constexpr int TK = KW == 4 ? 128 : (C::ROW > 256 ? 32 : 64);  // keys of a tile
-  static constexpr int NK = KW == 4 ? 1 : TK / 32;                // of those, 32s of a wavefront
-  static constexpr int TILE = TK * C::ROW;
+  static constexpr int NK = KW == 4 ? 1 : TK / 32;                     // of those, 32s of a wavefront
+  using Keys = KeyTiles<T, DP, TK, MASKED>;
+  static constexpr int TILE = Keys::TILE;
   static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
   static constexpr int LDS = STAGES * 2 * TILE;
 };
 
-template <typename T, int DP, int KW>
+template <typename T, int DP, int KW, bool MASKED>
 __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
     FwdArgs a) {
-  using F = Fwd<T, DP, KW>;
+  using F = Fwd<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
@@ -65,10 +68,8 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
                   s.flip, q[0]);
   const int last = s.causal ? t + s.off : s.Tk - 1;  // the lane's last key
-  // the wavefront's and the block's
-  const int first_t = min(r0, s.R - 1) / s.G;
-  const int wave_least = s.causal ? first_t + s.off : s.Tk - 1;
-  const int wave_last = s.causal ? min(r0 + 31, s.R - 1) / s.G + s.off : s.Tk - 1;
+  // the block's: its first row's last key, its last row's
+  const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
   const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
   int end = block_last < 0 ? 0 : block_last / F::TK + 1, at = 0;
   if (a.splits > 1) {
@@ -76,102 +77,75 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
     at = (int)((int64_t)all * split / a.splits);
     end = min(end, (int)((int64_t)all * (split + 1) / a.splits));
   }
-
-  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
-  const char *kp = a.k.p + b * a.k.b + hk * a.k.h, *vp = a.v.p + b * a.v.b + hk * a.v.h;
-  KeyBits<F::TK> cur, nxt;
-  auto seek = [&](int i, KeyBits<F::TK> &w) {  // the next tile that has keys
-    for (; i < end; ++i) {
-      w.load(bits, s.words, i);
-      if (w.any()) break;
-    }
-    return i;
-  };
-  auto copy = [&](int i, const KeyBits<F::TK> &w, char *buf) {
-    const int left = s.Tk - i * F::TK;
-    const bool whole = w.all();
-    const uint32_t kt = (uint32_t)a.k.t, vt = (uint32_t)a.v.t;
-    copy_tile<T, DP, F::TK>(kp + (int64_t)i * F::TK * a.k.t, s.nvec, buf, wave,
-                            [&](int row, bool *in) {
-                              *in = row < left && (whole || w.has(row));
-                              return (uint32_t)row * kt;
-                            });
-    copy_tile<T, DP, F::TK>(vp + (int64_t)i * F::TK * a.v.t, s.nvec, buf + F::TILE, wave,
-                            [&](int row, bool *in) {
-                              *in = row < left && (whole || w.has(row));
-                              return (uint32_t)row * vt;
-                            });
-  };
+  // every row of the block sees every key of the tiles before this one
+  const int full = MASKED ? 0 : min(end, (block_least + 1) / F::TK);
 
   floatx16 o[1][C::NB];
 #pragma unroll
   for (int n = 0; n < C::NB; ++n) o[0][n] = splat(0.f);
   float m = -kInf, sum = 0.f;  // sum: of the lane's own entries
 
-  at = seek(at, cur);
+  const typename F::Keys keys(s, a.k, a.v, b, hk, end);
+  typename F::Keys::Bits cur, nxt;
+  at = keys.seek(at, cur);
   int buf = 0;
-  if (at < end) copy(at, cur, smem);
-  while (at < end) {
-    const int next = seek(at + 1, nxt);
+  if (at < end) keys.copy(at, cur, smem, wave);
+  auto step = [&](auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE, wave);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
-    const int key0 = at * F::TK + (KW == 4 ? 32 * wave : 0);
-    if (key0 <= wave_last && key0 < s.Tk) {
-      const int kb0 = KW == 4 ? wave : 0;
-      floatx16 p[F::NK];
+    const int kb0 = KW == 4 ? wave : 0;
+    floatx16 p[F::NK];
 #pragma unroll
-      for (int i = 0; i < F::NK; ++i) {
-        floatx16 acc[1] = {splat(0.f)};
-        mma_rows<T, DP, 1>(kt, kb0 + i, q, acc);
-        p[i] = acc[0];
+    for (int i = 0; i < F::NK; ++i) {
+      floatx16 acc[1] = {splat(0.f)};
+      mma_rows<T, DP, 1>(kt, kb0 + i, q, acc);
+      p[i] = acc[0];
+      if constexpr (EDGE) {
+        const uint32_t live = live32(last - (at * F::TK + 32 * (kb0 + i)), cur.half(kb0 + i));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[i][e] = keep(p[i][e], live, e, kMinusInf);
       }
-      if (key0 + 32 * F::NK - 1 > min(wave_least, s.Tk - 1) || !cur.all()) {
+    }
+    float top = p[0][0];
 #pragma unroll
-        for (int i = 0; i < F::NK; ++i)
+    for (int i = 0; i < F::NK; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int in = 32 * i + entry(e);
-            const bool live = key0 + in <= last && cur.has(32 * kb0 + in);
-            p[i][e] = live ? p[i][e] : -kInf;
-          }
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, p[i][e]);
+    top = pair_max(top) * s.c - kBias<T>;
+    if (__any(top > m + kSlack)) {
+      const float up = fmaxf(m, top);
+      const float f = exp2_(m - (up == -kInf ? 0.f : up));
+      m = up;
+      sum *= f;
+#pragma unroll
+      for (int n = 0; n < C::NB; ++n) o[0][n] *= f;
+    }
+    const float base = m == -kInf ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < F::NK; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        p[i][e] = exp2_(fmaf(p[i][e], s.c, -base));
+        sum += p[i][e];
       }
-      float top = p[0][0];
-#pragma unroll
-      for (int i = 0; i < F::NK; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, p[i][e]);
-      top = pair_max(top) * s.c - kBias<T>;
-      if (__any(top > m + kSlack)) {
-        const float up = fmaxf(m, top);
-        const float f = exp2_(m - (up == -kInf ? 0.f : up));
-        m = up;
-        sum *= f;
-#pragma unroll
-        for (int n = 0; n < C::NB; ++n) o[0][n] *= f;
-      }
-      const float base = m == -kInf ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < F::NK; ++i) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          p[i][e] = exp2_(fmaf(p[i][e], s.c, -base));
-          sum += p[i][e];
-        }
-        Packed<T> x[1];
-        x[0].set(p[i]);
-        mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
-      }
+      Packed<T> x[1];
+      x[0].set(p[i]);
+      mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) copy(next, nxt, smem);
+      if (next < end) keys.copy(next, nxt, smem, wave);
     } else {
       buf ^= 1;
     }
     at = next;
     cur = nxt;
-  }
+  };
+  while (at < full) step(std::false_type{});
+  while (at < end) step(std::true_type{});
   sum = pair_sum(sum);
 
   if constexpr (KW == 4) {  // the four wavefronts' parts of the same rows
@@ -330,10 +304,14 @@ template <typename T, int DP>
 int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
   const unsigned grid =
       (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.splits);
-  if (p.kw == 4)
-    attn_fwd_kernel<T, DP, 4><<<grid, kThreads, 0, st>>>(a);
+  if (p.kw == 4 && a.s.bits)
+    attn_fwd_kernel<T, DP, 4, true><<<grid, kThreads, 0, st>>>(a);
+  else if (p.kw == 4)
+    attn_fwd_kernel<T, DP, 4, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.s.bits)
+    attn_fwd_kernel<T, DP, 1, true><<<grid, kThreads, 0, st>>>(a);
   else
-    attn_fwd_kernel<T, DP, 1><<<grid, kThreads, 0, st>>>(a);
+    attn_fwd_kernel<T, DP, 1, false><<<grid, kThreads, 0, st>>>(a);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
     attn_join_kernel<T, DP><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);

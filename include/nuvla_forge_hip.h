@@ -415,7 +415,8 @@ size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
                                 int64_t Hk, int64_t D, int has_mask, int keep,
                                 int dtype);
 size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                  int64_t Hk, int64_t D, int dtype);
+                                  int64_t Hk, int64_t D, int causal,
+                                  int dtype);
 int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
                      const void *k, int64_t k_b, int64_t k_t, int64_t k_h,
                      const void *v, int64_t v_b, int64_t v_t, int64_t v_h,
@@ -432,7 +433,8 @@ int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
  * dk and dv summed over the G heads of a group; dense, in `dtype`; any may be
  * NULL: not formed.  The same bits every run. */
 size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                  int64_t Hk, int64_t D, int dtype);
+                                  int64_t Hk, int64_t D, int causal,
+                                  int dtype);
 int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
                      const void *k, int64_t k_b, int64_t k_t, int64_t k_h,
                      const void *v, int64_t v_b, int64_t v_t, int64_t v_h,

@@ -289,6 +289,46 @@ __device__ __forceinline__ float keep(float x, uint32_t live, int i, uint32_t ot
 }
 constexpr uint32_t kMinusInf = 0xff800000u;
 
+// ---------------------------------------------------------------------------
+// work split along the summed axis
+// ---------------------------------------------------------------------------
+// A block's `len` tiles are cut into equal parts of about c where they are more than 1.5 c.
+__host__ __device__ __forceinline__ int parts_of(int len, int c) {
+  return len <= c + c / 2 ? 1 : (len + c - 1) / c;
+}
+constexpr int kMostParts = 128;
+
+// Tiles of keys that rows [tile br, + br) go over.
+template <int TK>
+__host__ __device__ __forceinline__ int key_tiles(const Shape &s, int tile, int br) {
+  const int64_t stop = (int64_t)tile * br + br;
+  const int rows_end = stop < s.R ? (int)stop : s.R;
+  const int last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
+  return last < 0 ? 0 : last / TK + 1;
+}
+// The first tile of TR rows that sees a key of keys [tile bk, + bk).
+template <int TR>
+__host__ __device__ __forceinline__ int first_row_tile(const Shape &s, int tile, int bk) {
+  const int end = (s.R + TR - 1) / TR;
+  const int64_t from = s.causal ? (int64_t)tile * bk - s.off : 0;
+  const int64_t at = from > 0 ? from * s.G / TR : 0;
+  return at < end ? (int)at : end;
+}
+
+// The part length for `tiles` blocks a head of up to `longest` tiles each (causal: down to few),
+// `slots` blocks at once on the chip: about two blocks a slot, no part under 4 tiles.  Calls that
+// have many blocks to deal out anyway are not cut.
+inline int part_length(int64_t heads, int64_t tiles, int64_t longest, bool causal, int slots) {
+  const int64_t blocks = heads * tiles;
+  if (blocks >= 4 * (int64_t)slots || (!causal && blocks >= slots)) return 1 << 28;
+  int64_t total = blocks * longest;
+  if (causal && tiles > 1) total = total / 2 + 1;
+  int64_t c = (total + 2 * slots - 1) / (2 * slots);
+  if (c < 4) c = 4;
+  if (c < (longest + kMostParts - 1) / kMostParts) c = (longest + kMostParts - 1) / kMostParts;
+  return (int)c;
+}
+
 // A key head's keys and values, tile by tile of TK, into LDS: K, then V.  MASKED: with the sample's
 // mask words; tiles without a key are passed over.
 template <typename T, int DP, int TK, bool MASKED>

@@ -25,7 +25,9 @@ struct BwdArgs {
   const float *lse;
   float *ndelta;  // [B Hk, R]: -delta
   char *dq, *dk, *dv;
-  int tiles;
+  // rows, or keys, in parts: dQ [most][B Hk R][DP], dK and dV [most][B Hk Tk][2][DP]
+  float *part;
+  int tiles, length, most;
 };
 
 // fp16 holds 2^-24 to 65504, and gradients may lie anywhere: dS is scaled by a power of two of its
@@ -88,13 +90,15 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
   int bh, job;
-  if (!place(s.B * s.Hk, a.tiles, &bh, &job)) return;
-  const int tile = a.tiles - 1 - job;
+  if (!place(s.B * s.Hk, a.tiles * a.most, &bh, &job)) return;
+  const int part = job / a.tiles;
+  const int tile = a.tiles - 1 - (job - part * a.tiles);  // causal: the longest first
+  const int len = key_tiles<F::TK>(s, tile, F::BR), parts = parts_of(len, a.length);
+  if (part >= parts) return;
   const int b = bh / s.Hk, hk = bh % s.Hk;
   const int l = threadIdx.x & 63, h = l >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r0 = tile * F::BR + (KW == 1 ? 32 * wave : 0);
-  const int rows_end = min(tile * F::BR + F::BR, s.R);
 
   const int r = r0 + (l & 31);
   const int rc = min(r, s.R - 1), t = rc / s.G, g = rc - t * s.G;
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
         nd = fmaf(-to_f32(d[i]), to_f32(o[i]) + to_f32(w[i]), nd);
     }
     nd = pair_sum(nd);
-    if (r < s.R && h == 0 && (KW == 1 || wave == 0)) a.ndelta[row] = nd;
+    if (r < s.R && h == 0 && (KW == 1 || wave == 0) && part == 0) a.ndelta[row] = nd;
   }
   if (!a.dq) return;  // the call is for delta alone
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
@@ -136,9 +140,8 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   const float lse = a.lse[row];
   const int last = s.causal ? t + s.off : s.Tk - 1;
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
-  const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
-  const int end = block_last < 0 ? 0 : block_last / F::TK + 1;
-  const int full = MASKED ? 0 : min(end, (block_least + 1) / F::TK);
+  const int end = (int)((int64_t)len * (part + 1) / parts);
+  const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
   floatx16 dq[1][C::NB];
 #pragma unroll
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
 
   const typename F::Keys keys(s, a.k, a.v, b, hk, end);
   typename F::Keys::Bits cur, nxt;
-  int at = keys.seek(0, cur), buf = 0;
+  int at = keys.seek((int)((int64_t)len * part / parts), cur), buf = 0;
   if (at < end) keys.copy(at, cur, smem, wave);
   auto step = [&](auto edge) {
     constexpr bool EDGE = decltype(edge)::value;
@@ -205,6 +208,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   }
   if (r >= s.R) return;
   T *to = reinterpret_cast<T *>(a.dq) + at_out;
+  float *sums = a.part + ((int64_t)part * s.B * s.Hk * s.R + row) * DP;
 #pragma unroll
   for (int n = 0; n < C::NB; ++n)
 #pragma unroll
@@ -213,7 +217,10 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
       float x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = dq[0][n][4 * e4 + i] * (KW == 4 ? 1.f : f);
-      store_quad<T>(to, 32 * n + entry(4 * e4), s.D, x);
+      if (parts > 1)
+        store_quad<float>(sums, 32 * n + entry(4 * e4), DP, x);
+      else
+        store_quad<T>(to, 32 * n + entry(4 * e4), s.D, x);
     }
 }
 
@@ -234,8 +241,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   using C = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
-  int bh, tile;
-  if (!place(s.B * s.Hk, a.tiles, &bh, &tile)) return;  // causal: the first keys have most rows
+  int bh, job;
+  if (!place(s.B * s.Hk, a.tiles * a.most, &bh, &job)) return;
+  const int part = job / a.tiles, tile = job - part * a.tiles;  // causal: the first have most rows
+  const int begin = first_row_tile<F::TR>(s, tile, F::BK), len = (s.R + F::TR - 1) / F::TR - begin;
+  const int parts = parts_of(len, a.length);
+  if (part >= parts) return;
   const int b = bh / s.Hk, hk = bh % s.Hk;
   const int l = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -251,9 +262,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int from = s.causal ? max(key - s.off, 0) : 0;
   const int64_t rmin64 = (int64_t)from * s.G;
   const int rmin = (int)(rmin64 < s.R ? rmin64 : s.R);
-  const int end = (s.R + F::TR - 1) / F::TR;
-  const int block_from = s.causal ? max(tile * F::BK - s.off, 0) : 0;
-  int at = (int)min((int64_t)block_from * s.G / F::TR, (int64_t)end);
+  int at = begin + (int)((int64_t)len * part / parts);
+  const int end = begin + (int)((int64_t)len * (part + 1) / parts);
   // from this tile on, every row sees every key of the block
   const int64_t every = s.causal ? (int64_t)max(tile * F::BK + F::BK - 1 - s.off, 0) * s.G : 0;
   const int full = (int)min((every + F::TR - 1) / F::TR, (int64_t)end);
@@ -324,49 +334,147 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   while (at < end) step(std::false_type{});
   if (key >= s.Tk) return;
   const int64_t to = (((int64_t)b * s.Tk + key) * s.Hk + hk) * s.D;
-  const float fv = live ? exp2_(-kPExp<T>) : 0.f;
-  const float fk = live ? s.scale * exp2_(-kPExp<T>) * range.undo() : 0.f;
+  float *sums = a.part + (((int64_t)part * s.B * s.Hk + bh) * s.Tk + key) * 2 * DP;
+  const float fv = exp2_(-kPExp<T>), fk = s.scale * exp2_(-kPExp<T>) * range.undo();
 #pragma unroll
   for (int n = 0; n < C::NB; ++n)
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
+      const int d = 32 * n + entry(4 * e4);
       float x[4], y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // a key that is left out: zeros, whatever was formed
         x[i] = live ? dk[0][n][4 * e4 + i] * fk : 0.f;
         y[i] = live ? dv[0][n][4 * e4 + i] * fv : 0.f;
       }
-      if (a.dk) store_quad<T>(reinterpret_cast<T *>(a.dk) + to, 32 * n + entry(4 * e4), s.D, x);
-      if (a.dv) store_quad<T>(reinterpret_cast<T *>(a.dv) + to, 32 * n + entry(4 * e4), s.D, y);
+      if (parts > 1) {
+        store_quad<float>(sums, d, DP, x);
+        store_quad<float>(sums + DP, d, DP, y);
+      } else {
+        if (a.dk) store_quad<T>(reinterpret_cast<T *>(a.dk) + to, d, s.D, x);
+        if (a.dv) store_quad<T>(reinterpret_cast<T *>(a.dv) + to, d, s.D, y);
+      }
     }
 }
 
-template <typename T, int DP>
-int launch(BwdArgs a, hipStream_t st) {
-  const int64_t heads = (int64_t)a.s.B * a.s.Hk;
-  if (a.s.R <= 32) {
-    a.tiles = 1;
-    const unsigned grid = (unsigned)place_grid(heads, a.tiles);
-    if (a.s.bits)
-      attn_dq_kernel<T, DP, 4, true><<<grid, kThreads, 0, st>>>(a);
-    else
-      attn_dq_kernel<T, DP, 4, false><<<grid, kThreads, 0, st>>>(a);
+// Sums the parts of a row of dQ (KW: its kernel's), or of a key's dK and dV (KW = 0), in their
+// order: a wavefront a row.
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
+  constexpr int W = KW ? DP : 2 * DP;  // of a row
+  const Shape &s = a.s;
+  const int per = KW ? s.R : s.Tk, l = threadIdx.x & 63;
+  const int64_t rows = (int64_t)s.B * s.Hk * per;
+  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t bh = row / per;
+  const int r = (int)(row - bh * per);
+  int len;
+  if constexpr (KW) {
+    using F = Dq<T, DP, KW ? KW : 1, false>;
+    len = key_tiles<F::TK>(s, r / F::BR, F::BR);
   } else {
-    a.tiles = (a.s.R + 32 * kWaves - 1) / (32 * kWaves);
-    const unsigned grid = (unsigned)place_grid(heads, a.tiles);
-    if (a.s.bits)
-      attn_dq_kernel<T, DP, 1, true><<<grid, kThreads, 0, st>>>(a);
-    else
-      attn_dq_kernel<T, DP, 1, false><<<grid, kThreads, 0, st>>>(a);
+    using F = Dkv<T, DP>;
+    len = (s.R + F::TR - 1) / F::TR - first_row_tile<F::TR>(s, r / F::BK, F::BK);
   }
+  const int n = parts_of(len, a.length);
+  if (n == 1) return;  // the row is written
+  float x[W / 64] = {};
+  const float *p = a.part + row * W + l;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i)
+#pragma unroll
+    for (int j = 0; j < W / 64; ++j) x[j] += p[(int64_t)i * rows * W + 64 * j];
+  const int64_t b = bh / s.Hk, hk = bh % s.Hk;
+#pragma unroll
+  for (int j = 0; j < W / 64; ++j) {
+    const int c = l + 64 * j, d = c % DP;
+    if (d >= s.D) continue;
+    if constexpr (KW) {
+      const int64_t t = r / s.G, g = r % s.G;
+      reinterpret_cast<T *>(a.dq)[((b * s.Tq + t) * s.H + hk * s.G + g) * s.D + d] =
+          from_f32<T>(x[j]);
+    } else {
+      T *to = reinterpret_cast<T *>(c < DP ? a.dk : a.dv);
+      if (to) to[((b * s.Tk + r) * s.Hk + hk) * s.D + d] = from_f32<T>(x[j]);
+    }
+  }
+}
+
+struct Plan {
+  int tiles, length, most;
+  size_t bytes;  // of the parts
+};
+
+Plan dq_plan(const Sizes &z, bool causal) {
+  const bool few = z.rows() <= 32, wide = z.dp() * z.es() > 256;
+  const int br = few ? 32 : 128, tk = few ? 128 : wide ? 32 : 64;
+  const int64_t heads = z.B * z.Hk, longest = (z.Tk + tk - 1) / tk;
+  Plan p;
+  p.tiles = (int)((z.rows() + br - 1) / br);
+  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.most = parts_of((int)longest, p.length);
+  p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.rows()) * (size_t)z.dp() * 4 : 0;
+  return p;
+}
+
+Plan dkv_plan(const Sizes &z, bool causal) {
+  const int tr = z.dp() * z.es() > 256 ? 32 : 64;
+  const int64_t heads = z.B * z.Hk, longest = (z.rows() + tr - 1) / tr;
+  Plan p;
+  p.tiles = (int)((z.Tk + 127) / 128);
+  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.most = parts_of((int)longest, p.length);
+  p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.Tk) * (size_t)z.dp() * 8 : 0;
+  return p;
+}
+
+size_t delta_bytes(const Sizes &z) {
+  return ((size_t)(z.B * z.Hk * z.rows()) * 4 + 255) / 256 * 256;
+}
+size_t bwd_bytes(const Sizes &z, bool causal) {
+  const size_t a = dq_plan(z, causal).bytes, b = dkv_plan(z, causal).bytes;
+  return delta_bytes(z) + (a > b ? a : b);  // dQ's parts are summed before dK's are formed
+}
+
+template <typename T, int DP, int KW>
+void launch_dq(BwdArgs &a, hipStream_t st) {
+  const unsigned grid = (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most);
+  if (a.s.bits)
+    attn_dq_kernel<T, DP, KW, true><<<grid, kThreads, 0, st>>>(a);
+  else
+    attn_dq_kernel<T, DP, KW, false><<<grid, kThreads, 0, st>>>(a);
+  if (a.most > 1 && a.dq) {
+    const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
+    attn_sum_kernel<T, DP, KW><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+  }
+}
+
+template <typename T, int DP>
+int launch(BwdArgs a, const Sizes &z, hipStream_t st) {
+  auto take = [&](const Plan &p) {
+    a.tiles = p.tiles;
+    a.length = p.length;
+    a.most = p.most;
+  };
+  take(dq_plan(z, a.s.causal));
+  if (!a.dq) a.most = 1, a.length = 1 << 28;  // for delta alone
+  if (a.s.R <= 32)
+    launch_dq<T, DP, 4>(a, st);
+  else
+    launch_dq<T, DP, 1>(a, st);
   if (a.dk || a.dv) {
-    a.tiles = (a.s.Tk + Dkv<T, DP>::BK - 1) / Dkv<T, DP>::BK;
-    attn_dkv_kernel<T, DP><<<(unsigned)place_grid(heads, a.tiles), kThreads, 0, st>>>(a);
+    take(dkv_plan(z, a.s.causal));
+    attn_dkv_kernel<T, DP>
+        <<<(unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most), kThreads, 0,
+           st>>>(a);
+    if (a.most > 1) {
+      const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.Tk;
+      attn_sum_kernel<T, DP, 0><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+    }
   }
   return check_launch("nf_attention_bwd");
 }
-
-size_t delta_bytes(const Sizes &z) { return (size_t)(z.B * z.Hk * z.rows()) * 4; }
 
 }  // namespace
 }  // namespace attn
@@ -376,9 +484,9 @@ using namespace nf;
 using namespace nf::attn;
 
 extern "C" size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                             int64_t Hk, int64_t D, int dtype) {
+                                             int64_t Hk, int64_t D, int causal, int dtype) {
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  return check_sizes("nf_attention_bwd_workspace", z) ? 0 : delta_bytes(z);
+  return check_sizes("nf_attention_bwd_workspace", z) ? 0 : bwd_bytes(z, causal);
 }
 
 extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
@@ -396,9 +504,9 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   if (B == 0 || Tq == 0 || (!dq && !dk && !dv)) return NF_OK;
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
   const State parts = state_of(z, has_mask, true);
-  if (state_bytes < parts.total || workspace_bytes < delta_bytes(z))
+  if (state_bytes < parts.total || workspace_bytes < bwd_bytes(z, causal))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
-                     state_bytes, parts.total, workspace_bytes, delta_bytes(z));
+                     state_bytes, parts.total, workspace_bytes, bwd_bytes(z, causal));
   if (!out || !state || !aligned16(state) || !workspace || !aligned16(workspace))
     return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
   BwdArgs a = {};
@@ -413,12 +521,13 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   a.low = z.es() == 2 ? st + parts.low : nullptr;
   a.lse = reinterpret_cast<const float *>(st + parts.lse);
   a.ndelta = static_cast<float *>(workspace);
+  a.part = a.ndelta + delta_bytes(z) / 4;
   a.dq = static_cast<char *>(dq);
   a.dk = static_cast<char *>(dk);
   a.dv = static_cast<char *>(dv);
   hipStream_t hs = static_cast<hipStream_t>(stream);
 #define NF_ATTN(DT, T) \
-  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, hs) : launch<T, 128>(a, hs);
+  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, z, hs) : launch<T, 128>(a, z, hs);
   NF_ATTN(NF_DTYPE_BF16, bf16)
   NF_ATTN(NF_DTYPE_F16, f16)
   NF_ATTN(NF_DTYPE_F32, float)

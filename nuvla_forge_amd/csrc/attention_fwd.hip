@@ -26,8 +26,8 @@ struct FwdArgs {
   char *out;     // [B, Tq, H, D]
   char *low;     // what out's rounding left, the same layout; null: not kept
   float *lse;    // [B Hk, R] in powers of two; null: not kept
-  float *part;   // splits > 1: O [splits][B Hk R][DP], then (m, l) pairs
-  int splits, tiles;
+  float *part;   // rows in parts: O [most][B Hk R][DP], then (m, l) pairs
+  int length, most, tiles;  // parts of about `length` tiles, at most `most`
 };
 
 // KW = 1: a wavefront has 32 rows of its own, a block 128.  KW = 4: a block has 32 rows, and a
@@ -52,14 +52,15 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
   int bh, job;
-  if (!place(s.B * s.Hk, a.tiles * a.splits, &bh, &job)) return;
-  const int split = job % a.splits;
-  const int tile = a.tiles - 1 - job / a.splits;  // causal: the longest first
+  if (!place(s.B * s.Hk, a.tiles * a.most, &bh, &job)) return;
+  const int part = job / a.tiles;
+  const int tile = a.tiles - 1 - (job - part * a.tiles);  // causal: the longest first
+  const int len = key_tiles<F::TK>(s, tile, F::BR), parts = parts_of(len, a.length);
+  if (part >= parts) return;
   const int b = bh / s.Hk, hk = bh % s.Hk;
   const int l = threadIdx.x & 63, h = l >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r0 = tile * F::BR + (KW == 1 ? 32 * wave : 0);  // the wavefront's first row
-  const int rows_end = min(tile * F::BR + F::BR, s.R);
 
   // the lane's row
   const int r = r0 + (l & 31);
@@ -68,17 +69,11 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
                   s.flip, q[0]);
   const int last = s.causal ? t + s.off : s.Tk - 1;  // the lane's last key
-  // the block's: its first row's last key, its last row's
-  const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
-  const int block_last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
-  int end = block_last < 0 ? 0 : block_last / F::TK + 1, at = 0;
-  if (a.splits > 1) {
-    const int all = (s.Tk + F::TK - 1) / F::TK;
-    at = (int)((int64_t)all * split / a.splits);
-    end = min(end, (int)((int64_t)all * (split + 1) / a.splits));
-  }
+  const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;  // its first row's
+  int at = (int)((int64_t)len * part / parts);
+  const int end = (int)((int64_t)len * (part + 1) / parts);
   // every row of the block sees every key of the tiles before this one
-  const int full = MASKED ? 0 : min(end, (block_least + 1) / F::TK);
+  const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
   floatx16 o[1][C::NB];
 #pragma unroll
@@ -186,9 +181,9 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   if (r >= s.R) return;
   const bool lead = KW == 1 || wave == 0;
   const int64_t row = (int64_t)bh * s.R + r;
-  if (a.splits > 1) {
+  if (parts > 1) {
     const int64_t rows = (int64_t)s.B * s.Hk * s.R;
-    float *op = a.part + ((int64_t)split * rows + row) * DP;
+    float *op = a.part + ((int64_t)part * rows + row) * DP;
 #pragma unroll
     for (int n = 0; n < C::NB; ++n)
 #pragma unroll
@@ -199,7 +194,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
         store_quad<float>(op, 32 * n + entry(4 * e4), DP, x);
       }
     if (lead && h == 0) {
-      float *ml = a.part + (int64_t)a.splits * rows * DP + ((int64_t)split * rows + row) * 2;
+      float *ml = a.part + (int64_t)a.most * rows * DP + ((int64_t)part * rows + row) * 2;
       ml[0] = m;
       ml[1] = sum;
     }
@@ -226,30 +221,61 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   if (a.lse && lead && h == 0) a.lse[row] = sum == 0.f ? kInf : m + __log2f(sum);
 }
 
-// Joins the splits of a row, in their order: one wavefront a row, a lane DP / 64 columns.
-template <typename T, int DP>
+// Joins the parts of a row, in a fixed order: W wavefronts a row, every W-th part each.
+template <typename T, int DP, int KW, int W>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
+  using F = Fwd<T, DP, KW, false>;
+  __shared__ float sums[kWaves][DP];
   const Shape &s = a.s;
   const int64_t rows = (int64_t)s.B * s.Hk * s.R;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * (kWaves / W) + wave / W;
   if (row >= rows) return;
-  const int l = threadIdx.x & 63;
-  const float *ml = a.part + (int64_t)a.splits * rows * DP;
-  float top = -kInf;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, ml[(i * rows + row) * 2]);
-  const float base = top == -kInf ? 0.f : top;
-  float sum = 0.f, o[DP / 64];
+  const int64_t bh = row / s.R;
+  const int r = (int)(row - bh * s.R);
+  const int n = parts_of(key_tiles<F::TK>(s, r / F::BR, F::BR), a.length);
+  if (n == 1) return;  // the row is written
+  const float *ml = a.part + (int64_t)a.most * rows * DP + row * 2;
+  float m[2], sum = 0.f, top = -kInf;
 #pragma unroll
-  for (int j = 0; j < DP / 64; ++j) o[j] = 0.f;
-  for (int i = 0; i < a.splits; ++i) {
-    const float f = exp2_(ml[(i * rows + row) * 2] - base);
-    sum += ml[(i * rows + row) * 2 + 1] * f;
+  for (int j = 0; j < 2; ++j) {
+    m[j] = l + 64 * j < n ? ml[(l + 64 * j) * rows * 2] : -kInf;
+    top = fmaxf(top, m[j]);
+  }
+  top = wave_max(top);
+  const float base = top == -kInf ? 0.f : top;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    m[j] = exp2_(m[j] - base);
+    if (l + 64 * j < n) sum += ml[(l + 64 * j) * rows * 2 + 1] * m[j];
+  }
+  sum = wave_sum(sum);
+  float o[DP / 64] = {};
+  auto add = [&](int i) {
+    const float f = __shfl(i < 64 ? m[0] : m[1], i & 63);
     const float *p = a.part + (i * rows + row) * DP;
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) o[j] += p[l + 64 * j] * f;
+    for (int j = 0; j < DP / 64; ++j) o[j] = fmaf(p[l + 64 * j], f, o[j]);
+  };
+  int i = wave % W;
+  for (; i + 3 * W < n; i += 4 * W) {
+    add(i);
+    add(i + W);
+    add(i + 2 * W);
+    add(i + 3 * W);
+  }
+  for (; i < n; i += W) add(i);
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) sums[wave][l + 64 * j] = o[j];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j)
+      o[j] = ((sums[0][l + 64 * j] + sums[1][l + 64 * j]) + sums[2][l + 64 * j]) +
+             sums[3][l + 64 * j];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t bh = row / s.R, r = row % s.R;
   const int64_t b = bh / s.Hk, hk = bh % s.Hk, t = r / s.G, g = r % s.G;
   const int64_t to = ((b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
 #pragma unroll
@@ -275,35 +301,43 @@ __global__ __launch_bounds__(kThreads) void attn_bits_kernel(const uint8_t *mask
 }
 
 struct Plan {
-  int kw, tiles, splits;
+  int kw, tiles, length, most;
 };
 
-// Up to 32 rows a key head: the wavefronts of a block share them.  The keys are split over blocks
-// where the blocks are fewer than kFill, into parts of at least 4 tiles.
-Plan plan_of(const Sizes &z) {
-  constexpr int64_t kFill = 512;
+// Up to 32 rows a key head: the wavefronts of a block share them.
+Plan plan_of(const Sizes &z, bool causal) {
   Plan p;
   const int64_t R = z.rows(), heads = z.B * z.Hk;
+  const bool wide = z.dp() * z.es() > 256;
   p.kw = R <= 32 ? 4 : 1;
   p.tiles = (int)((R + (p.kw == 4 ? 31 : 127)) / (p.kw == 4 ? 32 : 128));
-  const int tk = p.kw == 4 ? 128 : (z.dp() * z.es() > 256 ? 32 : 64);
-  const int64_t steps = (z.Tk + tk - 1) / tk, blocks = heads * p.tiles;
-  int64_t n = blocks >= kFill / 2 ? 1 : kFill / blocks;
-  if (n > steps / 4) n = steps / 4;
-  p.splits = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+  const int tk = p.kw == 4 ? 128 : wide ? 32 : 64;
+  const int64_t longest = (z.Tk + tk - 1) / tk;
+  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.most = parts_of((int)longest, p.length);
   return p;
 }
 
-size_t part_bytes(const Sizes &z) {
-  const Plan p = plan_of(z);
-  if (p.splits <= 1) return 0;
-  return (size_t)p.splits * (size_t)(z.B * z.Hk * z.rows()) * (size_t)(z.dp() + 2) * 4;
+size_t part_bytes(const Sizes &z, bool causal) {
+  const Plan p = plan_of(z, causal);
+  if (p.most <= 1) return 0;
+  return (size_t)p.most * (size_t)(z.B * z.Hk * z.rows()) * (size_t)(z.dp() + 2) * 4;
+}
+
+template <typename T, int DP, int KW>
+void join(const FwdArgs &a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
+  if (a.most > 8)
+    attn_join_kernel<T, DP, KW, kWaves><<<(unsigned)rows, kThreads, 0, st>>>(a);
+  else
+    attn_join_kernel<T, DP, KW, 1>
+        <<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
 }
 
 template <typename T, int DP>
 int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
   const unsigned grid =
-      (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.splits);
+      (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.most);
   if (p.kw == 4 && a.s.bits)
     attn_fwd_kernel<T, DP, 4, true><<<grid, kThreads, 0, st>>>(a);
   else if (p.kw == 4)
@@ -312,10 +346,10 @@ int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
     attn_fwd_kernel<T, DP, 1, true><<<grid, kThreads, 0, st>>>(a);
   else
     attn_fwd_kernel<T, DP, 1, false><<<grid, kThreads, 0, st>>>(a);
-  if (p.splits > 1) {
-    const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
-    attn_join_kernel<T, DP><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
-  }
+  if (p.most > 1 && p.kw == 4)
+    join<T, DP, 4>(a, st);
+  else if (p.most > 1)
+    join<T, DP, 1>(a, st);
   return check_launch("nf_attention_fwd");
 }
 
@@ -405,10 +439,10 @@ extern "C" size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, in
 }
 
 extern "C" size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                             int64_t Hk, int64_t D, int dtype) {
+                                             int64_t Hk, int64_t D, int causal, int dtype) {
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (check_sizes("nf_attention_fwd_workspace", z) || B * Tq * Tk == 0) return 0;
-  return part_bytes(z);
+  return part_bytes(z, causal);
 }
 
 extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
@@ -425,11 +459,11 @@ extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   if (B == 0 || Tq == 0) return NF_OK;
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
   const State parts = state_of(z, key_mask != nullptr, keep);
-  if (state_bytes < parts.total || workspace_bytes < part_bytes(z))
+  if (state_bytes < parts.total || workspace_bytes < part_bytes(z, causal))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
-                     state_bytes, parts.total, workspace_bytes, part_bytes(z));
+                     state_bytes, parts.total, workspace_bytes, part_bytes(z, causal));
   if (!out || (parts.total && (!state || !aligned16(state))) ||
-      (part_bytes(z) && (!workspace || !aligned16(workspace))))
+      (part_bytes(z, causal) && (!workspace || !aligned16(workspace))))
     return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
   FwdArgs a = {};
   if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
@@ -442,8 +476,9 @@ extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   a.low = keep && z.es() == 2 ? st + parts.low : nullptr;
   a.lse = keep ? reinterpret_cast<float *>(st + parts.lse) : nullptr;
   a.part = static_cast<float *>(workspace);
-  const Plan p = plan_of(z);
-  a.splits = p.splits;
+  const Plan p = plan_of(z, causal);
+  a.length = p.length;
+  a.most = p.most;
   a.tiles = p.tiles;
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (key_mask) {

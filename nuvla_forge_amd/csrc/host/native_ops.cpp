@@ -650,7 +650,7 @@ struct Attention : torch::autograd::Function<Attention> {
     Tensor out = at::empty({z.B, z.Tq, z.H, z.D}, q.t.options().requires_grad(false));
     const size_t n_state = nf_attention_state_bytes(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, mask.defined(),
                                                     keep, dt);
-    const size_t n_ws = nf_attention_fwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, dt);
+    const size_t n_ws = nf_attention_fwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, causal, dt);
     Tensor ws;
     if (n_state) state = bytes(n_state, out);
     if (n_ws) ws = bytes(n_ws, out);
@@ -692,7 +692,7 @@ struct Attention : torch::autograd::Function<Attention> {
     for (int i : {1, 2})
       if (ctx->needs_input_grad(i)) res[i] = at::empty({z.B, z.Tk, z.Hk, z.D}, opts);
     const int dt = code_of(out);
-    const size_t n_ws = nf_attention_bwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, dt);
+    const size_t n_ws = nf_attention_bwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, (int)s[0], dt);
     Tensor ws = bytes(n_ws, out);
     check(nf_attention_bwd(q.t.data_ptr(), q.b, q.s, q.h, k.t.data_ptr(), k.b, k.s, k.h,
                            v.t.data_ptr(), v.b, v.s, v.h, out.data_ptr(), g.t.data_ptr(), g.b, g.s,

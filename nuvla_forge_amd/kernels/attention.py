@@ -50,7 +50,7 @@ class _FusedAttention(torch.autograd.Function):
         dt, L = _lib.dtype_code(q), _lib.lib()
         sizes = (b, tq, tk, h, hk, d)
         n_state = L.nf_attention_state_bytes(*sizes, key_mask is not None, keep, dt)
-        n_ws = L.nf_attention_fwd_workspace(*sizes, dt)
+        n_ws = L.nf_attention_fwd_workspace(*sizes, causal, dt)
         state = torch.empty(max(n_state, 1), dtype=torch.uint8, device=q.device)
         ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=q.device)
         mask_strides = (0, 0)
@@ -82,7 +82,7 @@ class _FusedAttention(torch.autograd.Function):
                       for shape, need in zip(((b, tq, h, d), (b, tk, hk, d), (b, tk, hk, d)),
                                              ctx.needs_input_grad))
         dt, L = _lib.dtype_code(q), _lib.lib()
-        n_ws = L.nf_attention_bwd_workspace(*sizes, dt)
+        n_ws = L.nf_attention_bwd_workspace(*sizes, causal, dt)
         ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=q.device)
         with device_of(q):
             _lib.check(

@@ -189,8 +189,8 @@ def test_attention_c_abi_refusals(call):
 def test_attention_c_abi_workspaces():
     L = _lib.lib()
     # many rows: no split; a few rows over many keys: partial sums
-    assert L.nf_attention_fwd_workspace(8, 1176, 1176, 6, 6, 64, 1) == 0
-    few = L.nf_attention_fwd_workspace(1, 1, 65536, 8, 2, 128, 1)
+    assert L.nf_attention_fwd_workspace(8, 1176, 1176, 6, 6, 64, 0, 1) == 0
+    few = L.nf_attention_fwd_workspace(1, 1, 65536, 8, 2, 128, 0, 1)
     assert few > 0
     assert _fwd(Tq=1, Tk=65536, H=4, Hk=4, ws_bytes=16) == NF_ERR_WORKSPACE
     assert _fwd(Tq=1, Tk=65536, H=4, Hk=4, ws=None) == NF_ERR_ARG
@@ -206,8 +206,8 @@ def test_attention_c_abi_workspaces():
     assert L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 0, 1, 0) < kept  # fp32: nothing left over
     for bad in ((2, 3, 4, 4, 3, 16), (2, 3, 4, 4, 2, 200), (-2, 3, 4, 4, 2, 16)):
         assert L.nf_attention_state_bytes(*bad, 0, 1, 1) == 0
-        assert L.nf_attention_fwd_workspace(*bad, 1) == 0
-        assert L.nf_attention_bwd_workspace(*bad, 1) == 0
+        assert L.nf_attention_fwd_workspace(*bad, 0, 1) == 0
+        assert L.nf_attention_bwd_workspace(*bad, 0, 1) == 0
 
 
 # ---------------------------------------------------------------------------

@@ -398,8 +398,8 @@ def test_attention_buffers_of_exactly_the_size_asked_for(cuda, b, tq, tk, h, hk,
         return torch.full((n + 4096,), 171, dtype=torch.uint8, device=cuda), n
 
     state, fw, bw = (room(n) for n in (
-        L.nf_attention_state_bytes(*sizes, masked, 1, dt), L.nf_attention_fwd_workspace(*sizes, dt),
-        L.nf_attention_bwd_workspace(*sizes, dt)))
+        L.nf_attention_state_bytes(*sizes, masked, 1, dt), L.nf_attention_fwd_workspace(*sizes, 1, dt),
+        L.nf_attention_bwd_workspace(*sizes, 1, dt)))
     outs = [room(t.numel() * t.element_size()) for t in (q, q, k, v)]
     at = [(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)) for t in (q, k, v, do)]
     ms = (0, 0) if m is None else m.stride()

@@ -292,9 +292,11 @@ constexpr uint32_t kMinusInf = 0xff800000u;
 // ---------------------------------------------------------------------------
 // work split along the summed axis
 // ---------------------------------------------------------------------------
-// A block's `len` tiles are cut into equal parts of about c where they are more than 1.5 c.
+// A block's `len` tiles are cut every c, the last part being c / 2 to 1.5 c: blocks of the same part
+// go over the same tiles at the same time, which their L2 then holds.
 __host__ __device__ __forceinline__ int parts_of(int len, int c) {
-  return len <= c + c / 2 ? 1 : (len + c - 1) / c;
+  const int n = (int)(((int64_t)len + c / 2) / c);
+  return n > 1 ? n : 1;
 }
 constexpr int kMostParts = 128;
 
@@ -394,10 +396,40 @@ struct KeyTiles {
   }
 };
 
-// 16 accumulated columns of 4 consecutive rows: a lane's entries 4 quad .. + 3 of column block nb,
-// written to row p of D elements.
+// ---------------------------------------------------------------------------
+// results
+// ---------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Accumulated columns through LDS, so that memory is written a row at a time: a wavefront's 32 rows
+// of DP floats, 16-byte vectors XOR-swizzled by row.
+template <int DP>
+struct Turned {
+  static constexpr int BYTES = 32 * DP * 4;
+  static constexpr int V = DP / 4;  // vectors of a row
+  __device__ __forceinline__ static int at(int row, int v) {
+    return row * DP * 4 + ((v ^ (row & (V - 1) & 31)) << 4);
+  }
+  __device__ __forceinline__ static void put(char *lds, const floatx16 (&acc)[DP / 32], float f) {
+    const int row = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = acc[n][4 * e4 + i] * f;
+        *reinterpret_cast<f32x4 *>(lds + at(row, (32 * n + entry(4 * e4)) / 4)) = x;
+      }
+  }
+  __device__ __forceinline__ static f32x4 get(const char *lds, int row, int v) {
+    return *reinterpret_cast<const f32x4 *>(lds + at(row, v));
+  }
+};
+
+// Columns d .. d + 3 of a row p of D elements.
 template <typename T>
-__device__ __forceinline__ void store_quad(T *p, int d, int D, const float (&v)[4]) {
+__device__ __forceinline__ void store_quad(T *p, int d, int D, const f32x4 &v) {
   if (d + 4 <= D) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     t4 x;
@@ -409,6 +441,32 @@ __device__ __forceinline__ void store_quad(T *p, int d, int D, const float (&v)[
     for (int i = 0; i < 4; ++i)
       if (d + i < D) p[d + i] = from_f32<T>(v[i]);
   }
+}
+
+// A wavefront's 32 rows (KW = 1), or a block's 32 rows in four parts that are summed (KW = 4), as
+// `put` left them: each vector to store(row, column, values).
+template <int DP, int KW, class F>
+__device__ __forceinline__ void each_vector(const char *smem, int wave, F &&store) {
+  using U = Turned<DP>;
+  constexpr int PER = KW == 4 ? kThreads : 64;
+  const int first = KW == 4 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+#pragma unroll
+  for (int i = 0; i < 32 * U::V / PER; ++i) {
+    const int x = i * PER + first, row = x / U::V, v = x % U::V;
+    f32x4 y;
+    if constexpr (KW == 4)
+      y = ((U::get(smem, row, v) + U::get(smem + U::BYTES, row, v)) +
+           U::get(smem + 2 * U::BYTES, row, v)) + U::get(smem + 3 * U::BYTES, row, v);
+    else
+      y = U::get(smem + wave * U::BYTES, row, v);
+    store(row, 4 * v, y);
+  }
+}
+
+// a lane's 64-bit value, from every lane
+__device__ __forceinline__ int64_t from_lane(int64_t x, int lane) {
+  const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, lane);
+  return (int64_t)__shfl((int)(x >> 32), lane) << 32 | lo;
 }
 
 // ---------------------------------------------------------------------------

@@ -79,7 +79,8 @@ struct Dq {
   using Keys = KeyTiles<T, DP, TK, MASKED>;
   static constexpr int TILE = Keys::TILE;
   static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
-  static constexpr int LDS = STAGES * 2 * TILE;
+  static constexpr int END = kWaves * Turned<DP>::BYTES;
+  static constexpr int LDS = STAGES * 2 * TILE > END ? STAGES * 2 * TILE : END;
 };
 
 template <typename T, int DP, int KW, bool MASKED>
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   const float lse = a.lse[row];
   const int last = s.causal ? t + s.off : s.Tk - 1;
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
-  const int end = (int)((int64_t)len * (part + 1) / parts);
+  const int begin = part * a.length, end = part + 1 < parts ? begin + a.length : len;
   const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
   floatx16 dq[1][C::NB];
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
 
   const typename F::Keys keys(s, a.k, a.v, b, hk, end);
   typename F::Keys::Bits cur, nxt;
-  int at = keys.seek((int)((int64_t)len * part / parts), cur), buf = 0;
+  int at = keys.seek(begin, cur), buf = 0;
   if (at < end) keys.copy(at, cur, smem, wave);
   auto step = [&](auto edge) {
     constexpr bool EDGE = decltype(edge)::value;
@@ -188,40 +189,18 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   while (at < full) step(std::false_type{});
   while (at < end) step(std::true_type{});
   const float f = s.scale * range.undo();
-  if constexpr (KW == 4) {
-    __syncthreads();
-    float *os = reinterpret_cast<float *>(smem);  // [4][DP][32]
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        os[(wave * DP + 32 * n + entry(e)) * 32 + (l & 31)] = dq[0][n][e] * f;
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (((32 * n + 8 * (e / 4)) * 4) / DP != wave) continue;
-        const int i = (32 * n + entry(e)) * 32 + (l & 31);
-        dq[0][n][e] = ((os[i] + os[DP * 32 + i]) + os[2 * DP * 32 + i]) + os[3 * DP * 32 + i];
-      }
-  }
-  if (r >= s.R) return;
-  T *to = reinterpret_cast<T *>(a.dq) + at_out;
-  float *sums = a.part + ((int64_t)part * s.B * s.Hk * s.R + row) * DP;
-#pragma unroll
-  for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
-      float x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = dq[0][n][4 * e4 + i] * (KW == 4 ? 1.f : f);
-      if (parts > 1)
-        store_quad<float>(sums, 32 * n + entry(4 * e4), DP, x);
-      else
-        store_quad<T>(to, 32 * n + entry(4 * e4), s.D, x);
-    }
+  __syncthreads();
+  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, dq[0], f);
+  if (KW == 4) __syncthreads();
+  float *sums = a.part + ((int64_t)part * s.B * s.Hk * s.R + (int64_t)bh * s.R + r0) * DP;
+  each_vector<DP, KW>(smem, wave, [&](int i, int d, const f32x4 &x) {
+    const int64_t to = from_lane(at_out, i);
+    if (r0 + i >= s.R) return;
+    if (parts > 1)
+      store_quad<float>(sums + i * DP, d, DP, x);
+    else
+      store_quad<T>(reinterpret_cast<T *>(a.dq) + to, d, s.D, x);
+  });
 }
 
 // A block has 128 keys, a wavefront 32, and goes over the rows.
@@ -233,6 +212,7 @@ struct Dkv {
   static constexpr int TILE = TR * C::ROW;
   static constexpr int STAGE = 2 * TILE + 2 * 256;  // q, dout, log-sum-exps, -deltas
   static constexpr int LDS = 2 * STAGE;
+  static_assert(LDS >= kWaves * Turned<DP>::BYTES, "the results turn in the tiles' place");
 };
 
 template <typename T, int DP>
@@ -262,8 +242,8 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int from = s.causal ? max(key - s.off, 0) : 0;
   const int64_t rmin64 = (int64_t)from * s.G;
   const int rmin = (int)(rmin64 < s.R ? rmin64 : s.R);
-  int at = begin + (int)((int64_t)len * part / parts);
-  const int end = begin + (int)((int64_t)len * (part + 1) / parts);
+  const int end = begin + len - part * a.length;  // from the last row back
+  int at = part + 1 < parts ? end - a.length : begin;
   // from this tile on, every row sees every key of the block
   const int64_t every = s.causal ? (int64_t)max(tile * F::BK + F::BK - 1 - s.off, 0) * s.G : 0;
   const int full = (int)min((every + F::TR - 1) / F::TR, (int64_t)end);
@@ -332,29 +312,27 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   };
   while (at < full) step(std::true_type{});
   while (at < end) step(std::false_type{});
-  if (key >= s.Tk) return;
-  const int64_t to = (((int64_t)b * s.Tk + key) * s.Hk + hk) * s.D;
-  float *sums = a.part + (((int64_t)part * s.B * s.Hk + bh) * s.Tk + key) * 2 * DP;
+  __syncthreads();
   const float fv = exp2_(-kPExp<T>), fk = s.scale * exp2_(-kPExp<T>) * range.undo();
-#pragma unroll
-  for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      const int d = 32 * n + entry(4 * e4);
-      float x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // a key that is left out: zeros, whatever was formed
-        x[i] = live ? dk[0][n][4 * e4 + i] * fk : 0.f;
-        y[i] = live ? dv[0][n][4 * e4 + i] * fv : 0.f;
-      }
+  char *turned = smem + wave * Turned<DP>::BYTES;
+  const int64_t first = (int64_t)bh * s.Tk + key0;
+  auto put = [&](const floatx16(&acc)[C::NB], float f, void *out, int which) {
+    Turned<DP>::put(turned, acc, f);
+    each_vector<DP, 1>(smem, wave, [&](int i, int d, const f32x4 &y) {
+      // a key that is left out: zeros, whatever was formed
+      const f32x4 x = __shfl((int)live, i) ? y : f32x4{0.f, 0.f, 0.f, 0.f};
+      if (key0 + i >= s.Tk) return;
       if (parts > 1) {
-        store_quad<float>(sums, d, DP, x);
-        store_quad<float>(sums + DP, d, DP, y);
-      } else {
-        if (a.dk) store_quad<T>(reinterpret_cast<T *>(a.dk) + to, d, s.D, x);
-        if (a.dv) store_quad<T>(reinterpret_cast<T *>(a.dv) + to, d, s.D, y);
+        const int64_t rows = (int64_t)s.B * s.Hk * s.Tk;
+        store_quad<float>(a.part + (((int64_t)part * rows + first + i) * 2 + which) * DP, d, DP, x);
+      } else if (out) {
+        T *to = static_cast<T *>(out) + (((int64_t)b * s.Tk + key0 + i) * s.Hk + hk) * s.D;
+        store_quad<T>(to, d, s.D, x);
       }
-    }
+    });
+  };
+  put(dk[0], fk, a.dk, 0);
+  put(dv[0], fv, a.dv, 1);
 }
 
 // Sums the parts of a row of dQ (KW: its kernel's), or of a key's dK and dV (KW = 0), in their

@@ -41,7 +41,8 @@ struct Fwd {
   using Keys = KeyTiles<T, DP, TK, MASKED>;
   static constexpr int TILE = Keys::TILE;
   static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
-  static constexpr int LDS = STAGES * 2 * TILE;
+  static constexpr int END = kWaves * Turned<DP>::BYTES + (KW == 4 ? 1024 : 0);
+  static constexpr int LDS = STAGES * 2 * TILE > END ? STAGES * 2 * TILE : END;
 };
 
 template <typename T, int DP, int KW, bool MASKED>
@@ -70,8 +71,8 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
                   s.flip, q[0]);
   const int last = s.causal ? t + s.off : s.Tk - 1;  // the lane's last key
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;  // its first row's
-  int at = (int)((int64_t)len * part / parts);
-  const int end = (int)((int64_t)len * (part + 1) / parts);
+  int at = part * a.length;
+  const int end = part + 1 < parts ? at + a.length : len;
   // every row of the block sees every key of the tiles before this one
   const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
@@ -143,10 +144,10 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   while (at < end) step(std::true_type{});
   sum = pair_sum(sum);
 
+  __syncthreads();
+  float f = 1.f;
   if constexpr (KW == 4) {  // the four wavefronts' parts of the same rows
-    __syncthreads();
-    float *stat = reinterpret_cast<float *>(smem);  // [4][2][32], then O [4][DP][32]
-    float *os = stat + 4 * 64;
+    float *stat = reinterpret_cast<float *>(smem + kWaves * Turned<DP>::BYTES);  // [4][2][32]
     if (h == 0) {
       stat[wave * 64 + l] = m;
       stat[wave * 64 + 32 + l] = sum;
@@ -159,66 +160,41 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
 #pragma unroll
     for (int w = 0; w < 4; ++w)
       total += stat[w * 64 + 32 + (l & 31)] * exp2_(stat[w * 64 + (l & 31)] - base);
-    const float f = exp2_(m - base);
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        os[(wave * DP + 32 * n + entry(e)) * 32 + (l & 31)] = o[0][n][e] * f;
-    __syncthreads();
-    // wavefront w takes columns w DP / 4 .. of every row
+    f = exp2_(m - base);
     m = top;
     sum = total;
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (((32 * n + 8 * (e / 4)) * 4) / DP != wave) continue;
-        const int at_ = (32 * n + entry(e)) * 32 + (l & 31);
-        o[0][n][e] = ((os[at_] + os[DP * 32 + at_]) + os[2 * DP * 32 + at_]) + os[3 * DP * 32 + at_];
-      }
   }
-  if (r >= s.R) return;
-  const bool lead = KW == 1 || wave == 0;
-  const int64_t row = (int64_t)bh * s.R + r;
+  if (parts == 1) f *= sum == 0.f ? 0.f : 1.f / sum;  // no key: 0; a NaN stays one
+  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, o[0], f);
+  if (KW == 4) __syncthreads();
+  const int64_t row = (int64_t)bh * s.R + r;  // the lane's
+  const bool lead = r < s.R && h == 0 && (KW == 1 || wave == 0);
   if (parts > 1) {
     const int64_t rows = (int64_t)s.B * s.Hk * s.R;
-    float *op = a.part + ((int64_t)part * rows + row) * DP;
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
-        const float x[4] = {o[0][n][4 * e4], o[0][n][4 * e4 + 1], o[0][n][4 * e4 + 2],
-                            o[0][n][4 * e4 + 3]};
-        store_quad<float>(op, 32 * n + entry(4 * e4), DP, x);
-      }
-    if (lead && h == 0) {
+    float *op = a.part + ((int64_t)part * rows + (int64_t)bh * s.R + r0) * DP;
+    each_vector<DP, KW>(smem, wave, [&](int i, int d, const f32x4 &x) {
+      if (r0 + i < s.R) store_quad<float>(op + i * DP, d, DP, x);
+    });
+    if (lead) {
       float *ml = a.part + (int64_t)a.most * rows * DP + ((int64_t)part * rows + row) * 2;
       ml[0] = m;
       ml[1] = sum;
     }
     return;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: 0; a NaN stays one
   const int64_t to = (((int64_t)b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
-  T *out = reinterpret_cast<T *>(a.out) + to;
-  T *low = a.low ? reinterpret_cast<T *>(a.low) + to : nullptr;
+  each_vector<DP, KW>(smem, wave, [&](int i, int d, const f32x4 &x) {
+    const int64_t at_ = from_lane(to, i);
+    if (r0 + i >= s.R) return;
+    store_quad<T>(reinterpret_cast<T *>(a.out) + at_, d, s.D, x);
+    if (a.low) {
+      f32x4 y;
 #pragma unroll
-  for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      if (KW == 4 && ((32 * n + 8 * e4) * 4) / DP != wave) continue;
-      float x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = o[0][n][4 * e4 + i] * inv;
-        y[i] = x[i] - to_f32(from_f32<T>(x[i]));
-      }
-      store_quad<T>(out, 32 * n + entry(4 * e4), s.D, x);
-      if (low) store_quad<T>(low, 32 * n + entry(4 * e4), s.D, y);
+      for (int e = 0; e < 4; ++e) y[e] = x[e] - to_f32(from_f32<T>(x[e]));
+      store_quad<T>(reinterpret_cast<T *>(a.low) + at_, d, s.D, y);
     }
-  if (a.lse && lead && h == 0) a.lse[row] = sum == 0.f ? kInf : m + __log2f(sum);
+  });
+  if (a.lse && lead) a.lse[row] = sum == 0.f ? kInf : m + __log2f(sum);
 }
 
 // Joins the parts of a row, in a fixed order: W wavefronts a row, every W-th part each.

@@ -146,6 +146,35 @@ __device__ __forceinline__ floatx16 mma(const u32x4 &a, const u32x4 &b, floatx16
   }
 }
 
+// One step's left operand of mma_rows, and of mma_cols in 16 bits (step j: rows 16 (j / NB) .. + 15,
+// column block j % NB), for products that are placed one by one.
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 row_frag(const char *tile, int kb, int k) {
+  using C = Tile<T, DP>;
+  const int l = threadIdx.x & 63, h = l >> 5, row = l & 31;
+  return *reinterpret_cast<const u32x4 *>(tile + (kb * 32 + row) * C::ROW +
+                                          ((2 * k + h) ^ C::swz(row)) * 16);
+}
+// A transposing read: of each 16 lanes, lane a + 4 q addresses row q at columns 4 a .. 4 a + 3
+// and lane i receives column i of the four rows.
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 col_frag(const char *tile, int kb, int step) {
+  using C = Tile<T, DP>;
+  static_assert(sizeof(T) == 2, "16-bit elements");
+  const int l = threadIdx.x & 63, h = l >> 5, j = l & 15;
+  const int vec = 4 * (step % C::NB) + 2 * ((l >> 4) & 1) + ((j & 3) >> 1), in = (j & 1) * 8;
+  const int ra = 16 * (step / C::NB) + 4 * h + (j >> 2), rb = ra + 8;
+  const char *p = tile + kb * 32 * C::ROW + in;
+  const v4s u = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_v4s)(p + ra * C::ROW + ((vec ^ C::swz(ra)) << 4)));
+  const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_v4s)(p + rb * C::ROW + ((vec ^ C::swz(rb)) << 4)));
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// What comes before stays before: the order in which the source places reads, products and
+// vector operations is the order in which they issue.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // acc[n] += rows 32 kb .. + 31 of the tile times the columns held in b[n] (one row of DP elements
 // a lane: vector 2 k + lane / 32 of it at step k).
 template <typename T, int DP, int N>
@@ -206,24 +235,13 @@ __device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<
       }
     }
   } else {
-    // A transposing read: of each 16 lanes, lane a + 4 q addresses row q at columns 4 a .. 4 a + 3
-    // and lane i receives column i of the four rows.
-    const int j = l & 15, r0 = 4 * h + (j >> 2);
-    const int vec = 2 * ((l >> 4) & 1) + ((j & 3) >> 1), in = (j & 1) * 8;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int j = 0; j < 2 * C::NB; ++j) {
+      const u32x4 a = col_frag<T, DP>(tile, kb, j);
 #pragma unroll
-      for (int nb = 0; nb < C::NB; ++nb) {
-        const int ra = 16 * s + r0, rb = ra + 8;
-        const char *pa = p + ra * C::ROW + (((4 * nb + vec) ^ C::swz(ra)) << 4) + in;
-        const char *pb = p + rb * C::ROW + (((4 * nb + vec) ^ C::swz(rb)) << 4) + in;
-        const v4s u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)pa);
-        const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)pb);
-        const u32x4 a =
-            __builtin_bit_cast(u32x4, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int n = 0; n < N; ++n) acc[n][nb] = mma<T>(a, x[n].v[s], acc[n][nb]);
-      }
+      for (int n = 0; n < N; ++n)
+        acc[n][j % C::NB] = mma<T>(a, x[n].v[j / C::NB], acc[n][j % C::NB]);
+    }
   }
 }
 

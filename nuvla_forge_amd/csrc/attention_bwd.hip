@@ -283,29 +283,84 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
     if (at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
     const char *qt = smem + buf * F::STAGE, *dt = qt + F::TILE;
     const float *lse = reinterpret_cast<const float *>(qt + 2 * F::TILE), *nd = lse + 64;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < F::TR / 32; ++i) {
-      floatx16 p[1] = {splat(0.f)}, ds[1];
+      for (int i = 0; i < F::TR / 32; ++i) {
+        floatx16 p[1] = {splat(0.f)}, ds[1];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
-      mma_rows<T, DP, 1>(qt, i, k, p);
-      mma_rows<T, DP, 1>(dt, i, v, ds);
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
-      if constexpr (EDGE) {
+        for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
+        mma_rows<T, DP, 1>(qt, i, k, p);
+        mma_rows<T, DP, 1>(dt, i, v, ds);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
-      }
+          p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
+        if constexpr (EDGE) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
-      Packed<T> x[1];
-      x[0].set(p[0]);
-      mma_cols<T, DP, 1>(dt, i, x, dv);
-      range.fit(ds[0], dk[0]);
-      x[0].set(ds[0]);
-      mma_cols<T, DP, 1>(qt, i, x, dk);
+          for (int e = 0; e < 16; ++e)
+            p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
+        Packed<T> x[1];
+        x[0].set(p[0]);
+        mma_cols<T, DP, 1>(dt, i, x, dv);
+        range.fit(ds[0], dk[0]);
+        x[0].set(ds[0]);
+        mma_cols<T, DP, 1>(qt, i, x, dk);
+      }
+    } else {
+      // Four products of KS steps each, in an order that keeps the matrix pipe fed by a wavefront
+      // alone on its SIMD: a product's operands are read under the one before it, the exponentials
+      // form under dP and dS under dV.
+      constexpr int KS = C::KS, PER = (16 + KS - 2) / (KS - 1);  // entries a step after the first
+      static_assert(KS == 2 * C::NB, "as many steps along a row as down the columns");
+      u32x4 fa[KS], fb[KS];
+#pragma unroll
+      for (int j = 0; j < KS; ++j) fa[j] = row_frag<T, DP>(qt, 0, j);
+#pragma unroll
+      for (int i = 0; i < F::TR / 32; ++i) {
+        floatx16 p = splat(0.f), ds, ls;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          ds[e] = nd[32 * i + entry(e)];
+          ls[e] = lse[32 * i + entry(e)];
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          fb[j] = row_frag<T, DP>(dt, i, j);
+          p = mma<T>(fa[j], k[0][j], p);
+          in_order();
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          fa[j] = col_frag<T, DP>(dt, i, j);
+          ds = mma<T>(fb[j], v[0][j], ds);
+#pragma unroll
+          for (int e = (j - 1) * PER; e >= 0 && e < j * PER && e < 16; ++e) {
+            p[e] = exp2_(fmaf(p[e], s.c, kPExp<T> - ls[e]));
+            if constexpr (EDGE) p[e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[e] : 0.f;
+          }
+          in_order();
+        }
+        Packed<T> x;
+        x.set(p);
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          fb[j] = col_frag<T, DP>(qt, i, j);
+          dv[0][j % C::NB] = mma<T>(fa[j], x.v[j / C::NB], dv[0][j % C::NB]);
+#pragma unroll
+          for (int e = (j - 1) * PER; e >= 0 && e < j * PER && e < 16; ++e) ds[e] *= p[e];
+          in_order();
+        }
+        range.fit(ds, dk[0]);
+        x.set(ds);
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          if (i + 1 < F::TR / 32) fa[j] = row_frag<T, DP>(qt, i + 1, j);
+          dk[0][j % C::NB] = mma<T>(fb[j], x.v[j / C::NB], dk[0][j % C::NB]);
+          in_order();
+        }
+      }
     }
     buf ^= 1;
     ++at;

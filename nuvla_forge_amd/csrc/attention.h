@@ -106,25 +106,35 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char *p) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), (short)0, 0x7fffffff, 0x00020000);
 }
 
-// ROWS rows to LDS: `at(row, &in)` gives a row's byte offset from p and whether it exists.
-template <typename T, int DP, int ROWS, class F>
-__device__ __forceinline__ void copy_tile(const char *p, int nvec, char *lds, int wave, F &&at) {
+// The byte offsets at which a lane's copies of a tile of ROWS rows read, and the copies themselves:
+// 1 KB of the tile each, 64 / NV rows.
+template <typename T, int DP, int ROWS>
+struct TileCopy {
   using C = Tile<T, DP>;
-  constexpr int CW = ROWS * C::NV / kThreads;
+  static constexpr int CW = ROWS * C::NV / kThreads;
   static_assert(CW >= 1 && ROWS * C::NV % kThreads == 0, "a tile is whole 1 KB copies a wavefront");
-  const int l = threadIdx.x & 63;
-  const auto rsrc = buffer(p);
+  uint32_t off[CW];
+  // `at(row, &in)`: a row's byte offset and whether it exists
+  template <class F>
+  __device__ __forceinline__ void set(int nvec, int wave, F &&at) {
+    const int l = threadIdx.x & 63;
 #pragma unroll
-  for (int c = 0; c < CW; ++c) {
-    const int chunk = wave * CW + c;
-    const int row = chunk * (64 / C::NV) + l / C::NV;
-    const int vec = (l % C::NV) ^ C::swz(row);
-    bool in;
-    const uint32_t o = at(row, &in) + (uint32_t)vec * 16u;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(lds + chunk * 1024), 16,
-                                             in && vec < nvec ? o : kOob, 0, 0, 0);
+    for (int c = 0; c < CW; ++c) {
+      const int row = (wave * CW + c) * (64 / C::NV) + l / C::NV;
+      const int vec = (l % C::NV) ^ C::swz(row);
+      bool in = true;
+      const uint32_t o = at(row, &in) + (uint32_t)vec * 16u;
+      off[c] = in && vec < nvec ? o : kOob;
+    }
   }
-}
+  __device__ __forceinline__ void issue(const char *p, char *lds, int wave) const {
+    const auto rsrc = buffer(p);
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(lds + (wave * CW + c) * 1024), 16,
+                                               off[c], 0, 0, 0);
+  }
+};
 
 // ---------------------------------------------------------------------------
 // products
@@ -365,16 +375,24 @@ struct KeyTiles {
       return (uint32_t)(x >> (32 * (i & 1)));
     }
   };
+  using Copy = TileCopy<T, DP, TK>;
   const Shape &s;
   const char *k, *v;
   int64_t kt, vt;  // bytes from key to key
   const uint64_t *bits;
   int end;  // the first tile that is not wanted
+  int wave;
+  Copy kc, vc;  // of a whole tile
 
   __device__ __forceinline__ KeyTiles(const Shape &s_, const View &kv, const View &vv, int b,
-                                      int hk, int end_)
+                                      int hk, int end_, int wave_)
       : s(s_), k(kv.p + b * kv.b + hk * kv.h), v(vv.p + b * vv.b + hk * vv.h), kt(kv.t), vt(vv.t),
-        bits(MASKED ? s_.bits + (int64_t)b * s_.words : nullptr), end(end_) {}
+        bits(MASKED ? s_.bits + (int64_t)b * s_.words : nullptr), end(end_), wave(wave_) {
+    if constexpr (!MASKED) {
+      kc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)kt; });
+      vc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)vt; });
+    }
+  }
 
   // the first tile from i on that has keys, and its bits
   __device__ __forceinline__ int seek(int i, Bits &x) const {
@@ -394,23 +412,59 @@ struct KeyTiles {
     }
     return i;
   }
-  __device__ __forceinline__ void copy_one(const char *p, int64_t step, int i, const Bits &x,
-                                           char *lds, int wave) const {
+  __device__ __forceinline__ void copy_one(const char *p, int64_t step, const Copy &whole, int i,
+                                           const Bits &x, char *lds) const {
     const int left = s.Tk - i * TK;
-    const uint32_t st = (uint32_t)step;
-    copy_tile<T, DP, TK>(p + (int64_t)i * TK * step, s.nvec, lds, wave, [&](int row, bool *in) {
+    const char *at = p + (int64_t)i * TK * step;
+    if (!MASKED && left >= TK) return whole.issue(at, lds, wave);
+    Copy c;
+    c.set(s.nvec, wave, [&](int row, bool *in) {
       *in = row < left;
       if constexpr (MASKED) {
         uint64_t w = x.w[0];
         if constexpr (N == 2) w = row >= 64 ? x.w[1] : x.w[0];
         *in = *in && (w >> (row & 63) & 1);
       }
-      return (uint32_t)row * st;
+      return (uint32_t)row * (uint32_t)step;
+    });
+    c.issue(at, lds, wave);
+  }
+  __device__ __forceinline__ void copy(int i, const Bits &x, char *lds) const {
+    copy_one(k, kt, kc, i, x, lds);
+    copy_one(v, vt, vc, i, x, lds + TILE);
+  }
+};
+
+// A key head's rows of q or dout, tile by tile of TR, into LDS.
+template <typename T, int DP, int TR>
+struct RowTiles {
+  using Copy = TileCopy<T, DP, TR>;
+  const Shape &s;
+  const char *p;
+  int64_t t, h;  // bytes from token to token, head to head
+  int wave;
+  bool fixed;  // G divides TR: every tile begins with a token's first row
+  Copy whole;
+
+  __device__ __forceinline__ RowTiles(const Shape &s_, const View &v, int b, int hk, int wave_)
+      : s(s_), p(v.p + b * v.b + (int64_t)hk * s_.G * v.h), t(v.t), h(v.h), wave(wave_),
+        fixed(TR % s_.G == 0) {
+    set(whole, 0, TR);
+  }
+  __device__ __forceinline__ void set(Copy &c, int g0, int left) const {
+    c.set(s.nvec, wave, [&](int row, bool *in) {
+      *in = row < left;
+      const int x = g0 + row, dt = div_g(s, x), g = x - dt * s.G;
+      return (uint32_t)dt * (uint32_t)t + (uint32_t)g * (uint32_t)h;
     });
   }
-  __device__ __forceinline__ void copy(int i, const Bits &x, char *lds, int wave) const {
-    copy_one(k, kt, i, x, lds, wave);
-    copy_one(v, vt, i, x, lds + TILE, wave);
+  __device__ __forceinline__ void copy(int row0, char *lds) const {
+    const int t0 = row0 / s.G, left = s.R - row0;
+    const char *at = p + (int64_t)t0 * t;
+    if (fixed && left >= TR) return whole.issue(at, lds, wave);
+    Copy c;
+    set(c, row0 - t0 * s.G, left);
+    c.issue(at, lds, wave);
   }
 };
 

@@ -149,15 +149,15 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   for (int n = 0; n < C::NB; ++n) dq[0][n] = splat(0.f);
   Ranged<T, C::NB> range;
 
-  const typename F::Keys keys(s, a.k, a.v, b, hk, end);
+  const typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
-  int at = keys.seek(begin, cur), buf = 0;
-  if (at < end) keys.copy(at, cur, smem, wave);
-  auto step = [&](auto edge) {
+  int at = keys.seek(begin, cur);
+  if (at < end) keys.copy(at, cur, smem);
+  auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE, wave);
+    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
     const int kb0 = KW == 4 ? wave : 0;
 #pragma unroll
@@ -179,15 +179,21 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) keys.copy(next, nxt, smem, wave);
-    } else {
-      buf ^= 1;
+      if (next < end) keys.copy(next, nxt, smem);
     }
     at = next;
     cur = nxt;
   };
-  while (at < full) step(std::false_type{});
-  while (at < end) step(std::true_type{});
+  // tiles that every row sees whole, in pairs, so that the buffers' addresses are constants
+  while (at + 1 < full) {
+    step(std::false_type{}, 0);
+    step(std::false_type{}, F::STAGES - 1);
+  }
+  int buf = 0;
+  while (at < end) {
+    step(std::true_type{}, buf);
+    buf ^= F::STAGES - 1;
+  }
   const float f = s.scale * range.undo();
   __syncthreads();
   Turned<DP>::put(smem + wave * Turned<DP>::BYTES, dq[0], f);
@@ -248,21 +254,13 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int64_t every = s.causal ? (int64_t)max(tile * F::BK + F::BK - 1 - s.off, 0) * s.G : 0;
   const int full = (int)min((every + F::TR - 1) / F::TR, (int64_t)end);
 
-  const char *qp = a.q.p + b * a.q.b + (int64_t)hk * s.G * a.q.h;
-  const char *dp = a.dout.p + b * a.dout.b + (int64_t)hk * s.G * a.dout.h;
   const char *lp = reinterpret_cast<const char *>(a.lse + (int64_t)bh * s.R);
   const char *np = reinterpret_cast<const char *>(a.ndelta + (int64_t)bh * s.R);
+  const RowTiles<T, DP, F::TR> qs(s, a.q, b, hk, wave), dos(s, a.dout, b, hk, wave);
   auto copy = [&](int i, char *buf) {
-    const int row0 = i * F::TR, t0 = row0 / s.G, g0 = row0 - t0 * s.G, left = s.R - row0;
-    auto rows = [&](const View &w) {
-      return [&, wt = (uint32_t)w.t, wh = (uint32_t)w.h](int row, bool *in) {
-        *in = row < left;
-        const int x = g0 + row, dt = div_g(s, x), g = x - dt * s.G;
-        return (uint32_t)dt * wt + (uint32_t)g * wh;
-      };
-    };
-    copy_tile<T, DP, F::TR>(qp + (int64_t)t0 * a.q.t, s.nvec, buf, wave, rows(a.q));
-    copy_tile<T, DP, F::TR>(dp + (int64_t)t0 * a.dout.t, s.nvec, buf + F::TILE, wave, rows(a.dout));
+    const int row0 = i * F::TR, left = s.R - row0;
+    qs.copy(row0, buf);
+    dos.copy(row0, buf + F::TILE);
     if (wave < 2) {
       const auto rsrc = buffer((wave == 0 ? lp : np) + (int64_t)row0 * 4);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -275,9 +273,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   for (int n = 0; n < C::NB; ++n) dk[0][n] = dv[0][n] = splat(0.f);
   Ranged<T, C::NB> range;
 
-  int buf = 0;
-  if (at < end) copy(at, smem);
-  auto step = [&](auto edge) {
+  // The whole tiles that every row and key share come last, in pairs, so that the buffers' addresses
+  // are constants; an odd one goes with the edge.
+  const int pairs = max(end - max(at, full), 0) / 2, rest = end - 2 * pairs;
+  int buf = (rest - at) & 1;
+  if (at < end) copy(at, smem + buf * F::STAGE);
+  auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     gemm::wait_vm_barrier<0>();
     if (at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
@@ -362,11 +363,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
         }
       }
     }
-    buf ^= 1;
     ++at;
   };
-  while (at < full) step(std::true_type{});
-  while (at < end) step(std::false_type{});
+  while (at < rest) {
+    step(std::true_type{}, buf);
+    buf ^= 1;
+  }
+  while (at < end) {
+    step(std::false_type{}, 0);
+    step(std::false_type{}, 1);
+  }
   __syncthreads();
   const float fv = exp2_(-kPExp<T>), fk = s.scale * exp2_(-kPExp<T>) * range.undo();
   char *turned = smem + wave * Turned<DP>::BYTES;

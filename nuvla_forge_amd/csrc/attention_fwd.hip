@@ -81,16 +81,15 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   for (int n = 0; n < C::NB; ++n) o[0][n] = splat(0.f);
   float m = -kInf, sum = 0.f;  // sum: of the lane's own entries
 
-  const typename F::Keys keys(s, a.k, a.v, b, hk, end);
+  const typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
   at = keys.seek(at, cur);
-  int buf = 0;
-  if (at < end) keys.copy(at, cur, smem, wave);
-  auto step = [&](auto edge) {
+  if (at < end) keys.copy(at, cur, smem);
+  auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE, wave);
+    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
     const int kb0 = KW == 4 ? wave : 0;
     floatx16 p[F::NK];
@@ -133,15 +132,21 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) keys.copy(next, nxt, smem, wave);
-    } else {
-      buf ^= 1;
+      if (next < end) keys.copy(next, nxt, smem);
     }
     at = next;
     cur = nxt;
   };
-  while (at < full) step(std::false_type{});
-  while (at < end) step(std::true_type{});
+  // tiles that every row sees whole, in pairs, so that the buffers' addresses are constants
+  while (at + 1 < full) {
+    step(std::false_type{}, 0);
+    step(std::false_type{}, F::STAGES - 1);
+  }
+  int buf = 0;
+  while (at < end) {
+    step(std::true_type{}, buf);
+    buf ^= F::STAGES - 1;
+  }
   sum = pair_sum(sum);
 
   __syncthreads();

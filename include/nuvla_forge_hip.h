@@ -397,8 +397,8 @@ int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
  * Attention: out[b, i, h] = sum_j P[i, j] v[b, j, h / G],
  * P = softmax over the keys j that row i may attend of scale q[b, i, h] .
  * k[b, j, h / G], G = H / Hk (whole).  A key may be attended where key_mask
- * (bytes [B, Tk] with strides mask_b, mask_t, in bytes; NULL: all) is not 0
- * and, if `causal`, j <= i + Tk - Tq.  A row without a key gives zeros.  (The
+ * (bytes [B, Tk], samples mask_b bytes apart; NULL: all) is not 0 and, if
+ * `causal`, j <= i + Tk - Tq.  A row without a key gives zeros.  (The
  * reference's models call F.scaled_dot_product_attention, model/dit.py:92.)
  * q [B, Tq, H, D], k and v [B, Tk, Hk, D] with unit last stride and strides
  * *_b, *_t, *_h in elements (0: broadcast): every row starts on 16 bytes, and
@@ -406,28 +406,27 @@ int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
  * zeros.  out [B, Tq, H, D] dense.  D at most 128; Tk at least 1; 130 token
  * strides and H / Hk head strides below 2^30 bytes; scale finite.  Rows that
  * the mask drops from k and v are not read.
- * `state` (nf_attention_state_bytes) holds the mask in bits and, with `keep`
- * (a backward will come), each row's log-sum-exp and, for 16-bit types, what
- * the rounding of out left; `workspace` nothing between calls; both 16-byte
- * aligned.  A size call returns 0 for arguments beyond the kernels.
+ * `state` (nf_attention_state_bytes; NULL: no backward will come) takes each
+ * row's log-sum-exp and, for 16-bit types, what the rounding of out left;
+ * `workspace` holds nothing between calls; both 16-byte aligned.  A size call
+ * returns 0 for arguments beyond the kernels.
  * ---------------------------------------------------------------------- */
 size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                int64_t Hk, int64_t D, int has_mask, int keep,
-                                int dtype);
+                                int64_t Hk, int64_t D, int dtype);
 size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
                                   int64_t Hk, int64_t D, int causal,
                                   int dtype);
 int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
                      const void *k, int64_t k_b, int64_t k_t, int64_t k_h,
                      const void *v, int64_t v_b, int64_t v_t, int64_t v_h,
-                     const uint8_t *key_mask, int64_t mask_b, int64_t mask_t,
-                     int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk,
-                     int64_t D, int causal, float scale, int keep, int dtype,
-                     void *out, void *state, size_t state_bytes,
-                     void *workspace, size_t workspace_bytes, void *stream);
+                     const uint8_t *key_mask, int64_t mask_b, int64_t B,
+                     int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D,
+                     int causal, float scale, int dtype, void *out,
+                     void *state, size_t state_bytes, void *workspace,
+                     size_t workspace_bytes, void *stream);
 
 /* Its gradient for dout (strides g_*; rows as q's), out and `state` as the
- * forward left them with `keep` (has_mask: it had a key_mask):
+ * forward left them, the forward's key_mask:
  *   dv = P^T dout,  dS = P (dout v^T - rowsum(dout out)),
  *   dq = scale dS k,  dk = scale dS^T q,
  * dk and dv summed over the G heads of a group; dense, in `dtype`; any may be
@@ -438,12 +437,13 @@ size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
 int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
                      const void *k, int64_t k_b, int64_t k_t, int64_t k_h,
                      const void *v, int64_t v_b, int64_t v_t, int64_t v_h,
-                     const void *out, const void *dout, int64_t g_b,
-                     int64_t g_t, int64_t g_h, int64_t B, int64_t Tq,
-                     int64_t Tk, int64_t H, int64_t Hk, int64_t D, int causal,
-                     float scale, int has_mask, int dtype, const void *state,
-                     size_t state_bytes, void *dq, void *dk, void *dv,
-                     void *workspace, size_t workspace_bytes, void *stream);
+                     const uint8_t *key_mask, int64_t mask_b, const void *out,
+                     const void *dout, int64_t g_b, int64_t g_t, int64_t g_h,
+                     int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk,
+                     int64_t D, int causal, float scale, int dtype,
+                     const void *state, size_t state_bytes, void *dq, void *dk,
+                     void *dv, void *workspace, size_t workspace_bytes,
+                     void *stream);
 
 /* ------------------------------------------------------------------------
  * Rotary positions over 1 to 4 axes: with sections[a] pairs for axis a, P in

@@ -110,17 +110,17 @@ SIGNATURES = {
         _I32,
         [_P, _P, _I64, _F32, _I64, _I64, _I64, _P, _I32, _I32, _P, _SZ, _P],
     ),
-    "nf_attention_state_bytes": (_SZ, [*[_I64] * 6, _I32, _I32, _I32]),
+    "nf_attention_state_bytes": (_SZ, [*[_I64] * 6, _I32]),
     "nf_attention_fwd_workspace": (_SZ, [*[_I64] * 6, _I32, _I32]),
     "nf_attention_fwd": (
         _I32,
-        [*[_P, _I64, _I64, _I64] * 3, _P, _I64, _I64, *[_I64] * 6, _I32, _F32, _I32, _I32, _P,
-         _P, _SZ, _P, _SZ, _P],
+        [*[_P, _I64, _I64, _I64] * 3, _P, _I64, *[_I64] * 6, _I32, _F32, _I32, _P, _P, _SZ, _P,
+         _SZ, _P],
     ),
     "nf_attention_bwd_workspace": (_SZ, [*[_I64] * 6, _I32, _I32]),
     "nf_attention_bwd": (
         _I32,
-        [*[_P, _I64, _I64, _I64] * 3, _P, _P, _I64, _I64, _I64, *[_I64] * 6, _I32, _F32, _I32,
+        [*[_P, _I64, _I64, _I64] * 3, _P, _I64, _P, _P, _I64, _I64, _I64, *[_I64] * 6, _I32, _F32,
          _I32, _P, _SZ, _P, _P, _P, _P, _SZ, _P],
     ),
     "nf_rotary": (

@@ -20,7 +20,7 @@
 //
 // Tiles.  Rows of DP elements, copied from memory to LDS by the buffer unit; 16-byte vectors
 // XOR-swizzled by row.  Rows past the end, columns past D and keys that the mask drops come from
-// beyond the buffer's bound, as zeros: what memory holds there is never read.
+// beyond the buffer's bound, as zeros, or their results are replaced, not multiplied away.
 #pragma once
 
 #include "gemm_core.h"
@@ -52,12 +52,12 @@ struct Shape {
   int nvec;       // 16-byte vectors of a row that hold columns
   int off;        // causal: row t sees keys up to t + off = t + Tk - Tq
   int causal;
-  int words;      // mask words (64 keys each) of a sample
   uint32_t ginv;  // ceil(2^32 / G), 0 for G = 1
   float c;        // |scale| log2(e)
   float scale;
   uint32_t flip;  // scale < 0: the sign bits of one operand of S are flipped
-  const uint64_t *bits;  // [B, words]: the keys that may be attended; null: all
+  const uint8_t *mask;  // [B, Tk], bytes: the keys that may be attended (not 0); null: all
+  int64_t mask_b;       // from sample to sample
 };
 
 // x / G for the small x of a tile
@@ -222,6 +222,25 @@ struct Packed<float> {
   floatx16 v;
   __device__ __forceinline__ void set(const floatx16 &x) { v = x; }
 };
+// In two terms, the second what the first's rounding left: no rounding to 16 bits is then felt.
+// For the calls with few rows, which no matrix product bounds and whose results are sums of few
+// such terms.
+template <typename T>
+struct Twice {
+  Packed<T> hi, lo;
+  __device__ __forceinline__ void set(const floatx16 &x) {
+    floatx16 y;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = x[i] - to_f32(from_f32<T>(x[i]));
+    hi.set(x);
+    lo.set(y);
+  }
+};
+template <>
+struct Twice<float> {
+  Packed<float> hi;
+  __device__ __forceinline__ void set(const floatx16 &x) { hi.set(x); }
+};
 
 // acc[n][nb] += (columns 32 nb .. + 31 of rows 32 kb .. + 31 of the tile)^T x[n], over those rows
 // in the order in which the lanes hold x.
@@ -251,6 +270,24 @@ __device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<
 #pragma unroll
       for (int n = 0; n < N; ++n)
         acc[n][j % C::NB] = mma<T>(a, x[n].v[j / C::NB], acc[n][j % C::NB]);
+    }
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void mma_cols(const char *tile, int kb, const Twice<T> &x,
+                                         floatx16 (&acc)[1][Tile<T, DP>::NB]) {
+  using C = Tile<T, DP>;
+  if constexpr (sizeof(T) == 4) {
+    const Packed<T> y[1] = {x.hi};
+    mma_cols<T, DP, 1>(tile, kb, y, acc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2 * C::NB; ++j) {
+      const u32x4 a = col_frag<T, DP>(tile, kb, j);
+      floatx16 &to = acc[0][j % C::NB];
+      to = mma<T>(a, x.lo.v[j / C::NB], to);
+      to = mma<T>(a, x.hi.v[j / C::NB], to);
     }
   }
 }
@@ -299,10 +336,61 @@ __device__ __forceinline__ int entry(int i) {
 // ---------------------------------------------------------------------------
 // tiles of keys
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t uniform(uint64_t x) {  // in scalar registers
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
-         (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
-}
+// The mask of a sample in words of 64 keys, 64 words at a time: lane i holds word i of the chunk.
+// A word is read by readlane, and the next one that has a key found in the lanes' ballot.
+struct MaskWords {
+  const uint8_t *p;  // the sample's bytes
+  int keys;
+  int chunk;      // the one that is held
+  uint64_t mine;  // the lane's word
+  uint64_t some;  // the words that have a key
+
+  // not 0 for each byte, as 4 bits
+  __device__ __forceinline__ static uint32_t four(uint32_t x) {
+    x |= x >> 4;
+    x |= x >> 2;
+    x |= x >> 1;
+    return ((x & 0x01010101u) * 0x01020408u) >> 24 & 15u;
+  }
+  __device__ __forceinline__ void load(int c) {
+    const int l = threadIdx.x & 63;
+    mine = 0;
+    if (keys < 64) {
+      const uint64_t all = __ballot(l < keys && p[min(l, keys - 1)] != 0);
+      if (l == 0) mine = all;
+    } else {
+      const int64_t at = ((int64_t)c * 64 + l) * 64;
+      const int64_t from = at + 64 <= keys ? at : keys - 64;  // the last word: the last 64 bytes
+      if (at < keys) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x4 x;
+          __builtin_memcpy(&x, p + from + 16 * i, 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mine |= (uint64_t)four(x[j]) << (16 * i + 4 * j);
+        }
+        mine >>= at - from;
+      }
+    }
+    some = __ballot(mine != 0);
+    chunk = c;
+  }
+  __device__ __forceinline__ uint64_t word(int w) {
+    if (w >> 6 != chunk) load(w >> 6);
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), w & 63) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)mine, w & 63);
+  }
+  // the first word from w on that has a key, or `end`
+  __device__ __forceinline__ int next(int w, int end) {
+    while (w < end) {
+      if (w >> 6 != chunk) load(w >> 6);
+      const uint64_t from = some >> (w & 63);
+      if (from) return w + __builtin_ctzll(from);
+      w = (w | 63) + 1;
+    }
+    return end;
+  }
+};
 
 // The keys of 32 that a lane's row may attend: those up to `last` (of the 32; negative: none) whose
 // bit is in `word`, shifted so that entry i is bit 8 (i / 4) + i % 4 for every lane.
@@ -345,18 +433,30 @@ __host__ __device__ __forceinline__ int first_row_tile(const Shape &s, int tile,
   return at < end ? (int)at : end;
 }
 
-// The part length for `tiles` blocks a head of up to `longest` tiles each (causal: down to few),
-// `slots` blocks at once on the chip: about two blocks a slot, no part under 4 tiles.  Calls that
-// have many blocks to deal out anyway are not cut.
+// The part length for `tiles` blocks a head of up to `longest` tiles each, `slots` blocks at once on
+// the chip.  Blocks of one length go in rounds: as many parts as take the least time, in tiles a
+// block 1.5 beside its own, the join 3 and 1.2 for each part that a slot writes and reads.  A causal
+// call's blocks fall from the longest to few and fill up what it leaves: two parts a slot (dK and dV
+// of 2 x 4096 tokens, 4 key heads of 128: 585 us whole, 365 so, in 3 parts a slot 400, in 8 450).
 inline int part_length(int64_t heads, int64_t tiles, int64_t longest, bool causal, int slots) {
   const int64_t blocks = heads * tiles;
-  if (blocks >= 4 * (int64_t)slots || (!causal && blocks >= slots)) return 1 << 28;
-  int64_t total = blocks * longest;
-  if (causal && tiles > 1) total = total / 2 + 1;
-  int64_t c = (total + 2 * slots - 1) / (2 * slots);
-  if (c < 4) c = 4;
-  if (c < (longest + kMostParts - 1) / kMostParts) c = (longest + kMostParts - 1) / kMostParts;
-  return (int)c;
+  if (blocks >= 4 * (int64_t)slots) return 1 << 28;
+  if (causal && tiles > 1) {
+    const int64_t c = (blocks * longest / 2 + 2 * slots) / (2 * slots);
+    const int64_t least = c > 4 ? c : 4, most = (longest + kMostParts - 1) / kMostParts;
+    return (int)(least > most ? least : most);
+  }
+  int best = 1 << 28;
+  double time = 0.;
+  for (int n = 1; n <= kMostParts && n <= longest; ++n) {
+    const int64_t c = (longest + n - 1) / n, rounds = (blocks * n + slots - 1) / slots;
+    const double t = (double)rounds * ((double)c + 1.5) +
+                     (n > 1 ? 3. + 1.2 * n * (double)blocks / slots : 0.);
+    if (n > 1 && t >= time) continue;
+    time = t;
+    best = n == 1 ? 1 << 28 : (int)c;
+  }
+  return best;
 }
 
 // A key head's keys and values, tile by tile of TK, into LDS: K, then V.  MASKED: with the sample's
@@ -374,12 +474,18 @@ struct KeyTiles {
       if constexpr (N == 2) x = i >= 2 ? w[1] : w[0];
       return (uint32_t)(x >> (32 * (i & 1)));
     }
+    __device__ __forceinline__ bool all() const {
+      if constexpr (!MASKED) return true;
+      uint64_t x = w[0];
+      if constexpr (N == 2) x &= w[1];
+      return (TK == 32 ? x | ~0xffffffffull : x) == ~0ull;
+    }
   };
   using Copy = TileCopy<T, DP, TK>;
   const Shape &s;
   const char *k, *v;
   int64_t kt, vt;  // bytes from key to key
-  const uint64_t *bits;
+  MaskWords mask;
   int end;  // the first tile that is not wanted
   int wave;
   Copy kc, vc;  // of a whole tile
@@ -387,51 +493,74 @@ struct KeyTiles {
   __device__ __forceinline__ KeyTiles(const Shape &s_, const View &kv, const View &vv, int b,
                                       int hk, int end_, int wave_)
       : s(s_), k(kv.p + b * kv.b + hk * kv.h), v(vv.p + b * vv.b + hk * vv.h), kt(kv.t), vt(vv.t),
-        bits(MASKED ? s_.bits + (int64_t)b * s_.words : nullptr), end(end_), wave(wave_) {
-    if constexpr (!MASKED) {
-      kc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)kt; });
-      vc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)vt; });
+        end(end_), wave(wave_) {
+    if constexpr (MASKED) {
+      mask.p = s.mask + b * s.mask_b;
+      mask.keys = s.Tk;
+      mask.chunk = -1;
     }
+    kc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)kt; });
+    vc.set(s.nvec, wave, [&](int row, bool *) { return (uint32_t)row * (uint32_t)vt; });
   }
 
   // the first tile from i on that has keys, and its bits
-  __device__ __forceinline__ int seek(int i, Bits &x) const {
+  __device__ __forceinline__ int seek(int i, Bits &x) {
     if constexpr (MASKED) {
-      for (; i < end; ++i) {
-        uint64_t any = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if constexpr (TK == 32)
-            x.w[j] = uniform(bits[i >> 1] >> (32 * (i & 1))) & 0xffffffffull;
-          else
-            x.w[j] = i * N + j < s.words ? uniform(bits[i * N + j]) : 0ull;
-          any |= x.w[j];
+      const int stop = (s.Tk + 63) / 64;  // words
+      if constexpr (TK == 32) {
+        while (i < end) {
+          const int w = mask.next(i >> 1, stop);
+          if (w >= stop) return end;
+          if (i < 2 * w) i = 2 * w;
+          x.w[0] = mask.word(w) >> (32 * (i & 1)) & 0xffffffffull;
+          if (x.w[0]) break;
+          ++i;
         }
-        if (any) break;
+      } else {
+        const int w = mask.next(i * N, stop);
+        if (w >= stop) return end;
+        i = w / N;
+        if (i < end) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) x.w[j] = i * N + j < stop ? mask.word(i * N + j) : 0ull;
+        }
       }
+      if (i > end) i = end;
     }
     return i;
   }
+  // ZERO: the keys that the mask drops arrive as zeros; without, as they lie, for an operand of a
+  // product whose results for them are replaced
+  template <bool ZERO>
   __device__ __forceinline__ void copy_one(const char *p, int64_t step, const Copy &whole, int i,
                                            const Bits &x, char *lds) const {
     const int left = s.Tk - i * TK;
     const char *at = p + (int64_t)i * TK * step;
-    if (!MASKED && left >= TK) return whole.issue(at, lds, wave);
-    Copy c;
-    c.set(s.nvec, wave, [&](int row, bool *in) {
-      *in = row < left;
-      if constexpr (MASKED) {
-        uint64_t w = x.w[0];
-        if constexpr (N == 2) w = row >= 64 ? x.w[1] : x.w[0];
-        *in = *in && (w >> (row & 63) & 1);
-      }
-      return (uint32_t)row * (uint32_t)step;
-    });
+    if (left >= TK && (!(MASKED && ZERO) || x.all())) return whole.issue(at, lds, wave);
+    Copy c = whole;
+    constexpr int PER = 64 / Tile<T, DP>::NV, ROWS = Copy::CW * PER;  // rows of a copy, a wavefront
+    static_assert(ROWS <= 32, "a wavefront's rows are in one half of a word");
+    const int l = threadIdx.x & 63, row0 = wave * ROWS + l / Tile<T, DP>::NV;
+    uint32_t live = ~0u;
+    if constexpr (MASKED && ZERO) {
+      uint64_t w = x.w[0];
+      if constexpr (N == 2) w = wave >= kWaves / 2 ? x.w[1] : x.w[0];
+      live = (uint32_t)(w >> (row0 & 63));
+    }
+    const int rows = left - row0;  // from the lane's first on
+    if (rows < 32) live &= rows > 0 ? (1u << rows) - 1u : 0u;
+#pragma unroll
+    for (int j = 0; j < Copy::CW; ++j)
+      if (!(live & (1u << (j * PER)))) c.off[j] = kOob;
     c.issue(at, lds, wave);
   }
-  __device__ __forceinline__ void copy(int i, const Bits &x, char *lds) const {
-    copy_one(k, kt, kc, i, x, lds);
-    copy_one(v, vt, vc, i, x, lds + TILE);
+  template <bool ZERO>
+  __device__ __forceinline__ void copy_k(int i, const Bits &x, char *lds) const {
+    copy_one<ZERO>(k, kt, kc, i, x, lds);
+  }
+  template <bool ZERO>
+  __device__ __forceinline__ void copy_v(int i, const Bits &x, char *lds) const {
+    copy_one<ZERO>(v, vt, vc, i, x, lds + TILE);
   }
 };
 
@@ -549,20 +678,23 @@ struct Sizes {  // what a call is about, as its entry points take it
   int dtype;
   int es() const { return dtype == NF_DTYPE_F32 ? 4 : 2; }
   int64_t rows() const { return Tq * (H / Hk); }
-  int64_t words() const { return (Tk + 63) / 64; }
   int dp() const { return D <= 64 ? 64 : 128; }
 };
 // NF_OK, or the error that is set
 int check_sizes(const char *op, const Sizes &z);
 int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
               const Sizes &z, int64_t group, View *v);
-Shape make_shape(const Sizes &z, int causal, float scale, const uint64_t *bits);
+Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b);
 
-// The state's parts, in bytes from its start: log-sum-exps, mask words, what out's rounding left.
+// The state's parts, in bytes from its start: log-sum-exps, what out's rounding left.
 struct State {
-  size_t lse, bits, low, total;
+  size_t low, total;
 };
-State state_of(const Sizes &z, bool mask, bool keep);
+State state_of(const Sizes &z);
+// Whether the wavefronts of a block share its 32 rows (or keys) and split the other axis: `own` rows
+// or keys a head.  Wavefronts with 32 of their own read a tile once for 128; where the blocks of
+// 128 are fewer than fill the chip, four times the blocks are the faster.
+bool shared_blocks(const Sizes &z, int64_t own);
 
 }  // namespace attn
 }  // namespace nf

@@ -149,15 +149,19 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   for (int n = 0; n < C::NB; ++n) dq[0][n] = splat(0.f);
   Ranged<T, C::NB> range;
 
-  const typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
+  typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
+  auto copy = [&](int i, const typename F::Keys::Bits &x, char *lds) {
+    keys.template copy_k<true>(i, x, lds);   // a dropped key is multiplied by 0
+    keys.template copy_v<false>(i, x, lds);  // its value gives dS alone, which is replaced
+  };
   int at = keys.seek(begin, cur);
-  if (at < end) keys.copy(at, cur, smem);
+  if (at < end) copy(at, cur, smem);
   auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
     const int kb0 = KW == 4 ? wave : 0;
 #pragma unroll
@@ -173,13 +177,19 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
         for (int e = 0; e < 16; ++e) dp[0][e] = keep(dp[0][e], live, e, 0u);
       }
       range.fit(dp[0], dq[0]);
-      Packed<T> x[1];
-      x[0].set(dp[0]);
-      mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
+      if constexpr (KW == 4) {
+        Twice<T> x;
+        x.set(dp[0]);
+        mma_cols<T, DP>(kt, kb0 + i, x, dq);
+      } else {
+        Packed<T> x[1];
+        x[0].set(dp[0]);
+        mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
+      }
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) keys.copy(next, nxt, smem);
+      if (next < end) copy(next, nxt, smem);
     }
     at = next;
     cur = nxt;
@@ -209,21 +219,24 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   });
 }
 
-// A block has 128 keys, a wavefront 32, and goes over the rows.
-template <typename T, int DP>
+// KW = 1: a block has 128 keys, a wavefront 32, and goes over the rows.  KW = 4: a block has 32 keys,
+// and a wavefront a quarter of each tile's rows.
+template <typename T, int DP, int KW>
 struct Dkv {
   using C = Tile<T, DP>;
-  static constexpr int BK = 32 * kWaves;
-  static constexpr int TR = C::ROW > 256 ? 32 : 64;  // rows of a tile
+  static constexpr int BK = KW == 1 ? 32 * kWaves : 32;
+  static constexpr int TR = KW == 4 ? 128 : C::ROW > 256 ? 32 : 64;  // rows of a tile
+  static constexpr int NR = KW == 4 ? 1 : TR / 32;                   // of those, 32s of a wavefront
   static constexpr int TILE = TR * C::ROW;
-  static constexpr int STAGE = 2 * TILE + 2 * 256;  // q, dout, log-sum-exps, -deltas
-  static constexpr int LDS = 2 * STAGE;
+  static constexpr int STAGE = 2 * TILE + 2 * 4 * (TR < 64 ? 64 : TR);  // q, dout, lse, -delta
+  static constexpr int STAGES = 2 * STAGE <= 140 * 1024 ? 2 : 1;
+  static constexpr int LDS = STAGES * STAGE;
   static_assert(LDS >= kWaves * Turned<DP>::BYTES, "the results turn in the tiles' place");
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int KW>
 __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
-  using F = Dkv<T, DP>;
+  using F = Dkv<T, DP, KW>;
   using C = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
   const Shape &s = a.s;
@@ -237,10 +250,9 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   const int l = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  const int key0 = tile * F::BK + 32 * wave;
+  const int key0 = tile * F::BK + (KW == 1 ? 32 * wave : 0);
   const int key = key0 + (l & 31);
-  const uint64_t *bits = s.bits ? s.bits + (int64_t)b * s.words : nullptr;
-  const bool live = key < s.Tk && (!bits || (bits[key >> 6] >> (key & 63) & 1));
+  const bool live = key < s.Tk && (!s.mask || s.mask[b * s.mask_b + key]);
   u32x4 k[1][C::KS], v[1][C::KS];
   load_row<T, DP>(a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t, live, s.nvec, s.flip, k[0]);
   load_row<T, DP>(a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t, live, s.nvec, 0u, v[0]);
@@ -261,10 +273,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
     const int row0 = i * F::TR, left = s.R - row0;
     qs.copy(row0, buf);
     dos.copy(row0, buf + F::TILE);
-    if (wave < 2) {
-      const auto rsrc = buffer((wave == 0 ? lp : np) + (int64_t)row0 * 4);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (lds_ptr_t)(buf + 2 * F::TILE + 256 * wave), 4, l < left ? l * 4u : kOob, 0, 0, 0);
+    if (F::TR > 64 || wave < 2) {  // 64 values a wavefront: log-sum-exps, then -deltas
+      constexpr int EACH = F::TR > 64 ? 2 : 1;
+      const int at4 = (wave % EACH) * 64 + l;
+      const auto rsrc = buffer((wave < EACH ? lp : np) + (int64_t)row0 * 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(buf + 2 * F::TILE + 256 * wave), 4,
+                                               at4 < left ? at4 * 4u : kOob, 0, 0, 0);
     }
   };
 
@@ -276,17 +290,19 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   // The whole tiles that every row and key share come last, in pairs, so that the buffers' addresses
   // are constants; an odd one goes with the edge.
   const int pairs = max(end - max(at, full), 0) / 2, rest = end - 2 * pairs;
-  int buf = (rest - at) & 1;
+  int buf = (rest - at) & (F::STAGES - 1);
   if (at < end) copy(at, smem + buf * F::STAGE);
   auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     gemm::wait_vm_barrier<0>();
-    if (at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
+    if (F::STAGES == 2 && at + 1 < end) copy(at + 1, smem + (buf ^ 1) * F::STAGE);
     const char *qt = smem + buf * F::STAGE, *dt = qt + F::TILE;
-    const float *lse = reinterpret_cast<const float *>(qt + 2 * F::TILE), *nd = lse + 64;
-    if constexpr (sizeof(T) == 4) {
+    const float *lse = reinterpret_cast<const float *>(qt + 2 * F::TILE);
+    const float *nd = lse + (F::TR < 64 ? 64 : F::TR);
+    if constexpr (sizeof(T) == 4 || KW == 4) {
 #pragma unroll
-      for (int i = 0; i < F::TR / 32; ++i) {
+      for (int n = 0; n < F::NR; ++n) {
+        const int i = KW == 4 ? wave : n;
         floatx16 p[1] = {splat(0.f)}, ds[1];
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
@@ -302,12 +318,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
-        Packed<T> x[1];
-        x[0].set(p[0]);
-        mma_cols<T, DP, 1>(dt, i, x, dv);
+        Twice<T> x;
+        x.set(p[0]);
+        mma_cols<T, DP>(dt, i, x, dv);
         range.fit(ds[0], dk[0]);
-        x[0].set(ds[0]);
-        mma_cols<T, DP, 1>(qt, i, x, dk);
+        x.set(ds[0]);
+        mma_cols<T, DP>(qt, i, x, dk);
       }
     } else {
       // Four products of KS steps each, in an order that keeps the matrix pipe fed by a wavefront
@@ -364,22 +380,28 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
       }
     }
     ++at;
+    if (F::STAGES == 1) {
+      __syncthreads();
+      if (at < end) copy(at, smem);
+    }
   };
   while (at < rest) {
     step(std::true_type{}, buf);
-    buf ^= 1;
+    buf ^= F::STAGES - 1;
   }
   while (at < end) {
     step(std::false_type{}, 0);
-    step(std::false_type{}, 1);
+    step(std::false_type{}, F::STAGES - 1);
   }
   __syncthreads();
   const float fv = exp2_(-kPExp<T>), fk = s.scale * exp2_(-kPExp<T>) * range.undo();
   char *turned = smem + wave * Turned<DP>::BYTES;
   const int64_t first = (int64_t)bh * s.Tk + key0;
   auto put = [&](const floatx16(&acc)[C::NB], float f, void *out, int which) {
+    if (KW == 4) __syncthreads();
     Turned<DP>::put(turned, acc, f);
-    each_vector<DP, 1>(smem, wave, [&](int i, int d, const f32x4 &y) {
+    if (KW == 4) __syncthreads();
+    each_vector<DP, KW>(smem, wave, [&](int i, int d, const f32x4 &y) {
       // a key that is left out: zeros, whatever was formed
       const f32x4 x = __shfl((int)live, i) ? y : f32x4{0.f, 0.f, 0.f, 0.f};
       if (key0 + i >= s.Tk) return;
@@ -396,24 +418,24 @@ __global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
   put(dv[0], fv, a.dv, 1);
 }
 
-// Sums the parts of a row of dQ (KW: its kernel's), or of a key's dK and dV (KW = 0), in their
-// order: a wavefront a row.
-template <typename T, int DP, int KW>
+// Sums the parts of a row of dQ, or of a key's dK and dV (KEYS), in their order: a wavefront a row.
+// KW: as in the kernel that wrote them.
+template <typename T, int DP, int KW, bool KEYS>
 __global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
-  constexpr int W = KW ? DP : 2 * DP;  // of a row
+  constexpr int W = KEYS ? 2 * DP : DP;  // of a row
   const Shape &s = a.s;
-  const int per = KW ? s.R : s.Tk, l = threadIdx.x & 63;
+  const int per = KEYS ? s.Tk : s.R, l = threadIdx.x & 63;
   const int64_t rows = (int64_t)s.B * s.Hk * per;
   const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int64_t bh = row / per;
   const int r = (int)(row - bh * per);
   int len;
-  if constexpr (KW) {
-    using F = Dq<T, DP, KW ? KW : 1, false>;
+  if constexpr (!KEYS) {
+    using F = Dq<T, DP, KW, false>;
     len = key_tiles<F::TK>(s, r / F::BR, F::BR);
   } else {
-    using F = Dkv<T, DP>;
+    using F = Dkv<T, DP, KW>;
     len = (s.R + F::TR - 1) / F::TR - first_row_tile<F::TR>(s, r / F::BK, F::BK);
   }
   const int n = parts_of(len, a.length);
@@ -429,7 +451,7 @@ __global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
   for (int j = 0; j < W / 64; ++j) {
     const int c = l + 64 * j, d = c % DP;
     if (d >= s.D) continue;
-    if constexpr (KW) {
+    if constexpr (!KEYS) {
       const int64_t t = r / s.G, g = r % s.G;
       reinterpret_cast<T *>(a.dq)[((b * s.Tq + t) * s.H + hk * s.G + g) * s.D + d] =
           from_f32<T>(x[j]);
@@ -441,15 +463,16 @@ __global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
 }
 
 struct Plan {
-  int tiles, length, most;
+  int kw, tiles, length, most;
   size_t bytes;  // of the parts
 };
 
 Plan dq_plan(const Sizes &z, bool causal) {
-  const bool few = z.rows() <= 32, wide = z.dp() * z.es() > 256;
-  const int br = few ? 32 : 128, tk = few ? 128 : wide ? 32 : 64;
+  const bool shared = shared_blocks(z, z.rows()), wide = z.dp() * z.es() > 256;
+  const int br = shared ? 32 : 128, tk = shared ? 128 : wide ? 32 : 64;
   const int64_t heads = z.B * z.Hk, longest = (z.Tk + tk - 1) / tk;
   Plan p;
+  p.kw = shared ? 4 : 1;
   p.tiles = (int)((z.rows() + br - 1) / br);
   p.length = part_length(heads, p.tiles, longest, causal, 256);
   p.most = parts_of((int)longest, p.length);
@@ -458,10 +481,12 @@ Plan dq_plan(const Sizes &z, bool causal) {
 }
 
 Plan dkv_plan(const Sizes &z, bool causal) {
-  const int tr = z.dp() * z.es() > 256 ? 32 : 64;
+  const bool shared = shared_blocks(z, z.Tk);
+  const int bk = shared ? 32 : 128, tr = shared ? 128 : z.dp() * z.es() > 256 ? 32 : 64;
   const int64_t heads = z.B * z.Hk, longest = (z.rows() + tr - 1) / tr;
   Plan p;
-  p.tiles = (int)((z.Tk + 127) / 128);
+  p.kw = shared ? 4 : 1;
+  p.tiles = (int)((z.Tk + bk - 1) / bk);
   p.length = part_length(heads, p.tiles, longest, causal, 256);
   p.most = parts_of((int)longest, p.length);
   p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.Tk) * (size_t)z.dp() * 8 : 0;
@@ -479,13 +504,25 @@ size_t bwd_bytes(const Sizes &z, bool causal) {
 template <typename T, int DP, int KW>
 void launch_dq(BwdArgs &a, hipStream_t st) {
   const unsigned grid = (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most);
-  if (a.s.bits)
+  if (a.s.mask)
     attn_dq_kernel<T, DP, KW, true><<<grid, kThreads, 0, st>>>(a);
   else
     attn_dq_kernel<T, DP, KW, false><<<grid, kThreads, 0, st>>>(a);
   if (a.most > 1 && a.dq) {
     const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
-    attn_sum_kernel<T, DP, KW><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+    attn_sum_kernel<T, DP, KW, false><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+  }
+}
+
+template <typename T, int DP, int KW>
+void launch_dkv(BwdArgs &a, hipStream_t st) {
+  attn_dkv_kernel<T, DP, KW>
+      <<<(unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most), kThreads, 0,
+         st>>>(a);
+  if (a.most > 1) {
+    const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.Tk;
+    attn_sum_kernel<T, DP, KW, true>
+        <<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
   }
 }
 
@@ -495,22 +532,19 @@ int launch(BwdArgs a, const Sizes &z, hipStream_t st) {
     a.tiles = p.tiles;
     a.length = p.length;
     a.most = p.most;
+    return p.kw;
   };
-  take(dq_plan(z, a.s.causal));
+  const int kw = take(dq_plan(z, a.s.causal));
   if (!a.dq) a.most = 1, a.length = 1 << 28;  // for delta alone
-  if (a.s.R <= 32)
+  if (kw == 4)
     launch_dq<T, DP, 4>(a, st);
   else
     launch_dq<T, DP, 1>(a, st);
   if (a.dk || a.dv) {
-    take(dkv_plan(z, a.s.causal));
-    attn_dkv_kernel<T, DP>
-        <<<(unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most), kThreads, 0,
-           st>>>(a);
-    if (a.most > 1) {
-      const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.Tk;
-      attn_sum_kernel<T, DP, 0><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
-    }
+    if (take(dkv_plan(z, a.s.causal)) == 4)
+      launch_dkv<T, DP, 4>(a, st);
+    else
+      launch_dkv<T, DP, 1>(a, st);
   }
   return check_launch("nf_attention_bwd");
 }
@@ -530,19 +564,20 @@ extern "C" size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, 
 
 extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
                                 int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
-                                int64_t v_t, int64_t v_h, const void *out, const void *dout,
-                                int64_t g_b, int64_t g_t, int64_t g_h, int64_t B, int64_t Tq,
-                                int64_t Tk, int64_t H, int64_t Hk, int64_t D, int causal,
-                                float scale, int has_mask, int dtype, const void *state,
-                                size_t state_bytes, void *dq, void *dk, void *dv, void *workspace,
-                                size_t workspace_bytes, void *stream) {
+                                int64_t v_t, int64_t v_h, const uint8_t *key_mask, int64_t mask_b,
+                                const void *out, const void *dout, int64_t g_b, int64_t g_t,
+                                int64_t g_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
+                                int64_t Hk, int64_t D, int causal, float scale, int dtype,
+                                const void *state, size_t state_bytes, void *dq, void *dk, void *dv,
+                                void *workspace, size_t workspace_bytes, void *stream) {
   const char *op = "nf_attention_bwd";
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (const int rc = check_sizes(op, z)) return rc;
   if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
   if (B == 0 || Tq == 0 || (!dq && !dk && !dv)) return NF_OK;
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
-  const State parts = state_of(z, has_mask, true);
+  if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
+  const State parts = state_of(z);
   if (state_bytes < parts.total || workspace_bytes < bwd_bytes(z, causal))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
                      state_bytes, parts.total, workspace_bytes, bwd_bytes(z, causal));
@@ -554,11 +589,10 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
   if (const int rc = make_view(op, "dout", dout, g_b, g_t, g_h, z, H / Hk, &a.dout)) return rc;
   const char *st = static_cast<const char *>(state);
-  a.s = make_shape(z, causal, scale,
-                   has_mask ? reinterpret_cast<const uint64_t *>(st + parts.bits) : nullptr);
+  a.s = make_shape(z, causal, scale, key_mask, mask_b);
   a.out = static_cast<const char *>(out);
   a.low = z.es() == 2 ? st + parts.low : nullptr;
-  a.lse = reinterpret_cast<const float *>(st + parts.lse);
+  a.lse = reinterpret_cast<const float *>(st);
   a.ndelta = static_cast<float *>(workspace);
   a.part = a.ndelta + delta_bytes(z) / 4;
   a.dq = static_cast<char *>(dq);

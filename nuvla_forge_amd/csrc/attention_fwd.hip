@@ -81,15 +81,19 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
   for (int n = 0; n < C::NB; ++n) o[0][n] = splat(0.f);
   float m = -kInf, sum = 0.f;  // sum: of the lane's own entries
 
-  const typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
+  typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
+  auto copy = [&](int i, const typename F::Keys::Bits &x, char *lds) {
+    keys.template copy_k<false>(i, x, lds);  // a dropped key's logit is replaced
+    keys.template copy_v<true>(i, x, lds);   // its value is multiplied by 0
+  };
   at = keys.seek(at, cur);
-  if (at < end) keys.copy(at, cur, smem);
+  if (at < end) copy(at, cur, smem);
   auto step = [&](auto edge, int buf) {
     constexpr bool EDGE = decltype(edge)::value;
     const int next = keys.seek(at + 1, nxt);
     gemm::wait_vm_barrier<0>();
-    if (F::STAGES == 2 && next < end) keys.copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
+    if (F::STAGES == 2 && next < end) copy(next, nxt, smem + (buf ^ 1) * 2 * F::TILE);
     const char *kt = smem + buf * 2 * F::TILE, *vt = kt + F::TILE;
     const int kb0 = KW == 4 ? wave : 0;
     floatx16 p[F::NK];
@@ -126,13 +130,19 @@ __global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void a
         p[i][e] = exp2_(fmaf(p[i][e], s.c, -base));
         sum += p[i][e];
       }
-      Packed<T> x[1];
-      x[0].set(p[i]);
-      mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
+      if constexpr (KW == 4) {
+        Twice<T> x;
+        x.set(p[i]);
+        mma_cols<T, DP>(vt, kb0 + i, x, o);
+      } else {
+        Packed<T> x[1];
+        x[0].set(p[i]);
+        mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
+      }
     }
     if (F::STAGES == 1) {
       __syncthreads();
-      if (next < end) keys.copy(next, nxt, smem);
+      if (next < end) copy(next, nxt, smem);
     }
     at = next;
     cur = nxt;
@@ -270,27 +280,15 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
   if (a.lse && l == 0) a.lse[row] = sum == 0.f ? kInf : top + __log2f(sum);
 }
 
-// The mask's bytes [B, Tk] as words of 64 keys: a wavefront a word.
-__global__ __launch_bounds__(kThreads) void attn_bits_kernel(const uint8_t *mask, int64_t mb,
-                                                             int64_t mt, int B, int Tk, int words,
-                                                             uint64_t *bits) {
-  const int64_t i = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (i >= (int64_t)B * words) return;
-  const int64_t b = i / words, key = (i % words) * 64 + (threadIdx.x & 63);
-  const uint64_t w = __ballot(key < Tk && mask[b * mb + key * mt] != 0);
-  if ((threadIdx.x & 63) == 0) bits[i] = w;
-}
-
 struct Plan {
   int kw, tiles, length, most;
 };
 
-// Up to 32 rows a key head: the wavefronts of a block share them.
 Plan plan_of(const Sizes &z, bool causal) {
   Plan p;
   const int64_t R = z.rows(), heads = z.B * z.Hk;
   const bool wide = z.dp() * z.es() > 256;
-  p.kw = R <= 32 ? 4 : 1;
+  p.kw = shared_blocks(z, R) ? 4 : 1;
   p.tiles = (int)((R + (p.kw == 4 ? 31 : 127)) / (p.kw == 4 ? 32 : 128));
   const int tk = p.kw == 4 ? 128 : wide ? 32 : 64;
   const int64_t longest = (z.Tk + tk - 1) / tk;
@@ -319,11 +317,11 @@ template <typename T, int DP>
 int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
   const unsigned grid =
       (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.most);
-  if (p.kw == 4 && a.s.bits)
+  if (p.kw == 4 && a.s.mask)
     attn_fwd_kernel<T, DP, 4, true><<<grid, kThreads, 0, st>>>(a);
   else if (p.kw == 4)
     attn_fwd_kernel<T, DP, 4, false><<<grid, kThreads, 0, st>>>(a);
-  else if (a.s.bits)
+  else if (a.s.mask)
     attn_fwd_kernel<T, DP, 1, true><<<grid, kThreads, 0, st>>>(a);
   else
     attn_fwd_kernel<T, DP, 1, false><<<grid, kThreads, 0, st>>>(a);
@@ -373,7 +371,12 @@ int make_view(const char *op, const char *name, const void *p, int64_t sb, int64
   return NF_OK;
 }
 
-Shape make_shape(const Sizes &z, int causal, float scale, const uint64_t *bits) {
+bool shared_blocks(const Sizes &z, int64_t own) {
+  const double work = (double)(z.B * z.Hk) * (double)z.rows() * (double)z.Tk * z.dp();
+  return own <= 32 || (z.B * z.Hk * ((own + 127) / 128) < 256 && work <= 2147483648.0);
+}
+
+Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b) {
   Shape s;
   s.B = (int)z.B;
   s.Tq = (int)z.Tq;
@@ -387,23 +390,21 @@ Shape make_shape(const Sizes &z, int causal, float scale, const uint64_t *bits) 
   s.nvec = (int)((z.D + ve - 1) / ve);
   s.off = (int)(z.Tk - z.Tq);
   s.causal = causal;
-  s.words = (int)z.words();
   s.ginv = s.G == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + s.G - 1) / s.G);
   // 0 times a barred key's -infinity would be no number: a scale that rounds every logit to 0
   s.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
   s.scale = scale;
   s.flip = scale < 0.f ? (z.es() == 2 ? 0x80008000u : 0x80000000u) : 0u;
-  s.bits = bits;
+  s.mask = mask;
+  s.mask_b = mask_b;
   return s;
 }
 
-State state_of(const Sizes &z, bool mask, bool keep) {
+State state_of(const Sizes &z) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   State t;
-  t.lse = 0;
-  t.bits = keep ? up((size_t)(z.B * z.Hk * z.rows()) * 4) : 0;
-  t.low = t.bits + (mask ? up((size_t)(z.B * z.words()) * 8) : 0);
-  t.total = t.low + (keep && z.es() == 2 ? up((size_t)(z.B * z.Tq * z.H * z.D) * 2) : 0);
+  t.low = up((size_t)(z.B * z.Hk * z.rows()) * 4);
+  t.total = t.low + (z.es() == 2 ? up((size_t)(z.B * z.Tq * z.H * z.D) * 2) : 0);
   return t;
 }
 
@@ -414,9 +415,9 @@ using namespace nf;
 using namespace nf::attn;
 
 extern "C" size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk,
-                                           int64_t D, int has_mask, int keep, int dtype) {
+                                           int64_t D, int dtype) {
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  return check_sizes("nf_attention_state_bytes", z) ? 0 : state_of(z, has_mask, keep).total;
+  return check_sizes("nf_attention_state_bytes", z) ? 0 : state_of(z).total;
 }
 
 extern "C" size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
@@ -429,44 +430,38 @@ extern "C" size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, 
 extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
                                 int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
                                 int64_t v_t, int64_t v_h, const uint8_t *key_mask, int64_t mask_b,
-                                int64_t mask_t, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                int64_t Hk, int64_t D, int causal, float scale, int keep, int dtype,
-                                void *out, void *state, size_t state_bytes, void *workspace,
-                                size_t workspace_bytes, void *stream) {
+                                int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D,
+                                int causal, float scale, int dtype, void *out, void *state,
+                                size_t state_bytes, void *workspace, size_t workspace_bytes,
+                                void *stream) {
   const char *op = "nf_attention_fwd";
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (const int rc = check_sizes(op, z)) return rc;
   if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
   if (B == 0 || Tq == 0) return NF_OK;
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
-  const State parts = state_of(z, key_mask != nullptr, keep);
-  if (state_bytes < parts.total || workspace_bytes < part_bytes(z, causal))
+  if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
+  const State parts = state_of(z);
+  if ((state && state_bytes < parts.total) || workspace_bytes < part_bytes(z, causal))
     return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
                      state_bytes, parts.total, workspace_bytes, part_bytes(z, causal));
-  if (!out || (parts.total && (!state || !aligned16(state))) ||
-      (part_bytes(z, causal) && (!workspace || !aligned16(workspace))))
+  if (!out || !aligned16(state) || (part_bytes(z, causal) && (!workspace || !aligned16(workspace))))
     return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
   FwdArgs a = {};
   if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
   if (const int rc = make_view(op, "k", k, k_b, k_t, k_h, z, 0, &a.k)) return rc;
   if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
   char *st = static_cast<char *>(state);
-  uint64_t *bits = key_mask ? reinterpret_cast<uint64_t *>(st + parts.bits) : nullptr;
-  a.s = make_shape(z, causal, scale, bits);
+  a.s = make_shape(z, causal, scale, key_mask, mask_b);
   a.out = static_cast<char *>(out);
-  a.low = keep && z.es() == 2 ? st + parts.low : nullptr;
-  a.lse = keep ? reinterpret_cast<float *>(st + parts.lse) : nullptr;
+  a.low = st && z.es() == 2 ? st + parts.low : nullptr;
+  a.lse = reinterpret_cast<float *>(st);
   a.part = static_cast<float *>(workspace);
   const Plan p = plan_of(z, causal);
   a.length = p.length;
   a.most = p.most;
   a.tiles = p.tiles;
   hipStream_t hs = static_cast<hipStream_t>(stream);
-  if (key_mask) {
-    const int64_t n = B * z.words();
-    attn_bits_kernel<<<(unsigned)((n + kWaves - 1) / kWaves), kThreads, 0, hs>>>(
-        key_mask, mask_b, mask_t, a.s.B, a.s.Tk, a.s.words, bits);
-  }
 #define NF_ATTN(DT, T)                                                   \
   if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, p, hs) : launch<T, 128>(a, p, hs);
   NF_ATTN(NF_DTYPE_BF16, bf16)

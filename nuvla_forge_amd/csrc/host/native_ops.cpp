@@ -644,35 +644,43 @@ struct Attention : torch::autograd::Function<Attention> {
   static Sizes sizes(const Tensor &q, const Tensor &k) {
     return {q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), q.size(3)};
   }
+  // the mask with its keys side by side
+  static Tensor bytes_of(const Tensor &mask) {
+    if (!mask.defined() || mask.stride(1) == 1 || mask.size(1) == 1) return mask;
+    return mask.contiguous();
+  }
+  static int64_t step_of(const Tensor &mask) {
+    return mask.defined() && mask.size(0) > 1 ? mask.stride(0) : 0;
+  }
   static Tensor run(const Sizes &z, const Heads &q, const Heads &k, const Heads &v,
                     const Tensor &mask, bool causal, double scale, bool keep, Tensor &state) {
     const int dt = code_of(q.t);
     Tensor out = at::empty({z.B, z.Tq, z.H, z.D}, q.t.options().requires_grad(false));
-    const size_t n_state = nf_attention_state_bytes(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, mask.defined(),
-                                                    keep, dt);
+    const size_t n_state =
+        keep ? nf_attention_state_bytes(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, dt) : 0;
     const size_t n_ws = nf_attention_fwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, causal, dt);
     Tensor ws;
     if (n_state) state = bytes(n_state, out);
     if (n_ws) ws = bytes(n_ws, out);
-    const int64_t mb = mask.defined() && z.B > 1 ? mask.stride(0) : 0;
-    const int64_t mt = mask.defined() && z.Tk > 1 ? mask.stride(1) : 0;
     check(nf_attention_fwd(q.t.data_ptr(), q.b, q.s, q.h, k.t.data_ptr(), k.b, k.s, k.h,
-                           v.t.data_ptr(), v.b, v.s, v.h, (const uint8_t *)ptr(mask), mb, mt, z.B,
-                           z.Tq, z.Tk, z.H, z.Hk, z.D, causal, (float)scale, keep, dt,
-                           out.data_ptr(), ptr(state), n_state, ptr(ws), n_ws, stream_of(out)),
+                           v.t.data_ptr(), v.b, v.s, v.h, (const uint8_t *)ptr(mask),
+                           step_of(mask), z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, causal, (float)scale,
+                           dt, out.data_ptr(), ptr(state), n_state, ptr(ws), n_ws, stream_of(out)),
           "nf_attention_fwd");
     return out;
   }
   static Tensor forward(AutogradContext *ctx, const Tensor &q_in, const Tensor &k_in,
-                        const Tensor &v_in, const std::optional<Tensor> &mask, bool causal,
+                        const Tensor &v_in, const std::optional<Tensor> &mask_in, bool causal,
                         double scale) {
     const c10::DeviceGuard guard(q_in.device());
     const Heads q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in);
+    const Tensor mask = bytes_of(mask_in ? *mask_in : Tensor());
     Tensor state;
-    const Tensor out = run(sizes(q_in, k_in), q, k, v, mask ? *mask : Tensor(), causal, scale,
-                           true, state);
-    ctx->save_for_backward({q.t, k.t, v.t, out, state});
-    ctx->saved_data["s"] = std::vector<int64_t>{causal, mask.has_value(), q_in.size(3)};
+    const Tensor out = run(sizes(q_in, k_in), q, k, v, mask, causal, scale, true, state);
+    variable_list kept = {q.t, k.t, v.t, out, state};
+    if (mask.defined()) kept.push_back(mask);
+    ctx->save_for_backward(kept);
+    ctx->saved_data["s"] = std::vector<int64_t>{causal, q_in.size(3)};
     ctx->saved_data["f"] = scale;
     return out;
   }
@@ -681,25 +689,26 @@ struct Attention : torch::autograd::Function<Attention> {
     const variable_list t = ctx->get_saved_variables();
     const auto s = ctx->saved_data["s"].toIntVector();
     const Tensor &out = t[3], &state = t[4];
+    const Tensor mask = t.size() > 5 ? bytes_of(t[5]) : Tensor();
     const c10::DeviceGuard guard(out.device());
     TORCH_CHECK_VALUE(grads[0].device() == out.device(),
                       "fused_attention backward: dout is not on the forward's device");
     const Heads q(t[0]), k(t[1]), v(t[2]), g = head_rows(grads[0].to(out.scalar_type()));
     Sizes z = sizes(q.t, k.t);
-    z.D = s[2];
+    z.D = s[1];
+    const int causal = (int)s[0], dt = code_of(out);
     const auto opts = out.options().requires_grad(false);
     if (ctx->needs_input_grad(0)) res[0] = at::empty({z.B, z.Tq, z.H, z.D}, opts);
     for (int i : {1, 2})
       if (ctx->needs_input_grad(i)) res[i] = at::empty({z.B, z.Tk, z.Hk, z.D}, opts);
-    const int dt = code_of(out);
-    const size_t n_ws = nf_attention_bwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, (int)s[0], dt);
+    const size_t n_ws = nf_attention_bwd_workspace(z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, causal, dt);
     Tensor ws = bytes(n_ws, out);
     check(nf_attention_bwd(q.t.data_ptr(), q.b, q.s, q.h, k.t.data_ptr(), k.b, k.s, k.h,
-                           v.t.data_ptr(), v.b, v.s, v.h, out.data_ptr(), g.t.data_ptr(), g.b, g.s,
-                           g.h, z.B, z.Tq, z.Tk, z.H, z.Hk, z.D, (int)s[0],
-                           (float)ctx->saved_data["f"].toDouble(), (int)s[1], dt, state.data_ptr(),
-                           (size_t)state.numel(), ptr(res[0]), ptr(res[1]), ptr(res[2]),
-                           ws.data_ptr(), n_ws, stream_of(out)),
+                           v.t.data_ptr(), v.b, v.s, v.h, (const uint8_t *)ptr(mask),
+                           step_of(mask), out.data_ptr(), g.t.data_ptr(), g.b, g.s, g.h, z.B, z.Tq,
+                           z.Tk, z.H, z.Hk, z.D, causal, (float)ctx->saved_data["f"].toDouble(),
+                           dt, state.data_ptr(), (size_t)state.numel(), ptr(res[0]), ptr(res[1]),
+                           ptr(res[2]), ws.data_ptr(), n_ws, stream_of(out)),
           "nf_attention_bwd");
     return first_order_only("fused_attention", at::GradMode::is_enabled(), grads, std::move(res));
   }
@@ -1046,7 +1055,7 @@ PyObject *py_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const at::NoGradGuard no_grad;
     Tensor state;
     return Attention::run(Attention::sizes(t[0], t[1]), head_rows(t[0]), head_rows(t[1]),
-                          head_rows(t[2]), mask, causal, scale, false, state);
+                          head_rows(t[2]), Attention::bytes_of(mask), causal, scale, false, state);
   }));
   END_HANDLE_TH_ERRORS
 }

@@ -40,57 +40,64 @@ def _strides(t: torch.Tensor) -> list[int]:
     return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
+def _mask(key_mask):
+    """``key_mask`` with its keys side by side, and the bytes from sample to sample."""
+    if key_mask is None:
+        return None, 0
+    m = key_mask if key_mask.stride(1) == 1 or key_mask.shape[1] == 1 else key_mask.contiguous()
+    return m, 0 if m.shape[0] == 1 else m.stride(0)
+
+
 class _FusedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, causal, scale, keep):
         b, tq, h, d = q.shape
         tk, hk = k.shape[1:3]
         q2, k2, v2 = (_vector_rows(t) for t in (q, k, v))
+        mask, mask_b = _mask(key_mask)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dt, L = _lib.dtype_code(q), _lib.lib()
         sizes = (b, tq, tk, h, hk, d)
-        n_state = L.nf_attention_state_bytes(*sizes, key_mask is not None, keep, dt)
+        n_state = L.nf_attention_state_bytes(*sizes, dt) if keep else 0
         n_ws = L.nf_attention_fwd_workspace(*sizes, causal, dt)
-        state = torch.empty(max(n_state, 1), dtype=torch.uint8, device=q.device)
-        ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=q.device)
-        mask_strides = (0, 0)
-        if key_mask is not None:
-            mask_strides = [0 if n == 1 else s for n, s in zip(key_mask.shape, key_mask.stride())]
+        state, ws = (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+                     for n in (n_state, n_ws))
         with device_of(q):
             _lib.check(
                 L.nf_attention_fwd(q2.data_ptr(), *_strides(q2), k2.data_ptr(), *_strides(k2),
-                                   v2.data_ptr(), *_strides(v2), _lib.ptr(key_mask),
-                                   *mask_strides, *sizes, causal, scale, keep, dt, out.data_ptr(),
-                                   state.data_ptr(), n_state, ws.data_ptr(), n_ws,
-                                   _lib.stream_of(q)),
+                                   v2.data_ptr(), *_strides(v2), _lib.ptr(mask), mask_b, *sizes,
+                                   causal, scale, dt, out.data_ptr(), _lib.ptr(state), n_state,
+                                   _lib.ptr(ws), n_ws, _lib.stream_of(q)),
                 "nf_attention_fwd",
             )
         if keep:
-            ctx.save_for_backward(q2, k2, v2, out, state)
-            ctx.call = (sizes, causal, scale, key_mask is not None, n_state)
+            ctx.save_for_backward(q2, k2, v2, out, state, mask)
+            ctx.call = (sizes, causal, scale)
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, out, state = ctx.saved_tensors
-        sizes, causal, scale, masked, n_state = ctx.call
+        q, k, v, out, state, key_mask = ctx.saved_tensors
+        sizes, causal, scale = ctx.call
         b, tq, tk, h, hk, d = sizes
         check_devices("fused_attention backward", "the forward's q", dict(dout=grad),
                       device=q.device)
         g = _vector_rows(grad.to(q.dtype))
+        mask, mask_b = _mask(key_mask)
         dq, dk, dv = (torch.empty(shape, dtype=q.dtype, device=q.device) if need else None
                       for shape, need in zip(((b, tq, h, d), (b, tk, hk, d), (b, tk, hk, d)),
                                              ctx.needs_input_grad))
         dt, L = _lib.dtype_code(q), _lib.lib()
         n_ws = L.nf_attention_bwd_workspace(*sizes, causal, dt)
-        ws = torch.empty(max(n_ws, 1), dtype=torch.uint8, device=q.device)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device)
         with device_of(q):
             _lib.check(
                 L.nf_attention_bwd(q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k),
-                                   v.data_ptr(), *_strides(v), out.data_ptr(), g.data_ptr(),
-                                   *_strides(g), *sizes, causal, scale, masked, dt,
-                                   state.data_ptr(), n_state, _lib.ptr(dq), _lib.ptr(dk),
-                                   _lib.ptr(dv), ws.data_ptr(), n_ws, _lib.stream_of(q)),
+                                   v.data_ptr(), *_strides(v), _lib.ptr(mask), mask_b,
+                                   out.data_ptr(), g.data_ptr(), *_strides(g), *sizes, causal,
+                                   scale, dt, state.data_ptr(), state.numel(), _lib.ptr(dq),
+                                   _lib.ptr(dk), _lib.ptr(dv), ws.data_ptr(), n_ws,
+                                   _lib.stream_of(q)),
                 "nf_attention_bwd",
             )
         return first_order_only("fused_attention", (grad,), (dq, dk, dv, None, None, None, None))

@@ -147,24 +147,25 @@ def test_attention_refusals():
 
 def _fwd(**over):
     a = dict(q=FAKE, qs=(64, 64, 16), k=FAKE, ks=(64, 64, 16), v=FAKE, vs=(64, 64, 16), mask=None,
-             ms=(0, 0), B=1, Tq=2, Tk=2, H=4, Hk=4, D=16, causal=0, scale=0.25, keep=1, dtype=1,
+             mb=0, B=1, Tq=2, Tk=2, H=4, Hk=4, D=16, causal=0, scale=0.25, dtype=1,
              out=FAKE, state=FAKE, state_bytes=1 << 20, ws=FAKE, ws_bytes=1 << 20)
     a.update(over)
     return _lib.lib().nf_attention_fwd(
-        a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["mask"], *a["ms"], a["B"], a["Tq"],
-        a["Tk"], a["H"], a["Hk"], a["D"], a["causal"], a["scale"], a["keep"], a["dtype"], a["out"],
+        a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["mask"], a["mb"], a["B"], a["Tq"],
+        a["Tk"], a["H"], a["Hk"], a["D"], a["causal"], a["scale"], a["dtype"], a["out"],
         a["state"], a["state_bytes"], a["ws"], a["ws_bytes"], None)
 
 
 def _bwd(**over):
-    a = dict(q=FAKE, qs=(64, 64, 16), k=FAKE, ks=(64, 64, 16), v=FAKE, vs=(64, 64, 16), out=FAKE,
-             g=FAKE, gs=(64, 64, 16), B=1, Tq=2, Tk=2, H=4, Hk=4, D=16, causal=0, scale=0.25,
-             masked=0, dtype=1, state=FAKE, state_bytes=1 << 20, dq=FAKE, dk=FAKE, dv=FAKE,
+    a = dict(q=FAKE, qs=(64, 64, 16), k=FAKE, ks=(64, 64, 16), v=FAKE, vs=(64, 64, 16), mask=None,
+             mb=0, out=FAKE, g=FAKE, gs=(64, 64, 16), B=1, Tq=2, Tk=2, H=4, Hk=4, D=16, causal=0,
+             scale=0.25, dtype=1, state=FAKE, state_bytes=1 << 20, dq=FAKE, dk=FAKE, dv=FAKE,
              ws=FAKE, ws_bytes=1 << 20)
     a.update(over)
     return _lib.lib().nf_attention_bwd(
-        a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["out"], a["g"], *a["gs"], a["B"],
-        a["Tq"], a["Tk"], a["H"], a["Hk"], a["D"], a["causal"], a["scale"], a["masked"], a["dtype"],
+        a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["mask"], a["mb"], a["out"],
+        a["g"], *a["gs"], a["B"], a["Tq"], a["Tk"], a["H"], a["Hk"], a["D"], a["causal"], a["scale"],
+        a["dtype"],
         a["state"], a["state_bytes"], a["dq"], a["dk"], a["dv"], a["ws"], a["ws_bytes"], None)
 
 
@@ -177,7 +178,7 @@ def test_attention_c_abi_refusals(call):
                  dict(q=None), dict(k=None), dict(v=None), dict(q=FAKE + 2), dict(qs=(64, 60, 16)),
                  dict(ks=(64, 64, 12)), dict(vs=(4, 64, 16)), dict(ks=(64, -64, 16)),
                  dict(qs=(64, 1 << 22, 16)), dict(Hk=1, qs=(64, 64, 1 << 28)), dict(out=None),
-                 dict(state=None), dict(state=FAKE + 8)):
+                 dict(state=FAKE + 8), dict(mask=FAKE, mb=-1)):
         assert call(**over) == NF_ERR_ARG, over
         assert "nf_attention" in _err()
     for over in (dict(state_bytes=0), dict(state_bytes=256)):
@@ -197,15 +198,12 @@ def test_attention_c_abi_workspaces():
     assert _bwd(ws_bytes=16) == NF_ERR_WORKSPACE and _bwd(ws=None) == NF_ERR_ARG
     assert _bwd(g=None) == NF_ERR_ARG and _bwd(gs=(64, 64, 2)) == NF_ERR_ARG
     assert _bwd(dq=None, dk=None, dv=None) == NF_OK
-    # no mask and no backward to come: no state
-    assert L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 0, 0, 1) == 0
-    masked = L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 1, 0, 1)
-    kept = L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 0, 1, 1)
-    assert masked >= 2 * 8 and kept >= 2 * 3 * 4 * (4 + 16 * 2)
-    assert L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 1, 1, 1) >= masked + kept
-    assert L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 0, 1, 0) < kept  # fp32: nothing left over
+    kept = L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 1)
+    assert kept >= 2 * 3 * 4 * (4 + 16 * 2)
+    assert L.nf_attention_state_bytes(2, 3, 4, 4, 2, 16, 0) < kept  # fp32: nothing left over
+    assert _bwd(state=None) == NF_ERR_ARG
     for bad in ((2, 3, 4, 4, 3, 16), (2, 3, 4, 4, 2, 200), (-2, 3, 4, 4, 2, 16)):
-        assert L.nf_attention_state_bytes(*bad, 0, 1, 1) == 0
+        assert L.nf_attention_state_bytes(*bad, 1) == 0
         assert L.nf_attention_fwd_workspace(*bad, 0, 1) == 0
         assert L.nf_attention_bwd_workspace(*bad, 0, 1) == 0
 

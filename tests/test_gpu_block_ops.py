@@ -398,16 +398,16 @@ def test_attention_buffers_of_exactly_the_size_asked_for(cuda, b, tq, tk, h, hk,
         return torch.full((n + 4096,), 171, dtype=torch.uint8, device=cuda), n
 
     state, fw, bw = (room(n) for n in (
-        L.nf_attention_state_bytes(*sizes, masked, 1, dt), L.nf_attention_fwd_workspace(*sizes, 1, dt),
+        L.nf_attention_state_bytes(*sizes, dt), L.nf_attention_fwd_workspace(*sizes, 1, dt),
         L.nf_attention_bwd_workspace(*sizes, 1, dt)))
     outs = [room(t.numel() * t.element_size()) for t in (q, q, k, v)]
     at = [(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)) for t in (q, k, v, do)]
-    ms = (0, 0) if m is None else m.stride()
+    mask = (_lib.ptr(m), 0 if m is None else m.stride(0))
     _lib.check(L.nf_attention_fwd(
-        *at[0], *at[1], *at[2], _lib.ptr(m), *ms, *sizes, 1, d ** -0.5, 1, dt, outs[0][0].data_ptr(),
+        *at[0], *at[1], *at[2], *mask, *sizes, 1, d ** -0.5, dt, outs[0][0].data_ptr(),
         state[0].data_ptr(), state[1], fw[0].data_ptr(), fw[1], st), "fwd")
     _lib.check(L.nf_attention_bwd(
-        *at[0], *at[1], *at[2], outs[0][0].data_ptr(), *at[3], *sizes, 1, d ** -0.5, masked, dt,
+        *at[0], *at[1], *at[2], *mask, outs[0][0].data_ptr(), *at[3], *sizes, 1, d ** -0.5, dt,
         state[0].data_ptr(), state[1], *(o[0].data_ptr() for o in outs[1:]), bw[0].data_ptr(), bw[1],
         st), "bwd")
     for x, n in (state, fw, bw, *outs):
@@ -666,7 +666,7 @@ def test_block_ops_saved_tensors_go_through_the_hooks(cuda, route, name):
 
     with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v.to(cuda)):
         hooked = _all(op, args)
-    assert len(packed) == (1 if name == "rotary" else 5)
+    assert len(packed) == {"attention": 6, "few": 5, "rotary": 1}[name]
     assert all(torch.equal(a, b) for a, b in zip(plain, hooked, strict=True))
 
 

@@ -435,7 +435,7 @@ __host__ __device__ __forceinline__ int first_row_tile(const Shape &s, int tile,
 
 // The part length for `tiles` blocks a head of up to `longest` tiles each, `slots` blocks at once on
 // the chip.  Blocks of one length go in rounds: as many parts as take the least time, in tiles a
-// block 1.5 beside its own, the join 3 and 1.2 for each part that a slot writes and reads.  A causal
+// block 1.5 beside its own, the join 4 and 1.2 for each part that a slot writes and reads.  A causal
 // call's blocks fall from the longest to few and fill up what it leaves: two parts a slot (dK and dV
 // of 2 x 4096 tokens, 4 key heads of 128: 585 us whole, 365 so, in 3 parts a slot 400, in 8 450).
 inline int part_length(int64_t heads, int64_t tiles, int64_t longest, bool causal, int slots) {
@@ -451,7 +451,7 @@ inline int part_length(int64_t heads, int64_t tiles, int64_t longest, bool causa
   for (int n = 1; n <= kMostParts && n <= longest; ++n) {
     const int64_t c = (longest + n - 1) / n, rounds = (blocks * n + slots - 1) / slots;
     const double t = (double)rounds * ((double)c + 1.5) +
-                     (n > 1 ? 3. + 1.2 * n * (double)blocks / slots : 0.);
+                     (n > 1 ? 4. + 1.2 * n * (double)blocks / slots : 0.);
     if (n > 1 && t >= time) continue;
     time = t;
     best = n == 1 ? 1 << 28 : (int)c;

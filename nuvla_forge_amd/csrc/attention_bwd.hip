@@ -78,13 +78,13 @@ struct Dq {
   static constexpr int NK = KW == 4 ? 1 : TK / 32;
   using Keys = KeyTiles<T, DP, TK, MASKED>;
   static constexpr int TILE = Keys::TILE;
-  static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int STAGES = KW == 1 && 4 * TILE <= 128 * 1024 ? 2 : 1;
   static constexpr int END = kWaves * Turned<DP>::BYTES;
   static constexpr int LDS = STAGES * 2 * TILE > END ? STAGES * 2 * TILE : END;
 };
 
 template <typename T, int DP, int KW, bool MASKED>
-__global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP == 64) ? 2 : 1) void attn_dq_kernel(
     BwdArgs a) {
   using F = Dq<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
@@ -229,13 +229,15 @@ struct Dkv {
   static constexpr int NR = KW == 4 ? 1 : TR / 32;                   // of those, 32s of a wavefront
   static constexpr int TILE = TR * C::ROW;
   static constexpr int STAGE = 2 * TILE + 2 * 4 * (TR < 64 ? 64 : TR);  // q, dout, lse, -delta
-  static constexpr int STAGES = 2 * STAGE <= 140 * 1024 ? 2 : 1;
+  static constexpr bool TWO = KW == 4 && DP == 64 && sizeof(T) == 2;  // blocks on a CU
+  static constexpr int STAGES = !TWO && 2 * STAGE <= 140 * 1024 ? 2 : 1;
   static constexpr int LDS = STAGES * STAGE;
   static_assert(LDS >= kWaves * Turned<DP>::BYTES, "the results turn in the tiles' place");
 };
 
 template <typename T, int DP, int KW>
-__global__ __launch_bounds__(kThreads, 1) void attn_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_dkv_kernel(
+    BwdArgs a) {
   using F = Dkv<T, DP, KW>;
   using C = Tile<T, DP>;
   __shared__ __attribute__((aligned(16))) char smem[F::LDS];
@@ -474,7 +476,7 @@ Plan dq_plan(const Sizes &z, bool causal) {
   Plan p;
   p.kw = shared ? 4 : 1;
   p.tiles = (int)((z.rows() + br - 1) / br);
-  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 256 ? 512 : 256);
   p.most = parts_of((int)longest, p.length);
   p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.rows()) * (size_t)z.dp() * 4 : 0;
   return p;
@@ -487,7 +489,7 @@ Plan dkv_plan(const Sizes &z, bool causal) {
   Plan p;
   p.kw = shared ? 4 : 1;
   p.tiles = (int)((z.Tk + bk - 1) / bk);
-  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() == 128 ? 512 : 256);
   p.most = parts_of((int)longest, p.length);
   p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.Tk) * (size_t)z.dp() * 8 : 0;
   return p;

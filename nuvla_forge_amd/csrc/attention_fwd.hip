@@ -40,13 +40,13 @@ struct Fwd {
   static constexpr int NK = KW == 4 ? 1 : TK / 32;                     // of those, 32s of a wavefront
   using Keys = KeyTiles<T, DP, TK, MASKED>;
   static constexpr int TILE = Keys::TILE;
-  static constexpr int STAGES = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int STAGES = KW == 1 && 4 * TILE <= 128 * 1024 ? 2 : 1;
   static constexpr int END = kWaves * Turned<DP>::BYTES + (KW == 4 ? 1024 : 0);
   static constexpr int LDS = STAGES * 2 * TILE > END ? STAGES * 2 * TILE : END;
 };
 
 template <typename T, int DP, int KW, bool MASKED>
-__global__ __launch_bounds__(kThreads, KW == 1 && sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP == 64) ? 2 : 1) void attn_fwd_kernel(
     FwdArgs a) {
   using F = Fwd<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
@@ -292,7 +292,7 @@ Plan plan_of(const Sizes &z, bool causal) {
   p.tiles = (int)((R + (p.kw == 4 ? 31 : 127)) / (p.kw == 4 ? 32 : 128));
   const int tk = p.kw == 4 ? 128 : wide ? 32 : 64;
   const int64_t longest = (z.Tk + tk - 1) / tk;
-  p.length = part_length(heads, p.tiles, longest, causal, 256);
+  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 256 ? 512 : 256);
   p.most = parts_of((int)longest, p.length);
   return p;
 }

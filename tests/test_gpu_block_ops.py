@@ -98,6 +98,33 @@ def test_attention_lengths_at_tile_borders(cuda, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("mask", [None, "lengths", "random"])
+@pytest.mark.parametrize("b, tq, tk, h, hk, d", [
+    (64, 33, 33, 4, 4, 64), (64, 70, 129, 4, 4, 128), (64, 129, 64, 4, 4, 40),
+    (37, 65, 191, 21, 7, 72), (3, 300, 200, 86, 86, 64)])
+def test_attention_over_many_heads(cuda, b, tq, tk, h, hk, d, mask, causal, dtype):
+    """Blocks enough for every CU: each wavefront has rows, or keys, of its own."""
+    note(f"attention many heads {b} {tq} {tk} {h} {hk} {d} {mask} {causal} {dtype}")
+    _check(*_qkv(b, tq, tk, h, hk, d, dtype, cuda), causal=causal,
+           key_mask=_mask(mask, b, tk, cuda))
+
+
+@pytest.mark.parametrize("dtype, b, tq, tk, h, hk, d", [
+    (BF16, 1, 4100, 4100, 4, 2, 128), (BF16, 1, 200, 30000, 8, 4, 128), (F16, 1, 30000, 200, 8, 4, 64),
+    (F16, 2, 1700, 3300, 6, 3, 128), (F32, 1, 2100, 2100, 8, 4, 128), (F32, 1, 5000, 700, 16, 8, 96),
+    (BF16, 1, 3000, 3100, 12, 12, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("mask", [None, "holes"])
+def test_attention_long_axes_in_parts(cuda, dtype, b, tq, tk, h, hk, d, mask, causal):
+    """Few heads over long sequences: the keys of a row, the rows of a key, in parts that are
+    joined."""
+    note(f"attention parts {b} {tq} {tk} {h} {hk} {d} {mask} {causal} {dtype}")
+    _check(*_qkv(b, tq, tk, h, hk, d, dtype, cuda), causal=causal,
+           key_mask=_mask(mask, b, tk, cuda))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("d", [1, 2, 7, 8, 31, 37, 40, 63, 64, 65, 72, 96, 100, 127, 128])
 def test_attention_head_widths(cuda, d, dtype):
     note(f"attention width {d} {dtype}")
@@ -239,6 +266,7 @@ def test_attention_strided_operands(cuda, route):
         (q.transpose(1, 3).contiguous().transpose(1, 3), k, v, do, m),
         (q, k, v, do, m.t().contiguous().t()),
         (q, k, v, do, m[:1].expand(b, t)),
+        (q, k, v, do, torch.cat([m, m], 1)[:, 3:3 + t]),
         (q[:, ::2], k[:, ::2], v[:, 1::2], do[:, 1::2], m[:, ::2]),
         (q.flatten()[1:1 + 70 * 64].view(1, 70, 1, 64), *(x.flatten()[3:3 + 70 * 64].view(
             1, 70, 1, 64) for x in (k, v, do)), m[:1]),
@@ -342,9 +370,20 @@ def test_attention_in_a_graph(cuda, b, tq, tk, h, hk, d, mask):
         assert all(torch.equal(out, want) for _, out, want, _ in graphs)
 
 
+def test_attention_mask_that_changed_before_the_backward_raises(cuda, route):
+    note(f"attention changed mask {route}")
+    q, k, v, do = _qkv(2, 9, 70, 4, 2, 64, BF16, cuda)
+    m = _mask("random", 2, 70, cuda)
+    x = q.detach().requires_grad_(True)
+    out = fused_attention(x, k, v, key_mask=m)
+    m[0, 0] = ~m[0, 0]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, x, do)
+
+
 def test_attention_same_bits_every_run(cuda):
     note("attention determinism")
-    for shape in ((2, 300, 300, 8, 2, 128), (1, 2, 9000, 4, 1, 64)):
+    for shape in ((2, 300, 300, 8, 2, 128), (1, 2, 9000, 4, 1, 64), (1, 2000, 2000, 8, 4, 128)):
         args = _qkv(*shape, BF16, cuda)
         want = _run(*args, causal=True)
         for _ in range(4):
@@ -382,7 +421,8 @@ def test_block_ops_from_two_threads_on_two_streams(cuda):
 @pytest.mark.parametrize("b, tq, tk, h, hk, d, dtype, masked", [
     (2, 100, 130, 4, 2, 64, BF16, True), (1, 1, 5000, 8, 2, 128, BF16, False),
     (3, 33, 65, 3, 1, 40, F16, True), (1, 65, 65, 2, 2, 128, F32, True),
-    (2, 5, 9001, 2, 1, 64, F32, False)])
+    (2, 5, 9001, 2, 1, 64, F32, False), (1, 4100, 4100, 2, 1, 128, BF16, True),
+    (64, 40, 70, 4, 4, 64, BF16, True), (1, 300, 3000, 2, 2, 104, F16, False)])
 def test_attention_buffers_of_exactly_the_size_asked_for(cuda, b, tq, tk, h, hk, d, dtype, masked):
     """The C entries with a state and workspaces of the bytes that the size calls name, outputs
     with room behind them: what lies behind stays as it was, and the results are the public

@@ -88,7 +88,7 @@ inline int64_t place_grid(int64_t heads, int64_t tiles) {
 template <typename T, int DP>
 struct Tile {
   static constexpr int ROW = DP * (int)sizeof(T);  // bytes
-  static constexpr int NV = ROW / 16;              // vectors of a row: 8, 16 or 32
+  static constexpr int NV = ROW / 16;              // vectors of a row: 8, 12, 16 or 32
   static constexpr int KS = ROW / 32;              // steps of a product over a row
   static constexpr int NB = DP / 32;               // 32-wide column blocks
   static constexpr int VE = 16 / (int)sizeof(T);
@@ -97,6 +97,8 @@ struct Tile {
   __device__ __forceinline__ static int swz(int row) {
     if constexpr (NV == 8)  // two rows to a bank cycle
       return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    else if constexpr (NV == 12)  // rows lie 3/4 of a bank cycle apart
+      return (row >> 2) & 3;
     else
       return (row & 3) << 2 | ((row >> 2) & 3);
   }
@@ -107,21 +109,29 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char *p) {
 }
 
 // The byte offsets at which a lane's copies of a tile of ROWS rows read, and the copies themselves:
-// 1 KB of the tile each, 64 / NV rows.
+// 1 KB of the tile each.
 template <typename T, int DP, int ROWS>
 struct TileCopy {
   using C = Tile<T, DP>;
   static constexpr int CW = ROWS * C::NV / kThreads;
   static_assert(CW >= 1 && ROWS * C::NV % kThreads == 0, "a tile is whole 1 KB copies a wavefront");
   uint32_t off[CW];
+  // the lane's row in copy c
+  __device__ __forceinline__ static int row_of(int wave, int c) {
+    const int l = threadIdx.x & 63;
+    if constexpr (64 % C::NV == 0)
+      return (wave * CW + c) * (64 / C::NV) + l / C::NV;
+    else
+      return ((wave * CW + c) * 64 + l) / C::NV;
+  }
   // `at(row, &in)`: a row's byte offset and whether it exists
   template <class F>
   __device__ __forceinline__ void set(int nvec, int wave, F &&at) {
     const int l = threadIdx.x & 63;
 #pragma unroll
     for (int c = 0; c < CW; ++c) {
-      const int row = (wave * CW + c) * (64 / C::NV) + l / C::NV;
-      const int vec = (l % C::NV) ^ C::swz(row);
+      const int row = row_of(wave, c);
+      const int vec = ((wave * CW + c) * 64 + l - row * C::NV) ^ C::swz(row);
       bool in = true;
       const uint32_t o = at(row, &in) + (uint32_t)vec * 16u;
       off[c] = in && vec < nvec ? o : kOob;
@@ -538,20 +548,34 @@ struct KeyTiles {
     const char *at = p + (int64_t)i * TK * step;
     if (left >= TK && (!(MASKED && ZERO) || x.all())) return whole.issue(at, lds, wave);
     Copy c = whole;
-    constexpr int PER = 64 / Tile<T, DP>::NV, ROWS = Copy::CW * PER;  // rows of a copy, a wavefront
-    static_assert(ROWS <= 32, "a wavefront's rows are in one half of a word");
-    const int l = threadIdx.x & 63, row0 = wave * ROWS + l / Tile<T, DP>::NV;
-    uint32_t live = ~0u;
-    if constexpr (MASKED && ZERO) {
-      uint64_t w = x.w[0];
-      if constexpr (N == 2) w = wave >= kWaves / 2 ? x.w[1] : x.w[0];
-      live = (uint32_t)(w >> (row0 & 63));
-    }
-    const int rows = left - row0;  // from the lane's first on
-    if (rows < 32) live &= rows > 0 ? (1u << rows) - 1u : 0u;
+    if constexpr (64 % Tile<T, DP>::NV == 0) {
+      constexpr int PER = 64 / Tile<T, DP>::NV, ROWS = Copy::CW * PER;  // rows of a copy, a wavefront
+      static_assert(ROWS <= 32, "a wavefront's rows are in one half of a word");
+      const int row0 = Copy::row_of(wave, 0);
+      uint32_t live = ~0u;
+      if constexpr (MASKED && ZERO) {
+        uint64_t w = x.w[0];
+        if constexpr (N == 2) w = wave >= kWaves / 2 ? x.w[1] : x.w[0];
+        live = (uint32_t)(w >> (row0 & 63));
+      }
+      const int rows = left - row0;  // from the lane's first on
+      if (rows < 32) live &= rows > 0 ? (1u << rows) - 1u : 0u;
 #pragma unroll
-    for (int j = 0; j < Copy::CW; ++j)
-      if (!(live & (1u << (j * PER)))) c.off[j] = kOob;
+      for (int j = 0; j < Copy::CW; ++j)
+        if (!(live & (1u << (j * PER)))) c.off[j] = kOob;
+    } else {
+#pragma unroll
+      for (int j = 0; j < Copy::CW; ++j) {
+        const int row = Copy::row_of(wave, j);
+        bool in = row < left;
+        if constexpr (MASKED && ZERO) {
+          uint64_t w = x.w[0];
+          if constexpr (N == 2) w = row >= 64 ? x.w[1] : x.w[0];
+          in = in && (w >> (row & 63) & 1);
+        }
+        if (!in) c.off[j] = kOob;
+      }
+    }
     c.issue(at, lds, wave);
   }
   template <bool ZERO>
@@ -609,7 +633,7 @@ struct Turned {
   static constexpr int BYTES = 32 * DP * 4;
   static constexpr int V = DP / 4;  // vectors of a row
   __device__ __forceinline__ static int at(int row, int v) {
-    return row * DP * 4 + ((v ^ (row & (V - 1) & 31)) << 4);
+    return row * DP * 4 + ((v ^ (row & (V % 16 == 0 ? V - 1 : 7) & 31)) << 4);
   }
   __device__ __forceinline__ static void put(char *lds, const floatx16 (&acc)[DP / 32], float f) {
     const int row = threadIdx.x & 31;
@@ -678,7 +702,8 @@ struct Sizes {  // what a call is about, as its entry points take it
   int dtype;
   int es() const { return dtype == NF_DTYPE_F32 ? 4 : 2; }
   int64_t rows() const { return Tq * (H / Hk); }
-  int dp() const { return D <= 64 ? 64 : 128; }
+  // columns of a tile; fp32 rows of 96 would not swizzle
+  int dp() const { return D <= 64 ? 64 : D <= 96 && dtype != NF_DTYPE_F32 ? 96 : 128; }
 };
 // NF_OK, or the error that is set
 int check_sizes(const char *op, const Sizes &z);

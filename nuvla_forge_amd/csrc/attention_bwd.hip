@@ -442,17 +442,19 @@ __global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
   }
   const int n = parts_of(len, a.length);
   if (n == 1) return;  // the row is written
-  float x[W / 64] = {};
+  constexpr int NJ = (W + 63) / 64;
+  float x[NJ] = {};
   const float *p = a.part + row * W + l;
 #pragma unroll 4
   for (int i = 0; i < n; ++i)
 #pragma unroll
-    for (int j = 0; j < W / 64; ++j) x[j] += p[(int64_t)i * rows * W + 64 * j];
+    for (int j = 0; j < NJ; ++j)
+      if (l + 64 * j < W) x[j] += p[(int64_t)i * rows * W + 64 * j];
   const int64_t b = bh / s.Hk, hk = bh % s.Hk;
 #pragma unroll
-  for (int j = 0; j < W / 64; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     const int c = l + 64 * j, d = c % DP;
-    if (d >= s.D) continue;
+    if (c >= W || d >= s.D) continue;
     if constexpr (!KEYS) {
       const int64_t t = r / s.G, g = r % s.G;
       reinterpret_cast<T *>(a.dq)[((b * s.Tq + t) * s.H + hk * s.G + g) * s.D + d] =
@@ -601,11 +603,16 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   a.dk = static_cast<char *>(dk);
   a.dv = static_cast<char *>(dv);
   hipStream_t hs = static_cast<hipStream_t>(stream);
-#define NF_ATTN(DT, T) \
-  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, z, hs) : launch<T, 128>(a, z, hs);
-  NF_ATTN(NF_DTYPE_BF16, bf16)
-  NF_ATTN(NF_DTYPE_F16, f16)
-  NF_ATTN(NF_DTYPE_F32, float)
+#define NF_ATTN(DT, T, DP) \
+  if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, z, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16, 64)
+  NF_ATTN(NF_DTYPE_BF16, bf16, 96)
+  NF_ATTN(NF_DTYPE_BF16, bf16, 128)
+  NF_ATTN(NF_DTYPE_F16, f16, 64)
+  NF_ATTN(NF_DTYPE_F16, f16, 96)
+  NF_ATTN(NF_DTYPE_F16, f16, 128)
+  NF_ATTN(NF_DTYPE_F32, float, 64)
+  NF_ATTN(NF_DTYPE_F32, float, 128)
 #undef NF_ATTN
   return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
 }

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP == 64) ?
 template <typename T, int DP, int KW, int W>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
   using F = Fwd<T, DP, KW, false>;
-  __shared__ float sums[kWaves][DP];
+  __shared__ float sums[kWaves][(DP + 63) / 64 * 64];
   const Shape &s = a.s;
   const int64_t rows = (int64_t)s.B * s.Hk * s.R;
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
@@ -241,12 +241,14 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
     if (l + 64 * j < n) sum += ml[(l + 64 * j) * rows * 2 + 1] * m[j];
   }
   sum = wave_sum(sum);
-  float o[DP / 64] = {};
+  constexpr int NJ = (DP + 63) / 64;
+  float o[NJ] = {};
   auto add = [&](int i) {
     const float f = __shfl(i < 64 ? m[0] : m[1], i & 63);
     const float *p = a.part + (i * rows + row) * DP;
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) o[j] = fmaf(p[l + 64 * j], f, o[j]);
+    for (int j = 0; j < NJ; ++j)
+      if (l + 64 * j < DP) o[j] = fmaf(p[l + 64 * j], f, o[j]);
   };
   int i = wave % W;
   for (; i + 3 * W < n; i += 4 * W) {
@@ -258,11 +260,11 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
   for (; i < n; i += W) add(i);
   if constexpr (W > 1) {
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) sums[wave][l + 64 * j] = o[j];
+    for (int j = 0; j < NJ; ++j) sums[wave][l + 64 * j] = o[j];
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j)
+    for (int j = 0; j < NJ; ++j)
       o[j] = ((sums[0][l + 64 * j] + sums[1][l + 64 * j]) + sums[2][l + 64 * j]) +
              sums[3][l + 64 * j];
   }
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
   const int64_t b = bh / s.Hk, hk = bh % s.Hk, t = r / s.G, g = r % s.G;
   const int64_t to = ((b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
 #pragma unroll
-  for (int j = 0; j < DP / 64; ++j) {
+  for (int j = 0; j < NJ; ++j) {
     const int d = l + 64 * j;
     if (d >= s.D) continue;
     const float x = o[j] * inv;
@@ -462,11 +464,16 @@ extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   a.most = p.most;
   a.tiles = p.tiles;
   hipStream_t hs = static_cast<hipStream_t>(stream);
-#define NF_ATTN(DT, T)                                                   \
-  if (dtype == DT) return z.dp() == 64 ? launch<T, 64>(a, p, hs) : launch<T, 128>(a, p, hs);
-  NF_ATTN(NF_DTYPE_BF16, bf16)
-  NF_ATTN(NF_DTYPE_F16, f16)
-  NF_ATTN(NF_DTYPE_F32, float)
+#define NF_ATTN(DT, T, DP) \
+  if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, p, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16, 64)
+  NF_ATTN(NF_DTYPE_BF16, bf16, 96)
+  NF_ATTN(NF_DTYPE_BF16, bf16, 128)
+  NF_ATTN(NF_DTYPE_F16, f16, 64)
+  NF_ATTN(NF_DTYPE_F16, f16, 96)
+  NF_ATTN(NF_DTYPE_F16, f16, 128)
+  NF_ATTN(NF_DTYPE_F32, float, 64)
+  NF_ATTN(NF_DTYPE_F32, float, 128)
 #undef NF_ATTN
   return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
 }

@@ -88,7 +88,7 @@ inline int64_t place_grid(int64_t heads, int64_t tiles) {
 template <typename T, int DP>
 struct Tile {
   static constexpr int ROW = DP * (int)sizeof(T);  // bytes
-  static constexpr int NV = ROW / 16;              // vectors of a row: 8, 12, 16 or 32
+  static constexpr int NV = ROW / 16;              // vectors of a row: 4, 8, 12, 16 or 32
   static constexpr int KS = ROW / 32;              // steps of a product over a row
   static constexpr int NB = DP / 32;               // 32-wide column blocks
   static constexpr int VE = 16 / (int)sizeof(T);
@@ -97,7 +97,7 @@ struct Tile {
   __device__ __forceinline__ static int swz(int row) {
     if constexpr (NV == 8)  // two rows to a bank cycle
       return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
-    else if constexpr (NV == 12)  // rows lie 3/4 of a bank cycle apart
+    else if constexpr (NV == 4 || NV == 12)  // rows lie 1/4 or 3/4 of a bank cycle apart
       return (row >> 2) & 3;
     else
       return (row & 3) << 2 | ((row >> 2) & 3);
@@ -703,7 +703,9 @@ struct Sizes {  // what a call is about, as its entry points take it
   int es() const { return dtype == NF_DTYPE_F32 ? 4 : 2; }
   int64_t rows() const { return Tq * (H / Hk); }
   // columns of a tile; fp32 rows of 96 would not swizzle
-  int dp() const { return D <= 64 ? 64 : D <= 96 && dtype != NF_DTYPE_F32 ? 96 : 128; }
+  int dp() const {
+    return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 && dtype != NF_DTYPE_F32 ? 96 : 128;
+  }
 };
 // NF_OK, or the error that is set
 int check_sizes(const char *op, const Sizes &z);

@@ -84,7 +84,7 @@ struct Dq {
 };
 
 template <typename T, int DP, int KW, bool MASKED>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP == 64) ? 2 : 1) void attn_dq_kernel(
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ? 2 : 1) void attn_dq_kernel(
     BwdArgs a) {
   using F = Dq<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
@@ -229,7 +229,7 @@ struct Dkv {
   static constexpr int NR = KW == 4 ? 1 : TR / 32;                   // of those, 32s of a wavefront
   static constexpr int TILE = TR * C::ROW;
   static constexpr int STAGE = 2 * TILE + 2 * 4 * (TR < 64 ? 64 : TR);  // q, dout, lse, -delta
-  static constexpr bool TWO = KW == 4 && DP == 64 && sizeof(T) == 2;  // blocks on a CU
+  static constexpr bool TWO = KW == 4 && DP <= 64 && sizeof(T) == 2;  // blocks on a CU
   static constexpr int STAGES = !TWO && 2 * STAGE <= 140 * 1024 ? 2 : 1;
   static constexpr int LDS = STAGES * STAGE;
   static_assert(LDS >= kWaves * Turned<DP>::BYTES, "the results turn in the tiles' place");
@@ -491,7 +491,7 @@ Plan dkv_plan(const Sizes &z, bool causal) {
   Plan p;
   p.kw = shared ? 4 : 1;
   p.tiles = (int)((z.Tk + bk - 1) / bk);
-  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() == 128 ? 512 : 256);
+  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 128 ? 512 : 256);
   p.most = parts_of((int)longest, p.length);
   p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.Tk) * (size_t)z.dp() * 8 : 0;
   return p;
@@ -605,12 +605,15 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   hipStream_t hs = static_cast<hipStream_t>(stream);
 #define NF_ATTN(DT, T, DP) \
   if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, z, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16, 32)
   NF_ATTN(NF_DTYPE_BF16, bf16, 64)
   NF_ATTN(NF_DTYPE_BF16, bf16, 96)
   NF_ATTN(NF_DTYPE_BF16, bf16, 128)
+  NF_ATTN(NF_DTYPE_F16, f16, 32)
   NF_ATTN(NF_DTYPE_F16, f16, 64)
   NF_ATTN(NF_DTYPE_F16, f16, 96)
   NF_ATTN(NF_DTYPE_F16, f16, 128)
+  NF_ATTN(NF_DTYPE_F32, float, 32)
   NF_ATTN(NF_DTYPE_F32, float, 64)
   NF_ATTN(NF_DTYPE_F32, float, 128)
 #undef NF_ATTN

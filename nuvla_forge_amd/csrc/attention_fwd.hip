@@ -46,7 +46,7 @@ struct Fwd {
 };
 
 template <typename T, int DP, int KW, bool MASKED>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP == 64) ? 2 : 1) void attn_fwd_kernel(
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ? 2 : 1) void attn_fwd_kernel(
     FwdArgs a) {
   using F = Fwd<T, DP, KW, MASKED>;
   using C = Tile<T, DP>;
@@ -466,12 +466,15 @@ extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   hipStream_t hs = static_cast<hipStream_t>(stream);
 #define NF_ATTN(DT, T, DP) \
   if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, p, hs);
+  NF_ATTN(NF_DTYPE_BF16, bf16, 32)
   NF_ATTN(NF_DTYPE_BF16, bf16, 64)
   NF_ATTN(NF_DTYPE_BF16, bf16, 96)
   NF_ATTN(NF_DTYPE_BF16, bf16, 128)
+  NF_ATTN(NF_DTYPE_F16, f16, 32)
   NF_ATTN(NF_DTYPE_F16, f16, 64)
   NF_ATTN(NF_DTYPE_F16, f16, 96)
   NF_ATTN(NF_DTYPE_F16, f16, 128)
+  NF_ATTN(NF_DTYPE_F32, float, 32)
   NF_ATTN(NF_DTYPE_F32, float, 64)
   NF_ATTN(NF_DTYPE_F32, float, 128)
 #undef NF_ATTN

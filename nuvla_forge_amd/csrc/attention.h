@@ -539,21 +539,20 @@ struct KeyTiles {
     }
     return i;
   }
-  // ZERO: the keys that the mask drops arrive as zeros; without, as they lie, for an operand of a
+  // zero: the keys that the mask drops arrive as zeros; without, as they lie, for an operand of a
   // product whose results for them are replaced
-  template <bool ZERO>
   __device__ __forceinline__ void copy_one(const char *p, int64_t step, const Copy &whole, int i,
-                                           const Bits &x, char *lds) const {
+                                           const Bits &x, char *lds, bool zero) const {
     const int left = s.Tk - i * TK;
     const char *at = p + (int64_t)i * TK * step;
-    if (left >= TK && (!(MASKED && ZERO) || x.all())) return whole.issue(at, lds, wave);
+    if (left >= TK && (!(MASKED && zero) || x.all())) return whole.issue(at, lds, wave);
     Copy c = whole;
     if constexpr (64 % Tile<T, DP>::NV == 0) {
       constexpr int PER = 64 / Tile<T, DP>::NV, ROWS = Copy::CW * PER;  // rows of a copy, a wavefront
       static_assert(ROWS <= 32, "a wavefront's rows are in one half of a word");
       const int row0 = Copy::row_of(wave, 0);
       uint32_t live = ~0u;
-      if constexpr (MASKED && ZERO) {
+      if (MASKED && zero) {
         uint64_t w = x.w[0];
         if constexpr (N == 2) w = wave >= kWaves / 2 ? x.w[1] : x.w[0];
         live = (uint32_t)(w >> (row0 & 63));
@@ -568,7 +567,7 @@ struct KeyTiles {
       for (int j = 0; j < Copy::CW; ++j) {
         const int row = Copy::row_of(wave, j);
         bool in = row < left;
-        if constexpr (MASKED && ZERO) {
+        if (MASKED && zero) {
           uint64_t w = x.w[0];
           if constexpr (N == 2) w = row >= 64 ? x.w[1] : x.w[0];
           in = in && (w >> (row & 63) & 1);
@@ -578,13 +577,11 @@ struct KeyTiles {
     }
     c.issue(at, lds, wave);
   }
-  template <bool ZERO>
-  __device__ __forceinline__ void copy_k(int i, const Bits &x, char *lds) const {
-    copy_one<ZERO>(k, kt, kc, i, x, lds);
+  __device__ __forceinline__ void copy_k(int i, const Bits &x, char *lds, bool zero) const {
+    copy_one(k, kt, kc, i, x, lds, zero);
   }
-  template <bool ZERO>
-  __device__ __forceinline__ void copy_v(int i, const Bits &x, char *lds) const {
-    copy_one<ZERO>(v, vt, vc, i, x, lds + TILE);
+  __device__ __forceinline__ void copy_v(int i, const Bits &x, char *lds, bool zero) const {
+    copy_one(v, vt, vc, i, x, lds + TILE, zero);
   }
 };
 
@@ -712,6 +709,41 @@ int check_sizes(const char *op, const Sizes &z);
 int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
               const Sizes &z, int64_t group, View *v);
 Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b);
+
+struct FwdArgs {
+  Shape s;
+  View q, k, v;
+  char *out;     // [B, Tq, H, D]
+  char *low;     // what out's rounding left, the same layout; null: not kept
+  float *lse;    // [B Hk, R] in powers of two; null: not kept
+  float *part;   // rows in parts: O [most][B Hk R][DP], then (m, l) pairs
+  int length, most, tiles;  // parts of about `length` tiles, at most `most`
+};
+
+struct BwdArgs {
+  Shape s;
+  View q, k, v, dout;
+  const char *out, *low;
+  const float *lse;
+  float *ndelta;  // [B Hk, R]: -delta
+  char *dq, *dk, *dv;
+  // rows, or keys, in parts: dQ [most][B Hk R][DP], dK and dV [most][B Hk Tk][2][DP]
+  float *part;
+  int tiles, length, most;
+};
+
+struct Plan {
+  int kw, tiles, length, most;
+  size_t bytes;  // of the parts
+};
+Plan fwd_plan(const Sizes &z, bool causal);
+Plan dq_plan(const Sizes &z, bool causal);
+Plan dkv_plan(const Sizes &z, bool causal);
+// one translation unit for each type has their kernels
+template <typename T>
+int launch_fwd(const FwdArgs &a, const Sizes &z, hipStream_t st);
+template <typename T>
+int launch_bwd(const BwdArgs &a, const Sizes &z, hipStream_t st);
 
 // The state's parts, in bytes from its start: log-sum-exps, what out's rounding left.
 struct State {

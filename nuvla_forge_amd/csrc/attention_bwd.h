@@ -8,7 +8,7 @@
 // every run), at the price of S and dP formed twice (seven products of a tile where five would do).
 // delta is formed from O's two parts, rounded and left over: out of the rounded part alone it would
 // be the largest error of dS where a row attends few keys.
-#include <math.h>
+#pragma once
 
 #include <type_traits>
 
@@ -16,19 +16,6 @@
 
 namespace nf {
 namespace attn {
-namespace {
-
-struct BwdArgs {
-  Shape s;
-  View q, k, v, dout;
-  const char *out, *low;
-  const float *lse;
-  float *ndelta;  // [B Hk, R]: -delta
-  char *dq, *dk, *dv;
-  // rows, or keys, in parts: dQ [most][B Hk R][DP], dK and dV [most][B Hk Tk][2][DP]
-  float *part;
-  int tiles, length, most;
-};
 
 // fp16 holds 2^-24 to 65504, and gradients may lie anywhere: dS is scaled by a power of two of its
 // column's own (a row's in dQ, a key's in dK), chosen so that its largest entry so far is about
@@ -152,8 +139,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
   auto copy = [&](int i, const typename F::Keys::Bits &x, char *lds) {
-    keys.template copy_k<true>(i, x, lds);   // a dropped key is multiplied by 0
-    keys.template copy_v<false>(i, x, lds);  // its value gives dS alone, which is replaced
+    keys.copy_k(i, x, lds, true);   // a dropped key is multiplied by 0
+    keys.copy_v(i, x, lds, false);  // its value gives dS alone, which is replaced
   };
   int at = keys.seek(begin, cur);
   if (at < end) copy(at, cur, smem);
@@ -466,45 +453,6 @@ __global__ __launch_bounds__(kThreads) void attn_sum_kernel(BwdArgs a) {
   }
 }
 
-struct Plan {
-  int kw, tiles, length, most;
-  size_t bytes;  // of the parts
-};
-
-Plan dq_plan(const Sizes &z, bool causal) {
-  const bool shared = shared_blocks(z, z.rows()), wide = z.dp() * z.es() > 256;
-  const int br = shared ? 32 : 128, tk = shared ? 128 : wide ? 32 : 64;
-  const int64_t heads = z.B * z.Hk, longest = (z.Tk + tk - 1) / tk;
-  Plan p;
-  p.kw = shared ? 4 : 1;
-  p.tiles = (int)((z.rows() + br - 1) / br);
-  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 256 ? 512 : 256);
-  p.most = parts_of((int)longest, p.length);
-  p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.rows()) * (size_t)z.dp() * 4 : 0;
-  return p;
-}
-
-Plan dkv_plan(const Sizes &z, bool causal) {
-  const bool shared = shared_blocks(z, z.Tk);
-  const int bk = shared ? 32 : 128, tr = shared ? 128 : z.dp() * z.es() > 256 ? 32 : 64;
-  const int64_t heads = z.B * z.Hk, longest = (z.rows() + tr - 1) / tr;
-  Plan p;
-  p.kw = shared ? 4 : 1;
-  p.tiles = (int)((z.Tk + bk - 1) / bk);
-  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 128 ? 512 : 256);
-  p.most = parts_of((int)longest, p.length);
-  p.bytes = p.most > 1 ? (size_t)p.most * (size_t)(heads * z.Tk) * (size_t)z.dp() * 8 : 0;
-  return p;
-}
-
-size_t delta_bytes(const Sizes &z) {
-  return ((size_t)(z.B * z.Hk * z.rows()) * 4 + 255) / 256 * 256;
-}
-size_t bwd_bytes(const Sizes &z, bool causal) {
-  const size_t a = dq_plan(z, causal).bytes, b = dkv_plan(z, causal).bytes;
-  return delta_bytes(z) + (a > b ? a : b);  // dQ's parts are summed before dK's are formed
-}
-
 template <typename T, int DP, int KW>
 void launch_dq(BwdArgs &a, hipStream_t st) {
   const unsigned grid = (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)a.tiles * a.most);
@@ -531,7 +479,7 @@ void launch_dkv(BwdArgs &a, hipStream_t st) {
 }
 
 template <typename T, int DP>
-int launch(BwdArgs a, const Sizes &z, hipStream_t st) {
+int launch_bwd_dp(BwdArgs a, const Sizes &z, hipStream_t st) {
   auto take = [&](const Plan &p) {
     a.tiles = p.tiles;
     a.length = p.length;
@@ -553,69 +501,17 @@ int launch(BwdArgs a, const Sizes &z, hipStream_t st) {
   return check_launch("nf_attention_bwd");
 }
 
-}  // namespace
+template <typename T>
+int launch_bwd(const BwdArgs &a, const Sizes &z, hipStream_t st) {
+  switch (z.dp()) {
+    case 32: return launch_bwd_dp<T, 32>(a, z, st);
+    case 64: return launch_bwd_dp<T, 64>(a, z, st);
+    case 96:
+      if constexpr (sizeof(T) == 2) return launch_bwd_dp<T, 96>(a, z, st);
+      [[fallthrough]];
+    default: return launch_bwd_dp<T, 128>(a, z, st);
+  }
+}
+
 }  // namespace attn
 }  // namespace nf
-
-using namespace nf;
-using namespace nf::attn;
-
-extern "C" size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                             int64_t Hk, int64_t D, int causal, int dtype) {
-  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  return check_sizes("nf_attention_bwd_workspace", z) ? 0 : bwd_bytes(z, causal);
-}
-
-extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
-                                int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
-                                int64_t v_t, int64_t v_h, const uint8_t *key_mask, int64_t mask_b,
-                                const void *out, const void *dout, int64_t g_b, int64_t g_t,
-                                int64_t g_h, int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                int64_t Hk, int64_t D, int causal, float scale, int dtype,
-                                const void *state, size_t state_bytes, void *dq, void *dk, void *dv,
-                                void *workspace, size_t workspace_bytes, void *stream) {
-  const char *op = "nf_attention_bwd";
-  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  if (const int rc = check_sizes(op, z)) return rc;
-  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
-  if (B == 0 || Tq == 0 || (!dq && !dk && !dv)) return NF_OK;
-  if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
-  if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
-  const State parts = state_of(z);
-  if (state_bytes < parts.total || workspace_bytes < bwd_bytes(z, causal))
-    return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
-                     state_bytes, parts.total, workspace_bytes, bwd_bytes(z, causal));
-  if (!out || !state || !aligned16(state) || !workspace || !aligned16(workspace))
-    return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
-  BwdArgs a = {};
-  if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
-  if (const int rc = make_view(op, "k", k, k_b, k_t, k_h, z, 0, &a.k)) return rc;
-  if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
-  if (const int rc = make_view(op, "dout", dout, g_b, g_t, g_h, z, H / Hk, &a.dout)) return rc;
-  const char *st = static_cast<const char *>(state);
-  a.s = make_shape(z, causal, scale, key_mask, mask_b);
-  a.out = static_cast<const char *>(out);
-  a.low = z.es() == 2 ? st + parts.low : nullptr;
-  a.lse = reinterpret_cast<const float *>(st);
-  a.ndelta = static_cast<float *>(workspace);
-  a.part = a.ndelta + delta_bytes(z) / 4;
-  a.dq = static_cast<char *>(dq);
-  a.dk = static_cast<char *>(dk);
-  a.dv = static_cast<char *>(dv);
-  hipStream_t hs = static_cast<hipStream_t>(stream);
-#define NF_ATTN(DT, T, DP) \
-  if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, z, hs);
-  NF_ATTN(NF_DTYPE_BF16, bf16, 32)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 64)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 96)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 128)
-  NF_ATTN(NF_DTYPE_F16, f16, 32)
-  NF_ATTN(NF_DTYPE_F16, f16, 64)
-  NF_ATTN(NF_DTYPE_F16, f16, 96)
-  NF_ATTN(NF_DTYPE_F16, f16, 128)
-  NF_ATTN(NF_DTYPE_F32, float, 32)
-  NF_ATTN(NF_DTYPE_F32, float, 64)
-  NF_ATTN(NF_DTYPE_F32, float, 128)
-#undef NF_ATTN
-  return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
-}

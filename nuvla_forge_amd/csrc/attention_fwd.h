@@ -3,7 +3,7 @@
 // One pass over the keys with a running maximum m and sum l: with c = |scale| log2(e) and S the
 // bare products, p = 2^(c S - m), l += sum p, O += p v; where m grows, O and l are scaled by
 // 2^(m_old - m_new); out = O / l, and the row's log-sum-exp is m + log2(l).
-#include <math.h>
+#pragma once
 
 #include <type_traits>
 
@@ -11,7 +11,6 @@
 
 namespace nf {
 namespace attn {
-namespace {
 
 // m is raised only when a logit passes it by kSlack (in powers of two): p is then at most 2^kSlack,
 // which every type holds, and most tiles leave O as it is.
@@ -19,16 +18,6 @@ constexpr float kSlack = 8.f;
 // fp16 ends at 2^-24: p carries a factor 2^7, so that it is normal down to 2^-21 of the largest.
 template <typename T>
 constexpr float kBias = __is_same(T, f16) ? 7.f : 0.f;
-
-struct FwdArgs {
-  Shape s;
-  View q, k, v;
-  char *out;     // [B, Tq, H, D]
-  char *low;     // what out's rounding left, the same layout; null: not kept
-  float *lse;    // [B Hk, R] in powers of two; null: not kept
-  float *part;   // rows in parts: O [most][B Hk R][DP], then (m, l) pairs
-  int length, most, tiles;  // parts of about `length` tiles, at most `most`
-};
 
 // KW = 1: a wavefront has 32 rows of its own, a block 128.  KW = 4: a block has 32 rows, and a
 // wavefront a quarter of each tile's keys.
@@ -84,8 +73,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
   typename F::Keys::Bits cur, nxt;
   auto copy = [&](int i, const typename F::Keys::Bits &x, char *lds) {
-    keys.template copy_k<false>(i, x, lds);  // a dropped key's logit is replaced
-    keys.template copy_v<true>(i, x, lds);   // its value is multiplied by 0
+    keys.copy_k(i, x, lds, false);  // a dropped key's logit is replaced
+    keys.copy_v(i, x, lds, true);   // its value is multiplied by 0
   };
   at = keys.seek(at, cur);
   if (at < end) copy(at, cur, smem);
@@ -282,29 +271,6 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(FwdArgs a) {
   if (a.lse && l == 0) a.lse[row] = sum == 0.f ? kInf : top + __log2f(sum);
 }
 
-struct Plan {
-  int kw, tiles, length, most;
-};
-
-Plan plan_of(const Sizes &z, bool causal) {
-  Plan p;
-  const int64_t R = z.rows(), heads = z.B * z.Hk;
-  const bool wide = z.dp() * z.es() > 256;
-  p.kw = shared_blocks(z, R) ? 4 : 1;
-  p.tiles = (int)((R + (p.kw == 4 ? 31 : 127)) / (p.kw == 4 ? 32 : 128));
-  const int tk = p.kw == 4 ? 128 : wide ? 32 : 64;
-  const int64_t longest = (z.Tk + tk - 1) / tk;
-  p.length = part_length(heads, p.tiles, longest, causal, p.kw == 4 && z.dp() * z.es() <= 256 ? 512 : 256);
-  p.most = parts_of((int)longest, p.length);
-  return p;
-}
-
-size_t part_bytes(const Sizes &z, bool causal) {
-  const Plan p = plan_of(z, causal);
-  if (p.most <= 1) return 0;
-  return (size_t)p.most * (size_t)(z.B * z.Hk * z.rows()) * (size_t)(z.dp() + 2) * 4;
-}
-
 template <typename T, int DP, int KW>
 void join(const FwdArgs &a, hipStream_t st) {
   const int64_t rows = (int64_t)a.s.B * a.s.Hk * a.s.R;
@@ -316,7 +282,10 @@ void join(const FwdArgs &a, hipStream_t st) {
 }
 
 template <typename T, int DP>
-int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
+int launch_fwd_dp(FwdArgs a, const Plan &p, hipStream_t st) {
+  a.length = p.length;
+  a.most = p.most;
+  a.tiles = p.tiles;
   const unsigned grid =
       (unsigned)place_grid((int64_t)a.s.B * a.s.Hk, (int64_t)p.tiles * p.most);
   if (p.kw == 4 && a.s.mask)
@@ -334,149 +303,17 @@ int launch(const FwdArgs &a, const Plan &p, hipStream_t st) {
   return check_launch("nf_attention_fwd");
 }
 
-}  // namespace
-
-// ---------------------------------------------------------------------------
-// host, shared with the backward
-// ---------------------------------------------------------------------------
-constexpr int64_t kMaxBlocks = (int64_t)1 << 23;
-
-int check_sizes(const char *op, const Sizes &z) {
-  if (!is_dtype(z.dtype)) return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, z.dtype);
-  if (z.B < 0 || z.Tq < 0 || z.Tk < 0 || z.H <= 0 || z.Hk <= 0 || z.H % z.Hk)
-    return set_error(NF_ERR_ARG, "%s: B=%lld Tq=%lld Tk=%lld H=%lld Hk=%lld", op, (long long)z.B,
-                     (long long)z.Tq, (long long)z.Tk, (long long)z.H, (long long)z.Hk);
-  if (z.D <= 0 || z.D > 128)
-    return set_error(NF_ERR_ARG, "%s: D=%lld outside [1, 128]", op, (long long)z.D);
-  const int64_t most = (int64_t)1 << 30;
-  if (z.B > most || z.H > most / 1024 || z.Tq > most || z.Tk > most || z.rows() > most ||
-      z.B * z.Hk > most || z.B * z.Hk * ((z.rows() + 31) / 32 + 1) > kMaxBlocks ||
-      z.B * z.Hk * ((z.Tk + 31) / 32 + 1) > kMaxBlocks)
-    return set_error(NF_ERR_ARG, "%s: B=%lld Tq=%lld Tk=%lld H=%lld Hk=%lld too large", op,
-                     (long long)z.B, (long long)z.Tq, (long long)z.Tk, (long long)z.H,
-                     (long long)z.Hk);
-  return NF_OK;
-}
-
-// `group`: heads between the first and the last element that a tile of one key head reads.
-int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
-              const Sizes &z, int64_t group, View *v) {
-  const int es = z.es();
-  if (!p) return set_error(NF_ERR_ARG, "%s: %s is null", op, name);
-  if (!aligned16(p) || sb * es % 16 || st * es % 16 || sh * es % 16 || sb < 0 || st < 0 || sh < 0)
-    return set_error(NF_ERR_ARG, "%s: %s: rows of 16-byte vectors expected", op, name);
-  // a tile's offsets, 128 rows and a group of heads, fit the buffer unit's 31 bits
-  const int64_t most = (int64_t)1 << 30;
-  if (st > most / 512 || sh > most || 130 * st * es + group * sh * es >= most)
-    return set_error(NF_ERR_ARG, "%s: %s: strides too large", op, name);
-  *v = View{static_cast<const char *>(p), sb * es, st * es, sh * es};
-  return NF_OK;
-}
-
-bool shared_blocks(const Sizes &z, int64_t own) {
-  const double work = (double)(z.B * z.Hk) * (double)z.rows() * (double)z.Tk * z.dp();
-  return own <= 32 || (z.B * z.Hk * ((own + 127) / 128) < 256 && work <= 2147483648.0);
-}
-
-Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b) {
-  Shape s;
-  s.B = (int)z.B;
-  s.Tq = (int)z.Tq;
-  s.Tk = (int)z.Tk;
-  s.H = (int)z.H;
-  s.Hk = (int)z.Hk;
-  s.G = (int)(z.H / z.Hk);
-  s.D = (int)z.D;
-  s.R = (int)z.rows();
-  const int ve = 16 / z.es();
-  s.nvec = (int)((z.D + ve - 1) / ve);
-  s.off = (int)(z.Tk - z.Tq);
-  s.causal = causal;
-  s.ginv = s.G == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + s.G - 1) / s.G);
-  // 0 times a barred key's -infinity would be no number: a scale that rounds every logit to 0
-  s.c = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
-  s.scale = scale;
-  s.flip = scale < 0.f ? (z.es() == 2 ? 0x80008000u : 0x80000000u) : 0u;
-  s.mask = mask;
-  s.mask_b = mask_b;
-  return s;
-}
-
-State state_of(const Sizes &z) {
-  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  State t;
-  t.low = up((size_t)(z.B * z.Hk * z.rows()) * 4);
-  t.total = t.low + (z.es() == 2 ? up((size_t)(z.B * z.Tq * z.H * z.D) * 2) : 0);
-  return t;
+template <typename T>
+int launch_fwd(const FwdArgs &a, const Sizes &z, hipStream_t st) {
+  switch (z.dp()) {
+    case 32: return launch_fwd_dp<T, 32>(a, fwd_plan(z, a.s.causal), st);
+    case 64: return launch_fwd_dp<T, 64>(a, fwd_plan(z, a.s.causal), st);
+    case 96:
+      if constexpr (sizeof(T) == 2) return launch_fwd_dp<T, 96>(a, fwd_plan(z, a.s.causal), st);
+      [[fallthrough]];
+    default: return launch_fwd_dp<T, 128>(a, fwd_plan(z, a.s.causal), st);
+  }
 }
 
 }  // namespace attn
 }  // namespace nf
-
-using namespace nf;
-using namespace nf::attn;
-
-extern "C" size_t nf_attention_state_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk,
-                                           int64_t D, int dtype) {
-  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  return check_sizes("nf_attention_state_bytes", z) ? 0 : state_of(z).total;
-}
-
-extern "C" size_t nf_attention_fwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
-                                             int64_t Hk, int64_t D, int causal, int dtype) {
-  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  if (check_sizes("nf_attention_fwd_workspace", z) || B * Tq * Tk == 0) return 0;
-  return part_bytes(z, causal);
-}
-
-extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, const void *k,
-                                int64_t k_b, int64_t k_t, int64_t k_h, const void *v, int64_t v_b,
-                                int64_t v_t, int64_t v_h, const uint8_t *key_mask, int64_t mask_b,
-                                int64_t B, int64_t Tq, int64_t Tk, int64_t H, int64_t Hk, int64_t D,
-                                int causal, float scale, int dtype, void *out, void *state,
-                                size_t state_bytes, void *workspace, size_t workspace_bytes,
-                                void *stream) {
-  const char *op = "nf_attention_fwd";
-  const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
-  if (const int rc = check_sizes(op, z)) return rc;
-  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
-  if (B == 0 || Tq == 0) return NF_OK;
-  if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
-  if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
-  const State parts = state_of(z);
-  if ((state && state_bytes < parts.total) || workspace_bytes < part_bytes(z, causal))
-    return set_error(NF_ERR_WORKSPACE, "%s: state %zu of %zu bytes, workspace %zu of %zu", op,
-                     state_bytes, parts.total, workspace_bytes, part_bytes(z, causal));
-  if (!out || !aligned16(state) || (part_bytes(z, causal) && (!workspace || !aligned16(workspace))))
-    return set_error(NF_ERR_ARG, "%s: null or unaligned pointer", op);
-  FwdArgs a = {};
-  if (const int rc = make_view(op, "q", q, q_b, q_t, q_h, z, H / Hk, &a.q)) return rc;
-  if (const int rc = make_view(op, "k", k, k_b, k_t, k_h, z, 0, &a.k)) return rc;
-  if (const int rc = make_view(op, "v", v, v_b, v_t, v_h, z, 0, &a.v)) return rc;
-  char *st = static_cast<char *>(state);
-  a.s = make_shape(z, causal, scale, key_mask, mask_b);
-  a.out = static_cast<char *>(out);
-  a.low = st && z.es() == 2 ? st + parts.low : nullptr;
-  a.lse = reinterpret_cast<float *>(st);
-  a.part = static_cast<float *>(workspace);
-  const Plan p = plan_of(z, causal);
-  a.length = p.length;
-  a.most = p.most;
-  a.tiles = p.tiles;
-  hipStream_t hs = static_cast<hipStream_t>(stream);
-#define NF_ATTN(DT, T, DP) \
-  if (dtype == DT && z.dp() == DP) return launch<T, DP>(a, p, hs);
-  NF_ATTN(NF_DTYPE_BF16, bf16, 32)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 64)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 96)
-  NF_ATTN(NF_DTYPE_BF16, bf16, 128)
-  NF_ATTN(NF_DTYPE_F16, f16, 32)
-  NF_ATTN(NF_DTYPE_F16, f16, 64)
-  NF_ATTN(NF_DTYPE_F16, f16, 96)
-  NF_ATTN(NF_DTYPE_F16, f16, 128)
-  NF_ATTN(NF_DTYPE_F32, float, 32)
-  NF_ATTN(NF_DTYPE_F32, float, 64)
-  NF_ATTN(NF_DTYPE_F32, float, 128)
-#undef NF_ATTN
-  return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, dtype);
-}

@@ -216,8 +216,8 @@ struct Dkv {
   static constexpr int NR = KW == 4 ? 1 : TR / 32;                   // of those, 32s of a wavefront
   static constexpr int TILE = TR * C::ROW;
   static constexpr int STAGE = 2 * TILE + 2 * 4 * (TR < 64 ? 64 : TR);  // q, dout, lse, -delta
-  static constexpr bool TWO = KW == 4 && DP <= 64 && sizeof(T) == 2;  // blocks on a CU
-  static constexpr int STAGES = !TWO && 2 * STAGE <= 140 * 1024 ? 2 : 1;
+  static constexpr bool TWO = DP <= 64 && sizeof(T) == 2;  // blocks on a CU
+  static constexpr int STAGES = !(TWO && KW == 4) && 2 * STAGE <= 140 * 1024 ? 2 : 1;
   static constexpr int LDS = STAGES * STAGE;
   static_assert(LDS >= kWaves * Turned<DP>::BYTES, "the results turn in the tiles' place");
 };

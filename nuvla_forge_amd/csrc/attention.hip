@@ -41,9 +41,12 @@ int make_view(const char *op, const char *name, const void *p, int64_t sb, int64
   return NF_OK;
 }
 
+// Small calls alone: of 3 x 301 x 1003, 6 heads of 80 on 2, fp16, the three kernels and their joins
+// took 88 us with own rows in parts, 72 shared, in two terms; a large one reads K and V four times
+// as often and forms half as many products again.
 bool shared_blocks(const Sizes &z, int64_t own) {
   const double work = (double)(z.B * z.Hk) * (double)z.rows() * (double)z.Tk * z.dp();
-  return own <= 32 || (z.B * z.Hk * ((own + 127) / 128) < 256 && work <= 2147483648.0);
+  return own <= 32 || (z.B * z.Hk * ((own + 127) / 128) < 256 && work <= 0x1p31);
 }
 
 Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b) {

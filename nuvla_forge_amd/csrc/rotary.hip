@@ -7,7 +7,11 @@
 // would be off by 0.06 radians), then sine and cosine of the fraction in 32 bits.  The frequencies
 // come as kernel arguments, made in 64 bits on the host: no table in memory, no upload.
 //
-// A thread turns 8 pairs at a time, in 16-byte accesses at any alignment.
+// A thread turns 8 pairs at a time from the halves, or 4 neighbouring ones, in 16-byte accesses at any
+// alignment, lanes side by side.
+//
+// What bounds it: memory (bf16, 20 heads of 128, 65536 tokens: 135 us, 4.97 TB/s, neighbours paired
+// 153; a copy of 1 GiB runs at 5.10).
 #include <math.h>
 
 #include "nf_device.h"
@@ -18,7 +22,11 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kMaxPairs = 256, kMaxAxes = 4;
 constexpr int kTable = 2048;  // (cos, sin) pairs of a block: 16 KB
-constexpr int64_t kNtMinBytes = (int64_t)320 << 20;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// Stores take the non-temporal hint where a launch reads and writes more than the Infinity Cache
+// holds: bf16, 20 heads of 128, 65536 tokens (671 MB) 141.8 us plain, 135.1 hinted, 32768 74.1 and
+// 55.7; 16384 (168 MB) 30.6 and 30.4, where the attention that follows finds them cached.
+constexpr int64_t kNtMinBytes = (int64_t)256 << 20;
 
 struct RotaryArgs {
   const void *x[2];  // q, k (k may be absent: heads[1] = 0)
@@ -68,34 +76,40 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
                  (t0 + t) * a.st[which] + h * a.sh[which];
     T *y = static_cast<T *>(a.out[which]) +
            (((int64_t)b * a.T + t0 + t) * a.heads[which] + h) * a.D;
-    if (chunk < a.turned) {
+    if (chunk < a.turned && INTER) {  // 4 pairs, neighbours
+      const int j = chunk * 4, left = 2 * (a.P - j);
+      const f32x4 c = *reinterpret_cast<const f32x4 *>(cs + t * pitch + j);
+      const f32x4 s = *reinterpret_cast<const f32x4 *>(sn + t * pitch + j);
+      Any8<T> u;
+      u.load(x + 2 * j, left);
+      float p[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = to_f32(u.v[2 * k]), f = to_f32(u.v[2 * k + 1]);
+        p[2 * k] = e * c[k] - f * s[k];
+        p[2 * k + 1] = e * s[k] + f * c[k];
+      }
+      u.set(p);
+      u.template store<NT>(y + 2 * j, left);
+    } else if (chunk < a.turned) {  // 8 pairs, from the two halves
       const int j = chunk * 8, left = a.P - j;
       float c[8], s[8];
       Chunk8<float>::load(cs + t * pitch + j, c);
       Chunk8<float>::load(sn + t * pitch + j, s);
       Any8<T> u, v;
-      const T *xu = x + (INTER ? 2 * j : j), *xv = INTER ? xu + 8 : xu + a.P;
-      const int nu = INTER ? 2 * left : left, nv = INTER ? 2 * left - 8 : left;
-      u.load(xu, nu);
-      v.load(xv, nv);
+      u.load(x + j, left);
+      v.load(x + j + a.P, left);
       float p[8], q[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if constexpr (INTER) {  // pair k: elements 2 k, 2 k + 1 of the sixteen
-          const float e = k < 4 ? to_f32(u.v[2 * (k & 3)]) : to_f32(v.v[2 * (k & 3)]);
-          const float f = k < 4 ? to_f32(u.v[2 * (k & 3) + 1]) : to_f32(v.v[2 * (k & 3) + 1]);
-          (k < 4 ? p : q)[2 * (k & 3)] = e * c[k] - f * s[k];
-          (k < 4 ? p : q)[2 * (k & 3) + 1] = e * s[k] + f * c[k];
-        } else {
-          const float e = to_f32(u.v[k]), f = to_f32(v.v[k]);
-          p[k] = e * c[k] - f * s[k];
-          q[k] = e * s[k] + f * c[k];
-        }
+        const float e = to_f32(u.v[k]), f = to_f32(v.v[k]);
+        p[k] = e * c[k] - f * s[k];
+        q[k] = e * s[k] + f * c[k];
       }
       u.set(p);
       v.set(q);
-      u.template store<NT>(y + (INTER ? 2 * j : j), nu);
-      v.template store<NT>(y + (INTER ? 2 * j + 8 : j + a.P), nv);
+      u.template store<NT>(y + j, left);
+      v.template store<NT>(y + j + a.P, left);
     } else {  // past the pairs: as it is
       const int d = 2 * a.P + (chunk - a.turned) * 8;
       Any8<T> u;
@@ -175,7 +189,7 @@ extern "C" int nf_rotary(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, v
   a.D = (int)D;
   a.P = P;
   a.axes = axes;
-  a.turned = (P + 7) / 8;
+  a.turned = interleaved ? (P + 3) / 4 : (P + 7) / 8;
   a.chunks = a.turned + (int)((D - 2 * P + 7) / 8);
   const int all = (int)(H + Hk);
   a.heads_inv = all == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + all - 1) / all);

@@ -41,12 +41,16 @@ int make_view(const char *op, const char *name, const void *p, int64_t sb, int64
   return NF_OK;
 }
 
-// Small calls alone: of 3 x 301 x 1003, 6 heads of 80 on 2, fp16, the three kernels and their joins
-// took 88 us with own rows in parts, 72 shared, in two terms; a large one reads K and V four times
-// as often and forms half as many products again.
+// Small calls alone (a large one would read K and V four times as often and form half as many
+// products again), by the three kernels' time, own rows in parts -> shared: 3 x 301 x 1003, 6 heads
+// of 80 on 2, fp16 88 -> 72 us; 1024 tokens, 8 heads of 64 64 -> 44, 2048 105 -> 98; 512, 8 heads of
+// 128 on 4 68 -> 50, 1500 causal, 4 heads of 128 79 -> 87.  fp32 rows of 512 bytes leave a CU one
+// block: 900, 4 heads of 128 160 -> 271.
 bool shared_blocks(const Sizes &z, int64_t own) {
+  if (own <= 32) return true;
+  if (z.dp() * z.es() > 256 || z.B * z.Hk * ((own + 127) / 128) >= 256) return false;
   const double work = (double)(z.B * z.Hk) * (double)z.rows() * (double)z.Tk * z.dp();
-  return own <= 32 || (z.B * z.Hk * ((own + 127) / 128) < 256 && work <= 0x1p31);
+  return work <= (z.dp() <= 64 ? 0x1p31 : 0x1p30);
 }
 
 Shape make_shape(const Sizes &z, int causal, float scale, const uint8_t *mask, int64_t mask_b) {

@@ -7,11 +7,15 @@
 // would be off by 0.06 radians), then sine and cosine of the fraction in 32 bits.  The frequencies
 // come as kernel arguments, made in 64 bits on the host: no table in memory, no upload.
 //
-// A thread turns 8 pairs at a time from the halves, or 4 neighbouring ones, in 16-byte accesses at any
-// alignment, lanes side by side.
+// A thread turns two pieces of 16 bytes at a time, one in each half of a head, at any alignment, with
+// the lanes of a head side by side in both: the two elements of a pair where those lie half a head
+// apart, two runs of pairs where they are neighbours.  Pieces of 8 elements, alone where
+// neighbours pair, took 136 us (now 133: halves, the shape below), 153 (131: neighbours) and 143
+// (126: fp32, 32768 tokens).
 //
-// What bounds it: memory (bf16, 20 heads of 128, 65536 tokens: 135 us, 4.97 TB/s, neighbours paired
-// 153; a copy of 1 GiB runs at 5.10).
+// What bounds it: memory (bf16, 20 heads of 128, 65536 tokens: 133 us, 5.06 TB/s, neighbours paired
+// 131; fp32 at half the tokens 126, 5.3; a copy of 1 GiB runs at 5.10).  Rows that are no whole cache
+// lines reach less: 3.1 TB/s at 12 heads of 123, 3.4 at 100.
 #include <math.h>
 
 #include "nf_device.h"
@@ -22,7 +26,6 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kMaxPairs = 256, kMaxAxes = 4;
 constexpr int kTable = 2048;  // (cos, sin) pairs of a block: 16 KB
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 // Stores take the non-temporal hint where a launch reads and writes more than the Infinity Cache
 // holds: bf16, 20 heads of 128, 65536 tokens (671 MB) 141.8 us plain, 135.1 hinted, 32768 74.1 and
 // 55.7; 16384 (168 MB) 30.6 and 30.4, where the attention that follows finds them cached.
@@ -34,7 +37,7 @@ struct RotaryArgs {
   int64_t sb[2], st[2], sh[2];
   int heads[2];
   int T, D, P, axes, tiles, tokens;  // tokens of a block
-  int chunks, turned;                // 8-wide pieces of a head, of those turned
+  int chunks, turned;                // items of a head, of those turned
   uint32_t heads_inv;                // ceil(2^32 / heads), 0: one
   const void *pos;                   // [B or 1, T, axes]
   int64_t pos_b;                     // elements between samples, 0: shared
@@ -44,8 +47,55 @@ struct RotaryArgs {
   double turns[kMaxPairs];           // frequency / 2 pi
 };
 
+// 16 bytes at any alignment, or the first of them.  The sums below are written as fmaf, not left to
+// the compiler: an element that two pieces share comes out alike in both.
+template <typename T>
+struct Piece {
+  static constexpr int kSize = 16 / (int)sizeof(T);
+  T v[kSize];
+  __device__ __forceinline__ void load(const T *p, int valid) {
+    if (valid >= kSize) {
+      __builtin_memcpy(v, p, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i) v[i] = i < valid ? p[i] : static_cast<T>(0.f);
+    }
+  }
+  template <bool NT>
+  __device__ __forceinline__ void store(T *p, int valid) const {
+    if (valid >= kSize) {
+      u32x4 a;
+      __builtin_memcpy(&a, v, 16);
+      u32x4_any *q = reinterpret_cast<u32x4_any *>(p);
+      if constexpr (NT)
+        __builtin_nontemporal_store(a, q);
+      else
+        *q = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSize; ++i)
+        if (i < valid) p[i] = v[i];
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void turn_neighbours(Piece<T> &u, const float *cs, const float *sn) {
+  constexpr int H = Piece<T>::kSize / 2;
+  float c[H], s[H];
+  __builtin_memcpy(c, cs, sizeof(c));
+  __builtin_memcpy(s, sn, sizeof(s));
+#pragma unroll
+  for (int k = 0; k < H; ++k) {
+    const float e = to_f32(u.v[2 * k]), f = to_f32(u.v[2 * k + 1]);
+    u.v[2 * k] = from_f32<T>(fmaf(e, c[k], -(f * s[k])));
+    u.v[2 * k + 1] = from_f32<T>(fmaf(e, s[k], f * c[k]));
+  }
+}
+
 template <typename T, bool INTER, bool NT>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
+  constexpr int E = Piece<T>::kSize;
   __shared__ __attribute__((aligned(16))) float cs[kTable], sn[kTable];
   const int b = blockIdx.x / a.tiles, t0 = (blockIdx.x - b * a.tiles) * a.tokens;
   const int n = min(a.tokens, a.T - t0);
@@ -76,46 +126,38 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
                  (t0 + t) * a.st[which] + h * a.sh[which];
     T *y = static_cast<T *>(a.out[which]) +
            (((int64_t)b * a.T + t0 + t) * a.heads[which] + h) * a.D;
-    if (chunk < a.turned && INTER) {  // 4 pairs, neighbours
-      const int j = chunk * 4, left = 2 * (a.P - j);
-      const f32x4 c = *reinterpret_cast<const f32x4 *>(cs + t * pitch + j);
-      const f32x4 s = *reinterpret_cast<const f32x4 *>(sn + t * pitch + j);
-      Any8<T> u;
-      u.load(x + 2 * j, left);
-      float p[8];
+    // An item is two pieces of 16 bytes, one in each half of its run (the turned elements or the
+    // rest), so that lanes lie side by side in both.  A piece that would pass the run's end ends
+    // with it: what it shares with the piece before it is formed twice, to the same bits.
+    const bool turn = chunk < a.turned;
+    const int run = turn ? 2 * a.P : a.D - 2 * a.P, items = turn ? a.turned : a.chunks - a.turned;
+    const int first = turn ? 0 : 2 * a.P;
+    const int c0 = (turn ? chunk : chunk - a.turned) * E;
+    const bool halves = turn && !INTER;  // the second half is pair j's other element
+    const int size = halves ? a.P : run;
+    const bool whole = size >= E;
+    const int e0 = whole ? min(c0, size - E) : c0;
+    const int e1 = halves ? a.P + e0 : whole ? min(items * E + c0, size - E) : items * E + c0;
+    const int left0 = size - c0, left1 = halves ? left0 : size - items * E - c0;
+    Piece<T> u, v;
+    u.load(x + first + e0, whole ? E : left0);
+    v.load(x + first + e1, whole ? E : left1);
+    if (halves) {
+      float c[E], s[E];
+      __builtin_memcpy(c, cs + t * pitch + e0, sizeof(c));
+      __builtin_memcpy(s, sn + t * pitch + e0, sizeof(s));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float e = to_f32(u.v[2 * k]), f = to_f32(u.v[2 * k + 1]);
-        p[2 * k] = e * c[k] - f * s[k];
-        p[2 * k + 1] = e * s[k] + f * c[k];
-      }
-      u.set(p);
-      u.template store<NT>(y + 2 * j, left);
-    } else if (chunk < a.turned) {  // 8 pairs, from the two halves
-      const int j = chunk * 8, left = a.P - j;
-      float c[8], s[8];
-      Chunk8<float>::load(cs + t * pitch + j, c);
-      Chunk8<float>::load(sn + t * pitch + j, s);
-      Any8<T> u, v;
-      u.load(x + j, left);
-      v.load(x + j + a.P, left);
-      float p[8], q[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < E; ++k) {
         const float e = to_f32(u.v[k]), f = to_f32(v.v[k]);
-        p[k] = e * c[k] - f * s[k];
-        q[k] = e * s[k] + f * c[k];
+        u.v[k] = from_f32<T>(fmaf(e, c[k], -(f * s[k])));
+        v.v[k] = from_f32<T>(fmaf(e, s[k], f * c[k]));
       }
-      u.set(p);
-      v.set(q);
-      u.template store<NT>(y + j, left);
-      v.template store<NT>(y + j + a.P, left);
-    } else {  // past the pairs: as it is
-      const int d = 2 * a.P + (chunk - a.turned) * 8;
-      Any8<T> u;
-      u.load(x + d, a.D - d);
-      u.template store<NT>(y + d, a.D - d);
+    } else if (turn) {
+      turn_neighbours(u, cs + t * pitch + e0 / 2, sn + t * pitch + e0 / 2);
+      turn_neighbours(v, cs + t * pitch + e1 / 2, sn + t * pitch + e1 / 2);
     }
+    u.template store<NT>(y + first + e0, whole ? E : left0);
+    v.template store<NT>(y + first + e1, whole ? E : left1);
   }
 }
 
@@ -189,8 +231,9 @@ extern "C" int nf_rotary(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, v
   a.D = (int)D;
   a.P = P;
   a.axes = axes;
-  a.turned = interleaved ? (P + 3) / 4 : (P + 7) / 8;
-  a.chunks = a.turned + (int)((D - 2 * P + 7) / 8);
+  const int es = dtype == NF_DTYPE_F32 ? 4 : 2, e = 16 / es;
+  a.turned = (P + e - 1) / e;
+  a.chunks = a.turned + (int)((D - 2 * P + 2 * e - 1) / (2 * e));
   const int all = (int)(H + Hk);
   a.heads_inv = all == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + all - 1) / all);
   a.pos = positions;
@@ -210,7 +253,6 @@ extern "C" int nf_rotary(const void *q, int64_t q_b, int64_t q_t, int64_t q_h, v
   const int64_t grid = B * a.tiles;
   if (grid > kMaxLaunchThreads / kBlock)
     return set_error(NF_ERR_ARG, "%s: B=%lld T=%lld too large", op, (long long)B, (long long)T);
-  const int es = dtype == NF_DTYPE_F32 ? 4 : 2;
   const bool nt = 2 * B * T * all * D * es > kNtMinBytes;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == NF_DTYPE_F32) return launch<float>(a, grid, interleaved, nt, s);

@@ -140,7 +140,8 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
             h // (H / Hk).
         causal: query i attends keys up to i + Tk - Tq: the last query sees every key.
         key_mask: bool [B, Tk]; False: no query attends the key.  What such a key and its
-            value hold is never read (the unfilled part of a cache, padding).
+            value hold, NaN or infinity too, changes no bit of any result (the unfilled part of
+            a cache, padding).
         scale: multiplies the logits; 1 / sqrt(D) by default.
         force_reference: run the eager formulation instead.
 
@@ -148,8 +149,9 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
         [B, Tq, H, D], contiguous, q's type.  A row that may attend no key gives zeros and
         takes no part in any gradient.
 
-    Logits, statistics and sums are fp32; the probabilities are rounded to the inputs' type
-    for their products.  A NaN or an infinity in a key or value that some row may attend can
+    Logits, statistics and sums are fp32; for their products the probabilities (and the logits'
+    gradients) are rounded to the inputs' type, or to two terms of it where few rows or keys
+    make a block's waves share them.  A NaN or an infinity in a key or value that some row may attend can
     reach other rows of its head in the same sample.  First derivatives only on the device.
     Host tensors, heads wider than 128 and calls without a key take the eager formulation.
     """

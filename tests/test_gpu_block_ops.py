@@ -198,6 +198,30 @@ def test_attention_masked_places_are_never_read(cuda, tq, tk, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tq, tk, d", [(150, 150, 72), (40, 300, 128), (129, 65, 32)])
+def test_attention_masks_over_many_heads(cuda, tq, tk, d, dtype):
+    """Blocks enough for every CU: samples and rows without a key give zeros, and what masked
+    places hold changes no bit."""
+    note(f"attention masks over many heads {tq} {tk} {d} {dtype}")
+    q, k, v, do = _qkv(70, tq, tk, 8, 4, d, dtype, cuda)
+    m = _mask("random", 70, tk, cuda)
+    m[0, tk // 2:] = False
+    m[1] = False
+    m[2, : tk // 2] = False
+    first = max(0, tq - tk)
+    want = _check(q, k, v, do, causal=True, key_mask=m)
+    for x in (want[0], want[1]):
+        assert (x[1] == 0).all() and (x[:, :first] == 0).all()
+    for x in (want[2], want[3]):
+        assert (x[~m] == 0).all()
+    for bad in (math.nan, -math.inf, torch.finfo(dtype).max):
+        kb, vb = (torch.where(m[..., None, None], t, torch.tensor(bad, dtype=dtype, device=cuda))
+                  for t in (k, v))
+        got = _run(q, kb, vb, do, causal=True, key_mask=m)
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), bad
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("tq", [1, 100])
 def test_attention_a_nan_stays_in_its_head_and_sample(cuda, tq, dtype):
     note(f"attention nan {tq} {dtype}")
@@ -513,6 +537,25 @@ def test_rotary_values_and_gradients(cuda, b, t, h, hk, d, sections, ladder, int
         within(got[i], *rotary64(x, pos, *ref, inverse=inverse), f"result {i}")
         assert got[i].is_contiguous() and got[i].dtype == dtype
         assert torch.equal(got[i][..., 2 * sum(sections):], x[..., 2 * sum(sections):])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_widths(cuda, interleaved, dtype):
+    """Pairs and elements past them that are no whole pieces, and the widest heads; the same bits
+    every run where pieces share elements."""
+    for d, p in ((1024, 255), (1024, 256), (1024, 1), (1023, 250), (123, 18), (8, 1), (9, 4), (10, 1),
+                 (14, 3), (15, 7), (17, 8), (21, 5), (24, 4), (25, 8), (26, 9), (34, 17), (47, 15),
+                 (64, 9)):
+        note(f"rotary width {d} {p} {interleaved} {dtype}")
+        q, k = (randn((2, 40, n, d), gen(d), dtype, cuda) for n in (3, 1))
+        pos = torch.randint(0, 9000, (2, 40, 1), generator=gen(p)).to(cuda)
+        got = fused_rotary(q, k, pos, (p,), interleaved=interleaved)
+        for x, y in zip((q, k), got):
+            within(y, *rotary64(x, pos, (p,), interleaved=interleaved), f"{d} {p}")
+            assert torch.equal(y[..., 2 * p:], x[..., 2 * p:])
+        again = fused_rotary(q, k, pos, (p,), interleaved=interleaved)
+        assert all(torch.equal(x, y) for x, y in zip(got, again))
 
 
 def test_rotary_strides_positions_and_parts(cuda, route):

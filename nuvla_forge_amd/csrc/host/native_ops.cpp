@@ -688,12 +688,14 @@ struct Attention : torch::autograd::Function<Attention> {
     variable_list res(6);
     const variable_list t = ctx->get_saved_variables();
     const auto s = ctx->saved_data["s"].toIntVector();
-    const Tensor &out = t[3], &state = t[4];
+    // what a saved-tensor hook gives back may lie in memory in another way
+    const Tensor out = t[3].contiguous(), state = t[4].contiguous();
     const Tensor mask = t.size() > 5 ? bytes_of(t[5]) : Tensor();
     const c10::DeviceGuard guard(out.device());
     TORCH_CHECK_VALUE(grads[0].device() == out.device(),
                       "fused_attention backward: dout is not on the forward's device");
-    const Heads q(t[0]), k(t[1]), v(t[2]), g = head_rows(grads[0].to(out.scalar_type()));
+    const Heads q = head_rows(t[0]), k = head_rows(t[1]), v = head_rows(t[2]);
+    const Heads g = head_rows(grads[0].to(out.scalar_type()));
     Sizes z = sizes(q.t, k.t);
     z.D = s[1];
     const int causal = (int)s[0], dt = code_of(out);
@@ -773,7 +775,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     }
     variable_list res(6);
     if (!g[0].defined() && !g[1].defined()) return res;
-    const Tensor pos = ctx->get_saved_variables()[0];
+    const Tensor pos = ctx->get_saved_variables()[0].contiguous();  // a hook may have moved it
     const auto call = ctx->saved_data["c"].toIntVector();
     const double base = ctx->saved_data["b"].toDouble();
     const bool inverse = ctx->saved_data["i"].toBool();

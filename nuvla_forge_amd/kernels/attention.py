@@ -78,6 +78,8 @@ class _FusedAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         q, k, v, out, state, key_mask = ctx.saved_tensors
+        # what a saved-tensor hook gives back may lie in memory in another way
+        q, k, v, out, state = (*map(_vector_rows, (q, k, v)), out.contiguous(), state.contiguous())
         sizes, causal, scale = ctx.call
         b, tq, tk, h, hk, d = sizes
         check_devices("fused_attention backward", "the forward's q", dict(dout=grad),

@@ -61,6 +61,7 @@ class _FusedRotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
+        positions = positions.contiguous()  # a saved-tensor hook may have moved them
         call, inverse = ctx.call
         want = [g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad)]
         check_devices("fused_rotary backward", "the forward's positions",

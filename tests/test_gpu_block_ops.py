@@ -754,6 +754,21 @@ def test_block_ops_saved_tensors_go_through_the_hooks(cuda, route, name):
 
 
 @pytest.mark.parametrize("name", ["attention", "few", "rotary"])
+def test_block_ops_hooks_may_change_the_layout(cuda, route, name):
+    """Saved tensors that come back with other strides."""
+    note(f"block ops hooks that change strides {name} {route}")
+    op, args = _calls(cuda)[name]
+    plain = _all(op, args)
+
+    def turned(v):  # the same values, the last axis outermost
+        return v.movedim(-1, 0).contiguous().movedim(0, -1)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v, turned):
+        hooked = _all(op, args)
+    assert all(torch.equal(a, b) for a, b in zip(plain, hooked, strict=True))
+
+
+@pytest.mark.parametrize("name", ["attention", "few", "rotary"])
 def test_block_ops_under_modes_tracing_and_transforms(cuda, name):
     from torch.overrides import TorchFunctionMode
     from torch.utils._python_dispatch import TorchDispatchMode

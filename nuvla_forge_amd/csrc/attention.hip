@@ -8,6 +8,8 @@ namespace nf {
 namespace attn {
 
 constexpr int64_t kMaxBlocks = (int64_t)1 << 23;
+// div_g is exact while the rows of a tile and a group, times the group, are below 2^32
+constexpr int64_t kMaxGroup = 1 << 15;
 
 int check_sizes(const char *op, const Sizes &z) {
   if (!is_dtype(z.dtype)) return set_error(NF_ERR_DTYPE, "%s: dtype %d", op, z.dtype);
@@ -16,6 +18,9 @@ int check_sizes(const char *op, const Sizes &z) {
                      (long long)z.Tq, (long long)z.Tk, (long long)z.H, (long long)z.Hk);
   if (z.D <= 0 || z.D > 128)
     return set_error(NF_ERR_ARG, "%s: D=%lld outside [1, 128]", op, (long long)z.D);
+  if (z.H / z.Hk > kMaxGroup)
+    return set_error(NF_ERR_ARG, "%s: %lld query heads a key head; at most %lld", op,
+                     (long long)(z.H / z.Hk), (long long)kMaxGroup);
   const int64_t most = (int64_t)1 << 30;
   if (z.B > most || z.H > most / 1024 || z.Tq > most || z.Tk > most || z.rows() > most ||
       z.B * z.Hk > most || z.B * z.Hk * ((z.rows() + 31) / 32 + 1) > kMaxBlocks ||

@@ -138,8 +138,8 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     Args:
         q: [B, Tq, H, D], fp32, bf16 or fp16; any strides (a copy is made where rows are
             not whole 16-byte vectors).
-        k, v: [B, Tk, Hk, D], q's type; H a multiple of Hk: query head h attends key head
-            h // (H / Hk).
+        k, v: [B, Tk, Hk, D], q's type; H a multiple of Hk, up to 32768 times it: query head h
+            attends key head h // (H / Hk).
         causal: query i attends keys up to i + Tk - Tq: the last query sees every key.
         key_mask: bool [B, Tk]; False: no query attends the key.  What such a key and its
             value hold, NaN or infinity too, changes no bit of any result (the unfilled part of

@@ -187,6 +187,23 @@ def test_attention_c_abi_refusals(call):
     assert call(B=0) == NF_OK and call(Tq=0) == NF_OK
 
 
+def test_attention_c_abi_refuses_groups_beyond_the_row_division():
+    """x / G by a 32-bit reciprocal is exact for all x < G + 128 up to the limit; beyond it the
+    quotient of G - 1 can be 1."""
+    def quotient(x, g):
+        return x * -(-2 ** 32 // g) >> 32
+
+    for g in (2, 3, 7, 127, 129, 32765, 32767, 32768):
+        assert all(quotient(x, g) == x // g for x in (0, 1, g - 1, g, 2 * g - 1, g + 127) if
+                   x < g + 128)
+    assert quotient(100_002, 100_003) == 1
+    L = _lib.lib()
+    assert L.nf_attention_state_bytes(1, 1, 1, 32768, 1, 8, 1) > 0
+    assert L.nf_attention_state_bytes(1, 1, 1, 32769, 1, 8, 1) == 0
+    for f in (L.nf_attention_fwd_workspace, L.nf_attention_bwd_workspace):
+        assert f(1, 1, 1, 32769, 1, 8, 0, 1) == 0
+
+
 def test_attention_c_abi_workspaces():
     L = _lib.lib()
     # many rows: no split; a few rows over many keys: partial sums

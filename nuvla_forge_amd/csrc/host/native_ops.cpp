@@ -633,8 +633,13 @@ Heads head_rows(const Tensor &t) {
                      (t.stride(3) == 1 || d == 1) && v.b % e == 0 && v.s % e == 0 &&
                      v.h % e == 0 && v.s <= far / 512 && 130 * v.s + t.size(2) * v.h < far;
   if (whole) return v;
-  if (d % e) return Heads(at::constant_pad_nd(t, {0, e - d % e}, 0));
-  return Heads(t.clone(at::MemoryFormat::Contiguous));
+  // written out, not padded by the library: that keeps the order of t's axes, the tokens innermost
+  // where they are
+  Tensor c = at::empty({t.size(0), t.size(1), t.size(2), (d + e - 1) / e * e},
+                       t.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  c.narrow(3, 0, d).copy_(t);
+  if (d % e) c.narrow(3, d, e - d % e).zero_();
+  return Heads(c);
 }
 
 struct Attention : torch::autograd::Function<Attention> {

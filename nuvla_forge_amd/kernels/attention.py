@@ -32,8 +32,12 @@ def _vector_rows(t: torch.Tensor) -> torch.Tensor:
              and st <= far // 512 and 130 * st + t.shape[2] * sh < far)
     if whole:
         return t
-    return torch.nn.functional.pad(t, (0, -d % e)) if d % e else t.clone(
-        memory_format=torch.contiguous_format)
+    # written out, not padded by the library: that keeps the order of t's axes, the tokens
+    # innermost where they are
+    rows = torch.empty(*t.shape[:3], d + -d % e, dtype=t.dtype, device=t.device)
+    rows[..., :d] = t
+    rows[..., d:] = 0
+    return rows
 
 
 def _strides(t: torch.Tensor) -> list[int]:

@@ -13,6 +13,7 @@ import torch
 
 from nuvla_forge_amd import _lib
 from nuvla_forge_amd.kernels import fused_attention, fused_rotary
+from nuvla_forge_amd.kernels import attention
 from nuvla_forge_amd.kernels.utils import DeviceMismatchError
 
 from .block_ops_ref import attention64, near, rotary64, within
@@ -306,3 +307,26 @@ def test_rotary_c_abi_refusals():
         assert call(**over) == NF_ERR_ARG, over
         assert "nf_rotary" in _err()
     assert call(B=0) == NF_OK and call(T=0) == NF_OK and call(H=0, Hk=0) == NF_OK
+
+
+# ---------------------------------------------------------------------------
+# the layouts that the kernels are handed
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, d", [(BF16, 100), (F16, 7), (F32, 90), (F32, 1), (BF16, 64)])
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (0, 2, 3, 1), (0, 3, 2, 1), (3, 2, 0, 1),
+                                   (1, 3, 0, 2)])
+@pytest.mark.parametrize("b, t, h", [(2, 70, 4), (1, 70, 1), (2, 1, 3), (1, 1, 1)])
+def test_attention_rows_are_whole_vectors_whatever_the_layout(b, t, h, order, dtype, d):
+    """What the Python entry hands to the kernels holds the values, zeros up to a whole vector, and
+    strides that the C entry takes."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(b, t, h, d, generator=g).to(dtype)
+    y = x.permute(order).contiguous().permute([order.index(i) for i in range(4)])
+    for z in (y, x[:, :1, :1].expand(b, t, h, d), x[..., :1].expand(b, t, h, d)):
+        rows = attention._vector_rows(z)
+        e = 16 // z.element_size()
+        assert rows.shape[:3] == z.shape[:3] and rows.shape[3] == -(-d // e) * e
+        assert torch.equal(rows[..., :d], z) and (rows[..., d:] == 0).all()
+        sb, st, sh = attention._strides(rows)
+        assert rows.stride(3) == 1 or rows.shape[3] == 1
+        assert sb % e == 0 and st % e == 0 and sh % e == 0 and rows.data_ptr() % 16 == 0

@@ -1,0 +1,74 @@
+"""Attention and the rotary positions on the GPU: calls at the edges of what the documentation
+allows (layouts that need a copy, rows that attend nothing, axes of no length, odd arguments).
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from nuvla_forge_amd.kernels import fused_attention
+
+from .helpers import gen, note, randn
+from .test_gpu_block_ops import _mask, _qkv, _run
+from .test_gpu_token_ops_edges import route  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+BF16, F32, F16 = torch.bfloat16, torch.float32, torch.float16
+
+
+def _same(want, got, what=""):
+    for name, a, b in zip(("out", "dq", "dk", "dv"), want, got, strict=True):
+        assert torch.equal(a, b), f"{what} {name}"
+
+
+# ---------------------------------------------------------------------------
+# layouts
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, d", [(BF16, 100), (F16, 100), (BF16, 7), (F32, 90), (F32, 1)])
+@pytest.mark.parametrize("tq", [1, 70])
+def test_attention_token_axis_innermost(cuda, route, tq, dtype, d):
+    """Heads of no whole vectors whose tokens lie side by side, or are one: operands, gradients
+    and saved tensors give the bits of their dense copies."""
+    note(f"attention tokens innermost {tq} {d} {dtype} {route}")
+    q, k, v, do = _qkv(2, tq, 70, 4, 2, d, dtype, cuda)
+    m = _mask("random", 2, 70, cuda)
+    want = _run(q, k, v, do, key_mask=m)
+
+    def inner(x, order):  # the same values, the axes stored in this order
+        back = [order.index(i) for i in range(4)]
+        return x.permute(order).contiguous().permute(back)
+
+    for order in ((0, 2, 3, 1), (0, 3, 2, 1), (3, 2, 0, 1), (1, 3, 0, 2)):
+        a, b, c, e = (inner(x, order) for x in (q, k, v, do))
+        _same(want, _run(a, b, c, do, key_mask=m), f"operands {order}")
+        _same(want, _run(q, k, v, e, key_mask=m), f"gradient {order}")
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x, o=order: (
+                inner(x, o) if x.dim() == 4 else x)):
+            _same(want, _run(a, b, c, e, key_mask=m), f"saved {order}")
+    one = [x[:, :1, :1, :1].expand(x.shape) for x in (q, k, v, do)]
+    _same(_run(*(x.contiguous() for x in one)), _run(*one), "broadcast")
+
+
+@pytest.mark.parametrize("dtype, d", [(BF16, 100), (F32, 90)])
+def test_attention_before_a_convolution_over_tokens(cuda, route, dtype, d):
+    """What follows takes [B, H D, T], and gives its gradient in that order."""
+    note(f"attention before a convolution {d} {dtype} {route}")
+    q, k, v, _ = _qkv(2, 70, 70, 2, 2, d, dtype, cuda)
+    w = randn((3, 2 * d, 1), gen(5), dtype, cuda)
+    seen = []
+
+    def step(keep):
+        x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = fused_attention(*x, causal=True)
+        out.register_hook(lambda g: (seen.append(g), keep(g))[1])
+        y = torch.matmul(w[:, :, 0].float(), out.float().flatten(2).transpose(1, 2).contiguous())
+        return [out, *torch.autograd.grad(y.sum(), x)]
+
+    # the gradient as the product's backward leaves it, tokens innermost or not, and its dense copy
+    _same(step(lambda g: g.contiguous()), step(lambda g: g))
+    g = seen[0].permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    assert g.stride(1) == 1
+    _same(step(lambda _: g.contiguous()), step(lambda _: g))

@@ -2,6 +2,8 @@
 // attention_fwd.h and attention_bwd.h, compiled for one type in each attention_{fwd,bwd}_*.hip.
 #include <math.h>
 
+#include <initializer_list>
+
 #include "attention.h"
 
 namespace nf {
@@ -135,6 +137,37 @@ Plan dkv_plan(const Sizes &z, bool causal) {
   return p;
 }
 
+__global__ __launch_bounds__(256) void attn_zero_kernel(uint16_t *p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    p[i] = 0;
+}
+
+// Gradients of keys that no row attends.  The workspace and the rows, which say nothing then, are
+// not looked at; the memory is: a pointer that the runtime does not know is refused, and on a host
+// without a device there is none to write.
+int zero_gradients(const char *op, std::initializer_list<void *> grads, int64_t bytes,
+                   hipStream_t st) {
+  int devices = 0;
+  if (hipGetDeviceCount(&devices) != hipSuccess || devices == 0) {
+    (void)hipGetLastError();
+    return NF_OK;
+  }
+  for (void *p : grads) {
+    if (!p) continue;
+    hipPointerAttribute_t at = {};
+    if (hipPointerGetAttributes(&at, p) != hipSuccess || at.type == hipMemoryTypeUnregistered) {
+      (void)hipGetLastError();
+      return set_error(NF_ERR_ARG, "%s: a gradient is not in device memory", op);
+    }
+  }
+  const int64_t n = bytes / 2, blocks = (n + 255) / 256;
+  for (void *p : grads)
+    if (p)
+      attn_zero_kernel<<<(unsigned)(blocks < 1024 ? blocks : 1024), 256, 0, st>>>(
+          static_cast<uint16_t *>(p), n);
+  return check_launch(op);
+}
+
 size_t delta_bytes(const Sizes &z) {
   return ((size_t)(z.B * z.Hk * z.rows()) * 4 + 255) / 256 * 256;
 }
@@ -216,7 +249,11 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (const int rc = check_sizes(op, z)) return rc;
   if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
-  if (B == 0 || Tq == 0 || (!dq && !dk && !dv)) return NF_OK;
+  if (B == 0 || (!dq && !dk && !dv)) return NF_OK;
+  if (Tq == 0)  // dq is empty, dk and dv are empty sums
+    return Tk == 0 || (!dk && !dv)
+               ? NF_OK
+               : zero_gradients(op, {dk, dv}, B * Tk * Hk * D * z.es(), static_cast<hipStream_t>(stream));
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
   if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
   const State parts = state_of(z);

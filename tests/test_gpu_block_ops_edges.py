@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from nuvla_forge_amd import _lib
 from nuvla_forge_amd.kernels import fused_attention
 
 from .helpers import gen, note, randn
@@ -72,3 +73,69 @@ def test_attention_before_a_convolution_over_tokens(cuda, route, dtype, d):
     g = seen[0].permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
     assert g.stride(1) == 1
     _same(step(lambda _: g.contiguous()), step(lambda _: g))
+
+
+# ---------------------------------------------------------------------------
+# axes of no length
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("b, tk, hk, d", [(1, 1, 1, 1), (2, 70, 2, 64), (3, 1001, 5, 33)])
+def test_attention_gradients_of_no_rows_are_zeros(cuda, b, tk, hk, d, dtype):
+    """The C entry over keys without a query: dk and dv are empty sums, and what lies behind them
+    stays; also inside a captured graph."""
+    note(f"attention no rows {b} {tk} {hk} {d} {dtype}")
+    dt = _lib.dtype_code(dtype)
+    n = b * tk * hk * d
+    empty = torch.empty(256, dtype=torch.uint8, device=cuda)
+    p = empty.data_ptr()
+
+    def call(dk, dv, stream):
+        return _lib.lib().nf_attention_bwd(
+            *(p, 0, 0, 0) * 3, None, 0, p, p, 0, 0, 0, b, 0, tk, 2 * hk, hk, d, 1, 1.0, dt, p, 0, None,
+            dk, dv, None, 0, stream)
+
+    def outs():
+        return [torch.full((n + 64,), 5.0, dtype=dtype, device=cuda) for _ in range(2)]
+
+    x = outs()
+    stream = _lib.stream_of(x[0])
+    for pick in ((True, True), (True, False), (False, True), (False, False)):
+        x = outs()
+        assert call(*(t.data_ptr() if w else None for t, w in zip(x, pick)), stream) == 0
+        for t, w in zip(x, pick):
+            assert (t[:n] == (0.0 if w else 5.0)).all() and (t[n:] == 5.0).all()
+    x = outs()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        assert call(x[0].data_ptr(), x[1].data_ptr(), _lib.stream_of(x[0])) == 0
+    for _ in range(3):
+        for t in x:
+            t.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all((t[:n] == 0).all() and (t[n:] == 5.0).all() for t in x)
+
+
+def test_attention_without_rows_through_the_public_call(cuda, route):
+    note(f"attention without rows {route}")
+    q, k, v, _ = _qkv(2, 3, 40, 4, 2, 64, BF16, cuda)
+    x = [t.detach().requires_grad_(True) for t in (q[:, :0], k, v)]
+    out = fused_attention(*x)
+    assert out.shape == (2, 0, 4, 64)
+    got = torch.autograd.grad(out, x, torch.empty_like(out))
+    assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(got, x))
+
+
+def test_attention_gradients_of_no_rows_outside_device_memory_are_refused(cuda):
+    """The one call that looks at no operand asks the runtime where its gradients are, before any
+    launch."""
+    note("attention no rows, a gradient on the host")
+    host, dev = torch.full((64,), 5.0), torch.full((64,), 5.0, device=cuda)
+    p = dev.data_ptr()
+    for dk, dv in ((host.data_ptr(), p), (p, host.data_ptr()), (4096, None)):
+        rc = _lib.lib().nf_attention_bwd(
+            *(p, 0, 0, 0) * 3, None, 0, p, p, 0, 0, 0, 1, 0, 4, 2, 1, 16, 1, 1.0, 0, p, 0, None, dk, dv,
+            None, 0, _lib.stream_of(dev))
+        assert rc == -1 and "nf_attention_bwd" in _lib.lib().nf_last_error().decode()
+    assert (dev == 5.0).all() and (host == 5.0).all()

@@ -124,26 +124,29 @@ def dropout_ref(x, threshold, seed, offset, residual):
 
 def attention_ref(q, k, v, causal, key_mask, scale):
     """softmax(scale q k^T) v in fp32 over the keys that a row may attend, cast to q's type; a
-    row without one gives 0.  Keys that ``key_mask`` drops are replaced, not multiplied away."""
+    row without one gives 0.  Keys that ``key_mask`` drops and rows without a key are replaced, not
+    multiplied away."""
     b, tq, h, d = q.shape
     tk, hk = k.shape[1:3]
-    if key_mask is not None:
-        k, v = (torch.where(key_mask[..., None, None], t, 0.0) for t in (k, v))
-    qf = q.float().reshape(b, tq, hk, h // hk, d).permute(0, 2, 3, 1, 4)  # [B, Hk, G, Tq, D]
-    kf = k.float().permute(0, 2, 3, 1).contiguous()[:, :, None]
-    vf = v.float().permute(0, 2, 1, 3).contiguous()[:, :, None]
-    z = torch.matmul(qf, kf) * scale
     barred = torch.zeros(b, 1, 1, tq, tk, dtype=torch.bool, device=q.device)
     if causal:
         barred = barred | torch.ones(tq, tk, dtype=torch.bool, device=q.device).triu(tk - tq + 1)
     if key_mask is not None:
         barred = barred | ~key_mask[:, None, None, None]
+        k, v = (torch.where(key_mask[..., None, None], t, 0.0) for t in (k, v))
+    attends = (~barred).any(-1).view(b, tq, 1, 1)
+    q = torch.where(attends, q, 0.0)
+    qf = q.float().reshape(b, tq, hk, h // hk, d).permute(0, 2, 3, 1, 4)  # [B, Hk, G, Tq, D]
+    kf = k.float().permute(0, 2, 3, 1).contiguous()[:, :, None]
+    vf = v.float().permute(0, 2, 1, 3).contiguous()[:, :, None]
+    z = torch.matmul(qf, kf) * scale
     z = z.masked_fill(barred, -math.inf)
     top = z.detach().amax(-1, keepdim=True) if tk else z.new_zeros(*z.shape[:-1], 1)
     e = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
     total = e.sum(-1, keepdim=True)
     out = torch.matmul(e / torch.where(total == 0.0, 1.0, total), vf)
-    return out.permute(0, 3, 1, 2, 4).reshape(b, tq, h, d).to(q.dtype)
+    out = out.permute(0, 3, 1, 2, 4).reshape(b, tq, h, d).to(q.dtype)
+    return torch.where(attends, out, 0.0)
 
 
 def rotary_ref(x, positions, sections, base, joint, interleaved):

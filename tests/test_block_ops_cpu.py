@@ -330,3 +330,24 @@ def test_attention_rows_are_whole_vectors_whatever_the_layout(b, t, h, order, dt
         sb, st, sh = attention._strides(rows)
         assert rows.stride(3) == 1 or rows.shape[3] == 1
         assert sb % e == 0 and st % e == 0 and sh % e == 0 and rows.data_ptr() % 16 == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("mask", [False, True])
+def test_attention_rows_without_a_key_reach_no_gradient_on_the_host(mask, dtype):
+    q, k, v = _qkv(2, 7, 4, 2, 1, 6, dtype)
+    dout = torch.randn(q.shape, generator=torch.Generator().manual_seed(2)).to(dtype)
+    m = torch.tensor([[False, False, True, True], [False] * 4]) if mask else None
+    bare = torch.arange(7)[None].expand(2, 7) < (torch.tensor([[5], [7]]) if mask else 3)
+
+    def run(q, dout):
+        x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = fused_attention(*x, causal=True, key_mask=m)
+        return [out, *torch.autograd.grad(out, x, dout)]
+
+    want = run(q, dout)
+    assert (want[0][bare] == 0).all() and (want[1][bare] == 0).all()
+    for bad in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
+        q2, d2 = (torch.where(bare[..., None, None], torch.tensor(bad, dtype=dtype), t)
+                  for t in (q, dout))
+        assert all(torch.equal(a, b) for a, b in zip(want, run(q2, d2))), bad

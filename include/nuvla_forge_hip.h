@@ -431,8 +431,9 @@ int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
  *   dv = P^T dout,  dS = P (dout v^T - rowsum(dout out)),
  *   dq = scale dS k,  dk = scale dS^T q,
  * dk and dv summed over the G heads of a group; dense, in `dtype`; any may be
- * NULL: not formed.  Without a query (Tq = 0) dk and dv are zeros, and nothing
- * else is looked at.  The same bits every run. */
+ * NULL: not formed.  What q and dout hold in a row without a key changes no
+ * bit of any gradient.  Without a query (Tq = 0) dk and dv are zeros, and
+ * nothing else is looked at.  The same bits every run. */
 size_t nf_attention_bwd_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t H,
                                   int64_t Hk, int64_t D, int causal,
                                   int dtype);

@@ -585,35 +585,40 @@ struct KeyTiles {
   }
 };
 
-// A key head's rows of q or dout, tile by tile of TR, into LDS.
+// A key head's rows of q or dout, tile by tile of TR, into LDS; those before `first` and past the
+// last arrive as zeros.
 template <typename T, int DP, int TR>
 struct RowTiles {
   using Copy = TileCopy<T, DP, TR>;
   const Shape &s;
   const char *p;
   int64_t t, h;  // bytes from token to token, head to head
-  int wave;
-  bool fixed;  // G divides TR: every tile begins with a token's first row
+  int wave, first;
+  // the tiles that begin with a token's first row and have every row
+  int whole_from;
+  uint32_t whole_count;
   Copy whole;
 
-  __device__ __forceinline__ RowTiles(const Shape &s_, const View &v, int b, int hk, int wave_)
+  __device__ __forceinline__ RowTiles(const Shape &s_, const View &v, int b, int hk, int wave_,
+                                      int first_)
       : s(s_), p(v.p + b * v.b + (int64_t)hk * s_.G * v.h), t(v.t), h(v.h), wave(wave_),
-        fixed(TR % s_.G == 0) {
-    set(whole, 0, TR);
+        first(first_), whole_from((first_ + TR - 1) / TR),
+        whole_count(TR % s_.G == 0 ? (uint32_t)max(s_.R / TR - whole_from, 0) : 0u) {
+    set(whole, 0, 0, TR);
   }
-  __device__ __forceinline__ void set(Copy &c, int g0, int left) const {
+  __device__ __forceinline__ void set(Copy &c, int g0, int from, int to) const {
     c.set(s.nvec, wave, [&](int row, bool *in) {
-      *in = row < left;
+      *in = row >= from && row < to;
       const int x = g0 + row, dt = div_g(s, x), g = x - dt * s.G;
       return (uint32_t)dt * (uint32_t)t + (uint32_t)g * (uint32_t)h;
     });
   }
-  __device__ __forceinline__ void copy(int row0, char *lds) const {
-    const int t0 = row0 / s.G, left = s.R - row0;
+  __device__ __forceinline__ void copy(int tile, char *lds) const {
+    const int row0 = tile * TR, t0 = row0 / s.G;
     const char *at = p + (int64_t)t0 * t;
-    if (fixed && left >= TR) return whole.issue(at, lds, wave);
+    if ((uint32_t)(tile - whole_from) < whole_count) return whole.issue(at, lds, wave);
     Copy c;
-    set(c, row0 - t0 * s.G, left);
+    set(c, row0 - t0 * s.G, first - row0, s.R - row0);
     c.issue(at, lds, wave);
   }
 };

@@ -103,6 +103,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   u32x4 q[1][C::KS], dout[1][C::KS];
   load_row<T, DP>(a.dout.p + b * a.dout.b + t * a.dout.t + (int64_t)(hk * s.G + g) * a.dout.h,
                   r < s.R, s.nvec, 0u, dout[0]);
+  const float lse = a.lse[row];
   float nd = 0.f;  // -delta: the lane's half of the columns, then both
   {
     const T *out = reinterpret_cast<const T *>(a.out) + at_out;
@@ -128,12 +129,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
         nd = fmaf(-to_f32(d[i]), to_f32(o[i]) + to_f32(w[i]), nd);
     }
     nd = pair_sum(nd);
+    if (lse == kInf) nd = 0.f;  // no key: whatever dO holds
     if (r < s.R && h == 0 && (KW == 1 || wave == 0) && part == 0) a.ndelta[row] = nd;
   }
   if (!a.dq) return;  // the call is for delta alone
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
                   s.flip, q[0]);
-  const float lse = a.lse[row];
   const int last = s.causal ? t + s.off : s.Tk - 1;
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
   const int begin = part * a.length, end = part + 1 < parts ? begin + a.length : len;
@@ -257,19 +258,39 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
   const int from = s.causal ? max(key - s.off, 0) : 0;
   const int64_t rmin64 = (int64_t)from * s.G;
   const int rmin = (int)(rmin64 < s.R ? rmin64 : s.R);
+  // Causal: the first row that may attend a key, the first one or, under a mask, the first that it
+  // leaves the block.  The rows before it are not read: a NaN or an infinity there, in the query or dO
+  // of a row without a key for one, would be one in the gradients too, multiplied by 0.  (What they
+  // read as is 0; -delta is 0 and the log-sum-exp infinity for a row without a key.)
+  int least = 0, row_first = 0;
+  if (s.causal) {
+    if (s.mask) {
+      least = s.Tk;
+#pragma unroll
+      for (int i = F::BK / 32 - 1; i >= 0; --i) {  // lanes l and l + 32 ask for the same key
+        const int j = tile * F::BK + 32 * i + (l & 31);
+        const uint32_t some =
+            (uint32_t)__ballot(KW == 4 ? live : j < s.Tk && s.mask[b * s.mask_b + j] != 0);
+        if (some) least = tile * F::BK + 32 * i + __builtin_ctz(some);
+      }
+    }
+    row_first = (int)min((int64_t)max(least - s.off, 0) * s.G, (int64_t)s.R);
+  }
   const int end = begin + len - part * a.length;  // from the last row back
   int at = part + 1 < parts ? end - a.length : begin;
+  at = least == s.Tk ? end : min(max(at, row_first / F::TR), end);  // no key: no row
   // from this tile on, every row sees every key of the block
   const int64_t every = s.causal ? (int64_t)max(tile * F::BK + F::BK - 1 - s.off, 0) * s.G : 0;
   const int full = (int)min((every + F::TR - 1) / F::TR, (int64_t)end);
 
   const char *lp = reinterpret_cast<const char *>(a.lse + (int64_t)bh * s.R);
   const char *np = reinterpret_cast<const char *>(a.ndelta + (int64_t)bh * s.R);
-  const RowTiles<T, DP, F::TR> qs(s, a.q, b, hk, wave), dos(s, a.dout, b, hk, wave);
+  const RowTiles<T, DP, F::TR> qs(s, a.q, b, hk, wave, row_first),
+      dos(s, a.dout, b, hk, wave, row_first);
   auto copy = [&](int i, char *buf) {
     const int row0 = i * F::TR, left = s.R - row0;
-    qs.copy(row0, buf);
-    dos.copy(row0, buf + F::TILE);
+    qs.copy(i, buf);
+    dos.copy(i, buf + F::TILE);
     if (F::TR > 64 || wave < 2) {  // 64 values a wavefront: log-sum-exps, then -deltas
       constexpr int EACH = F::TR > 64 ? 2 : 1;
       const int at4 = (wave % EACH) * 64 + l;

@@ -153,12 +153,13 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
 
     Returns:
         [B, Tq, H, D], contiguous, q's type.  A row that may attend no key gives zeros and
-        takes no part in any gradient.
+        takes no part in any gradient, whatever its query and its output's gradient hold.
 
     Logits, statistics and sums are fp32; for their products the probabilities (and the logits'
     gradients) are rounded to the inputs' type, or to two terms of it where few rows or keys
-    make a block's waves share them.  A NaN or an infinity in a key or value that some row may attend can
-    reach other rows of its head in the same sample.  First derivatives only on the device.
+    make a block's waves share them.  A NaN or an infinity in a key or value that some row may
+    attend, or in the query or the gradient of a row that attends one, can reach other rows of its
+    head and the gradients of other keys in the same sample.  First derivatives only on the device.
     Host tensors, heads wider than 128 and calls without a key take the eager formulation.
     """
     fused = use_fused(q, "fused_attention", force_reference)

@@ -13,7 +13,7 @@ from nuvla_forge_amd import _lib
 from nuvla_forge_amd.kernels import fused_attention
 
 from .helpers import gen, note, randn
-from .test_gpu_block_ops import _mask, _qkv, _run
+from .test_gpu_block_ops import _check, _mask, _qkv, _run
 from .test_gpu_token_ops_edges import route  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -76,8 +76,67 @@ def test_attention_before_a_convolution_over_tokens(cuda, route, dtype, d):
 
 
 # ---------------------------------------------------------------------------
-# axes of no length
+# rows that attend no key, axes of no length
 # ---------------------------------------------------------------------------
+def _padded(kind, b, tk, dev):
+    """Masks that leave a sample's first keys out, one sample none, one all of them."""
+    if kind is None:
+        return None
+    m = torch.ones(b, tk, dtype=torch.bool)
+    for i in range(b):
+        m[i, : i * tk // (b + 1)] = False
+    if kind == "holes":
+        m &= torch.rand(b, tk, generator=gen(b)) > 0.3
+    m[-1] = False
+    return m.to(dev)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("mask", [None, "left", "holes"])
+@pytest.mark.parametrize("b, tq, tk, h, hk, d", [
+    (3, 20, 9, 4, 2, 64), (3, 200, 150, 4, 2, 72), (3, 33, 200, 6, 2, 128), (2, 5, 3, 3, 1, 40),
+    (4, 1, 70, 4, 2, 32), (70, 150, 130, 8, 4, 72), (70, 150, 150, 8, 4, 128), (66, 70, 70, 9, 3, 32),
+    (2, 2300, 2000, 4, 2, 64), (3, 2000, 2000, 2, 1, 128)])
+def test_attention_rows_without_a_key_reach_no_gradient(cuda, b, tq, tk, h, hk, d, mask, dtype):
+    """NaN, infinities and the type's largest values in the queries and output gradients of rows
+    that attend no key change no bit of any result."""
+    note(f"attention keyless rows {b} {tq} {tk} {h} {hk} {d} {mask} {dtype}")
+    q, k, v, do = _qkv(b, tq, tk, h, hk, d, dtype, cuda)
+    m = _padded(mask, b, tk, cuda)
+    live = torch.ones(b, tk, dtype=torch.bool, device=cuda) if m is None else m
+    seen = torch.arange(tq, device=cuda) + tk - tq  # the row's last key
+    count = torch.cat([torch.zeros(b, 1, device=cuda), live.float().cumsum(1)], 1)
+    bare = count.gather(1, (seen + 1).clamp(min=0).expand(b, tq)) == 0
+    if not bare.any():
+        bare = torch.zeros_like(bare)
+    want = _run(q, k, v, do, causal=True, key_mask=m)
+    for x in want[:2]:
+        assert (x[bare] == 0).all()
+    for bad in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
+        fill = torch.tensor(bad, dtype=dtype, device=cuda)
+        q2, do2 = (torch.where(bare[..., None, None], fill, t) for t in (q, do))
+        _same(want, _run(q2, k, v, do, causal=True, key_mask=m), f"q {bad}")
+        _same(want, _run(q2, k, v, do2, causal=True, key_mask=m), f"q, dout {bad}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("b, t, h, hk, d", [(2, 300, 4, 2, 64), (2, 2000, 4, 2, 128), (70, 140, 8, 4, 96)])
+def test_attention_blocks_without_a_key_give_zeros(cuda, b, t, h, hk, d, dtype):
+    """Stretches of keys that the mask drops whole, at either end and between, causal or not: zero
+    gradients there, whatever the rows hold elsewhere."""
+    note(f"attention dropped blocks {b} {t} {h} {hk} {d} {dtype}")
+    q, k, v, do = _qkv(b, t, t, h, hk, d, dtype, cuda)
+    m = torch.ones(b, t, dtype=torch.bool, device=cuda)
+    m[0, : t // 2] = False
+    m[1, t // 2:] = False
+    m[-1, t // 4: 3 * t // 4] = False
+    for causal in (False, True):
+        _check(q, k, v, do, causal=causal, key_mask=m)
+        got = _run(q, k, v, do, causal=causal, key_mask=m)
+        for x in got[2:]:
+            assert (x[~m] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("b, tk, hk, d", [(1, 1, 1, 1), (2, 70, 2, 64), (3, 1001, 5, 33)])
 def test_attention_gradients_of_no_rows_are_zeros(cuda, b, tk, hk, d, dtype):

@@ -670,13 +670,24 @@ __device__ __forceinline__ void store_quad(T *p, int d, int D, const f32x4 &v) {
   }
 }
 
-// A wavefront's 32 rows (KW = 1), or a block's 32 rows in four parts that are summed (KW = 4), as
-// `put` left them: each vector to store(row, column, values).
+// What other lanes of the wavefront wrote to LDS before this is seen after it, and what they read
+// before it is not overwritten by what comes after.  A wavefront's LDS operations go in order, so it
+// is no instruction (the forward's code is the same with it; dK and dV of 2 x 4096 rows, 16 heads of
+// 128: 582 us without and with); but without it nothing holds the compiler to that order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// A wavefront's 32 rows (KW = 1), or a block's 32 rows in four parts that are summed (KW = 4; barriers
+// around it are the caller's), as `put` left them: each vector to store(row, column, values).
 template <int DP, int KW, class F>
 __device__ __forceinline__ void each_vector(const char *smem, int wave, F &&store) {
   using U = Turned<DP>;
   constexpr int PER = KW == 4 ? kThreads : 64;
   const int first = KW == 4 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+  if (KW == 1) wave_order();
 #pragma unroll
   for (int i = 0; i < 32 * U::V / PER; ++i) {
     const int x = i * PER + first, row = x / U::V, v = x % U::V;
@@ -688,6 +699,7 @@ __device__ __forceinline__ void each_vector(const char *smem, int wave, F &&stor
       y = U::get(smem + wave * U::BYTES, row, v);
     store(row, 4 * v, y);
   }
+  if (KW == 1) wave_order();  // the next `put` goes to the same place
 }
 
 // a lane's 64-bit value, from every lane

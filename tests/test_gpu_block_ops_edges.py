@@ -198,3 +198,17 @@ def test_attention_gradients_of_no_rows_outside_device_memory_are_refused(cuda):
             None, 0, _lib.stream_of(dev))
         assert rc == -1 and "nf_attention_bwd" in _lib.lib().nf_last_error().decode()
     assert (dev == 5.0).all() and (host == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [24, 32, 57, 64, 88, 96, 120, 128])
+def test_attention_results_that_turn_in_one_place(cuda, d, dtype):
+    """Blocks whose wavefronts have rows, or keys, of their own lay dk and then dv out in the same
+    LDS: each is the one of a call for it alone, and both are right."""
+    note(f"attention results in turn {d} {dtype}")
+    q, k, v, do = _qkv(64, 130, 130, 4, 4, d, dtype, cuda)
+    want = _check(q, k, v, do)
+    for i in (1, 2):
+        x = [t.detach().requires_grad_(i == j) for j, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(fused_attention(*x), x[i], do)[0]
+        assert torch.equal(got, want[1 + i])

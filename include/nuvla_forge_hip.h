@@ -405,7 +405,7 @@ int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
  * where D is no multiple of 16 bytes the elements up to the next one are
  * zeros.  out [B, Tq, H, D] dense.  D at most 128, H / Hk at most 32768; Tk
  * at least 1; 130 token strides and H / Hk head strides below 2^30 bytes;
- * scale finite.  What rows that the mask drops from k and v hold, NaN or
+ * |scale| at most 2^127.  What rows that the mask drops from k and v hold, NaN or
  * infinity too, changes no bit of any result; their memory has to be readable.
  * `state` (nf_attention_state_bytes; NULL: no backward will come) takes each
  * row's log-sum-exp and, for 16-bit types, what the rounding of out left;

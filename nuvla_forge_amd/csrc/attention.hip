@@ -33,6 +33,12 @@ int check_sizes(const char *op, const Sizes &z) {
   return NF_OK;
 }
 
+// times log2(e) it has to be an fp32 number
+int check_scale(const char *op, float scale) {
+  if (fabsf(scale) <= 0x1p127f) return NF_OK;
+  return set_error(NF_ERR_ARG, "%s: scale %g is beyond 2^127", op, (double)scale);
+}
+
 // `group`: heads between the first and the last element that a tile of one key head reads.
 int make_view(const char *op, const char *name, const void *p, int64_t sb, int64_t st, int64_t sh,
               const Sizes &z, int64_t group, View *v) {
@@ -205,7 +211,7 @@ extern "C" int nf_attention_fwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   const char *op = "nf_attention_fwd";
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (const int rc = check_sizes(op, z)) return rc;
-  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
+  if (const int rc = check_scale(op, scale)) return rc;
   if (B == 0 || Tq == 0) return NF_OK;
   if (Tk == 0) return set_error(NF_ERR_ARG, "%s: Tk=0", op);
   if (key_mask && mask_b < 0) return set_error(NF_ERR_ARG, "%s: mask_b < 0", op);
@@ -248,7 +254,7 @@ extern "C" int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t
   const char *op = "nf_attention_bwd";
   const Sizes z{B, Tq, Tk, H, Hk, D, dtype};
   if (const int rc = check_sizes(op, z)) return rc;
-  if (!isfinite(scale)) return set_error(NF_ERR_ARG, "%s: scale is not finite", op);
+  if (const int rc = check_scale(op, scale)) return rc;
   if (B == 0 || (!dq && !dk && !dv)) return NF_OK;
   if (Tq == 0)  // dq is empty, dk and dv are empty sums
     return Tk == 0 || (!dk && !dv)

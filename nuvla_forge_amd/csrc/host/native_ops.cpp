@@ -1052,7 +1052,7 @@ PyObject *py_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   }
   const bool causal = args[4] == Py_True;
   const double scale = PyFloat_AS_DOUBLE(args[5]);
-  if (!std::isfinite((float)scale)) Py_RETURN_NONE;
+  if (!(std::fabs(scale) <= 0x1p127)) Py_RETURN_NONE;
   return THPVariable_Wrap(unlocked([&]() -> Tensor {
     if (wants_grad({&t[0], &t[1], &t[2]}))
       return Attention::apply(t[0], t[1], t[2],

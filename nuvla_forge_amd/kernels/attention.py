@@ -20,6 +20,7 @@ from .reference import attention_ref
 from .utils import check_devices, device_of, first_order_only, use_fused
 
 MAX_HEAD = 128  # widest head the kernels take
+MAX_SCALE = 2.0 ** 127  # times log2(e) is still an fp32 number
 
 
 def _vector_rows(t: torch.Tensor) -> torch.Tensor:
@@ -129,8 +130,8 @@ def _check(q, k, v, key_mask, scale):
         if key_mask.shape != k.shape[:2]:
             raise ValueError(f"fused_attention: key_mask [B, Tk] = {tuple(k.shape[:2])} expected, "
                              f"got {tuple(key_mask.shape)}")
-    if not math.isfinite(scale):
-        raise ValueError(f"fused_attention: scale must be finite, got {scale}")
+    if not abs(scale) <= MAX_SCALE:
+        raise ValueError(f"fused_attention: scale must be finite in fp32 (at most 2^127), got {scale}")
     check_devices("fused_attention", "q", dict(q=q, k=k, v=v, key_mask=key_mask))
 
 
@@ -148,7 +149,7 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
         key_mask: bool [B, Tk]; False: no query attends the key.  What such a key and its
             value hold, NaN or infinity too, changes no bit of any result (the unfilled part of
             a cache, padding).
-        scale: multiplies the logits; 1 / sqrt(D) by default.
+        scale: multiplies the logits, in fp32; 1 / sqrt(D) by default.
         force_reference: run the eager formulation instead.
 
     Returns:

@@ -351,3 +351,16 @@ def test_attention_rows_without_a_key_reach_no_gradient_on_the_host(mask, dtype)
         q2, d2 = (torch.where(bare[..., None, None], torch.tensor(bad, dtype=dtype), t)
                   for t in (q, dout))
         assert all(torch.equal(a, b) for a, b in zip(want, run(q2, d2))), bad
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, 2e38, math.nextafter(2.0 ** 127, math.inf)])
+def test_attention_scales_beyond_fp32_are_refused(scale):
+    """2^127 log2(e) is below fp32's largest number, about 2^128."""
+    q, k, v = _qkv(2, 3, 4, 4, 2, 8)
+    with pytest.raises(ValueError, match="fused_attention: scale"):
+        fused_attention(q, k, v, scale=scale)
+    for s in (2.0 ** 127, -2.0 ** 127, 0.0):
+        assert fused_attention(q * 0.0, k, v, scale=s).isfinite().all()
+    for call in (_fwd, _bwd):
+        if abs(scale) < 3.4e38 and ctypes.c_float(scale).value != 2.0 ** 127:
+            assert call(scale=scale) == NF_ERR_ARG and "scale" in _err()

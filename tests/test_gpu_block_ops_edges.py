@@ -212,3 +212,25 @@ def test_attention_results_that_turn_in_one_place(cuda, d, dtype):
         x = [t.detach().requires_grad_(i == j) for j, t in enumerate((q, k, v))]
         got = torch.autograd.grad(fused_attention(*x), x[i], do)[0]
         assert torch.equal(got, want[1 + i])
+
+
+# ---------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, 2e38, math.inf, -math.inf, math.nan])
+def test_attention_scale_beyond_fp32_is_refused(cuda, route, scale):
+    note(f"attention scale {scale} {route}")
+    q, k, v, _ = _qkv(2, 3, 4, 4, 2, 64, BF16, cuda)
+    with pytest.raises(ValueError, match="fused_attention: scale"):
+        fused_attention(q, k, v, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -2.0 ** 127, 2.0 ** -149, 1e-300])
+def test_attention_scales_at_the_ends_of_fp32(cuda, route, scale):
+    """Logits of 0 stay 0: each row's output is its values' mean, its queries' gradient 0 or what
+    the scale makes of it."""
+    note(f"attention scale {scale} {route}")
+    q, k, v, do = _qkv(2, 3, 8, 4, 2, 64, F32, cuda)
+    out, _, dk, dv = _run(torch.zeros_like(q), k, v, do, scale=scale)
+    want = _run(torch.zeros_like(q), k, v, do, scale=1.0)
+    assert torch.equal(out, want[0]) and torch.equal(dv, want[3]) and (dk == 0).all()

@@ -1110,7 +1110,7 @@ PyObject *py_rotary(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   const at::ScalarType pt = pos.scalar_type();
   if (pairs < 1 || pairs > kMaxPairs || 2 * pairs > D || D > kMaxTurned || !(base > 0.0) ||
       !std::isfinite(base) || (pt != at::kLong && pt != at::kInt && pt != at::kFloat) ||
-      pos.size(-1) != axes || pos.dim() < 2 || pos.dim() > 3 || pos.size(-2) != T ||
+      pos.dim() < 2 || pos.dim() > 3 || pos.size(-1) != axes || pos.size(-2) != T ||
       (pos.dim() == 3 && pos.size(0) != B && pos.size(0) != 1))
     Py_RETURN_NONE;
   const variable_list r = unlocked([&]() -> variable_list {

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from nuvla_forge_amd import _lib
-from nuvla_forge_amd.kernels import fused_attention
+from nuvla_forge_amd.kernels import fused_attention, fused_rotary
 
 from .helpers import gen, note, randn
 from .test_gpu_block_ops import _check, _mask, _qkv, _run
@@ -234,3 +234,11 @@ def test_attention_scales_at_the_ends_of_fp32(cuda, route, scale):
     out, _, dk, dv = _run(torch.zeros_like(q), k, v, do, scale=scale)
     want = _run(torch.zeros_like(q), k, v, do, scale=1.0)
     assert torch.equal(out, want[0]) and torch.equal(dv, want[3]) and (dk == 0).all()
+
+
+@pytest.mark.parametrize("shape", [(), (2,), (3,), (1, 1, 3, 2), (0, 2)])
+def test_rotary_positions_of_the_wrong_dimensions_are_refused(cuda, route, shape):
+    note(f"rotary positions {shape} {route}")
+    q = randn((2, 3, 4, 16), gen(0), BF16, cuda)
+    with pytest.raises(ValueError, match="fused_rotary: positions"):
+        fused_rotary(q, None, torch.zeros(shape, dtype=torch.long, device=cuda), (4, 4))

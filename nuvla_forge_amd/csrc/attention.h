@@ -195,11 +195,11 @@ __device__ __forceinline__ u32x4 col_frag(const char *tile, int kb, int step) {
 // vector operations is the order in which they issue.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// acc[n] += rows 32 kb .. + 31 of the tile times the columns held in b[n] (one row of DP elements
-// a lane: vector 2 k + lane / 32 of it at step k).
-template <typename T, int DP, int N>
+// acc += rows 32 kb .. + 31 of the tile times the columns held in b (one row of DP elements a lane:
+// vector 2 k + lane / 32 of it at step k).
+template <typename T, int DP>
 __device__ __forceinline__ void mma_rows(const char *tile, int kb,
-                                         const u32x4 (&b)[N][Tile<T, DP>::KS], floatx16 (&acc)[N]) {
+                                         const u32x4 (&b)[Tile<T, DP>::KS], floatx16 &acc) {
   using C = Tile<T, DP>;
   const int l = threadIdx.x & 63, h = l >> 5, row = l & 31;
   const char *p = tile + (kb * 32 + row) * C::ROW;
@@ -207,8 +207,7 @@ __device__ __forceinline__ void mma_rows(const char *tile, int kb,
 #pragma unroll
   for (int k = 0; k < C::KS; ++k) {
     const u32x4 a = *reinterpret_cast<const u32x4 *>(p + ((2 * k + h) ^ sw) * 16);
-#pragma unroll
-    for (int n = 0; n < N; ++n) acc[n] = mma<T>(a, b[n][k], acc[n]);
+    acc = mma<T>(a, b[k], acc);
   }
 }
 
@@ -252,11 +251,11 @@ struct Twice<float> {
   __device__ __forceinline__ void set(const floatx16 &x) { hi.set(x); }
 };
 
-// acc[n][nb] += (columns 32 nb .. + 31 of rows 32 kb .. + 31 of the tile)^T x[n], over those rows
-// in the order in which the lanes hold x.
-template <typename T, int DP, int N>
-__device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<T> (&x)[N],
-                                         floatx16 (&acc)[N][Tile<T, DP>::NB]) {
+// acc[nb] += (columns 32 nb .. + 31 of rows 32 kb .. + 31 of the tile)^T x, over those rows in the
+// order in which the lanes hold x.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<T> &x,
+                                         floatx16 (&acc)[Tile<T, DP>::NB]) {
   using C = Tile<T, DP>;
   const int l = threadIdx.x & 63, h = l >> 5;
   const char *p = tile + kb * 32 * C::ROW;
@@ -268,34 +267,29 @@ __device__ __forceinline__ void mma_cols(const char *tile, int kb, const Packed<
       for (int nb = 0; nb < C::NB; ++nb) {
         const int vec = (8 * nb + (l & 31) / 4) ^ C::swz(row);
         const float a = *reinterpret_cast<const float *>(p + row * C::ROW + vec * 16 + (l & 3) * 4);
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-          acc[n][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[n].v[i], acc[n][nb], 0, 0, 0);
+        acc[nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x.v[i], acc[nb], 0, 0, 0);
       }
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 2 * C::NB; ++j) {
       const u32x4 a = col_frag<T, DP>(tile, kb, j);
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        acc[n][j % C::NB] = mma<T>(a, x[n].v[j / C::NB], acc[n][j % C::NB]);
+      acc[j % C::NB] = mma<T>(a, x.v[j / C::NB], acc[j % C::NB]);
     }
   }
 }
 
 template <typename T, int DP>
 __device__ __forceinline__ void mma_cols(const char *tile, int kb, const Twice<T> &x,
-                                         floatx16 (&acc)[1][Tile<T, DP>::NB]) {
+                                         floatx16 (&acc)[Tile<T, DP>::NB]) {
   using C = Tile<T, DP>;
   if constexpr (sizeof(T) == 4) {
-    const Packed<T> y[1] = {x.hi};
-    mma_cols<T, DP, 1>(tile, kb, y, acc);
+    mma_cols<T, DP>(tile, kb, x.hi, acc);
   } else {
 #pragma unroll
     for (int j = 0; j < 2 * C::NB; ++j) {
       const u32x4 a = col_frag<T, DP>(tile, kb, j);
-      floatx16 &to = acc[0][j % C::NB];
+      floatx16 &to = acc[j % C::NB];
       to = mma<T>(a, x.lo.v[j / C::NB], to);
       to = mma<T>(a, x.hi.v[j / C::NB], to);
     }
@@ -428,7 +422,7 @@ constexpr int kMostParts = 128;
 
 // Tiles of keys that rows [tile br, + br) go over.
 template <int TK>
-__host__ __device__ __forceinline__ int key_tiles(const Shape &s, int tile, int br) {
+__device__ __forceinline__ int key_tiles(const Shape &s, int tile, int br) {
   const int64_t stop = (int64_t)tile * br + br;
   const int rows_end = stop < s.R ? (int)stop : s.R;
   const int last = s.causal ? (rows_end - 1) / s.G + s.off : s.Tk - 1;
@@ -436,7 +430,7 @@ __host__ __device__ __forceinline__ int key_tiles(const Shape &s, int tile, int 
 }
 // The first tile of TR rows that sees a key of keys [tile bk, + bk).
 template <int TR>
-__host__ __device__ __forceinline__ int first_row_tile(const Shape &s, int tile, int bk) {
+__device__ __forceinline__ int first_row_tile(const Shape &s, int tile, int bk) {
   const int end = (s.R + TR - 1) / TR;
   const int64_t from = s.causal ? (int64_t)tile * bk - s.off : 0;
   const int64_t at = from > 0 ? from * s.G / TR : 0;

@@ -100,9 +100,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   const int rc = min(r, s.R - 1), t = rc / s.G, g = rc - t * s.G;
   const int64_t row = (int64_t)bh * s.R + rc;
   const int64_t at_out = (((int64_t)b * s.Tq + t) * s.H + hk * s.G + g) * s.D;
-  u32x4 q[1][C::KS], dout[1][C::KS];
+  u32x4 q[C::KS], dout[C::KS];
   load_row<T, DP>(a.dout.p + b * a.dout.b + t * a.dout.t + (int64_t)(hk * s.G + g) * a.dout.h,
-                  r < s.R, s.nvec, 0u, dout[0]);
+                  r < s.R, s.nvec, 0u, dout);
   const float lse = a.lse[row];
   float nd = 0.f;  // -delta: the lane's half of the columns, then both
   {
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
       const int col = (2 * k + h) * C::VE;
       const int valid = min(max(s.D - col, 0), C::VE);
       T d[C::VE], o[C::VE] = {}, w[C::VE] = {};
-      __builtin_memcpy(d, &dout[0][k], 16);
+      __builtin_memcpy(d, &dout[k], 16);
       if (valid == C::VE) {
         __builtin_memcpy(o, out + col, 16);
         if (low) __builtin_memcpy(w, low + col, 16);
@@ -134,15 +134,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   }
   if (!a.dq) return;  // the call is for delta alone
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
-                  s.flip, q[0]);
+                  s.flip, q);
   const int last = s.causal ? t + s.off : s.Tk - 1;
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;
   const int begin = part * a.length, end = part + 1 < parts ? begin + a.length : len;
   const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
-  floatx16 dq[1][C::NB];
+  floatx16 dq[C::NB];
 #pragma unroll
-  for (int n = 0; n < C::NB; ++n) dq[0][n] = splat(0.f);
+  for (int n = 0; n < C::NB; ++n) dq[n] = splat(0.f);
   Ranged<T, C::NB> range;
 
   typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
@@ -162,25 +162,25 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
     const int kb0 = KW == 4 ? wave : 0;
 #pragma unroll
     for (int i = 0; i < F::NK; ++i) {
-      floatx16 p[1] = {splat(0.f)}, dp[1] = {splat(nd)};
-      mma_rows<T, DP, 1>(kt, kb0 + i, q, p);
-      mma_rows<T, DP, 1>(vt, kb0 + i, dout, dp);
+      floatx16 p = splat(0.f), dp = splat(nd);
+      mma_rows<T, DP>(kt, kb0 + i, q, p);
+      mma_rows<T, DP>(vt, kb0 + i, dout, dp);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dp[0][e] *= exp2_(fmaf(p[0][e], s.c, -lse));
+      for (int e = 0; e < 16; ++e) dp[e] *= exp2_(fmaf(p[e], s.c, -lse));
       if constexpr (EDGE) {
         const uint32_t live = live32(last - (at * F::TK + 32 * (kb0 + i)), cur.half(kb0 + i));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dp[0][e] = keep(dp[0][e], live, e, 0u);
+        for (int e = 0; e < 16; ++e) dp[e] = keep(dp[e], live, e, 0u);
       }
-      range.fit(dp[0], dq[0]);
+      range.fit(dp, dq);
       if constexpr (KW == 4) {
         Twice<T> x;
-        x.set(dp[0]);
+        x.set(dp);
         mma_cols<T, DP>(kt, kb0 + i, x, dq);
       } else {
-        Packed<T> x[1];
-        x[0].set(dp[0]);
-        mma_cols<T, DP, 1>(kt, kb0 + i, x, dq);
+        Packed<T> x;
+        x.set(dp);
+        mma_cols<T, DP>(kt, kb0 + i, x, dq);
       }
     }
     if (F::STAGES == 1) {
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   }
   const float f = s.scale * range.undo();
   __syncthreads();
-  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, dq[0], f);
+  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, dq, f);
   if (KW == 4) __syncthreads();
   float *sums = a.part + ((int64_t)part * s.B * s.Hk * s.R + (int64_t)bh * s.R + r0) * DP;
   each_vector<DP, KW>(smem, wave, [&](int i, int d, const f32x4 &x) {
@@ -251,9 +251,9 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
   const int key0 = tile * F::BK + (KW == 1 ? 32 * wave : 0);
   const int key = key0 + (l & 31);
   const bool live = key < s.Tk && (!s.mask || s.mask[b * s.mask_b + key]);
-  u32x4 k[1][C::KS], v[1][C::KS];
-  load_row<T, DP>(a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t, live, s.nvec, s.flip, k[0]);
-  load_row<T, DP>(a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t, live, s.nvec, 0u, v[0]);
+  u32x4 k[C::KS], v[C::KS];
+  load_row<T, DP>(a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t, live, s.nvec, s.flip, k);
+  load_row<T, DP>(a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t, live, s.nvec, 0u, v);
   // causal: row r sees the key from r = (key - off) G on
   const int from = s.causal ? max(key - s.off, 0) : 0;
   const int64_t rmin64 = (int64_t)from * s.G;
@@ -300,9 +300,9 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
     }
   };
 
-  floatx16 dk[1][C::NB], dv[1][C::NB];
+  floatx16 dk[C::NB], dv[C::NB];
 #pragma unroll
-  for (int n = 0; n < C::NB; ++n) dk[0][n] = dv[0][n] = splat(0.f);
+  for (int n = 0; n < C::NB; ++n) dk[n] = dv[n] = splat(0.f);
   Ranged<T, C::NB> range;
 
   // The whole tiles that every row and key share come last, in pairs, so that the buffers' addresses
@@ -321,26 +321,26 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
 #pragma unroll
       for (int n = 0; n < F::NR; ++n) {
         const int i = KW == 4 ? wave : n;
-        floatx16 p[1] = {splat(0.f)}, ds[1];
+        floatx16 p = splat(0.f), ds;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ds[0][e] = nd[32 * i + entry(e)];
-        mma_rows<T, DP, 1>(qt, i, k, p);
-        mma_rows<T, DP, 1>(dt, i, v, ds);
+        for (int e = 0; e < 16; ++e) ds[e] = nd[32 * i + entry(e)];
+        mma_rows<T, DP>(qt, i, k, p);
+        mma_rows<T, DP>(dt, i, v, ds);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          p[0][e] = exp2_(fmaf(p[0][e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
+          p[e] = exp2_(fmaf(p[e], s.c, kPExp<T> - lse[32 * i + entry(e)]));
         if constexpr (EDGE) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            p[0][e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[0][e] : 0.f;
+            p[e] = at * F::TR + 32 * i + entry(e) >= rmin ? p[e] : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ds[0][e] *= p[0][e];
+        for (int e = 0; e < 16; ++e) ds[e] *= p[e];
         Twice<T> x;
-        x.set(p[0]);
+        x.set(p);
         mma_cols<T, DP>(dt, i, x, dv);
-        range.fit(ds[0], dk[0]);
-        x.set(ds[0]);
+        range.fit(ds, dk);
+        x.set(ds);
         mma_cols<T, DP>(qt, i, x, dk);
       }
     } else {
@@ -363,13 +363,13 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           fb[j] = row_frag<T, DP>(dt, i, j);
-          p = mma<T>(fa[j], k[0][j], p);
+          p = mma<T>(fa[j], k[j], p);
           in_order();
         }
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           fa[j] = col_frag<T, DP>(dt, i, j);
-          ds = mma<T>(fb[j], v[0][j], ds);
+          ds = mma<T>(fb[j], v[j], ds);
 #pragma unroll
           for (int e = (j - 1) * PER; e >= 0 && e < j * PER && e < 16; ++e) {
             p[e] = exp2_(fmaf(p[e], s.c, kPExp<T> - ls[e]));
@@ -382,17 +382,17 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           fb[j] = col_frag<T, DP>(qt, i, j);
-          dv[0][j % C::NB] = mma<T>(fa[j], x.v[j / C::NB], dv[0][j % C::NB]);
+          dv[j % C::NB] = mma<T>(fa[j], x.v[j / C::NB], dv[j % C::NB]);
 #pragma unroll
           for (int e = (j - 1) * PER; e >= 0 && e < j * PER && e < 16; ++e) ds[e] *= p[e];
           in_order();
         }
-        range.fit(ds, dk[0]);
+        range.fit(ds, dk);
         x.set(ds);
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           if (i + 1 < F::TR / 32) fa[j] = row_frag<T, DP>(qt, i + 1, j);
-          dk[0][j % C::NB] = mma<T>(fb[j], x.v[j / C::NB], dk[0][j % C::NB]);
+          dk[j % C::NB] = mma<T>(fb[j], x.v[j / C::NB], dk[j % C::NB]);
           in_order();
         }
       }
@@ -432,8 +432,8 @@ __global__ __launch_bounds__(kThreads, (Dkv<T, DP, KW>::TWO ? 2 : 1)) void attn_
       }
     });
   };
-  put(dk[0], fk, a.dk, 0);
-  put(dv[0], fv, a.dv, 1);
+  put(dk, fk, a.dk, 0);
+  put(dv, fv, a.dv, 1);
 }
 
 // Sums the parts of a row of dQ, or of a key's dK and dV (KEYS), in their order: a wavefront a row.

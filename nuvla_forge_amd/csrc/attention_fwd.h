@@ -66,9 +66,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   // the lane's row
   const int r = r0 + (l & 31);
   const int rc = min(r, s.R - 1), t = rc / s.G, g = rc - t * s.G;
-  u32x4 q[1][C::KS];
+  u32x4 q[C::KS];
   load_row<T, DP>(a.q.p + b * a.q.b + t * a.q.t + (int64_t)(hk * s.G + g) * a.q.h, r < s.R, s.nvec,
-                  s.flip, q[0]);
+                  s.flip, q);
   const int last = s.causal ? t + s.off : s.Tk - 1;  // the lane's last key
   const int block_least = s.causal ? tile * F::BR / s.G + s.off : s.Tk - 1;  // its first row's
   int at = part * a.length;
@@ -76,9 +76,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
   // every row of the block sees every key of the tiles before this one
   const int full = MASKED ? 0 : min(end, max(block_least + 1, 0) / F::TK);
 
-  floatx16 o[1][C::NB];
+  floatx16 o[C::NB];
 #pragma unroll
-  for (int n = 0; n < C::NB; ++n) o[0][n] = splat(0.f);
+  for (int n = 0; n < C::NB; ++n) o[n] = splat(0.f);
   float m = -kInf, sum = 0.f;  // sum: of the lane's own entries
 
   typename F::Keys keys(s, a.k, a.v, b, hk, end, wave);
@@ -99,9 +99,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
     floatx16 p[F::NK];
 #pragma unroll
     for (int i = 0; i < F::NK; ++i) {
-      floatx16 acc[1] = {splat(0.f)};
-      mma_rows<T, DP, 1>(kt, kb0 + i, q, acc);
-      p[i] = acc[0];
+      floatx16 acc = splat(0.f);
+      mma_rows<T, DP>(kt, kb0 + i, q, acc);
+      p[i] = acc;
       if constexpr (EDGE) {
         const uint32_t live = live32(last - (at * F::TK + 32 * (kb0 + i)), cur.half(kb0 + i));
 #pragma unroll
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
       m = up;
       sum *= f;
 #pragma unroll
-      for (int n = 0; n < C::NB; ++n) o[0][n] *= f;
+      for (int n = 0; n < C::NB; ++n) o[n] *= f;
     }
     const float base = m == -kInf ? 0.f : m;
 #pragma unroll
@@ -135,9 +135,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
         x.set(p[i]);
         mma_cols<T, DP>(vt, kb0 + i, x, o);
       } else {
-        Packed<T> x[1];
-        x[0].set(p[i]);
-        mma_cols<T, DP, 1>(vt, kb0 + i, x, o);
+        Packed<T> x;
+        x.set(p[i]);
+        mma_cols<T, DP>(vt, kb0 + i, x, o);
       }
     }
     if (F::STAGES == 1) {
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 || (KW == 4 && DP <= 64) ?
     sum = total;
   }
   if (parts == 1) f *= sum == 0.f ? 0.f : 1.f / sum;  // no key: 0; a NaN stays one
-  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, o[0], f);
+  Turned<DP>::put(smem + wave * Turned<DP>::BYTES, o, f);
   if (KW == 4) __syncthreads();
   const int64_t row = (int64_t)bh * s.R + r;  // the lane's
   const bool lead = r < s.R && h == 0 && (KW == 1 || wave == 0);

@@ -12,7 +12,7 @@ import torch
 from nuvla_forge_amd import _lib
 from nuvla_forge_amd.kernels import fused_attention, fused_rotary
 
-from .helpers import gen, note, randn
+from .helpers import assert_graph_replays_match, gen, note, randn
 from .test_gpu_block_ops import _check, _mask, _qkv, _run
 from .test_gpu_token_ops_edges import route  # noqa: F401  (a fixture)
 
@@ -242,3 +242,90 @@ def test_rotary_positions_of_the_wrong_dimensions_are_refused(cuda, route, shape
     q = randn((2, 3, 4, 16), gen(0), BF16, cuda)
     with pytest.raises(ValueError, match="fused_rotary: positions"):
         fused_rotary(q, None, torch.zeros(shape, dtype=torch.long, device=cuda), (4, 4))
+
+
+# ---------------------------------------------------------------------------
+# calls that copy their operands, in graphs and under what sees or replaces a call
+# ---------------------------------------------------------------------------
+def _copied(t, d, dtype, dev):
+    """Operands of no whole vectors, k and the mask with their tokens innermost."""
+    q, k, v, do = _qkv(2, t, 70, 4, 2, d, dtype, dev)
+    k = k.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    return (q, k, v, do), _mask("random", 2, 70, dev).t().contiguous().t()
+
+
+@pytest.mark.parametrize("dtype, d", [(BF16, 100), (F32, 90)])
+@pytest.mark.parametrize("t", [1, 70])
+def test_attention_with_copies_in_a_graph(cuda, t, dtype, d):
+    note(f"attention copies in a graph {t} {d} {dtype}")
+    args, m = _copied(t, d, dtype, cuda)
+
+    def make():
+        x = [a.clone(memory_format=torch.preserve_format).requires_grad_(True) for a in args[:3]]
+
+        def step():
+            out = fused_attention(*x, causal=True, key_mask=m)
+            return [out.detach(), *torch.autograd.grad(out, x, args[3])]
+
+        return step
+
+    assert_graph_replays_match(make)
+
+
+@pytest.mark.parametrize("dtype, d", [(BF16, 100), (F32, 90)])
+def test_attention_with_copies_under_modes_and_create_graph(cuda, route, dtype, d):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    note(f"attention copies under modes {d} {dtype} {route}")
+    (q, k, v, do), m = _copied(70, d, dtype, cuda)
+    want = _run(q, k, v, do, causal=True, key_mask=m)
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, a=(), kw=None):
+            return func(*a, **(kw or {}))
+
+    with Dispatch():
+        _same(want, _run(q, k, v, do, causal=True, key_mask=m), "mode")
+    op = lambda *x: fused_attention(*x, causal=True, key_mask=m)  # noqa: E731
+    traced = torch.jit.trace(op, (q, k, v), check_trace=False)
+    assert torch.equal(traced(q, k, v), want[0])
+    x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    up = do.clone().requires_grad_(True)
+    got = torch.autograd.grad(op(*x), x, up, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want[1:], got))
+    for leaf in (*x, up):
+        with pytest.raises(RuntimeError, match="fused_attention: second derivatives"):
+            torch.autograd.grad(sum((t.float() ** 2).sum() for t in got), leaf, retain_graph=True,
+                                allow_unused=True)
+
+
+def test_attention_rows_without_a_key_in_a_graph_and_on_two_streams(cuda):
+    """A batch padded on the left, NaN in the padding: replays and calls on other streams give the
+    bits of zeros there."""
+    note("attention keyless rows in a graph")
+    (q, k, v, do) = _qkv(3, 150, 150, 4, 2, 64, BF16, cuda)
+    m = torch.arange(150, device=cuda)[None] >= torch.tensor([[0], [61], [149]], device=cuda)
+    pad = ~m[..., None, None]
+    want = _run(*(t.masked_fill(pad, 0.0) for t in (q, k, v, do)), causal=True, key_mask=m)
+    args = [t.masked_fill(pad, math.nan) for t in (q, k, v, do)]
+
+    def make():
+        x = [t.clone().requires_grad_(True) for t in args[:3]]
+
+        def step():
+            out = fused_attention(*x, causal=True, key_mask=m)
+            return [out.detach(), *torch.autograd.grad(out, x, args[3])]
+
+        return step
+
+    _same(want, make()())
+    assert_graph_replays_match(make)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams * 2:
+        with torch.cuda.stream(s):
+            got.append(make()())
+    torch.cuda.synchronize()
+    for x in got:
+        _same(want, x)

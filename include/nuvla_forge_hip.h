@@ -404,7 +404,9 @@ int nf_dropout(const void *x, const void *residual, void *out, int64_t n,
  * *_b, *_t, *_h in elements (0: broadcast): every row starts on 16 bytes, and
  * where D is no multiple of 16 bytes the elements up to the next one are
  * zeros.  out [B, Tq, H, D] dense.  D at most 128, H / Hk at most 32768; Tk
- * at least 1; 130 token strides and H / Hk head strides below 2^30 bytes;
+ * at least 1; 130 token strides and H / Hk head strides (of k and v 130 token
+ * strides alone) below 2^30 bytes; B Hk times the tiles of 32 rows, Tq H / Hk
+ * of them, and of 32 keys, each and one more, at most 2^23;
  * |scale| at most 2^127.  What rows that the mask drops from k and v hold, NaN or
  * infinity too, changes no bit of any result; their memory has to be readable.
  * `state` (nf_attention_state_bytes; NULL: no backward will come) takes each
@@ -459,7 +461,8 @@ int nf_attention_bwd(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
  * (H or Hk may be 0) with unit last stride and strides in elements; outputs
  * dense, apart from the inputs.  positions [B, T, axes] dense, pos_b elements
  * between samples (0: one for all), pos_kind 0 int64, 1 int32, 2 fp32.
- * `sections` is read on the host.  P at most 256 and D / 2, D at most 1024.
+ * `sections` is read on the host.  P at most 256 and D / 2, D at most 1024,
+ * H + Hk at most 65536.
  * ---------------------------------------------------------------------- */
 int nf_rotary(const void *q, int64_t q_b, int64_t q_t, int64_t q_h,
               void *q_out, int64_t H, const void *k, int64_t k_b, int64_t k_t,

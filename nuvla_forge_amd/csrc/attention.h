@@ -440,8 +440,8 @@ __device__ __forceinline__ int first_row_tile(const Shape &s, int tile, int bk) 
 // The part length for `tiles` blocks a head of up to `longest` tiles each, `slots` blocks at once on
 // the chip.  Blocks of one length go in rounds: as many parts as take the least time, in tiles a
 // block 1.5 beside its own, the join 4 and 1.2 for each part that a slot writes and reads.  A causal
-// call's blocks fall from the longest to few and fill up what it leaves: two parts a slot (dK and dV
-// of 2 x 4096 tokens, 4 key heads of 128: 585 us whole, 365 so, in 3 parts a slot 400, in 8 450).
+// call's blocks fall from the longest to few and fill up what it leaves: two parts a slot (delta, dK
+// and dV of 2 x 4096 tokens, 16 heads on 4 of 128: 366 us, in 3 parts a slot 392, in 4 409, in 8 461).
 inline int part_length(int64_t heads, int64_t tiles, int64_t longest, bool causal, int slots) {
   const int64_t blocks = heads * tiles;
   if (blocks >= 4 * (int64_t)slots) return 1 << 28;

@@ -59,6 +59,8 @@ int make_view(const char *op, const char *name, const void *p, int64_t sb, int64
 // of 80 on 2, fp16 88 -> 72 us; 1024 tokens, 8 heads of 64 64 -> 44, 2048 105 -> 98; 512, 8 heads of
 // 128 on 4 68 -> 50, 1500 causal, 4 heads of 128 79 -> 87.  fp32 rows of 512 bytes leave a CU one
 // block: 900, 4 heads of 128 160 -> 271.
+// (The two-term products of shared blocks round less, so that a sample's 16-bit results also depend,
+// within those roundings, on how many others are in its call.)
 bool shared_blocks(const Sizes &z, int64_t own) {
   if (own <= 32) return true;
   if (z.dp() * z.es() > 256 || z.B * z.Hk * ((own + 127) / 128) >= 256) return false;
@@ -98,7 +100,12 @@ State state_of(const Sizes &z) {
   return t;
 }
 
-// Blocks at once on the chip: two a CU of those whose wavefronts share rows of up to `narrow` bytes.
+// The blocks that part_length counts as running at once: two a CU of those whose wavefronts share
+// rows of up to `narrow` bytes, else one, although the 16-bit forward and dQ, and dK and dV of up to
+// 64 columns, leave room for two.  Counted as two, causal calls are cut too finely (4096 tokens,
+// 16 heads on 4 of 128: forward 105.5 -> 113.9 us, dQ 138.5 -> 151.5); without a causal line 264
+// blocks are cut with nothing gained by it (3 x 1400, 8 heads of 128: 49.2 us uncut -> 63.6, dQ
+// 62.7 -> 84.3), 288 in one sequence of 4600 133.5 against 130.8; others of 272 to 504 come out alike.
 static int slots_of(int kw, const Sizes &z, int narrow) {
   return kw == 4 && z.dp() * z.es() <= narrow ? 512 : 256;
 }

@@ -16,6 +16,10 @@
 // What bounds it: as the forward, with the exponentials a smaller share: 2 x 4096 tokens, 16 heads of
 // 128: dQ 358 us (1.15 PFLOP/s of its three products), dK and dV 570 (0.96 of four; a wavefront
 // alone on its SIMD); of 64 208 and 284.
+//
+// What does not fit its registers: dQ in bf16, 96 columns, rows of a wavefront's own, unmasked keeps 10
+// of them (44 bytes a lane) in scratch memory; dK and dV in fp16, 128 columns, 4 to 10 in accumulation
+// registers; dK and dV in fp32, 128 columns, shared (calls of up to 32 keys) 608 bytes a lane in scratch.
 #pragma once
 
 #include <type_traits>

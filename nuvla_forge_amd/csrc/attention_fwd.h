@@ -10,6 +10,8 @@
 // 2 x 4096 tokens, 16 heads 265 us (1.04 PFLOP/s); 16384 causal tokens on 4 key heads 1.02 ms.
 // Heads of 64: the exponentials (160 us, 0.86).  Few rows: reading K and V (65536 keys of 4 heads
 // of 128, one token: 25 us, 5.4 TB/s).  fp32 runs on the fp32 matrix instructions (157 TFLOP/s).
+// Under a key mask every tile is tested entry by entry, whole ones too: 2 x 4096 causal tokens, 16
+// heads on 4, 153 us, with lengths between half and full 183 (dQ 198 and 227).
 #pragma once
 
 #include <type_traits>
@@ -19,8 +21,8 @@
 namespace nf {
 namespace attn {
 
-// m is raised only when a logit passes it by kSlack (in powers of two): p is then at most 2^kSlack,
-// which every type holds, and most tiles leave O as it is.
+// m is raised only when a logit passes it by kSlack (in powers of two): p is then at most
+// 2^(kSlack + kBias), 2^15 in fp16, which every type holds, and most tiles leave O as it is.
 constexpr float kSlack = 8.f;
 // fp16 ends at 2^-24: p carries a factor 2^7, so that it is normal down to 2^-21 of the largest.
 template <typename T>

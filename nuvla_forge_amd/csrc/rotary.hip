@@ -3,8 +3,8 @@
 //
 // A block takes a few tokens of a sample, forms their cosines and sines once (P a token) in LDS,
 // and turns every head with them.  Angles are kept in turns: the product of position and frequency
-// and its fraction in 64 bits, so that far positions lose nothing (in 32 bits a position of 10^6
-// would be off by 0.06 radians), then sine and cosine of the fraction in 32 bits.  The frequencies
+// and its fraction in 64 bits, so that angles of up to about 2^27 turns lose nothing (in 32 bits a
+// position of 10^6 would be off by 0.06 radians; in 64, farther ones by 2^-52 of theirs), then sine and cosine of the fraction in 32 bits.  The frequencies
 // come as kernel arguments, made in 64 bits on the host: no table in memory, no upload.
 //
 // A thread turns two pieces of 16 bytes at a time, one in each half of a head, at any alignment, with

@@ -141,10 +141,14 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     """``softmax(scale q k^T) v`` over the keys that each row may attend.
 
     Args:
-        q: [B, Tq, H, D], fp32, bf16 or fp16; any strides (a copy is made where rows are
-            not whole 16-byte vectors).
+        q: [B, Tq, H, D], fp32, bf16 or fp16; any strides.  q, k and v are read where they
+            lie if their rows are whole 16-byte vectors, a token's stride is at most 2 MiB, and
+            130 token strides and the heads' strides together span less than 1 GiB; else a
+            copy is made in each call (a cache stored head by head, [B, Hk, T, D], from 1 GiB
+            a sample on).
         k, v: [B, Tk, Hk, D], q's type; H a multiple of Hk, up to 32768 times it: query head h
-            attends key head h // (H / Hk).
+            attends key head h // (H / Hk).  At most about 2^28 keys over all samples' key heads,
+            and as many rows.
         causal: query i attends keys up to i + Tk - Tq: the last query sees every key.
         key_mask: bool [B, Tk]; False: no query attends the key.  What such a key and its
             value hold, NaN or infinity too, changes no bit of any result (the unfilled part of
@@ -158,7 +162,8 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
 
     Logits, statistics and sums are fp32; for their products the probabilities (and the logits'
     gradients) are rounded to the inputs' type, or to two terms of it where few rows or keys
-    make a block's waves share them.  A NaN or an infinity in a key or value that some row may
+    make a block's waves share them: a sample's 16-bit results may differ by that rounding with the
+    size of the batch that it is in.  A NaN or an infinity in a key or value that some row may
     attend, or in the query or the gradient of a row that attends one, can reach other rows of its
     head and the gradients of other keys in the same sample.  First derivatives only on the device.
     Host tensors, heads wider than 128 and calls without a key take the eager formulation.

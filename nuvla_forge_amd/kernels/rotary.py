@@ -2,7 +2,7 @@
 
 ``fused_rotary`` turns the heads of q and k in one launch (``nf_rotary``), each pair by
 the coordinate of its axis: the angles are formed in the kernel, once a token, in 64 bits,
-so there is no table to keep and no position too far.  The gradient turns back.
+so there is no table to keep and no last position that one would hold.  The gradient turns back.
 """
 
 from __future__ import annotations
@@ -125,9 +125,10 @@ def fused_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     Returns:
         (q, k) turned, contiguous; k is None where it was.
 
-    Positions of any size keep their angle to fp32's precision (64-bit products).  Linear in
-    q and k: derivatives of any order.  Host tensors, more than 256 pairs and heads wider
-    than 1024 take the eager formulation.
+    Angles are formed in 64 bits: those of up to about 2^27 turns to fp32's precision, farther
+    ones off by 2^-52 of themselves.  Linear in q and k: derivatives of any order.  Host
+    tensors, more than 256 pairs and heads wider than 1024 take the eager formulation; on the
+    device q and k have at most 65536 heads together.
     """
     fused = use_fused(q, "fused_rotary", force_reference)
     if fused and type(sections) in (tuple, list):
